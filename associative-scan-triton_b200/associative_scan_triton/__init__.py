@@ -5,6 +5,10 @@ Drop-in for the Python API of the reference package of the same name
 functions, launcher objects, argument dicts and custom-op names.  Every op runs
 hand-written CUDA kernels from the native library ``libascan_b200.so`` (C ABI
 in include/ascan.h); CUDA tensors only, no CPU fallback.
+
+Beside the reference's names (``__all__``) the package has the operators of a
+gated linear-attention layer: ``matrix_scan_causal``, ``matrix_scan_step`` and
+``qk_norm_rotate`` (matrix_scan.py).
 """
 
 __version__ = "1.0.0"
@@ -32,6 +36,11 @@ from associative_scan_triton.scan_eager import scan_causal, scan_bidirectional_b
 from associative_scan_triton.scan_compiled import (  # noqa: E402
   scan_causal_compiled,
   scan_bidirectional_branched_compiled,
+)
+from associative_scan_triton.matrix_scan import (  # noqa: E402
+  matrix_scan_causal,
+  matrix_scan_step,
+  qk_norm_rotate,
 )
 from associative_scan_triton._lib import (  # noqa: E402
   ScanError,

@@ -34,6 +34,7 @@ DEV_ERR_CU_END = 0x1
 DEV_ERR_CU_ORDER = 0x2
 DEV_ERR_LOOKBACK = 0x4
 DEV_ERR_EXCHANGE = 0x8
+DEV_ERR_INDEX = 0x10
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 INDEX_CODES = {torch.int32: 0, torch.int64: 1}
@@ -61,6 +62,13 @@ EXPORTED_SYMBOLS = (
   "ascan_forward_bidi",
   "ascan_backward_bidi",
   "ascan_shift_pad",
+  "ascan_matrix_scan_workspace",
+  "ascan_matrix_scan_forward",
+  "ascan_matrix_scan_backward",
+  "ascan_matrix_scan_step",
+  "ascan_qk_norm_rotate",
+  "ascan_qk_norm_rotate_workspace",
+  "ascan_qk_norm_rotate_backward",
   "ascan_set_implementation",
   "ascan_get_implementation",
   "ascan_set_tile_width",
@@ -72,6 +80,13 @@ EXPORTED_SYMBOLS = (
 )
 
 IMPLEMENTATIONS = {"auto": 0, "simple": 1, "tma": 2, "tma-flat": 3, "tma-row": 4}
+
+
+class Rows(ctypes.Structure):
+  """``ascan_rows``: a [tokens, heads, dim] tensor with unit stride along dim."""
+
+  _fields_ = [("data", ctypes.c_void_p), ("stride_token", ctypes.c_int64),
+              ("stride_head", ctypes.c_int64), ("heads", ctypes.c_int32)]
 
 
 class ScanError(RuntimeError):
@@ -131,6 +146,27 @@ def _bind(lib) -> None:
                                       p, sz, p]
   lib.ascan_shift_pad.restype = ci
   lib.ascan_shift_pad.argtypes = [p, p, p, ci, i64, i64, i64, ci, ctypes.c_double, ci, ci, p]
+  f, rows = ctypes.c_float, ctypes.POINTER(Rows)
+  lib.ascan_matrix_scan_workspace.restype = sz
+  lib.ascan_matrix_scan_workspace.argtypes = [i64, i64, ci, ci, ci, ci, ci, ci, ci, ci]
+  lib.ascan_matrix_scan_forward.restype = ci
+  lib.ascan_matrix_scan_forward.argtypes = [rows, rows, rows, rows, ci, p, ci, i64, i64, ci, ci, ci,
+                                            ci, f, p, p, p, p, sz, p]
+  lib.ascan_matrix_scan_backward.restype = ci
+  lib.ascan_matrix_scan_backward.argtypes = [rows, rows, rows, rows, ci, rows, p, p, p, p, ci, i64,
+                                             i64, ci, ci, ci, ci, f, p, p, p, p, p, p, sz, p]
+  lib.ascan_matrix_scan_step.restype = ci
+  lib.ascan_matrix_scan_step.argtypes = [rows, rows, rows, rows, ci, p, i64, i64, ci, ci, ci, ci, f,
+                                         p, p, p, p]
+  lib.ascan_qk_norm_rotate.restype = ci
+  lib.ascan_qk_norm_rotate.argtypes = [rows, rows, p, p, ci, p, p, i64, ci, ci, p, p, ci, i64, i64,
+                                       ci, ci, f, p, p, p]
+  lib.ascan_qk_norm_rotate_workspace.restype = sz
+  lib.ascan_qk_norm_rotate_workspace.argtypes = [i64, ci, ci, ci]
+  lib.ascan_qk_norm_rotate_backward.restype = ci
+  lib.ascan_qk_norm_rotate_backward.argtypes = [rows, rows, p, p, ci, p, p, i64, ci, ci, p, p, ci,
+                                                i64, i64, ci, ci, f, rows, rows, p, p, p, p, p, sz,
+                                                p]
   lib.ascan_set_implementation.restype = ci
   lib.ascan_set_implementation.argtypes = [ci]
   lib.ascan_get_implementation.restype = ci
@@ -238,6 +274,8 @@ def describe_device_error(code: int) -> str:
   if code & DEV_ERR_EXCHANGE:
     parts.append("a peer rank's time-shard record or release did not arrive within the "
                  "bounded wait")
+  if code & DEV_ERR_INDEX:
+    parts.append("a state slot or a position lies outside its table")
   return "; ".join(parts) or f"device error {code:#x}"
 
 

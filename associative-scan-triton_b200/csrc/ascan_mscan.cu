@@ -1,0 +1,798 @@
+// ascan_mscan.cu -- compilation unit of the scan library: the matrix-state
+// recurrence (ascan_mscan.cuh has the mathematics), its plain kernel for
+// every type and head size, the carry chain, the gate gradients, the sums
+// over shared heads, and the one-token step.
+#include "ascan_impl.cuh"
+#include "ascan_mscan.cuh"
+
+namespace ascan {
+namespace mscan {
+
+constexpr int kPlainThreads = 256;
+constexpr int kPlainChunk = 32;
+
+// cu_seqlens as the scans check it; every other read of it is clamped.
+__device__ void check_cu(const Problem& p) {
+  if (p.cu64) validate_cu(static_cast<const int64_t*>(p.cu), p.N, p.BL, p.err);
+  else validate_cu(static_cast<const int32_t*>(p.cu), p.N, p.BL, p.err);
+}
+
+// ---------------------------------------------------------------------------
+// The plain kernel: one CTA per (segment, head, form), fused multiply-adds.
+// The state stays in shared memory from chunk to chunk; a chunk of 32 tokens
+// costs 32*(da*dc) products with the state for the outputs, as many for its
+// update and 32*32*(da + dc) for the scores and values, so it is bound by
+// fused multiply-adds and shared-memory reads.  It serves float32, float16
+// and whatever the tensor-core kernel does not take.
+// ---------------------------------------------------------------------------
+
+template <int DM>
+struct PlainSmem {
+  static constexpr int kLd = DM + 4;
+  float s[DM * DM];
+  float a[kPlainChunk * kLd];
+  float b[kPlainChunk * kLd];
+  float c[kPlainChunk * kLd];
+  float p[kPlainChunk * (kPlainChunk + 1)];
+  double g[kPlainChunk];
+  float row[kPlainChunk], col[kPlainChunk];
+  float total;
+};
+
+template <typename T, int LD, int DM>
+__device__ __forceinline__ void load_rows(float* dst, const Rows& r, long long t0, int len, int h, int dim) {
+  const T* base = static_cast<const T*>(r.p) + t0 * r.st + (h / r.share) * r.sh;
+  for (int e = threadIdx.x; e < kPlainChunk * DM; e += kPlainThreads) {
+    const int i = e / DM, d = e % DM;
+    dst[i * LD + d] = (i < len && d < dim) ? to_f(base[i * r.st + d]) : 0.f;
+  }
+}
+
+template <typename T, int DM>
+__global__ void __launch_bounds__(kPlainThreads)
+    plain_kernel(const __grid_constant__ Launch L, const bool state_only) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  using Sm = PlainSmem<DM>;
+  Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
+  constexpr int LD = Sm::kLd;
+  constexpr int TX = DM / 4;                              // threads along the values
+  constexpr int RPT = kPlainChunk / (kPlainThreads / TX);  // rows per thread
+  const Problem& p = L.p;
+  const Form& f = L.f[blockIdx.z];
+  const int tid = threadIdx.x, j = blockIdx.x, h = blockIdx.y;
+  const bool rev = f.rev != 0;
+  const int da = f.da, dc = f.dc;
+  const long long mat = static_cast<long long>(da) * dc;
+  const long long t0 = j * p.seg, t1 = min(t0 + p.seg, p.BL);
+
+  if (!state_only) {
+    if (j == 0 && h == 0 && blockIdx.z == 0) check_cu(p);
+    // rows that belong to no sequence
+    const long long c0 = min(t1, cu_at(p, 0)), c1 = max(t0, cu_at(p, p.N));
+    for (long long t = t0; t < t1; ++t) {
+      if (t >= c0 && t < c1) { t = c1 - 1; continue; }
+      for (int d = tid; d < dc; d += kPlainThreads) {
+        const long long at = (t * p.H + h) * dc + d;
+        if (f.out_f32) static_cast<float*>(f.out)[at] = 0.f;
+        else static_cast<T*>(f.out)[at] = from_f<T>(0.f);
+      }
+      if (f.rowdot && tid == 0) f.rowdot[h * p.BL + t] = 0.f;
+    }
+    if (f.fin && j == 0)  // empty sequences hand their state through
+      for (long long n = 0; n < p.N; ++n)
+        if (cu_at(p, n + 1) <= cu_at(p, n))
+          for (long long e = tid; e < mat; e += kPlainThreads)
+            f.fin[(n * p.H + h) * mat + e] = f.init ? f.init[(n * p.H + h) * mat + e] : 0.f;
+  }
+
+  const long long n_first = first_beyond(p, t0);
+  const long long n_last = first_from(p, t1);  // one past the last sequence that starts before t1
+  for (long long m = 0; m < n_last - n_first; ++m) {
+    const long long n = rev ? n_last - 1 - m : n_first + m;
+    const long long b0 = cu_at(p, n), b1 = cu_at(p, n + 1);
+    const long long ps = max(b0, t0), pe = min(b1, t1);
+    if (pe <= ps) continue;
+    const bool from_start = rev ? pe == b1 : ps == b0;  // the state begins in this piece
+    const bool to_end = rev ? ps == b0 : pe == b1;      // ... and ends in it
+    if (state_only && to_end) continue;
+    const float* from = from_start ? (f.init ? f.init + (n * p.H + h) * mat : nullptr)
+                                   : f.carry + (static_cast<long long>(rev ? j + 1 : j - 1) * p.H + h) * mat;
+    const bool zero = from == nullptr || (state_only && !from_start);
+    const long long fi = from_start ? f.si : dc, fj = from_start ? f.sj : 1;
+    for (int e = tid; e < DM * DM; e += kPlainThreads) {
+      const int i = e / DM, d = e % DM;
+      sm.s[e] = (!zero && i < da && d < dc) ? from[i * fi + d * fj] : 0.f;
+    }
+    const int chunks = static_cast<int>((pe - ps + kPlainChunk - 1) / kPlainChunk);
+    float decay = 1.f;
+    for (int cc = 0; cc < chunks; ++cc) {
+      const long long s0 = ps + static_cast<long long>(rev ? chunks - 1 - cc : cc) * kPlainChunk;
+      const int len = static_cast<int>(min(static_cast<long long>(kPlainChunk), pe - s0));
+      __syncthreads();
+      if (f.snap && !state_only) {
+        const long long at = rev ? s0 + len : s0;
+        if (at > ps && at < pe && (at - ps) % kRestart == 0)
+          for (int e = tid; e < mat; e += kPlainThreads)
+            f.snap[(snap_slot(at) * p.H + h) * mat + e] = sm.s[(e / dc) * DM + e % dc];
+      }
+      if (!state_only) load_rows<T, LD, DM>(sm.a, f.a, s0, len, h, da);
+      load_rows<T, LD, DM>(sm.b, f.b, s0, len, h, da);
+      load_rows<T, LD, DM>(sm.c, f.c, s0, len, h, dc);
+      if (tid < 32) {
+        double g = tid < len ? static_cast<double>(load_gate(p, s0 + tid, h)) : 0.0;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const double up = __shfl_up_sync(kFull, g, o);
+          if (tid >= o) g += up;
+        }
+        const double end = __shfl_sync(kFull, g, 31);
+        const float head = expf(static_cast<float>(g)), tail = expf(static_cast<float>(end - g));
+        sm.g[tid] = g;
+        sm.row[tid] = (rev ? tail : head) * f.sr;
+        sm.col[tid] = (rev ? head : tail) * f.sc;
+        if (tid == 31) sm.total = head;
+      }
+      __syncthreads();
+      if (!state_only) {
+        {  // scores: 4 columns of one row per thread
+          const int r = tid / 8, c0 = tid % 8;
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int d = 0; d < da; d += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&sm.a[r * LD + d]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float4 y = *reinterpret_cast<const float4*>(&sm.b[(c0 + 8 * q) * LD + d]);
+              acc[q] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, acc[q]))));
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = c0 + 8 * q;
+            const bool on = (rev ? c >= r : c <= r) && c < len;
+            const double dg = rev ? sm.g[c] - sm.g[r] : sm.g[r] - sm.g[c];
+            sm.p[r * (kPlainChunk + 1) + c] = on ? acc[q] * f.sp * expf(static_cast<float>(dg)) : 0.f;
+          }
+        }
+        __syncthreads();
+        const int tx = tid % TX, r0 = (tid / TX) * RPT;
+        float acc[RPT][4] = {};
+        for (int i = 0; i < da; ++i) {
+          const float4 y = *reinterpret_cast<const float4*>(&sm.s[i * DM + tx * 4]);
+#pragma unroll
+          for (int r = 0; r < RPT; ++r) {
+            const float x = sm.a[(r0 + r) * LD + i];
+            acc[r][0] = fmaf(x, y.x, acc[r][0]);
+            acc[r][1] = fmaf(x, y.y, acc[r][1]);
+            acc[r][2] = fmaf(x, y.z, acc[r][2]);
+            acc[r][3] = fmaf(x, y.w, acc[r][3]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RPT; ++r)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[r][q] *= sm.row[r0 + r];
+        for (int c = 0; c < len; ++c) {
+          const float4 y = *reinterpret_cast<const float4*>(&sm.c[c * LD + tx * 4]);
+#pragma unroll
+          for (int r = 0; r < RPT; ++r) {
+            // masked tokens are left out, not multiplied by zero: a NaN or
+            // infinity there must not reach this row
+            if (rev ? c < r0 + r : c > r0 + r) continue;
+            const float x = sm.p[(r0 + r) * (kPlainChunk + 1) + c];
+            acc[r][0] = fmaf(x, y.x, acc[r][0]);
+            acc[r][1] = fmaf(x, y.y, acc[r][1]);
+            acc[r][2] = fmaf(x, y.z, acc[r][2]);
+            acc[r][3] = fmaf(x, y.w, acc[r][3]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) {
+          const bool on = r0 + r < len;
+          const long long t = s0 + r0 + r;
+          float dot = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int d = tx * 4 + q;
+            if (on && d < dc) {
+              const long long at = (t * p.H + h) * dc + d;
+              if (f.out_f32) static_cast<float*>(f.out)[at] = acc[r][q];
+              else static_cast<T*>(f.out)[at] = from_f<T>(acc[r][q]);
+              if (f.rowdot)
+                dot = fmaf(acc[r][q],
+                           to_f(static_cast<const T*>(f.dot.p)[t * f.dot.st + (h / f.dot.share) * f.dot.sh + d]), dot);
+            }
+          }
+          if (f.rowdot) {
+#pragma unroll
+            for (int o = TX / 2; o > 0; o /= 2) dot += __shfl_xor_sync(kFull, dot, o);
+            if (on && tx == 0) f.rowdot[h * p.BL + t] = dot;
+          }
+        }
+        __syncthreads();
+      }
+      // state: a (DM/16)^2 tile per thread, columns in quads 64 apart
+      {
+        constexpr int R = DM / 16, Q = DM / 64;
+        const int i0 = (tid / 16) * R, d0 = (tid % 16) * 4;
+        float st[R][Q * 4] = {};
+        for (int c = 0; c < len; ++c) {
+          float x[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[r] = sm.b[c * LD + i0 + r] * sm.col[c];
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            const float4 y = *reinterpret_cast<const float4*>(&sm.c[c * LD + d0 + 64 * q]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              st[r][q * 4 + 0] = fmaf(x[r], y.x, st[r][q * 4 + 0]);
+              st[r][q * 4 + 1] = fmaf(x[r], y.y, st[r][q * 4 + 1]);
+              st[r][q * 4 + 2] = fmaf(x[r], y.z, st[r][q * 4 + 2]);
+              st[r][q * 4 + 3] = fmaf(x[r], y.w, st[r][q * 4 + 3]);
+            }
+          }
+        }
+        const float total = sm.total;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            float4* at = reinterpret_cast<float4*>(&sm.s[(i0 + r) * DM + d0 + 64 * q]);
+            const float4 o = *at;
+            *at = make_float4(fmaf(total, o.x, st[r][q * 4 + 0]), fmaf(total, o.y, st[r][q * 4 + 1]),
+                              fmaf(total, o.z, st[r][q * 4 + 2]), fmaf(total, o.w, st[r][q * 4 + 3]));
+          }
+        decay *= total;
+      }
+    }
+    __syncthreads();
+    if (state_only) {
+      float* to = f.carry + (static_cast<long long>(j) * p.H + h) * mat;
+      for (int e = tid; e < mat; e += kPlainThreads) to[e] = sm.s[(e / dc) * DM + e % dc];
+      // a piece that holds the sequence's start takes nothing from before
+      if (tid == 0) f.dec[j * p.H + h] = from_start ? -1.f : decay;
+    } else if (to_end && f.fin) {
+      float* to = f.fin + (n * p.H + h) * mat;
+      for (int e = tid; e < mat; e += kPlainThreads)
+        to[(e / dc) * f.si + (e % dc) * f.sj] = sm.s[(e / dc) * DM + e % dc];
+    }
+    __syncthreads();
+  }
+}
+
+// Chains the segments' own contributions in scan order: carry[j] becomes the
+// state that leaves segment j.  One thread per element; a segment that no
+// sequence leaves restarts the chain (its carry is never read).
+__global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Launch L) {
+  const Problem& p = L.p;
+  const Form& f = L.f[blockIdx.z];
+  const int h = blockIdx.y;
+  const long long mat = static_cast<long long>(f.da) * f.dc;
+  const long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= mat) return;
+  float state = 0.f;
+  bool have = false;
+  for (int m = 0; m + 1 < p.J; ++m) {
+    const int j = f.rev ? p.J - 1 - m : m;
+    const long long edge = f.rev ? j * p.seg : min((j + 1) * p.seg, p.BL);  // token after the boundary
+    const long long n = first_beyond(p, edge);
+    if (n >= p.N || cu_at(p, n) >= edge) {  // no sequence crosses
+      have = false;
+      continue;
+    }
+    const float dec = f.dec[j * p.H + h];
+    float* at = f.carry + (static_cast<long long>(j) * p.H + h) * mat + e;
+    float x = *at;
+    if (dec >= 0.f && have) {
+      x = fmaf(dec, state, x);
+      *at = x;
+    }
+    state = x;
+    have = true;
+  }
+}
+
+// Gate gradients of one stretch of at most kRestart tokens: the product of
+// the two states at its end, then the reverse sum of q.dq - k.dk over it.
+// blockIdx.z takes every gridDim.z-th stretch of the segment.
+__global__ void __launch_bounds__(256)
+    gate_grad_kernel(const __grid_constant__ Launch L, const float* __restrict__ final_state,
+                     const float* __restrict__ d_final, float* __restrict__ part, void* __restrict__ out,
+                     int out_type) {
+  const Problem& p = L.p;
+  const Form& fq = L.f[0];
+  const Form& fk = L.f[1];
+  const int tid = threadIdx.x, j = blockIdx.x, h = blockIdx.y, lane = tid & 31, warp = tid >> 5;
+  const long long mat = static_cast<long long>(fq.da) * fq.dc;
+  const long long t0 = j * p.seg, t1 = min(t0 + p.seg, p.BL);
+  __shared__ float red[8];
+  auto put = [&](long long t, float x) {
+    if (part) part[t * p.H + h] = x;
+    else store_any(out, out_type, t * p.H + h, x);
+  };
+  if (blockIdx.z == 0) {
+    const long long c0 = min(t1, cu_at(p, 0)), c1 = max(t0, cu_at(p, p.N));
+    for (long long t = t0 + tid; t < t1; t += 256)
+      if (t < c0 || t >= c1) put(t, 0.f);
+  }
+  int stretch = 0;
+  for (long long n = first_beyond(p, t0); n < p.N && cu_at(p, n) < t1; ++n) {
+    const long long b1 = cu_at(p, n + 1);
+    const long long ps = max(cu_at(p, n), t0), pe = min(b1, t1);
+    for (long long s0 = ps; s0 < pe; s0 += kRestart, ++stretch) {
+      if (stretch % gridDim.z != blockIdx.z) continue;
+      const long long s1 = min(s0 + kRestart, pe);
+      const float *x = nullptr, *y = nullptr;
+      if (s1 < pe) {
+        x = fq.snap + (snap_slot(s1) * p.H + h) * mat;
+        y = fk.snap + (snap_slot(s1) * p.H + h) * mat;
+      } else if (pe < b1) {
+        x = fq.carry + (static_cast<long long>(j) * p.H + h) * mat;
+        y = fk.carry + (static_cast<long long>(j + 1) * p.H + h) * mat;
+      } else if (d_final) {
+        x = final_state + (n * p.H + h) * mat;
+        y = d_final + (n * p.H + h) * mat;
+      }
+      float dot = 0.f;
+      if (x)
+        for (long long e = tid; e < mat; e += 256) dot = fmaf(x[e], y[e], dot);
+      // four tokens a thread, latest first
+      float v[4], sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const long long t = s1 - 1 - (tid * 4 + q);
+        v[q] = t >= s0 ? fq.rowdot[h * p.BL + t] - fk.rowdot[h * p.BL + t] : 0.f;
+        sum += v[q];
+      }
+      float inc = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const float up = __shfl_up_sync(kFull, inc, o);
+        if (lane >= o) inc += up;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) dot += __shfl_xor_sync(kFull, dot, o);
+      __syncthreads();
+      if (lane == 0) red[warp] = dot;
+      __syncthreads();
+      float base = 0.f;
+      for (int w = 0; w < 8; ++w) base += red[w];
+      __syncthreads();
+      if (lane == 31) red[warp] = inc;
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) base += red[w];
+      base += inc - sum;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const long long t = s1 - 1 - (tid * 4 + q);
+        base += v[q];
+        if (t >= s0) put(t, base);
+      }
+    }
+  }
+}
+
+// Sums the float32 parts of heads that share one input head, in head order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    share_sum_kernel(const float* __restrict__ part, T* __restrict__ out, long long n, int share, int dim) {
+  for (long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; e < n;
+       e += static_cast<long long>(gridDim.x) * 256) {
+    const long long row = e / dim, d = e % dim;
+    float x = 0.f;
+    for (int s = 0; s < share; ++s) x += part[(row * share + s) * dim + d];
+    out[e] = from_f<T>(x);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// One token: out = scale * q (e^g S + k v^T), the new state written back.
+// Bound by reading and writing the state; a CTA takes `cols` columns of one
+// (request, head), a lane four of them, and its warps share the rows.
+// ---------------------------------------------------------------------------
+
+struct StepArgs {
+  Rows q, k, v, gate;
+  const int* slots;
+  const float* state;
+  float* state_out;
+  void* out;
+  long long pool;
+  int H, dk, dv, gate_type, vec;
+  float scale;
+  uint32_t* err;
+};
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepArgs a) {
+  constexpr int RPP = 256 / LANES;  // rows per pass
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+  const int lane = tid % LANES, r0 = tid / LANES;
+  const int d = (blockIdx.x * LANES + lane) * 4;
+  const int nv = max(0, min(4, a.dv - d));
+  const long long slot = a.slots ? a.slots[b] : b;
+  T* out = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.H + h) * a.dv;
+  if (slot < 0 || slot >= a.pool) {
+    // negative: a row without a request; too large: reported, nothing touched
+    if (slot >= a.pool && tid == 0 && h == 0 && blockIdx.x == 0) report(ASCAN_DEV_ERR_INDEX, slot, a.err);
+    if (r0 == 0)
+      for (int q = 0; q < nv; ++q) out[d + q] = from_f<T>(0.f);
+    return;
+  }
+  const T* q = static_cast<const T*>(a.q.p) + b * a.q.st + (h / a.q.share) * a.q.sh;
+  const T* k = static_cast<const T*>(a.k.p) + b * a.k.st + (h / a.k.share) * a.k.sh;
+  const T* v = static_cast<const T*>(a.v.p) + b * a.v.st + (h / a.v.share) * a.v.sh;
+  const float decay = expf(load_any(a.gate.p, a.gate_type, b * a.gate.st + (h / a.gate.share) * a.gate.sh));
+  const long long base = (slot * a.H + h) * a.dk * static_cast<long long>(a.dv);
+  const float* src = a.state + base;
+  float* dst = a.state_out + base;
+  float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < 4; ++x) vv[x] = x < nv ? to_f(v[d + x]) : 0.f;
+  if (a.vec && nv == 4) {
+    constexpr int U = LANES == 32 ? 8 : 4;  // rows in flight per thread
+    for (int i0 = r0; i0 < a.dk; i0 += RPP * U) {
+      float4 s[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * RPP < a.dk)
+          s[u] = __ldcs(reinterpret_cast<const float4*>(src + static_cast<long long>(i0 + u * RPP) * a.dv + d));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * RPP;
+        if (i < a.dk) {
+          const float ki = to_f(k[i]), qi = to_f(q[i]);
+          s[u].x = fmaf(ki, vv[0], decay * s[u].x);
+          s[u].y = fmaf(ki, vv[1], decay * s[u].y);
+          s[u].z = fmaf(ki, vv[2], decay * s[u].z);
+          s[u].w = fmaf(ki, vv[3], decay * s[u].w);
+          __stcs(reinterpret_cast<float4*>(dst + static_cast<long long>(i) * a.dv + d), s[u]);
+          acc[0] = fmaf(qi, s[u].x, acc[0]);
+          acc[1] = fmaf(qi, s[u].y, acc[1]);
+          acc[2] = fmaf(qi, s[u].z, acc[2]);
+          acc[3] = fmaf(qi, s[u].w, acc[3]);
+        }
+      }
+    }
+  } else {
+    for (int i = r0; i < a.dk; i += RPP) {
+      const float ki = to_f(k[i]), qi = to_f(q[i]);
+      for (int x = 0; x < nv; ++x) {
+        const long long at = static_cast<long long>(i) * a.dv + d + x;
+        const float s = fmaf(ki, vv[x], decay * src[at]);
+        dst[at] = s;
+        acc[x] = fmaf(qi, s, acc[x]);
+      }
+    }
+  }
+  __shared__ float4 part[256];
+  part[tid] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (r0 == 0) {
+    for (int r = 1; r < RPP; ++r) {
+      const float4 o = part[r * LANES + lane];
+      acc[0] += o.x, acc[1] += o.y, acc[2] += o.z, acc[3] += o.w;
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (x < nv) out[d + x] = from_f<T>(acc[x] * a.scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+constexpr long long kSms = 148;
+constexpr int kSegGranule = 256;  // segments are multiples of this many tokens
+
+// Segments: the launch should fill the SMs, and a split that a sequence
+// crosses costs a second pass over two of the operands, about half of the
+// main pass's time.  Over all counts the cheapest estimate of
+// waves * segment length (* 1.5 when there are more segments than sequences)
+// is taken; equal sequences split at their own ends.
+static long long pick_segments(long long BL, long long N, long long lanes, int granule) {
+  const long long most = min(min((BL + granule - 1) / granule, 4096ll), 65535ll);
+  const double inf = 1e30;
+  long long best = 1;
+  double best_cost = inf;
+  for (long long J = 1; J <= most; J = J < 64 ? J + 1 : J + 8) {
+    const long long seg = ((BL + J - 1) / J + granule - 1) / granule * granule;
+    const long long waves = (J * lanes + kSms - 1) / kSms;
+    const double cost = static_cast<double>(waves) * (seg + 2.0 * granule) * (J > N ? 1.5 : 1.0);
+    if (cost < best_cost * 0.97) best = J, best_cost = cost;
+    if (J * lanes > 16 * kSms) break;
+  }
+  return best;
+}
+
+template <typename T, int DM>
+static int plain_launch(const Launch& l, int roles, bool state_only, cudaStream_t s) {
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaFuncSetAttribute(plain_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(sizeof(PlainSmem<DM>)));
+  });
+  plain_kernel<T, DM><<<dim3(l.p.J, l.p.H, roles), kPlainThreads, sizeof(PlainSmem<DM>), s>>>(l, state_only);
+  return launch_status();
+}
+
+static int plain_run(const Launch& l, int roles, bool state_only, int dtype, cudaStream_t s) {
+  int dm = 64;
+  for (int r = 0; r < roles; ++r) dm = max(dm, max(l.f[r].da, l.f[r].dc) > 64 ? 128 : 64);
+#define MSCAN_PLAIN(T) (dm == 64 ? plain_launch<T, 64>(l, roles, state_only, s) : plain_launch<T, 128>(l, roles, state_only, s))
+  if (dtype == ASCAN_F32) return MSCAN_PLAIN(float);
+  if (dtype == ASCAN_F16) return MSCAN_PLAIN(__half);
+  return MSCAN_PLAIN(__nv_bfloat16);
+#undef MSCAN_PLAIN
+}
+
+static int run_forms(const Launch& l, int roles, int dtype, cudaStream_t s) {
+  int rc = ASCAN_OK;
+  if (l.p.J > 1) {
+    rc = plain_run(l, roles, true, dtype, s);
+    if (rc != ASCAN_OK) return rc;
+    long long mat = 0;
+    for (int r = 0; r < roles; ++r) mat = max(mat, static_cast<long long>(l.f[r].da) * l.f[r].dc);
+    chain_kernel<<<dim3(static_cast<unsigned>((mat + 255) / 256), l.p.H, roles), 256, 0, s>>>(l);
+    rc = launch_status();
+    if (rc != ASCAN_OK) return rc;
+  }
+  return plain_run(l, roles, false, dtype, s);
+}
+
+struct Plan {
+  long long J, seg, slots;
+  size_t carry, snap, part_q, part_k, part_v, part_g, rowdot, total;
+};
+
+static size_t up(size_t x) { return (x + 255) / 256 * 256; }
+
+// Layout of the workspace; the same arithmetic serves the size query.
+static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, int hg, int dk, int dv,
+                      bool backward) {
+  Plan w{};
+  w.J = pick_segments(BL, N, static_cast<long long>(H) * (backward ? 3 : 1), kSegGranule);
+  w.seg = ((BL + w.J - 1) / w.J + kSegGranule - 1) / kSegGranule * kSegGranule;
+  w.J = (BL + w.seg - 1) / w.seg;
+  const size_t mat = static_cast<size_t>(dk) * dv * H * 4;
+  w.carry = w.J > 1 ? up(w.J * mat) + up(static_cast<size_t>(w.J) * H * 4) : 0;
+  w.slots = BL / kRestart + 1;
+  const size_t rows = static_cast<size_t>(BL) * H * 4;
+  w.total = w.carry * (backward ? 3 : 1);
+  if (backward) {
+    w.snap = up(w.slots * mat);
+    w.rowdot = up(rows);
+    w.part_q = hq < H ? up(rows * dk) : 0;
+    w.part_k = hk < H ? up(rows * dk) : 0;
+    w.part_v = hv < H ? up(rows * dv) : 0;
+    w.part_g = hg < H ? up(rows) : 0;
+    w.total += 2 * w.snap + 2 * w.rowdot + w.part_q + w.part_k + w.part_v + w.part_g;
+  }
+  w.total += 256;
+  return w;
+}
+
+static bool rows_ok(const ascan_rows* r, int H) {
+  return r && r->data && r->heads > 0 && r->heads <= H && H % r->heads == 0 && r->stride_token >= 0 &&
+         r->stride_head >= 0;
+}
+
+static Rows rows_of(const ascan_rows* r, int H) {
+  return Rows{r->data, r->stride_token, r->stride_head, H / r->heads};
+}
+
+static Rows packed_rows(const void* p, int heads, int dim, int H) {
+  return Rows{p, static_cast<long long>(heads) * dim, dim, H / heads};
+}
+
+static int check(const ascan_rows* q, const ascan_rows* k, const ascan_rows* v, const ascan_rows* g, int gate_dtype,
+                 const void* cu, int cu_type, int64_t N, int64_t BL, int H, int dk, int dv, int dtype) {
+  if (!cu || N < 0 || BL < 0 || H <= 0 || H > 65535 || dk <= 0 || dv <= 0) return ASCAN_EINVAL;
+  if (dk > ASCAN_MATRIX_SCAN_MAX_DIM || dv > ASCAN_MATRIX_SCAN_MAX_DIM) return ASCAN_EINVAL;
+  if (cu_type != ASCAN_I32 && cu_type != ASCAN_I64) return ASCAN_EINVAL;
+  if (dtype < ASCAN_F32 || dtype > ASCAN_BF16 || gate_dtype < ASCAN_F32 || gate_dtype > ASCAN_BF16) return ASCAN_EINVAL;
+  if (BL > (1ll << 40)) return ASCAN_EINVAL;
+  if (BL == 0 || N == 0) return ASCAN_OK;
+  if (!rows_ok(q, H) || !rows_ok(k, H) || !rows_ok(v, H) || !rows_ok(g, H)) return ASCAN_EINVAL;
+  return ASCAN_OK;
+}
+
+static Problem problem_of(const Plan& w, const ascan_rows* g, int gate_dtype, const void* cu, int cu_type, int64_t N,
+                          int64_t BL, int H) {
+  Problem p{};
+  p.cu = cu;
+  p.cu64 = cu_type == ASCAN_I64;
+  p.J = static_cast<int>(w.J);
+  p.H = H;
+  p.gate_type = gate_dtype;
+  p.N = N;
+  p.BL = BL;
+  p.seg = w.seg;
+  p.gate = rows_of(g, H);
+  p.err = g_err_host;
+  return p;
+}
+
+}  // namespace mscan
+}  // namespace ascan
+
+using namespace ascan;
+using namespace ascan::mscan;
+
+extern "C" {
+
+size_t ascan_matrix_scan_workspace(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads, int key_heads,
+                                   int value_heads, int gate_heads, int key_dim, int value_dim, int backward) {
+  if (seq_total <= 0 || num_seq <= 0 || num_heads <= 0 || key_dim <= 0 || value_dim <= 0) return 256;
+  return make_plan(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads, gate_heads, key_dim, value_dim,
+                   backward != 0)
+      .total;
+}
+
+int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                              const ascan_rows* log_gates, int gate_dtype, const void* cu_seqlens, int cu_index_type,
+                              int64_t num_seq, int64_t seq_total, int num_heads, int key_dim, int value_dim, int dtype,
+                              float scale, const float* initial_state, void* out, float* final_state, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  int rc = check(queries, keys, values, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, num_heads,
+                 key_dim, value_dim, dtype);
+  if (rc != ASCAN_OK) return rc;
+  if (seq_total == 0 || num_seq == 0) return ASCAN_OK;
+  if (!out) return ASCAN_EINVAL;
+  const Plan w = make_plan(seq_total, num_seq, num_heads, queries->heads, keys->heads, values->heads, log_gates->heads,
+                           key_dim, value_dim, false);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
+  Launch l{};
+  l.p = problem_of(w, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, num_heads);
+  char* at = static_cast<char*>(workspace);
+  Form& f = l.f[0];
+  f.a = rows_of(queries, num_heads);
+  f.b = rows_of(keys, num_heads);
+  f.c = rows_of(values, num_heads);
+  f.da = key_dim;
+  f.dc = value_dim;
+  f.sp = f.sr = scale;
+  f.sc = 1.f;
+  f.out = out;
+  f.init = initial_state;
+  f.fin = final_state;
+  f.si = value_dim;
+  f.sj = 1;
+  f.carry = reinterpret_cast<float*>(at);
+  f.dec = reinterpret_cast<float*>(at + up(static_cast<size_t>(w.J) * key_dim * value_dim * num_heads * 4));
+  f.out_f32 = dtype == ASCAN_F32;
+  return run_forms(l, 1, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                               const ascan_rows* log_gates, int gate_dtype, const ascan_rows* d_out,
+                               const float* initial_state, const float* final_state, const float* d_final_state,
+                               const void* cu_seqlens, int cu_index_type, int64_t num_seq, int64_t seq_total,
+                               int num_heads, int key_dim, int value_dim, int dtype, float scale, void* d_queries,
+                               void* d_keys, void* d_values, void* d_log_gates, float* d_initial_state,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(queries, keys, values, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, num_heads,
+                 key_dim, value_dim, dtype);
+  if (rc != ASCAN_OK) return rc;
+  if (seq_total == 0 || num_seq == 0) return ASCAN_OK;
+  if (!d_queries || !d_keys || !d_values || !d_log_gates || !rows_ok(d_out, num_heads) || d_out->heads != num_heads)
+    return ASCAN_EINVAL;
+  if (d_final_state && !final_state) return ASCAN_EINVAL;
+  const int H = num_heads, dk = key_dim, dv = value_dim;
+  const Plan w = make_plan(seq_total, num_seq, H, queries->heads, keys->heads, values->heads, log_gates->heads, dk, dv, true);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Launch l{};
+  l.p = problem_of(w, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, H);
+  char* at = static_cast<char*>(workspace);
+  auto take = [&](size_t n) {
+    char* p = n ? at : nullptr;
+    at += n;
+    return reinterpret_cast<float*>(p);
+  };
+  const Rows q = rows_of(queries, H), k = rows_of(keys, H), v = rows_of(values, H), o = rows_of(d_out, H);
+  const size_t mat = up(static_cast<size_t>(w.J) * dk * dv * H * 4);
+  for (int r = 0; r < 3; ++r) {
+    Form& f = l.f[r];
+    f.carry = take(w.carry);
+    f.dec = w.carry ? reinterpret_cast<float*>(reinterpret_cast<char*>(f.carry) + mat) : nullptr;
+    f.rev = r != 0;
+    f.sp = scale;
+    f.sr = r == 0 ? scale : 1.f;
+    f.sc = r == 0 ? 1.f : scale;
+    f.da = r == 2 ? dk : dv;
+    f.dc = r == 2 ? dv : dk;
+    f.si = r == 2 ? dv : 1;  // the user's states are [dk, dv]; dq and dk hold theirs transposed
+    f.sj = r == 2 ? 1 : dv;
+    f.a = r == 0 ? o : (r == 1 ? v : k);
+    f.b = r == 0 ? v : (r == 1 ? o : q);
+    f.c = r == 0 ? k : (r == 1 ? q : o);
+    f.init = r == 0 ? initial_state : d_final_state;
+    f.out_f32 = dtype == ASCAN_F32;
+  }
+  l.f[2].fin = d_initial_state;
+  l.f[0].snap = take(w.snap);
+  l.f[1].snap = take(w.snap);
+  l.f[0].rowdot = take(w.rowdot);
+  l.f[1].rowdot = take(w.rowdot);
+  l.f[0].dot = q;
+  l.f[1].dot = k;
+  float* parts[3] = {take(w.part_q), take(w.part_k), take(w.part_v)};
+  float* part_g = take(w.part_g);
+  void* outs[3] = {d_queries, d_keys, d_values};
+  const int heads[3] = {queries->heads, keys->heads, values->heads};
+  for (int r = 0; r < 3; ++r) {
+    l.f[r].out = parts[r] ? parts[r] : outs[r];
+    if (parts[r]) l.f[r].out_f32 = 1;
+  }
+  rc = run_forms(l, 3, dtype, s);
+  if (rc != ASCAN_OK) return rc;
+  gate_grad_kernel<<<dim3(l.p.J, H, static_cast<unsigned>(min(8ll, (w.seg + kRestart - 1) / kRestart))), 256, 0, s>>>(
+      l, final_state, d_final_state, part_g, d_log_gates, gate_dtype);
+  rc = launch_status();
+  auto sum = [&](const float* part, void* out, int heads_x, int dim, int type) {
+    if (!part || rc != ASCAN_OK) return;
+    const long long n = seq_total * heads_x * dim;
+    const unsigned grid = static_cast<unsigned>(min((n + 255) / 256, kSms * 16));
+    if (type == ASCAN_F32)
+      share_sum_kernel<float><<<grid, 256, 0, s>>>(part, static_cast<float*>(out), n, H / heads_x, dim);
+    else if (type == ASCAN_F16)
+      share_sum_kernel<__half><<<grid, 256, 0, s>>>(part, static_cast<__half*>(out), n, H / heads_x, dim);
+    else
+      share_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(part, static_cast<__nv_bfloat16*>(out), n, H / heads_x, dim);
+    rc = launch_status();
+  };
+  for (int r = 0; r < 3; ++r) sum(parts[r], outs[r], heads[r], r == 2 ? dv : dk, dtype);
+  sum(part_g, d_log_gates, log_gates->heads, 1, gate_dtype);
+  return rc;
+}
+
+int ascan_matrix_scan_step(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                           const ascan_rows* log_gates, int gate_dtype, const int32_t* slots, int64_t num_rows,
+                           int64_t pool_size, int num_heads, int key_dim, int value_dim, int dtype, float scale,
+                           const float* state, float* state_out, void* out, void* stream) {
+  if (num_rows < 0 || num_rows > 65535 || pool_size < 0 || num_heads <= 0 || num_heads > 65535 || key_dim <= 0 ||
+      value_dim <= 0 || value_dim > (1 << 20))
+    return ASCAN_EINVAL;
+  if (dtype < ASCAN_F32 || dtype > ASCAN_BF16 || gate_dtype < ASCAN_F32 || gate_dtype > ASCAN_BF16) return ASCAN_EINVAL;
+  if (num_rows == 0) return ASCAN_OK;
+  if (!rows_ok(queries, num_heads) || !rows_ok(keys, num_heads) || !rows_ok(values, num_heads) ||
+      !rows_ok(log_gates, num_heads) || !state || !state_out || !out)
+    return ASCAN_EINVAL;
+  if (!slots && num_rows > pool_size) return ASCAN_EINVAL;
+  StepArgs a{};
+  a.q = rows_of(queries, num_heads);
+  a.k = rows_of(keys, num_heads);
+  a.v = rows_of(values, num_heads);
+  a.gate = rows_of(log_gates, num_heads);
+  a.slots = slots;
+  a.state = state;
+  a.state_out = state_out;
+  a.out = out;
+  a.pool = pool_size;
+  a.H = num_heads;
+  a.dk = key_dim;
+  a.dv = value_dim;
+  a.gate_type = gate_dtype;
+  a.vec = value_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(state_out)) & 15u) == 0;
+  a.scale = scale;
+  a.err = g_err_host;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // Few (request, head) pairs: 32 columns a CTA instead of 128, four times
+  // the CTAs for the same bytes.
+  const bool narrow = num_rows * num_heads < kSms;
+  const unsigned cols = narrow ? 32 : 128;
+  const dim3 grid((value_dim + cols - 1) / cols, num_heads, static_cast<unsigned>(num_rows));
+#define MSCAN_STEP(T) (narrow ? (void)(step_kernel<T, 8><<<grid, 256, 0, s>>>(a)) : (void)(step_kernel<T, 32><<<grid, 256, 0, s>>>(a)))
+  if (dtype == ASCAN_F32) MSCAN_STEP(float);
+  else if (dtype == ASCAN_F16) MSCAN_STEP(__half);
+  else MSCAN_STEP(__nv_bfloat16);
+#undef MSCAN_STEP
+  return launch_status();
+}
+
+}  // extern "C"
+
+namespace ascan {
+ASCAN_UNIT_ERROR_ACCESSORS(mscan)
+}  // namespace ascan

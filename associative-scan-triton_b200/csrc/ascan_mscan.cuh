@@ -1,0 +1,156 @@
+// ascan_mscan.cuh -- the matrix-state recurrence: what its kernels share.
+//
+//   S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T        o[t] = scale * q[t] S[t]
+//
+// per head, S a [Dk, Dv] matrix in float32.  Over a chunk of tokens with
+// G[t] the inclusive sum of g inside the chunk this is
+//
+//   o[t]  = scale * (e^{G[t]} q[t] S_in + sum_{s<=t} e^{G[t]-G[s]} (q[t].k[s]) v[s])
+//   S_out = e^{G[C]} S_in + sum_s e^{G[C]-G[s]} k[s] v[s]^T
+//
+// i.e. two masked products and two products with the state.  The gradients
+// are the same form with the operands in other places:
+//
+//   dq: rows do, columns v, values k, forwards      (state: sum v k^T)
+//   dk: rows v, columns do, values q, backwards     (state: sum do q^T)
+//   dv: rows k, columns q, values do, backwards     (state: sum q do^T)
+//
+// where "backwards" masks s >= t, swaps the row factor e^{G[t]} with the
+// column factor e^{G[C]-G[s]} and walks the chunks from the last.  So one
+// kernel per data type serves the forward and all three gradients (`Form`).
+// The gate's gradient follows from the rows of two of them: with
+// a[t] = q[t].dq[t] and b[t] = k[t].dk[t],
+//
+//   dg[t] = sum_{u=t..e} (a[u] - b[u]) + <S[e], dS[e]>
+//
+// for any later token e of the sequence.  Taking e at most kRestart tokens
+// away (both state matrices are stored there) keeps the differences short;
+// one sum over a long sequence would lose the digits that the many terms
+// share.
+//
+// Work is split over heads and over segments of `seg` tokens of the packed
+// axis.  A segment that a sequence crosses needs the state that enters it: a
+// first launch computes each segment's own contribution (state_only), a
+// second one chains them, and the main launch starts every segment from its
+// carry.  Chunks never span two sequences, so no value of one sequence, not
+// even a NaN, meets another's.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ascan.h"
+
+namespace ascan {
+namespace mscan {
+
+constexpr int kRestart = 1024;     // tokens between stored states (gate gradients)
+constexpr float kGateFloor = -200.f;  // e^-200 is 0 in float32; keeps -inf out of differences
+
+struct Rows {  // [tokens, heads, dim] with unit stride along dim
+  const void* p;
+  long long st, sh;  // strides in elements
+  int share;         // problem heads per head of this tensor
+};
+
+struct Form {
+  Rows a, b, c;  // row, column and value operands
+  Rows dot;      // optional: row dots of the output with this tensor
+  int da, dc, rev;
+  float sp, sr, sc;  // factors of the scores, of the rows and of the columns
+  void* out;         // [BL, H, dc]
+  int out_f32;
+  float* rowdot;      // [H, BL]
+  const float* init;  // per sequence and head, element (i, j) at i*si + j*sj; may be null
+  float* fin;
+  long long si, sj;
+  float* carry;  // [J, H, da*dc]: the state that leaves a segment
+  float* dec;    // [J, H]: the decay over the segment's crossing piece
+  float* snap;   // [slots, H, da*dc] or null
+};
+
+struct Problem {
+  const void* cu;
+  int cu64, J, H, gate_type;
+  long long N, BL, seg;
+  Rows gate;  // [BL, heads, 1]
+  uint32_t* err;
+};
+
+struct Launch {
+  Problem p;
+  Form f[3];
+};
+
+__device__ __forceinline__ long long cu_at(const Problem& p, long long i) {
+  const long long v = p.cu64 ? static_cast<const long long*>(p.cu)[i]
+                             : static_cast<long long>(static_cast<const int*>(p.cu)[i]);
+  return v < 0 ? 0 : (v > p.BL ? p.BL : v);
+}
+
+// The first sequence whose end lies beyond token t (N if none does).
+__device__ __forceinline__ long long first_beyond(const Problem& p, long long t) {
+  long long lo = 0, hi = p.N;
+  while (lo < hi) {
+    const long long mid = (lo + hi) >> 1;
+    if (cu_at(p, mid + 1) > t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// The first sequence that starts at or after token t (N if none does).
+__device__ __forceinline__ long long first_from(const Problem& p, long long t) {
+  long long lo = 0, hi = p.N;
+  while (lo < hi) {
+    const long long mid = (lo + hi) >> 1;
+    if (cu_at(p, mid) >= t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ float load_any(const void* p, int type, long long i) {
+  if (type == ASCAN_F32) return static_cast<const float*>(p)[i];
+  if (type == ASCAN_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_any(void* p, int type, long long i, float x) {
+  if (type == ASCAN_F32) static_cast<float*>(p)[i] = x;
+  else if (type == ASCAN_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+}
+
+// A log gate; -inf (the state is dropped) and all that is 0 after exp in
+// float32 become one finite value, NaN stays NaN.
+__device__ __forceinline__ float load_gate(const Problem& p, long long t, int h) {
+  const float g = load_any(p.gate.p, p.gate_type, t * p.gate.st + (h / p.gate.share) * p.gate.sh);
+  return g < kGateFloor ? kGateFloor : g;
+}
+
+// Slot of the state stored at token `at`: stored positions of one sequence
+// are kRestart apart and at least as far from those of the next, so the
+// quotient is unique.
+__device__ __forceinline__ long long snap_slot(long long at) { return at / kRestart; }
+
+// The tensor-core kernel (ascan_mscan_tc.cu).
+bool tc_usable(const Launch& l, int roles, int dtype);
+int tc_run(const Launch& l, int roles, bool state_only, int dtype, cudaStream_t s);
+
+}  // namespace mscan
+}  // namespace ascan

@@ -64,6 +64,7 @@ enum ascan_status {
 #define ASCAN_DEV_ERR_CU_ORDER 0x2u     /* cu_seqlens not monotone / out of [0, seq_total] */
 #define ASCAN_DEV_ERR_LOOKBACK 0x4u     /* a tile predecessor never published (bounded wait expired) */
 #define ASCAN_DEV_ERR_EXCHANGE 0x8u     /* a peer rank's record or release never came (bounded wait expired) */
+#define ASCAN_DEV_ERR_INDEX 0x10u       /* a state slot or a position lies outside its table */
 
 /* Library identification. */
 ASCAN_API int ascan_abi_version(void);
@@ -322,6 +323,116 @@ ASCAN_API int ascan_backward_bidi(const void* grad_fwd, const void* gates_fwd,
                                   const void* cu_seqlens, int cu_index_type, int64_t num_seq,
                                   int64_t num_channels, int64_t seq_total, int dtype,
                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Matrix-state operators: the recurrence with a [Dk, Dv] state per head,
+ *
+ *   S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T,      o[t] = scale * q[t] S[t],
+ *
+ * its gradients and its one-token form, and the norm and rotation of queries
+ * and keys that stand before it.  No counterpart in the reference.
+ *
+ * Tokens are rows here: a tensor is [seq_total, heads, dim] with unit stride
+ * along dim and any token and head stride (views of a packed projection).
+ * num_heads is the number of states per sequence; the heads of every tensor
+ * divide it, and problem head h reads head h / (num_heads / heads).  States
+ * are float32 [num_seq, num_heads, key_dim, value_dim], contiguous.
+ */
+typedef struct ascan_rows {
+  const void* data;
+  int64_t stride_token, stride_head; /* in elements */
+  int32_t heads;
+} ascan_rows;
+
+#define ASCAN_MATRIX_SCAN_MAX_DIM 128 /* of key_dim and value_dim */
+
+/*
+ * Bytes of workspace of ascan_matrix_scan_forward (backward = 0) or
+ * ascan_matrix_scan_backward (backward = 1).
+ */
+ASCAN_API size_t ascan_matrix_scan_workspace(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads,
+                                             int key_heads, int value_heads, int gate_heads, int key_dim,
+                                             int value_dim, int backward);
+
+/*
+ * The recurrence over packed sequences (cu_seqlens as above).
+ *
+ *   log_gates      g, [seq_total, heads] of gate_dtype (dim is 1); -inf drops
+ *                  the state before the token
+ *   initial_state  NULL (zero) or the state before each sequence
+ *   out            [seq_total, num_heads, value_dim] contiguous; rows of no
+ *                  sequence are zeroed
+ *   final_state    NULL, or receives the state after each sequence (an empty
+ *                  sequence hands its initial state through)
+ */
+ASCAN_API int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                                        const ascan_rows* log_gates, int gate_dtype, const void* cu_seqlens,
+                                        int cu_index_type, int64_t num_seq, int64_t seq_total, int num_heads,
+                                        int key_dim, int value_dim, int dtype, float scale,
+                                        const float* initial_state, void* out, float* final_state, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
+/*
+ * Its gradients: d_queries, d_keys, d_values (contiguous, the inputs' heads),
+ * d_log_gates ([seq_total, gate heads] contiguous, gate_dtype) and, unless
+ * NULL, d_initial_state.  d_final_state may be NULL (zero); with it,
+ * final_state must hold the forward's.
+ */
+ASCAN_API int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                                         const ascan_rows* log_gates, int gate_dtype, const ascan_rows* d_out,
+                                         const float* initial_state, const float* final_state,
+                                         const float* d_final_state, const void* cu_seqlens, int cu_index_type,
+                                         int64_t num_seq, int64_t seq_total, int num_heads, int key_dim,
+                                         int value_dim, int dtype, float scale, void* d_queries, void* d_keys,
+                                         void* d_values, void* d_log_gates, float* d_initial_state, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
+/*
+ * One token of num_rows requests over a pool of states
+ * [pool_size, num_heads, key_dim, value_dim].  Row b uses state slots[b]
+ * (b itself when slots is NULL) and writes the new state to the same slot of
+ * state_out, which may be state; other slots are untouched.  A negative slot
+ * marks a row without a request: its output is zero.  A slot beyond the pool
+ * does the same and sets ASCAN_DEV_ERR_INDEX.  No two rows may name one slot.
+ */
+ASCAN_API int ascan_matrix_scan_step(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                                     const ascan_rows* log_gates, int gate_dtype, const int32_t* slots,
+                                     int64_t num_rows, int64_t pool_size, int num_heads, int key_dim, int value_dim,
+                                     int dtype, float scale, const float* state, float* state_out, void* out,
+                                     void* stream);
+
+/*
+ * RMS norm of every query and key head, weight, and rotation by position:
+ *
+ *   n = x * rsqrt(mean(x^2) + eps) * w
+ *   (n[i], n[j]) -> (n[i] cos - n[j] sin, n[j] cos + n[i] sin)
+ *
+ * over the first 2 * half elements of a head; pairs are (i, i + half), or
+ * (2i, 2i + 1) when interleaved.  cos and sin are float32 [table_rows, half].
+ * The position of a token is positions[t] (int32 or int64) or, when
+ * positions is NULL, its place in its sequence; tokens of no sequence give
+ * zero rows.  A position outside the table gives a zero row and sets
+ * ASCAN_DEV_ERR_INDEX.  Weights have weight_dtype.  Outputs are contiguous.
+ */
+ASCAN_API int ascan_qk_norm_rotate(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
+                                   const void* key_weight, int weight_dtype, const float* cos_table,
+                                   const float* sin_table, int64_t table_rows, int half, int interleaved,
+                                   const void* positions, const void* cu_seqlens, int index_type, int64_t num_seq,
+                                   int64_t tokens, int dim, int dtype, float eps, void* out_queries, void* out_keys,
+                                   void* stream);
+
+/* Bytes of workspace of ascan_qk_norm_rotate_backward. */
+ASCAN_API size_t ascan_qk_norm_rotate_workspace(int64_t tokens, int query_heads, int key_heads, int dim);
+
+/* Its gradients; d_query_weight and d_key_weight have weight_dtype. */
+ASCAN_API int ascan_qk_norm_rotate_backward(const ascan_rows* queries, const ascan_rows* keys,
+                                            const void* query_weight, const void* key_weight, int weight_dtype,
+                                            const float* cos_table, const float* sin_table, int64_t table_rows,
+                                            int half, int interleaved, const void* positions, const void* cu_seqlens,
+                                            int index_type, int64_t num_seq, int64_t tokens, int dim, int dtype,
+                                            float eps, const ascan_rows* d_out_queries, const ascan_rows* d_out_keys,
+                                            void* d_queries, void* d_keys, void* d_query_weight, void* d_key_weight,
+                                            void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Shift by one position inside every sequence and pad the vacated slot.

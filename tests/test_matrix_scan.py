@@ -1,0 +1,542 @@
+"""The matrix-state scan and its one-token step against a token-by-token float64 oracle.
+
+Tolerances (relative 2-norm per output, then largest error over the output's
+root mean square) follow from the arithmetic:
+
+* float32: sums of at most a few hundred float32 products, each rounded by
+  2^-24: 1e-5, ten times the root of the count.
+* 16-bit outputs: one rounding of the result (2^-8 for bfloat16, 2^-11 for
+  float16 at most, less than half of it as a root mean square) and at most one
+  of an operand inside each product, which averages to as much again: 2^-8 and
+  2^-11; single elements may cancel, so 16 times that against the root mean
+  square.
+* float32 outputs of 16-bit inputs (states, gate gradients): the inputs are
+  exact, operands that are computed keep at least 16 bits: 2e-5.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import associative_scan_triton as ast
+from associative_scan_triton import _lib
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TOL = {F32: 1e-5, F16: 2.0**-11, BF16: 2.0**-8}
+STATE_TOL = 2e-5
+
+
+def oracle(q, k, v, g, lengths, scale, s0=None, first=0):
+  """Token by token in float64; leaves may require gradients.  (out, final)."""
+  heads = max(x.shape[1] for x in (q, k, v, g))
+  q, k, v, g = (x.repeat_interleave(heads // x.shape[1], 1) for x in (q, k, v, g))
+  outs = [q.new_zeros(first, heads, v.shape[2])]
+  finals, at = [], first
+  for n, length in enumerate(lengths):
+    state = s0[n] if s0 is not None else q.new_zeros(heads, q.shape[2], v.shape[2])
+    for t in range(at, at + length):
+      state = state * torch.exp(g[t])[:, None, None] + k[t][:, :, None] * v[t][:, None, :]
+      outs.append(scale * (q[t][:, :, None] * state).sum(1)[None])
+    finals.append(state)
+    at += length
+  return torch.cat(outs), torch.stack(finals)
+
+
+def close(name, got, want, tol):
+  got, want = got.detach().double().cpu(), want.detach().double().cpu()
+  assert got.shape == want.shape, (name, got.shape, want.shape)
+  assert torch.isfinite(got).all(), f"{name} has values that are not finite"
+  rms = float(want.square().mean().sqrt()) if want.numel() else 0.0
+  err = (got - want).abs()
+  norm = float(want.norm())
+  assert float(err.norm()) <= tol * norm + 1e-30, (name, float(err.norm()) / max(norm, 1e-30), tol)
+  if want.numel():
+    worst = float((err / torch.clamp(want.abs(), min=rms)).max()) if rms else float(err.max())
+    assert worst <= 16 * tol, (name, worst, 16 * tol)
+
+
+def make(lengths, heads, dims, dtype, seed=0, gate_dtype=F32, carry=False, first=0, rate=0.3):
+  """Inputs on the CPU in their type: q, k, v, g, s0, d_out, d_final."""
+  gen = torch.Generator().manual_seed(seed)
+  hq, hk, hv, hg = heads
+  h, (dk, dv), n = max(heads), dims, first + sum(lengths)
+
+  def normal(*shape):
+    return torch.randn(shape, generator=gen)
+
+  q = normal(n, hq, dk).to(dtype)
+  k = normal(n, hk, dk).to(dtype)
+  v = normal(n, hv, dv).to(dtype)
+  g = (-rate * torch.rand(n, hg, generator=gen)**2).to(gate_dtype)
+  s0 = normal(len(lengths), h, dk, dv) * 2 if carry else None
+  d_out = normal(n, h, dv).to(dtype)
+  d_final = normal(len(lengths), h, dk, dv) if carry else None
+  return q, k, v, g, s0, d_out, d_final
+
+
+def cu_of(lengths, first=0, dtype=torch.int32):
+  ends = [first]
+  for m in lengths:
+    ends.append(ends[-1] + m)
+  return torch.tensor(ends, dtype=dtype, device=DEV)
+
+
+def check_forward(lengths, heads, dims, dtype, **kw):
+  q, k, v, g, s0, _, _ = make(lengths, heads, dims, dtype, **kw)
+  first = kw.get("first", 0)
+  out, final = ast.matrix_scan_causal(
+    q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), {"cu_seqlens": cu_of(lengths, first)},
+    initial_state=None if s0 is None else s0.to(DEV), return_final_state=True)
+  assert out.dtype == dtype and final.dtype == F32
+  want, want_final = oracle(q.double(), k.double(), v.double(), g.double(), lengths,
+                            dims[0]**-0.5, None if s0 is None else s0.double(), first)
+  close("out", out, want, TOL[dtype])
+  close("final_state", final, want_final, STATE_TOL)
+
+
+LENGTHS = [[1], [2], [0, 1, 0, 2, 0], [31, 32, 33], [127, 128, 129], [64, 0, 257, 5], [700, 1, 511]]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_forward_lengths(lengths, dtype):
+  check_forward(lengths, (2, 2, 2, 2), (64, 64), dtype, carry=True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dims", [(128, 128), (64, 128), (128, 64), (16, 8), (1, 1), (40, 72), (96, 33),
+                                  (127, 80), (3, 128), (128, 1)], ids=str)
+def test_forward_head_sizes(dims, dtype):
+  check_forward([150, 3], (3, 3, 3, 3), dims, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads", [(1, 1, 1, 1), (4, 1, 1, 1), (2, 2, 4, 4), (1, 2, 4, 1), (6, 3, 2, 6),
+                                   (4, 4, 1, 4)], ids=str)
+def test_forward_shared_heads(heads, dtype):
+  check_forward([130, 70], heads, (64, 64), dtype, gate_dtype=dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lengths", [[2600], [1024, 1024, 512], [100, 2300, 3]], ids=str)
+def test_forward_across_segments(lengths, dtype):
+  # one head of few tokens per SM: the packed axis is cut into many segments
+  check_forward(lengths, (1, 1, 1, 1), (64, 64), dtype, carry=True, rate=0.02)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_tokens_of_no_sequence(dtype):
+  # rows before cu_seqlens[0] hold NaN: they are not read, and come out zero
+  q, k, v, g, _, _, _ = make([60, 90], (2, 2, 2, 2), (64, 64), dtype, first=37)
+  clean = [x.clone() for x in (q, k, v, g)]
+  for x in (q, k, v, g):
+    x[:37] = math.nan
+  out = ast.matrix_scan_causal(*(x.to(DEV) for x in (q, k, v, g)),
+                               {"cu_seqlens": cu_of([60, 90], 37, torch.int64)})
+  want, _ = oracle(*(x.double() for x in clean), [60, 90], 64**-0.5, first=37)
+  assert not out[:37].any()
+  close("out", out, want, TOL[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("gates", ["drop", "one", "steep", "mixed", "growing"])
+def test_gates(gates, dtype):
+  lengths = [200, 77]
+  q, k, v, g, s0, _, _ = make(lengths, (2, 2, 2, 2), (64, 64), dtype, carry=True)
+  if gates == "drop":  # nothing is kept anywhere: every row sees itself alone
+    g.fill_(-math.inf)
+  elif gates == "one":
+    g.zero_()
+  elif gates == "steep":  # sums of thousands inside a chunk
+    g.fill_(-37.5)
+    g[::3] = -0.01
+  elif gates == "mixed":
+    g[torch.randperm(277, generator=torch.Generator().manual_seed(3))[:60]] = -math.inf
+  else:
+    g = g * -0.1
+  out, final = ast.matrix_scan_causal(*(x.to(DEV) for x in (q, k, v, g)),
+                                      {"cu_seqlens": cu_of(lengths)}, initial_state=s0.to(DEV),
+                                      return_final_state=True)
+  want, want_final = oracle(q.double(), k.double(), v.double(), g.double(), lengths, 64**-0.5,
+                            s0.double())
+  close("out", out, want, TOL[dtype])
+  close("final_state", final, want_final, STATE_TOL)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("where", [0, 1, 2])
+def test_values_that_are_not_finite_stay_behind_the_mask(where, bad, dtype):
+  # a bad query, key or value at token t touches no earlier token of its
+  # sequence and no token of another
+  lengths = [90, 150, 40]
+  tensors = list(make(lengths, (2, 2, 2, 2), (64, 64), dtype)[:4])
+  want, _ = oracle(*(x.double() for x in tensors), lengths, 64**-0.5)
+  t = 90 + 71
+  tensors[where][t, 1, 5] = bad
+  out = ast.matrix_scan_causal(*(x.to(DEV) for x in tensors), {"cu_seqlens": cu_of(lengths)})
+  keep = torch.ones(280, 2, dtype=torch.bool)
+  keep[t if where == 0 else slice(t, 240), 1] = False
+  close("out", out.cpu()[keep], want[keep], TOL[dtype])
+  assert not torch.isfinite(out[t, 1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strided_and_misaligned_inputs(dtype):
+  # views of one packed projection, and the same shifted by one element
+  lengths, h, d = [100, 61], 3, 64
+  gen = torch.Generator().manual_seed(5)
+  flat = torch.randn(161 * (3 * h * d + h) + 1, generator=gen).to(dtype).to(DEV)
+  gates = (-0.2 * torch.rand(h, 161, generator=gen)).to(DEV).t()
+  for shift in (0, 1):
+    packed = flat[shift:shift + 161 * (3 * h * d + h)].view(161, -1)
+    q, k, v = (packed[:, i * h * d:(i + 1) * h * d].view(161, h, d) for i in range(3))
+    out = ast.matrix_scan_causal(q, k, v, gates, {"cu_seqlens": cu_of(lengths)})
+    want, _ = oracle(*(x.double().cpu() for x in (q, k, v, gates)), lengths, d**-0.5)
+    close(f"out shifted by {shift}", out, want, TOL[dtype])
+
+
+def run_gradients(tensors, lengths, scale=None, first=0, use=("out", "final")):
+  """(our gradients, the oracle's) of sum(out*d_out) + sum(final*d_final)."""
+  q, k, v, g, s0, d_out, d_final = tensors
+  leaves = [x.to(DEV).requires_grad_(True) for x in (q, k, v, g)]
+  init = None if s0 is None else s0.to(DEV).requires_grad_(True)
+  out, final = ast.matrix_scan_causal(*leaves, {"cu_seqlens": cu_of(lengths, first)}, scale=scale,
+                                      initial_state=init, return_final_state=True)
+  ends = [x for x, name in ((out, "out"), (final, "final")) if name in use]
+  grads = [x.to(DEV) for x, name in ((d_out, "out"), (d_final, "final")) if name in use]
+  wrt = leaves + ([init] if init is not None else [])
+  ours = torch.autograd.grad(ends, wrt, grads)
+  leaves = [x.double().requires_grad_(True) for x in (q, k, v, g)]
+  init = None if s0 is None else s0.double().requires_grad_(True)
+  out, final = oracle(*leaves, lengths, scale if scale is not None else q.shape[2]**-0.5, init, first)
+  ends = [x for x, name in ((out, "out"), (final, "final")) if name in use]
+  wrt = leaves + ([init] if init is not None else [])
+  gold = torch.autograd.grad(ends, wrt, [x.cpu().double() for x in grads], allow_unused=True)
+  return ours, [torch.zeros_like(w) if x is None else x for x, w in zip(gold, wrt)]
+
+
+NAMES = ("d_queries", "d_keys", "d_values", "d_log_gates", "d_initial_state")
+
+
+def check_gradients(tensors, lengths, dtype, gate_dtype=F32, **kw):
+  ours, gold = run_gradients(tensors, lengths, **kw)
+  for name, a, b in zip(NAMES, ours, gold):
+    tol = TOL[dtype]
+    if name == "d_initial_state" or (name == "d_log_gates" and gate_dtype == F32):
+      tol = STATE_TOL
+    assert a.dtype == (F32 if name == "d_initial_state" else
+                       gate_dtype if name == "d_log_gates" else dtype)
+    close(name, a, b, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_gradient_lengths(lengths, dtype):
+  check_gradients(make(lengths, (2, 2, 2, 2), (64, 64), dtype, carry=True), lengths, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dims", [(128, 128), (64, 128), (128, 64), (40, 72), (5, 1)], ids=str)
+def test_gradient_head_sizes(dims, dtype):
+  check_gradients(make([140, 9], (2, 2, 2, 2), dims, dtype), [140, 9], dtype, use=("out",))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads", [(4, 1, 1, 1), (2, 2, 4, 4), (1, 2, 4, 1), (6, 3, 2, 6)], ids=str)
+def test_gradient_shared_heads(heads, dtype):
+  tensors = make([90, 50], heads, (64, 64), dtype, gate_dtype=dtype)
+  check_gradients(tensors, [90, 50], dtype, gate_dtype=dtype, use=("out",))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rate", [0.002, 0.3, 6.0])
+def test_gradient_across_segments_and_stored_states(rate, dtype):
+  lengths = [100, 2500]
+  tensors = make(lengths, (1, 1, 1, 1), (64, 64), dtype, carry=True, rate=rate)
+  check_gradients(tensors, lengths, dtype)
+
+
+@gpu
+def test_gradient_of_the_final_state_alone():
+  tensors = make([70, 0, 200], (2, 2, 2, 2), (64, 64), F32, carry=True)
+  check_gradients(tensors, [70, 0, 200], F32, use=("final",))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_scale_gates_and_outside_tokens(dtype):
+  tensors = list(make([80, 75], (2, 1, 2, 2), (64, 64), dtype, first=11))
+  tensors[3][30::17] = -math.inf
+  ours, gold = run_gradients(tensors, [80, 75], scale=0.3, first=11, use=("out",))
+  for name, a, b in zip(NAMES, ours, gold):
+    if name == "d_log_gates":  # exp's own gradient at -inf is 0; so is ours
+      b = torch.where(torch.isfinite(tensors[3].double()), b, torch.zeros_like(b))
+    close(name, a, b, STATE_TOL if name == "d_log_gates" else TOL[dtype])
+    assert not a[:11].any()
+
+
+@gpu
+def test_gradient_by_differences():
+  # central differences of a float64 evaluation of the loss at float32 inputs
+  # moved by +-h: truncation h^2 ~ 1e-8, so only our own 1e-5 remains; 1e-4
+  lengths = [50, 90]
+  tensors = make(lengths, (2, 1, 2, 2), (32, 32), F32, carry=True)
+  q, k, v, g, s0, d_out, d_final = tensors
+  ours, _ = run_gradients(tensors, lengths)
+  gen = torch.Generator().manual_seed(9)
+  base = [x.double() for x in (q, k, v, g, s0)]
+
+  def loss(parts):
+    out, final = oracle(*parts[:4], lengths, 32**-0.5, parts[4])
+    return float((out * d_out.double()).sum() + (final * d_final.double()).sum())
+
+  for i, name in enumerate(NAMES):
+    direction = torch.randn(base[i].shape, generator=gen, dtype=torch.float64)
+    h = 1e-4
+    up = [x + h * direction if j == i else x for j, x in enumerate(base)]
+    down = [x - h * direction if j == i else x for j, x in enumerate(base)]
+    slope = (loss(up) - loss(down)) / (2 * h)
+    ours_slope = float((ours[i].double().cpu() * direction).sum())
+    size = float(ours[i].double().norm())
+    assert abs(slope - ours_slope) <= 1e-4 * size, (name, slope, ours_slope)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
+  lengths = [300, 1000]
+  q, k, v, g, s0, _, _ = (x if x is None else x.to(DEV)
+                          for x in make(lengths, (2, 2, 2, 2), (64, 64), dtype, carry=True))
+  args = {"cu_seqlens": cu_of(lengths)}
+
+  def call():
+    return ast.matrix_scan_causal(q, k, v, g, args, initial_state=s0, return_final_state=True)
+
+  first = call()
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    second = call()
+  torch.cuda.current_stream().wait_stream(side)
+  sync_check = _lib.sync_check_enabled()
+  _lib.set_sync_check(False)  # a synchronisation is not allowed while capturing
+  try:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      third = call()
+    for x in third:
+      x.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+  finally:
+    _lib.set_sync_check(sync_check)
+  for a, b, c in zip(first, second, third):
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@gpu
+def test_empty_inputs():
+  q = torch.empty(0, 2, 16, device=DEV, requires_grad=True)
+  g = torch.empty(0, 2, device=DEV)
+  s0 = torch.randn(2, 2, 16, 16, device=DEV)
+  out, final = ast.matrix_scan_causal(q, q, q, g, {"cu_seqlens": cu_of([0, 0])}, initial_state=s0,
+                                      return_final_state=True)
+  assert out.shape == (0, 2, 16) and torch.equal(final, s0)
+  out.sum().backward()
+  assert q.grad.shape == q.shape
+
+
+@gpu
+def test_malformed_sequences_are_reported():
+  q = torch.randn(50, 1, 32, device=DEV)
+  g = torch.zeros(50, 1, device=DEV)
+  for cu in ([0, 49], [0, 60], [0, 30, 20, 50], [-3, 50]):
+    with pytest.raises(ast.ScanError, match="cu_seqlens"):
+      ast.matrix_scan_causal(q, q, q, g, {"cu_seqlens": torch.tensor(cu, device=DEV)})
+      ast.check_device_error()
+
+
+@gpu
+def test_refusals():
+  q = torch.randn(10, 2, 32, device=DEV)
+  g = torch.zeros(10, 2, device=DEV)
+  args = {"cu_seqlens": cu_of([10])}
+
+  def refused(error, match, q=q, k=q, v=q, g=g, **kw):
+    with pytest.raises(error, match=match):
+      ast.matrix_scan_causal(q, k, v, g, {**args, **kw.pop("args", {})}, **kw)
+
+  refused(ValueError, "CUDA tensors only", q=q.cpu())
+  refused(TypeError, "keys has dtype", k=q.half())
+  refused(TypeError, "unsupported dtype", q=q.double())
+  refused(TypeError, "log_gates must be", g=g.half())
+  refused(ValueError, "3 dimensions", v=q[0])
+  refused(ValueError, "2 dimensions", g=q)
+  refused(ValueError, "rows", v=q[:9])
+  refused(ValueError, "head size", k=q[..., :16])
+  refused(ValueError, "unit stride", v=q.transpose(1, 2).contiguous().transpose(1, 2))
+  refused(ValueError, "divide", v=torch.randn(10, 3, 32, device=DEV))
+  refused(ValueError, "head sizes up to 128", v=torch.randn(10, 2, 129, device=DEV))
+  refused(TypeError, "int32 or int64", args={"cu_seqlens": args["cu_seqlens"].float()})
+  refused(ValueError, "one dimension", args={"cu_seqlens": args["cu_seqlens"][None]})
+  refused(ValueError, "initial_state has shape", initial_state=torch.zeros(1, 2, 32, 31, device=DEV))
+  refused(TypeError, "initial_state must be float32",
+          initial_state=torch.zeros(1, 2, 32, 32, device=DEV, dtype=F16))
+
+
+def test_cpu_tensors_are_refused():
+  q = torch.zeros(4, 1, 8)
+  g = torch.zeros(4, 1)
+  cu = torch.tensor([0, 4])
+  with pytest.raises(ValueError, match="CUDA tensors only"):
+    ast.matrix_scan_causal(q, q, q, g, {"cu_seqlens": cu})
+  with pytest.raises(ValueError, match="CUDA tensors only"):
+    ast.matrix_scan_step(q, q, q, g, torch.zeros(4, 1, 8, 8))
+
+
+def test_abi_rejects_bad_arguments_without_a_gpu():
+  import ctypes
+  lib = _lib.load()
+  r = ctypes.byref(_lib.Rows(1 << 20, 8, 8, 1))
+  three = ctypes.byref(_lib.Rows(1 << 20, 8, 8, 3))
+  none = ctypes.byref(_lib.Rows(None, 8, 8, 1))
+  ok = [r, r, r, r, 0, 1 << 20, 0, 1, 4, 2, 8, 8, 0, 1.0, None, 1 << 20, None, None, 0, None]
+
+  def rc(**changes):
+    a = list(ok)
+    for at, value in changes.items():
+      a[int(at[1:])] = value
+    return lib.ascan_matrix_scan_forward(*a)
+
+  assert rc() == -2  # everything in order but the workspace
+  for changes in ({"_0": three}, {"_1": none}, {"_4": 3}, {"_5": None}, {"_6": 2}, {"_7": -1},
+                  {"_8": -1}, {"_9": 0}, {"_10": 129}, {"_11": 0}, {"_12": 5}, {"_15": None}):
+    assert rc(**changes) == -1, changes
+  assert rc(_8=0) == 0 and rc(_7=0) == 0
+  assert lib.ascan_matrix_scan_workspace(0, 0, 0, 0, 0, 0, 0, 0, 0, 0) >= 256
+  small = lib.ascan_matrix_scan_workspace(4096, 1, 2, 2, 2, 2, 2, 64, 64, 0)
+  assert lib.ascan_matrix_scan_workspace(4096, 1, 2, 2, 2, 2, 2, 64, 64, 1) > small
+
+
+# ---------------------------------------------------------------------------
+# one token
+# ---------------------------------------------------------------------------
+
+
+def step_oracle(q, k, v, g, state, scale):
+  heads = state.shape[1]
+  q, k, v, g = (x.double().repeat_interleave(heads // x.shape[1], 1) for x in (q, k, v, g))
+  new = state.double() * torch.exp(g)[..., None, None] + k[..., :, None] * v[..., None, :]
+  return scale * (q[..., None] * new).sum(-2), new
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dims", [(128, 128), (64, 32), (40, 72), (7, 5), (200, 260)], ids=str)
+@pytest.mark.parametrize("batch", [1, 3, 170])
+def test_step(batch, dims, dtype):
+  heads, (dk, dv) = (2, 1, 4, 4), dims
+  q, k, v, g, _, _, _ = (x if x is None else x.to(DEV) for x in make([batch], heads, dims, dtype))
+  gen = torch.Generator().manual_seed(1)
+  pool = torch.randn(batch + 5, 4, dk, dv, generator=gen).to(DEV)
+  slots = torch.randperm(batch + 5, generator=gen)[:batch].to(torch.int32).to(DEV)
+  want, new = step_oracle(q, k, v, g, pool[slots.long()], 0.5)
+  before = pool.clone()
+  other = torch.full_like(pool, 7.0)
+  out = ast.matrix_scan_step(q, k, v, g, pool, slots=slots, scale=0.5, state_out=other)
+  assert torch.equal(pool, before)
+  close("out", out, want, TOL[dtype])
+  close("state", other[slots.long()], new, 1e-6)
+  idle = torch.ones(batch + 5, dtype=torch.bool, device=DEV)
+  idle[slots.long()] = False
+  assert (other[idle] == 7.0).all()
+  again = ast.matrix_scan_step(q, k, v, g, pool, slots=slots, scale=0.5)
+  assert torch.equal(out, again) and torch.equal(pool[slots.long()], other[slots.long()])
+  assert torch.equal(pool[idle], before[idle])
+
+
+@gpu
+def test_step_idle_rows_and_slots_outside_the_pool():
+  q, k, v, g, _, _, _ = (x if x is None else x.to(DEV) for x in make([3], (2, 2, 2, 2), (32, 32), F32))
+  pool = torch.randn(4, 2, 32, 32, device=DEV)
+  before = pool.clone()
+  q[1] = k[1] = v[1] = math.nan
+  slots = torch.tensor([2, -1, 0], dtype=torch.int32, device=DEV)
+  want, new = step_oracle(q, k, v, g, before[slots.long()], 32**-0.5)
+  out = ast.matrix_scan_step(q, k, v, g, pool, slots=slots)
+  assert not out[1].any()
+  close("out", out[[0, 2]], want[[0, 2]], 1e-5)
+  assert torch.equal(pool[[1, 3]], before[[1, 3]])
+  with pytest.raises(ast.ScanError, match="slot"):
+    ast.matrix_scan_step(q, k, v, g, pool, slots=slots + 2)
+    ast.check_device_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_step_continues_the_scan(dtype):
+  lengths = [40, 3]
+  q, k, v, g, s0, _, _ = (x if x is None else x.to(DEV)
+                          for x in make(lengths, (2, 2, 2, 2), (64, 64), dtype, carry=True))
+  whole, final = ast.matrix_scan_causal(q, k, v, g, {"cu_seqlens": cu_of(lengths)}, initial_state=s0,
+                                        return_final_state=True)
+  head = torch.cat((torch.arange(39), torch.arange(40, 42))).to(DEV)
+  _, state = ast.matrix_scan_causal(*(x[head] for x in (q, k, v, g)), {"cu_seqlens": cu_of([39, 2])},
+                                    initial_state=s0, return_final_state=True)
+  last = torch.tensor([39, 42], device=DEV)
+  out = ast.matrix_scan_step(*(x[last] for x in (q, k, v, g)), state)
+  close("out", out, whole[last].double(), 2 * TOL[dtype])
+  close("state", state, final.double(), 2 * STATE_TOL)
+
+
+@gpu
+def test_step_refusals():
+  q = torch.randn(3, 2, 16, device=DEV)
+  g = torch.zeros(3, 2, device=DEV)
+  pool = torch.zeros(4, 2, 16, 16, device=DEV)
+  slots = torch.arange(3, dtype=torch.int32, device=DEV)
+
+  def refused(error, match, g=g, state=pool, **kw):
+    with pytest.raises(error, match=match):
+      ast.matrix_scan_step(q, q, q, g, state, **kw)
+
+  refused(ValueError, "state has shape", state=pool[:, :1])
+  refused(TypeError, "state must be float32", state=pool.half())
+  refused(ValueError, "slots must be", slots=slots.long())
+  refused(ValueError, "slots must be", slots=slots[:2])
+  refused(ValueError, "need 3 states", state=pool[:2].contiguous())
+  both = torch.zeros(5, 2, 16, 16, device=DEV)
+  refused(ValueError, "overlaps", state=both[:4], state_out=both[1:])
+  refused(ValueError, "no backward", g=g.clone().requires_grad_(True))
+
+
+@gpu
+@pytest.mark.slow
+def test_step_pool_beyond_32_bit_offsets():
+  slots_total = 2**31 // (128 * 128) + 3
+  pool = torch.empty(slots_total, 1, 128, 128, device=DEV)
+  q, k, v, g, _, _, _ = (x if x is None else x.to(DEV) for x in make([2], (1, 1, 1, 1), (128, 128), F32))
+  slots = torch.tensor([slots_total - 1, 0], dtype=torch.int32, device=DEV)
+  pool[slots.long()] = torch.randn(2, 1, 128, 128, device=DEV)
+  want, new = step_oracle(q, k, v, g, pool[slots.long()], 128**-0.5)
+  out = ast.matrix_scan_step(q, k, v, g, pool, slots=slots)
+  close("out", out, want, 1e-5)
+  close("state", pool[slots.long()], new, 1e-6)
