@@ -35,6 +35,7 @@ DEV_ERR_CU_ORDER = 0x2
 DEV_ERR_LOOKBACK = 0x4
 DEV_ERR_EXCHANGE = 0x8
 DEV_ERR_INDEX = 0x10
+DEV_ERR_STAGE = 0x20
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 INDEX_CODES = {torch.int32: 0, torch.int64: 1}
@@ -276,6 +277,8 @@ def describe_device_error(code: int) -> str:
                  "bounded wait")
   if code & DEV_ERR_INDEX:
     parts.append("a state slot or a position lies outside its table")
+  if code & DEV_ERR_STAGE:
+    parts.append("a stage of the matrix scan did not finish within the bounded wait")
   return "; ".join(parts) or f"device error {code:#x}"
 
 

@@ -4,18 +4,13 @@
 // over shared heads, and the one-token step.
 #include "ascan_impl.cuh"
 #include "ascan_mscan.cuh"
+#include "ascan_mscan_common.cuh"
 
 namespace ascan {
 namespace mscan {
 
 constexpr int kPlainThreads = 256;
 constexpr int kPlainChunk = 32;
-
-// cu_seqlens as the scans check it; every other read of it is clamped.
-__device__ void check_cu(const Problem& p) {
-  if (p.cu64) validate_cu(static_cast<const int64_t*>(p.cu), p.N, p.BL, p.err);
-  else validate_cu(static_cast<const int32_t*>(p.cu), p.N, p.BL, p.err);
-}
 
 // ---------------------------------------------------------------------------
 // The plain kernel: one CTA per (segment, head, form), fused multiply-adds.
@@ -65,25 +60,7 @@ __global__ void __launch_bounds__(kPlainThreads)
   const long long mat = static_cast<long long>(da) * dc;
   const long long t0 = j * p.seg, t1 = min(t0 + p.seg, p.BL);
 
-  if (!state_only) {
-    if (j == 0 && h == 0 && blockIdx.z == 0) check_cu(p);
-    // rows that belong to no sequence
-    const long long c0 = min(t1, cu_at(p, 0)), c1 = max(t0, cu_at(p, p.N));
-    for (long long t = t0; t < t1; ++t) {
-      if (t >= c0 && t < c1) { t = c1 - 1; continue; }
-      for (int d = tid; d < dc; d += kPlainThreads) {
-        const long long at = (t * p.H + h) * dc + d;
-        if (f.out_f32) static_cast<float*>(f.out)[at] = 0.f;
-        else static_cast<T*>(f.out)[at] = from_f<T>(0.f);
-      }
-      if (f.rowdot && tid == 0) f.rowdot[h * p.BL + t] = 0.f;
-    }
-    if (f.fin && j == 0)  // empty sequences hand their state through
-      for (long long n = 0; n < p.N; ++n)
-        if (cu_at(p, n + 1) <= cu_at(p, n))
-          for (long long e = tid; e < mat; e += kPlainThreads)
-            f.fin[(n * p.H + h) * mat + e] = f.init ? f.init[(n * p.H + h) * mat + e] : 0.f;
-  }
+  if (!state_only) fill_outside<T>(p, f);
 
   const long long n_first = first_beyond(p, t0);
   const long long n_last = first_from(p, t1);  // one past the last sequence that starts before t1
@@ -528,8 +505,9 @@ static int plain_run(const Launch& l, int roles, bool state_only, int dtype, cud
 
 static int run_forms(const Launch& l, int roles, int dtype, cudaStream_t s) {
   int rc = ASCAN_OK;
+  const bool tc = tc_usable(l, roles, dtype);
   if (l.p.J > 1) {
-    rc = plain_run(l, roles, true, dtype, s);
+    rc = tc ? tc_run(l, roles, true, s) : plain_run(l, roles, true, dtype, s);
     if (rc != ASCAN_OK) return rc;
     long long mat = 0;
     for (int r = 0; r < roles; ++r) mat = max(mat, static_cast<long long>(l.f[r].da) * l.f[r].dc);
@@ -537,7 +515,7 @@ static int run_forms(const Launch& l, int roles, int dtype, cudaStream_t s) {
     rc = launch_status();
     if (rc != ASCAN_OK) return rc;
   }
-  return plain_run(l, roles, false, dtype, s);
+  return tc ? tc_run(l, roles, false, s) : plain_run(l, roles, false, dtype, s);
 }
 
 struct Plan {
@@ -579,10 +557,6 @@ static bool rows_ok(const ascan_rows* r, int H) {
 
 static Rows rows_of(const ascan_rows* r, int H) {
   return Rows{r->data, r->stride_token, r->stride_head, H / r->heads};
-}
-
-static Rows packed_rows(const void* p, int heads, int dim, int H) {
-  return Rows{p, static_cast<long long>(heads) * dim, dim, H / heads};
 }
 
 static int check(const ascan_rows* q, const ascan_rows* k, const ascan_rows* v, const ascan_rows* g, int gate_dtype,
@@ -697,6 +671,7 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
     f.carry = take(w.carry);
     f.dec = w.carry ? reinterpret_cast<float*>(reinterpret_cast<char*>(f.carry) + mat) : nullptr;
     f.rev = r != 0;
+    f.exact = r != 2;  // the gate's gradient needs their rows in float32
     f.sp = scale;
     f.sr = r == 0 ? scale : 1.f;
     f.sc = r == 0 ? 1.f : scale;

@@ -59,6 +59,7 @@ struct Form {
   Rows a, b, c;  // row, column and value operands
   Rows dot;      // optional: row dots of the output with this tensor
   int da, dc, rev;
+  int exact;         // tensor cores: keep 16 bits of every computed operand
   float sp, sr, sc;  // factors of the scores, of the rows and of the columns
   void* out;         // [BL, H, dc]
   int out_f32;
@@ -150,7 +151,7 @@ __device__ __forceinline__ long long snap_slot(long long at) { return at / kRest
 
 // The tensor-core kernel (ascan_mscan_tc.cu).
 bool tc_usable(const Launch& l, int roles, int dtype);
-int tc_run(const Launch& l, int roles, bool state_only, int dtype, cudaStream_t s);
+int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s);
 
 }  // namespace mscan
 }  // namespace ascan

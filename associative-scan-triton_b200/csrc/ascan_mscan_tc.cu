@@ -1,0 +1,853 @@
+// ascan_mscan_tc.cu -- compilation unit of the scan library: the matrix-state
+// recurrence on the fifth-generation tensor cores (bfloat16).
+//
+// One CTA per (segment, head, form) walks its chunks of 128 tokens.  Per chunk
+//
+//   scores = A B^T            A, B from shared memory            [128, 128]
+//   O      = A S              S the state entering the chunk     [128, dc]
+//   U     += (col . B)^T C    the state, kept in tensor memory   [da, dc]
+//   O      = row . O + P C    P = masked, decayed scores
+//
+// with float32 accumulators in tensor memory.  What is computed on the way to
+// an operand would lose digits as one bfloat16: col.B is split into two
+// (16 bits together), and so are P and S where a float32 result (the gate's
+// gradient) depends on them.  A and C come as stored, so they are exact.
+//
+// Roles, by warp (one CTA per SM; every hand-over is an mbarrier):
+//   0-3    row warps: scores -> P in place in tensor memory, scale O by the
+//          row factors, store the finished rows
+//   4-7    state warps: the state from tensor memory to the operand S in
+//          shared memory, scaled back for the next update
+//   8-11   column warps: (col . B)^T transposed into tensor memory; tails and
+//          values that are not finite in C
+//   12     TMA loads of the A, B, C tiles into a ring of shared-memory slots
+//   13     issues the products
+//   14     the chunk's gate sums, row and column factors
+//
+// Tensor memory (512 columns of 128 lanes): scores/P 128, O 128, U 128,
+// (col.B)^T 64 + 64.  Lanes are tokens for scores and O, state rows for U.
+//
+// A token whose value is not finite would reach earlier rows of its chunk
+// through 0 * NaN; the column warps replace such values by zero and note the
+// first token of each column, and the row and state warps put NaN where the
+// mask lets the value through.
+//
+// Every wait is bounded: one that runs out sets the device error word and an
+// abort flag, every role then leaves its loop, loads and products in flight
+// are waited for, and tensor memory is freed.
+#include "ascan_impl.cuh"
+#include "ascan_mscan.cuh"
+#include "ascan_mscan_common.cuh"
+
+namespace ascan {
+namespace mscan {
+
+constexpr int kC = 128;             // tokens of a chunk
+constexpr int kTcWarps = 15;
+constexpr int kTcThreads = kTcWarps * 32;
+constexpr int kMaxSlots = 8;
+constexpr uint32_t kColSc = 0, kColO = 128, kColU = 256, kColK = 384;
+constexpr unsigned long long kStageTimeoutNs = 2000000000ull;
+constexpr size_t kSmemLimit = 232448;
+
+struct TcMaps {
+  CUtensorMap m[3][3];  // per form: A, B, C
+};
+
+// Shared memory after the ring and the S operand.
+struct TcTail {
+  float2 lg[kC];  // gate sums in units of log 2, as a float and its remainder
+  float col[kC];
+  // per value column, the chunk's first token that is not finite: chunk number
+  // + 1 in the high bits, and below them its rank from the far end, so that
+  // a maximum finds it and nothing has to be cleared
+  uint32_t bad[2][kC];
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready, u_full, s_ready, o_full, o_free, drain;
+  float2 end;  // the chunk's whole gate sum
+  float total;
+  int bad_chunk[2];  // chunk number + 1 when bad[] holds something
+  int abort;
+  uint32_t tmem;
+};
+
+struct TcGeom {
+  int slot_bytes, slots, s_bytes;  // bytes of a ring slot and of one term of S
+};
+
+__host__ __device__ inline TcGeom tc_geom(int da, int dc) {
+  TcGeom g;
+  g.slot_bytes = (da > 64 || dc > 64) ? 32768 : 16384;
+  g.s_bytes = (da > 64 ? 128 : 64) * 128 * (dc > 64 ? 2 : 1);
+  g.slots = static_cast<int>((kSmemLimit - sizeof(TcTail) - 2 * g.s_bytes) / g.slot_bytes);
+  if (g.slots > kMaxSlots) g.slots = kMaxSlots;
+  return g;
+}
+
+// ---- instructions ----------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+#define TC_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define TC_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+
+// 32 columns of the warp's 32 lanes; volatile, and the wait follows before use.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : TC_R8(r, 0), TC_R8(r, 8), TC_R8(r, 16), TC_R8(r, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      TC_I8(r, 0), TC_I8(r, 8), TC_I8(r, 16), TC_I8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      TC_I8(r, 0), TC_I8(r, 8)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two floats to packed bfloat16 (a low, b high)
+__device__ __forceinline__ uint32_t bf2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// Shared-memory operand descriptors, 128-byte swizzle.  Along the unit-stride
+// side a row is 64 elements; `lbo` is the distance of the next 64 (used when
+// that side is not the products' inner one), rows of 8 are 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// float32 accumulators, bfloat16 operands, M = 128; b_mn: B's unit stride is
+// along N.
+__device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ bool not_finite2(uint32_t x) {
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
+// Token of a bad[] entry if it is chunk `it`'s, else -1.
+__device__ __forceinline__ int first_bad(uint32_t key, uint32_t it, bool rev) {
+  if (key >> 8 != it + 1) return -1;
+  const int rank = static_cast<int>(key & 255u);
+  return rev ? rank : kC - 1 - rank;
+}
+
+struct Ctl {
+  TcTail* t;
+  uint32_t* err;
+  // All lanes of a role wait; false once the CTA gives up.
+  __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) const {
+    if (bar_try(b, parity)) return true;
+    const unsigned long long start = now_ns();
+    volatile int* ab = &t->abort;
+    while (true) {
+      for (int i = 0; i < 16; ++i)
+        if (bar_try(b, parity)) return true;
+      if (*ab) return false;
+      if (now_ns() - start > kStageTimeoutNs) {
+        *ab = 1;
+        report(ASCAN_DEV_ERR_STAGE, (static_cast<unsigned long long>(blockIdx.x) << 32) | threadIdx.x, err);
+        return false;
+      }
+    }
+  }
+  __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) const {
+    return __all_sync(kFull, wait(b, parity));
+  }
+};
+
+// The CTA's chunks in scan order.
+struct Walk {
+  const Problem& p;
+  bool rev, state_only;
+  int j;
+  long long t0, t1, n0, n1, m;      // segment, its sequences, sequences done
+  long long n, ps, pe, s0;          // sequence, piece, chunk start
+  int chunks, cc, len;              // of the piece; chunk; its tokens
+  bool from_start, to_end;
+
+  __device__ __forceinline__ Walk(const Problem& p_, bool rev_, bool so)
+      : p(p_), rev(rev_), state_only(so), j(blockIdx.x), m(0), chunks(0), cc(-1) {
+    t0 = static_cast<long long>(j) * p.seg;
+    t1 = min(t0 + p.seg, p.BL);
+    n0 = first_beyond(p, t0);
+    n1 = first_from(p, t1);
+  }
+  __device__ __forceinline__ bool next() {
+    if (++cc >= chunks) {
+      cc = 0;
+      while (true) {
+        if (m >= n1 - n0) return false;
+        n = rev ? n1 - 1 - m : n0 + m;
+        ++m;
+        const long long b0 = cu_at(p, n), b1 = cu_at(p, n + 1);
+        ps = max(b0, t0);
+        pe = min(b1, t1);
+        if (pe <= ps) continue;
+        from_start = rev ? pe == b1 : ps == b0;
+        to_end = rev ? ps == b0 : pe == b1;
+        if (state_only && to_end) continue;
+        break;
+      }
+      chunks = static_cast<int>((pe - ps + kC - 1) / kC);
+    }
+    s0 = ps + static_cast<long long>(rev ? chunks - 1 - cc : cc) * kC;
+    len = static_cast<int>(min(static_cast<long long>(kC), pe - s0));
+    return true;
+  }
+  __device__ __forceinline__ bool last() const { return cc == chunks - 1; }
+};
+
+// 32 floats of a state row to global memory, columns d0.. of dc.
+__device__ __forceinline__ void put_state(float* to, long long sj, int d0, int dc, const float* v) {
+  if (sj == 1 && d0 + 32 <= dc) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4*>(to + d0 + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q)
+      if (d0 + q < dc) to[(d0 + q) * sj] = v[q];
+  }
+}
+
+__device__ __forceinline__ void get_state(const float* from, long long sj, int d0, int dc, float* v) {
+  if (sj == 1 && d0 + 32 <= dc) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 x = *reinterpret_cast<const float4*>(from + d0 + 4 * q);
+      v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = d0 + q < dc ? from[(d0 + q) * sj] : 0.f;
+  }
+}
+
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tc_kernel(const __grid_constant__ Launch L, const __grid_constant__ TcMaps maps, const bool state_only) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const Problem& p = L.p;
+  const Form& f = L.f[blockIdx.z];
+  const CUtensorMap* map = maps.m[blockIdx.z];
+  const int da = f.da, dc = f.dc, h = blockIdx.y;
+  const bool rev = f.rev != 0, two = f.exact != 0;
+  const TcGeom geo = tc_geom(da, dc);
+  unsigned char* s_op = smem + geo.slots * geo.slot_bytes;
+  TcTail& t = *reinterpret_cast<TcTail*>(s_op + 2 * geo.s_bytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Ctl ctl{&t, p.err};
+
+  if (smem_u32(smem) & 1023u) {  // the swizzled layouts need it
+    if (tid == 0) report(ASCAN_DEV_ERR_STAGE, 0xffffffffull, p.err);
+    return;
+  }
+  if (!state_only) fill_outside<__nv_bfloat16>(p, f);
+  if (tid == 0) {
+    for (int i = 0; i < kMaxSlots; ++i) bar_init(&t.full[i], 1), bar_init(&t.empty[i], 1);
+    bar_init(&t.tab_full, 1);
+    bar_init(&t.tab_empty, state_only ? 8 : 12);
+    bar_init(&t.sc_full, 1);
+    bar_init(&t.in_full, 1);
+    bar_init(&t.p_ready, 4);
+    bar_init(&t.kt_ready, 4);
+    bar_init(&t.u_full, 1);
+    bar_init(&t.s_ready, 4);
+    bar_init(&t.o_full, 1);
+    bar_init(&t.o_free, 4);
+    bar_init(&t.drain, 1);
+    t.abort = 0;
+    t.bad_chunk[0] = t.bad_chunk[1] = 0;
+    static_assert(sizeof(TcTail) <= 3072, "the ring of 128-wide tiles leaves no more");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
+  }
+  for (int i = tid; i < 2 * kC; i += kTcThreads) t.bad[i / kC][i % kC] = 0;
+  if (warp == 13) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&t.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  const uint32_t tm = t.tmem;
+  const int nb = (dc + 31) / 32;          // 32-column blocks of the values
+  const int blocks_a = da > 64 ? 2 : 1, blocks_c = dc > 64 ? 2 : 1;
+  const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's quarter of tensor memory
+  Walk w(p, rev, state_only);
+
+  if (warp < 4) {
+    // ---- row warps ----
+    const int row = warp * 32 + lane;
+    for (uint32_t it = 0; !state_only && w.next(); ++it) {
+      const uint32_t ph = it & 1;
+      if (!ctl.warp_wait(&t.tab_full, ph)) break;
+      const float2 lt = t.lg[row];
+      const float rf = (rev ? ex2((t.end.x - lt.x) + (t.end.y - lt.y)) : ex2(lt.x)) * f.sr;
+      if (!ctl.warp_wait(&t.sc_full, ph)) break;
+      fence_after();
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t hi[16], lo[16];
+        const bool some = (rev ? b >= warp : b <= warp) && 32 * b < w.len;
+        if (some) {
+          uint32_t s[32];
+          tmem_ld32(tm + lanes + kColSc + 32 * b, s);
+          wait_ld();
+          const bool edge = b == warp || 32 * b + 32 > w.len;
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float4 l2 = *reinterpret_cast<const float4*>(&t.lg[32 * b + c]);
+            float x0 = (lt.x - l2.x) + (lt.y - l2.y), x1 = (lt.x - l2.z) + (lt.y - l2.w);
+            if (rev) x0 = -x0, x1 = -x1;
+            float p0 = __uint_as_float(s[c]) * f.sp * ex2(x0), p1 = __uint_as_float(s[c + 1]) * f.sp * ex2(x1);
+            if (edge) {
+              const int c0 = 32 * b + c;
+              p0 = (rev ? c0 >= row : c0 <= row) && c0 < w.len ? p0 : 0.f;
+              p1 = (rev ? c0 + 1 >= row : c0 + 1 <= row) && c0 + 1 < w.len ? p1 : 0.f;
+            }
+            hi[c / 2] = bf2(p0, p1);
+            if (two) lo[c / 2] = bf2(p0 - lo_f(hi[c / 2]), p1 - hi_f(hi[c / 2]));
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) hi[c] = lo[c] = 0u;
+        }
+        tmem_st16(tm + lanes + kColSc + 32 * b, hi);
+        if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, lo);
+      }
+      if (!ctl.warp_wait(&t.in_full, ph)) break;
+      fence_after();
+      for (int b = 0; b < nb; ++b) {
+        uint32_t v[32];
+        tmem_ld32(tm + lanes + kColO + 32 * b, v);
+        wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * rf);
+        tmem_st32(tm + lanes + kColO + 32 * b, v);
+      }
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.p_ready), bar_arrive(&t.tab_empty);
+
+      if (!ctl.warp_wait(&t.o_full, ph)) break;
+      fence_after();
+      const long long tok = w.s0 + row;
+      const bool on = row < w.len;
+      const bool bad = t.bad_chunk[ph] == static_cast<int>(it) + 1;
+      const __nv_bfloat16* drow =
+          f.rowdot ? static_cast<const __nv_bfloat16*>(f.dot.p) + tok * f.dot.st + (h / f.dot.share) * f.dot.sh : nullptr;
+      float dot = 0.f;
+      for (int b = 0; b < nb; ++b) {
+        uint32_t v[32];
+        tmem_ld32(tm + lanes + kColO + 32 * b, v);
+        wait_ld();
+        if (bad) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int first = first_bad(t.bad[ph][32 * b + c], it, rev);
+            if (first >= 0 && (rev ? row <= first : row >= first)) v[c] = 0x7fffffffu;
+          }
+        }
+        if (on) {
+          const long long at = (tok * p.H + h) * dc + 32 * b;
+          if (f.out_f32) {
+            float* o = static_cast<float*>(f.out) + at;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              if (32 * b + c < dc) *reinterpret_cast<uint4*>(o + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+          } else {
+            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(f.out) + at;
+#pragma unroll
+            for (int c = 0; c < 32; c += 8)
+              if (32 * b + c < dc)
+                *reinterpret_cast<uint4*>(o + c) =
+                    make_uint4(bf2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])),
+                               bf2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])),
+                               bf2(__uint_as_float(v[c + 4]), __uint_as_float(v[c + 5])),
+                               bf2(__uint_as_float(v[c + 6]), __uint_as_float(v[c + 7])));
+          }
+          if (drow) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 8)
+              if (32 * b + c < dc) {
+                const uint4 x = __ldg(reinterpret_cast<const uint4*>(drow + 32 * b + c));
+                const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  dot = fmaf(__uint_as_float(v[c + 2 * q]), lo_f(e[q]), dot);
+                  dot = fmaf(__uint_as_float(v[c + 2 * q + 1]), hi_f(e[q]), dot);
+                }
+              }
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.o_free);
+      if (on && drow) f.rowdot[h * p.BL + tok] = dot;
+    }
+  } else if (warp < 8) {
+    // ---- state warps ----
+    const int i = tid - 128;
+    const int rows = (da + 15) / 16 * 16;  // the product with S runs over whole sixteens
+    const bool work = (warp - 4) * 32 < rows;
+    const long long mat = static_cast<long long>(da) * dc;
+    float decay = 1.f;
+    for (uint32_t it = 0; w.next(); ++it) {
+      const uint32_t ph = it & 1;
+      const bool first = w.cc == 0;
+      if (first) decay = 1.f;
+      const float* from = nullptr;
+      long long sj = 1;
+      if (first && !(state_only && !w.from_start)) {
+        if (w.from_start) {
+          if (f.init) from = f.init + (w.n * p.H + h) * mat + i * f.si, sj = f.sj;
+        } else {
+          from = f.carry + (static_cast<long long>(rev ? w.j + 1 : w.j - 1) * p.H + h) * mat + static_cast<long long>(i) * dc;
+        }
+      }
+      if (!ctl.warp_wait(&t.tab_full, ph)) break;
+      const float total = t.total;
+      decay *= total;
+      if (it > 0) {  // the update before this chunk; it also follows the last use of S
+        if (!ctl.warp_wait(&t.u_full, ph ^ 1)) break;
+        fence_after();
+      }
+      const bool bad = !first && t.bad_chunk[ph ^ 1] == static_cast<int>(it);
+      const long long edge = rev ? w.s0 + w.len : w.s0;
+      const bool snap = f.snap && !state_only && edge > w.ps && edge < w.pe && (edge - w.ps) % kRestart == 0;
+      float* snap_to = snap ? f.snap + (snap_slot(edge) * p.H + h) * mat + static_cast<long long>(i) * dc : nullptr;
+      if (work) {
+        for (int b = 0; b < nb; ++b) {
+          float v[32];
+          if (first) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = 0.f;
+            if (from && i < da) get_state(from, sj, 32 * b, dc, v);
+          } else {
+            tmem_ld32(tm + lanes + kColU + 32 * b, reinterpret_cast<uint32_t*>(v));
+            wait_ld();
+            if (bad) {
+#pragma unroll
+              for (int q = 0; q < 32; ++q)
+                if (first_bad(t.bad[ph ^ 1][32 * b + q], it - 1, rev) >= 0) v[q] = __uint_as_float(0x7fffffffu);
+            }
+          }
+          if (snap && i < da) put_state(snap_to, 1, 32 * b, dc, v);
+          if (!state_only && i < rows) {
+            // S: row i of 64 columns is 128 bytes; four 16-byte pieces per 32 columns
+            unsigned char* base = s_op + (b >> 1) * (geo.s_bytes / blocks_c) + i * 128;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = v[8 * q + 2 * e], y = v[8 * q + 2 * e + 1];
+                hi[e] = bf2(x, y);
+                lo[e] = bf2(x - lo_f(hi[e]), y - hi_f(hi[e]));
+              }
+              const int at = (((b & 1) * 4 + q) ^ (i & 7)) * 16;
+              *reinterpret_cast<uint4*>(base + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              if (two) *reinterpret_cast<uint4*>(base + geo.s_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 32; ++q) v[q] *= total;
+          tmem_st32(tm + lanes + kColU + 32 * b, reinterpret_cast<const uint32_t*>(v));
+        }
+        wait_st();
+      }
+      fence_async();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.s_ready), bar_arrive(&t.tab_empty);
+      if (w.last() && (state_only || (w.to_end && f.fin))) {
+        if (!ctl.warp_wait(&t.u_full, ph)) break;
+        fence_after();
+        const bool hurt = t.bad_chunk[ph] == static_cast<int>(it) + 1;
+        float* to = state_only ? f.carry + (static_cast<long long>(w.j) * p.H + h) * mat + static_cast<long long>(i) * dc
+                               : f.fin + (w.n * p.H + h) * mat + i * f.si;
+        if (work)
+          for (int b = 0; b < nb; ++b) {
+            float v[32];
+            tmem_ld32(tm + lanes + kColU + 32 * b, reinterpret_cast<uint32_t*>(v));
+            wait_ld();
+            if (hurt) {
+#pragma unroll
+              for (int q = 0; q < 32; ++q)
+                if (first_bad(t.bad[ph][32 * b + q], it, rev) >= 0) v[q] = __uint_as_float(0x7fffffffu);
+            }
+            if (i < da) put_state(to, state_only ? 1 : f.sj, 32 * b, dc, v);
+          }
+        // a piece that holds the sequence's start takes nothing from before
+        if (state_only && i == 0) f.dec[w.j * p.H + h] = w.from_start ? -1.f : decay;
+      }
+    }
+  } else if (warp < 12) {
+    // ---- column warps ----
+    const int i = tid - 256;
+    const bool work = i < blocks_a * 64;
+    const int chunk16 = (i & 63) >> 3;
+    int off[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) off[e] = (i >> 6) * 16384 + e * 128 + ((chunk16 ^ e) << 4) + (i & 7) * 2;
+    const int per = state_only ? 2 : 3;
+    int slot = 0, round = 0;  // of the next tile
+    for (uint32_t it = 0; w.next(); ++it) {
+      const uint32_t ph = it & 1;
+      const unsigned char* bt = smem + slot * geo.slot_bytes;
+      uint64_t* bfull = &t.full[slot];
+      const uint32_t bph = round & 1;
+      for (int k = 1; k < per; ++k)
+        if (++slot == geo.slots) slot = 0, ++round;
+      unsigned char* ct = smem + slot * geo.slot_bytes;
+      uint64_t* cfull = &t.full[slot];
+      const uint32_t cph = round & 1;
+      if (++slot == geo.slots) slot = 0, ++round;
+
+      // The previous update is done: its operand may be overwritten, and the
+      // row and state warps have read what bad[ph] held two chunks ago.
+      if (it > 0) {
+        if (!ctl.warp_wait(&t.u_full, ph ^ 1)) break;
+        fence_after();
+      }
+      if (!ctl.warp_wait(cfull, cph)) break;
+      {  // one token row of C per thread
+        bool bad = false;
+        const bool live = i < w.len;
+        for (int b = 0; b < blocks_c; ++b)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uint4* at = reinterpret_cast<uint4*>(ct + b * 16384 + i * 128 + ((q ^ (i & 7)) << 4));
+            if (live) {
+              const uint4 x = *at;
+              bad |= not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w);
+            } else {
+              *at = make_uint4(0, 0, 0, 0);  // another sequence's token, or past the end
+            }
+          }
+        if (bad) {  // note and clear
+          for (int d = 0; d < blocks_c * 64; ++d) {
+            uint16_t* at = reinterpret_cast<uint16_t*>(ct + (d >> 6) * 16384 + i * 128 + ((((d & 63) >> 3) ^ (i & 7)) << 4) + (d & 7) * 2);
+            if ((*at & 0x7f80u) == 0x7f80u) {
+              *at = 0;
+              atomicMax(&t.bad[ph][d], ((it + 1) << 8) | static_cast<uint32_t>(rev ? i : kC - 1 - i));
+            }
+          }
+          t.bad_chunk[ph] = static_cast<int>(it) + 1;
+        }
+      }
+      fence_async();
+      if (!ctl.warp_wait(&t.tab_full, ph)) break;
+      if (!ctl.warp_wait(bfull, bph)) break;
+      if (work) {
+#pragma unroll
+        for (int s0 = 0; s0 < kC; s0 += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int g = 0; g < 32; g += 8) {
+            const unsigned char* src = bt + (s0 + g) * 128;
+            float x[8];
+            const float4 c0 = *reinterpret_cast<const float4*>(&t.col[s0 + g]);
+            const float4 c1 = *reinterpret_cast<const float4*>(&t.col[s0 + g + 4]);
+            const float cf[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t raw = *reinterpret_cast<const uint16_t*>(src + off[e]);
+              x[e] = s0 + g + e < w.len ? __uint_as_float(raw << 16) * cf[e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t v = bf2(x[2 * e], x[2 * e + 1]);
+              hi[g / 2 + e] = v;
+              lo[g / 2 + e] = bf2(x[2 * e] - lo_f(v), x[2 * e + 1] - hi_f(v));
+            }
+          }
+          tmem_st16(tm + lanes + kColK + s0 / 2, hi);
+          tmem_st16(tm + lanes + kColK + 64 + s0 / 2, lo);
+        }
+        wait_st();
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.kt_ready), bar_arrive(&t.tab_empty);
+    }
+  } else if (warp == 12) {
+    // ---- loads ----
+    if (lane == 0) {
+      uint32_t tile = 0;
+      bool ok = true;
+      auto load = [&](int which, int blocks, const Rows& r) {
+        const int slot = tile % geo.slots;
+        if (tile >= static_cast<uint32_t>(geo.slots) && !ctl.wait(&t.empty[slot], (tile / geo.slots - 1) & 1)) return false;
+        bar_expect(&t.full[slot], blocks * 16384);
+        for (int b = 0; b < blocks; ++b)
+          asm volatile(
+              "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+                  "r"(smem_u32(smem + slot * geo.slot_bytes + b * 16384)),
+              "l"(&map[which]), "r"(b * 64), "r"(h / r.share), "r"(static_cast<int>(w.s0)), "r"(smem_u32(&t.full[slot]))
+              : "memory");
+        ++tile;
+        return true;
+      };
+      while (ok && w.next()) {
+        ok = load(1, blocks_a, f.b);
+        if (ok && !state_only) ok = load(0, blocks_a, f.a);
+        if (ok) ok = load(2, blocks_c, f.c);
+      }
+      // a load in flight must land before the CTA leaves (only after a give-up)
+      const uint32_t from = tile > static_cast<uint32_t>(geo.slots) ? tile - geo.slots : 0;
+      for (uint32_t k = from; k < tile; ++k) {
+        const unsigned long long start = now_ns();
+        while (!bar_try(&t.full[k % geo.slots], (k / geo.slots) & 1) && now_ns() - start < kStageTimeoutNs) {
+        }
+      }
+    }
+  } else if (warp == 13) {
+    // ---- products ----
+    if (lane == 0) {
+      const uint32_t id_sc = idesc(kC, false), id_v = idesc((dc + 15) / 16 * 16, true);
+      const int ka = (da + 15) / 16;
+      const uint32_t lbo_s = geo.s_bytes / blocks_c;
+      int slot = 0, round = 0;
+      auto take = [&](uint64_t** full, uint64_t** empty, uint32_t* ph) {
+        const uint32_t a = smem_u32(smem + slot * geo.slot_bytes);
+        *full = &t.full[slot];
+        *empty = &t.empty[slot];
+        *ph = round & 1;
+        if (++slot == geo.slots) slot = 0, ++round;
+        return a;
+      };
+      for (uint32_t it = 0; w.next(); ++it) {
+        const uint32_t ph = it & 1;
+        uint64_t *fb, *eb, *fa = nullptr, *ea = nullptr, *fc, *ec;
+        uint32_t pb, pa = 0, pc, aa = 0;
+        const uint32_t ab = take(&fb, &eb, &pb);
+        if (!state_only) aa = take(&fa, &ea, &pa);
+        const uint32_t ac = take(&fc, &ec, &pc);
+        if (!ctl.wait(fb, pb)) break;
+        if (!state_only) {
+          if (!ctl.wait(fa, pa)) break;
+          // the scores go where the previous chunk's P lies until its product is done
+          if (it > 0 && !ctl.wait(&t.o_full, ph ^ 1)) break;
+          fence_after();
+          for (int k = 0; k < ka; ++k) {
+            const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
+            mma_smem(tm + kColSc, desc(aa + o, 16), desc(ab + o, 16), id_sc, k > 0);
+          }
+          commit(&t.sc_full);
+          if (!ctl.wait(&t.s_ready, ph)) break;
+          if (it > 0 && !ctl.wait(&t.o_free, ph ^ 1)) break;
+          fence_after();
+          for (int term = 0; term < (two ? 2 : 1); ++term)
+            for (int k = 0; k < ka; ++k)
+              mma_smem(tm + kColO, desc(aa + (k >> 2) * 16384 + (k & 3) * 32, 16),
+                       desc(smem_u32(s_op) + term * geo.s_bytes + k * 2048, lbo_s), id_v, term + k > 0);
+          commit(&t.in_full);
+          commit(ea);
+        } else if (!ctl.wait(&t.s_ready, ph)) {
+          break;
+        }
+        if (!ctl.wait(&t.kt_ready, ph)) break;
+        if (!ctl.wait(fc, pc)) break;
+        fence_after();
+        for (int term = 0; term < 2; ++term)
+          for (int k = 0; k < kC / 16; ++k)
+            mma_tmem(tm + kColU, tm + kColK + term * 64 + k * 8, desc(ac + k * 2048, 16384), id_v, true);
+        commit(&t.u_full);
+        commit(eb);
+        if (!state_only) {
+          if (!ctl.wait(&t.p_ready, ph)) break;
+          fence_after();
+          for (int term = 0; term < (two ? 2 : 1); ++term)
+            for (int k = 0; k < kC / 16; ++k)
+              mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, desc(ac + k * 2048, 16384), id_v, true);
+          commit(&t.o_full);
+        }
+        commit(ec);
+      }
+      commit(&t.drain);  // nothing of this CTA's is in flight after it
+      const unsigned long long start = now_ns();
+      while (!bar_try(&t.drain, 0) && now_ns() - start < kStageTimeoutNs) {
+      }
+    }
+  } else {
+    // ---- gates: four tokens a lane ----
+    for (uint32_t it = 0; w.next(); ++it) {
+      double g[4], sum = 0.0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int s = lane * 4 + q;
+        sum += s < w.len ? static_cast<double>(load_gate(p, w.s0 + s, h)) : 0.0;
+        g[q] = sum;
+      }
+      double inc = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const double u = __shfl_up_sync(kFull, inc, o);
+        if (lane >= o) inc += u;
+      }
+      const double end = __shfl_sync(kFull, inc, 31);
+      float2 lg[4];
+      float col[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const double x = (inc - sum + g[q]) * 1.4426950408889634, y = end * 1.4426950408889634;
+        lg[q].x = static_cast<float>(x);
+        lg[q].y = static_cast<float>(x - static_cast<double>(lg[q].x));
+        const float head = exp2f(static_cast<float>(x)), tail = exp2f(static_cast<float>(y - x));
+        col[q] = (rev ? head : tail) * f.sc;
+      }
+      if (it > 0 && !ctl.warp_wait(&t.tab_empty, (it & 1) ^ 1)) break;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t.lg[lane * 4 + q] = lg[q];
+      *reinterpret_cast<float4*>(&t.col[lane * 4]) = make_float4(col[0], col[1], col[2], col[3]);
+      if (lane == 31) {
+        t.total = exp2f(lg[3].x);
+        t.end = lg[3];
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.tab_full);
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
+  }
+}
+
+static bool map_rows(CUtensorMap* m, const Rows& r, int dim, long long BL, int H) {
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const int heads = H / r.share;
+  const long long sh = heads > 1 ? r.sh : (dim + 7) / 8 * 8;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(BL)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(r.st) * 2};
+  const cuuint32_t box[3] = {64, 1, kC}, one[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(r.p), dims, strides, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// bfloat16 rows that a tensor map can describe: 16-byte bases and strides,
+// head sizes in whole 16-byte pieces, heads that do not overlap.
+static bool rows_usable(const Rows& r, int dim, int H) {
+  if (!r.p) return true;
+  if ((reinterpret_cast<uintptr_t>(r.p) & 15u) || dim % 8 || r.st % 8 || r.st < dim || r.st >= (1ll << 38)) return false;
+  return H / r.share == 1 || (r.sh % 8 == 0 && r.sh >= dim && r.sh < (1ll << 38));
+}
+
+bool tc_usable(const Launch& l, int roles, int dtype) {
+  if (dtype != ASCAN_BF16 || l.p.BL > 0x7fffff00ll) return false;
+  for (int r = 0; r < roles; ++r) {
+    const Form& f = l.f[r];
+    if (!rows_usable(f.a, f.da, l.p.H) || !rows_usable(f.b, f.da, l.p.H) || !rows_usable(f.c, f.dc, l.p.H) ||
+        !rows_usable(f.dot, f.dc, l.p.H) || (reinterpret_cast<uintptr_t>(f.out) & 15u) ||
+        (reinterpret_cast<uintptr_t>(f.init) & 15u) || (reinterpret_cast<uintptr_t>(f.fin) & 15u))
+      return false;
+  }
+  return encode_fn() != nullptr;
+}
+
+int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
+  TcMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  size_t smem = 0;
+  for (int r = 0; r < roles; ++r) {
+    const Form& f = l.f[r];
+    if (!map_rows(&maps.m[r][0], f.a, f.da, l.p.BL, l.p.H) || !map_rows(&maps.m[r][1], f.b, f.da, l.p.BL, l.p.H) ||
+        !map_rows(&maps.m[r][2], f.c, f.dc, l.p.BL, l.p.H))
+      return ASCAN_EINVAL;
+    const TcGeom g = tc_geom(f.da, f.dc);
+    const size_t need = static_cast<size_t>(g.slots) * g.slot_bytes + 2 * g.s_bytes + sizeof(TcTail);
+    if (need > smem) smem = need;
+  }
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaFuncSetAttribute(tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
+  });
+  tc_kernel<<<dim3(l.p.J, l.p.H, roles), kTcThreads, smem, s>>>(l, maps, state_only);
+  return launch_status();
+}
+
+}  // namespace mscan
+
+ASCAN_UNIT_ERROR_ACCESSORS(mscan_tc)
+
+}  // namespace ascan

@@ -65,6 +65,7 @@ enum ascan_status {
 #define ASCAN_DEV_ERR_LOOKBACK 0x4u     /* a tile predecessor never published (bounded wait expired) */
 #define ASCAN_DEV_ERR_EXCHANGE 0x8u     /* a peer rank's record or release never came (bounded wait expired) */
 #define ASCAN_DEV_ERR_INDEX 0x10u       /* a state slot or a position lies outside its table */
+#define ASCAN_DEV_ERR_STAGE 0x20u       /* a stage of the matrix scan did not finish (bounded wait expired) */
 
 /* Library identification. */
 ASCAN_API int ascan_abi_version(void);
