@@ -56,7 +56,9 @@ struct TcMaps {
 
 // Shared memory after the ring and the S operand.
 struct TcTail {
-  float2 lg[kC];  // gate sums in units of log 2, as a float and its remainder
+  // Negated gate sums (of the mask's direction) in units of log 2, two tokens
+  // an entry: floats of both, then what the floats leave over
+  float4 lg[kC / 2];
   float col[kC];
   // per value column, the chunk's first token that is not finite: chunk number
   // + 1 in the high bits, and below them its rank from the far end, so that
@@ -64,7 +66,7 @@ struct TcTail {
   uint32_t bad[2][kC];
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready, u_full, s_ready, o_full, o_free, drain;
-  float2 end;  // the chunk's whole gate sum
+  float2 end;  // the chunk's whole gate sum, same form
   float total;
   int bad_chunk[2];  // chunk number + 1 when bad[] holds something
   int abort;
@@ -164,6 +166,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
       : "memory");
 }
 
+// 16 lanes by 16 columns; a pair of registers holds 4 columns: lane l of the
+// warp has column l % 4 of row l / 4, then of row l / 4 + 8.
+__device__ __forceinline__ void tmem_st16x128(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), TC_I8(r, 0)
+               : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -175,8 +184,42 @@ __device__ __forceinline__ uint32_t bf2(float a, float b) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
+// Two floats in one register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 __device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// The pair as packed bfloat16, and what that leaves over as another.
+__device__ __forceinline__ uint32_t round2(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  return bf2(a, b);
+}
+__device__ __forceinline__ uint32_t rest2(uint64_t x, uint32_t hi) {
+  return round2(fma2(pair(lo_f(hi), hi_f(hi)), pair(-1.f, -1.f), x));
+}
 
 // Shared-memory operand descriptors, 128-byte swizzle.  Along the unit-stride
 // side a row is 64 elements; `lbo` is the distance of the next 64 (used when
@@ -190,10 +233,6 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
 __device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
-}
-
-__device__ __forceinline__ bool not_finite2(uint32_t x) {
-  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
 }
 
 // Token of a bad[] entry if it is chunk `it`'s, else -1.
@@ -350,51 +389,73 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp < 4) {
     // ---- row warps ----
     const int row = warp * 32 + lane;
+    const uint64_t sp2 = pair(f.sp, f.sp);
     for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
-      const float2 lt = t.lg[row];
-      const float rf = (rev ? ex2((t.end.x - lt.x) + (t.end.y - lt.y)) : ex2(lt.x)) * f.sr;
+      const float4 l4 = t.lg[row >> 1];
+      const float lx = (row & 1) ? -l4.y : -l4.x, ly = (row & 1) ? -l4.w : -l4.z;
+      const uint64_t lx2 = pair(lx, lx), ly2 = pair(ly, ly);
+      // backwards lx is minus the sum to the row
+      const float rf = (rev ? ex2((t.end.x + lx) + (t.end.y + ly)) : ex2(lx)) * f.sr;
       if (!ctl.warp_wait(&t.sc_full, ph)) break;
       fence_after();
-#pragma unroll
+#pragma unroll 1
       for (int b = 0; b < 4; ++b) {
+        const uint32_t col = tm + lanes + kColSc + 32 * b;
         uint32_t hi[16], lo[16];
         const bool some = (rev ? b >= warp : b <= warp) && 32 * b < w.len;
         if (some) {
           uint32_t s[32];
-          tmem_ld32(tm + lanes + kColSc + 32 * b, s);
+          tmem_ld32(col, s);
           wait_ld();
-          const bool edge = b == warp || 32 * b + 32 > w.len;
+          uint64_t pv[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float4 l2 = *reinterpret_cast<const float4*>(&t.lg[32 * b + c]);
-            float x0 = (lt.x - l2.x) + (lt.y - l2.y), x1 = (lt.x - l2.z) + (lt.y - l2.w);
-            if (rev) x0 = -x0, x1 = -x1;
-            float p0 = __uint_as_float(s[c]) * f.sp * ex2(x0), p1 = __uint_as_float(s[c + 1]) * f.sp * ex2(x1);
-            if (edge) {
-              const int c0 = 32 * b + c;
+          for (int c = 0; c < 16; ++c) {
+            const float4 m = t.lg[16 * b + c];
+            const uint64_t x = add2(add2(lx2, pair(m.x, m.y)), add2(ly2, pair(m.z, m.w)));
+            float x0, x1;
+            unpair(x, x0, x1);
+            pv[c] = mul2(mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sp2), pair(ex2(x0), ex2(x1)));
+          }
+          if (b == warp || 32 * b + 32 > w.len) {  // the mask's edge: select, not multiply
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const int c0 = 32 * b + 2 * c;
+              float p0, p1;
+              unpair(pv[c], p0, p1);
               p0 = (rev ? c0 >= row : c0 <= row) && c0 < w.len ? p0 : 0.f;
               p1 = (rev ? c0 + 1 >= row : c0 + 1 <= row) && c0 + 1 < w.len ? p1 : 0.f;
+              pv[c] = pair(p0, p1);
             }
-            hi[c / 2] = bf2(p0, p1);
-            if (two) lo[c / 2] = bf2(p0 - lo_f(hi[c / 2]), p1 - hi_f(hi[c / 2]));
+          }
+#pragma unroll
+          for (int c = 0; c < 16; ++c) hi[c] = round2(pv[c]);
+          if (two) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) lo[c] = rest2(pv[c], hi[c]);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < 16; ++c) hi[c] = lo[c] = 0u;
         }
-        tmem_st16(tm + lanes + kColSc + 32 * b, hi);
-        if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, lo);
+        tmem_st16(col, hi);
+        if (two) tmem_st16(col + 16, lo);
       }
       if (!ctl.warp_wait(&t.in_full, ph)) break;
       fence_after();
+      const uint64_t rf2 = pair(rf, rf);
+#pragma unroll 1
       for (int b = 0; b < nb; ++b) {
         uint32_t v[32];
         tmem_ld32(tm + lanes + kColO + 32 * b, v);
         wait_ld();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * rf);
+        for (int c = 0; c < 32; c += 2) {
+          float x, y;
+          unpair(mul2(pair(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), rf2), x, y);
+          v[c] = __float_as_uint(x), v[c + 1] = __float_as_uint(y);
+        }
         tmem_st32(tm + lanes + kColO + 32 * b, v);
       }
       wait_st();
@@ -410,6 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const __nv_bfloat16* drow =
           f.rowdot ? static_cast<const __nv_bfloat16*>(f.dot.p) + tok * f.dot.st + (h / f.dot.share) * f.dot.sh : nullptr;
       float dot = 0.f;
+#pragma unroll 1
       for (int b = 0; b < nb; ++b) {
         uint32_t v[32];
         tmem_ld32(tm + lanes + kColO + 32 * b, v);
@@ -490,7 +552,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const long long edge = rev ? w.s0 + w.len : w.s0;
       const bool snap = f.snap && !state_only && edge > w.ps && edge < w.pe && (edge - w.ps) % kRestart == 0;
       float* snap_to = snap ? f.snap + (snap_slot(edge) * p.H + h) * mat + static_cast<long long>(i) * dc : nullptr;
+      const uint64_t total2 = pair(total, total);
       if (work) {
+#pragma unroll 1
         for (int b = 0; b < nb; ++b) {
           float v[32];
           if (first) {
@@ -515,9 +579,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               uint32_t hi[4], lo[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float x = v[8 * q + 2 * e], y = v[8 * q + 2 * e + 1];
-                hi[e] = bf2(x, y);
-                lo[e] = bf2(x - lo_f(hi[e]), y - hi_f(hi[e]));
+                const uint64_t x = pair(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
+                hi[e] = round2(x);
+                lo[e] = rest2(x, hi[e]);
               }
               const int at = (((b & 1) * 4 + q) ^ (i & 7)) * 16;
               *reinterpret_cast<uint4*>(base + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -525,7 +589,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
 #pragma unroll
-          for (int q = 0; q < 32; ++q) v[q] *= total;
+          for (int q = 0; q < 32; q += 2) unpair(mul2(pair(v[q], v[q + 1]), total2), v[q], v[q + 1]);
           tmem_st32(tm + lanes + kColU + 32 * b, reinterpret_cast<const uint32_t*>(v));
         }
         wait_st();
@@ -541,6 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float* to = state_only ? f.carry + (static_cast<long long>(w.j) * p.H + h) * mat + static_cast<long long>(i) * dc
                                : f.fin + (w.n * p.H + h) * mat + i * f.si;
         if (work)
+#pragma unroll 1
           for (int b = 0; b < nb; ++b) {
             float v[32];
             tmem_ld32(tm + lanes + kColU + 32 * b, reinterpret_cast<uint32_t*>(v));
@@ -560,10 +625,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---- column warps ----
     const int i = tid - 256;
     const bool work = i < blocks_a * 64;
-    const int chunk16 = (i & 63) >> 3;
-    int off[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) off[e] = (i >> 6) * 16384 + e * 128 + ((chunk16 ^ e) << 4) + (i & 7) * 2;
+    // The warp's 32 rows of (col.B)^T: matrix m of a load has rows 8 m.. and 8
+    // tokens; lane r of it points at token r's 16 bytes.
+    const int lead = (i >> 6) * 16384 + (lane & 7) * 128 + ((((i & 32) >> 3) + (lane >> 3) ^ (lane & 7)) << 4);
     const int per = state_only ? 2 : 3;
     int slot = 0, round = 0;  // of the next tile
     for (uint32_t it = 0; w.next(); ++it) {
@@ -586,19 +650,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (!ctl.warp_wait(cfull, cph)) break;
       {  // one token row of C per thread
-        bool bad = false;
         const bool live = i < w.len;
-        for (int b = 0; b < blocks_c; ++b)
+        const __nv_bfloat162 none = __float2bfloat162_rn(0.f);
+        __nv_bfloat162 sum = none;  // sum of 0 * x: NaN if any x is not finite
+#pragma unroll 1
+        for (int b = 0; b < blocks_c; ++b) {
+          unsigned char* at = ct + b * 16384 + i * 128;
+          if (live) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            uint4* at = reinterpret_cast<uint4*>(ct + b * 16384 + i * 128 + ((q ^ (i & 7)) << 4));
-            if (live) {
-              const uint4 x = *at;
-              bad |= not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w);
-            } else {
-              *at = make_uint4(0, 0, 0, 0);  // another sequence's token, or past the end
+            for (int q = 0; q < 8; ++q) {
+              const uint4 x = *reinterpret_cast<const uint4*>(at + ((q ^ (i & 7)) << 4));
+              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), none, sum);
+              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), none, sum);
+              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), none, sum);
+              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), none, sum);
             }
+          } else {  // another sequence's token, or past the end
+#pragma unroll
+            for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(at + ((q ^ (i & 7)) << 4)) = make_uint4(0, 0, 0, 0);
           }
+        }
+        const bool bad = !(__low2float(sum) == 0.f && __high2float(sum) == 0.f);
         if (bad) {  // note and clear
           for (int d = 0; d < blocks_c * 64; ++d) {
             uint16_t* at = reinterpret_cast<uint16_t*>(ct + (d >> 6) * 16384 + i * 128 + ((((d & 63) >> 3) ^ (i & 7)) << 4) + (d & 7) * 2);
@@ -614,30 +686,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       if (!ctl.warp_wait(bfull, bph)) break;
       if (work) {
-#pragma unroll
+        const uint32_t src = smem_u32(bt) + lead;
+        const bool tail = w.len < kC;
+#pragma unroll 1
         for (int s0 = 0; s0 < kC; s0 += 32) {
-          uint32_t hi[16], lo[16];
+          uint32_t hi[16], lo[16];  // [half of the rows][8 tokens][rows 0-7, 8-15]
 #pragma unroll
-          for (int g = 0; g < 32; g += 8) {
-            const unsigned char* src = bt + (s0 + g) * 128;
-            float x[8];
-            const float4 c0 = *reinterpret_cast<const float4*>(&t.col[s0 + g]);
-            const float4 c1 = *reinterpret_cast<const float4*>(&t.col[s0 + g + 4]);
-            const float cf[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+          for (int g = 0; g < 4; ++g) {
+            uint32_t r[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                         : "r"(src + (s0 + 8 * g) * 128)
+                         : "memory");
+            const int s = s0 + 8 * g + 2 * (lane & 3);
+            const float2 cf = *reinterpret_cast<const float2*>(&t.col[s]);
+            if (tail) {  // select, not multiply: the rows there are another sequence's
+              const uint32_t keep = (s < w.len ? 0xffffu : 0u) | (s + 1 < w.len ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t raw = *reinterpret_cast<const uint16_t*>(src + off[e]);
-              x[e] = s0 + g + e < w.len ? __uint_as_float(raw << 16) * cf[e] : 0.f;
+              for (int m = 0; m < 4; ++m) r[m] &= keep;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t v = bf2(x[2 * e], x[2 * e + 1]);
-              hi[g / 2 + e] = v;
-              lo[g / 2 + e] = bf2(x[2 * e] - lo_f(v), x[2 * e + 1] - hi_f(v));
+            for (int m = 0; m < 4; ++m) {
+              const uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), pair(cf.x, cf.y));
+              const int at = (m >> 1) * 8 + g * 2 + (m & 1);
+              hi[at] = round2(x);
+              lo[at] = rest2(x, hi[at]);
             }
           }
-          tmem_st16(tm + lanes + kColK + s0 / 2, hi);
-          tmem_st16(tm + lanes + kColK + 64 + s0 / 2, lo);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t to = tm + lanes + (static_cast<uint32_t>(m) << 20) + kColK + s0 / 2;
+            tmem_st16x128(to, hi + 8 * m);
+            tmem_st16x128(to + 64, lo + 8 * m);
+          }
         }
         wait_st();
       }
@@ -761,23 +842,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane >= o) inc += u;
       }
       const double end = __shfl_sync(kFull, inc, 31);
-      float2 lg[4];
-      float col[4];
+      float lx[4], ly[4], col[4];
+      float2 whole;
+      const double y = end * (rev ? 1.4426950408889634 : -1.4426950408889634);
+      whole.x = static_cast<float>(y);
+      whole.y = static_cast<float>(y - static_cast<double>(whole.x));
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const double x = (inc - sum + g[q]) * 1.4426950408889634, y = end * 1.4426950408889634;
-        lg[q].x = static_cast<float>(x);
-        lg[q].y = static_cast<float>(x - static_cast<double>(lg[q].x));
-        const float head = exp2f(static_cast<float>(x)), tail = exp2f(static_cast<float>(y - x));
-        col[q] = (rev ? head : tail) * f.sc;
+        const double x = (inc - sum + g[q]) * (rev ? 1.4426950408889634 : -1.4426950408889634);
+        lx[q] = static_cast<float>(x);
+        ly[q] = static_cast<float>(x - static_cast<double>(lx[q]));
+        col[q] = ex2(rev ? lx[q] : lx[q] - whole.x + (ly[q] - whole.y)) * f.sc;
       }
       if (it > 0 && !ctl.warp_wait(&t.tab_empty, (it & 1) ^ 1)) break;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) t.lg[lane * 4 + q] = lg[q];
+      t.lg[lane * 2] = make_float4(lx[0], lx[1], ly[0], ly[1]);
+      t.lg[lane * 2 + 1] = make_float4(lx[2], lx[3], ly[2], ly[3]);
       *reinterpret_cast<float4*>(&t.col[lane * 4]) = make_float4(col[0], col[1], col[2], col[3]);
-      if (lane == 31) {
-        t.total = exp2f(lg[3].x);
-        t.end = lg[3];
+      if (lane == 0) {
+        t.total = ex2(rev ? whole.x : -whole.x);
+        t.end = whole;
       }
       __syncwarp();
       if (lane == 0) bar_arrive(&t.tab_full);
