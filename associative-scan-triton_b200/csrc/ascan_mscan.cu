@@ -238,33 +238,43 @@ __global__ void __launch_bounds__(kPlainThreads)
 
 // Chains the segments' own contributions in scan order: carry[j] becomes the
 // state that leaves segment j.  One thread per element; a segment that no
-// sequence leaves restarts the chain (its carry is never read).
+// sequence leaves restarts the chain (its carry is never read).  The decays
+// of 256 segments are looked up side by side, and four segments' elements are
+// in flight at once.
 __global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Launch L) {
   const Problem& p = L.p;
   const Form& f = L.f[blockIdx.z];
-  const int h = blockIdx.y;
+  const int h = blockIdx.y, tid = threadIdx.x;
   const long long mat = static_cast<long long>(f.da) * f.dc;
-  const long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= mat) return;
+  const long long e = static_cast<long long>(blockIdx.x) * 256 + tid;
+  __shared__ float dec[256];  // of the segment; -1: starts anew; -2: nothing crosses
   float state = 0.f;
-  bool have = false;
-  for (int m = 0; m + 1 < p.J; ++m) {
-    const int j = f.rev ? p.J - 1 - m : m;
-    const long long edge = f.rev ? j * p.seg : min((j + 1) * p.seg, p.BL);  // token after the boundary
-    const long long n = first_beyond(p, edge);
-    if (n >= p.N || cu_at(p, n) >= edge) {  // no sequence crosses
-      have = false;
-      continue;
+  const long long hop = static_cast<long long>(p.H) * mat;
+  for (int m0 = 0; m0 + 1 < p.J; m0 += 256) {
+    const int count = min(256, p.J - 1 - m0);
+    __syncthreads();
+    if (tid < count) {
+      const int j = f.rev ? p.J - 1 - (m0 + tid) : m0 + tid;
+      const long long edge = f.rev ? j * p.seg : min((j + 1) * p.seg, p.BL);  // token after the boundary
+      const long long n = first_beyond(p, edge);
+      dec[tid] = n >= p.N || cu_at(p, n) >= edge ? -2.f : f.dec[j * p.H + h];
     }
-    const float dec = f.dec[j * p.H + h];
-    float* at = f.carry + (static_cast<long long>(j) * p.H + h) * mat + e;
-    float x = *at;
-    if (dec >= 0.f && have) {
-      x = fmaf(dec, state, x);
-      *at = x;
+    __syncthreads();
+    if (e >= mat) continue;
+    const long long step = f.rev ? -hop : hop;
+    float* at = f.carry + ((f.rev ? p.J - 1 - m0 : m0) * static_cast<long long>(p.H) + h) * mat + e;
+    for (int m = 0; m < count; m += 4, at += 4 * step) {
+      float x[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = m + q < count && dec[m + q] > -2.f ? at[q * step] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (m + q >= count || dec[m + q] == -2.f) continue;
+        // an anew segment keeps its own; else what entered it has come through
+        state = dec[m + q] < 0.f ? x[q] : fmaf(dec[m + q], state, x[q]);
+        if (dec[m + q] >= 0.f) at[q * step] = state;
+      }
     }
-    state = x;
-    have = true;
   }
 }
 

@@ -51,7 +51,7 @@ constexpr unsigned long long kStageTimeoutNs = 2000000000ull;
 constexpr size_t kSmemLimit = 232448;
 
 struct TcMaps {
-  CUtensorMap m[3][3];  // per form: A, B, C
+  CUtensorMap m[3][4];  // per form: A, B, C, and the rows to take dots with
 };
 
 // Shared memory after the ring and the S operand.
@@ -65,7 +65,7 @@ struct TcTail {
   // a maximum finds it and nothing has to be cleared
   uint32_t bad[2][kC];
   uint64_t full[kMaxSlots], empty[kMaxSlots];
-  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready, u_full, s_ready, o_full, o_free, drain;
+  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready, u_full, s_ready, o_full, o_free, d_full, drain;
   float2 end;  // the chunk's whole gate sum, same form
   float total;
   int bad_chunk[2];  // chunk number + 1 when bad[] holds something
@@ -114,6 +114,13 @@ __device__ __forceinline__ unsigned long long now_ns() {
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
 }
+// 128 tokens by 64 elements of one head, from column x (a multiple of 64).
+__device__ __forceinline__ void tma_rows(uint32_t to, const CUtensorMap* m, int x, int head, int token, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
+      "l"(m), "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
@@ -157,6 +164,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
       TC_I8(r, 0), TC_I8(r, 8), TC_I8(r, 16), TC_I8(r, 24)
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : TC_R8(r, 0) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), TC_I8(r, 0)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
@@ -242,96 +256,134 @@ __device__ __forceinline__ int first_bad(uint32_t key, uint32_t it, bool rev) {
   return rev ? rank : kC - 1 - rank;
 }
 
+// The long way of a wait, out of line: three warps of different roles share a
+// scheduler's instruction cache, and what is rare must not take room in it.
+__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, TcTail* t, uint32_t* err) {
+  const unsigned long long start = now_ns();
+  volatile int* ab = &t->abort;
+  while (true) {
+    for (int i = 0; i < 16; ++i)
+      if (bar_try(b, parity)) return true;
+    if (*ab) return false;
+    if (now_ns() - start > kStageTimeoutNs) {
+      *ab = 1;
+      report(ASCAN_DEV_ERR_STAGE, (static_cast<unsigned long long>(blockIdx.x) << 32) | threadIdx.x, err);
+      return false;
+    }
+  }
+}
+
 struct Ctl {
   TcTail* t;
   uint32_t* err;
   // All lanes of a role wait; false once the CTA gives up.
   __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) const {
-    if (bar_try(b, parity)) return true;
-    const unsigned long long start = now_ns();
-    volatile int* ab = &t->abort;
-    while (true) {
-      for (int i = 0; i < 16; ++i)
-        if (bar_try(b, parity)) return true;
-      if (*ab) return false;
-      if (now_ns() - start > kStageTimeoutNs) {
-        *ab = 1;
-        report(ASCAN_DEV_ERR_STAGE, (static_cast<unsigned long long>(blockIdx.x) << 32) | threadIdx.x, err);
-        return false;
-      }
-    }
+    return bar_try(b, parity) || wait_slow(b, parity, t, err);
   }
   __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) const {
     return __all_sync(kFull, wait(b, parity));
   }
 };
 
+// The part of one sequence that lies in the CTA's segment.
+struct Piece {
+  long long n, ps, pe;
+  int m;  // how far the search came; -1: none left
+  bool from_start, to_end;
+};
+
+__device__ __noinline__ Piece next_piece(const Problem* pp, bool rev, bool state_only, int m) {
+  const Problem& p = *pp;
+  const long long t0 = static_cast<long long>(blockIdx.x) * p.seg, t1 = min(t0 + p.seg, p.BL);
+  const long long n0 = first_beyond(p, t0), n1 = first_from(p, t1);
+  Piece x;
+  while (m < n1 - n0) {
+    x.n = rev ? n1 - 1 - m : n0 + m;
+    ++m;
+    const long long b0 = cu_at(p, x.n), b1 = cu_at(p, x.n + 1);
+    x.ps = max(b0, t0);
+    x.pe = min(b1, t1);
+    x.from_start = rev ? x.pe == b1 : x.ps == b0;
+    x.to_end = rev ? x.ps == b0 : x.pe == b1;
+    x.m = m;
+    if (x.pe > x.ps && !(state_only && x.to_end)) return x;
+  }
+  x.m = -1;
+  return x;
+}
+
 // The CTA's chunks in scan order.
 struct Walk {
   const Problem& p;
-  bool rev, state_only;
-  int j;
-  long long t0, t1, n0, n1, m;      // segment, its sequences, sequences done
-  long long n, ps, pe, s0;          // sequence, piece, chunk start
-  int chunks, cc, len;              // of the piece; chunk; its tokens
-  bool from_start, to_end;
+  const bool rev, state_only;
+  Piece x;
+  long long s0;         // chunk start
+  int chunks, cc, len;  // of the piece; chunk; its tokens
 
-  __device__ __forceinline__ Walk(const Problem& p_, bool rev_, bool so)
-      : p(p_), rev(rev_), state_only(so), j(blockIdx.x), m(0), chunks(0), cc(-1) {
-    t0 = static_cast<long long>(j) * p.seg;
-    t1 = min(t0 + p.seg, p.BL);
-    n0 = first_beyond(p, t0);
-    n1 = first_from(p, t1);
+  __device__ __forceinline__ Walk(const Problem& p_, bool rev_, bool so) : p(p_), rev(rev_), state_only(so), chunks(0), cc(-1) {
+    x.m = 0;
   }
   __device__ __forceinline__ bool next() {
     if (++cc >= chunks) {
+      x = next_piece(&p, rev, state_only, x.m);
+      if (x.m < 0) return false;
       cc = 0;
-      while (true) {
-        if (m >= n1 - n0) return false;
-        n = rev ? n1 - 1 - m : n0 + m;
-        ++m;
-        const long long b0 = cu_at(p, n), b1 = cu_at(p, n + 1);
-        ps = max(b0, t0);
-        pe = min(b1, t1);
-        if (pe <= ps) continue;
-        from_start = rev ? pe == b1 : ps == b0;
-        to_end = rev ? ps == b0 : pe == b1;
-        if (state_only && to_end) continue;
-        break;
-      }
-      chunks = static_cast<int>((pe - ps + kC - 1) / kC);
+      chunks = static_cast<int>((x.pe - x.ps + kC - 1) / kC);
     }
-    s0 = ps + static_cast<long long>(rev ? chunks - 1 - cc : cc) * kC;
-    len = static_cast<int>(min(static_cast<long long>(kC), pe - s0));
+    s0 = x.ps + static_cast<long long>(rev ? chunks - 1 - cc : cc) * kC;
+    len = static_cast<int>(min(static_cast<long long>(kC), x.pe - s0));
     return true;
   }
   __device__ __forceinline__ bool last() const { return cc == chunks - 1; }
 };
 
-// 32 floats of a state row to global memory, columns d0.. of dc.
-__device__ __forceinline__ void put_state(float* to, long long sj, int d0, int dc, const float* v) {
-  if (sj == 1 && d0 + 32 <= dc) {
+// Row i of a state between tensor memory and global memory, eight columns at
+// a time; `on` is false for lanes without a row.
+__device__ __noinline__ void put_state(uint32_t tm, float* to, long long sj, int dc, bool on) {
+#pragma unroll 1
+  for (int d = 0; d < dc; d += 8) {
+    uint32_t v[8];
+    tmem_ld8(tm + d, v);
+    wait_ld();
+    if (!on) continue;
+    if (sj == 1) {
+      *reinterpret_cast<uint4*>(to + d) = make_uint4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<uint4*>(to + d + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+    } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      *reinterpret_cast<float4*>(to + d0 + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 32; ++q)
-      if (d0 + q < dc) to[(d0 + q) * sj] = v[q];
+      for (int q = 0; q < 8; ++q) to[(d + q) * sj] = __uint_as_float(v[q]);
+    }
   }
 }
 
-__device__ __forceinline__ void get_state(const float* from, long long sj, int d0, int dc, float* v) {
-  if (sj == 1 && d0 + 32 <= dc) {
+// `from` null: zeros.  Columns up to the next 32 are written too.
+__device__ __noinline__ void get_state(uint32_t tm, const float* from, long long sj, int dc, bool on) {
+#pragma unroll 1
+  for (int d = 0; d < (dc + 31) / 32 * 32; d += 8) {
+    uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (from && on && d < dc) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float4 x = *reinterpret_cast<const float4*>(from + d0 + 4 * q);
-      v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
+      for (int q = 0; q < 8; ++q) v[q] = __float_as_uint(from[(d + q) * sj]);
     }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 32; ++q) v[q] = d0 + q < dc ? from[(d0 + q) * sj] : 0.f;
+    tmem_st8(tm + d, v);
   }
+  wait_st();
+}
+
+// NaN for what a value that is not finite reaches: rows from its token on
+// (row < 0: all of the lanes, the state).
+__device__ __noinline__ void spread_bad(uint32_t tm, const uint32_t* bad, uint32_t it, bool rev, int row, int dc) {
+#pragma unroll 1
+  for (int d = 0; d < dc; ++d) {
+    const int first = first_bad(bad[d], it, rev);
+    if (first < 0) continue;
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(tm + d));
+    wait_ld();
+    if (row < 0 || (rev ? row <= first : row >= first)) v = 0x7fffffffu;
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tm + d), "r"(v) : "memory");
+  }
+  wait_st();
 }
 
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -354,7 +406,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   if (!state_only) fill_outside<__nv_bfloat16>(p, f);
   if (tid == 0) {
-    for (int i = 0; i < kMaxSlots; ++i) bar_init(&t.full[i], 1), bar_init(&t.empty[i], 1);
+    for (int i = 0; i < kMaxSlots; ++i) bar_init(&t.full[i], 1), bar_init(&t.empty[i], state_only ? 1 : 5);
     bar_init(&t.tab_full, 1);
     bar_init(&t.tab_empty, state_only ? 8 : 12);
     bar_init(&t.sc_full, 1);
@@ -365,6 +417,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bar_init(&t.s_ready, 4);
     bar_init(&t.o_full, 1);
     bar_init(&t.o_free, 4);
+    bar_init(&t.d_full, 1);
     bar_init(&t.drain, 1);
     t.abort = 0;
     t.bad_chunk[0] = t.bad_chunk[1] = 0;
@@ -390,8 +443,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---- row warps ----
     const int row = warp * 32 + lane;
     const uint64_t sp2 = pair(f.sp, f.sp);
+    const bool dots = f.rowdot != nullptr;
+    uint32_t dot_loads = 0;
+    int slot = 0;
+    auto take = [&] {
+      const int x = slot;
+      if (++slot == geo.slots) slot = 0;
+      return x;
+    };
     for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
+      const int slot_b = take(), slot_a = take(), slot_c = take();
+      unsigned char* stage = smem + slot_a * geo.slot_bytes;
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       const float4 l4 = t.lg[row >> 1];
       const float lx = (row & 1) ? -l4.y : -l4.x, ly = (row & 1) ? -l4.w : -l4.z;
@@ -444,6 +507,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (!ctl.warp_wait(&t.in_full, ph)) break;
       fence_after();
+      // The products have read A: its slot holds first the rows to take dots
+      // with, then the finished rows on their way to whole-line stores.
+      if (dots && tid == 0) {
+        bar_expect(&t.d_full, blocks_c * 16384);
+        for (int b = 0; b < blocks_c; ++b)
+          tma_rows(smem_u32(stage + b * 16384), &map[3], b * 64, h / f.dot.share, static_cast<int>(w.s0), &t.d_full);
+        ++dot_loads;
+      }
       const uint64_t rf2 = pair(rf, rf);
 #pragma unroll 1
       for (int b = 0; b < nb; ++b) {
@@ -461,65 +532,85 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(&t.p_ready), bar_arrive(&t.tab_empty);
+      if (lane == 0) {
+        bar_arrive(&t.p_ready);
+        bar_arrive(&t.tab_empty);
+        bar_arrive(&t.empty[slot_b]);
+        bar_arrive(&t.empty[slot_c]);
+      }
 
+      if (dots && !ctl.warp_wait(&t.d_full, ph)) break;
       if (!ctl.warp_wait(&t.o_full, ph)) break;
       fence_after();
-      const long long tok = w.s0 + row;
-      const bool on = row < w.len;
-      const bool bad = t.bad_chunk[ph] == static_cast<int>(it) + 1;
-      const __nv_bfloat16* drow =
-          f.rowdot ? static_cast<const __nv_bfloat16*>(f.dot.p) + tok * f.dot.st + (h / f.dot.share) * f.dot.sh : nullptr;
-      float dot = 0.f;
+      if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(tm + lanes + kColO, t.bad[ph], it, rev, row, dc);
+      unsigned char* mine = stage + row * 128;
+      uint64_t dot2 = 0;
 #pragma unroll 1
       for (int b = 0; b < nb; ++b) {
         uint32_t v[32];
         tmem_ld32(tm + lanes + kColO + 32 * b, v);
         wait_ld();
-        if (bad) {
+        unsigned char* at = mine + (b >> 1) * 16384;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const int first = first_bad(t.bad[ph][32 * b + c], it, rev);
-            if (first >= 0 && (rev ? row <= first : row >= first)) v[c] = 0x7fffffffu;
+        for (int q = 0; q < 4; ++q) {
+          uint4* piece = reinterpret_cast<uint4*>(at + ((((b & 1) * 4 + q) ^ (row & 7)) << 4));
+          uint64_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = pair(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
+          if (dots) {
+            const uint4 y = *piece;
+            dot2 = fma2(x[0], pair(lo_f(y.x), hi_f(y.x)), dot2);
+            dot2 = fma2(x[1], pair(lo_f(y.y), hi_f(y.y)), dot2);
+            dot2 = fma2(x[2], pair(lo_f(y.z), hi_f(y.z)), dot2);
+            dot2 = fma2(x[3], pair(lo_f(y.w), hi_f(y.w)), dot2);
           }
+          if (!f.out_f32) *piece = make_uint4(round2(x[0]), round2(x[1]), round2(x[2]), round2(x[3]));
         }
-        if (on) {
-          const long long at = (tok * p.H + h) * dc + 32 * b;
-          if (f.out_f32) {
-            float* o = static_cast<float*>(f.out) + at;
+      }
+      if (f.out_f32) {
+        // 32 columns of float32 fill a row of the stage
+#pragma unroll 1
+        for (int b = 0; b < nb; ++b) {
+          uint32_t v[32];
+          tmem_ld32(tm + lanes + kColO + 32 * b, v);
+          wait_ld();
+          __syncwarp();
 #pragma unroll
-            for (int c = 0; c < 32; c += 4)
-              if (32 * b + c < dc) *reinterpret_cast<uint4*>(o + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-          } else {
-            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(f.out) + at;
-#pragma unroll
-            for (int c = 0; c < 32; c += 8)
-              if (32 * b + c < dc)
-                *reinterpret_cast<uint4*>(o + c) =
-                    make_uint4(bf2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])),
-                               bf2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])),
-                               bf2(__uint_as_float(v[c + 4]), __uint_as_float(v[c + 5])),
-                               bf2(__uint_as_float(v[c + 6]), __uint_as_float(v[c + 7])));
-          }
-          if (drow) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 8)
-              if (32 * b + c < dc) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(drow + 32 * b + c));
-                const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  dot = fmaf(__uint_as_float(v[c + 2 * q]), lo_f(e[q]), dot);
-                  dot = fmaf(__uint_as_float(v[c + 2 * q + 1]), hi_f(e[q]), dot);
-                }
-              }
-          }
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<uint4*>(mine + ((q ^ (row & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          __syncwarp();
+          if (32 * b + (lane & 7) * 4 < dc)
+#pragma unroll 1
+            for (int r = warp * 32 + (lane >> 3); r < min(warp * 32 + 32, w.len); r += 4)
+              *reinterpret_cast<uint4*>(static_cast<float*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 32 * b + (lane & 7) * 4) =
+                  *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
         }
       }
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&t.o_free);
-      if (on && drow) f.rowdot[h * p.BL + tok] = dot;
+      if (!f.out_f32) {
+        const int wide = dc > 64 ? 4 : 3, q = lane & ((1 << wide) - 1);  // lanes of a row
+        if (8 * q < dc)
+#pragma unroll 2
+          for (int r = warp * 32 + (lane >> wide); r < min(warp * 32 + 32, w.len); r += 32 >> wide)
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 8 * q) =
+                *reinterpret_cast<const uint4*>(stage + (q >> 3) * 16384 + r * 128 + (((q & 7) ^ (r & 7)) << 4));
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.empty[slot_a]);
+      if (dots && row < w.len) {
+        float x, y;
+        unpair(dot2, x, y);
+        f.rowdot[h * p.BL + w.s0 + row] = x + y;
+      }
+    }
+    if (dot_loads && !state_only) {  // in flight only after a give-up
+      const unsigned long long start = now_ns();
+      while (!bar_try(&t.d_full, (dot_loads - 1) & 1) && now_ns() - start < kStageTimeoutNs) {
+      }
     }
   } else if (warp < 8) {
     // ---- state warps ----
@@ -532,15 +623,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t ph = it & 1;
       const bool first = w.cc == 0;
       if (first) decay = 1.f;
-      const float* from = nullptr;
-      long long sj = 1;
-      if (first && !(state_only && !w.from_start)) {
-        if (w.from_start) {
-          if (f.init) from = f.init + (w.n * p.H + h) * mat + i * f.si, sj = f.sj;
-        } else {
-          from = f.carry + (static_cast<long long>(rev ? w.j + 1 : w.j - 1) * p.H + h) * mat + static_cast<long long>(i) * dc;
-        }
-      }
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       const float total = t.total;
       decay *= total;
@@ -548,29 +630,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ctl.warp_wait(&t.u_full, ph ^ 1)) break;
         fence_after();
       }
-      const bool bad = !first && t.bad_chunk[ph ^ 1] == static_cast<int>(it);
-      const long long edge = rev ? w.s0 + w.len : w.s0;
-      const bool snap = f.snap && !state_only && edge > w.ps && edge < w.pe && (edge - w.ps) % kRestart == 0;
-      float* snap_to = snap ? f.snap + (snap_slot(edge) * p.H + h) * mat + static_cast<long long>(i) * dc : nullptr;
+      const uint32_t ut = tm + lanes + kColU;
+      if (first) {
+        const float* from = nullptr;
+        long long sj = 1;
+        if (!(state_only && !w.x.from_start)) {
+          if (!w.x.from_start)
+            from = f.carry + (static_cast<long long>(blockIdx.x + (rev ? 1 : -1)) * p.H + h) * mat + static_cast<long long>(i) * dc;
+          else if (f.init)
+            from = f.init + (w.x.n * p.H + h) * mat + i * f.si, sj = f.sj;
+        }
+        if (work) get_state(ut, from, sj, dc, i < da);
+      } else if (work && t.bad_chunk[ph ^ 1] == static_cast<int>(it)) {
+        spread_bad(ut, t.bad[ph ^ 1], it - 1, rev, -1, dc);
+      }
+      if (f.snap && !state_only && work) {
+        const long long edge = rev ? w.s0 + w.len : w.s0;
+        if (edge > w.x.ps && edge < w.x.pe && (edge - w.x.ps) % kRestart == 0)
+          put_state(ut, f.snap + (snap_slot(edge) * p.H + h) * mat + static_cast<long long>(i) * dc, 1, dc, i < da);
+      }
       const uint64_t total2 = pair(total, total);
       if (work) {
 #pragma unroll 1
         for (int b = 0; b < nb; ++b) {
           float v[32];
-          if (first) {
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = 0.f;
-            if (from && i < da) get_state(from, sj, 32 * b, dc, v);
-          } else {
-            tmem_ld32(tm + lanes + kColU + 32 * b, reinterpret_cast<uint32_t*>(v));
-            wait_ld();
-            if (bad) {
-#pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (first_bad(t.bad[ph ^ 1][32 * b + q], it - 1, rev) >= 0) v[q] = __uint_as_float(0x7fffffffu);
-            }
-          }
-          if (snap && i < da) put_state(snap_to, 1, 32 * b, dc, v);
+          tmem_ld32(ut + 32 * b, reinterpret_cast<uint32_t*>(v));
+          wait_ld();
           if (!state_only && i < rows) {
             // S: row i of 64 columns is 128 bytes; four 16-byte pieces per 32 columns
             unsigned char* base = s_op + (b >> 1) * (geo.s_bytes / blocks_c) + i * 128;
@@ -590,7 +675,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
 #pragma unroll
           for (int q = 0; q < 32; q += 2) unpair(mul2(pair(v[q], v[q + 1]), total2), v[q], v[q + 1]);
-          tmem_st32(tm + lanes + kColU + 32 * b, reinterpret_cast<const uint32_t*>(v));
+          tmem_st32(ut + 32 * b, reinterpret_cast<const uint32_t*>(v));
         }
         wait_st();
       }
@@ -598,27 +683,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&t.s_ready), bar_arrive(&t.tab_empty);
-      if (w.last() && (state_only || (w.to_end && f.fin))) {
+      if (w.last() && (state_only || (w.x.to_end && f.fin))) {
         if (!ctl.warp_wait(&t.u_full, ph)) break;
         fence_after();
-        const bool hurt = t.bad_chunk[ph] == static_cast<int>(it) + 1;
-        float* to = state_only ? f.carry + (static_cast<long long>(w.j) * p.H + h) * mat + static_cast<long long>(i) * dc
-                               : f.fin + (w.n * p.H + h) * mat + i * f.si;
-        if (work)
-#pragma unroll 1
-          for (int b = 0; b < nb; ++b) {
-            float v[32];
-            tmem_ld32(tm + lanes + kColU + 32 * b, reinterpret_cast<uint32_t*>(v));
-            wait_ld();
-            if (hurt) {
-#pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (first_bad(t.bad[ph][32 * b + q], it, rev) >= 0) v[q] = __uint_as_float(0x7fffffffu);
-            }
-            if (i < da) put_state(to, state_only ? 1 : f.sj, 32 * b, dc, v);
-          }
+        float* to = state_only ? f.carry + (static_cast<long long>(blockIdx.x) * p.H + h) * mat + static_cast<long long>(i) * dc
+                               : f.fin + (w.x.n * p.H + h) * mat + i * f.si;
+        if (work) {
+          if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(ut, t.bad[ph], it, rev, -1, dc);
+          put_state(ut, to, state_only ? 1 : f.sj, dc, i < da);
+        }
         // a piece that holds the sequence's start takes nothing from before
-        if (state_only && i == 0) f.dec[w.j * p.H + h] = w.from_start ? -1.f : decay;
+        if (state_only && i == 0) f.dec[blockIdx.x * p.H + h] = w.x.from_start ? -1.f : decay;
       }
     }
   } else if (warp < 12) {
@@ -736,11 +811,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (tile >= static_cast<uint32_t>(geo.slots) && !ctl.wait(&t.empty[slot], (tile / geo.slots - 1) & 1)) return false;
         bar_expect(&t.full[slot], blocks * 16384);
         for (int b = 0; b < blocks; ++b)
-          asm volatile(
-              "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-                  "r"(smem_u32(smem + slot * geo.slot_bytes + b * 16384)),
-              "l"(&map[which]), "r"(b * 64), "r"(h / r.share), "r"(static_cast<int>(w.s0)), "r"(smem_u32(&t.full[slot]))
-              : "memory");
+          tma_rows(smem_u32(smem + slot * geo.slot_bytes + b * 16384), &map[which], b * 64, h / r.share,
+                   static_cast<int>(w.s0), &t.full[slot]);
         ++tile;
         return true;
       };
@@ -785,6 +857,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // the scores go where the previous chunk's P lies until its product is done
           if (it > 0 && !ctl.wait(&t.o_full, ph ^ 1)) break;
           fence_after();
+#pragma unroll 1
           for (int k = 0; k < ka; ++k) {
             const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
             mma_smem(tm + kColSc, desc(aa + o, 16), desc(ab + o, 16), id_sc, k > 0);
@@ -794,6 +867,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (it > 0 && !ctl.wait(&t.o_free, ph ^ 1)) break;
           fence_after();
           for (int term = 0; term < (two ? 2 : 1); ++term)
+#pragma unroll 1
             for (int k = 0; k < ka; ++k)
               mma_smem(tm + kColO, desc(aa + (k >> 2) * 16384 + (k & 3) * 32, 16),
                        desc(smem_u32(s_op) + term * geo.s_bytes + k * 2048, lbo_s), id_v, term + k > 0);
@@ -806,6 +880,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ctl.wait(fc, pc)) break;
         fence_after();
         for (int term = 0; term < 2; ++term)
+#pragma unroll 1
           for (int k = 0; k < kC / 16; ++k)
             mma_tmem(tm + kColU, tm + kColK + term * 64 + k * 8, desc(ac + k * 2048, 16384), id_v, true);
         commit(&t.u_full);
@@ -814,6 +889,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (!ctl.wait(&t.p_ready, ph)) break;
           fence_after();
           for (int term = 0; term < (two ? 2 : 1); ++term)
+#pragma unroll 1
             for (int k = 0; k < kC / 16; ++k)
               mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, desc(ac + k * 2048, 16384), id_v, true);
           commit(&t.o_full);
@@ -915,7 +991,8 @@ int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
   for (int r = 0; r < roles; ++r) {
     const Form& f = l.f[r];
     if (!map_rows(&maps.m[r][0], f.a, f.da, l.p.BL, l.p.H) || !map_rows(&maps.m[r][1], f.b, f.da, l.p.BL, l.p.H) ||
-        !map_rows(&maps.m[r][2], f.c, f.dc, l.p.BL, l.p.H))
+        !map_rows(&maps.m[r][2], f.c, f.dc, l.p.BL, l.p.H) ||
+        (f.rowdot && !map_rows(&maps.m[r][3], f.dot, f.dc, l.p.BL, l.p.H)))
       return ASCAN_EINVAL;
     const TcGeom g = tc_geom(f.da, f.dc);
     const size_t need = static_cast<size_t>(g.slots) * g.slot_bytes + 2 * g.s_bytes + sizeof(TcTail);
