@@ -59,7 +59,11 @@ struct TcTail {
   // Negated gate sums (of the mask's direction) in units of log 2, two tokens
   // an entry: floats of both, then what the floats leave over
   float4 lg[kC / 2];
+  // col[s]: the decay between token s and the edge of its 32 tokens (their
+  // last, or backwards the token before their first); far[b]: from there to
+  // the end (start) of the chunk.  The column factor is the product of both.
   float col[kC];
+  float far[4];
   // per value column, the chunk's first token that is not finite: chunk number
   // + 1 in the high bits, and below them its rank from the far end, so that
   // a maximum finds it and nothing has to be cleared
@@ -180,10 +184,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
       : "memory");
 }
 
-// 16 lanes by 16 columns; a pair of registers holds 4 columns: lane l of the
+// 16 lanes by 8 columns; a pair of registers holds 4 columns: lane l of the
 // warp has column l % 4 of row l / 4, then of row l / 4 + 8.
 __device__ __forceinline__ void tmem_st16x128(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), TC_I8(r, 0)
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
                : "memory");
 }
 
@@ -313,14 +318,14 @@ __device__ __noinline__ Piece next_piece(const Problem* pp, bool rev, bool state
 }
 
 // The CTA's chunks in scan order.
+template <bool rev, bool state_only>
 struct Walk {
   const Problem& p;
-  const bool rev, state_only;
   Piece x;
   long long s0;         // chunk start
   int chunks, cc, len;  // of the piece; chunk; its tokens
 
-  __device__ __forceinline__ Walk(const Problem& p_, bool rev_, bool so) : p(p_), rev(rev_), state_only(so), chunks(0), cc(-1) {
+  __device__ __forceinline__ explicit Walk(const Problem& p_) : p(p_), chunks(0), cc(-1) {
     x.m = 0;
   }
   __device__ __forceinline__ bool next() {
@@ -386,14 +391,15 @@ __device__ __noinline__ void spread_bad(uint32_t tm, const uint32_t* bad, uint32
   wait_st();
 }
 
-__global__ void __launch_bounds__(kTcThreads, 1)
-    tc_kernel(const __grid_constant__ Launch L, const __grid_constant__ TcMaps maps, const bool state_only) {
+// One form over the CTA's segment.  What differs between the forms is fixed
+// at compile time: the code that a CTA runs has to fit the instruction caches
+// (with all variants in one body the row warps waited longer for instructions
+// than for anything else).
+template <bool REV, bool TWO, bool STATE>
+__device__ __forceinline__ void body(const Problem& p, const Form& f, const CUtensorMap* map) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  const Problem& p = L.p;
-  const Form& f = L.f[blockIdx.z];
-  const CUtensorMap* map = maps.m[blockIdx.z];
+  constexpr bool rev = REV, two = TWO, state_only = STATE;
   const int da = f.da, dc = f.dc, h = blockIdx.y;
-  const bool rev = f.rev != 0, two = f.exact != 0;
   const TcGeom geo = tc_geom(da, dc);
   unsigned char* s_op = smem + geo.slots * geo.slot_bytes;
   TcTail& t = *reinterpret_cast<TcTail*>(s_op + 2 * geo.s_bytes);
@@ -437,13 +443,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int nb = (dc + 31) / 32;          // 32-column blocks of the values
   const int blocks_a = da > 64 ? 2 : 1, blocks_c = dc > 64 ? 2 : 1;
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's quarter of tensor memory
-  Walk w(p, rev, state_only);
+  Walk<REV, STATE> w(p);
 
   if (warp < 4) {
     // ---- row warps ----
     const int row = warp * 32 + lane;
     const uint64_t sp2 = pair(f.sp, f.sp);
-    const bool dots = f.rowdot != nullptr;
+    constexpr bool dots = TWO;  // the forms whose rows the gate's gradient needs
     uint32_t dot_loads = 0;
     int slot = 0;
     auto take = [&] {
@@ -463,47 +469,75 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float rf = (rev ? ex2((t.end.x + lx) + (t.end.y + ly)) : ex2(lx)) * f.sr;
       if (!ctl.warp_wait(&t.sc_full, ph)) break;
       fence_after();
+      // Blocks of 32 columns wholly inside the mask: the decay is that of the
+      // row to the block's edge times col[], two products an element.
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
+      for (int b = rev ? warp + 1 : 0; b < (rev ? 4 : warp); ++b) {
         const uint32_t col = tm + lanes + kColSc + 32 * b;
-        uint32_t hi[16], lo[16];
-        const bool some = (rev ? b >= warp : b <= warp) && 32 * b < w.len;
-        if (some) {
-          uint32_t s[32];
-          tmem_ld32(col, s);
-          wait_ld();
-          uint64_t pv[16];
+        uint32_t s[32], hi[16];
+        tmem_ld32(col, s);
+        const float4 e4 = t.lg[rev ? 16 * b - 1 : 16 * b + 15];
+        const float rd = ex2((lx + e4.y) + (ly + e4.w)) * f.sp;
+        const uint64_t rd2 = pair(rd, rd);
+        wait_ld();
+        const bool tail = rev && 32 * b + 32 > w.len;  // forwards such columns meet no row that counts
+        uint64_t pv[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float2 m = *reinterpret_cast<const float2*>(&t.col[32 * b + 2 * c]);
+          pv[c] = mul2(mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), pair(m.x, m.y)), rd2);
+        }
+        if (tail) {
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            const float4 m = t.lg[16 * b + c];
+            float p0, p1;
+            unpair(pv[c], p0, p1);
+            pv[c] = pair(32 * b + 2 * c < w.len ? p0 : 0.f, 32 * b + 2 * c + 1 < w.len ? p1 : 0.f);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) hi[c] = round2(pv[c]);
+        tmem_st16(col, hi);
+        if (two) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) hi[c] = rest2(pv[c], hi[c]);
+          tmem_st16(col + 16, hi);
+        }
+      }
+      {  // the mask's edge: every decay by itself, and select, not multiply
+        const uint32_t col = tm + lanes + kColSc + 32 * warp;
+        uint32_t s[32];
+        tmem_ld32(col, s);
+        wait_ld();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const int at = 16 * half + 2 * c, c0 = 32 * warp + at;
+            const float4 m = t.lg[16 * warp + 8 * half + c];
             const uint64_t x = add2(add2(lx2, pair(m.x, m.y)), add2(ly2, pair(m.z, m.w)));
             float x0, x1;
             unpair(x, x0, x1);
-            pv[c] = mul2(mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sp2), pair(ex2(x0), ex2(x1)));
+            const uint64_t y = mul2(mul2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), sp2), pair(ex2(x0), ex2(x1)));
+            unpair(y, x0, x1);
+            x0 = (rev ? c0 >= row && c0 < w.len : c0 <= row) ? x0 : 0.f;
+            x1 = (rev ? c0 + 1 >= row && c0 + 1 < w.len : c0 + 1 <= row) ? x1 : 0.f;
+            const uint64_t z = pair(x0, x1);
+            hi[c] = round2(z);
+            if (two) lo[c] = rest2(z, hi[c]);
           }
-          if (b == warp || 32 * b + 32 > w.len) {  // the mask's edge: select, not multiply
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const int c0 = 32 * b + 2 * c;
-              float p0, p1;
-              unpair(pv[c], p0, p1);
-              p0 = (rev ? c0 >= row : c0 <= row) && c0 < w.len ? p0 : 0.f;
-              p1 = (rev ? c0 + 1 >= row : c0 + 1 <= row) && c0 + 1 < w.len ? p1 : 0.f;
-              pv[c] = pair(p0, p1);
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < 16; ++c) hi[c] = round2(pv[c]);
-          if (two) {
-#pragma unroll
-            for (int c = 0; c < 16; ++c) lo[c] = rest2(pv[c], hi[c]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 16; ++c) hi[c] = lo[c] = 0u;
+          tmem_st8(col + 8 * half, hi);
+          if (two) tmem_st8(col + 16 + 8 * half, lo);
         }
-        tmem_st16(col, hi);
-        if (two) tmem_st16(col + 16, lo);
+      }
+#pragma unroll 1
+      for (int b = rev ? 0 : warp + 1; b < (rev ? warp : 4); ++b) {  // outside the mask
+        uint32_t none[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) none[c] = 0u;
+        tmem_st16(tm + lanes + kColSc + 32 * b, none);
+        if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, none);
       }
       if (!ctl.warp_wait(&t.in_full, ph)) break;
       fence_after();
@@ -764,10 +798,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t src = smem_u32(bt) + lead;
         const bool tail = w.len < kC;
 #pragma unroll 1
-        for (int s0 = 0; s0 < kC; s0 += 32) {
-          uint32_t hi[16], lo[16];  // [half of the rows][8 tokens][rows 0-7, 8-15]
+        for (int s0 = 0; s0 < kC; s0 += 16) {
+          uint32_t hi[8], lo[8];  // [half of the rows][8 tokens][rows 0-7, 8-15]
+          const float fb = t.far[s0 >> 5];
+          const uint64_t fb2 = pair(fb, fb);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < 2; ++g) {
             uint32_t r[4];
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -780,10 +816,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int m = 0; m < 4; ++m) r[m] &= keep;
             }
+            const uint64_t cf2 = mul2(pair(cf.x, cf.y), fb2);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-              const uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), pair(cf.x, cf.y));
-              const int at = (m >> 1) * 8 + g * 2 + (m & 1);
+              const uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), cf2);
+              const int at = (m >> 1) * 4 + g * 2 + (m & 1);
               hi[at] = round2(x);
               lo[at] = rest2(x, hi[at]);
             }
@@ -791,8 +828,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint32_t to = tm + lanes + (static_cast<uint32_t>(m) << 20) + kColK + s0 / 2;
-            tmem_st16x128(to, hi + 8 * m);
-            tmem_st16x128(to + 64, lo + 8 * m);
+            tmem_st16x128(to, hi + 4 * m);
+            tmem_st16x128(to + 64, lo + 4 * m);
           }
         }
         wait_st();
@@ -834,67 +871,70 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (lane == 0) {
       const uint32_t id_sc = idesc(kC, false), id_v = idesc((dc + 15) / 16 * 16, true);
       const int ka = (da + 15) / 16;
-      const uint32_t lbo_s = geo.s_bytes / blocks_c;
-      int slot = 0, round = 0;
-      auto take = [&](uint64_t** full, uint64_t** empty, uint32_t* ph) {
-        const uint32_t a = smem_u32(smem + slot * geo.slot_bytes);
-        *full = &t.full[slot];
-        *empty = &t.empty[slot];
-        *ph = round & 1;
+      const uint64_t ds = desc(smem_u32(s_op), geo.s_bytes / blocks_c);
+      int slot = 0;
+      uint32_t round = 0;
+      auto take = [&] {
+        const int x = slot;
         if (++slot == geo.slots) slot = 0, ++round;
-        return a;
+        return x;
       };
+      auto rows_desc = [&](int x, uint32_t lbo) { return desc(smem_u32(smem) + x * geo.slot_bytes, lbo); };
       for (uint32_t it = 0; w.next(); ++it) {
         const uint32_t ph = it & 1;
-        uint64_t *fb, *eb, *fa = nullptr, *ea = nullptr, *fc, *ec;
-        uint32_t pb, pa = 0, pc, aa = 0;
-        const uint32_t ab = take(&fb, &eb, &pb);
-        if (!state_only) aa = take(&fa, &ea, &pa);
-        const uint32_t ac = take(&fc, &ec, &pc);
-        if (!ctl.wait(fb, pb)) break;
+        uint32_t r = round;
+        const int sb = take();
+        if (!ctl.wait(&t.full[sb], r & 1)) break;
+        int sa = 0;
         if (!state_only) {
-          if (!ctl.wait(fa, pa)) break;
+          r = round;
+          sa = take();
+          if (!ctl.wait(&t.full[sa], r & 1)) break;
           // the scores go where the previous chunk's P lies until its product is done
           if (it > 0 && !ctl.wait(&t.o_full, ph ^ 1)) break;
           fence_after();
+          const uint64_t a = rows_desc(sa, 16), b = rows_desc(sb, 16);
 #pragma unroll 1
           for (int k = 0; k < ka; ++k) {
-            const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
-            mma_smem(tm + kColSc, desc(aa + o, 16), desc(ab + o, 16), id_sc, k > 0);
+            const uint32_t o = (k >> 2) * 1024 + (k & 3) * 2;  // in 16 bytes: the next 64 columns, 16 of them
+            mma_smem(tm + kColSc, a + o, b + o, id_sc, k > 0);
           }
           commit(&t.sc_full);
           if (!ctl.wait(&t.s_ready, ph)) break;
           if (it > 0 && !ctl.wait(&t.o_free, ph ^ 1)) break;
           fence_after();
+#pragma unroll 1
           for (int term = 0; term < (two ? 2 : 1); ++term)
 #pragma unroll 1
             for (int k = 0; k < ka; ++k)
-              mma_smem(tm + kColO, desc(aa + (k >> 2) * 16384 + (k & 3) * 32, 16),
-                       desc(smem_u32(s_op) + term * geo.s_bytes + k * 2048, lbo_s), id_v, term + k > 0);
+              mma_smem(tm + kColO, a + (k >> 2) * 1024 + (k & 3) * 2, ds + term * (geo.s_bytes >> 4) + k * 128, id_v, term + k > 0);
           commit(&t.in_full);
-          commit(ea);
+          commit(&t.empty[sa]);
         } else if (!ctl.wait(&t.s_ready, ph)) {
           break;
         }
+        r = round;
+        const int sc = take();
         if (!ctl.wait(&t.kt_ready, ph)) break;
-        if (!ctl.wait(fc, pc)) break;
+        if (!ctl.wait(&t.full[sc], r & 1)) break;
         fence_after();
-        for (int term = 0; term < 2; ++term)
+        const uint64_t c = rows_desc(sc, 16384);
 #pragma unroll 1
-          for (int k = 0; k < kC / 16; ++k)
-            mma_tmem(tm + kColU, tm + kColK + term * 64 + k * 8, desc(ac + k * 2048, 16384), id_v, true);
+        for (int k = 0; k < 2 * kC / 16; ++k)  // both terms lie side by side
+          mma_tmem(tm + kColU, tm + kColK + k * 8, c + (k & 7) * 128, id_v, true);
         commit(&t.u_full);
-        commit(eb);
+        commit(&t.empty[sb]);
         if (!state_only) {
           if (!ctl.wait(&t.p_ready, ph)) break;
           fence_after();
+#pragma unroll 1
           for (int term = 0; term < (two ? 2 : 1); ++term)
 #pragma unroll 1
             for (int k = 0; k < kC / 16; ++k)
-              mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, desc(ac + k * 2048, 16384), id_v, true);
+              mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, c + k * 128, id_v, true);
           commit(&t.o_full);
         }
-        commit(ec);
+        commit(&t.empty[sc]);
       }
       commit(&t.drain);  // nothing of this CTA's is in flight after it
       const unsigned long long start = now_ns();
@@ -905,10 +945,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---- gates: four tokens a lane ----
     for (uint32_t it = 0; w.next(); ++it) {
       double g[4], sum = 0.0;
+      float raw[4] = {0.f, 0.f, 0.f, 0.f};
+      const long long at = w.s0 * p.gate.st + (h / p.gate.share) * p.gate.sh;
+      if (p.gate_type == ASCAN_F32) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (lane * 4 + q < w.len) raw[q] = __ldg(static_cast<const float*>(p.gate.p) + at + (lane * 4 + q) * p.gate.st);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (lane * 4 + q < w.len)
+            raw[q] = __uint_as_float(static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(p.gate.p) + at + (lane * 4 + q) * p.gate.st)) << 16);
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int s = lane * 4 + q;
-        sum += s < w.len ? static_cast<double>(load_gate(p, w.s0 + s, h)) : 0.0;
+        sum += static_cast<double>(raw[q] < kGateFloor ? kGateFloor : raw[q]);
         g[q] = sum;
       }
       double inc = sum;
@@ -928,12 +979,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const double x = (inc - sum + g[q]) * (rev ? 1.4426950408889634 : -1.4426950408889634);
         lx[q] = static_cast<float>(x);
         ly[q] = static_cast<float>(x - static_cast<double>(lx[q]));
-        col[q] = ex2(rev ? lx[q] : lx[q] - whole.x + (ly[q] - whole.y)) * f.sc;
       }
+      // the edge of the lane's 32 tokens: their last, or the one before them
+      const float ex = rev ? __shfl_sync(kFull, lx[3], (lane & 24) - 1) : __shfl_sync(kFull, lx[3], lane | 7);
+      const float ey = rev ? __shfl_sync(kFull, ly[3], (lane & 24) - 1) : __shfl_sync(kFull, ly[3], lane | 7);
+      const bool zero = rev && lane < 8;  // before the chunk's first token the sum is zero
+#pragma unroll
+      for (int q = 0; q < 4; ++q) col[q] = zero ? ex2(lx[q]) : ex2((lx[q] - ex) + (ly[q] - ey));
+      const float far = (rev ? (zero ? 1.f : ex2(ex)) : ex2((ex - whole.x) + (ey - whole.y))) * f.sc;
       if (it > 0 && !ctl.warp_wait(&t.tab_empty, (it & 1) ^ 1)) break;
       t.lg[lane * 2] = make_float4(lx[0], lx[1], ly[0], ly[1]);
       t.lg[lane * 2 + 1] = make_float4(lx[2], lx[3], ly[2], ly[3]);
       *reinterpret_cast<float4*>(&t.col[lane * 4]) = make_float4(col[0], col[1], col[2], col[3]);
+      if ((lane & 7) == 0) t.far[lane >> 3] = far;
       if (lane == 0) {
         t.total = ex2(rev ? whole.x : -whole.x);
         t.end = whole;
@@ -948,6 +1006,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 13) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
+  }
+}
+
+template <bool STATE>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tc_kernel(const __grid_constant__ Launch L, const __grid_constant__ TcMaps maps) {
+  const Form& f = L.f[blockIdx.z];
+  const CUtensorMap* map = maps.m[blockIdx.z];
+  if (STATE) {
+    if (f.rev) body<true, false, true>(L.p, f, map);
+    else body<false, false, true>(L.p, f, map);
+  } else if (f.exact) {
+    if (f.rev) body<true, true, false>(L.p, f, map);
+    else body<false, true, false>(L.p, f, map);
+  } else {
+    if (f.rev) body<true, false, false>(L.p, f, map);
+    else body<false, false, false>(L.p, f, map);
   }
 }
 
@@ -1000,9 +1075,12 @@ int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
   }
   static std::once_flag once;
   std::call_once(once, [] {
-    cudaFuncSetAttribute(tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
+    cudaFuncSetAttribute(tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
+    cudaFuncSetAttribute(tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
   });
-  tc_kernel<<<dim3(l.p.J, l.p.H, roles), kTcThreads, smem, s>>>(l, maps, state_only);
+  const dim3 grid(l.p.J, l.p.H, roles);
+  if (state_only) tc_kernel<true><<<grid, kTcThreads, smem, s>>>(l, maps);
+  else tc_kernel<false><<<grid, kTcThreads, smem, s>>>(l, maps);
   return launch_status();
 }
 
