@@ -51,7 +51,7 @@ constexpr unsigned long long kStageTimeoutNs = 2000000000ull;
 constexpr size_t kSmemLimit = 232448;
 
 struct TcMaps {
-  CUtensorMap m[3][4];  // per form: A, B, C, and the rows to take dots with
+  CUtensorMap m[3][5];  // per form: A, B, C, the rows to take dots with, the output
 };
 
 // Shared memory after the ring and the S operand.
@@ -69,7 +69,7 @@ struct TcTail {
   // a maximum finds it and nothing has to be cleared
   uint32_t bad[2][kC];
   uint64_t full[kMaxSlots], empty[kMaxSlots];
-  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready, u_full, s_ready, o_full, o_free, d_full, drain;
+  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
   float2 end;  // the chunk's whole gate sum, same form
   float total;
   int bad_chunk[2];  // chunk number + 1 when bad[] holds something
@@ -412,14 +412,16 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   }
   if (!state_only) fill_outside<__nv_bfloat16>(p, f);
   if (tid == 0) {
-    for (int i = 0; i < kMaxSlots; ++i) bar_init(&t.full[i], 1), bar_init(&t.empty[i], state_only ? 1 : 5);
+    for (int i = 0; i < kMaxSlots; ++i) bar_init(&t.full[i], 1), bar_init(&t.empty[i], 5);  // four warps and the products
     bar_init(&t.tab_full, 1);
     bar_init(&t.tab_empty, state_only ? 8 : 12);
     bar_init(&t.sc_full, 1);
     bar_init(&t.in_full, 1);
     bar_init(&t.p_ready, 4);
-    bar_init(&t.kt_ready, 4);
-    bar_init(&t.u_full, 1);
+    bar_init(&t.kt_ready[0], 4);
+    bar_init(&t.kt_ready[1], 4);
+    bar_init(&t.u_full[0], 1);
+    bar_init(&t.u_full[1], 1);
     bar_init(&t.s_ready, 4);
     bar_init(&t.o_full, 1);
     bar_init(&t.o_free, 4);
@@ -451,7 +453,14 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     const uint64_t sp2 = pair(f.sp, f.sp);
     constexpr bool dots = TWO;  // the forms whose rows the gate's gradient needs
     uint32_t dot_loads = 0;
-    int slot = 0;
+    int slot = 0, held = -1;  // held: slot that the last rows leave from
+    auto release = [&] {
+      if (held >= 0 && lane == 0) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        bar_arrive(&t.empty[held]);
+      }
+      held = -1;
+    };
     auto take = [&] {
       const int x = slot;
       if (++slot == geo.slots) slot = 0;
@@ -459,7 +468,8 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     };
     for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
-      const int slot_b = take(), slot_a = take(), slot_c = take();
+      take();
+      const int slot_a = take(), slot_c = take();
       unsigned char* stage = smem + slot_a * geo.slot_bytes;
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       const float4 l4 = t.lg[row >> 1];
@@ -539,6 +549,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         tmem_st16(tm + lanes + kColSc + 32 * b, none);
         if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, none);
       }
+      release();
       if (!ctl.warp_wait(&t.in_full, ph)) break;
       fence_after();
       // The products have read A: its slot holds first the rows to take dots
@@ -569,7 +580,6 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       if (lane == 0) {
         bar_arrive(&t.p_ready);
         bar_arrive(&t.tab_empty);
-        bar_arrive(&t.empty[slot_b]);
         bar_arrive(&t.empty[slot_c]);
       }
 
@@ -624,23 +634,39 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&t.o_free);
-      if (!f.out_f32) {
-        const int wide = dc > 64 ? 4 : 3, q = lane & ((1 << wide) - 1);  // lanes of a row
-        if (8 * q < dc)
-#pragma unroll 2
-          for (int r = warp * 32 + (lane >> wide); r < min(warp * 32 + 32, w.len); r += 32 >> wide)
-            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 8 * q) =
-                *reinterpret_cast<const uint4*>(stage + (q >> 3) * 16384 + r * 128 + (((q & 7) ^ (r & 7)) << 4));
-      }
+      // The warp's 32 rows to memory: whole ones by bulk copies that the slot
+      // waits for one chunk later, those at a piece's end by the lanes.
       fence_async();
       __syncwarp();
-      if (lane == 0) bar_arrive(&t.empty[slot_a]);
+      if (!f.out_f32) {
+        if (warp * 32 + 32 <= w.len) {
+          if (lane == 0) {
+            for (int b = 0; b < blocks_c; ++b)
+              asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(&map[4]),
+                           "r"(b * 64), "r"(h), "r"(static_cast<int>(w.s0) + warp * 32),
+                           "r"(smem_u32(stage + b * 16384 + warp * 4096))
+                           : "memory");
+          }
+        } else {
+#pragma unroll 1
+          for (int e = lane; e < 32 * 16; e += 32) {
+            const int r = warp * 32 + (e >> 4), q = e & 15;
+            if (r < w.len && 8 * q < dc)
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 8 * q) =
+                  *reinterpret_cast<const uint4*>(stage + (q >> 3) * 16384 + r * 128 + (((q & 7) ^ (r & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      }
+      if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      held = slot_a;
       if (dots && row < w.len) {
         float x, y;
         unpair(dot2, x, y);
         f.rowdot[h * p.BL + w.s0 + row] = x + y;
       }
     }
+    if (!state_only && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (dot_loads && !state_only) {  // in flight only after a give-up
       const unsigned long long start = now_ns();
       while (!bar_try(&t.d_full, (dot_loads - 1) & 1) && now_ns() - start < kStageTimeoutNs) {
@@ -661,7 +687,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const float total = t.total;
       decay *= total;
       if (it > 0) {  // the update before this chunk; it also follows the last use of S
-        if (!ctl.warp_wait(&t.u_full, ph ^ 1)) break;
+        if (!ctl.warp_wait(&t.u_full[ph ^ 1], ((it - 1) >> 1) & 1)) break;
         fence_after();
       }
       const uint32_t ut = tm + lanes + kColU;
@@ -670,7 +696,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         long long sj = 1;
         if (!(state_only && !w.x.from_start)) {
           if (!w.x.from_start)
-            from = f.carry + (static_cast<long long>(blockIdx.x + (rev ? 1 : -1)) * p.H + h) * mat + static_cast<long long>(i) * dc;
+            from = f.carry + ((static_cast<long long>(blockIdx.x) + (rev ? 1 : -1)) * p.H + h) * mat + static_cast<long long>(i) * dc;
           else if (f.init)
             from = f.init + (w.x.n * p.H + h) * mat + i * f.si, sj = f.sj;
         }
@@ -718,7 +744,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       __syncwarp();
       if (lane == 0) bar_arrive(&t.s_ready), bar_arrive(&t.tab_empty);
       if (w.last() && (state_only || (w.x.to_end && f.fin))) {
-        if (!ctl.warp_wait(&t.u_full, ph)) break;
+        if (!ctl.warp_wait(&t.u_full[ph], (it >> 1) & 1)) break;
         fence_after();
         float* to = state_only ? f.carry + (static_cast<long long>(blockIdx.x) * p.H + h) * mat + static_cast<long long>(i) * dc
                                : f.fin + (w.x.n * p.H + h) * mat + i * f.si;
@@ -741,24 +767,32 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     int slot = 0, round = 0;  // of the next tile
     for (uint32_t it = 0; w.next(); ++it) {
       const uint32_t ph = it & 1;
+      const int slot_b = slot;
       const unsigned char* bt = smem + slot * geo.slot_bytes;
-      uint64_t* bfull = &t.full[slot];
       const uint32_t bph = round & 1;
       for (int k = 1; k < per; ++k)
         if (++slot == geo.slots) slot = 0, ++round;
+      const int slot_c = slot;
       unsigned char* ct = smem + slot * geo.slot_bytes;
-      uint64_t* cfull = &t.full[slot];
       const uint32_t cph = round & 1;
       if (++slot == geo.slots) slot = 0, ++round;
 
-      // The previous update is done: its operand may be overwritten, and the
-      // row and state warps have read what bad[ph] held two chunks ago.
-      if (it > 0) {
-        if (!ctl.warp_wait(&t.u_full, ph ^ 1)) break;
+      // An update is done: its operand may be overwritten.  The previous one's,
+      // when outputs are computed, which also shows that the row and state
+      // warps have read what bad[ph] held two chunks ago; else the one before,
+      // since the scores' place holds a second operand.
+      const uint32_t before = state_only ? 2 : 1;
+      if (it >= before) {
+        if (!ctl.warp_wait(&t.u_full[(it - before) & 1], ((it - before) >> 1) & 1)) break;
         fence_after();
       }
-      if (!ctl.warp_wait(cfull, cph)) break;
-      {  // one token row of C per thread
+      const uint32_t kt = tm + lanes + (state_only && ph ? kColSc : kColK);
+      if (!state_only || w.len < kC)
+        if (!ctl.warp_wait(&t.full[slot_c], cph)) break;
+      if (state_only) {
+        if (i >= w.len)  // another sequence's token, or past the end
+          for (int q = 0; q < 8 * blocks_c; ++q) *reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + ((q & 7) << 4)) = make_uint4(0, 0, 0, 0);
+      } else {  // one token row of C per thread
         const bool live = i < w.len;
         const __nv_bfloat162 none = __float2bfloat162_rn(0.f);
         __nv_bfloat162 sum = none;  // sum of 0 * x: NaN if any x is not finite
@@ -793,7 +827,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       fence_async();
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
-      if (!ctl.warp_wait(bfull, bph)) break;
+      if (!ctl.warp_wait(&t.full[slot_b], bph)) break;
       if (work) {
         const uint32_t src = smem_u32(bt) + lead;
         const bool tail = w.len < kC;
@@ -827,7 +861,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           }
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            const uint32_t to = tm + lanes + (static_cast<uint32_t>(m) << 20) + kColK + s0 / 2;
+            const uint32_t to = kt + (static_cast<uint32_t>(m) << 20) + s0 / 2;
             tmem_st16x128(to, hi + 4 * m);
             tmem_st16x128(to + 64, lo + 4 * m);
           }
@@ -836,7 +870,12 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(&t.kt_ready), bar_arrive(&t.tab_empty);
+      if (lane == 0) {
+        bar_arrive(&t.kt_ready[ph]);
+        bar_arrive(&t.tab_empty);
+        bar_arrive(&t.empty[slot_b]);
+        if (state_only) bar_arrive(&t.empty[slot_c]);
+      }
     }
   } else if (warp == 12) {
     // ---- loads ----
@@ -894,18 +933,19 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           if (it > 0 && !ctl.wait(&t.o_full, ph ^ 1)) break;
           fence_after();
           const uint64_t a = rows_desc(sa, 16), b = rows_desc(sb, 16);
-#pragma unroll 1
+#pragma unroll 4
           for (int k = 0; k < ka; ++k) {
             const uint32_t o = (k >> 2) * 1024 + (k & 3) * 2;  // in 16 bytes: the next 64 columns, 16 of them
             mma_smem(tm + kColSc, a + o, b + o, id_sc, k > 0);
           }
           commit(&t.sc_full);
+          commit(&t.empty[sb]);
           if (!ctl.wait(&t.s_ready, ph)) break;
           if (it > 0 && !ctl.wait(&t.o_free, ph ^ 1)) break;
           fence_after();
 #pragma unroll 1
           for (int term = 0; term < (two ? 2 : 1); ++term)
-#pragma unroll 1
+#pragma unroll 4
             for (int k = 0; k < ka; ++k)
               mma_smem(tm + kColO, a + (k >> 2) * 1024 + (k & 3) * 2, ds + term * (geo.s_bytes >> 4) + k * 128, id_v, term + k > 0);
           commit(&t.in_full);
@@ -915,21 +955,22 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         }
         r = round;
         const int sc = take();
-        if (!ctl.wait(&t.kt_ready, ph)) break;
+        if (!ctl.wait(&t.kt_ready[ph], (it >> 1) & 1)) break;
         if (!ctl.wait(&t.full[sc], r & 1)) break;
         fence_after();
         const uint64_t c = rows_desc(sc, 16384);
-#pragma unroll 1
+        const uint32_t kt = tm + (state_only && ph ? kColSc : kColK);
+#pragma unroll 4
         for (int k = 0; k < 2 * kC / 16; ++k)  // both terms lie side by side
-          mma_tmem(tm + kColU, tm + kColK + k * 8, c + (k & 7) * 128, id_v, true);
-        commit(&t.u_full);
-        commit(&t.empty[sb]);
+          mma_tmem(tm + kColU, kt + k * 8, c + (k & 7) * 128, id_v, true);
+        commit(&t.u_full[ph]);
+        if (state_only) commit(&t.empty[sb]);
         if (!state_only) {
           if (!ctl.wait(&t.p_ready, ph)) break;
           fence_after();
 #pragma unroll 1
           for (int term = 0; term < (two ? 2 : 1); ++term)
-#pragma unroll 1
+#pragma unroll 4
             for (int k = 0; k < kC / 16; ++k)
               mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, c + k * 128, id_v, true);
           commit(&t.o_full);
@@ -1026,14 +1067,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-static bool map_rows(CUtensorMap* m, const Rows& r, int dim, long long BL, int H) {
+static bool map_rows(CUtensorMap* m, const Rows& r, int dim, long long BL, int H, int tokens = kC) {
   const auto fn = encode_fn();
   if (!fn) return false;
   const int heads = H / r.share;
   const long long sh = heads > 1 ? r.sh : (dim + 7) / 8 * 8;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(BL)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(r.st) * 2};
-  const cuuint32_t box[3] = {64, 1, kC}, one[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(tokens)}, one[3] = {1, 1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(r.p), dims, strides, box, one,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1067,7 +1108,8 @@ int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
     const Form& f = l.f[r];
     if (!map_rows(&maps.m[r][0], f.a, f.da, l.p.BL, l.p.H) || !map_rows(&maps.m[r][1], f.b, f.da, l.p.BL, l.p.H) ||
         !map_rows(&maps.m[r][2], f.c, f.dc, l.p.BL, l.p.H) ||
-        (f.rowdot && !map_rows(&maps.m[r][3], f.dot, f.dc, l.p.BL, l.p.H)))
+        (f.rowdot && !map_rows(&maps.m[r][3], f.dot, f.dc, l.p.BL, l.p.H)) ||
+        (!f.out_f32 && !map_rows(&maps.m[r][4], Rows{f.out, static_cast<long long>(l.p.H) * f.dc, f.dc, 1}, f.dc, l.p.BL, l.p.H, 32)))
       return ASCAN_EINVAL;
     const TcGeom g = tc_geom(f.da, f.dc);
     const size_t need = static_cast<size_t>(g.slots) * g.slot_bytes + 2 * g.s_bytes + sizeof(TcTail);
