@@ -327,7 +327,12 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const long long t = s1 - 1 - (tid * 4 + q);
-        v[q] = t >= s0 ? fq.rowdot[h * p.BL + t] - fk.rowdot[h * p.BL + t] : 0.f;
+        v[q] = 0.f;
+        if (t >= s0) {
+          const long long at = h * p.BL + t, half = p.H * p.BL;
+          const float a = fq.rowdot[at] + (fq.dot_parts > 1 ? fq.rowdot[at + half] : 0.f);
+          v[q] = a - (fk.rowdot[at] + (fk.dot_parts > 1 ? fk.rowdot[at + half] : 0.f));
+        }
         sum += v[q];
       }
       float inc = sum;
@@ -513,9 +518,10 @@ static int plain_run(const Launch& l, int roles, bool state_only, int dtype, cud
 #undef MSCAN_PLAIN
 }
 
-static int run_forms(const Launch& l, int roles, int dtype, cudaStream_t s) {
+static int run_forms(Launch& l, int roles, int dtype, cudaStream_t s) {
   int rc = ASCAN_OK;
   const bool tc = tc_usable(l, roles, dtype);
+  for (int r = 0; r < roles; ++r) l.f[r].dot_parts = tc ? tc_dot_parts(l.f[r]) : 1;
   if (l.p.J > 1) {
     rc = tc ? tc_run(l, roles, true, s) : plain_run(l, roles, true, dtype, s);
     if (rc != ASCAN_OK) return rc;
@@ -549,7 +555,7 @@ static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, 
   w.total = w.carry * (backward ? 3 : 1);
   if (backward) {
     w.snap = up(w.slots * mat);
-    w.rowdot = up(rows);
+    w.rowdot = up(2 * rows);
     w.part_q = hq < H ? up(rows * dk) : 0;
     w.part_k = hk < H ? up(rows * dk) : 0;
     w.part_v = hv < H ? up(rows * dv) : 0;

@@ -63,7 +63,8 @@ struct Form {
   float sp, sr, sc;  // factors of the scores, of the rows and of the columns
   void* out;         // [BL, H, dc]
   int out_f32;
-  float* rowdot;      // [H, BL]
+  float* rowdot;      // [2, H, BL]: sums over halves of the columns
+  int dot_parts;      // how many of them the kernel wrote (set before the launch)
   const float* init;  // per sequence and head, element (i, j) at i*si + j*sj; may be null
   float* fin;
   long long si, sj;
@@ -151,6 +152,7 @@ __device__ __forceinline__ long long snap_slot(long long at) { return at / kRest
 
 // The tensor-core kernel (ascan_mscan_tc.cu).
 bool tc_usable(const Launch& l, int roles, int dtype);
+int tc_dot_parts(const Form& f);
 int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s);
 
 }  // namespace mscan

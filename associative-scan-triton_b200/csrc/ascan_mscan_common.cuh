@@ -31,7 +31,6 @@ __device__ __forceinline__ void fill_outside(const Problem& p, const Form& f) {
       if (f.out_f32) static_cast<float*>(f.out)[at] = 0.f;
       else static_cast<T*>(f.out)[at] = from_f<T>(0.f);
     }
-    if (f.rowdot && tid == 0) f.rowdot[h * p.BL + t] = 0.f;
   }
   if (f.fin && j == 0) {
     const long long mat = static_cast<long long>(f.da) * f.dc;

@@ -14,15 +14,16 @@
 // gradient) depends on them.  A and C come as stored, so they are exact.
 //
 // Roles, by warp (one CTA per SM; every hand-over is an mbarrier):
-//   0-3    row warps: scores -> P in place in tensor memory, scale O by the
-//          row factors, store the finished rows
-//   4-7    state warps: the state from tensor memory to the operand S in
+//   0-7    row warps, two for each 32 tokens: scores -> P in place in tensor
+//          memory, scale O by the row factors, store the finished rows (each
+//          takes one half of the columns; P is the longest part of a chunk)
+//   8-11   state warps: the state from tensor memory to the operand S in
 //          shared memory, scaled back for the next update
-//   8-11   column warps: (col . B)^T transposed into tensor memory; tails and
+//   12-15  column warps: (col . B)^T transposed into tensor memory; tails and
 //          values that are not finite in C
-//   12     TMA loads of the A, B, C tiles into a ring of shared-memory slots
-//   13     issues the products
-//   14     the chunk's gate sums, row and column factors
+//   16     TMA loads of the A, B, C tiles into shared-memory slots
+//   17     issues the products
+//   18     the chunk's gate sums, row and column factors
 //
 // Tensor memory (512 columns of 128 lanes): scores/P 128, O 128, U 128,
 // (col.B)^T 64 + 64.  Lanes are tokens for scores and O, state rows for U.
@@ -43,9 +44,8 @@ namespace ascan {
 namespace mscan {
 
 constexpr int kC = 128;             // tokens of a chunk
-constexpr int kTcWarps = 15;
+constexpr int kTcWarps = 19;
 constexpr int kTcThreads = kTcWarps * 32;
-constexpr int kMaxSlots = 8;
 constexpr uint32_t kColSc = 0, kColO = 128, kColU = 256, kColK = 384;
 constexpr unsigned long long kStageTimeoutNs = 2000000000ull;
 constexpr size_t kSmemLimit = 232448;
@@ -54,7 +54,7 @@ struct TcMaps {
   CUtensorMap m[3][5];  // per form: A, B, C, the rows to take dots with, the output
 };
 
-// Shared memory after the ring and the S operand.
+// Shared memory after the tile slots and the S operand.
 struct TcTail {
   // Negated gate sums (of the mask's direction) in units of log 2, two tokens
   // an entry: floats of both, then what the floats leave over
@@ -68,7 +68,7 @@ struct TcTail {
   // + 1 in the high bits, and below them its rank from the far end, so that
   // a maximum finds it and nothing has to be cleared
   uint32_t bad[2][kC];
-  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t full[6], empty[6];  // slots of A: 0, 1; of C: 2, 3; of B: 4 and, if there is room, 5
   uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
   float2 end;  // the chunk's whole gate sum, same form
   float total;
@@ -77,16 +77,20 @@ struct TcTail {
   uint32_t tmem;
 };
 
+// A slot waits for its rows to leave the chip and C's for the last product, so
+// both are double; B is done with early, and a second slot of it is a bonus.
 struct TcGeom {
-  int slot_bytes, slots, s_bytes;  // bytes of a ring slot and of one term of S
+  int slot_bytes, s_bytes;  // bytes of a slot and of one term of S
+  int b_slots;
+  __host__ __device__ int bytes() const { return (4 + b_slots) * slot_bytes + 2 * s_bytes; }
 };
 
 __host__ __device__ inline TcGeom tc_geom(int da, int dc) {
   TcGeom g;
   g.slot_bytes = (da > 64 || dc > 64) ? 32768 : 16384;
   g.s_bytes = (da > 64 ? 128 : 64) * 128 * (dc > 64 ? 2 : 1);
-  g.slots = static_cast<int>((kSmemLimit - sizeof(TcTail) - 2 * g.s_bytes) / g.slot_bytes);
-  if (g.slots > kMaxSlots) g.slots = kMaxSlots;
+  g.b_slots = 2;
+  if (g.bytes() + sizeof(TcTail) > kSmemLimit) g.b_slots = 1;
   return g;
 }
 
@@ -125,17 +129,23 @@ __device__ __forceinline__ void tma_rows(uint32_t to, const CUtensorMap* m, int 
       "l"(m), "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
       : "memory");
 }
+// One lane of the warp, by the instruction that the compiler knows to pick
+// one: behind it operands stay in uniform registers, and a product takes 50
+// cycles to issue instead of 90 (it runs for 64).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
       : "memory");
 }
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
       : "memory");
 }
@@ -161,19 +171,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
       : TC_R8(r, 0), TC_R8(r, 8), TC_R8(r, 16), TC_R8(r, 24)
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      TC_I8(r, 0), TC_I8(r, 8), TC_I8(r, 16), TC_I8(r, 24)
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : TC_R8(r, 0), TC_R8(r, 8)
+      : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : TC_R8(r, 0) : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), TC_I8(r, 0)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3])
                : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
@@ -361,10 +374,10 @@ __device__ __noinline__ void put_state(uint32_t tm, float* to, long long sj, int
   }
 }
 
-// `from` null: zeros.  Columns up to the next 32 are written too.
+// `from` null: zeros.  Columns up to the next 16 are written too.
 __device__ __noinline__ void get_state(uint32_t tm, const float* from, long long sj, int dc, bool on) {
 #pragma unroll 1
-  for (int d = 0; d < (dc + 31) / 32 * 32; d += 8) {
+  for (int d = 0; d < (dc + 15) / 16 * 16; d += 8) {
     uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (from && on && d < dc) {
 #pragma unroll
@@ -377,9 +390,9 @@ __device__ __noinline__ void get_state(uint32_t tm, const float* from, long long
 
 // NaN for what a value that is not finite reaches: rows from its token on
 // (row < 0: all of the lanes, the state).
-__device__ __noinline__ void spread_bad(uint32_t tm, const uint32_t* bad, uint32_t it, bool rev, int row, int dc) {
+__device__ __noinline__ void spread_bad(uint32_t tm, const uint32_t* bad, uint32_t it, bool rev, int row, int d0, int d1) {
 #pragma unroll 1
-  for (int d = 0; d < dc; ++d) {
+  for (int d = d0; d < d1; ++d) {
     const int first = first_bad(bad[d], it, rev);
     if (first < 0) continue;
     uint32_t v;
@@ -401,7 +414,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   constexpr bool rev = REV, two = TWO, state_only = STATE;
   const int da = f.da, dc = f.dc, h = blockIdx.y;
   const TcGeom geo = tc_geom(da, dc);
-  unsigned char* s_op = smem + geo.slots * geo.slot_bytes;
+  unsigned char* s_op = smem + (4 + geo.b_slots) * geo.slot_bytes;
   TcTail& t = *reinterpret_cast<TcTail*>(s_op + 2 * geo.s_bytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Ctl ctl{&t, p.err};
@@ -412,19 +425,22 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   }
   if (!state_only) fill_outside<__nv_bfloat16>(p, f);
   if (tid == 0) {
-    for (int i = 0; i < kMaxSlots; ++i) bar_init(&t.full[i], 1), bar_init(&t.empty[i], 5);  // four warps and the products
+    for (int i = 0; i < 6; ++i) {
+      bar_init(&t.full[i], 1);
+      bar_init(&t.empty[i], i < 2 ? (state_only ? 5 : 9) : (i < 4 ? 1 : 5));  // the products, and the row or column warps
+    }
     bar_init(&t.tab_full, 1);
-    bar_init(&t.tab_empty, state_only ? 8 : 12);
+    bar_init(&t.tab_empty, state_only ? 8 : 16);
     bar_init(&t.sc_full, 1);
     bar_init(&t.in_full, 1);
-    bar_init(&t.p_ready, 4);
+    bar_init(&t.p_ready, 8);
     bar_init(&t.kt_ready[0], 4);
     bar_init(&t.kt_ready[1], 4);
     bar_init(&t.u_full[0], 1);
     bar_init(&t.u_full[1], 1);
     bar_init(&t.s_ready, 4);
     bar_init(&t.o_full, 1);
-    bar_init(&t.o_free, 4);
+    bar_init(&t.o_free, 8);
     bar_init(&t.d_full, 1);
     bar_init(&t.drain, 1);
     t.abort = 0;
@@ -434,7 +450,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     fence_async();
   }
   for (int i = tid; i < 2 * kC; i += kTcThreads) t.bad[i / kC][i % kC] = 0;
-  if (warp == 13) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&t.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     fence_before();
@@ -442,18 +458,23 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   __syncthreads();
   fence_after();
   const uint32_t tm = t.tmem;
-  const int nb = (dc + 31) / 32;          // 32-column blocks of the values
+  const int n16 = (dc + 15) / 16;  // 16-column pieces of the values
   const int blocks_a = da > 64 ? 2 : 1, blocks_c = dc > 64 ? 2 : 1;
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's quarter of tensor memory
+  auto slot_at = [&](int x) { return smem + x * geo.slot_bytes; };
+  // without rows B has A's slots
+  auto slot_of_b = [&](uint32_t it) { return state_only ? static_cast<int>(it & 1) : (geo.b_slots == 2 ? 4 + static_cast<int>(it & 1) : 4); };
+  auto phase_of_b = [&](uint32_t it) { return state_only || geo.b_slots == 2 ? (it >> 1) & 1 : it & 1; };
   Walk<REV, STATE> w(p);
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---- row warps ----
-    const int row = warp * 32 + lane;
+    const int quad = warp & 3, side = warp >> 2, row = quad * 32 + lane;
     const uint64_t sp2 = pair(f.sp, f.sp);
     constexpr bool dots = TWO;  // the forms whose rows the gate's gradient needs
     uint32_t dot_loads = 0;
-    int slot = 0, held = -1;  // held: slot that the last rows leave from
+    uint32_t park[8] = {};
+    int held = -1;  // slot that the last rows leave from
     auto release = [&] {
       if (held >= 0 && lane == 0) {
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -461,71 +482,81 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       held = -1;
     };
-    auto take = [&] {
-      const int x = slot;
-      if (++slot == geo.slots) slot = 0;
-      return x;
-    };
     for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
-      take();
-      const int slot_a = take(), slot_c = take();
-      unsigned char* stage = smem + slot_a * geo.slot_bytes;
+      const int slot_a = ph;
+      unsigned char* stage = slot_at(slot_a);
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       const float4 l4 = t.lg[row >> 1];
       const float lx = (row & 1) ? -l4.y : -l4.x, ly = (row & 1) ? -l4.w : -l4.z;
       const uint64_t lx2 = pair(lx, lx), ly2 = pair(ly, ly);
       // backwards lx is minus the sum to the row
       const float rf = (rev ? ex2((t.end.x + lx) + (t.end.y + ly)) : ex2(lx)) * f.sr;
+      release();
       if (!ctl.warp_wait(&t.sc_full, ph)) break;
       fence_after();
       // Blocks of 32 columns wholly inside the mask: the decay is that of the
-      // row to the block's edge times col[], two products an element.
+      // row to the block's edge times col[], two products an element.  (Loop
+      // bodies here and below are kept to sixteen columns: longer ones run
+      // once or twice a chunk and wait for their instructions.)
+      const int cheap0 = 2 * max(2 * side, rev ? quad + 1 : 0), cheap1 = 2 * min(2 * side + 2, rev ? 4 : quad);
 #pragma unroll 1
-      for (int b = rev ? warp + 1 : 0; b < (rev ? 4 : warp); ++b) {
-        const uint32_t col = tm + lanes + kColSc + 32 * b;
-        uint32_t s[32], hi[16];
-        tmem_ld32(col, s);
-        const float4 e4 = t.lg[rev ? 16 * b - 1 : 16 * b + 15];
+      for (int b = cheap0; b < cheap1; ++b) {
+        const uint32_t col = tm + lanes + kColSc + 32 * (b >> 1);
+        uint32_t s[16], hi[8];
+        tmem_ld16(col + 16 * (b & 1), s);
+        const float4 e4 = t.lg[rev ? 16 * (b >> 1) - 1 : 16 * (b >> 1) + 15];
         const float rd = ex2((lx + e4.y) + (ly + e4.w)) * f.sp;
         const uint64_t rd2 = pair(rd, rd);
         wait_ld();
-        const bool tail = rev && 32 * b + 32 > w.len;  // forwards such columns meet no row that counts
-        uint64_t pv[16];
+        uint64_t pv[8];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float2 m = *reinterpret_cast<const float2*>(&t.col[32 * b + 2 * c]);
+        for (int c = 0; c < 8; c += 2) {
+          const float4 m = *reinterpret_cast<const float4*>(&t.col[16 * b + 2 * c]);
           pv[c] = mul2(mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), pair(m.x, m.y)), rd2);
+          pv[c + 1] = mul2(mul2(pair(__uint_as_float(s[2 * c + 2]), __uint_as_float(s[2 * c + 3])), pair(m.z, m.w)), rd2);
         }
-        if (tail) {
+        if (rev && 16 * b + 16 > w.len) {  // forwards such columns meet no row that counts
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
+          for (int c = 0; c < 8; ++c) {
             float p0, p1;
             unpair(pv[c], p0, p1);
-            pv[c] = pair(32 * b + 2 * c < w.len ? p0 : 0.f, 32 * b + 2 * c + 1 < w.len ? p1 : 0.f);
+            pv[c] = pair(16 * b + 2 * c < w.len ? p0 : 0.f, 16 * b + 2 * c + 1 < w.len ? p1 : 0.f);
           }
         }
+        // P's place is the block's own: first terms in its lower half, second
+        // in its upper.  The upper half's scores must be read before, so the
+        // first step of a block parks its terms in registers.
 #pragma unroll
-        for (int c = 0; c < 16; ++c) hi[c] = round2(pv[c]);
-        tmem_st16(col, hi);
+        for (int c = 0; c < 8; ++c) hi[c] = round2(pv[c]);
+        uint32_t lo[8];
         if (two) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) hi[c] = rest2(pv[c], hi[c]);
-          tmem_st16(col + 16, hi);
+          for (int c = 0; c < 8; ++c) lo[c] = rest2(pv[c], hi[c]);
+        }
+        tmem_st8(col + 8 * (b & 1), hi);
+        if (two) {
+          if (b & 1) {
+            tmem_st8(col + 16, park);
+            tmem_st8(col + 24, lo);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) park[c] = lo[c];
+          }
         }
       }
-      {  // the mask's edge: every decay by itself, and select, not multiply
-        const uint32_t col = tm + lanes + kColSc + 32 * warp;
+      if (quad >> 1 == side) {  // the mask's edge: every decay by itself, and select, not multiply
+        const uint32_t col = tm + lanes + kColSc + 32 * quad;
         uint32_t s[32];
         tmem_ld32(col, s);
         wait_ld();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t hi[8], lo[8];
+        for (int part = 0; part < 4; ++part) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const int at = 16 * half + 2 * c, c0 = 32 * warp + at;
-            const float4 m = t.lg[16 * warp + 8 * half + c];
+          for (int c = 0; c < 4; ++c) {
+            const int at = 8 * part + 2 * c, c0 = 32 * quad + at;
+            const float4 m = t.lg[16 * quad + 4 * part + c];
             const uint64_t x = add2(add2(lx2, pair(m.x, m.y)), add2(ly2, pair(m.z, m.w)));
             float x0, x1;
             unpair(x, x0, x1);
@@ -537,19 +568,18 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
             hi[c] = round2(z);
             if (two) lo[c] = rest2(z, hi[c]);
           }
-          tmem_st8(col + 8 * half, hi);
-          if (two) tmem_st8(col + 16 + 8 * half, lo);
+          tmem_st4(col + 4 * part, hi);
+          if (two) tmem_st4(col + 16 + 4 * part, lo);
         }
       }
 #pragma unroll 1
-      for (int b = rev ? 0 : warp + 1; b < (rev ? warp : 4); ++b) {  // outside the mask
+      for (int b = max(2 * side, rev ? 0 : quad + 1); b < min(2 * side + 2, rev ? quad : 4); ++b) {  // outside the mask
         uint32_t none[16];
 #pragma unroll
         for (int c = 0; c < 16; ++c) none[c] = 0u;
         tmem_st16(tm + lanes + kColSc + 32 * b, none);
         if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, none);
       }
-      release();
       if (!ctl.warp_wait(&t.in_full, ph)) break;
       fence_after();
       // The products have read A: its slot holds first the rows to take dots
@@ -562,17 +592,17 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       const uint64_t rf2 = pair(rf, rf);
 #pragma unroll 1
-      for (int b = 0; b < nb; ++b) {
-        uint32_t v[32];
-        tmem_ld32(tm + lanes + kColO + 32 * b, v);
+      for (int b = 4 * side; b < min(4 * side + 4, n16); ++b) {
+        uint32_t v[16];
+        tmem_ld16(tm + lanes + kColO + 16 * b, v);
         wait_ld();
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
+        for (int c = 0; c < 16; c += 2) {
           float x, y;
           unpair(mul2(pair(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), rf2), x, y);
           v[c] = __float_as_uint(x), v[c + 1] = __float_as_uint(y);
         }
-        tmem_st32(tm + lanes + kColO + 32 * b, v);
+        tmem_st16(tm + lanes + kColO + 16 * b, v);
       }
       wait_st();
       fence_before();
@@ -580,24 +610,22 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       if (lane == 0) {
         bar_arrive(&t.p_ready);
         bar_arrive(&t.tab_empty);
-        bar_arrive(&t.empty[slot_c]);
       }
 
       if (dots && !ctl.warp_wait(&t.d_full, ph)) break;
       if (!ctl.warp_wait(&t.o_full, ph)) break;
       fence_after();
-      if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(tm + lanes + kColO, t.bad[ph], it, rev, row, dc);
-      unsigned char* mine = stage + row * 128;
+      if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(tm + lanes + kColO, t.bad[ph], it, rev, row, 64 * side, min(dc, 64 * side + 64));
+      unsigned char* mine = stage + side * 16384 + row * 128;
       uint64_t dot2 = 0;
 #pragma unroll 1
-      for (int b = 0; b < nb; ++b) {
-        uint32_t v[32];
-        tmem_ld32(tm + lanes + kColO + 32 * b, v);
+      for (int b = 4 * side; b < min(4 * side + 4, n16); ++b) {
+        uint32_t v[16];
+        tmem_ld16(tm + lanes + kColO + 16 * b, v);
         wait_ld();
-        unsigned char* at = mine + (b >> 1) * 16384;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint4* piece = reinterpret_cast<uint4*>(at + ((((b & 1) * 4 + q) ^ (row & 7)) << 4));
+        for (int q = 0; q < 2; ++q) {
+          uint4* piece = reinterpret_cast<uint4*>(mine + ((((b & 3) * 2 + q) ^ (row & 7)) << 4));
           uint64_t x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -613,22 +641,24 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         }
       }
       if (f.out_f32) {
-        // 32 columns of float32 fill a row of the stage
+        // 16 columns of float32 fill half a row of the side's stage
 #pragma unroll 1
-        for (int b = 0; b < nb; ++b) {
-          uint32_t v[32];
-          tmem_ld32(tm + lanes + kColO + 32 * b, v);
+        for (int b = 4 * side; b < min(4 * side + 4, n16); ++b) {
+          uint32_t v[16];
+          tmem_ld16(tm + lanes + kColO + 16 * b, v);
           wait_ld();
+          const int half = (b & 1) * 4;
           __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<uint4*>(mine + ((q ^ (row & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(mine + (((half + q) ^ (row & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           __syncwarp();
-          if (32 * b + (lane & 7) * 4 < dc)
-#pragma unroll 1
-            for (int r = warp * 32 + (lane >> 3); r < min(warp * 32 + 32, w.len); r += 4)
-              *reinterpret_cast<uint4*>(static_cast<float*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 32 * b + (lane & 7) * 4) =
-                  *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          const int q = lane & 3, r0 = quad * 32 + (lane >> 2);
+          if (16 * b + q * 4 < dc)
+#pragma unroll 2
+            for (int r = r0; r < min(quad * 32 + 32, w.len); r += 8)
+              *reinterpret_cast<uint4*>(static_cast<float*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 16 * b + q * 4) =
+                  *reinterpret_cast<const uint4*>(stage + side * 16384 + r * 128 + (((half + q) ^ (r & 7)) << 4));
         }
       }
       fence_before();
@@ -638,32 +668,30 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       // waits for one chunk later, those at a piece's end by the lanes.
       fence_async();
       __syncwarp();
-      if (!f.out_f32) {
-        if (warp * 32 + 32 <= w.len) {
-          if (lane == 0) {
-            for (int b = 0; b < blocks_c; ++b)
-              asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(&map[4]),
-                           "r"(b * 64), "r"(h), "r"(static_cast<int>(w.s0) + warp * 32),
-                           "r"(smem_u32(stage + b * 16384 + warp * 4096))
-                           : "memory");
-          }
+      if (!f.out_f32 && side < blocks_c) {
+        if (quad * 32 + 32 <= w.len) {
+          if (lane == 0)
+            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(&map[4]),
+                         "r"(side * 64), "r"(h), "r"(static_cast<int>(w.s0) + quad * 32),
+                         "r"(smem_u32(stage + side * 16384 + quad * 4096))
+                         : "memory");
         } else {
 #pragma unroll 1
-          for (int e = lane; e < 32 * 16; e += 32) {
-            const int r = warp * 32 + (e >> 4), q = e & 15;
-            if (r < w.len && 8 * q < dc)
-              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 8 * q) =
-                  *reinterpret_cast<const uint4*>(stage + (q >> 3) * 16384 + r * 128 + (((q & 7) ^ (r & 7)) << 4));
+          for (int e = lane; e < 32 * 8; e += 32) {
+            const int r = quad * 32 + (e >> 3), q = e & 7;
+            if (r < w.len && 64 * side + 8 * q < dc)
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 64 * side + 8 * q) =
+                  *reinterpret_cast<const uint4*>(stage + side * 16384 + r * 128 + ((q ^ (r & 7)) << 4));
           }
           __syncwarp();
         }
       }
       if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       held = slot_a;
-      if (dots && row < w.len) {
+      if (dots && row < w.len && side < blocks_c) {
         float x, y;
         unpair(dot2, x, y);
-        f.rowdot[h * p.BL + w.s0 + row] = x + y;
+        f.rowdot[(static_cast<long long>(side) * p.H + h) * p.BL + w.s0 + row] = x + y;
       }
     }
     if (!state_only && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -672,11 +700,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       while (!bar_try(&t.d_full, (dot_loads - 1) & 1) && now_ns() - start < kStageTimeoutNs) {
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < 12) {
     // ---- state warps ----
-    const int i = tid - 128;
+    const int i = tid - 256;
     const int rows = (da + 15) / 16 * 16;  // the product with S runs over whole sixteens
-    const bool work = (warp - 4) * 32 < rows;
+    const bool work = (warp - 8) * 32 < rows;
     const long long mat = static_cast<long long>(da) * dc;
     float decay = 1.f;
     for (uint32_t it = 0; w.next(); ++it) {
@@ -702,7 +730,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         }
         if (work) get_state(ut, from, sj, dc, i < da);
       } else if (work && t.bad_chunk[ph ^ 1] == static_cast<int>(it)) {
-        spread_bad(ut, t.bad[ph ^ 1], it - 1, rev, -1, dc);
+        spread_bad(ut, t.bad[ph ^ 1], it - 1, rev, -1, 0, dc);
       }
       if (f.snap && !state_only && work) {
         const long long edge = rev ? w.s0 + w.len : w.s0;
@@ -712,15 +740,15 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const uint64_t total2 = pair(total, total);
       if (work) {
 #pragma unroll 1
-        for (int b = 0; b < nb; ++b) {
-          float v[32];
-          tmem_ld32(ut + 32 * b, reinterpret_cast<uint32_t*>(v));
+        for (int b = 0; b < n16; ++b) {
+          float v[16];
+          tmem_ld16(ut + 16 * b, reinterpret_cast<uint32_t*>(v));
           wait_ld();
           if (!state_only && i < rows) {
-            // S: row i of 64 columns is 128 bytes; four 16-byte pieces per 32 columns
-            unsigned char* base = s_op + (b >> 1) * (geo.s_bytes / blocks_c) + i * 128;
+            // S: row i of 64 columns is 128 bytes; two 16-byte pieces per 16 columns
+            unsigned char* base = s_op + (b >> 2) * (geo.s_bytes / blocks_c) + i * 128;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
               uint32_t hi[4], lo[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -728,14 +756,14 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
                 hi[e] = round2(x);
                 lo[e] = rest2(x, hi[e]);
               }
-              const int at = (((b & 1) * 4 + q) ^ (i & 7)) * 16;
+              const int at = (((b & 3) * 2 + q) ^ (i & 7)) * 16;
               *reinterpret_cast<uint4*>(base + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
               if (two) *reinterpret_cast<uint4*>(base + geo.s_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
           }
 #pragma unroll
-          for (int q = 0; q < 32; q += 2) unpair(mul2(pair(v[q], v[q + 1]), total2), v[q], v[q + 1]);
-          tmem_st32(ut + 32 * b, reinterpret_cast<const uint32_t*>(v));
+          for (int q = 0; q < 16; q += 2) unpair(mul2(pair(v[q], v[q + 1]), total2), v[q], v[q + 1]);
+          tmem_st16(ut + 16 * b, reinterpret_cast<const uint32_t*>(v));
         }
         wait_st();
       }
@@ -749,34 +777,25 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         float* to = state_only ? f.carry + (static_cast<long long>(blockIdx.x) * p.H + h) * mat + static_cast<long long>(i) * dc
                                : f.fin + (w.x.n * p.H + h) * mat + i * f.si;
         if (work) {
-          if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(ut, t.bad[ph], it, rev, -1, dc);
+          if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(ut, t.bad[ph], it, rev, -1, 0, dc);
           put_state(ut, to, state_only ? 1 : f.sj, dc, i < da);
         }
         // a piece that holds the sequence's start takes nothing from before
         if (state_only && i == 0) f.dec[blockIdx.x * p.H + h] = w.x.from_start ? -1.f : decay;
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // ---- column warps ----
-    const int i = tid - 256;
+    const int i = tid - 384;
     const bool work = i < blocks_a * 64;
     // The warp's 32 rows of (col.B)^T: matrix m of a load has rows 8 m.. and 8
     // tokens; lane r of it points at token r's 16 bytes.
     const int lead = (i >> 6) * 16384 + (lane & 7) * 128 + ((((i & 32) >> 3) + (lane >> 3) ^ (lane & 7)) << 4);
-    const int per = state_only ? 2 : 3;
-    int slot = 0, round = 0;  // of the next tile
     for (uint32_t it = 0; w.next(); ++it) {
       const uint32_t ph = it & 1;
-      const int slot_b = slot;
-      const unsigned char* bt = smem + slot * geo.slot_bytes;
-      const uint32_t bph = round & 1;
-      for (int k = 1; k < per; ++k)
-        if (++slot == geo.slots) slot = 0, ++round;
-      const int slot_c = slot;
-      unsigned char* ct = smem + slot * geo.slot_bytes;
-      const uint32_t cph = round & 1;
-      if (++slot == geo.slots) slot = 0, ++round;
-
+      const int slot_b = slot_of_b(it), slot_c = 2 + ph;
+      const unsigned char* bt = slot_at(slot_b);
+      unsigned char* ct = slot_at(slot_c);
       // An update is done: its operand may be overwritten.  The previous one's,
       // when outputs are computed, which also shows that the row and state
       // warps have read what bad[ph] held two chunks ago; else the one before,
@@ -788,7 +807,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       const uint32_t kt = tm + lanes + (state_only && ph ? kColSc : kColK);
       if (!state_only || w.len < kC)
-        if (!ctl.warp_wait(&t.full[slot_c], cph)) break;
+        if (!ctl.warp_wait(&t.full[slot_c], (it >> 1) & 1)) break;
       if (state_only) {
         if (i >= w.len)  // another sequence's token, or past the end
           for (int q = 0; q < 8 * blocks_c; ++q) *reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + ((q & 7) << 4)) = make_uint4(0, 0, 0, 0);
@@ -796,21 +815,17 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         const bool live = i < w.len;
         const __nv_bfloat162 none = __float2bfloat162_rn(0.f);
         __nv_bfloat162 sum = none;  // sum of 0 * x: NaN if any x is not finite
-#pragma unroll 1
-        for (int b = 0; b < blocks_c; ++b) {
-          unsigned char* at = ct + b * 16384 + i * 128;
+#pragma unroll 2
+        for (int q = 0; q < 8 * blocks_c; ++q) {
+          uint4* at = reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + (((q & 7) ^ (i & 7)) << 4));
           if (live) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const uint4 x = *reinterpret_cast<const uint4*>(at + ((q ^ (i & 7)) << 4));
-              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), none, sum);
-              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), none, sum);
-              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), none, sum);
-              sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), none, sum);
-            }
-          } else {  // another sequence's token, or past the end
-#pragma unroll
-            for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(at + ((q ^ (i & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            const uint4 x = *at;
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), none, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), none, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), none, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), none, sum);
+          } else {
+            *at = make_uint4(0, 0, 0, 0);  // another sequence's token, or past the end
           }
         }
         const bool bad = !(__low2float(sum) == 0.f && __high2float(sum) == 0.f);
@@ -827,7 +842,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       fence_async();
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
-      if (!ctl.warp_wait(&t.full[slot_b], bph)) break;
+      if (!ctl.warp_wait(&t.full[slot_b], phase_of_b(it))) break;
       if (work) {
         const uint32_t src = smem_u32(bt) + lead;
         const bool tail = w.len < kC;
@@ -874,113 +889,120 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         bar_arrive(&t.kt_ready[ph]);
         bar_arrive(&t.tab_empty);
         bar_arrive(&t.empty[slot_b]);
-        if (state_only) bar_arrive(&t.empty[slot_c]);
       }
     }
-  } else if (warp == 12) {
-    // ---- loads ----
+  } else if (warp == 16) {
+    // ---- loads: what comes free first is asked for first ----
     if (lane == 0) {
-      uint32_t tile = 0;
+      uint32_t count = 0;  // chunks
       bool ok = true;
-      auto load = [&](int which, int blocks, const Rows& r) {
-        const int slot = tile % geo.slots;
-        if (tile >= static_cast<uint32_t>(geo.slots) && !ctl.wait(&t.empty[slot], (tile / geo.slots - 1) & 1)) return false;
+      auto load = [&](int slot, uint32_t use, int which, int blocks, const Rows& r) {
+        if (use > 0 && !ctl.wait(&t.empty[slot], (use - 1) & 1)) return false;
         bar_expect(&t.full[slot], blocks * 16384);
+#pragma unroll 1
         for (int b = 0; b < blocks; ++b)
-          tma_rows(smem_u32(smem + slot * geo.slot_bytes + b * 16384), &map[which], b * 64, h / r.share,
-                   static_cast<int>(w.s0), &t.full[slot]);
-        ++tile;
+          tma_rows(smem_u32(slot_at(slot) + b * 16384), &map[which], b * 64, h / r.share, static_cast<int>(w.s0), &t.full[slot]);
         return true;
       };
+      uint32_t a_loads = 0, b_loads = 0, c_loads = 0;
       while (ok && w.next()) {
-        ok = load(1, blocks_a, f.b);
-        if (ok && !state_only) ok = load(0, blocks_a, f.a);
-        if (ok) ok = load(2, blocks_c, f.c);
+        ok = load(2 + (count & 1), count >> 1, 2, blocks_c, f.c);
+        c_loads += ok;
+        if (ok) {
+          ok = load(slot_of_b(count), state_only || geo.b_slots == 2 ? count >> 1 : count, 1, blocks_a, f.b);
+          b_loads += ok;
+        }
+        if (ok && !state_only) {
+          ok = load(count & 1, count >> 1, 0, blocks_a, f.a);
+          a_loads += ok;
+        }
+        ++count;
       }
       // a load in flight must land before the CTA leaves (only after a give-up)
-      const uint32_t from = tile > static_cast<uint32_t>(geo.slots) ? tile - geo.slots : 0;
-      for (uint32_t k = from; k < tile; ++k) {
+      auto land = [&](int slot, uint32_t uses) {
         const unsigned long long start = now_ns();
-        while (!bar_try(&t.full[k % geo.slots], (k / geo.slots) & 1) && now_ns() - start < kStageTimeoutNs) {
+        while (uses > 0 && !bar_try(&t.full[slot], (uses - 1) & 1) && now_ns() - start < kStageTimeoutNs) {
         }
+      };
+      for (int x = 0; x < 2; ++x) {
+        land(x, ((state_only ? b_loads : a_loads) + 1 - x) >> 1);
+        land(2 + x, (c_loads + 1 - x) >> 1);
+        if (state_only) continue;
+        if (geo.b_slots == 2) land(4 + x, (b_loads + 1 - x) >> 1);
+        else if (x == 0) land(4, b_loads);
       }
     }
-  } else if (warp == 13) {
+  } else if (warp == 17) {
     // ---- products ----
-    if (lane == 0) {
-      const uint32_t id_sc = idesc(kC, false), id_v = idesc((dc + 15) / 16 * 16, true);
-      const int ka = (da + 15) / 16;
-      const uint64_t ds = desc(smem_u32(s_op), geo.s_bytes / blocks_c);
-      int slot = 0;
-      uint32_t round = 0;
-      auto take = [&] {
-        const int x = slot;
-        if (++slot == geo.slots) slot = 0, ++round;
-        return x;
-      };
-      auto rows_desc = [&](int x, uint32_t lbo) { return desc(smem_u32(smem) + x * geo.slot_bytes, lbo); };
-      for (uint32_t it = 0; w.next(); ++it) {
-        const uint32_t ph = it & 1;
-        uint32_t r = round;
-        const int sb = take();
-        if (!ctl.wait(&t.full[sb], r & 1)) break;
-        int sa = 0;
-        if (!state_only) {
-          r = round;
-          sa = take();
-          if (!ctl.wait(&t.full[sa], r & 1)) break;
-          // the scores go where the previous chunk's P lies until its product is done
-          if (it > 0 && !ctl.wait(&t.o_full, ph ^ 1)) break;
-          fence_after();
-          const uint64_t a = rows_desc(sa, 16), b = rows_desc(sb, 16);
-#pragma unroll 4
+    const uint32_t id_sc = idesc(kC, false), id_v = idesc((dc + 15) / 16 * 16, true);
+    const int ka = (da + 15) / 16;
+    const uint64_t ds = desc(smem_u32(s_op), geo.s_bytes / blocks_c);
+    for (uint32_t it = 0; w.next(); ++it) {
+      const uint32_t ph = it & 1;
+      const int sa = ph, sb = slot_of_b(it), sc = 2 + ph;
+      if (!ctl.warp_wait(&t.full[sb], phase_of_b(it))) break;
+      if (!state_only) {
+        if (!ctl.warp_wait(&t.full[sa], (it >> 1) & 1)) break;
+        // the scores go where the previous chunk's P lies until its product is done
+        if (it > 0 && !ctl.warp_wait(&t.o_full, ph ^ 1)) break;
+        fence_after();
+        const uint64_t a = desc(smem_u32(slot_at(sa)), 16), b = desc(smem_u32(slot_at(sb)), 16);
+        if (elect_one()) {
+#pragma unroll 1
           for (int k = 0; k < ka; ++k) {
             const uint32_t o = (k >> 2) * 1024 + (k & 3) * 2;  // in 16 bytes: the next 64 columns, 16 of them
             mma_smem(tm + kColSc, a + o, b + o, id_sc, k > 0);
           }
           commit(&t.sc_full);
           commit(&t.empty[sb]);
-          if (!ctl.wait(&t.s_ready, ph)) break;
-          if (it > 0 && !ctl.wait(&t.o_free, ph ^ 1)) break;
-          fence_after();
+        }
+        if (!ctl.warp_wait(&t.s_ready, ph)) break;
+        if (it > 0 && !ctl.warp_wait(&t.o_free, ph ^ 1)) break;
+        fence_after();
+        if (elect_one()) {
 #pragma unroll 1
           for (int term = 0; term < (two ? 2 : 1); ++term)
-#pragma unroll 4
+#pragma unroll 1
             for (int k = 0; k < ka; ++k)
               mma_smem(tm + kColO, a + (k >> 2) * 1024 + (k & 3) * 2, ds + term * (geo.s_bytes >> 4) + k * 128, id_v, term + k > 0);
           commit(&t.in_full);
           commit(&t.empty[sa]);
-        } else if (!ctl.wait(&t.s_ready, ph)) {
-          break;
         }
-        r = round;
-        const int sc = take();
-        if (!ctl.wait(&t.kt_ready[ph], (it >> 1) & 1)) break;
-        if (!ctl.wait(&t.full[sc], r & 1)) break;
-        fence_after();
-        const uint64_t c = rows_desc(sc, 16384);
-        const uint32_t kt = tm + (state_only && ph ? kColSc : kColK);
-#pragma unroll 4
+      } else if (!ctl.warp_wait(&t.s_ready, ph)) {
+        break;
+      }
+      if (!ctl.warp_wait(&t.kt_ready[ph], (it >> 1) & 1)) break;
+      if (!ctl.warp_wait(&t.full[sc], (it >> 1) & 1)) break;
+      fence_after();
+      const uint64_t c = desc(smem_u32(slot_at(sc)), 16384);
+      const uint32_t kt = tm + (state_only && ph ? kColSc : kColK);
+      if (elect_one()) {
+#pragma unroll 1
         for (int k = 0; k < 2 * kC / 16; ++k)  // both terms lie side by side
           mma_tmem(tm + kColU, kt + k * 8, c + (k & 7) * 128, id_v, true);
         commit(&t.u_full[ph]);
-        if (state_only) commit(&t.empty[sb]);
-        if (!state_only) {
-          if (!ctl.wait(&t.p_ready, ph)) break;
-          fence_after();
+        if (state_only) {
+          commit(&t.empty[sb]);
+          commit(&t.empty[sc]);
+        }
+      }
+      if (!state_only) {
+        if (!ctl.warp_wait(&t.p_ready, ph)) break;
+        fence_after();
+        if (elect_one()) {
 #pragma unroll 1
           for (int term = 0; term < (two ? 2 : 1); ++term)
-#pragma unroll 4
+#pragma unroll 1
             for (int k = 0; k < kC / 16; ++k)
               mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, c + k * 128, id_v, true);
           commit(&t.o_full);
+          commit(&t.empty[sc]);
         }
-        commit(&t.empty[sc]);
       }
-      commit(&t.drain);  // nothing of this CTA's is in flight after it
-      const unsigned long long start = now_ns();
-      while (!bar_try(&t.drain, 0) && now_ns() - start < kStageTimeoutNs) {
-      }
+    }
+    if (elect_one()) commit(&t.drain);  // nothing of this CTA's is in flight after it
+    const unsigned long long start = now_ns();
+    while (!bar_try(&t.drain, 0) && now_ns() - start < kStageTimeoutNs) {
     }
   } else {
     // ---- gates: four tokens a lane ----
@@ -1044,7 +1066,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 17) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
   }
@@ -1088,6 +1110,8 @@ static bool rows_usable(const Rows& r, int dim, int H) {
   return H / r.share == 1 || (r.sh % 8 == 0 && r.sh >= dim && r.sh < (1ll << 38));
 }
 
+int tc_dot_parts(const Form& f) { return f.dc > 64 ? 2 : 1; }
+
 bool tc_usable(const Launch& l, int roles, int dtype) {
   if (dtype != ASCAN_BF16 || l.p.BL > 0x7fffff00ll) return false;
   for (int r = 0; r < roles; ++r) {
@@ -1112,7 +1136,7 @@ int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
         (!f.out_f32 && !map_rows(&maps.m[r][4], Rows{f.out, static_cast<long long>(l.p.H) * f.dc, f.dc, 1}, f.dc, l.p.BL, l.p.H, 32)))
       return ASCAN_EINVAL;
     const TcGeom g = tc_geom(f.da, f.dc);
-    const size_t need = static_cast<size_t>(g.slots) * g.slot_bytes + 2 * g.s_bytes + sizeof(TcTail);
+    const size_t need = g.bytes() + sizeof(TcTail);
     if (need > smem) smem = need;
   }
   static std::once_flag once;
