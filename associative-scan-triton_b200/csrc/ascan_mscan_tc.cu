@@ -184,11 +184,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), TC_I8(r, 0)
                : "memory");
 }
-__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3])
-               : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -242,6 +237,9 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 __device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// The n lowest of 32 bits (none below 0, all above 31).
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
 // The pair as packed bfloat16, and what that leaves over as another.
 __device__ __forceinline__ uint32_t round2(uint64_t x) {
@@ -492,47 +490,63 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const uint64_t lx2 = pair(lx, lx), ly2 = pair(ly, ly);
       // backwards lx is minus the sum to the row
       const float rf = (rev ? ex2((t.end.x + lx) + (t.end.y + ly)) : ex2(lx)) * f.sr;
-      release();
       if (!ctl.warp_wait(&t.sc_full, ph)) break;
       fence_after();
-      // Blocks of 32 columns wholly inside the mask: the decay is that of the
-      // row to the block's edge times col[], two products an element.  (Loop
-      // bodies here and below are kept to sixteen columns: longer ones run
-      // once or twice a chunk and wait for their instructions.)
-      const int cheap0 = 2 * max(2 * side, rev ? quad + 1 : 0), cheap1 = 2 * min(2 * side + 2, rev ? 4 : quad);
+      // Sixteen columns at a time, those that the mask leaves something of.
+      // Where a block of 32 lies wholly inside, the decay is that of the row
+      // to the block's edge times col[], two products an element; in the
+      // row's own block every decay is computed by itself, and masked scores
+      // are cleared as bits (a product with zero would keep a NaN).  (Longer loop bodies would run once or
+      // twice a chunk and wait for their instructions.)
+      const int b0 = 2 * max(2 * side, rev ? quad : 0), b1 = 2 * min(2 * side + 2, rev ? 4 : quad + 1);
 #pragma unroll 1
-      for (int b = cheap0; b < cheap1; ++b) {
+      for (int b = b0; b < b1; ++b) {
         const uint32_t col = tm + lanes + kColSc + 32 * (b >> 1);
         uint32_t s[16], hi[8];
         tmem_ld16(col + 16 * (b & 1), s);
-        const float4 e4 = t.lg[rev ? 16 * (b >> 1) - 1 : 16 * (b >> 1) + 15];
-        const float rd = ex2((lx + e4.y) + (ly + e4.w)) * f.sp;
-        const uint64_t rd2 = pair(rd, rd);
-        wait_ld();
         uint64_t pv[8];
+        if (b >> 1 != quad) {
+          const float4 e4 = t.lg[rev ? 16 * (b >> 1) - 1 : 16 * (b >> 1) + 15];
+          const float rd = ex2((lx + e4.y) + (ly + e4.w)) * f.sp;
+          const uint64_t rd2 = pair(rd, rd);
 #pragma unroll
-        for (int c = 0; c < 8; c += 2) {
-          const float4 m = *reinterpret_cast<const float4*>(&t.col[16 * b + 2 * c]);
-          pv[c] = mul2(mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), pair(m.x, m.y)), rd2);
-          pv[c + 1] = mul2(mul2(pair(__uint_as_float(s[2 * c + 2]), __uint_as_float(s[2 * c + 3])), pair(m.z, m.w)), rd2);
-        }
-        if (rev && 16 * b + 16 > w.len) {  // forwards such columns meet no row that counts
+          for (int c = 0; c < 8; c += 2) {
+            const float4 m = *reinterpret_cast<const float4*>(&t.col[16 * b + 2 * c]);
+            pv[c] = mul2(pair(m.x, m.y), rd2);
+            pv[c + 1] = mul2(pair(m.z, m.w), rd2);
+          }
+        } else {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            float p0, p1;
-            unpair(pv[c], p0, p1);
-            pv[c] = pair(16 * b + 2 * c < w.len ? p0 : 0.f, 16 * b + 2 * c + 1 < w.len ? p1 : 0.f);
+            const float4 m = t.lg[8 * b + c];
+            float x0, x1;
+            unpair(add2(add2(lx2, pair(m.x, m.y)), add2(ly2, pair(m.z, m.w))), x0, x1);
+            pv[c] = mul2(sp2, pair(ex2(x0), ex2(x1)));
           }
         }
+        wait_ld();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) pv[c] = mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), pv[c]);
         // P's place is the block's own: first terms in its lower half, second
         // in its upper.  The upper half's scores must be read before, so the
-        // first step of a block parks its terms in registers.
+        // first step of a block parks its second terms in registers.
 #pragma unroll
         for (int c = 0; c < 8; ++c) hi[c] = round2(pv[c]);
         uint32_t lo[8];
         if (two) {
 #pragma unroll
           for (int c = 0; c < 8; ++c) lo[c] = rest2(pv[c], hi[c]);
+        }
+        if (b >> 1 == quad || (rev && 16 * b + 16 > w.len)) {
+          // the columns that count, as the bits of the packed pairs
+          const int from = (rev ? row : 0) - 16 * b, to = (rev ? w.len : row + 1) - 16 * b;
+          const uint32_t keep = below(to) & ~below(from);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t bits = (keep & (1u << (2 * c)) ? 0xffffu : 0u) | (keep & (2u << (2 * c)) ? 0xffff0000u : 0u);
+            hi[c] &= bits;
+            if (two) lo[c] &= bits;
+          }
         }
         tmem_st8(col + 8 * (b & 1), hi);
         if (two) {
@@ -545,33 +559,6 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           }
         }
       }
-      if (quad >> 1 == side) {  // the mask's edge: every decay by itself, and select, not multiply
-        const uint32_t col = tm + lanes + kColSc + 32 * quad;
-        uint32_t s[32];
-        tmem_ld32(col, s);
-        wait_ld();
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int at = 8 * part + 2 * c, c0 = 32 * quad + at;
-            const float4 m = t.lg[16 * quad + 4 * part + c];
-            const uint64_t x = add2(add2(lx2, pair(m.x, m.y)), add2(ly2, pair(m.z, m.w)));
-            float x0, x1;
-            unpair(x, x0, x1);
-            const uint64_t y = mul2(mul2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), sp2), pair(ex2(x0), ex2(x1)));
-            unpair(y, x0, x1);
-            x0 = (rev ? c0 >= row && c0 < w.len : c0 <= row) ? x0 : 0.f;
-            x1 = (rev ? c0 + 1 >= row && c0 + 1 < w.len : c0 + 1 <= row) ? x1 : 0.f;
-            const uint64_t z = pair(x0, x1);
-            hi[c] = round2(z);
-            if (two) lo[c] = rest2(z, hi[c]);
-          }
-          tmem_st4(col + 4 * part, hi);
-          if (two) tmem_st4(col + 16 + 4 * part, lo);
-        }
-      }
 #pragma unroll 1
       for (int b = max(2 * side, rev ? 0 : quad + 1); b < min(2 * side + 2, rev ? quad : 4); ++b) {  // outside the mask
         uint32_t none[16];
@@ -580,6 +567,9 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         tmem_st16(tm + lanes + kColSc + 32 * b, none);
         if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, none);
       }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.tab_empty);
+      release();
       if (!ctl.warp_wait(&t.in_full, ph)) break;
       fence_after();
       // The products have read A: its slot holds first the rows to take dots
@@ -607,10 +597,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) {
-        bar_arrive(&t.p_ready);
-        bar_arrive(&t.tab_empty);
-      }
+      if (lane == 0) bar_arrive(&t.p_ready);
 
       if (dots && !ctl.warp_wait(&t.d_full, ph)) break;
       if (!ctl.warp_wait(&t.o_full, ph)) break;
@@ -713,6 +700,8 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       if (first) decay = 1.f;
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       const float total = t.total;
+      __syncwarp();
+      if (lane == 0) bar_arrive(&t.tab_empty);
       decay *= total;
       if (it > 0) {  // the update before this chunk; it also follows the last use of S
         if (!ctl.warp_wait(&t.u_full[ph ^ 1], ((it - 1) >> 1) & 1)) break;
@@ -770,7 +759,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       fence_async();
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(&t.s_ready), bar_arrive(&t.tab_empty);
+      if (lane == 0) bar_arrive(&t.s_ready);
       if (w.last() && (state_only || (w.x.to_end && f.fin))) {
         if (!ctl.warp_wait(&t.u_full[ph], (it >> 1) & 1)) break;
         fence_after();
