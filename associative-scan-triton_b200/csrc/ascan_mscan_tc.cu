@@ -469,6 +469,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     // ---- row warps ----
     const int quad = warp & 3, side = warp >> 2, row = quad * 32 + lane;
     const uint64_t sp2 = pair(f.sp, f.sp);
+    // The side's columns: half of the whole.  At 64 columns and fewer the two
+    // sides share a stage block, each a half of its rows.
+    const bool wide = dc > 64;
+    const int c16 = side * (wide ? 4 : 2), c16_end = min(c16 + (wide ? 4 : 2), n16);
+    const int block = wide ? side : 0;
     constexpr bool dots = TWO;  // the forms whose rows the gate's gradient needs
     uint32_t dot_loads = 0;
     uint32_t park[8] = {};
@@ -582,7 +587,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       const uint64_t rf2 = pair(rf, rf);
 #pragma unroll 1
-      for (int b = 4 * side; b < min(4 * side + 4, n16); ++b) {
+      for (int b = c16; b < c16_end; ++b) {
         uint32_t v[16];
         tmem_ld16(tm + lanes + kColO + 16 * b, v);
         wait_ld();
@@ -602,11 +607,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       if (dots && !ctl.warp_wait(&t.d_full, ph)) break;
       if (!ctl.warp_wait(&t.o_full, ph)) break;
       fence_after();
-      if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(tm + lanes + kColO, t.bad[ph], it, rev, row, 64 * side, min(dc, 64 * side + 64));
-      unsigned char* mine = stage + side * 16384 + row * 128;
+      if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(tm + lanes + kColO, t.bad[ph], it, rev, row, 16 * c16, min(dc, 16 * c16_end));
+      unsigned char* mine = stage + block * 16384 + row * 128;
       uint64_t dot2 = 0;
 #pragma unroll 1
-      for (int b = 4 * side; b < min(4 * side + 4, n16); ++b) {
+      for (int b = c16; b < c16_end; ++b) {
         uint32_t v[16];
         tmem_ld16(tm + lanes + kColO + 16 * b, v);
         wait_ld();
@@ -628,24 +633,23 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         }
       }
       if (f.out_f32) {
-        // 16 columns of float32 fill half a row of the side's stage
+        // 16 columns of float32 fill half a row of the stage
 #pragma unroll 1
-        for (int b = 4 * side; b < min(4 * side + 4, n16); ++b) {
+        for (int b = c16; b < c16_end; ++b) {
           uint32_t v[16];
           tmem_ld16(tm + lanes + kColO + 16 * b, v);
           wait_ld();
-          const int half = (b & 1) * 4;
+          const int half = (wide ? b & 1 : side) * 4, q = lane & 3, r0 = quad * 32 + (lane >> 2);
           __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(mine + (((half + q) ^ (row & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(mine + (((half + c) ^ (row & 7)) << 4)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
           __syncwarp();
-          const int q = lane & 3, r0 = quad * 32 + (lane >> 2);
           if (16 * b + q * 4 < dc)
 #pragma unroll 2
             for (int r = r0; r < min(quad * 32 + 32, w.len); r += 8)
               *reinterpret_cast<uint4*>(static_cast<float*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 16 * b + q * 4) =
-                  *reinterpret_cast<const uint4*>(stage + side * 16384 + r * 128 + (((half + q) ^ (r & 7)) << 4));
+                  *reinterpret_cast<const uint4*>(stage + block * 16384 + r * 128 + (((half + q) ^ (r & 7)) << 4));
         }
       }
       fence_before();
@@ -655,27 +659,26 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       // waits for one chunk later, those at a piece's end by the lanes.
       fence_async();
       __syncwarp();
-      if (!f.out_f32 && side < blocks_c) {
-        if (quad * 32 + 32 <= w.len) {
+      if (!f.out_f32) {
+        if (wide && quad * 32 + 32 <= w.len) {
           if (lane == 0)
             asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(&map[4]),
                          "r"(side * 64), "r"(h), "r"(static_cast<int>(w.s0) + quad * 32),
                          "r"(smem_u32(stage + side * 16384 + quad * 4096))
                          : "memory");
         } else {
+          const int bits = wide ? 3 : 2, q = (lane & ((1 << bits) - 1)) + (wide ? 0 : side * 4);
 #pragma unroll 1
-          for (int e = lane; e < 32 * 8; e += 32) {
-            const int r = quad * 32 + (e >> 3), q = e & 7;
-            if (r < w.len && 64 * side + 8 * q < dc)
-              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 64 * side + 8 * q) =
-                  *reinterpret_cast<const uint4*>(stage + side * 16384 + r * 128 + ((q ^ (r & 7)) << 4));
-          }
+          for (int r = quad * 32 + (lane >> bits); r < min(quad * 32 + 32, w.len); r += 32 >> bits)
+            if (64 * block + 8 * q < dc)
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(f.out) + ((w.s0 + r) * p.H + h) * dc + 64 * block + 8 * q) =
+                  *reinterpret_cast<const uint4*>(stage + block * 16384 + r * 128 + ((q ^ (r & 7)) << 4));
           __syncwarp();
         }
       }
       if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       held = slot_a;
-      if (dots && row < w.len && side < blocks_c) {
+      if (dots && row < w.len && c16 < c16_end) {
         float x, y;
         unpair(dot2, x, y);
         f.rowdot[(static_cast<long long>(side) * p.H + h) * p.BL + w.s0 + row] = x + y;
@@ -1099,7 +1102,7 @@ static bool rows_usable(const Rows& r, int dim, int H) {
   return H / r.share == 1 || (r.sh % 8 == 0 && r.sh >= dim && r.sh < (1ll << 38));
 }
 
-int tc_dot_parts(const Form& f) { return f.dc > 64 ? 2 : 1; }
+int tc_dot_parts(const Form& f) { return f.dc > 32 ? 2 : 1; }
 
 bool tc_usable(const Launch& l, int roles, int dtype) {
   if (dtype != ASCAN_BF16 || l.p.BL > 0x7fffff00ll) return false;
