@@ -1117,6 +1117,11 @@ bool tc_usable(const Launch& l, int roles, int dtype) {
 }
 
 int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
+  // Tensor maps are made through the driver, which wants a current context;
+  // a thread whose first CUDA call this is (autograd's, with every buffer out
+  // of torch's cache) has none until the runtime is told its device.
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return ASCAN_EDEVICE;
   TcMaps maps;
   memset(&maps, 0, sizeof(maps));
   size_t smem = 0;
@@ -1126,7 +1131,7 @@ int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
         !map_rows(&maps.m[r][2], f.c, f.dc, l.p.BL, l.p.H) ||
         (f.rowdot && !map_rows(&maps.m[r][3], f.dot, f.dc, l.p.BL, l.p.H)) ||
         (!f.out_f32 && !map_rows(&maps.m[r][4], Rows{f.out, static_cast<long long>(l.p.H) * f.dc, f.dc, 1}, f.dc, l.p.BL, l.p.H, 32)))
-      return ASCAN_EINVAL;
+      return ASCAN_ECUDA;
     const TcGeom g = tc_geom(f.da, f.dc);
     const size_t need = g.bytes() + sizeof(TcTail);
     if (need > smem) smem = need;

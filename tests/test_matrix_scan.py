@@ -353,6 +353,42 @@ def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("backward", [False, True])
+def test_a_thread_without_a_cuda_context(backward):
+  # a new thread whose first CUDA work is this call, every buffer coming from
+  # torch's cache: nothing has made a context current in it yet
+  import threading
+
+  from associative_scan_triton import matrix_scan
+  q, k, v, g, _, d_out, _ = (x if x is None else x.to(DEV)
+                             for x in make([70], (2, 2, 2, 2), (64, 64), BF16))
+  cu = cu_of([70])
+
+  def call():
+    if backward:
+      return matrix_scan._scan_backward(q, k, v, g, cu, 0.125, None, None, d_out, None)[:4]
+    return matrix_scan._scan_forward(q, k, v, g, cu, 0.125, None, True)
+
+  want = call()
+  found = []
+  for x in want:  # leaves free blocks of every size that the call needs
+    found.append(x.clone())
+  want, found = found, []
+  torch.cuda.synchronize()
+  sync_check = _lib.sync_check_enabled()
+  _lib.set_sync_check(False)
+  try:
+    thread = threading.Thread(target=lambda: found.append(call()))
+    thread.start()
+    thread.join()
+  finally:
+    _lib.set_sync_check(sync_check)
+  assert found, "the call failed in the new thread"
+  for a, b in zip(found[0], want):
+    assert torch.equal(a, b)
+
+
+@gpu
 def test_empty_inputs():
   q = torch.empty(0, 2, 16, device=DEV, requires_grad=True)
   g = torch.empty(0, 2, device=DEV)
