@@ -147,7 +147,7 @@ def _bind(lib) -> None:
                                       p, sz, p]
   lib.ascan_shift_pad.restype = ci
   lib.ascan_shift_pad.argtypes = [p, p, p, ci, i64, i64, i64, ci, ctypes.c_double, ci, ci, p]
-  f, rows = ctypes.c_float, ctypes.POINTER(Rows)
+  f, rows = ctypes.c_float, p  # rows: a pointer to ascan_rows
   lib.ascan_matrix_scan_workspace.restype = sz
   lib.ascan_matrix_scan_workspace.argtypes = [i64, i64, ci, ci, ci, ci, ci, ci, ci, ci]
   lib.ascan_matrix_scan_forward.restype = ci

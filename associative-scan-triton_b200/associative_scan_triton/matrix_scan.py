@@ -23,15 +23,29 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODES, INDEX_CODES, Rows
+from ._lib import DTYPE_CODES, INDEX_CODES
 
 MAX_DIM = 128  # of a matrix state's sides
 
+_ROWS = {n: ctypes.c_int64 * (4 * n) for n in (2, 4)}
 
-def _rows(t: torch.Tensor):
-  """``ascan_rows`` of a [tokens, heads, dim] or [tokens, heads] tensor."""
-  st = t.stride()
-  return ctypes.byref(Rows(t.data_ptr(), st[0], st[1], t.shape[1]))
+
+def _rows(*tensors: torch.Tensor):
+  """``ascan_rows`` of [tokens, heads, dim] or [tokens, heads] tensors, one pointer each.
+
+  One array holds them all (pointer, two strides, heads: four words), which
+  costs a call less than a structure for each.
+  """
+  words = []
+  for t in tensors:
+    st = t.stride()
+    words += (t.data_ptr(), st[0], st[1], t.shape[1])
+  block = _ROWS[len(tensors)](*words)
+  return [ctypes.byref(block, 32 * i) for i in range(len(tensors))]
+
+
+def _stream(device: torch.device) -> int:
+  return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -81,6 +95,22 @@ def _check_state(name: str, t: torch.Tensor, device, shape) -> None:
 
 def _check_operands(queries, keys, values, log_gates, max_dim):
   """Checks the four inputs; returns (device, tokens, heads, key_dim, value_dim)."""
+  try:  # the usual call in one expression; whatever fails it is looked at below
+    (n, hq, dk), (nk, hk, dkk), (nv, hv, dv), (ng, hg) = (queries.shape, keys.shape, values.shape,
+                                                         log_gates.shape)
+    device, dtype, gate_dtype = queries.device, queries.dtype, log_gates.dtype
+    heads = max(hq, hk, hv, hg)
+    if (queries.is_cuda and keys.device == device and values.device == device
+        and log_gates.device == device and dtype in DTYPE_CODES and keys.dtype == dtype
+        and values.dtype == dtype and (gate_dtype == torch.float32 or gate_dtype == dtype)
+        and nk == n and nv == n and ng == n and dkk == dk and dk > 1 and dv > 1
+        and (max_dim is None or (dk <= max_dim and dv <= max_dim)) and heads <= 65535
+        and hq > 0 and hk > 0 and hv > 0 and hg > 0
+        and not (heads % hq or heads % hk or heads % hv or heads % hg)
+        and queries.stride(2) == 1 and keys.stride(2) == 1 and values.stride(2) == 1):
+      return device, n, heads, dk, dv
+  except (AttributeError, TypeError, ValueError):
+    pass
   _check_rows("queries", queries, None, None)
   device, tokens, key_dim = queries.device, queries.shape[0], queries.shape[2]
   _check_rows("keys", keys, device, queries.dtype, tokens, key_dim)
@@ -105,7 +135,7 @@ class _on:
   __slots__ = ("guard",)
 
   def __init__(self, device):
-    self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
   def __enter__(self):
     if self.guard is not None:
@@ -148,10 +178,10 @@ def _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_s
                                       values.shape[1], log_gates.shape[1], key_dim, value_dim, 0),
       dtype=torch.uint8, device=device)
     rc = lib.ascan_matrix_scan_forward(
-      _rows(queries), _rows(keys), _rows(values), _rows(log_gates), DTYPE_CODES[log_gates.dtype],
+      *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],
       cu_seqlens.data_ptr(), INDEX_CODES[cu_seqlens.dtype], num_seq, tokens, heads, key_dim,
       value_dim, DTYPE_CODES[queries.dtype], scale, _ptr(initial_state), out.data_ptr(),
-      _ptr(final), ws.data_ptr(), ws.numel(), _lib._stream_ptr(device))
+      _ptr(final), ws.data_ptr(), ws.numel(), _stream(device))
   _lib._finish(rc, "ascan_matrix_scan_forward", device)
   return out, final
 
@@ -183,12 +213,12 @@ def _scan_backward(queries, keys, values, log_gates, cu_seqlens, scale, initial_
                                       values.shape[1], log_gates.shape[1], key_dim, value_dim, 1),
       dtype=torch.uint8, device=device)
     rc = lib.ascan_matrix_scan_backward(
-      _rows(queries), _rows(keys), _rows(values), _rows(log_gates), DTYPE_CODES[log_gates.dtype],
-      _rows(d_out), _ptr(initial_state), _ptr(final_state), _ptr(d_final), cu_seqlens.data_ptr(),
+      *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],
+      *_rows(d_out, d_out)[:1], _ptr(initial_state), _ptr(final_state), _ptr(d_final), cu_seqlens.data_ptr(),
       INDEX_CODES[cu_seqlens.dtype], num_seq, tokens, heads, key_dim, value_dim,
       DTYPE_CODES[queries.dtype], scale, d_queries.data_ptr(), d_keys.data_ptr(),
       d_values.data_ptr(), d_gates.data_ptr(), _ptr(d_initial), ws.data_ptr(), ws.numel(),
-      _lib._stream_ptr(device))
+      _stream(device))
   _lib._finish(rc, "ascan_matrix_scan_backward", device)
   return d_queries, d_keys, d_values, d_gates, d_initial
 
@@ -247,8 +277,9 @@ def matrix_scan_causal(
   """
   scale = float(queries.shape[-1]) ** -0.5 if scale is None else float(scale)
   cu_seqlens = args["cu_seqlens"]
-  if torch.is_grad_enabled() and any(
-      t is not None and t.requires_grad for t in (queries, keys, values, log_gates, initial_state)):
+  if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad
+                                  or values.requires_grad or log_gates.requires_grad
+                                  or (initial_state is not None and initial_state.requires_grad)):
     out, final = MatrixScanCausal.apply(queries, keys, values, log_gates, cu_seqlens, scale,
                                         initial_state, bool(return_final_state))
   else:
@@ -315,9 +346,9 @@ def matrix_scan_step(
   scale = float(key_dim) ** -0.5 if scale is None else float(scale)
   with _on(device):
     rc = _lib.load().ascan_matrix_scan_step(
-      _rows(queries), _rows(keys), _rows(values), _rows(log_gates), DTYPE_CODES[log_gates.dtype],
+      *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],
       _ptr(slots), batch, state.shape[0], heads, key_dim, value_dim, DTYPE_CODES[queries.dtype],
-      scale, state.data_ptr(), state_out.data_ptr(), out.data_ptr(), _lib._stream_ptr(device))
+      scale, state.data_ptr(), state_out.data_ptr(), out.data_ptr(), _stream(device))
   _lib._finish(rc, "ascan_matrix_scan_step", device)
   return out
 
@@ -331,7 +362,7 @@ def _rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions,
                    interleaved):
   """The leading arguments that the two native calls share, by name of their place."""
   index = positions if positions is not None else cu_seqlens
-  return (_rows(queries), _rows(keys), query_weight.data_ptr(), key_weight.data_ptr(),
+  return (*_rows(queries, keys), query_weight.data_ptr(), key_weight.data_ptr(),
           DTYPE_CODES[query_weight.dtype], cos.data_ptr(), sin.data_ptr(), cos.shape[0],
           cos.shape[1], int(interleaved), _ptr(positions),
           None if positions is not None else cu_seqlens.data_ptr(), INDEX_CODES[index.dtype],
@@ -379,7 +410,7 @@ def _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions
     rc = _lib.load().ascan_qk_norm_rotate(
       *_rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
                       eps, interleaved),
-      out_q.data_ptr(), out_k.data_ptr(), _lib._stream_ptr(device))
+      out_q.data_ptr(), out_k.data_ptr(), _stream(device))
   _lib._finish(rc, "ascan_qk_norm_rotate", device)
   return out_q, out_k
 
@@ -405,8 +436,8 @@ def _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, position
     rc = lib.ascan_qk_norm_rotate_backward(
       *_rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
                       eps, interleaved),
-      _rows(grads[0]), _rows(grads[1]), d_q.data_ptr(), d_k.data_ptr(), d_qw.data_ptr(),
-      d_kw.data_ptr(), ws.data_ptr(), ws.numel(), _lib._stream_ptr(device))
+      *_rows(grads[0], grads[1]), d_q.data_ptr(), d_k.data_ptr(), d_qw.data_ptr(),
+      d_kw.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
   _lib._finish(rc, "ascan_qk_norm_rotate_backward", device)
   return d_q, d_k, d_qw, d_kw
 

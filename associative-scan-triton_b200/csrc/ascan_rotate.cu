@@ -8,12 +8,12 @@
 // calls and launch latency small ones.  A group of lanes holds one head as
 // one 16-byte vector per lane; the rotation's partner comes by a shuffle (or
 // sits in the same vector when pairs are adjacent), and the sums go over the
-// group by shuffles.  A group takes up to four heads of one token together:
-// their loads are in flight at once and the token's cosines are read once.
-// Queries and keys share a launch: the first CTAs take the query heads, the
-// rest the key heads.  The weights' gradients stay in registers over all of
-// a group's heads, meet in shared memory, and a second launch adds the CTAs'
-// rows in a fixed order, so results repeat bit for bit.
+// group by shuffles.  A group walks the heads of consecutive tokens with
+// several heads' loads in flight and a token's angles read once for all of
+// them.  Queries and keys share a launch: the first CTAs take the query heads,
+// the rest the key heads.  The weights' gradients stay in registers over all
+// of a group's heads, meet in shared memory, and a second launch adds the
+// CTAs' rows in a fixed order, so results repeat bit for bit.
 #include "ascan_impl.cuh"
 #include "ascan_mscan.cuh"
 
@@ -37,6 +37,8 @@ struct Side {  // queries or keys
   float* part;   // [CTAs, dim]: rows of the weight gradient
   void* dw;
   int heads, ctas;
+  int slices, heads_per;  // vector kernel: groups per token, heads of each
+  long long span;         // tokens in a row per group
 };
 
 struct Args {
@@ -110,73 +112,111 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// The lane's part of a token's rotation: how its elements turn, and where the
-// partners sit.
-template <typename T>
+// Sequence lookups of tokens that come in order: the last one found serves
+// until the token leaves it.
+struct Place {
+  long long start = 0, end = -1;
+};
+
+// Table row of token t in order; -1: zero row.
+__device__ __forceinline__ long long next_row(const Args& a, long long t, Place& at) {
+  if (a.positions || t >= at.end || t < at.start) {
+    const long long row = table_row(a, t);
+    if (!a.positions && row >= 0) {
+      at.start = t - row;
+      at.end = at.start;
+      long long lo = 0, hi = a.N;
+      while (lo < hi) {
+        const long long mid = (lo + hi) >> 1;
+        if (index_at(a.cu, a.index64, mid + 1) > t) hi = mid;
+        else lo = mid + 1;
+      }
+      at.end = index_at(a.cu, a.index64, lo + 1);
+    }
+    return row;
+  }
+  const long long row = t - at.start;
+  if (row >= a.rows) {
+    report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(t), a.err);
+    return -1;
+  }
+  return row;
+}
+
+// How the lane's elements of a token turn: y[i] = x[i] p[i] + x'[i] q[i] with x'
+// the partner, for the forward with the weights in p and q (w[i] cos, +-w' sin),
+// for the gradients of the transposed turn without them (cos, -+sin).
+template <typename T, bool BWD>
 struct Turn {
   static constexpr int V = Vec<T>::V;
-  float c[V], s[V];  // per element; s carries the sign of the partner's term
-  int partner;       // lane of the group that holds the partners
+  float p[V], q[V];
 
-  __device__ __forceinline__ void load(const Args& a, long long row, int gl) {
+  __device__ __forceinline__ void load(const Args& a, const Side& sd, long long row, int gl, int partner) {
+    float c[V], s[V];
     const int hv = a.half / V;
-    partner = gl;
-    if (row < 0 || gl >= 2 * hv) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) c[i] = 1.f, s[i] = 0.f;
-      return;
-    }
-    const float* ct = a.cos_table + row * a.half;
-    const float* st = a.sin_table + row * a.half;
-    if (a.interleaved) {
+    for (int i = 0; i < V; ++i) c[i] = 1.f, s[i] = 0.f;
+    if (row >= 0 && gl < 2 * hv) {
+      const float* ct = a.cos_table + row * a.half;
+      const float* st = a.sin_table + row * a.half;
+      if (a.interleaved) {
 #pragma unroll
-      for (int i = 0; i < V; i += 2) {
-        const int at = (gl * V + i) / 2;
-        c[i] = c[i + 1] = __ldg(ct + at);
-        const float v = __ldg(st + at);
-        s[i] = -v, s[i + 1] = v;
-      }
-    } else {
-      const bool low = gl < hv;
-      const int at = (low ? gl : gl - hv) * V;
-      partner = low ? gl + hv : gl - hv;
+        for (int i = 0; i < V; i += 2) {
+          const int at = (gl * V + i) / 2;
+          c[i] = c[i + 1] = __ldg(ct + at);
+          const float v = __ldg(st + at);
+          s[i] = -v, s[i + 1] = v;
+        }
+      } else {
+        const int at = (gl < hv ? gl : gl - hv) * V;
+        const float sign = gl < hv ? -1.f : 1.f;
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 cv = __ldg(reinterpret_cast<const float4*>(ct + at + i));
-        const float4 sv = __ldg(reinterpret_cast<const float4*>(st + at + i));
-        c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
-        s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
-        if (low) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i + e] = -s[i + e];
+        for (int i = 0; i < V; i += 4) {
+          const float4 cv = __ldg(reinterpret_cast<const float4*>(ct + at + i));
+          const float4 sv = __ldg(reinterpret_cast<const float4*>(st + at + i));
+          c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
+          s[i] = sign * sv.x, s[i + 1] = sign * sv.y, s[i + 2] = sign * sv.z, s[i + 3] = sign * sv.w;
         }
       }
     }
-  }
-
-  // y = R n, or with dir = -1 y = R^T n.  Every lane of the warp takes part.
-  template <int G>
-  __device__ __forceinline__ void apply(const Args& a, const float* n, float* y, float dir) const {
-    if (a.interleaved) {
 #pragma unroll
-      for (int i = 0; i < V; i += 2) {
-        y[i] = fmaf(dir * s[i], n[i + 1], c[i] * n[i]);
-        y[i + 1] = fmaf(dir * s[i + 1], n[i], c[i + 1] * n[i + 1]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float o = __shfl_sync(kFull, n[i], partner, G);
-        // an unrotated element has s = 0 and itself as the partner; select, so
-        // that an infinity there does not become 0 * inf
-        y[i] = s[i] == 0.f ? c[i] * n[i] : fmaf(dir * s[i], o, c[i] * n[i]);
+    for (int i = 0; i < V; ++i) {
+      if (BWD) {
+        p[i] = c[i], q[i] = -s[i];
+      } else {
+        const int mine = gl * V + i, other = a.interleaved ? mine ^ 1 : partner * V + i;
+        p[i] = mine < a.dim ? c[i] * load_any(sd.w, a.wtype, mine) : 0.f;
+        q[i] = s[i] != 0.f ? s[i] * load_any(sd.w, a.wtype, other) : 0.f;
       }
     }
   }
+
+  // Every lane of the warp takes part.
+  template <int G>
+  __device__ __forceinline__ void apply(const Args& a, const uint4& raw, int partner, const float* x, float* y) const {
+    float o[V];
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = x[i ^ 1];
+    } else {
+      uint4 r;
+      r.x = __shfl_sync(kFull, raw.x, partner, G);
+      r.y = __shfl_sync(kFull, raw.y, partner, G);
+      r.z = __shfl_sync(kFull, raw.z, partner, G);
+      r.w = __shfl_sync(kFull, raw.w, partner, G);
+      unpack<T>(r, o);
+    }
+    // an element that does not turn has q = 0; select, so that an infinity in
+    // its place of the pair does not become 0 * inf
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = q[i] == 0.f ? x[i] * p[i] : fmaf(o[i], q[i], x[i] * p[i]);
+  }
 };
 
-template <typename T, int G, int HPG, bool BWD>
-__global__ void __launch_bounds__(kRotThreads) vec_kernel(const __grid_constant__ Args a) {
+// A group walks `span` tokens in order and, for each, heads [h0, h1) of its
+// side.  DEPTH heads' loads are always in flight, over token boundaries too.
+template <typename T, int G, int DEPTH, bool BWD>
+__global__ void __launch_bounds__(kRotThreads, BWD ? 2 : 3) vec_kernel(const __grid_constant__ Args a) {
   constexpr int V = Vec<T>::V;
   constexpr int GROUPS = kRotThreads / G;
   const bool is_key = static_cast<int>(blockIdx.x) >= a.side[0].ctas;
@@ -184,70 +224,76 @@ __global__ void __launch_bounds__(kRotThreads) vec_kernel(const __grid_constant_
   const int cta = is_key ? blockIdx.x - a.side[0].ctas : blockIdx.x;
   const int gl = threadIdx.x % G, group = threadIdx.x / G;
   const bool on = gl * V < a.dim;
+  const int hv = a.half / V;
+  const int partner = gl < hv ? gl + hv : (gl < 2 * hv ? gl - hv : gl);
   check_cu(a);
+  const long long g = static_cast<long long>(cta) * GROUPS + group;
+  const int slice = static_cast<int>(g % sd.slices);
+  const int h0 = slice * sd.heads_per, h1 = min(h0 + sd.heads_per, sd.heads);
+  const long long first = g / sd.slices * sd.span;
+  const long long tokens = max(0ll, min(static_cast<long long>(sd.span), a.tokens - first));
+  // every group of a warp runs the same number of rounds: the shuffles need them
+  const int items = static_cast<int>(sd.span) * sd.heads_per;
   float w[V], dw[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    w[i] = on ? load_any(sd.w, a.wtype, gl * V + i) : 0.f;
+    w[i] = BWD && on ? load_any(sd.w, a.wtype, gl * V + i) : 0.f;
     dw[i] = 0.f;
   }
-  const int per = (sd.heads + HPG - 1) / HPG;
-  const long long units = a.tokens * per;
   const float inv = 1.f / static_cast<float>(a.dim);
-  const long long step = static_cast<long long>(sd.ctas) * GROUPS;
-  // all groups of a warp run the same number of rounds: the shuffles need them
-  const long long rounds = (units + step - 1) / step;
-  for (long long r = 0; r < rounds; ++r) {
-    const long long unit = r * step + static_cast<long long>(cta) * GROUPS + group;
-    const bool live = unit < units;
-    const long long t = live ? unit / per : 0;
-    const int h0 = live ? static_cast<int>(unit % per) * HPG : 0;
-    const T* src = static_cast<const T*>(sd.x) + t * sd.st + h0 * sd.sh + gl * V;
-    const T* dsrc = BWD ? static_cast<const T*>(sd.dy) + t * sd.dst + h0 * sd.dsh + gl * V : nullptr;
-    uint4 raw[HPG], draw[HPG];
+  const T* src = static_cast<const T*>(sd.x) + gl * V;
+  const T* dsrc = BWD ? static_cast<const T*>(sd.dy) + gl * V : nullptr;
+  uint4 raw[DEPTH], draw[BWD ? DEPTH : 1];
+  int lt = 0, lh = h0;  // the next load
+  auto load = [&](int q) {
+    const bool ok = on && lt < tokens && lh < h1;
+    raw[q] = ok ? __ldcs(reinterpret_cast<const uint4*>(src + (first + lt) * sd.st + lh * sd.sh)) : make_uint4(0, 0, 0, 0);
+    if (BWD) draw[q] = ok ? __ldcs(reinterpret_cast<const uint4*>(dsrc + (first + lt) * sd.dst + lh * sd.dsh)) : make_uint4(0, 0, 0, 0);
+    if (++lh >= h0 + sd.heads_per) lh = h0, ++lt;
+  };
 #pragma unroll
-    for (int q = 0; q < HPG; ++q) {
-      const bool ok = live && on && h0 + q < sd.heads;
-      raw[q] = ok ? *reinterpret_cast<const uint4*>(src + q * sd.sh) : make_uint4(0, 0, 0, 0);
-      if (BWD) draw[q] = ok ? *reinterpret_cast<const uint4*>(dsrc + q * sd.dsh) : make_uint4(0, 0, 0, 0);
-    }
-    const long long row = live ? table_row(a, t) : -1;
-    Turn<T> turn;
-    turn.load(a, row, gl);
-    T* dst = static_cast<T*>(sd.out) + (t * sd.heads + h0) * a.dim + gl * V;
+  for (int q = 0; q < DEPTH; ++q) load(q);
+  Turn<T, BWD> turn;
+  Place place;
+  long long row = -1;
+  int ct = 0, ch = h0;  // the next head to finish
+  for (int r = 0; r < items; r += DEPTH) {
 #pragma unroll
-    for (int q = 0; q < HPG; ++q) {
-      float x[V], sq = 0.f;
+    for (int q = 0; q < DEPTH; ++q) {
+      const long long t = first + ct;
+      const bool live = ct < tokens && ch < h1;
+      if (ch == h0) {
+        row = ct < tokens ? next_row(a, t, place) : -1;
+        turn.load(a, sd, row, gl, partner);
+      }
+      float x[V], y[V], sq = 0.f;
       unpack<T>(raw[q], x);
 #pragma unroll
       for (int i = 0; i < V; ++i) sq = fmaf(x[i], x[i], sq);
       const float rs = rsqrtf(fmaf(group_sum<G>(sq), inv, a.eps));
-      float y[V];
       if (!BWD) {
-        float n[V];
+        turn.template apply<G>(a, raw[q], partner, x, y);
 #pragma unroll
-        for (int i = 0; i < V; ++i) n[i] = x[i] * rs * w[i];
-        turn.template apply<G>(a, n, y, 1.f);
+        for (int i = 0; i < V; ++i) y[i] = row >= 0 ? y[i] * rs : 0.f;
       } else {
         float dy[V], dz[V], sum = 0.f;
         unpack<T>(draw[q], dy);
-        turn.template apply<G>(a, dy, dz, -1.f);
+        turn.template apply<G>(a, draw[q], partner, dy, dz);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           x[i] *= rs;  // xh
-          const float g = dz[i] * x[i];
-          if (row >= 0) dw[i] += g;
-          sum = fmaf(g, w[i], sum);
+          const float gw = dz[i] * x[i];
+          if (live && row >= 0) dw[i] += gw;
+          sum = fmaf(gw, w[i], sum);
         }
         const float mean = group_sum<G>(sum) * inv;
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = rs * fmaf(-x[i], mean, w[i] * dz[i]);
+        for (int i = 0; i < V; ++i) y[i] = row >= 0 ? rs * fmaf(-x[i], mean, w[i] * dz[i]) : 0.f;
       }
-      if (row < 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = 0.f;
-      }
-      if (live && on && h0 + q < sd.heads) *reinterpret_cast<uint4*>(dst + q * a.dim) = pack<T>(y);
+      load(q);
+      if (live && on)
+        __stcs(reinterpret_cast<uint4*>(static_cast<T*>(sd.out) + (t * sd.heads + ch) * a.dim + gl * V), pack<T>(y));
+      if (++ch >= h0 + sd.heads_per) ch = h0, ++ct;
     }
   }
   if (BWD) {
@@ -257,7 +303,7 @@ __global__ void __launch_bounds__(kRotThreads) vec_kernel(const __grid_constant_
     __syncthreads();
     for (int d = threadIdx.x; d < a.dim; d += kRotThreads) {
       float x = 0.f;
-      for (int g = 0; g < GROUPS; ++g) x += red[g][d];
+      for (int e = 0; e < GROUPS; ++e) x += red[e][d];
       sd.part[static_cast<long long>(cta) * a.dim + d] = x;
     }
   }
@@ -349,34 +395,53 @@ __global__ void __launch_bounds__(kRotThreads) any_kernel(const __grid_constant_
   }
 }
 
-// Adds the CTAs' rows: 32 columns and 8 slices of the rows per CTA, the
+// Adds the CTAs' rows: 32 columns and 32 slices of the rows per CTA, the
 // slices joined in order.
-__global__ void __launch_bounds__(256) weight_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(1024) weight_kernel(const __grid_constant__ Args a) {
   const Side& sd = a.side[blockIdx.y];
   const int d = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-  __shared__ float red[8][32];
+  __shared__ float red[32][32];
   float x = 0.f;
-  if (d < a.dim)
-    for (int c = slice; c < sd.ctas; c += 8) x += sd.part[static_cast<long long>(c) * a.dim + d];
+  if (d < a.dim) {
+#pragma unroll 4
+    for (int c = slice; c < sd.ctas; c += 32) x += sd.part[static_cast<long long>(c) * a.dim + d];
+  }
   red[slice][threadIdx.x & 31] = x;
   __syncthreads();
   if (slice == 0 && d < a.dim) {
-    for (int s = 1; s < 8; ++s) x += red[s][threadIdx.x];
+    for (int s = 1; s < 32; ++s) x += red[s][threadIdx.x];
     store_any(sd.dw, a.wtype, d, x);
   }
 }
 
-constexpr long long kMaxCtas = 148 * 8;
+constexpr long long kMaxCtas = 148 * 6;
 
-// CTAs for one side: its share of the heads, at most what its work fills.
-static void split(Args& a, long long per_cta, int hpg) {
-  const long long cap = kMaxCtas;
+// CTAs of the plain form for one side: its share of the heads, at most what
+// its work fills.
+static void split(Args& a, long long per_cta) {
   const long long total = a.side[0].heads + a.side[1].heads;
   for (int s = 0; s < 2; ++s) {
-    const long long units = a.tokens * ((a.side[s].heads + hpg - 1) / hpg);
-    const long long fill = (units + per_cta - 1) / per_cta;
-    const long long share = max(1ll, cap * a.side[s].heads / total);
+    const long long fill = (a.tokens * a.side[s].heads + per_cta - 1) / per_cta;
+    const long long share = max(1ll, kMaxCtas * a.side[s].heads / total);
     a.side[s].ctas = static_cast<int>(min(fill, share));
+  }
+}
+
+// Groups of the vector kernel.  Each side gets its share (by heads) of the
+// groups that are resident at once.  With fewer tokens than groups a token's
+// heads are dealt to several groups, for the shortest chain; with more, a
+// group takes whole tokens, several in a row, and reads their angles once.
+static void split_groups(Args& a, int groups_per_cta, int ctas_per_sm) {
+  const long long total = a.side[0].heads + a.side[1].heads, room = 148ll * ctas_per_sm;
+  for (int s = 0; s < 2; ++s) {
+    Side& sd = a.side[s];
+    const long long groups = max(1ll, room * sd.heads / total) * groups_per_cta;
+    const long long slices = max(1ll, min(static_cast<long long>(sd.heads), groups / max(1ll, a.tokens)));
+    sd.heads_per = static_cast<int>((sd.heads + slices - 1) / slices);
+    sd.slices = (sd.heads + sd.heads_per - 1) / sd.heads_per;
+    sd.span = (a.tokens * sd.slices + groups - 1) / groups;
+    const long long used = (a.tokens + sd.span - 1) / sd.span * sd.slices;
+    sd.ctas = static_cast<int>((used + groups_per_cta - 1) / groups_per_cta);
   }
 }
 
@@ -385,25 +450,19 @@ static int run(Args& a, bool vec, cudaStream_t s) {
   if (vec) {
     const int lanes = a.dim / Vec<T>::V;
     const int g = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32);
-    // several heads a group once that still fills the card: their loads overlap
-    // and share the cosines; one head a group below that, for the shortest chain
-    const bool four = a.tokens * (a.side[0].heads + a.side[1].heads) >= 4 * 148 * 8 * (kRotThreads / g);
-    split(a, kRotThreads / g, four ? (BWD ? 2 : 4) : 1);
+    split_groups(a, kRotThreads / g, BWD ? 2 : 3);
     const unsigned grid = a.side[0].ctas + a.side[1].ctas;
-#define ROT_CASE(GG)                                                                        \
-  (four ? (void)(vec_kernel<T, GG, BWD ? 2 : 4, BWD><<<grid, kRotThreads, 0, s>>>(a))       \
-        : (void)(vec_kernel<T, GG, 1, BWD><<<grid, kRotThreads, 0, s>>>(a)))
-    if (g == 8) ROT_CASE(8);
-    else if (g == 16) ROT_CASE(16);
-    else ROT_CASE(32);
-#undef ROT_CASE
+    constexpr int D = BWD ? 2 : 4;
+    if (g == 8) vec_kernel<T, 8, D, BWD><<<grid, kRotThreads, 0, s>>>(a);
+    else if (g == 16) vec_kernel<T, 16, D, BWD><<<grid, kRotThreads, 0, s>>>(a);
+    else vec_kernel<T, 32, D, BWD><<<grid, kRotThreads, 0, s>>>(a);
   } else {
-    split(a, kRotThreads / 32, 1);
+    split(a, kRotThreads / 32);
     any_kernel<T, BWD><<<a.side[0].ctas + a.side[1].ctas, kRotThreads, 0, s>>>(a);
   }
   int rc = launch_status();
   if (BWD && rc == ASCAN_OK) {
-    weight_kernel<<<dim3((a.dim + 31) / 32, 2), 256, 0, s>>>(a);
+    weight_kernel<<<dim3((a.dim + 31) / 32, 2), 1024, 0, s>>>(a);
     rc = launch_status();
   }
   return rc;
