@@ -8,7 +8,8 @@
 // calls and launch latency small ones.  A group of lanes holds one head as
 // one 16-byte vector per lane; the rotation's partner comes by a shuffle (or
 // sits in the same vector when pairs are adjacent), and the sums go over the
-// group by shuffles.  A group walks the heads of consecutive tokens with
+// group by shuffles.  Where the whole head turns, a lane holds 8 bytes of each
+// half instead and has both sides of its pairs.  A group walks the heads of consecutive tokens with
 // several heads' loads in flight and a token's angles read once for all of
 // them.  Queries and keys share a launch: the first CTAs take the query heads,
 // the rest the key heads.  The weights' gradients stay in registers over all
@@ -89,20 +90,82 @@ struct Vec {
   static constexpr int V = 16 / sizeof(T);
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& u, float* x) {
-  const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < Vec<T>::V; ++i) x[i] = to_f(e[i]);
+// Two floats in one register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
+// A lane's 16 bytes as register pairs of floats and back.
 template <typename T>
-__device__ __forceinline__ uint4 pack(const float* x) {
-  uint4 u;
-  T* e = reinterpret_cast<T*>(&u);
+__device__ __forceinline__ void unpack(const uint4& u, uint64_t* x);
+template <>
+__device__ __forceinline__ void unpack<float>(const uint4& u, uint64_t* x) {
+  x[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
+  x[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
+}
+template <>
+__device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& u, uint64_t* x) {
+  const uint32_t e[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < Vec<T>::V; ++i) e[i] = from_f<T>(x[i]);
-  return u;
+  for (int i = 0; i < 4; ++i) x[i] = pair(__uint_as_float(e[i] << 16), __uint_as_float(e[i] & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ void unpack<__half>(const uint4& u, uint64_t* x) {
+  const uint32_t e[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&e[i]));
+    x[i] = pair(f.x, f.y);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const uint64_t* x);
+template <>
+__device__ __forceinline__ uint4 pack<float>(const uint64_t* x) {
+  const float2 a = unpair(x[0]), b = unpair(x[1]);
+  return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+}
+template <>
+__device__ __forceinline__ uint4 pack<__nv_bfloat16>(const uint64_t* x) {
+  uint32_t e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = unpair(x[i]);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(e[i]) : "f"(a.y), "f"(a.x));
+  }
+  return make_uint4(e[0], e[1], e[2], e[3]);
+}
+template <>
+__device__ __forceinline__ uint4 pack<__half>(const uint64_t* x) {
+  uint32_t e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = unpair(x[i]);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(e[i]) : "f"(a.y), "f"(a.x));
+  }
+  return make_uint4(e[0], e[1], e[2], e[3]);
 }
 
 template <int G>
@@ -143,61 +206,82 @@ __device__ __forceinline__ long long next_row(const Args& a, long long t, Place&
   return row;
 }
 
-// How the lane's elements of a token turn: y[i] = x[i] p[i] + x'[i] q[i] with x'
-// the partner, for the forward with the weights in p and q (w[i] cos, +-w' sin),
-// for the gradients of the transposed turn without them (cos, -+sin).
-template <typename T, bool BWD>
+// Where a lane's 16 bytes of a head lie.
+//   kSplit: the whole head turns in halves; a lane has 8 bytes of each, so both
+//           sides of its pairs
+//   kAdjacent: pairs are neighbours
+//   kPart: part of the head turns in halves; 16 bytes in a row, the partner's
+//          come by shuffles
+enum Pairing { kSplit, kAdjacent, kPart };
+
+// How the lane's elements of a token turn: y = x p + x' q with x' the partner,
+// for the forward with the weights in p and q (w cos, +-w' sin), for the
+// gradients of the transposed turn without them (cos, -+sin).
+template <typename T, Pairing P, bool BWD>
 struct Turn {
   static constexpr int V = Vec<T>::V;
-  float p[V], q[V];
+  uint64_t p[V / 2], q[V / 2];
 
-  __device__ __forceinline__ void load(const Args& a, const Side& sd, long long row, int gl, int partner) {
-    float c[V], s[V];
-    const int hv = a.half / V;
+  // Element of the head that the lane's i-th is.
+  static __device__ __forceinline__ int element(const Args& a, int gl, int i) {
+    if (P == kSplit) return i < V / 2 ? gl * (V / 2) + i : a.half + gl * (V / 2) + i - V / 2;
+    return gl * V + i;
+  }
+
+  // `w`: the side's weights as floats, in shared memory.
+  __device__ __forceinline__ void load(const Args& a, const float* w, long long row, int gl) {
+    constexpr int A = P == kPart ? V : V / 2;  // angles of the lane
+    float c[A], s[A];
 #pragma unroll
-    for (int i = 0; i < V; ++i) c[i] = 1.f, s[i] = 0.f;
-    if (row >= 0 && gl < 2 * hv) {
-      const float* ct = a.cos_table + row * a.half;
-      const float* st = a.sin_table + row * a.half;
-      if (a.interleaved) {
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          const int at = (gl * V + i) / 2;
-          c[i] = c[i + 1] = __ldg(ct + at);
-          const float v = __ldg(st + at);
-          s[i] = -v, s[i + 1] = v;
-        }
+    for (int i = 0; i < A; ++i) c[i] = 1.f, s[i] = 0.f;
+    // kPart: lanes of the second half have the same angles as their partners
+    const int hv = a.half / V, first = P == kPart ? (gl < hv ? gl : gl - hv) * V : gl * (V / 2);
+    const bool turns = row >= 0 && first < a.half;
+    if (turns) {
+      const float* ct = a.cos_table + row * a.half + first;
+      const float* st = a.sin_table + row * a.half + first;
+      if (A == 2) {
+        const float2 x = __ldg(reinterpret_cast<const float2*>(ct)), y = __ldg(reinterpret_cast<const float2*>(st));
+        c[0] = x.x, c[1] = x.y, s[0] = y.x, s[1] = y.y;
       } else {
-        const int at = (gl < hv ? gl : gl - hv) * V;
-        const float sign = gl < hv ? -1.f : 1.f;
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-          const float4 cv = __ldg(reinterpret_cast<const float4*>(ct + at + i));
-          const float4 sv = __ldg(reinterpret_cast<const float4*>(st + at + i));
-          c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
-          s[i] = sign * sv.x, s[i + 1] = sign * sv.y, s[i + 2] = sign * sv.z, s[i + 3] = sign * sv.w;
+        for (int i = 0; i < A; i += 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(ct + i)), y = __ldg(reinterpret_cast<const float4*>(st + i));
+          c[i] = x.x, c[i + 1] = x.y, c[i + 2] = x.z, c[i + 3] = x.w;
+          s[i] = y.x, s[i + 1] = y.y, s[i + 2] = y.z, s[i + 3] = y.w;
         }
       }
     }
+    float pv[V], qv[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (BWD) {
-        p[i] = c[i], q[i] = -s[i];
-      } else {
-        const int mine = gl * V + i, other = a.interleaved ? mine ^ 1 : partner * V + i;
-        p[i] = mine < a.dim ? c[i] * load_any(sd.w, a.wtype, mine) : 0.f;
-        q[i] = s[i] != 0.f ? s[i] * load_any(sd.w, a.wtype, other) : 0.f;
+      const int d = element(a, gl, i), at = P == kSplit ? i % A : (P == kAdjacent ? i / 2 : i);
+      const bool low = P == kSplit ? i < A : (P == kAdjacent ? i % 2 == 0 : gl < hv);
+      pv[i] = c[at];
+      qv[i] = low == BWD ? s[at] : -s[at];
+      if (!BWD) {
+        const int other = P == kAdjacent ? d ^ 1 : (low ? d + a.half : d - a.half);
+        pv[i] *= d < a.dim ? w[d] : 0.f;
+        qv[i] *= turns ? w[other] : 0.f;
       }
     }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = pair(pv[2 * i], pv[2 * i + 1]), q[i] = pair(qv[2 * i], qv[2 * i + 1]);
   }
 
   // Every lane of the warp takes part.
   template <int G>
-  __device__ __forceinline__ void apply(const Args& a, const uint4& raw, int partner, const float* x, float* y) const {
-    float o[V];
-    if (a.interleaved) {
+  __device__ __forceinline__ void apply(const uint4& raw, int partner, const uint64_t* x, uint64_t* y) const {
+    uint64_t o[V / 2];
+    if (P == kSplit) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = x[i ^ 1];
+      for (int i = 0; i < V / 2; ++i) o[i] = x[(i + V / 4) % (V / 2)];
+    } else if (P == kAdjacent) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const float2 e = unpair(x[i]);
+        o[i] = pair(e.y, e.x);
+      }
     } else {
       uint4 r;
       r.x = __shfl_sync(kFull, raw.x, partner, G);
@@ -206,18 +290,35 @@ struct Turn {
       r.w = __shfl_sync(kFull, raw.w, partner, G);
       unpack<T>(r, o);
     }
-    // an element that does not turn has q = 0; select, so that an infinity in
-    // its place of the pair does not become 0 * inf
 #pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = q[i] == 0.f ? x[i] * p[i] : fmaf(o[i], q[i], x[i] * p[i]);
+    for (int i = 0; i < V / 2; ++i) y[i] = fma2(o[i], q[i], mul2(x[i], p[i]));
   }
 };
 
-// A group walks `span` tokens in order and, for each, heads [h0, h1) of its
-// side.  DEPTH heads' loads are always in flight, over token boundaries too.
-template <typename T, int G, int DEPTH, bool BWD>
+// A lane's 16 bytes of a head: in one piece, or 8 bytes of each half.
+template <Pairing P>
+__device__ __forceinline__ uint4 get(const char* at, long long half_bytes) {
+  if (P != kSplit) return __ldcs(reinterpret_cast<const uint4*>(at));
+  const uint2 a = __ldcs(reinterpret_cast<const uint2*>(at)), b = __ldcs(reinterpret_cast<const uint2*>(at + half_bytes));
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <Pairing P>
+__device__ __forceinline__ void put(char* at, long long half_bytes, const uint4& v) {
+  if (P != kSplit) {
+    __stcs(reinterpret_cast<uint4*>(at), v);
+  } else {
+    __stcs(reinterpret_cast<uint2*>(at), make_uint2(v.x, v.y));
+    __stcs(reinterpret_cast<uint2*>(at + half_bytes), make_uint2(v.z, v.w));
+  }
+}
+
+// A group walks `span` tokens in order and, for each, heads [h0, h0 + heads_per)
+// of its side.  DEPTH heads' loads are always in flight, over token boundaries
+// too.  The arithmetic runs on register pairs: with single floats this kernel
+// was bound by instructions, not memory.
+template <typename T, int G, int DEPTH, Pairing P, bool BWD>
 __global__ void __launch_bounds__(kRotThreads, BWD ? 2 : 3) vec_kernel(const __grid_constant__ Args a) {
-  constexpr int V = Vec<T>::V;
+  constexpr int V = Vec<T>::V, H = V / 2;
   constexpr int GROUPS = kRotThreads / G;
   const bool is_key = static_cast<int>(blockIdx.x) >= a.side[0].ctas;
   const Side& sd = a.side[is_key];
@@ -225,81 +326,110 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? 2 : 3) vec_kernel(const __g
   const int gl = threadIdx.x % G, group = threadIdx.x / G;
   const bool on = gl * V < a.dim;
   const int hv = a.half / V;
-  const int partner = gl < hv ? gl + hv : (gl < 2 * hv ? gl - hv : gl);
+  const int partner = gl < hv ? gl + hv : (gl < 2 * hv ? gl - hv : gl);  // kPart
   check_cu(a);
   const long long g = static_cast<long long>(cta) * GROUPS + group;
-  const int slice = static_cast<int>(g % sd.slices);
-  const int h0 = slice * sd.heads_per, h1 = min(h0 + sd.heads_per, sd.heads);
+  const int h0 = static_cast<int>(g % sd.slices) * sd.heads_per, heads = min(sd.heads_per, sd.heads - h0);
   const long long first = g / sd.slices * sd.span;
-  const long long tokens = max(0ll, min(static_cast<long long>(sd.span), a.tokens - first));
+  const int tokens = static_cast<int>(max(0ll, min(sd.span, a.tokens - first)));
   // every group of a warp runs the same number of rounds: the shuffles need them
   const int items = static_cast<int>(sd.span) * sd.heads_per;
-  float w[V], dw[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    w[i] = BWD && on ? load_any(sd.w, a.wtype, gl * V + i) : 0.f;
-    dw[i] = 0.f;
-  }
   const float inv = 1.f / static_cast<float>(a.dim);
-  const T* src = static_cast<const T*>(sd.x) + gl * V;
-  const T* dsrc = BWD ? static_cast<const T*>(sd.dy) + gl * V : nullptr;
+  constexpr int E = sizeof(T);
+  const long long half_bytes = static_cast<long long>(a.half) * E;
+  const int lane_bytes = gl * (P == kSplit ? 8 : 16);
+  // running addresses: next head, and from the last head to the next token
+  const char* src = static_cast<const char*>(sd.x) + (first * sd.st + h0 * sd.sh) * E + lane_bytes;
+  const char* dsrc = BWD ? static_cast<const char*>(sd.dy) + (first * sd.dst + h0 * sd.dsh) * E + lane_bytes : nullptr;
+  const long long hop = sd.sh * E, wrap = (sd.st - (sd.heads_per - 1) * sd.sh) * E;
+  const long long dhop = sd.dsh * E, dwrap = (sd.dst - (sd.heads_per - 1) * sd.dsh) * E;
+  char* dst = static_cast<char*>(sd.out) + (first * sd.heads + h0) * a.dim * E + lane_bytes;
+  const int out_hop = a.dim * E, out_wrap = (sd.heads - sd.heads_per + 1) * a.dim * E;
   uint4 raw[DEPTH], draw[BWD ? DEPTH : 1];
-  int lt = 0, lh = h0;  // the next load
+  int lt = 0, lh = 0;  // the next load
   auto load = [&](int q) {
-    const bool ok = on && lt < tokens && lh < h1;
-    raw[q] = ok ? __ldcs(reinterpret_cast<const uint4*>(src + (first + lt) * sd.st + lh * sd.sh)) : make_uint4(0, 0, 0, 0);
-    if (BWD) draw[q] = ok ? __ldcs(reinterpret_cast<const uint4*>(dsrc + (first + lt) * sd.dst + lh * sd.dsh)) : make_uint4(0, 0, 0, 0);
-    if (++lh >= h0 + sd.heads_per) lh = h0, ++lt;
+    raw[q] = make_uint4(0, 0, 0, 0);
+    if (BWD) draw[q] = make_uint4(0, 0, 0, 0);
+    if (on && lt < tokens && lh < heads) {
+      raw[q] = get<P>(src, half_bytes);
+      if (BWD) draw[q] = get<P>(dsrc, half_bytes);
+    }
+    const bool end = ++lh == sd.heads_per;
+    src += end ? wrap : hop;
+    if (BWD) dsrc += end ? dwrap : dhop;
+    if (end) lh = 0, ++lt;
   };
 #pragma unroll
   for (int q = 0; q < DEPTH; ++q) load(q);
-  Turn<T, BWD> turn;
+  Turn<T, P, BWD> turn;
   Place place;
-  long long row = -1;
-  int ct = 0, ch = h0;  // the next head to finish
+  long long row = tokens > 0 ? next_row(a, first, place) : -1;
+  __shared__ float weights[G * V];
+  for (int d = threadIdx.x; d < a.dim; d += kRotThreads) weights[d] = load_any(sd.w, a.wtype, d);
+  __syncthreads();
+  uint64_t w[BWD ? H : 1], dw[BWD ? H : 1];
+  if (BWD) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const int d = Turn<T, P, BWD>::element(a, gl, 2 * i);
+      w[i] = on ? pair(weights[d], weights[d + 1]) : 0;
+      dw[i] = 0;
+    }
+  }
+  int ct = 0, ch = 0;  // the next head to finish
   for (int r = 0; r < items; r += DEPTH) {
 #pragma unroll
     for (int q = 0; q < DEPTH; ++q) {
-      const long long t = first + ct;
-      const bool live = ct < tokens && ch < h1;
-      if (ch == h0) {
-        row = ct < tokens ? next_row(a, t, place) : -1;
-        turn.load(a, sd, row, gl, partner);
+      if (r + q >= items) break;
+      if (ch == 0) {
+        if (ct > 0) row = ct < tokens ? next_row(a, first + ct, place) : -1;
+        turn.load(a, weights, row, gl);
       }
-      float x[V], y[V], sq = 0.f;
+      const bool live = ct < tokens && ch < heads;
+      uint64_t x[H], y[H], acc;
       unpack<T>(raw[q], x);
+      acc = mul2(x[0], x[0]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) sq = fmaf(x[i], x[i], sq);
-      const float rs = rsqrtf(fmaf(group_sum<G>(sq), inv, a.eps));
+      for (int i = 1; i < H; ++i) acc = fma2(x[i], x[i], acc);
+      float2 s2 = unpair(acc);
+      const float rs = rsqrtf(fmaf(group_sum<G>(s2.x + s2.y), inv, a.eps));
+      const uint64_t rs2 = pair(rs, rs);
       if (!BWD) {
-        turn.template apply<G>(a, raw[q], partner, x, y);
+        turn.template apply<G>(raw[q], partner, x, y);
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = row >= 0 ? y[i] * rs : 0.f;
+        for (int i = 0; i < H; ++i) y[i] = mul2(y[i], rs2);
       } else {
-        float dy[V], dz[V], sum = 0.f;
+        uint64_t dy[H], dz[H];
         unpack<T>(draw[q], dy);
-        turn.template apply<G>(a, draw[q], partner, dy, dz);
+        turn.template apply<G>(draw[q], partner, dy, dz);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[i] *= rs;  // xh
-          const float gw = dz[i] * x[i];
-          if (live && row >= 0) dw[i] += gw;
-          sum = fmaf(gw, w[i], sum);
+        for (int i = 0; i < H; ++i) {
+          x[i] = mul2(x[i], rs2);  // xh
+          const uint64_t gw = mul2(dz[i], x[i]);
+          if (live && row >= 0) dw[i] = add2(dw[i], gw);
+          acc = i == 0 ? mul2(gw, w[i]) : fma2(gw, w[i], acc);
         }
-        const float mean = group_sum<G>(sum) * inv;
+        s2 = unpair(acc);
+        const float mean = -group_sum<G>(s2.x + s2.y) * inv;
+        const uint64_t mean2 = pair(mean, mean);
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = row >= 0 ? rs * fmaf(-x[i], mean, w[i] * dz[i]) : 0.f;
+        for (int i = 0; i < H; ++i) y[i] = mul2(rs2, fma2(x[i], mean2, mul2(w[i], dz[i])));
       }
       load(q);
-      if (live && on)
-        __stcs(reinterpret_cast<uint4*>(static_cast<T*>(sd.out) + (t * sd.heads + ch) * a.dim + gl * V), pack<T>(y));
-      if (++ch >= h0 + sd.heads_per) ch = h0, ++ct;
+      if (live && on) put<P>(dst, half_bytes, row >= 0 ? pack<T>(y) : make_uint4(0, 0, 0, 0));
+      const bool end = ++ch == sd.heads_per;
+      dst += end ? out_wrap : out_hop;
+      if (end) ch = 0, ++ct;
     }
   }
   if (BWD) {
     __shared__ float red[GROUPS][G * V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[group][gl * V + i] = dw[i];
+    for (int i = 0; i < H; ++i) {
+      const float2 e = unpair(dw[i]);
+      const int d = Turn<T, P, BWD>::element(a, gl, 2 * i);
+      if (on) red[group][d] = e.x, red[group][d + 1] = e.y;
+    }
     __syncthreads();
     for (int d = threadIdx.x; d < a.dim; d += kRotThreads) {
       float x = 0.f;
@@ -452,10 +582,18 @@ static int run(Args& a, bool vec, cudaStream_t s) {
     const int g = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32);
     split_groups(a, kRotThreads / g, BWD ? 2 : 3);
     const unsigned grid = a.side[0].ctas + a.side[1].ctas;
+    const Pairing pairing = a.interleaved ? kAdjacent : (2 * a.half == a.dim ? kSplit : kPart);
     constexpr int D = BWD ? 2 : 4;
-    if (g == 8) vec_kernel<T, 8, D, BWD><<<grid, kRotThreads, 0, s>>>(a);
-    else if (g == 16) vec_kernel<T, 16, D, BWD><<<grid, kRotThreads, 0, s>>>(a);
-    else vec_kernel<T, 32, D, BWD><<<grid, kRotThreads, 0, s>>>(a);
+#define ROT_LAUNCH(GG, PP) vec_kernel<T, GG, D, PP, BWD><<<grid, kRotThreads, 0, s>>>(a)
+#define ROT_CASE(GG)                                \
+  if (pairing == kSplit) ROT_LAUNCH(GG, kSplit);    \
+  else if (pairing == kAdjacent) ROT_LAUNCH(GG, kAdjacent); \
+  else ROT_LAUNCH(GG, kPart)
+    if (g == 8) { ROT_CASE(8); }
+    else if (g == 16) { ROT_CASE(16); }
+    else { ROT_CASE(32); }
+#undef ROT_CASE
+#undef ROT_LAUNCH
   } else {
     split(a, kRotThreads / 32);
     any_kernel<T, BWD><<<a.side[0].ctas + a.side[1].ctas, kRotThreads, 0, s>>>(a);
