@@ -425,15 +425,15 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) {
       bar_init(&t.full[i], 1);
-      bar_init(&t.empty[i], i < 2 ? (state_only ? 5 : 9) : (i < 4 ? 1 : 5));  // the products, and the row or column warps
+      bar_init(&t.empty[i], i < 2 ? 9 : (i < 4 ? 1 : 5));  // the products, and the row or column warps
     }
     bar_init(&t.tab_full, 1);
-    bar_init(&t.tab_empty, state_only ? 8 : 16);
+    bar_init(&t.tab_empty, state_only ? 12 : 16);
     bar_init(&t.sc_full, 1);
     bar_init(&t.in_full, 1);
     bar_init(&t.p_ready, 8);
-    bar_init(&t.kt_ready[0], 4);
-    bar_init(&t.kt_ready[1], 4);
+    bar_init(&t.kt_ready[0], state_only ? 8 : 4);
+    bar_init(&t.kt_ready[1], state_only ? 8 : 4);
     bar_init(&t.u_full[0], 1);
     bar_init(&t.u_full[1], 1);
     bar_init(&t.s_ready, 4);
@@ -465,6 +465,117 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   auto phase_of_b = [&](uint32_t it) { return state_only || geo.b_slots == 2 ? (it >> 1) & 1 : it & 1; };
   Walk<REV, STATE> w(p);
 
+  // The column role.  Without rows the first four row warps take it too, and
+  // each four build one half of the chunk's operand.
+  auto columns = [&](int part) {
+    constexpr int span = state_only ? kC / 2 : kC;
+    const int i = (warp & 3) * 32 + lane;
+    const bool work = i < blocks_a * 64;
+    // The warp's 32 rows of (col.B)^T: matrix m of a load has rows 8 m.. and 8
+    // tokens; lane r of it points at token r's 16 bytes.
+    const int lead = (i >> 6) * 16384 + (lane & 7) * 128 + ((((i & 32) >> 3) + (lane >> 3) ^ (lane & 7)) << 4);
+    for (uint32_t it = 0; w.next(); ++it) {
+      const uint32_t ph = it & 1;
+      const int slot_b = slot_of_b(it), slot_c = 2 + ph;
+      const unsigned char* bt = slot_at(slot_b);
+      unsigned char* ct = slot_at(slot_c);
+      // An update is done: its operand may be overwritten.  The previous one's,
+      // when outputs are computed, which also shows that the row and state
+      // warps have read what bad[ph] held two chunks ago; else the one before,
+      // since the scores' place holds a second operand.
+      const uint32_t before = state_only ? 2 : 1;
+      if (it >= before) {
+        if (!ctl.warp_wait(&t.u_full[(it - before) & 1], ((it - before) >> 1) & 1)) break;
+        fence_after();
+      }
+      const uint32_t kt = tm + lanes + (state_only && ph ? kColSc : kColK);
+      if (!state_only || w.len < kC)
+        if (!ctl.warp_wait(&t.full[slot_c], (it >> 1) & 1)) break;
+      if (state_only) {
+        if (i >= w.len && part == 0)  // another sequence's token, or past the end
+          for (int q = 0; q < 8 * blocks_c; ++q) *reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + ((q & 7) << 4)) = make_uint4(0, 0, 0, 0);
+      } else {  // one token row of C per thread
+        const bool live = i < w.len;
+        const __nv_bfloat162 none = __float2bfloat162_rn(0.f);
+        __nv_bfloat162 sum = none;  // sum of 0 * x: NaN if any x is not finite
+#pragma unroll 2
+        for (int q = 0; q < 8 * blocks_c; ++q) {
+          uint4* at = reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + (((q & 7) ^ (i & 7)) << 4));
+          if (live) {
+            const uint4 x = *at;
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), none, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), none, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), none, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), none, sum);
+          } else {
+            *at = make_uint4(0, 0, 0, 0);  // another sequence's token, or past the end
+          }
+        }
+        const bool bad = !(__low2float(sum) == 0.f && __high2float(sum) == 0.f);
+        if (bad) {  // note and clear
+          for (int d = 0; d < blocks_c * 64; ++d) {
+            uint16_t* at = reinterpret_cast<uint16_t*>(ct + (d >> 6) * 16384 + i * 128 + ((((d & 63) >> 3) ^ (i & 7)) << 4) + (d & 7) * 2);
+            if ((*at & 0x7f80u) == 0x7f80u) {
+              *at = 0;
+              atomicMax(&t.bad[ph][d], ((it + 1) << 8) | static_cast<uint32_t>(rev ? i : kC - 1 - i));
+            }
+          }
+          t.bad_chunk[ph] = static_cast<int>(it) + 1;
+        }
+      }
+      fence_async();
+      if (!ctl.warp_wait(&t.tab_full, ph)) break;
+      if (!ctl.warp_wait(&t.full[slot_b], phase_of_b(it))) break;
+      if (work) {
+        const uint32_t src = smem_u32(bt) + lead;
+        const bool tail = w.len < kC;
+#pragma unroll 1
+        for (int s0 = part * span; s0 < part * span + span; s0 += 16) {
+          uint32_t hi[8], lo[8];  // [half of the rows][8 tokens][rows 0-7, 8-15]
+          const float fb = t.far[s0 >> 5];
+          const uint64_t fb2 = pair(fb, fb);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            uint32_t r[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                         : "r"(src + (s0 + 8 * g) * 128)
+                         : "memory");
+            const int s = s0 + 8 * g + 2 * (lane & 3);
+            const float2 cf = *reinterpret_cast<const float2*>(&t.col[s]);
+            if (tail) {  // select, not multiply: the rows there are another sequence's
+              const uint32_t keep = (s < w.len ? 0xffffu : 0u) | (s + 1 < w.len ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int m = 0; m < 4; ++m) r[m] &= keep;
+            }
+            const uint64_t cf2 = mul2(pair(cf.x, cf.y), fb2);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), cf2);
+              const int at = (m >> 1) * 4 + g * 2 + (m & 1);
+              hi[at] = round2(x);
+              lo[at] = rest2(x, hi[at]);
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t to = kt + (static_cast<uint32_t>(m) << 20) + s0 / 2;
+            tmem_st16x128(to, hi + 4 * m);
+            tmem_st16x128(to + 64, lo + 4 * m);
+          }
+        }
+        wait_st();
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        bar_arrive(&t.kt_ready[ph]);
+        bar_arrive(&t.tab_empty);
+        bar_arrive(&t.empty[slot_b]);
+      }
+    }
+  };
+
   if (warp < 8) {
     // ---- row warps ----
     const int quad = warp & 3, side = warp >> 2, row = quad * 32 + lane;
@@ -485,6 +596,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       held = -1;
     };
+    if (state_only && warp < 4) columns(0);
     for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
       const int slot_a = ph;
@@ -777,112 +889,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
     }
   } else if (warp < 16) {
-    // ---- column warps ----
-    const int i = tid - 384;
-    const bool work = i < blocks_a * 64;
-    // The warp's 32 rows of (col.B)^T: matrix m of a load has rows 8 m.. and 8
-    // tokens; lane r of it points at token r's 16 bytes.
-    const int lead = (i >> 6) * 16384 + (lane & 7) * 128 + ((((i & 32) >> 3) + (lane >> 3) ^ (lane & 7)) << 4);
-    for (uint32_t it = 0; w.next(); ++it) {
-      const uint32_t ph = it & 1;
-      const int slot_b = slot_of_b(it), slot_c = 2 + ph;
-      const unsigned char* bt = slot_at(slot_b);
-      unsigned char* ct = slot_at(slot_c);
-      // An update is done: its operand may be overwritten.  The previous one's,
-      // when outputs are computed, which also shows that the row and state
-      // warps have read what bad[ph] held two chunks ago; else the one before,
-      // since the scores' place holds a second operand.
-      const uint32_t before = state_only ? 2 : 1;
-      if (it >= before) {
-        if (!ctl.warp_wait(&t.u_full[(it - before) & 1], ((it - before) >> 1) & 1)) break;
-        fence_after();
-      }
-      const uint32_t kt = tm + lanes + (state_only && ph ? kColSc : kColK);
-      if (!state_only || w.len < kC)
-        if (!ctl.warp_wait(&t.full[slot_c], (it >> 1) & 1)) break;
-      if (state_only) {
-        if (i >= w.len)  // another sequence's token, or past the end
-          for (int q = 0; q < 8 * blocks_c; ++q) *reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + ((q & 7) << 4)) = make_uint4(0, 0, 0, 0);
-      } else {  // one token row of C per thread
-        const bool live = i < w.len;
-        const __nv_bfloat162 none = __float2bfloat162_rn(0.f);
-        __nv_bfloat162 sum = none;  // sum of 0 * x: NaN if any x is not finite
-#pragma unroll 2
-        for (int q = 0; q < 8 * blocks_c; ++q) {
-          uint4* at = reinterpret_cast<uint4*>(ct + (q >> 3) * 16384 + i * 128 + (((q & 7) ^ (i & 7)) << 4));
-          if (live) {
-            const uint4 x = *at;
-            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), none, sum);
-            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), none, sum);
-            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), none, sum);
-            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), none, sum);
-          } else {
-            *at = make_uint4(0, 0, 0, 0);  // another sequence's token, or past the end
-          }
-        }
-        const bool bad = !(__low2float(sum) == 0.f && __high2float(sum) == 0.f);
-        if (bad) {  // note and clear
-          for (int d = 0; d < blocks_c * 64; ++d) {
-            uint16_t* at = reinterpret_cast<uint16_t*>(ct + (d >> 6) * 16384 + i * 128 + ((((d & 63) >> 3) ^ (i & 7)) << 4) + (d & 7) * 2);
-            if ((*at & 0x7f80u) == 0x7f80u) {
-              *at = 0;
-              atomicMax(&t.bad[ph][d], ((it + 1) << 8) | static_cast<uint32_t>(rev ? i : kC - 1 - i));
-            }
-          }
-          t.bad_chunk[ph] = static_cast<int>(it) + 1;
-        }
-      }
-      fence_async();
-      if (!ctl.warp_wait(&t.tab_full, ph)) break;
-      if (!ctl.warp_wait(&t.full[slot_b], phase_of_b(it))) break;
-      if (work) {
-        const uint32_t src = smem_u32(bt) + lead;
-        const bool tail = w.len < kC;
-#pragma unroll 1
-        for (int s0 = 0; s0 < kC; s0 += 16) {
-          uint32_t hi[8], lo[8];  // [half of the rows][8 tokens][rows 0-7, 8-15]
-          const float fb = t.far[s0 >> 5];
-          const uint64_t fb2 = pair(fb, fb);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint32_t r[4];
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                         : "r"(src + (s0 + 8 * g) * 128)
-                         : "memory");
-            const int s = s0 + 8 * g + 2 * (lane & 3);
-            const float2 cf = *reinterpret_cast<const float2*>(&t.col[s]);
-            if (tail) {  // select, not multiply: the rows there are another sequence's
-              const uint32_t keep = (s < w.len ? 0xffffu : 0u) | (s + 1 < w.len ? 0xffff0000u : 0u);
-#pragma unroll
-              for (int m = 0; m < 4; ++m) r[m] &= keep;
-            }
-            const uint64_t cf2 = mul2(pair(cf.x, cf.y), fb2);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), cf2);
-              const int at = (m >> 1) * 4 + g * 2 + (m & 1);
-              hi[at] = round2(x);
-              lo[at] = rest2(x, hi[at]);
-            }
-          }
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const uint32_t to = kt + (static_cast<uint32_t>(m) << 20) + s0 / 2;
-            tmem_st16x128(to, hi + 4 * m);
-            tmem_st16x128(to + 64, lo + 4 * m);
-          }
-        }
-        wait_st();
-      }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        bar_arrive(&t.kt_ready[ph]);
-        bar_arrive(&t.tab_empty);
-        bar_arrive(&t.empty[slot_b]);
-      }
-    }
+    columns(state_only ? 1 : 0);
   } else if (warp == 16) {
     // ---- loads: what comes free first is asked for first ----
     if (lane == 0) {
