@@ -425,7 +425,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) {
       bar_init(&t.full[i], 1);
-      bar_init(&t.empty[i], i < 2 ? 9 : (i < 4 ? 1 : 5));  // the products, and the row or column warps
+      bar_init(&t.empty[i], i < 2 ? (state_only ? 8 : 9) : (i < 4 ? 1 : 5));  // the products, and the row or column warps
     }
     bar_init(&t.tab_full, 1);
     bar_init(&t.tab_empty, state_only ? 12 : 16);
@@ -980,10 +980,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         for (int k = 0; k < 2 * kC / 16; ++k)  // both terms lie side by side
           mma_tmem(tm + kColU, kt + k * 8, c + (k & 7) * 128, id_v, true);
         commit(&t.u_full[ph]);
-        if (state_only) {
-          commit(&t.empty[sb]);
-          commit(&t.empty[sc]);
-        }
+        if (state_only) commit(&t.empty[sc]);
       }
       if (!state_only) {
         if (!ctl.warp_wait(&t.p_ready, ph)) break;
