@@ -576,3 +576,21 @@ def test_step_pool_beyond_32_bit_offsets():
   out = ast.matrix_scan_step(q, k, v, g, pool, slots=slots)
   close("out", out, want, 1e-5)
   close("state", pool[slots.long()], new, 1e-6)
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+
+
+@gpu
+def test_example_trains_and_decodes(capsys):
+  import importlib.util
+
+  from conftest import REPO
+  spec = importlib.util.spec_from_file_location("gla_example",
+                                                REPO / "examples" / "gated_linear_attention.py")
+  example = importlib.util.module_from_spec(spec)
+  spec.loader.exec_module(example)
+  assert example.main(["--steps", "12", "--dim", "128", "--heads", "2"]) == 0
+  assert "step by step" in capsys.readouterr().out
