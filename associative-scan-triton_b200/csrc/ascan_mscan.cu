@@ -10,48 +10,98 @@ namespace ascan {
 namespace mscan {
 
 constexpr int kPlainThreads = 256;
-constexpr int kPlainChunk = 32;
+constexpr int kPlainChunk = 64;
 
 // ---------------------------------------------------------------------------
-// The plain kernel: one CTA per (segment, head, form), fused multiply-adds.
-// The state stays in shared memory from chunk to chunk; a chunk of 32 tokens
-// costs 32*(da*dc) products with the state for the outputs, as many for its
-// update and 32*32*(da + dc) for the scores and values, so it is bound by
-// fused multiply-adds and shared-memory reads.  It serves float32, float16
-// and whatever the tensor-core kernel does not take.
+// The plain kernel: one CTA per (segment, head, form), float32 fused
+// multiply-adds, for float32, float16 and what the tensor-core kernel does not
+// take.  A chunk of 64 tokens lies in shared memory, A and B with the tokens
+// along the rows' unit stride, C as stored; the state stays there from chunk
+// to chunk.  Every product gives a thread a tile of 4 x 4 values (8 x 4 at 128
+// wide), so two (three) 16-byte reads feed 16 (32) multiply-adds.
 // ---------------------------------------------------------------------------
 
 template <int DM>
 struct PlainSmem {
-  static constexpr int kLd = DM + 4;
+  static constexpr int kLt = kPlainChunk + 4, kLd = DM + 4;
   float s[DM * DM];
-  float a[kPlainChunk * kLd];
-  float b[kPlainChunk * kLd];
-  float c[kPlainChunk * kLd];
-  float p[kPlainChunk * (kPlainChunk + 1)];
+  float at[DM * kLt];  // [dim][token]
+  float bt[DM * kLt];
+  float c[kPlainChunk * kLd];            // [token][dim]
+  float pt[kPlainChunk * kLt];           // [column token][row token]
   double g[kPlainChunk];
   float row[kPlainChunk], col[kPlainChunk];
   float total;
 };
 
-template <typename T, int LD, int DM>
-__device__ __forceinline__ void load_rows(float* dst, const Rows& r, long long t0, int len, int h, int dim) {
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+
+// acc += x (a row of four values)
+__device__ __forceinline__ void fma4(float* acc, float x, const float4& y) {
+  acc[0] = fmaf(x, y.x, acc[0]);
+  acc[1] = fmaf(x, y.y, acc[1]);
+  acc[2] = fmaf(x, y.z, acc[2]);
+  acc[3] = fmaf(x, y.w, acc[3]);
+}
+
+// Four elements of a row, zero beyond dim.
+template <typename T>
+__device__ __forceinline__ float4 row4(const T* p, int d, int dim, bool vec) {
+  if (vec && d + 4 <= dim) {
+    if (sizeof(T) == 4) return *reinterpret_cast<const float4*>(p + d);
+    const uint2 u = *reinterpret_cast<const uint2*>(p + d);
+    const T* e = reinterpret_cast<const T*>(&u);
+    return make_float4(to_f(e[0]), to_f(e[1]), to_f(e[2]), to_f(e[3]));
+  }
+  return make_float4(d < dim ? to_f(p[d]) : 0.f, d + 1 < dim ? to_f(p[d + 1]) : 0.f, d + 2 < dim ? to_f(p[d + 2]) : 0.f,
+                     d + 3 < dim ? to_f(p[d + 3]) : 0.f);
+}
+
+template <typename T>
+__device__ __forceinline__ bool rows_aligned(const Rows& r) {
+  return (reinterpret_cast<uintptr_t>(r.p) % (4 * sizeof(T))) == 0 && r.st % 4 == 0 && r.sh % 4 == 0;
+}
+
+// Tokens along the unit stride: a lane takes one token, so the stores spread
+// over the banks.
+template <typename T, int DM>
+__device__ __forceinline__ void load_turned(float* dst, const Rows& r, long long t0, int len, int h, int dim) {
+  constexpr int LT = PlainSmem<DM>::kLt, THREADS = kPlainThreads;
+  const bool vec = rows_aligned<T>(r);
   const T* base = static_cast<const T*>(r.p) + t0 * r.st + (h / r.share) * r.sh;
-  for (int e = threadIdx.x; e < kPlainChunk * DM; e += kPlainThreads) {
-    const int i = e / DM, d = e % DM;
-    dst[i * LD + d] = (i < len && d < dim) ? to_f(base[i * r.st + d]) : 0.f;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < kPlainChunk * DM / 4; e += THREADS) {
+    const int t = e % kPlainChunk, d = e / kPlainChunk * 4;
+    const float4 x = t < len ? row4(base + t * r.st, d, dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    dst[d * LT + t] = x.x;
+    dst[(d + 1) * LT + t] = x.y;
+    dst[(d + 2) * LT + t] = x.z;
+    dst[(d + 3) * LT + t] = x.w;
   }
 }
 
 template <typename T, int DM>
-__global__ void __launch_bounds__(kPlainThreads)
+__device__ __forceinline__ void load_rows(float* dst, const Rows& r, long long t0, int len, int h, int dim) {
+  constexpr int LD = PlainSmem<DM>::kLd, THREADS = kPlainThreads;
+  const bool vec = rows_aligned<T>(r);
+  const T* base = static_cast<const T*>(r.p) + t0 * r.st + (h / r.share) * r.sh;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < kPlainChunk * DM / 4; e += THREADS) {
+    const int t = e / (DM / 4), d = e % (DM / 4) * 4;
+    *reinterpret_cast<float4*>(dst + t * LD + d) =
+        t < len ? row4(base + t * r.st, d, dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
+template <typename T, int DM>
+__global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 2 : 1)
     plain_kernel(const __grid_constant__ Launch L, const bool state_only) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   using Sm = PlainSmem<DM>;
   Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
-  constexpr int LD = Sm::kLd;
-  constexpr int TX = DM / 4;                              // threads along the values
-  constexpr int RPT = kPlainChunk / (kPlainThreads / TX);  // rows per thread
+  constexpr int LT = Sm::kLt, LD = Sm::kLd, THREADS = kPlainThreads;
+  constexpr int TX = DM / 4;             // threads along the values, four each
+  constexpr int R = TX * kPlainChunk / THREADS;  // rows per thread: 4 or 8
   const Problem& p = L.p;
   const Form& f = L.f[blockIdx.z];
   const int tid = threadIdx.x, j = blockIdx.x, h = blockIdx.y;
@@ -59,6 +109,7 @@ __global__ void __launch_bounds__(kPlainThreads)
   const int da = f.da, dc = f.dc;
   const long long mat = static_cast<long long>(da) * dc;
   const long long t0 = j * p.seg, t1 = min(t0 + p.seg, p.BL);
+  const int tx = tid % TX, ty = tid / TX, d0 = tx * 4, r0 = ty * R;
 
   if (!state_only) fill_outside<T>(p, f);
 
@@ -76,7 +127,7 @@ __global__ void __launch_bounds__(kPlainThreads)
                                    : f.carry + (static_cast<long long>(rev ? j + 1 : j - 1) * p.H + h) * mat;
     const bool zero = from == nullptr || (state_only && !from_start);
     const long long fi = from_start ? f.si : dc, fj = from_start ? f.sj : 1;
-    for (int e = tid; e < DM * DM; e += kPlainThreads) {
+    for (int e = tid; e < DM * DM; e += THREADS) {
       const int i = e / DM, d = e % DM;
       sm.s[e] = (!zero && i < da && d < dc) ? from[i * fi + d * fj] : 0.f;
     }
@@ -88,95 +139,114 @@ __global__ void __launch_bounds__(kPlainThreads)
       __syncthreads();
       if (f.snap && !state_only) {
         const long long at = rev ? s0 + len : s0;
-        if (at > ps && at < pe && (at - ps) % kRestart == 0)
-          for (int e = tid; e < mat; e += kPlainThreads)
-            f.snap[(snap_slot(at) * p.H + h) * mat + e] = sm.s[(e / dc) * DM + e % dc];
+        if (at > ps && at < pe && (at - ps) % p.restart == 0)
+          for (int e = tid; e < mat; e += THREADS)
+            f.snap[(snap_slot(p, at) * p.H + h) * mat + e] = sm.s[(e / dc) * DM + e % dc];
       }
-      if (!state_only) load_rows<T, LD, DM>(sm.a, f.a, s0, len, h, da);
-      load_rows<T, LD, DM>(sm.b, f.b, s0, len, h, da);
-      load_rows<T, LD, DM>(sm.c, f.c, s0, len, h, dc);
+      if (!state_only) load_turned<T, DM>(sm.at, f.a, s0, len, h, da);
+      load_turned<T, DM>(sm.bt, f.b, s0, len, h, da);
+      load_rows<T, DM>(sm.c, f.c, s0, len, h, dc);
       if (tid < 32) {
-        double g = tid < len ? static_cast<double>(load_gate(p, s0 + tid, h)) : 0.0;
+        const double g0 = 2 * tid < len ? static_cast<double>(load_gate(p, s0 + 2 * tid, h)) : 0.0;
+        const double g1 = 2 * tid + 1 < len ? static_cast<double>(load_gate(p, s0 + 2 * tid + 1, h)) : 0.0;
+        double inc = g0 + g1;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-          const double up = __shfl_up_sync(kFull, g, o);
-          if (tid >= o) g += up;
+          const double u = __shfl_up_sync(kFull, inc, o);
+          if (tid >= o) inc += u;
         }
-        const double end = __shfl_sync(kFull, g, 31);
-        const float head = expf(static_cast<float>(g)), tail = expf(static_cast<float>(end - g));
-        sm.g[tid] = g;
-        sm.row[tid] = (rev ? tail : head) * f.sr;
-        sm.col[tid] = (rev ? head : tail) * f.sc;
-        if (tid == 31) sm.total = head;
+        const double end = __shfl_sync(kFull, inc, 31);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const double g = q ? inc : inc - g1;
+          const float head = expf(static_cast<float>(g)), tail = expf(static_cast<float>(end - g));
+          sm.g[2 * tid + q] = g;
+          sm.row[2 * tid + q] = (rev ? tail : head) * f.sr;
+          sm.col[2 * tid + q] = (rev ? head : tail) * f.sc;
+        }
+        if (tid == 31) sm.total = expf(static_cast<float>(end));
       }
       __syncthreads();
       if (!state_only) {
-        {  // scores: 4 columns of one row per thread
-          const int r = tid / 8, c0 = tid % 8;
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int d = 0; d < da; d += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&sm.a[r * LD + d]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float4 y = *reinterpret_cast<const float4*>(&sm.b[(c0 + 8 * q) * LD + d]);
-              acc[q] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, acc[q]))));
+        {  // scores: 4 rows by 4 columns; blocks outside the mask are zero
+          const int sr0 = (tid / 16) * 4, sc0 = (tid % 16) * 4;
+          float acc[4][4] = {};
+          if (rev ? sc0 + 3 >= sr0 : sc0 <= sr0 + 3) {
+#pragma unroll 4
+            for (int d = 0; d < da; ++d) {
+              const float4 y = ld4(&sm.bt[d * LT + sc0]);
+              const float4 x = ld4(&sm.at[d * LT + sr0]);
+              fma4(acc[0], x.x, y);
+              fma4(acc[1], x.y, y);
+              fma4(acc[2], x.z, y);
+              fma4(acc[3], x.w, y);
             }
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = c0 + 8 * q;
-            const bool on = (rev ? c >= r : c <= r) && c < len;
-            const double dg = rev ? sm.g[c] - sm.g[r] : sm.g[r] - sm.g[c];
-            sm.p[r * (kPlainChunk + 1) + c] = on ? acc[q] * f.sp * expf(static_cast<float>(dg)) : 0.f;
+          for (int c = 0; c < 4; ++c) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = sr0 + e, at = sc0 + c;
+              const bool on = (rev ? at >= r : at <= r) && at < len;
+              const double dg = rev ? sm.g[at] - sm.g[r] : sm.g[r] - sm.g[at];
+              v[e] = on ? acc[e][c] * f.sp * expf(static_cast<float>(dg)) : 0.f;
+            }
+            *reinterpret_cast<float4*>(&sm.pt[(sc0 + c) * LT + sr0]) = make_float4(v[0], v[1], v[2], v[3]);
           }
         }
-        __syncthreads();
-        const int tx = tid % TX, r0 = (tid / TX) * RPT;
-        float acc[RPT][4] = {};
-        for (int i = 0; i < da; ++i) {
-          const float4 y = *reinterpret_cast<const float4*>(&sm.s[i * DM + tx * 4]);
+        float acc[R][4] = {};
+        // acc += (R values of a row of x) times (four values of y)
+        auto outer = [&](const float* x, const float4& y) {
 #pragma unroll
-          for (int r = 0; r < RPT; ++r) {
-            const float x = sm.a[(r0 + r) * LD + i];
-            acc[r][0] = fmaf(x, y.x, acc[r][0]);
-            acc[r][1] = fmaf(x, y.y, acc[r][1]);
-            acc[r][2] = fmaf(x, y.z, acc[r][2]);
-            acc[r][3] = fmaf(x, y.w, acc[r][3]);
+          for (int q = 0; q < R; q += 4) {
+            const float4 v = ld4(x + q);
+            fma4(acc[q], v.x, y), fma4(acc[q + 1], v.y, y), fma4(acc[q + 2], v.z, y), fma4(acc[q + 3], v.w, y);
           }
-        }
+        };
+#pragma unroll 4
+        for (int i = 0; i < da; ++i) outer(&sm.at[i * LT + r0], ld4(&sm.s[i * DM + d0]));
 #pragma unroll
-        for (int r = 0; r < RPT; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[r][q] *= sm.row[r0 + r];
-        for (int c = 0; c < len; ++c) {
-          const float4 y = *reinterpret_cast<const float4*>(&sm.c[c * LD + tx * 4]);
+        __syncthreads();
+        // columns before (after) the thread's rows meet all of them
+        const int c_from = rev ? r0 + R : 0, c_to = rev ? len : min(r0, len);
+#pragma unroll 4
+        for (int c = c_from; c < c_to; ++c) outer(&sm.pt[c * LT + r0], ld4(&sm.c[c * LD + d0]));
+        // the columns of the rows themselves: masked ones are left out, not
+        // multiplied by zero, so that a NaN there reaches no row
 #pragma unroll
-          for (int r = 0; r < RPT; ++r) {
-            // masked tokens are left out, not multiplied by zero: a NaN or
-            // infinity there must not reach this row
-            if (rev ? c < r0 + r : c > r0 + r) continue;
-            const float x = sm.p[(r0 + r) * (kPlainChunk + 1) + c];
-            acc[r][0] = fmaf(x, y.x, acc[r][0]);
-            acc[r][1] = fmaf(x, y.y, acc[r][1]);
-            acc[r][2] = fmaf(x, y.z, acc[r][2]);
-            acc[r][3] = fmaf(x, y.w, acc[r][3]);
-          }
+        for (int q = 0; q < R; ++q) {
+          if (r0 + q >= len) continue;
+          const float4 y = ld4(&sm.c[(r0 + q) * LD + d0]);
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (rev ? q >= r : q <= r) fma4(acc[r], sm.pt[(r0 + q) * LT + r0 + r], y);
         }
+        const bool vec = dc % 4 == 0 && (reinterpret_cast<uintptr_t>(f.out) & 15u) == 0;
 #pragma unroll
-        for (int r = 0; r < RPT; ++r) {
+        for (int r = 0; r < R; ++r) {
           const bool on = r0 + r < len;
-          const long long t = s0 + r0 + r;
+          const long long t = s0 + r0 + r, at = (t * p.H + h) * dc + d0;
           float dot = 0.f;
+          if (on && d0 < dc) {
+            if (vec && (f.out_f32 || sizeof(T) == 4)) {
+              *reinterpret_cast<float4*>(static_cast<float*>(f.out) + at) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+            } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int d = tx * 4 + q;
-            if (on && d < dc) {
-              const long long at = (t * p.H + h) * dc + d;
-              if (f.out_f32) static_cast<float*>(f.out)[at] = acc[r][q];
-              else static_cast<T*>(f.out)[at] = from_f<T>(acc[r][q]);
-              if (f.rowdot)
-                dot = fmaf(acc[r][q],
-                           to_f(static_cast<const T*>(f.dot.p)[t * f.dot.st + (h / f.dot.share) * f.dot.sh + d]), dot);
+              for (int q = 0; q < 4; ++q)
+                if (d0 + q < dc) {
+                  if (f.out_f32) static_cast<float*>(f.out)[at + q] = acc[r][q];
+                  else static_cast<T*>(f.out)[at + q] = from_f<T>(acc[r][q]);
+                }
+            }
+            if (f.rowdot) {
+              const T* x = static_cast<const T*>(f.dot.p) + t * f.dot.st + (h / f.dot.share) * f.dot.sh;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (d0 + q < dc) dot = fmaf(acc[r][q], to_f(x[d0 + q]), dot);
             }
           }
           if (f.rowdot) {
@@ -185,51 +255,47 @@ __global__ void __launch_bounds__(kPlainThreads)
             if (on && tx == 0) f.rowdot[h * p.BL + t] = dot;
           }
         }
-        __syncthreads();
       }
-      // state: a (DM/16)^2 tile per thread, columns in quads 64 apart
-      {
-        constexpr int R = DM / 16, Q = DM / 64;
-        const int i0 = (tid / 16) * R, d0 = (tid % 16) * 4;
-        float st[R][Q * 4] = {};
-        for (int c = 0; c < len; ++c) {
-          float x[R];
+      {  // the update: R rows a pass, four tokens a step
+        const float total = sm.total;
+        decay *= total;
+        if (!state_only) __syncthreads();  // every thread has read the old state
+        for (int i0 = ty * R; i0 < DM; i0 += kPlainChunk) {
+          float st[R][4] = {};
+#pragma unroll 2
+          for (int c = 0; c < len; c += 4) {  // rows past the end are zero in both operands
+            const float4 k = ld4(&sm.col[c]);
+            float4 y[4];
 #pragma unroll
-          for (int r = 0; r < R; ++r) x[r] = sm.b[c * LD + i0 + r] * sm.col[c];
-#pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            const float4 y = *reinterpret_cast<const float4*>(&sm.c[c * LD + d0 + 64 * q]);
+            for (int q = 0; q < 4; ++q) y[q] = ld4(&sm.c[(c + q) * LD + d0]);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-              st[r][q * 4 + 0] = fmaf(x[r], y.x, st[r][q * 4 + 0]);
-              st[r][q * 4 + 1] = fmaf(x[r], y.y, st[r][q * 4 + 1]);
-              st[r][q * 4 + 2] = fmaf(x[r], y.z, st[r][q * 4 + 2]);
-              st[r][q * 4 + 3] = fmaf(x[r], y.w, st[r][q * 4 + 3]);
+              const float4 x = ld4(&sm.bt[(i0 + r) * LT + c]);
+              fma4(st[r], x.x * k.x, y[0]);
+              fma4(st[r], x.y * k.y, y[1]);
+              fma4(st[r], x.z * k.z, y[2]);
+              fma4(st[r], x.w * k.w, y[3]);
             }
           }
-        }
-        const float total = sm.total;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            float4* at = reinterpret_cast<float4*>(&sm.s[(i0 + r) * DM + d0 + 64 * q]);
-            const float4 o = *at;
-            *at = make_float4(fmaf(total, o.x, st[r][q * 4 + 0]), fmaf(total, o.y, st[r][q * 4 + 1]),
-                              fmaf(total, o.z, st[r][q * 4 + 2]), fmaf(total, o.w, st[r][q * 4 + 3]));
+          for (int r = 0; r < R; ++r) {
+            float4* to = reinterpret_cast<float4*>(&sm.s[(i0 + r) * DM + d0]);
+            const float4 o = *to;
+            *to = make_float4(fmaf(total, o.x, st[r][0]), fmaf(total, o.y, st[r][1]), fmaf(total, o.z, st[r][2]),
+                              fmaf(total, o.w, st[r][3]));
           }
-        decay *= total;
+        }
       }
     }
     __syncthreads();
     if (state_only) {
       float* to = f.carry + (static_cast<long long>(j) * p.H + h) * mat;
-      for (int e = tid; e < mat; e += kPlainThreads) to[e] = sm.s[(e / dc) * DM + e % dc];
+      for (int e = tid; e < mat; e += THREADS) to[e] = sm.s[(e / dc) * DM + e % dc];
       // a piece that holds the sequence's start takes nothing from before
       if (tid == 0) f.dec[j * p.H + h] = from_start ? -1.f : decay;
     } else if (to_end && f.fin) {
       float* to = f.fin + (n * p.H + h) * mat;
-      for (int e = tid; e < mat; e += kPlainThreads)
+      for (int e = tid; e < mat; e += THREADS)
         to[(e / dc) * f.si + (e % dc) * f.sj] = sm.s[(e / dc) * DM + e % dc];
     }
     __syncthreads();
@@ -278,7 +344,7 @@ __global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Laun
   }
 }
 
-// Gate gradients of one stretch of at most kRestart tokens: the product of
+// Gate gradients of one stretch of at most p.restart (256 or 1024) tokens: the product of
 // the two states at its end, then the reverse sum of q.dq - k.dk over it.
 // blockIdx.z takes every gridDim.z-th stretch of the segment.
 __global__ void __launch_bounds__(256)
@@ -305,13 +371,13 @@ __global__ void __launch_bounds__(256)
   for (long long n = first_beyond(p, t0); n < p.N && cu_at(p, n) < t1; ++n) {
     const long long b1 = cu_at(p, n + 1);
     const long long ps = max(cu_at(p, n), t0), pe = min(b1, t1);
-    for (long long s0 = ps; s0 < pe; s0 += kRestart, ++stretch) {
+    for (long long s0 = ps; s0 < pe; s0 += p.restart, ++stretch) {
       if (stretch % gridDim.z != blockIdx.z) continue;
-      const long long s1 = min(s0 + kRestart, pe);
+      const long long s1 = min(s0 + p.restart, pe);
       const float *x = nullptr, *y = nullptr;
       if (s1 < pe) {
-        x = fq.snap + (snap_slot(s1) * p.H + h) * mat;
-        y = fk.snap + (snap_slot(s1) * p.H + h) * mat;
+        x = fq.snap + (snap_slot(p, s1) * p.H + h) * mat;
+        y = fk.snap + (snap_slot(p, s1) * p.H + h) * mat;
       } else if (pe < b1) {
         x = fq.carry + (static_cast<long long>(j) * p.H + h) * mat;
         y = fk.carry + (static_cast<long long>(j + 1) * p.H + h) * mat;
@@ -320,8 +386,15 @@ __global__ void __launch_bounds__(256)
         y = d_final + (n * p.H + h) * mat;
       }
       float dot = 0.f;
-      if (x)
+      if (x && mat % 4 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0) {
+#pragma unroll 4
+        for (long long e = tid; e < mat / 4; e += 256) {
+          const float4 a = __ldcs(reinterpret_cast<const float4*>(x) + e), b = __ldcs(reinterpret_cast<const float4*>(y) + e);
+          dot = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, dot))));
+        }
+      } else if (x) {
         for (long long e = tid; e < mat; e += 256) dot = fmaf(x[e], y[e], dot);
+      }
       // four tokens a thread, latest first
       float v[4], sum = 0.f;
 #pragma unroll
@@ -521,6 +594,7 @@ static int plain_run(const Launch& l, int roles, bool state_only, int dtype, cud
 static int run_forms(Launch& l, int roles, int dtype, cudaStream_t s) {
   int rc = ASCAN_OK;
   const bool tc = tc_usable(l, roles, dtype);
+  l.p.restart = tc && l.p.gate_type != ASCAN_F32 ? kRestart : kRestartMin;
   for (int r = 0; r < roles; ++r) l.f[r].dot_parts = tc ? tc_dot_parts(l.f[r]) : 1;
   if (l.p.J > 1) {
     rc = tc ? tc_run(l, roles, true, s) : plain_run(l, roles, true, dtype, s);
@@ -550,7 +624,7 @@ static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, 
   w.J = (BL + w.seg - 1) / w.seg;
   const size_t mat = static_cast<size_t>(dk) * dv * H * 4;
   w.carry = w.J > 1 ? up(w.J * mat) + up(static_cast<size_t>(w.J) * H * 4) : 0;
-  w.slots = BL / kRestart + 1;
+  w.slots = BL / kRestartMin + 1;
   const size_t rows = static_cast<size_t>(BL) * H * 4;
   w.total = w.carry * (backward ? 3 : 1);
   if (backward) {
@@ -718,7 +792,7 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
   }
   rc = run_forms(l, 3, dtype, s);
   if (rc != ASCAN_OK) return rc;
-  gate_grad_kernel<<<dim3(l.p.J, H, static_cast<unsigned>(min(8ll, (w.seg + kRestart - 1) / kRestart))), 256, 0, s>>>(
+  gate_grad_kernel<<<dim3(l.p.J, H, static_cast<unsigned>(min(8ll, (w.seg + l.p.restart - 1) / l.p.restart))), 256, 0, s>>>(
       l, final_state, d_final_state, part_g, d_log_gates, gate_dtype);
   rc = launch_status();
   auto sum = [&](const float* part, void* out, int heads_x, int dim, int type) {

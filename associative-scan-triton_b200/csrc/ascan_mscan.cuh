@@ -23,7 +23,7 @@
 //
 //   dg[t] = sum_{u=t..e} (a[u] - b[u]) + <S[e], dS[e]>
 //
-// for any later token e of the sequence.  Taking e at most kRestart tokens
+// for any later token e of the sequence.  Taking e at most `restart` tokens
 // away (both state matrices are stored there) keeps the differences short;
 // one sum over a long sequence would lose the digits that the many terms
 // share.
@@ -46,7 +46,12 @@
 namespace ascan {
 namespace mscan {
 
-constexpr int kRestart = 1024;     // tokens between stored states (gate gradients)
+// Tokens between stored states.  A float32 gate gradient carries the rounding
+// of every row dot between them: with 1024 tokens 1.1e-5 of its norm on the
+// tensor cores (16-bit operand terms) and 1.3e-6 in float32 arithmetic, with
+// 256 half of that.  A 16-bit gradient needs no more than the longer stretch,
+// whose stores of up to 64 KB a head weigh less.
+constexpr int kRestart = 1024, kRestartMin = 256;
 constexpr float kGateFloor = -200.f;  // e^-200 is 0 in float32; keeps -inf out of differences
 
 struct Rows {  // [tokens, heads, dim] with unit stride along dim
@@ -76,6 +81,7 @@ struct Form {
 struct Problem {
   const void* cu;
   int cu64, J, H, gate_type;
+  int restart;  // tokens between stored states, set before the launch
   long long N, BL, seg;
   Rows gate;  // [BL, heads, 1]
   uint32_t* err;
@@ -146,9 +152,9 @@ __device__ __forceinline__ float load_gate(const Problem& p, long long t, int h)
 }
 
 // Slot of the state stored at token `at`: stored positions of one sequence
-// are kRestart apart and at least as far from those of the next, so the
+// are `restart` apart and at least as far from those of the next, so the
 // quotient is unique.
-__device__ __forceinline__ long long snap_slot(long long at) { return at / kRestart; }
+__device__ __forceinline__ long long snap_slot(const Problem& p, long long at) { return at / p.restart; }
 
 // The tensor-core kernel (ascan_mscan_tc.cu).
 bool tc_usable(const Launch& l, int roles, int dtype);

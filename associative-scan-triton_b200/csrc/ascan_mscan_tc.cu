@@ -354,8 +354,9 @@ struct Walk {
 };
 
 // Row i of a state between tensor memory and global memory, eight columns at
-// a time; `on` is false for lanes without a row.
-__device__ __noinline__ void put_state(uint32_t tm, float* to, long long sj, int dc, bool on) {
+// a time; `on` is false for lanes without a row.  With unit stride the eights
+// are `hop` floats apart.
+__device__ __noinline__ void put_state(uint32_t tm, float* to, int hop, long long sj, int dc, bool on) {
 #pragma unroll 1
   for (int d = 0; d < dc; d += 8) {
     uint32_t v[8];
@@ -363,8 +364,9 @@ __device__ __noinline__ void put_state(uint32_t tm, float* to, long long sj, int
     wait_ld();
     if (!on) continue;
     if (sj == 1) {
-      *reinterpret_cast<uint4*>(to + d) = make_uint4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<uint4*>(to + d + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+      *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<uint4*>(to + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+      to += hop;
     } else {
 #pragma unroll
       for (int q = 0; q < 8; ++q) to[(d + q) * sj] = __uint_as_float(v[q]);
@@ -838,8 +840,10 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       if (f.snap && !state_only && work) {
         const long long edge = rev ? w.s0 + w.len : w.s0;
-        if (edge > w.x.ps && edge < w.x.pe && (edge - w.x.ps) % kRestart == 0)
-          put_state(ut, f.snap + (snap_slot(edge) * p.H + h) * mat + static_cast<long long>(i) * dc, 1, dc, i < da);
+        if (edge > w.x.ps && edge < w.x.pe && (edge - w.x.ps) % p.restart == 0)
+          // both forms' stored states only meet each other, so they may lie as
+          // the lanes hold them: whole lines a store
+          put_state(ut, f.snap + (snap_slot(p, edge) * p.H + h) * mat + i * 8, 8 * da, 1, dc, i < da);
       }
       const uint64_t total2 = pair(total, total);
       if (work) {
@@ -882,7 +886,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
                                : f.fin + (w.x.n * p.H + h) * mat + i * f.si;
         if (work) {
           if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(ut, t.bad[ph], it, rev, -1, 0, dc);
-          put_state(ut, to, state_only ? 1 : f.sj, dc, i < da);
+          put_state(ut, to, 8, state_only ? 1 : f.sj, dc, i < da);
         }
         // a piece that holds the sequence's start takes nothing from before
         if (state_only && i == 0) f.dec[blockIdx.x * p.H + h] = w.x.from_start ? -1.f : decay;
