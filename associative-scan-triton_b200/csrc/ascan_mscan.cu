@@ -554,18 +554,19 @@ constexpr int kSegGranule = 256;  // segments are multiples of this many tokens
 // crosses costs a second pass over two of the operands, about half of the
 // main pass's time.  Over all counts the cheapest estimate of
 // waves * segment length (* 1.5 when there are more segments than sequences)
-// is taken; equal sequences split at their own ends.
-static long long pick_segments(long long BL, long long N, long long lanes, int granule) {
+// is taken; equal sequences split at their own ends.  `room`: CTAs that run
+// at once.
+static long long pick_segments(long long BL, long long N, long long lanes, int granule, long long room) {
   const long long most = min(min((BL + granule - 1) / granule, 4096ll), 65535ll);
   const double inf = 1e30;
   long long best = 1;
   double best_cost = inf;
   for (long long J = 1; J <= most; J = J < 64 ? J + 1 : J + 8) {
     const long long seg = ((BL + J - 1) / J + granule - 1) / granule * granule;
-    const long long waves = (J * lanes + kSms - 1) / kSms;
+    const long long waves = (J * lanes + room - 1) / room;
     const double cost = static_cast<double>(waves) * (seg + 2.0 * granule) * (J > N ? 1.5 : 1.0);
     if (cost < best_cost * 0.97) best = J, best_cost = cost;
-    if (J * lanes > 16 * kSms) break;
+    if (J * lanes > 16 * room) break;
   }
   return best;
 }
@@ -615,11 +616,17 @@ struct Plan {
 
 static size_t up(size_t x) { return (x + 255) / 256 * 256; }
 
+// CTAs of the kernel for this type that run at once: the plain one's fit two
+// to an SM up to 64 wide.
+static long long room_for(int dtype, int dk, int dv) {
+  return dtype != ASCAN_BF16 && max(dk, dv) <= 64 ? 2 * kSms : kSms;
+}
+
 // Layout of the workspace; the same arithmetic serves the size query.
 static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, int hg, int dk, int dv,
-                      bool backward) {
+                      bool backward, long long room) {
   Plan w{};
-  w.J = pick_segments(BL, N, static_cast<long long>(H) * (backward ? 3 : 1), kSegGranule);
+  w.J = pick_segments(BL, N, static_cast<long long>(H) * (backward ? 3 : 1), kSegGranule, room);
   w.seg = ((BL + w.J - 1) / w.J + kSegGranule - 1) / kSegGranule * kSegGranule;
   w.J = (BL + w.seg - 1) / w.seg;
   const size_t mat = static_cast<size_t>(dk) * dv * H * 4;
@@ -688,9 +695,12 @@ extern "C" {
 size_t ascan_matrix_scan_workspace(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads, int key_heads,
                                    int value_heads, int gate_heads, int key_dim, int value_dim, int backward) {
   if (seq_total <= 0 || num_seq <= 0 || num_heads <= 0 || key_dim <= 0 || value_dim <= 0) return 256;
-  return make_plan(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads, gate_heads, key_dim, value_dim,
-                   backward != 0)
-      .total;
+  size_t need = 0;  // the type is not known here: the larger of its two plans
+  for (long long room : {kSms, 2 * kSms})
+    need = max(need, make_plan(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads, gate_heads, key_dim,
+                               value_dim, backward != 0, room)
+                         .total);
+  return need;
 }
 
 int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
@@ -704,7 +714,7 @@ int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys,
   if (seq_total == 0 || num_seq == 0) return ASCAN_OK;
   if (!out) return ASCAN_EINVAL;
   const Plan w = make_plan(seq_total, num_seq, num_heads, queries->heads, keys->heads, values->heads, log_gates->heads,
-                           key_dim, value_dim, false);
+                           key_dim, value_dim, false, room_for(dtype, key_dim, value_dim));
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
   Launch l{};
   l.p = problem_of(w, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, num_heads);
@@ -743,7 +753,8 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
     return ASCAN_EINVAL;
   if (d_final_state && !final_state) return ASCAN_EINVAL;
   const int H = num_heads, dk = key_dim, dv = value_dim;
-  const Plan w = make_plan(seq_total, num_seq, H, queries->heads, keys->heads, values->heads, log_gates->heads, dk, dv, true);
+  const Plan w = make_plan(seq_total, num_seq, H, queries->heads, keys->heads, values->heads, log_gates->heads, dk, dv, true,
+                           room_for(dtype, dk, dv));
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Launch l{};
