@@ -25,10 +25,9 @@ template <int DM>
 struct PlainSmem {
   static constexpr int kLt = kPlainChunk + 4, kLd = DM + 4;
   float s[DM * DM];
-  float at[DM * kLt];  // [dim][token]
-  float bt[DM * kLt];
-  float c[kPlainChunk * kLd];            // [token][dim]
-  float pt[kPlainChunk * kLt];           // [column token][row token]
+  float at[DM * kLt];          // [dim][token]; then the masked scores, [column token][row token]
+  float bt[DM * kLt];          // [dim][token]
+  float c[kPlainChunk * kLd];  // [token][dim]
   double g[kPlainChunk];
   float row[kPlainChunk], col[kPlainChunk];
   float total;
@@ -94,7 +93,7 @@ __device__ __forceinline__ void load_rows(float* dst, const Rows& r, long long t
 }
 
 template <typename T, int DM>
-__global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 3 : 1)
     plain_kernel(const __grid_constant__ Launch L, const bool state_only) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   using Sm = PlainSmem<DM>;
@@ -168,31 +167,18 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 2 : 1)
       }
       __syncthreads();
       if (!state_only) {
-        {  // scores: 4 rows by 4 columns; blocks outside the mask are zero
-          const int sr0 = (tid / 16) * 4, sc0 = (tid % 16) * 4;
-          float acc[4][4] = {};
-          if (rev ? sc0 + 3 >= sr0 : sc0 <= sr0 + 3) {
+        // scores: 4 rows by 4 columns; blocks outside the mask are zero
+        const int sr0 = (tid / 16) * 4, sc0 = (tid % 16) * 4;
+        float sacc[4][4] = {};
+        if (rev ? sc0 + 3 >= sr0 : sc0 <= sr0 + 3) {
 #pragma unroll 4
-            for (int d = 0; d < da; ++d) {
-              const float4 y = ld4(&sm.bt[d * LT + sc0]);
-              const float4 x = ld4(&sm.at[d * LT + sr0]);
-              fma4(acc[0], x.x, y);
-              fma4(acc[1], x.y, y);
-              fma4(acc[2], x.z, y);
-              fma4(acc[3], x.w, y);
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = sr0 + e, at = sc0 + c;
-              const bool on = (rev ? at >= r : at <= r) && at < len;
-              const double dg = rev ? sm.g[at] - sm.g[r] : sm.g[r] - sm.g[at];
-              v[e] = on ? acc[e][c] * f.sp * expf(static_cast<float>(dg)) : 0.f;
-            }
-            *reinterpret_cast<float4*>(&sm.pt[(sc0 + c) * LT + sr0]) = make_float4(v[0], v[1], v[2], v[3]);
+          for (int d = 0; d < da; ++d) {
+            const float4 y = ld4(&sm.bt[d * LT + sc0]);
+            const float4 x = ld4(&sm.at[d * LT + sr0]);
+            fma4(sacc[0], x.x, y);
+            fma4(sacc[1], x.y, y);
+            fma4(sacc[2], x.z, y);
+            fma4(sacc[3], x.w, y);
           }
         }
         float acc[R][4] = {};
@@ -210,11 +196,25 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 2 : 1)
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[r][q] *= sm.row[r0 + r];
+        __syncthreads();  // A has been read: the scores take its place
+        float* pt = sm.at;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = sr0 + e, at = sc0 + c;
+            const bool on = (rev ? at >= r : at <= r) && at < len;
+            const double dg = rev ? sm.g[at] - sm.g[r] : sm.g[r] - sm.g[at];
+            v[e] = on ? sacc[e][c] * f.sp * expf(static_cast<float>(dg)) : 0.f;
+          }
+          *reinterpret_cast<float4*>(&pt[(sc0 + c) * LT + sr0]) = make_float4(v[0], v[1], v[2], v[3]);
+        }
         __syncthreads();
         // columns before (after) the thread's rows meet all of them
         const int c_from = rev ? r0 + R : 0, c_to = rev ? len : min(r0, len);
 #pragma unroll 4
-        for (int c = c_from; c < c_to; ++c) outer(&sm.pt[c * LT + r0], ld4(&sm.c[c * LD + d0]));
+        for (int c = c_from; c < c_to; ++c) outer(&pt[c * LT + r0], ld4(&sm.c[c * LD + d0]));
         // the columns of the rows themselves: masked ones are left out, not
         // multiplied by zero, so that a NaN there reaches no row
 #pragma unroll
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 2 : 1)
           const float4 y = ld4(&sm.c[(r0 + q) * LD + d0]);
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            if (rev ? q >= r : q <= r) fma4(acc[r], sm.pt[(r0 + q) * LT + r0 + r], y);
+            if (rev ? q >= r : q <= r) fma4(acc[r], pt[(r0 + q) * LT + r0 + r], y);
         }
         const bool vec = dc % 4 == 0 && (reinterpret_cast<uintptr_t>(f.out) & 15u) == 0;
 #pragma unroll
@@ -548,7 +548,15 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepA
 // ---------------------------------------------------------------------------
 
 constexpr long long kSms = 148;
-constexpr int kSegGranule = 256;  // segments are multiples of this many tokens
+
+// What runs at once, and of how many tokens segments are multiples: a chunk of
+// the tensor-core kernel costs about 3 us however few of its tokens are there
+// (128 instead of 256: 257 tokens took 44 us, not 22), the plain one's half
+// chunks do not (128: float32 training 697 us, 256: 777 us).
+struct Fit {
+  long long room;
+  int granule;
+};
 
 // Segments: the launch should fill the SMs, and a split that a sequence
 // crosses costs a second pass over two of the operands, about half of the
@@ -616,18 +624,18 @@ struct Plan {
 
 static size_t up(size_t x) { return (x + 255) / 256 * 256; }
 
-// CTAs of the kernel for this type that run at once: the plain one's fit two
-// to an SM up to 64 wide.
-static long long room_for(int dtype, int dk, int dv) {
-  return dtype != ASCAN_BF16 && max(dk, dv) <= 64 ? 2 * kSms : kSms;
+// The plain kernel's CTAs fit three to an SM up to 64 wide.
+static Fit fit_for(int dtype, int dk, int dv) {
+  if (dtype == ASCAN_BF16) return {kSms, 256};
+  return {max(dk, dv) <= 64 ? 3 * kSms : kSms, 128};
 }
 
 // Layout of the workspace; the same arithmetic serves the size query.
 static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, int hg, int dk, int dv,
-                      bool backward, long long room) {
+                      bool backward, Fit fit) {
   Plan w{};
-  w.J = pick_segments(BL, N, static_cast<long long>(H) * (backward ? 3 : 1), kSegGranule, room);
-  w.seg = ((BL + w.J - 1) / w.J + kSegGranule - 1) / kSegGranule * kSegGranule;
+  w.J = pick_segments(BL, N, static_cast<long long>(H) * (backward ? 3 : 1), fit.granule, fit.room);
+  w.seg = ((BL + w.J - 1) / w.J + fit.granule - 1) / fit.granule * fit.granule;
   w.J = (BL + w.seg - 1) / w.seg;
   const size_t mat = static_cast<size_t>(dk) * dv * H * 4;
   w.carry = w.J > 1 ? up(w.J * mat) + up(static_cast<size_t>(w.J) * H * 4) : 0;
@@ -695,10 +703,10 @@ extern "C" {
 size_t ascan_matrix_scan_workspace(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads, int key_heads,
                                    int value_heads, int gate_heads, int key_dim, int value_dim, int backward) {
   if (seq_total <= 0 || num_seq <= 0 || num_heads <= 0 || key_dim <= 0 || value_dim <= 0) return 256;
-  size_t need = 0;  // the type is not known here: the larger of its two plans
-  for (long long room : {kSms, 2 * kSms})
+  size_t need = 0;  // the type is not known here: the larger of its plans
+  for (int dtype : {ASCAN_F32, ASCAN_BF16})
     need = max(need, make_plan(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads, gate_heads, key_dim,
-                               value_dim, backward != 0, room)
+                               value_dim, backward != 0, fit_for(dtype, key_dim, value_dim))
                          .total);
   return need;
 }
@@ -714,7 +722,7 @@ int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys,
   if (seq_total == 0 || num_seq == 0) return ASCAN_OK;
   if (!out) return ASCAN_EINVAL;
   const Plan w = make_plan(seq_total, num_seq, num_heads, queries->heads, keys->heads, values->heads, log_gates->heads,
-                           key_dim, value_dim, false, room_for(dtype, key_dim, value_dim));
+                           key_dim, value_dim, false, fit_for(dtype, key_dim, value_dim));
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
   Launch l{};
   l.p = problem_of(w, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, num_heads);
@@ -754,7 +762,7 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
   if (d_final_state && !final_state) return ASCAN_EINVAL;
   const int H = num_heads, dk = key_dim, dv = value_dim;
   const Plan w = make_plan(seq_total, num_seq, H, queries->heads, keys->heads, values->heads, log_gates->heads, dk, dv, true,
-                           room_for(dtype, dk, dv));
+                           fit_for(dtype, dk, dv));
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Launch l{};

@@ -34,10 +34,13 @@ __device__ __forceinline__ void fill_outside(const Problem& p, const Form& f) {
   }
   if (f.fin && j == 0) {
     const long long mat = static_cast<long long>(f.da) * f.dc;
-    for (long long n = 0; n < p.N; ++n)
-      if (cu_at(p, n + 1) <= cu_at(p, n))
-        for (long long e = tid; e < mat; e += step)
-          f.fin[(n * p.H + h) * mat + e] = f.init ? f.init[(n * p.H + h) * mat + e] : 0.f;
+    bool empty = false;
+    for (long long n = tid; n < p.N; n += step) empty |= cu_at(p, n + 1) <= cu_at(p, n);
+    if (__syncthreads_or(empty))
+      for (long long n = 0; n < p.N; ++n)
+        if (cu_at(p, n + 1) <= cu_at(p, n))
+          for (long long e = tid; e < mat; e += step)
+            f.fin[(n * p.H + h) * mat + e] = f.init ? f.init[(n * p.H + h) * mat + e] : 0.f;
   }
 }
 

@@ -376,14 +376,21 @@ __device__ __noinline__ void put_state(uint32_t tm, float* to, int hop, long lon
 
 // `from` null: zeros.  Columns up to the next 16 are written too.
 __device__ __noinline__ void get_state(uint32_t tm, const float* from, long long sj, int dc, bool on) {
+  // sixteen columns' loads in flight
 #pragma unroll 1
-  for (int d = 0; d < (dc + 15) / 16 * 16; d += 8) {
-    uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (from && on && d < dc) {
+  for (int d = 0; d < dc; d += 16) {
+    uint32_t v[16];
+    if (from && on && sj == 1) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = __float_as_uint(from[(d + q) * sj]);
+      for (int q = 0; q < 16; q += 4) {
+        const uint4 x = d + q < dc ? __ldg(reinterpret_cast<const uint4*>(from + d + q)) : make_uint4(0, 0, 0, 0);
+        v[q] = x.x, v[q + 1] = x.y, v[q + 2] = x.z, v[q + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 16; ++q) v[q] = from && on && d + q < dc ? __float_as_uint(__ldg(from + (d + q) * sj)) : 0u;
     }
-    tmem_st8(tm + d, v);
+    tmem_st16(tm + d, v);
   }
   wait_st();
 }
