@@ -8,7 +8,7 @@ in include/ascan.h); CUDA tensors only, no CPU fallback.
 
 Beside the reference's names (``__all__``) the package has the operators of a
 gated linear-attention layer: ``matrix_scan_causal``, ``matrix_scan_step`` and
-``qk_norm_rotate`` (matrix_scan.py).
+``qk_norm_rotate`` (matrix_scan.py), each with a ``*_compiled`` variant.
 """
 
 __version__ = "1.0.0"
@@ -39,8 +39,11 @@ from associative_scan_triton.scan_compiled import (  # noqa: E402
 )
 from associative_scan_triton.matrix_scan import (  # noqa: E402
   matrix_scan_causal,
+  matrix_scan_causal_compiled,
   matrix_scan_step,
+  matrix_scan_step_compiled,
   qk_norm_rotate,
+  qk_norm_rotate_compiled,
 )
 from associative_scan_triton._lib import (  # noqa: E402
   ScanError,

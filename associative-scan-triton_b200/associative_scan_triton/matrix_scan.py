@@ -371,6 +371,25 @@ def _rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions,
 
 
 def _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens):
+  try:  # the usual call in one expression; whatever fails it is looked at below
+    (n, hq, d), (nk, hk, dk), (rows, half) = queries.shape, keys.shape, cos.shape
+    device, dtype, wtype = queries.device, queries.dtype, query_weight.dtype
+    index = positions if cu_seqlens is None else cu_seqlens
+    if (queries.is_cuda and keys.device == device and query_weight.device == device
+        and key_weight.device == device and cos.device == device and sin.device == device
+        and index.device == device and (positions is None) != (cu_seqlens is None)
+        and dtype in DTYPE_CODES and keys.dtype == dtype and key_weight.dtype == wtype
+        and (wtype == torch.float32 or wtype == dtype) and cos.dtype == torch.float32
+        and sin.dtype == torch.float32 and index.dtype in INDEX_CODES and nk == n and dk == d
+        and d > 1 and 0 < hq <= 65535 and 0 < hk <= 65535 and 2 * half <= d
+        and query_weight.shape == (d,) and key_weight.shape == (d,) and sin.shape == (rows, half)
+        and index.dim() == 1 and (index.shape[0] == n if cu_seqlens is None else index.shape[0] > 0)
+        and queries.stride(2) == 1 and keys.stride(2) == 1 and index.is_contiguous()
+        and query_weight.is_contiguous() and key_weight.is_contiguous() and cos.is_contiguous()
+        and sin.is_contiguous()):
+      return _lib._enable_error_flag()
+  except (AttributeError, TypeError, ValueError):
+    pass
   _check_rows("queries", queries, None, None)
   device, tokens, dim = queries.device, queries.shape[0], queries.shape[2]
   _check_rows("keys", keys, device, queries.dtype, tokens, dim)
@@ -500,3 +519,158 @@ def qk_norm_rotate(
                               cu_seqlens, float(eps), bool(interleaved))
   return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
                          float(eps), bool(interleaved))
+
+
+# ---------------------------------------------------------------------------
+# torch.compile-safe variants: custom ops with fake kernels and gradients
+# ---------------------------------------------------------------------------
+
+_NS = "associative_scan_triton"
+
+
+def _none(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+  """An op returns tensors only: what is not asked for comes out empty."""
+  return t if t is not None else like.new_empty(0, dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::matrix_scan_fwd", mutates_args=())
+def matrix_scan_fwd_op(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                       log_gates: torch.Tensor, cu_seqlens: torch.Tensor, scale: float,
+                       initial_state: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+  """matrix_scan_causal; returns (out, final_state)."""
+  return _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_state, True)
+
+
+@matrix_scan_fwd_op.register_fake
+def _matrix_scan_fwd_fake(queries, keys, values, log_gates, cu_seqlens, scale, initial_state):
+  heads = max(t.shape[1] for t in (queries, keys, values, log_gates))
+  return (values.new_empty(values.shape[0], heads, values.shape[2]),
+          values.new_empty((cu_seqlens.shape[0] - 1, heads, queries.shape[2], values.shape[2]),
+                           dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::matrix_scan_bwd", mutates_args=())
+def matrix_scan_bwd_op(
+  queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, log_gates: torch.Tensor,
+  cu_seqlens: torch.Tensor, scale: float, initial_state: torch.Tensor | None,
+  final_state: torch.Tensor, d_out: torch.Tensor | None, d_final: torch.Tensor | None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+  """Gradients of queries, keys, values, log_gates and (empty without one) initial_state."""
+  *grads, d_initial = _scan_backward(queries, keys, values, log_gates, cu_seqlens, scale,
+                                     initial_state, final_state, d_out, d_final)
+  return (*grads, _none(d_initial, queries))
+
+
+@matrix_scan_bwd_op.register_fake
+def _matrix_scan_bwd_fake(queries, keys, values, log_gates, cu_seqlens, scale, initial_state,
+                          final_state, d_out, d_final):
+  grads = tuple(t.new_empty(t.shape) for t in (queries, keys, values, log_gates))
+  d_initial = queries.new_empty(0 if initial_state is None else initial_state.shape,
+                                dtype=torch.float32)
+  return (*grads, d_initial)
+
+
+def _matrix_scan_setup(ctx, inputs, output) -> None:
+  queries, keys, values, log_gates, cu_seqlens, scale, initial_state = inputs
+  ctx.save_for_backward(queries, keys, values, log_gates, cu_seqlens, initial_state, output[1])
+  ctx.scale = scale
+  ctx.set_materialize_grads(False)
+
+
+def _matrix_scan_backward(ctx, d_out, d_final):
+  queries, keys, values, log_gates, cu_seqlens, initial_state, final = ctx.saved_tensors
+  if d_out is None and d_final is None:
+    return (None,) * 7
+  *grads, d_initial = matrix_scan_bwd_op(queries, keys, values, log_gates, cu_seqlens, ctx.scale,
+                                         initial_state, final, d_out, d_final)
+  return (*grads, None, None, d_initial if initial_state is not None else None)
+
+
+matrix_scan_fwd_op.register_autograd(_matrix_scan_backward, setup_context=_matrix_scan_setup)
+
+
+def matrix_scan_causal_compiled(queries, keys, values, log_gates, args, scale=None,
+                                initial_state=None, return_final_state=False):
+  """matrix_scan_causal that torch.compile can trace (same arguments and results)."""
+  scale = float(queries.shape[-1]) ** -0.5 if scale is None else float(scale)
+  out, final = matrix_scan_fwd_op(queries, keys, values, log_gates, args["cu_seqlens"], scale,
+                                  initial_state)
+  return (out, final) if return_final_state else out
+
+
+@torch.library.custom_op(f"{_NS}::matrix_scan_step", mutates_args=("state",))
+def matrix_scan_step_op(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                        log_gates: torch.Tensor, state: torch.Tensor, slots: torch.Tensor | None,
+                        scale: float) -> torch.Tensor:
+  """matrix_scan_step in place."""
+  return matrix_scan_step(queries, keys, values, log_gates, state, slots=slots, scale=scale)
+
+
+@matrix_scan_step_op.register_fake
+def _matrix_scan_step_fake(queries, keys, values, log_gates, state, slots, scale):
+  return values.new_empty(values.shape[0], state.shape[1], values.shape[2])
+
+
+def matrix_scan_step_compiled(queries, keys, values, log_gates, state, slots=None, scale=None):
+  """matrix_scan_step, in place, that torch.compile can trace."""
+  scale = float(queries.shape[-1]) ** -0.5 if scale is None else float(scale)
+  return matrix_scan_step_op(queries, keys, values, log_gates, state, slots, scale)
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rotate_fwd", mutates_args=())
+def qk_norm_rotate_fwd_op(queries: torch.Tensor, keys: torch.Tensor, query_weight: torch.Tensor,
+                          key_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                          positions: torch.Tensor | None, cu_seqlens: torch.Tensor | None,
+                          eps: float, interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+  """qk_norm_rotate."""
+  return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
+                         eps, interleaved)
+
+
+@qk_norm_rotate_fwd_op.register_fake
+def _qk_norm_rotate_fwd_fake(queries, keys, query_weight, key_weight, cos, sin, positions,
+                             cu_seqlens, eps, interleaved):
+  return queries.new_empty(queries.shape), keys.new_empty(keys.shape)
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rotate_bwd", mutates_args=())
+def qk_norm_rotate_bwd_op(
+  queries: torch.Tensor, keys: torch.Tensor, query_weight: torch.Tensor, key_weight: torch.Tensor,
+  cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None,
+  cu_seqlens: torch.Tensor | None, eps: float, interleaved: bool, d_queries: torch.Tensor | None,
+  d_keys: torch.Tensor | None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+  """Gradients of queries, keys and the two weights."""
+  return _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
+                          eps, interleaved, d_queries, d_keys)
+
+
+@qk_norm_rotate_bwd_op.register_fake
+def _qk_norm_rotate_bwd_fake(queries, keys, query_weight, key_weight, cos, sin, positions,
+                             cu_seqlens, eps, interleaved, d_queries, d_keys):
+  return tuple(t.new_empty(t.shape) for t in (queries, keys, query_weight, key_weight))
+
+
+def _qk_norm_rotate_setup(ctx, inputs, output) -> None:
+  *tensors, ctx.eps, ctx.interleaved = inputs
+  ctx.save_for_backward(*tensors)
+  ctx.set_materialize_grads(False)
+
+
+def _qk_norm_rotate_backward(ctx, d_queries, d_keys):
+  if d_queries is None and d_keys is None:
+    return (None,) * 10
+  return (*qk_norm_rotate_bwd_op(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_queries, d_keys),
+          *(None,) * 6)
+
+
+qk_norm_rotate_fwd_op.register_autograd(_qk_norm_rotate_backward,
+                                        setup_context=_qk_norm_rotate_setup)
+
+
+def qk_norm_rotate_compiled(queries, keys, query_weight, key_weight, cos, sin, args=None,
+                            positions=None, eps=1e-6, interleaved=False):
+  """qk_norm_rotate that torch.compile can trace (same arguments and results)."""
+  return qk_norm_rotate_fwd_op(queries, keys, query_weight, key_weight, cos, sin, positions,
+                               None if args is None else args["cu_seqlens"], float(eps),
+                               bool(interleaved))

@@ -369,8 +369,8 @@ __global__ void __launch_bounds__(256)
   }
   int stretch = 0;
   for (long long n = first_beyond(p, t0); n < p.N && cu_at(p, n) < t1; ++n) {
-    const long long b1 = cu_at(p, n + 1);
-    const long long ps = max(cu_at(p, n), t0), pe = min(b1, t1);
+    const long long b0 = cu_at(p, n), b1 = cu_at(p, n + 1);
+    const long long ps = max(b0, t0), pe = min(b1, t1);
     for (long long s0 = ps; s0 < pe; s0 += p.restart, ++stretch) {
       if (stretch % gridDim.z != blockIdx.z) continue;
       const long long s1 = min(s0 + p.restart, pe);
@@ -430,7 +430,11 @@ __global__ void __launch_bounds__(256)
       for (int q = 0; q < 4; ++q) {
         const long long t = s1 - 1 - (tid * 4 + q);
         base += v[q];
-        if (t >= s0) put(t, base);
+        if (t < s0) continue;
+        // no state before the token, or a gate that drops it: nothing passes,
+        // and the sums' rounding must not stand in for that
+        const bool none = (!fq.init && t == b0) || expf(load_gate(p, t, h)) == 0.f;
+        put(t, none ? 0.f : base);
       }
     }
   }
@@ -581,11 +585,9 @@ static long long pick_segments(long long BL, long long N, long long lanes, int g
 
 template <typename T, int DM>
 static int plain_launch(const Launch& l, int roles, bool state_only, cudaStream_t s) {
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaFuncSetAttribute(plain_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(sizeof(PlainSmem<DM>)));
-  });
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(plain_kernel<T, DM>, sizeof(PlainSmem<DM>), done);
+  if (rc != ASCAN_OK) return rc;
   plain_kernel<T, DM><<<dim3(l.p.J, l.p.H, roles), kPlainThreads, sizeof(PlainSmem<DM>), s>>>(l, state_only);
   return launch_status();
 }

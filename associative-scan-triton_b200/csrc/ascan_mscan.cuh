@@ -41,6 +41,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/ascan.h"
 
 namespace ascan {
@@ -155,6 +157,20 @@ __device__ __forceinline__ float load_gate(const Problem& p, long long t, int h)
 // are `restart` apart and at least as far from those of the next, so the
 // quotient is unique.
 __device__ __forceinline__ long long snap_slot(const Problem& p, long long at) { return at / p.restart; }
+
+// A kernel's dynamic shared memory beyond 48 KB has to be allowed once on
+// every device that runs it; `done` holds a bit for each.
+template <typename K>
+inline int allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return ASCAN_EDEVICE;
+  const unsigned long long bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return ASCAN_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess)
+    return ASCAN_ECUDA;
+  done.fetch_or(bit, std::memory_order_release);
+  return ASCAN_OK;
+}
 
 // The tensor-core kernel (ascan_mscan_tc.cu).
 bool tc_usable(const Launch& l, int roles, int dtype);

@@ -1120,7 +1120,7 @@ static bool rows_usable(const Rows& r, int dim, int H) {
 int tc_dot_parts(const Form& f) { return f.dc > 32 ? 2 : 1; }
 
 bool tc_usable(const Launch& l, int roles, int dtype) {
-  if (dtype != ASCAN_BF16 || l.p.BL > 0x7fffff00ll) return false;
+  if (dtype != ASCAN_BF16 || l.p.gate_type == ASCAN_F16 || l.p.BL > 0x7fffff00ll) return false;
   for (int r = 0; r < roles; ++r) {
     const Form& f = l.f[r];
     if (!rows_usable(f.a, f.da, l.p.H) || !rows_usable(f.b, f.da, l.p.H) || !rows_usable(f.c, f.dc, l.p.H) ||
@@ -1151,11 +1151,9 @@ int tc_run(const Launch& l, int roles, bool state_only, cudaStream_t s) {
     const size_t need = g.bytes() + sizeof(TcTail);
     if (need > smem) smem = need;
   }
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaFuncSetAttribute(tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
-    cudaFuncSetAttribute(tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
-  });
+  static std::atomic<unsigned long long> done[2]{};
+  const int rc = state_only ? allow_smem(tc_kernel<true>, kSmemLimit, done[1]) : allow_smem(tc_kernel<false>, kSmemLimit, done[0]);
+  if (rc != ASCAN_OK) return rc;
   const dim3 grid(l.p.J, l.p.H, roles);
   if (state_only) tc_kernel<true><<<grid, kTcThreads, smem, s>>>(l, maps);
   else tc_kernel<false><<<grid, kTcThreads, smem, s>>>(l, maps);

@@ -294,6 +294,23 @@ def test_gradient_scale_gates_and_outside_tokens(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gates_that_nothing_passes_have_no_gradient(dtype):
+  # the first token of a sequence without an initial state, and a dropped gate:
+  # zero, not what rounding leaves of sums that cancel
+  lengths = [1, 1, 300, 1]
+  q, k, v, g, _, d_out, _ = make(lengths, (2, 2, 2, 2), (64, 64), dtype)
+  g[50] = -math.inf
+  g[77] = -150.0
+  leaf = g.to(DEV).requires_grad_(True)
+  out = ast.matrix_scan_causal(q.to(DEV), k.to(DEV), v.to(DEV), leaf, {"cu_seqlens": cu_of(lengths)})
+  (d_gates,) = torch.autograd.grad(out, leaf, d_out.to(DEV))
+  for t in (0, 1, 2, 50, 77, 302):
+    assert not d_gates[t].any(), t
+  assert d_gates[3:50].any() and torch.isfinite(d_gates).all()
+
+
+@gpu
 def test_gradient_by_differences():
   # central differences of a float64 evaluation of the loss at float32 inputs
   # moved by +-h: truncation h^2 ~ 1e-8, so only our own 1e-5 remains; 1e-4
@@ -594,3 +611,61 @@ def test_example_trains_and_decodes(capsys):
   spec.loader.exec_module(example)
   assert example.main(["--steps", "12", "--dim", "128", "--heads", "2"]) == 0
   assert "step by step" in capsys.readouterr().out
+
+
+def test_custom_ops_have_fake_kernels():
+  from torch._subclasses.fake_tensor import FakeTensorMode
+  ops = torch.ops.associative_scan_triton
+  with FakeTensorMode():
+    q = torch.empty(9, 2, 16, device="cuda")
+    v = torch.empty(9, 4, 8, device="cuda", dtype=torch.float32)
+    g = torch.empty(9, 4, device="cuda")
+    cu = torch.empty(3, dtype=torch.int32, device="cuda")
+    out, final = ops.matrix_scan_fwd(q, q, v, g, cu, 1.0, None)
+    assert out.shape == (9, 4, 8) and final.shape == (2, 4, 16, 8) and final.dtype == F32
+    grads = ops.matrix_scan_bwd(q, q, v, g, cu, 1.0, None, final, out, None)
+    assert [x.shape for x in grads[:4]] == [q.shape, q.shape, v.shape, g.shape]
+    assert grads[4].numel() == 0
+    state = torch.empty(12, 4, 16, 8, device="cuda")
+    assert ops.matrix_scan_step(q, q, v, g, state, None, 1.0).shape == (9, 4, 8)
+    w, t = torch.empty(16, device="cuda"), torch.empty(5, 8, device="cuda")
+    yq, yk = ops.qk_norm_rotate_fwd(q, v[..., :4].new_empty(9, 1, 16), w, w, t, t, cu, None, 1e-6, False)
+    assert yq.shape == q.shape and yk.shape == (9, 1, 16)
+
+
+@gpu
+def test_compiled_layer_matches_eager():
+  # forward, gradients and a step traced in one piece
+  lengths, h, d = [70, 0, 131], 2, 32
+  gen = torch.Generator().manual_seed(11)
+  packed = torch.randn(201, 3 * h * d, generator=gen).to(DEV).requires_grad_(True)
+  gates = (-0.1 * torch.rand(201, h, generator=gen)).to(DEV).requires_grad_(True)
+  weight = torch.ones(d, device=DEV, requires_grad=True)
+  angle = torch.rand(140, d // 2, generator=gen).to(DEV)
+  cos, sin, args = angle.cos(), angle.sin(), {"cu_seqlens": cu_of(lengths)}
+
+  def layer(packed, gates, weight, scan, rotate):
+    q, k, v = packed.view(-1, 3, h, d).unbind(1)
+    q, k = rotate(q, k, weight, weight, cos, sin, args)
+    out, final = scan(q, k, v, gates, args, return_final_state=True)
+    return (out * 2.0).sum(-1), final
+
+  def compiled(packed, gates, weight):
+    return layer(packed, gates, weight, ast.matrix_scan_causal_compiled, ast.qk_norm_rotate_compiled)
+
+  found = []
+  for run in (lambda: layer(packed, gates, weight, ast.matrix_scan_causal, ast.qk_norm_rotate),
+              lambda: torch.compile(compiled, fullgraph=True, backend="aot_eager")(packed, gates, weight)):
+    out, final = run()
+    found.append((out, final, *torch.autograd.grad((out.square().sum() + final.sum()), (packed, gates, weight))))
+  for a, b in zip(*found):
+    assert torch.equal(a, b)
+
+  q, k, v = (torch.randn(3, h, d, generator=gen).to(DEV) for _ in range(3))
+  g = torch.zeros(3, h, device=DEV)
+  pools = [torch.ones(4, h, d, d, device=DEV) for _ in range(2)]
+  slots = torch.tensor([2, -1, 0], dtype=torch.int32, device=DEV)
+  step = torch.compile(ast.matrix_scan_step_compiled, fullgraph=True, backend="aot_eager")
+  a = ast.matrix_scan_step(q, k, v, g, pools[0], slots=slots)
+  b = step(q, k, v, g, pools[1], slots)
+  assert torch.equal(a, b) and torch.equal(*pools)
