@@ -444,8 +444,25 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 __global__ void __launch_bounds__(256)
     share_sum_kernel(const float* __restrict__ part, T* __restrict__ out, long long n, int share, int dim) {
-  for (long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; e < n;
-       e += static_cast<long long>(gridDim.x) * 256) {
+  const long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<long long>(gridDim.x) * 256;
+  if (dim % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T))) == 0) {
+    const int quads = dim / 4;
+    for (long long e = first; e < n / 4; e += step) {
+      const long long row = e / quads;
+      const float4* at = reinterpret_cast<const float4*>(part) + row * share * quads + e % quads;
+      float4 x = __ldcs(at);
+#pragma unroll 4
+      for (int s = 1; s < share; ++s) {
+        const float4 y = __ldcs(at + static_cast<long long>(s) * quads);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      }
+      T v[4] = {from_f<T>(x.x), from_f<T>(x.y), from_f<T>(x.z), from_f<T>(x.w)};
+      if (sizeof(T) == 4) reinterpret_cast<float4*>(out)[e] = x;
+      else reinterpret_cast<uint2*>(out)[e] = *reinterpret_cast<const uint2*>(v);
+    }
+    return;
+  }
+  for (long long e = first; e < n; e += step) {
     const long long row = e / dim, d = e % dim;
     float x = 0.f;
     for (int s = 0; s < share; ++s) x += part[(row * share + s) * dim + d];
