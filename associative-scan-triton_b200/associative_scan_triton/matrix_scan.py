@@ -19,6 +19,7 @@ its workspace from torch's allocator.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -42,6 +43,21 @@ def _rows(*tensors: torch.Tensor):
     words += (t.data_ptr(), st[0], st[1], t.shape[1])
   block = _ROWS[len(tensors)](*words)
   return [ctypes.byref(block, 32 * i) for i in range(len(tensors))]
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+  """Uninitialised, contiguous, of the same shape, type and device."""
+  return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=256)
+def _scan_workspace(*sizes: int) -> int:
+  return _lib.load().ascan_matrix_scan_workspace(*sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _rotate_workspace(*sizes: int) -> int:
+  return _lib.load().ascan_qk_norm_rotate_workspace(*sizes)
 
 
 def _stream(device: torch.device) -> int:
@@ -174,7 +190,7 @@ def _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_s
   lib = _lib.load()
   with _on(device):
     ws = torch.empty(
-      lib.ascan_matrix_scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1],
+      _scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1],
                                       values.shape[1], log_gates.shape[1], key_dim, value_dim, 0),
       dtype=torch.uint8, device=device)
     rc = lib.ascan_matrix_scan_forward(
@@ -191,8 +207,8 @@ def _scan_backward(queries, keys, values, log_gates, cu_seqlens, scale, initial_
   device, tokens, heads, key_dim, value_dim = _check_operands(queries, keys, values, log_gates,
                                                               MAX_DIM)
   num_seq = cu_seqlens.numel() - 1
-  d_queries, d_keys, d_values, d_gates = (torch.empty(t.shape, dtype=t.dtype, device=device)
-                                          for t in (queries, keys, values, log_gates))
+  d_queries, d_keys, d_values, d_gates = (_like(queries), _like(keys), _like(values),
+                                          _like(log_gates))
   d_initial = torch.empty_like(initial_state) if initial_state is not None else None
   if tokens == 0 or num_seq == 0:
     for t in (d_queries, d_keys, d_values, d_gates):
@@ -209,7 +225,7 @@ def _scan_backward(queries, keys, values, log_gates, cu_seqlens, scale, initial_
   lib = _lib.load()
   with _on(device):
     ws = torch.empty(
-      lib.ascan_matrix_scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1],
+      _scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1],
                                       values.shape[1], log_gates.shape[1], key_dim, value_dim, 1),
       dtype=torch.uint8, device=device)
     rc = lib.ascan_matrix_scan_backward(
@@ -230,19 +246,19 @@ class MatrixScanCausal(torch.autograd.Function):
   def forward(ctx, queries, keys, values, log_gates, cu_seqlens, scale, initial_state, want_final):
     out, final = _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_state,
                                want_final)
-    ctx.save_for_backward(queries, keys, values, log_gates, cu_seqlens, initial_state, final)
-    ctx.scale = scale
+    ctx.save_for_backward(queries, keys, values, log_gates, initial_state, final)
+    ctx.cu_seqlens, ctx.scale = cu_seqlens, scale
     ctx.set_materialize_grads(False)
     return out, final
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, d_out, d_final):
-    queries, keys, values, log_gates, cu_seqlens, initial_state, final = ctx.saved_tensors
+    queries, keys, values, log_gates, initial_state, final = ctx.saved_tensors
     if d_out is None and d_final is None:
       return (None,) * 8
     d_queries, d_keys, d_values, d_gates, d_initial = _scan_backward(
-      queries, keys, values, log_gates, cu_seqlens, ctx.scale, initial_state, final, d_out, d_final)
+      queries, keys, values, log_gates, ctx.cu_seqlens, ctx.scale, initial_state, final, d_out, d_final)
     return d_queries, d_keys, d_values, d_gates, None, None, d_initial, None
 
 
@@ -421,8 +437,7 @@ def _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions
                     interleaved):
   _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens)
   device = queries.device
-  out_q = torch.empty(queries.shape, dtype=queries.dtype, device=device)
-  out_k = torch.empty(keys.shape, dtype=keys.dtype, device=device)
+  out_q, out_k = _like(queries), _like(keys)
   if queries.shape[0] == 0:
     return out_q, out_k
   with _on(device):
@@ -437,8 +452,7 @@ def _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions
 def _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
                      interleaved, d_out_q, d_out_k):
   device, tokens = queries.device, queries.shape[0]
-  d_q = torch.empty(queries.shape, dtype=queries.dtype, device=device)
-  d_k = torch.empty(keys.shape, dtype=keys.dtype, device=device)
+  d_q, d_k = _like(queries), _like(keys)
   d_qw, d_kw = torch.empty_like(query_weight), torch.empty_like(key_weight)
   if tokens == 0:
     return d_q, d_k, d_qw.zero_(), d_kw.zero_()
@@ -450,7 +464,7 @@ def _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, position
   lib = _lib.load()
   with _on(device):
     ws = torch.empty(
-      lib.ascan_qk_norm_rotate_workspace(tokens, queries.shape[1], keys.shape[1],
+      _rotate_workspace(tokens, queries.shape[1], keys.shape[1],
                                          queries.shape[2]), dtype=torch.uint8, device=device)
     rc = lib.ascan_qk_norm_rotate_backward(
       *_rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
@@ -467,8 +481,8 @@ class QkNormRotate(torch.autograd.Function):
   @staticmethod
   def forward(ctx, queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
               interleaved):
-    ctx.save_for_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens)
-    ctx.eps, ctx.interleaved = eps, interleaved
+    ctx.save_for_backward(queries, keys, query_weight, key_weight)
+    ctx.rest = (cos, sin, positions, cu_seqlens, eps, interleaved)  # no gradients among them
     ctx.set_materialize_grads(False)
     return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
                            eps, interleaved)
@@ -478,8 +492,7 @@ class QkNormRotate(torch.autograd.Function):
   def backward(ctx, d_q, d_k):
     if d_q is None and d_k is None:
       return (None,) * 10
-    return (*_rotate_backward(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_q, d_k),
-            *(None,) * 6)
+    return (*_rotate_backward(*ctx.saved_tensors, *ctx.rest, d_q, d_k), *(None,) * 6)
 
 
 def qk_norm_rotate(
