@@ -18,7 +18,11 @@ constexpr int kPlainChunk = 64;
 // take.  A chunk of 64 tokens lies in shared memory, A and B with the tokens
 // along the rows' unit stride, C as stored; the state stays there from chunk
 // to chunk.  Every product gives a thread a tile of 4 x 4 values (8 x 4 at 128
-// wide), so two (three) 16-byte reads feed 16 (32) multiply-adds.
+// wide), so two (three) 16-byte reads feed 16 (32) multiply-adds.  Measured at
+// 6001 tokens of 12 heads of 64 x 64, float32, forward and gradients: 657 us,
+// a tenth of the multiply-add rate; tiles are loaded without overlap, and
+// three CTAs an SM hide it in part (two: 737 us; tiles of 2 x 4 over 32
+// tokens: 1280 us).
 // ---------------------------------------------------------------------------
 
 template <int DM>
@@ -472,8 +476,10 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------------------
 // One token: out = scale * q (e^g S + k v^T), the new state written back.
-// Bound by reading and writing the state; a CTA takes `cols` columns of one
-// (request, head), a lane four of them, and its warps share the rows.
+// Bound by reading and writing the state; a CTA takes 128 columns of one
+// (request, head), a lane four of them, and its warps share the rows, eight in
+// flight each.  256 requests of 12 heads of 128 x 128: 66 us, 6.1 TB/s; one
+// request (32 columns a CTA): 3.2 us.
 // ---------------------------------------------------------------------------
 
 struct StepArgs {

@@ -9,12 +9,18 @@
 // one 16-byte vector per lane; the rotation's partner comes by a shuffle (or
 // sits in the same vector when pairs are adjacent), and the sums go over the
 // group by shuffles.  Where the whole head turns, a lane holds 8 bytes of each
-// half instead and has both sides of its pairs.  A group walks the heads of consecutive tokens with
-// several heads' loads in flight and a token's angles read once for all of
-// them.  Queries and keys share a launch: the first CTAs take the query heads,
-// the rest the key heads.  The weights' gradients stay in registers over all
-// of a group's heads, meet in shared memory, and a second launch adds the
-// CTAs' rows in a fixed order, so results repeat bit for bit.
+// half instead and has both sides of its pairs.  A group walks the heads of
+// consecutive tokens with several heads' loads in flight and a token's angles
+// read once for all of them.  Queries and keys share a launch: the first CTAs
+// take the query heads, the rest the key heads.  The weights' gradients stay
+// in registers over all of a group's heads, meet in shared memory, and a
+// second launch adds the CTAs' rows in a fixed order, so results repeat bit
+// for bit.
+//
+// Measured, bfloat16 heads of 128: 16384 tokens of 24 heads 38 us forward (5.3
+// TB/s), 66 + 2 us gradients (4.6 TB/s); 65536 tokens of 20 heads 138 us (5.1
+// TB/s); 16 tokens 2.9 us.  Six or eight loads in flight: no faster or slower;
+// three CTAs an SM for the gradients: 76 us.
 #include "ascan_impl.cuh"
 #include "ascan_mscan.cuh"
 

@@ -337,7 +337,8 @@ ASCAN_API int ascan_backward_bidi(const void* grad_fwd, const void* gates_fwd,
  * along dim and any token and head stride (views of a packed projection).
  * num_heads is the number of states per sequence; the heads of every tensor
  * divide it, and problem head h reads head h / (num_heads / heads).  States
- * are float32 [num_seq, num_heads, key_dim, value_dim], contiguous.
+ * are float32 [num_seq, num_heads, key_dim, value_dim], contiguous.  As in the
+ * scans, nothing is launched or written when num_seq or seq_total is 0.
  */
 typedef struct ascan_rows {
   const void* data;
