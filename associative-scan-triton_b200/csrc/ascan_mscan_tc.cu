@@ -350,12 +350,14 @@ struct Walk {
   }
   __device__ __forceinline__ bool next() {
     if (++cc >= chunks) {
-      x = next_piece(&p, rev, state_only, x.m);
-      if (x.m < 0) return false;
+      const Piece y = next_piece(&p, rev, state_only, x.m);
+      if (y.m < 0) return false;
+      x = y;
       cc = 0;
       chunks = static_cast<int>((x.pe - x.ps + kC - 1) / kC);
     }
-    s0 = x.ps + static_cast<long long>(rev ? chunks - 1 - cc : cc) * kC;
+    // without rows against the scan: see the gates
+    s0 = x.ps + static_cast<long long>(rev != state_only ? chunks - 1 - cc : cc) * kC;
     len = static_cast<int>(min(static_cast<long long>(kC), x.pe - s0));
     return true;
   }
@@ -826,35 +828,73 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     const int rows = (da + 15) / 16 * 16;  // the product with S runs over whole sixteens
     const bool work = (warp - 8) * 32 < rows;
     const long long mat = static_cast<long long>(da) * dc;
-    float decay = 1.f;
-    for (uint32_t it = 0; w.next(); ++it) {
+    const uint32_t ut = tm + lanes + kColU;
+    if (state_only) {
+      // One piece: from zero, and at its end what came in, decayed, on top.
+      uint32_t it = 0;
+      float decay = 0.f;
+      bool ok = true;
+      for (; ok && w.next(); ++it) {
+        if (it == 0) {
+          if (work) get_state(ut, nullptr, 1, dc, false);
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&t.s_ready);
+        }
+        ok = ctl.warp_wait(&t.tab_full, it & 1);
+        decay = t.total;
+        // in step with the products, so that no phase is missed
+        if (ok && it > 0) ok = ctl.warp_wait(&t.u_full[(it - 1) & 1], ((it - 1) >> 1) & 1);
+        if (lane == 0) bar_arrive(&t.tab_empty);
+      }
+      if (ok && it > 0 && ctl.warp_wait(&t.u_full[(it - 1) & 1], ((it - 1) >> 1) & 1)) {
+        fence_after();
+        if (work) {
+          const bool begins = w.x.from_start && f.init;
+          const float* from = f.init + (w.x.n * p.H + h) * mat + i * f.si;
+          float* to = f.carry + (static_cast<long long>(blockIdx.x) * p.H + h) * mat + static_cast<long long>(i) * dc;
+#pragma unroll 1
+          for (int d = 0; d < dc; d += 8) {
+            uint32_t v[8];
+            tmem_ld8(ut + d, v);
+            wait_ld();
+            if (i >= da) continue;
+            if (begins) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                v[q] = __float_as_uint(fmaf(decay, __ldg(from + (d + q) * f.sj), __uint_as_float(v[q])));
+            }
+            *reinterpret_cast<uint4*>(to + d) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(to + d + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+          }
+        }
+        // a piece that holds the sequence's start takes nothing from before
+        if (i == 0) f.dec[blockIdx.x * p.H + h] = w.x.from_start ? -1.f : decay;
+      }
+    }
+    for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
       const bool first = w.cc == 0;
-      if (first) decay = 1.f;
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       const float total = t.total;
       __syncwarp();
       if (lane == 0) bar_arrive(&t.tab_empty);
-      decay *= total;
       if (it > 0) {  // the update before this chunk; it also follows the last use of S
         if (!ctl.warp_wait(&t.u_full[ph ^ 1], ((it - 1) >> 1) & 1)) break;
         fence_after();
       }
-      const uint32_t ut = tm + lanes + kColU;
       if (first) {
         const float* from = nullptr;
         long long sj = 1;
-        if (!(state_only && !w.x.from_start)) {
-          if (!w.x.from_start)
-            from = f.carry + ((static_cast<long long>(blockIdx.x) + (rev ? 1 : -1)) * p.H + h) * mat + static_cast<long long>(i) * dc;
-          else if (f.init)
-            from = f.init + (w.x.n * p.H + h) * mat + i * f.si, sj = f.sj;
-        }
+        if (!w.x.from_start)
+          from = f.carry + ((static_cast<long long>(blockIdx.x) + (rev ? 1 : -1)) * p.H + h) * mat + static_cast<long long>(i) * dc;
+        else if (f.init)
+          from = f.init + (w.x.n * p.H + h) * mat + i * f.si, sj = f.sj;
         if (work) get_state(ut, from, sj, dc, i < da);
       } else if (work && t.bad_chunk[ph ^ 1] == static_cast<int>(it)) {
         spread_bad(ut, t.bad[ph ^ 1], it - 1, rev, -1, 0, dc);
       }
-      if (f.snap && !state_only && work) {
+      if (f.snap && work) {
         const long long edge = rev ? w.s0 + w.len : w.s0;
         if (edge > w.x.ps && edge < w.x.pe && (edge - w.x.ps) % p.restart == 0)
           // both forms' stored states only meet each other, so they may lie as
@@ -868,7 +908,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           float v[16];
           tmem_ld16(ut + 16 * b, reinterpret_cast<uint32_t*>(v));
           wait_ld();
-          if (!state_only && i < rows) {
+          if (i < rows) {
             // S: row i of 64 columns is 128 bytes; two 16-byte pieces per 16 columns
             unsigned char* base = s_op + (b >> 2) * (geo.s_bytes / blocks_c) + i * 128;
 #pragma unroll
@@ -895,17 +935,13 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&t.s_ready);
-      if (w.last() && (state_only || (w.x.to_end && f.fin))) {
+      if (w.last() && w.x.to_end && f.fin) {
         if (!ctl.warp_wait(&t.u_full[ph], (it >> 1) & 1)) break;
         fence_after();
-        float* to = state_only ? f.carry + (static_cast<long long>(blockIdx.x) * p.H + h) * mat + static_cast<long long>(i) * dc
-                               : f.fin + (w.x.n * p.H + h) * mat + i * f.si;
         if (work) {
           if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(ut, t.bad[ph], it, rev, -1, 0, dc);
-          put_state(ut, to, 8, state_only ? 1 : f.sj, dc, i < da);
+          put_state(ut, f.fin + (w.x.n * p.H + h) * mat + i * f.si, 8, f.sj, dc, i < da);
         }
-        // a piece that holds the sequence's start takes nothing from before
-        if (state_only && i == 0) f.dec[blockIdx.x * p.H + h] = w.x.from_start ? -1.f : decay;
       }
     }
   } else if (warp < 16) {
@@ -987,7 +1023,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           commit(&t.in_full);
           commit(&t.empty[sa]);
         }
-      } else if (!ctl.warp_wait(&t.s_ready, ph)) {
+      } else if (it == 0 && !ctl.warp_wait(&t.s_ready, 0)) {
         break;
       }
       if (!ctl.warp_wait(&t.kt_ready[ph], (it >> 1) & 1)) break;
@@ -1022,6 +1058,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     }
   } else {
     // ---- gates: four tokens a lane ----
+    // Without rows the chunks come against the scan's order, and the column
+    // factors reach to the far end of the piece: what the chunks before this
+    // one (after it in the scan) decay by is in `passed`.  The update then adds
+    // up in tensor memory with nothing to scale between chunks.
+    double passed = 0.0;
     for (uint32_t it = 0; w.next(); ++it) {
       double g[4], sum = 0.0;
       float raw[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1065,14 +1106,20 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const bool zero = rev && lane < 8;  // before the chunk's first token the sum is zero
 #pragma unroll
       for (int q = 0; q < 4; ++q) col[q] = zero ? ex2(lx[q]) : ex2((lx[q] - ex) + (ly[q] - ey));
-      const float far = (rev ? (zero ? 1.f : ex2(ex)) : ex2((ex - whole.x) + (ey - whole.y))) * f.sc;
+      float far = (rev ? (zero ? 1.f : ex2(ex)) : ex2((ex - whole.x) + (ey - whole.y))) * f.sc;
+      float all = ex2(rev ? whole.x : -whole.x);
+      if (state_only) {
+        far *= ex2(static_cast<float>(passed * 1.4426950408889634));
+        passed += end;
+        all = ex2(static_cast<float>(passed * 1.4426950408889634));
+      }
       if (it > 0 && !ctl.warp_wait(&t.tab_empty, (it & 1) ^ 1)) break;
       t.lg[lane * 2] = make_float4(lx[0], lx[1], ly[0], ly[1]);
       t.lg[lane * 2 + 1] = make_float4(lx[2], lx[3], ly[2], ly[3]);
       *reinterpret_cast<float4*>(&t.col[lane * 4]) = make_float4(col[0], col[1], col[2], col[3]);
       if ((lane & 7) == 0) t.far[lane >> 3] = far;
       if (lane == 0) {
-        t.total = ex2(rev ? whole.x : -whole.x);
+        t.total = all;
         t.end = whole;
       }
       __syncwarp();
