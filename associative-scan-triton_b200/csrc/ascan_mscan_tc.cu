@@ -39,7 +39,7 @@
 // cycle, and besides waiting for other roles its warps wait longest for
 // instructions.  Hence one body per form, loop bodies of sixteen columns, and
 // rare work out of line.  65536 tokens: 180 us for the rows (4.5 TB/s of
-// operands and results) after 94 us of carries, at four products of which the
+// operands and results) after 83 us of carries, at four products of which the
 // causal half of two is wasted.
 //
 // Every wait is bounded: one that runs out sets the device error word and an
