@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Laun
   }
 }
 
-// Gate gradients of one stretch of at most p.restart (256 or 1024) tokens: the product of
+// Gate gradients of one stretch of at most p.restart (128, 256 or 1024) tokens: the product of
 // the two states at its end, then the reverse sum of q.dq - k.dk over it.
 // blockIdx.z takes every gridDim.z-th stretch of the segment.
 __global__ void __launch_bounds__(256)
@@ -628,7 +628,7 @@ static int plain_run(const Launch& l, int roles, bool state_only, int dtype, cud
 static int run_forms(Launch& l, int roles, int dtype, cudaStream_t s) {
   int rc = ASCAN_OK;
   const bool tc = tc_usable(l, roles, dtype);
-  l.p.restart = tc && l.p.gate_type != ASCAN_F32 ? kRestart : kRestartMin;
+  l.p.restart = !tc ? kRestartPlain : l.p.gate_type == ASCAN_F32 ? kRestartMin : kRestart;
   for (int r = 0; r < roles; ++r) l.f[r].dot_parts = tc ? tc_dot_parts(l.f[r]) : 1;
   if (l.p.J > 1) {
     rc = tc ? tc_run(l, roles, true, s) : plain_run(l, roles, true, dtype, s);

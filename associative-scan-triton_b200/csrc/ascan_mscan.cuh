@@ -49,11 +49,14 @@ namespace ascan {
 namespace mscan {
 
 // Tokens between stored states.  A float32 gate gradient carries the rounding
-// of every row dot between them: with 1024 tokens 1.1e-5 of its norm on the
-// tensor cores (16-bit operand terms) and 1.3e-6 in float32 arithmetic, with
-// 256 half of that.  A 16-bit gradient needs no more than the longer stretch,
-// whose stores of up to 64 KB a head weigh less.
-constexpr int kRestart = 1024, kRestartMin = 256;
+// of every row dot between them.  On the tensor cores (16-bit operand terms)
+// one chunk's stretch leaves 4.2e-6 of its norm at the median of 700 sizes and
+// 9.4e-6 at most, 256 tokens 5.1e-6 and 1.35e-5; the states' own rounding is
+// the rest, so a rare input still reaches 1.1e-5.  The stores cost 299 -> 340 us
+// at 8 x 2048 tokens x 12 heads of 128 x 128.  Float32 arithmetic takes 256
+// tokens.  A 16-bit gradient needs no more than the longest stretch, whose
+// stores of up to 64 KB a head weigh less.
+constexpr int kRestart = 1024, kRestartPlain = 256, kRestartMin = 128;
 constexpr float kGateFloor = -200.f;  // e^-200 is 0 in float32; keeps -inf out of differences
 
 struct Rows {  // [tokens, heads, dim] with unit stride along dim

@@ -244,6 +244,19 @@ def check_gradients(tensors, lengths, dtype, gate_dtype=F32, **kw):
 
 
 @gpu
+@pytest.mark.parametrize("lengths,heads,dims", [([244], 5, (128, 64)), ([130, 200, 1, 180], 5, (64, 128)),
+                                                ([700, 556], 4, (128, 128)), ([206], 8, (40, 72))], ids=str)
+def test_float32_gate_gradients_of_bfloat16_inputs(lengths, heads, dims):
+  # computed operands keep 16 bits, 2^-17 = 7.6e-6 of a term at most, and the
+  # stretch of rows that a gradient sums is a chunk: below 1e-5 of its norm
+  ours, gold = run_gradients(make(lengths, (heads,) * 4, dims, BF16, carry=True), lengths)
+  at = NAMES.index("d_log_gates")
+  want = gold[at].double()
+  error = ((ours[at].double().cpu() - want).norm() / want.norm()).item()
+  assert error <= 1e-5, error
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("lengths", LENGTHS, ids=str)
 def test_gradient_lengths(lengths, dtype):
