@@ -805,7 +805,6 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
     f.carry = take(w.carry);
     f.dec = w.carry ? reinterpret_cast<float*>(reinterpret_cast<char*>(f.carry) + mat) : nullptr;
     f.rev = r != 0;
-    f.exact = r != 2;  // the gate's gradient needs their rows in float32
     f.sp = scale;
     f.sr = r == 0 ? scale : 1.f;
     f.sc = r == 0 ? 1.f : scale;

@@ -69,7 +69,6 @@ struct Form {
   Rows a, b, c;  // row, column and value operands
   Rows dot;      // optional: row dots of the output with this tensor
   int da, dc, rev;
-  int exact;         // tensor cores: keep 16 bits of every computed operand
   float sp, sr, sc;  // factors of the scores, of the rows and of the columns
   void* out;         // [BL, H, dc]
   int out_f32;

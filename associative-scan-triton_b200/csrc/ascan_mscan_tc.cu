@@ -9,9 +9,9 @@
 //   O      = row . O + P C    P = masked, decayed scores
 //
 // with float32 accumulators in tensor memory.  What is computed on the way to
-// an operand would lose digits as one bfloat16: col.B is split into two
-// (16 bits together), and so are P and S where a float32 result (the gate's
-// gradient) depends on them.  A and C come as stored, so they are exact.
+// an operand would lose digits as one bfloat16: col.B, P and S are each split
+// into two (16 bits together), so that a result keeps its own rounding only,
+// 2^-16 of its size before it.  A and C come as stored, so they are exact.
 //
 // Roles, by warp (one CTA per SM; every hand-over is an mbarrier):
 //   0-7    row warps, two for each 32 tokens: scores -> P in place in tensor
@@ -426,10 +426,10 @@ __device__ __noinline__ void spread_bad(uint32_t tm, const uint32_t* bad, uint32
 // at compile time: the code that a CTA runs has to fit the instruction caches
 // (with all variants in one body the row warps waited longer for instructions
 // than for anything else).
-template <bool REV, bool TWO, bool STATE>
+template <bool REV, bool DOTS, bool STATE>
 __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUtensorMap* map) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  constexpr bool rev = REV, two = TWO, state_only = STATE;
+  constexpr bool rev = REV, state_only = STATE;
   const int da = f.da, dc = f.dc, h = blockIdx.y;
   const TcGeom geo = tc_geom(da, dc);
   unsigned char* s_op = smem + (4 + geo.b_slots) * geo.slot_bytes;
@@ -605,7 +605,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     const bool wide = dc > 64;
     const int c16 = side * (wide ? 4 : 2), c16_end = min(c16 + (wide ? 4 : 2), n16);
     const int block = wide ? side : 0;
-    constexpr bool dots = TWO;  // the forms whose rows the gate's gradient needs
+    constexpr bool dots = DOTS;  // the forms whose rows the gate's gradient needs
     uint32_t dot_loads = 0;
     uint32_t park[8] = {};
     int held = -1;  // slot that the last rows leave from
@@ -670,10 +670,8 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
 #pragma unroll
         for (int c = 0; c < 8; ++c) hi[c] = round2(pv[c]);
         uint32_t lo[8];
-        if (two) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) lo[c] = rest2(pv[c], hi[c]);
-        }
+        for (int c = 0; c < 8; ++c) lo[c] = rest2(pv[c], hi[c]);
         if (b >> 1 == quad || (rev && 16 * b + 16 > w.len)) {
           // the columns that count, as the bits of the packed pairs
           const int from = (rev ? row : 0) - 16 * b, to = (rev ? w.len : row + 1) - 16 * b;
@@ -682,18 +680,16 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           for (int c = 0; c < 8; ++c) {
             const uint32_t bits = (keep & (1u << (2 * c)) ? 0xffffu : 0u) | (keep & (2u << (2 * c)) ? 0xffff0000u : 0u);
             hi[c] &= bits;
-            if (two) lo[c] &= bits;
+            lo[c] &= bits;
           }
         }
         tmem_st8(col + 8 * (b & 1), hi);
-        if (two) {
-          if (b & 1) {
-            tmem_st8(col + 16, park);
-            tmem_st8(col + 24, lo);
-          } else {
+        if (b & 1) {
+          tmem_st8(col + 16, park);
+          tmem_st8(col + 24, lo);
+        } else {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) park[c] = lo[c];
-          }
+          for (int c = 0; c < 8; ++c) park[c] = lo[c];
         }
       }
 #pragma unroll 1
@@ -702,7 +698,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
 #pragma unroll
         for (int c = 0; c < 16; ++c) none[c] = 0u;
         tmem_st16(tm + lanes + kColSc + 32 * b, none);
-        if (two) tmem_st16(tm + lanes + kColSc + 32 * b + 16, none);
+        tmem_st16(tm + lanes + kColSc + 32 * b + 16, none);
       }
       __syncwarp();
       if (lane == 0) bar_arrive(&t.tab_empty);
@@ -922,7 +918,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
               }
               const int at = (((b & 3) * 2 + q) ^ (i & 7)) * 16;
               *reinterpret_cast<uint4*>(base + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              if (two) *reinterpret_cast<uint4*>(base + geo.s_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              *reinterpret_cast<uint4*>(base + geo.s_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
           }
 #pragma unroll
@@ -1016,7 +1012,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         fence_after();
         if (elect_one()) {
 #pragma unroll 1
-          for (int term = 0; term < (two ? 2 : 1); ++term)
+          for (int term = 0; term < 2; ++term)
 #pragma unroll 1
             for (int k = 0; k < ka; ++k)
               mma_smem(tm + kColO, a + (k >> 2) * 1024 + (k & 3) * 2, ds + term * (geo.s_bytes >> 4) + k * 128, id_v, term + k > 0);
@@ -1043,7 +1039,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         fence_after();
         if (elect_one()) {
 #pragma unroll 1
-          for (int term = 0; term < (two ? 2 : 1); ++term)
+          for (int term = 0; term < 2; ++term)
 #pragma unroll 1
             for (int k = 0; k < kC / 16; ++k)
               mma_tmem(tm + kColO, tm + kColSc + (k >> 1) * 32 + (k & 1) * 8 + term * 16, c + k * 128, id_v, true);
@@ -1143,7 +1139,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (STATE) {
     if (f.rev) body<true, false, true>(L.p, f, map);
     else body<false, false, true>(L.p, f, map);
-  } else if (f.exact) {
+  } else if (f.rowdot) {
     if (f.rev) body<true, true, false>(L.p, f, map);
     else body<false, true, false>(L.p, f, map);
   } else {

@@ -350,6 +350,28 @@ def test_gradient_by_differences():
 
 
 @gpu
+@pytest.mark.parametrize("lengths,heads,dims", [([300], (2, 2, 2, 2), (128, 128)), ([130, 0, 71, 400], (4, 2, 4, 4), (64, 128)),
+                                                ([1100], (1, 1, 1, 1), (40, 72)), ([5], (3, 3, 3, 3), (64, 64))], ids=str)
+def test_bfloat16_results_are_rounded_once(lengths, heads, dims):
+  # Computed operands (masked scores, the state, what enters it) keep 16 bits,
+  # so a result is within 2^-16 of its size before its rounding, d = 1.5e-5.  It
+  # then differs from the rounded exact value where a rounding boundary lies
+  # between: in a share d / ulp of the elements, by one ulp (2^-7 of a value at
+  # most), so by sqrt(d * 2^-7) = 3.5e-4 of the norm.  One operand of 8 bits
+  # gives 2^-9 and more.
+  tensors = make(lengths, heads, dims, BF16, seed=2, carry=True)
+  ours, gold = run_gradients(tensors, lengths)
+  q, k, v, g, s0, _, _ = tensors
+  out = ast.matrix_scan_causal(q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), {"cu_seqlens": cu_of(lengths)},
+                               initial_state=s0.to(DEV))
+  want, _ = oracle(q.double(), k.double(), v.double(), g.double(), lengths, dims[0]**-0.5, s0.double())
+  for name, a, b in zip(("out",) + NAMES[:3], (out, *ours), (want, *gold)):
+    rounded = b.to(BF16).double()
+    apart = float((a.double().cpu() - rounded).norm() / rounded.norm())
+    assert apart <= 2.0**-11, (name, apart)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
   lengths = [300, 1000]
