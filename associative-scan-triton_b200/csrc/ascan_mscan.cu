@@ -220,14 +220,15 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 3 : 1)
 #pragma unroll 4
         for (int c = c_from; c < c_to; ++c) outer(&pt[c * LT + r0], ld4(&sm.c[c * LD + d0]));
         // the columns of the rows themselves: masked ones are left out, not
-        // multiplied by zero, so that a NaN there reaches no row
+        // multiplied by zero, so that a NaN there reaches no row; a row's own
+        // comes after the dots, which leave it out
 #pragma unroll
         for (int q = 0; q < R; ++q) {
           if (r0 + q >= len) continue;
           const float4 y = ld4(&sm.c[(r0 + q) * LD + d0]);
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            if (rev ? q >= r : q <= r) fma4(acc[r], pt[(r0 + q) * LT + r0 + r], y);
+            if (rev ? q > r : q < r) fma4(acc[r], pt[(r0 + q) * LT + r0 + r], y);
         }
         const bool vec = dc % 4 == 0 && (reinterpret_cast<uintptr_t>(f.out) & 15u) == 0;
 #pragma unroll
@@ -235,6 +236,13 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 3 : 1)
           const bool on = r0 + r < len;
           const long long t = s0 + r0 + r, at = (t * p.H + h) * dc + d0;
           float dot = 0.f;
+          if (f.rowdot && on && d0 < dc) {
+            const T* x = static_cast<const T*>(f.dot.p) + t * f.dot.st + (h / f.dot.share) * f.dot.sh;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (d0 + q < dc) dot = fmaf(acc[r][q], to_f(x[d0 + q]), dot);
+          }
+          if (on) fma4(acc[r], pt[(r0 + r) * LT + r0 + r], ld4(&sm.c[(r0 + r) * LD + d0]));
           if (on && d0 < dc) {
             if (vec && (f.out_f32 || sizeof(T) == 4)) {
               *reinterpret_cast<float4*>(static_cast<float*>(f.out) + at) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
@@ -245,12 +253,6 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 3 : 1)
                   if (f.out_f32) static_cast<float*>(f.out)[at + q] = acc[r][q];
                   else static_cast<T*>(f.out)[at + q] = from_f<T>(acc[r][q]);
                 }
-            }
-            if (f.rowdot) {
-              const T* x = static_cast<const T*>(f.dot.p) + t * f.dot.st + (h / f.dot.share) * f.dot.sh;
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (d0 + q < dc) dot = fmaf(acc[r][q], to_f(x[d0 + q]), dot);
             }
           }
           if (f.rowdot) {

@@ -26,7 +26,9 @@
 // for any later token e of the sequence.  Taking e at most `restart` tokens
 // away (both state matrices are stored there) keeps the differences short;
 // one sum over a long sequence would lose the digits that the many terms
-// share.
+// share.  Both dots leave out the token's own term (s = t), which is the same
+// in a and b: it does not depend on any gate, while all the rest shrinks with
+// e^g, so at g = -8 a float32 a - b with it would keep two or three digits.
 //
 // Work is split over heads and over segments of `seg` tokens of the packed
 // axis.  A segment that a sequence crosses needs the state that enters it: a
@@ -67,7 +69,7 @@ struct Rows {  // [tokens, heads, dim] with unit stride along dim
 
 struct Form {
   Rows a, b, c;  // row, column and value operands
-  Rows dot;      // optional: row dots of the output with this tensor
+  Rows dot;      // optional: row dots of the output, without each token's own term, with this tensor
   int da, dc, rev;
   float sp, sr, sc;  // factors of the scores, of the rows and of the columns
   void* out;         // [BL, H, dc]

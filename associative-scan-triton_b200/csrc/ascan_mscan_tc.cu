@@ -79,6 +79,7 @@ struct TcTail {
   uint32_t bad[2][kC];
   uint64_t full[6], empty[6];  // slots of A: 0, 1; of C: 2, 3; of B: 4 and, if there is room, 5
   uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
+  uint64_t own_read[4];  // by 32 tokens: the second row warp has its rows' own scores
   float2 end;  // the chunk's whole gate sum, same form
   float total;
   int bad_chunk[2];  // chunk number + 1 when bad[] holds something
@@ -274,6 +275,19 @@ __device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {
          (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
+// Element i of N (a power of two), without indexing registers.
+template <int N>
+__device__ __forceinline__ uint32_t pick(const uint32_t* x, int i) {
+  uint32_t y[N / 2];
+#pragma unroll
+  for (int c = 0; c < N / 2; ++c) y[c] = i & (N / 2) ? x[c + N / 2] : x[c];
+#pragma unroll
+  for (int half = N / 4; half > 0; half /= 2)
+#pragma unroll
+    for (int c = 0; c < half; ++c) y[c] = i & half ? y[c + half] : y[c];
+  return y[0];
+}
+
 // Token of a bad[] entry if it is chunk `it`'s, else -1.
 __device__ __forceinline__ int first_bad(uint32_t key, uint32_t it, bool rev) {
   if (key >> 8 != it + 1) return -1;
@@ -445,7 +459,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) {
       bar_init(&t.full[i], 1);
-      bar_init(&t.empty[i], i < 2 ? (state_only ? 8 : 9) : (i < 4 ? 1 : 5));  // the products, and the row or column warps
+      bar_init(&t.empty[i], i < 2 ? (state_only ? 8 : 9) : (i < 4 ? (DOTS ? 9 : 1) : 5));  // the products, and the row or column warps
     }
     bar_init(&t.tab_full, 1);
     bar_init(&t.tab_empty, state_only ? 12 : 16);
@@ -461,6 +475,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     bar_init(&t.o_free, 8);
     bar_init(&t.d_full, 1);
     bar_init(&t.drain, 1);
+    for (int i = 0; i < 4; ++i) bar_init(&t.own_read[i], 1);
     t.abort = 0;
     t.bad_chunk[0] = t.bad_chunk[1] = 0;
     static_assert(sizeof(TcTail) <= 3072, "the ring of 128-wide tiles leaves no more");
@@ -629,6 +644,21 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const float rf = (rev ? ex2((t.end.x + lx) + (t.end.y + ly)) : ex2(lx)) * f.sr;
       if (!ctl.warp_wait(&t.sc_full, ph)) break;
       fence_after();
+      // A token's own term does not depend on any gate, and with it the dots
+      // would lose the digits of what does: P leaves it out, and it is added
+      // after the dots.  Both warps of the 32 tokens need it; the one whose
+      // columns these are not reads its rows' own scores before P takes their
+      // place.
+      float own = 0.f;
+      if (dots && side != quad >> 1) {
+        uint32_t s[32];
+        tmem_ld32(tm + lanes + kColSc + 32 * quad, s);
+        wait_ld();
+        own = __uint_as_float(pick<32>(s, lane));
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&t.own_read[quad]);
+      }
       // Sixteen columns at a time, those that the mask leaves something of.
       // Where a block of 32 lies wholly inside, the decay is that of the row
       // to the block's edge times col[], two products an element; in the
@@ -636,8 +666,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       // are cleared as bits (a product with zero would keep a NaN).  (Longer loop bodies would run once or
       // twice a chunk and wait for their instructions.)
       const int b0 = 2 * max(2 * side, rev ? quad : 0), b1 = 2 * min(2 * side + 2, rev ? 4 : quad + 1);
+      // The row's own block comes last.
+      bool ok = true;
 #pragma unroll 1
-      for (int b = b0; b < b1; ++b) {
+      for (int i = b0; i < b1; ++i) {
+        const int b = rev ? b0 + b1 - 2 - i + 2 * (i & 1) : i;
         const uint32_t col = tm + lanes + kColSc + 32 * (b >> 1);
         uint32_t s[16], hi[8];
         tmem_ld16(col + 16 * (b & 1), s);
@@ -662,6 +695,17 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           }
         }
         wait_ld();
+        if (dots && b >> 1 == quad) {
+          const float x = __uint_as_float(pick<16>(s, lane & 15));
+          if (b & 1) {
+            own = lane & 16 ? x : own;
+          } else {
+            own = x;
+            ok = ctl.warp_wait(&t.own_read[quad], ph);
+            if (!ok) break;
+            fence_after();
+          }
+        }
 #pragma unroll
         for (int c = 0; c < 8; ++c) pv[c] = mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), pv[c]);
         // P's place is the block's own: first terms in its lower half, second
@@ -674,7 +718,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         for (int c = 0; c < 8; ++c) lo[c] = rest2(pv[c], hi[c]);
         if (b >> 1 == quad || (rev && 16 * b + 16 > w.len)) {
           // the columns that count, as the bits of the packed pairs
-          const int from = (rev ? row : 0) - 16 * b, to = (rev ? w.len : row + 1) - 16 * b;
+          const int from = (rev ? row + dots : 0) - 16 * b, to = (rev ? w.len : row + 1 - dots) - 16 * b;
           const uint32_t keep = below(to) & ~below(from);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -692,6 +736,9 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           for (int c = 0; c < 8; ++c) park[c] = lo[c];
         }
       }
+      if (!ok) break;
+      own *= f.sp;
+      const uint64_t own2 = pair(own, own);
 #pragma unroll 1
       for (int b = max(2 * side, rev ? 0 : quad + 1); b < min(2 * side + 2, rev ? quad : 4); ++b) {  // outside the mask
         uint32_t none[16];
@@ -733,10 +780,20 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       if (lane == 0) bar_arrive(&t.p_ready);
 
       if (dots && !ctl.warp_wait(&t.d_full, ph)) break;
+      if (dots && !ctl.warp_wait(&t.full[2 + ph], (it >> 1) & 1)) break;
       if (!ctl.warp_wait(&t.o_full, ph)) break;
       fence_after();
       if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(tm + lanes + kColO, t.bad[ph], it, rev, row, 16 * c16, min(dc, 16 * c16_end));
       unsigned char* mine = stage + block * 16384 + row * 128;
+      const unsigned char* values = slot_at(2 + ph) + block * 16384 + row * 128;
+      // the own term of eight columns
+      auto add_own = [&](uint64_t* x, int piece) {
+        const uint4 y = *reinterpret_cast<const uint4*>(values + ((piece ^ (row & 7)) << 4));
+        x[0] = fma2(own2, pair(lo_f(y.x), hi_f(y.x)), x[0]);
+        x[1] = fma2(own2, pair(lo_f(y.y), hi_f(y.y)), x[1]);
+        x[2] = fma2(own2, pair(lo_f(y.z), hi_f(y.z)), x[2]);
+        x[3] = fma2(own2, pair(lo_f(y.w), hi_f(y.w)), x[3]);
+      };
       uint64_t dot2 = 0;
 #pragma unroll 1
       for (int b = c16; b < c16_end; ++b) {
@@ -756,6 +813,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
             dot2 = fma2(x[1], pair(lo_f(y.y), hi_f(y.y)), dot2);
             dot2 = fma2(x[2], pair(lo_f(y.z), hi_f(y.z)), dot2);
             dot2 = fma2(x[3], pair(lo_f(y.w), hi_f(y.w)), dot2);
+            if (!f.out_f32) add_own(x, (b & 3) * 2 + q);
           }
           if (!f.out_f32) *piece = make_uint4(round2(x[0]), round2(x[1]), round2(x[2]), round2(x[3]));
         }
@@ -768,6 +826,21 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           tmem_ld16(tm + lanes + kColO + 16 * b, v);
           wait_ld();
           const int half = (wide ? b & 1 : side) * 4, q = lane & 3, r0 = quad * 32 + (lane >> 2);
+          if (dots) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint64_t x[4];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) x[c] = pair(__uint_as_float(v[8 * e + 2 * c]), __uint_as_float(v[8 * e + 2 * c + 1]));
+              add_own(x, (b & 3) * 2 + e);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float lo, hi;
+                unpair(x[c], lo, hi);
+                v[8 * e + 2 * c] = __float_as_uint(lo), v[8 * e + 2 * c + 1] = __float_as_uint(hi);
+              }
+            }
+          }
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -782,7 +855,10 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(&t.o_free);
+      if (lane == 0) {
+        bar_arrive(&t.o_free);
+        if (dots) bar_arrive(&t.empty[2 + ph]);
+      }
       // The warp's 32 rows to memory: whole ones by bulk copies that the slot
       // waits for one chunk later, those at a piece's end by the lanes.
       fence_async();

@@ -372,6 +372,31 @@ def test_bfloat16_results_are_rounded_once(lengths, heads, dims):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("gate", [-1.0, -4.0, -8.0, -12.0])
+@pytest.mark.parametrize("lengths,heads,dims", [([300], 2, (64, 64)), ([70, 1, 401], 2, (128, 128)), ([190], 3, (40, 24))],
+                         ids=str)
+def test_gate_gradients_at_strong_decay(lengths, heads, dims, gate, dtype):
+  # every term of a gate's gradient carries the decay e^gate, and so must the
+  # terms that are summed for it: the usual bounds hold at any gate
+  tensors = list(make(lengths, (heads,) * 4, dims, dtype, seed=6))
+  tensors[3].fill_(gate)
+  ours, gold = run_gradients(tensors, lengths, use=("out",))
+  at = NAMES.index("d_log_gates")
+  close("d_log_gates", ours[at], gold[at], STATE_TOL if dtype != F32 else TOL[F32])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gate_gradients_at_strong_decay_with_states_and_shared_heads(dtype):
+  lengths = [150, 260]
+  tensors = list(make(lengths, (2, 4, 1, 4), (64, 64), dtype, seed=8, carry=True))
+  tensors[3].fill_(-8.0)
+  tensors[3][140:160] = -0.1  # some of the state leaves the first sequence, and enters the second
+  check_gradients(tensors, lengths, dtype)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
   lengths = [300, 1000]
