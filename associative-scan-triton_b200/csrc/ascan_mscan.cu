@@ -152,20 +152,24 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 3 : 1)
       if (tid < 32) {
         const double g0 = 2 * tid < len ? static_cast<double>(load_gate(p, s0 + 2 * tid, h)) : 0.0;
         const double g1 = 2 * tid + 1 < len ? static_cast<double>(load_gate(p, s0 + 2 * tid + 1, h)) : 0.0;
+        // sums in the scan's direction (backwards of all later tokens), never
+        // differences of longer ones: a gate that is not finite must not reach
+        // the tokens before it
         double inc = g0 + g1;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-          const double u = __shfl_up_sync(kFull, inc, o);
-          if (tid >= o) inc += u;
+          const double u = rev ? __shfl_down_sync(kFull, inc, o) : __shfl_up_sync(kFull, inc, o);
+          if (rev ? tid + o < 32 : tid >= o) inc += u;
         }
-        const double end = __shfl_sync(kFull, inc, 31);
+        const double end = __shfl_sync(kFull, inc, rev ? 0 : 31);
+        double before = rev ? __shfl_down_sync(kFull, inc, 1) : __shfl_up_sync(kFull, inc, 1);
+        if (tid == (rev ? 31 : 0)) before = 0.0;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const double g = q ? inc : inc - g1;
-          const float head = expf(static_cast<float>(g)), tail = expf(static_cast<float>(end - g));
+          const double g = rev ? (q ? before : before + g1) : (q ? inc : before + g0);
           sm.g[2 * tid + q] = g;
-          sm.row[2 * tid + q] = (rev ? tail : head) * f.sr;
-          sm.col[2 * tid + q] = (rev ? head : tail) * f.sc;
+          sm.row[2 * tid + q] = expf(static_cast<float>(g)) * f.sr;
+          sm.col[2 * tid + q] = expf(static_cast<float>(end - g)) * f.sc;
         }
         if (tid == 31) sm.total = expf(static_cast<float>(end));
       }
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(kPlainThreads, DM == 64 ? 3 : 1)
           for (int e = 0; e < 4; ++e) {
             const int r = sr0 + e, at = sc0 + c;
             const bool on = (rev ? at >= r : at <= r) && at < len;
-            const double dg = rev ? sm.g[at] - sm.g[r] : sm.g[r] - sm.g[at];
+            const double dg = sm.g[r] - sm.g[at];
             v[e] = on ? sacc[e][c] * f.sp * expf(static_cast<float>(dg)) : 0.f;
           }
           *reinterpret_cast<float4*>(&pt[(sc0 + c) * LT + sr0]) = make_float4(v[0], v[1], v[2], v[3]);

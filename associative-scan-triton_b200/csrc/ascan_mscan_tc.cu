@@ -65,8 +65,9 @@ struct TcMaps {
 
 // Shared memory after the tile slots and the S operand.
 struct TcTail {
-  // Negated gate sums (of the mask's direction) in units of log 2, two tokens
-  // an entry: floats of both, then what the floats leave over
+  // Negated gate sums in units of log 2, up to and with the token (backwards:
+  // of all after it), two tokens an entry: floats of both, then what the
+  // floats leave over
   float4 lg[kC / 2];
   // col[s]: the decay between token s and the edge of its 32 tokens (their
   // last, or backwards the token before their first); far[b]: from there to
@@ -80,7 +81,6 @@ struct TcTail {
   uint64_t full[6], empty[6];  // slots of A: 0, 1; of C: 2, 3; of B: 4 and, if there is room, 5
   uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
   uint64_t own_read[4];  // by 32 tokens: the second row warp has its rows' own scores
-  float2 end;  // the chunk's whole gate sum, same form
   float total;
   int bad_chunk[2];  // chunk number + 1 when bad[] holds something
   int abort;
@@ -640,8 +640,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const float4 l4 = t.lg[row >> 1];
       const float lx = (row & 1) ? -l4.y : -l4.x, ly = (row & 1) ? -l4.w : -l4.z;
       const uint64_t lx2 = pair(lx, lx), ly2 = pair(ly, ly);
-      // backwards lx is minus the sum to the row
-      const float rf = (rev ? ex2((t.end.x + lx) + (t.end.y + ly)) : ex2(lx)) * f.sr;
+      const float rf = ex2(lx) * f.sr;
       if (!ctl.warp_wait(&t.sc_full, ph)) break;
       fence_after();
       // A token's own term does not depend on any gate, and with it the dots
@@ -1149,37 +1148,43 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           if (lane * 4 + q < w.len)
             raw[q] = __uint_as_float(static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(p.gate.p) + at + (lane * 4 + q) * p.gate.st)) << 16);
       }
+      // Sums run in the scan's direction and are never differences of longer
+      // ones: a gate that is not finite must not reach the tokens before it.
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int e = 0; e < 4; ++e) {
+        const int q = rev ? 3 - e : e;
+        if (rev) g[q] = sum;
         sum += static_cast<double>(raw[q] < kGateFloor ? kGateFloor : raw[q]);
-        g[q] = sum;
+        if (!rev) g[q] = sum;
       }
       double inc = sum;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
-        const double u = __shfl_up_sync(kFull, inc, o);
-        if (lane >= o) inc += u;
+        const double u = rev ? __shfl_down_sync(kFull, inc, o) : __shfl_up_sync(kFull, inc, o);
+        if (rev ? lane + o < 32 : lane >= o) inc += u;
       }
-      const double end = __shfl_sync(kFull, inc, 31);
+      const double end = __shfl_sync(kFull, inc, rev ? 0 : 31);
+      double before = rev ? __shfl_down_sync(kFull, inc, 1) : __shfl_up_sync(kFull, inc, 1);
+      if (lane == (rev ? 31 : 0)) before = 0.0;
       float lx[4], ly[4], col[4];
       float2 whole;
-      const double y = end * (rev ? 1.4426950408889634 : -1.4426950408889634);
+      const double y = end * -1.4426950408889634;
       whole.x = static_cast<float>(y);
       whole.y = static_cast<float>(y - static_cast<double>(whole.x));
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const double x = (inc - sum + g[q]) * (rev ? 1.4426950408889634 : -1.4426950408889634);
+        const double x = (before + g[q]) * -1.4426950408889634;
         lx[q] = static_cast<float>(x);
         ly[q] = static_cast<float>(x - static_cast<double>(lx[q]));
       }
       // the edge of the lane's 32 tokens: their last, or the one before them
-      const float ex = rev ? __shfl_sync(kFull, lx[3], (lane & 24) - 1) : __shfl_sync(kFull, lx[3], lane | 7);
-      const float ey = rev ? __shfl_sync(kFull, ly[3], (lane & 24) - 1) : __shfl_sync(kFull, ly[3], lane | 7);
-      const bool zero = rev && lane < 8;  // before the chunk's first token the sum is zero
+      float ex = __shfl_sync(kFull, lx[3], rev ? (lane & 24) - 1 : lane | 7);
+      float ey = __shfl_sync(kFull, ly[3], rev ? (lane & 24) - 1 : lane | 7);
+      if (rev && lane < 8) ex = whole.x, ey = whole.y;  // before the chunk's first token
 #pragma unroll
-      for (int q = 0; q < 4; ++q) col[q] = zero ? ex2(lx[q]) : ex2((lx[q] - ex) + (ly[q] - ey));
-      float far = (rev ? (zero ? 1.f : ex2(ex)) : ex2((ex - whole.x) + (ey - whole.y))) * f.sc;
-      float all = ex2(rev ? whole.x : -whole.x);
+      for (int q = 0; q < 4; ++q) col[q] = ex2((lx[q] - ex) + (ly[q] - ey));
+      float far = ex2((ex - whole.x) + (ey - whole.y)) * f.sc;
+      float all = ex2(-whole.x);
       if (state_only) {
         far *= ex2(static_cast<float>(passed * 1.4426950408889634));
         passed += end;
@@ -1190,10 +1195,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       t.lg[lane * 2 + 1] = make_float4(lx[2], lx[3], ly[2], ly[3]);
       *reinterpret_cast<float4*>(&t.col[lane * 4]) = make_float4(col[0], col[1], col[2], col[3]);
       if ((lane & 7) == 0) t.far[lane >> 3] = far;
-      if (lane == 0) {
-        t.total = all;
-        t.end = whole;
-      }
+      if (lane == 0) t.total = all;
       __syncwarp();
       if (lane == 0) bar_arrive(&t.tab_full);
     }

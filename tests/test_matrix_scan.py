@@ -397,6 +397,66 @@ def test_gate_gradients_at_strong_decay_with_states_and_shared_heads(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 31, 32, 127, 130, 257])
+def test_gates_that_are_not_finite_stay_behind_the_mask(at, bad, dtype):
+  # a bad gate at token t reaches no earlier output, no gradient of a later
+  # key or value (their paths start behind it), no earlier query's gradient,
+  # and nothing of another sequence or head
+  lengths = [90, 300, 40]
+  q, k, v, g, _, d_out, _ = make(lengths, (2, 2, 2, 2), (64, 64), dtype)
+  ours_g = g.clone()
+  t = 90 + at
+  ours_g[t, 1] = bad
+  leaves = [x.to(DEV).requires_grad_(True) for x in (q, k, v, ours_g)]
+  out = ast.matrix_scan_causal(*leaves, {"cu_seqlens": cu_of(lengths)})
+  d_q, d_k, d_v, d_g = (x.cpu() for x in torch.autograd.grad(out, leaves, d_out.to(DEV)))
+  gold = [x.double().requires_grad_(True) for x in (q, k, v, g)]
+  want, _ = oracle(*gold, lengths, 64**-0.5)
+  want_q, want_k, want_v, want_g = torch.autograd.grad(want, gold, d_out.double())
+  before = torch.ones(430, 2, dtype=torch.bool)
+  before[t:390, 1] = False  # what the bad gate is not before
+  after = torch.ones(430, 2, dtype=torch.bool)
+  after[90:t, 1] = False
+  apart = before & after  # ... nor its gradient's terms
+  apart[90:390, 1] = False
+  if at > 0:
+    assert not torch.isfinite(out[t, 1]).all()
+  for name, got, gold, keep in (("out", out.detach().cpu(), want, before), ("d_queries", d_q, want_q, before),
+                                ("d_keys", d_k, want_k, after), ("d_values", d_v, want_v, after)):
+    close(name, got[keep], gold[keep], TOL[dtype])
+  close("d_log_gates", d_g[apart], want_g[apart], STATE_TOL)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("where", [0, 1, 2, 3])
+def test_gradients_of_values_that_are_not_finite_stay_behind_the_mask(where, bad, dtype):
+  # queries and upstream gradients reach their own and earlier tokens' key and
+  # value gradients, keys and values the later queries' and each other's row
+  lengths = [90, 150, 40]
+  q, k, v, g, _, d_out, _ = make(lengths, (2, 2, 2, 2), (64, 64), dtype)
+  gold = [x.double().requires_grad_(True) for x in (q, k, v)]
+  want, _ = oracle(*gold, g.double(), lengths, 64**-0.5)
+  want = torch.autograd.grad(want, gold, d_out.double())
+  inputs = [q, k, v, d_out]
+  t = 90 + 71
+  inputs[where] = inputs[where].clone()
+  inputs[where][t, 1, 5] = bad
+  leaves = [x.to(DEV).requires_grad_(True) for x in inputs[:3]]
+  out = ast.matrix_scan_causal(*leaves, g.to(DEV), {"cu_seqlens": cu_of(lengths)})
+  found = torch.autograd.grad(out, leaves, inputs[3].to(DEV))
+  row, earlier, later, none = slice(t, t + 1), slice(90, t + 1), slice(t, 240), slice(0, 0)
+  reached = ((none, earlier, earlier), (later, none, row), (later, row, none), (row, earlier, earlier))[where]
+  for name, got, gold, rows in zip(NAMES, found, want, reached):
+    keep = torch.ones(280, 2, dtype=torch.bool)
+    keep[rows, 1] = False
+    close(name, got.cpu()[keep], gold[keep], TOL[dtype])
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
   lengths = [300, 1000]
