@@ -324,7 +324,9 @@ def matrix_scan_step(
   Args:
     queries, keys: [B, heads, Dk]; values: [B, heads, Dv]; log_gates: [B, heads].
     state: [S, H, Dk, Dv] float32, a pool of states; updated in place unless
-      ``state_out`` (same shape) receives the new states instead.
+      ``state_out`` (same shape) receives the new states instead.  The write
+      counts as one of torch's in-place operations: a backward that saved the
+      tensor raises.
     slots: [B] int32, each request's state in the pool (no two alike); row b
       itself if None.  A negative slot marks a row without a request: its
       output is zero and no state is touched.
@@ -365,6 +367,8 @@ def matrix_scan_step(
       *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],
       _ptr(slots), batch, state.shape[0], heads, key_dim, value_dim, DTYPE_CODES[queries.dtype],
       scale, state.data_ptr(), state_out.data_ptr(), out.data_ptr(), _stream(device))
+  # the write goes past torch: a scan that saved this state must refuse its backward
+  torch.autograd.graph.increment_version(state_out)
   _lib._finish(rc, "ascan_matrix_scan_step", device)
   return out
 

@@ -715,6 +715,39 @@ def test_step_pool_beyond_32_bit_offsets():
   close("state", pool[slots.long()], new, 1e-6)
 
 
+@gpu
+@pytest.mark.parametrize("stepped", ["final_state", "initial_state", "other"])
+def test_backward_refuses_a_state_that_a_step_has_overwritten(stepped):
+  # the scan's gradients need the states as they were; a step in place shows in
+  # the tensor's version like any of torch's own writes
+  q, k, v, g, s0, _, d_final = (x.to(DEV) for x in make([20, 9], (2, 2, 2, 2), (16, 16), F32, carry=True))
+  out, final = ast.matrix_scan_causal(q.clone().requires_grad_(True), k, v, g, {"cu_seqlens": cu_of([20, 9])},
+                                      initial_state=s0, return_final_state=True)
+  pool = {"final_state": final.detach(), "initial_state": s0, "other": torch.zeros_like(s0)}[stepped]
+  version = pool._version
+  ast.matrix_scan_step(q[:2], k[:2], v[:2], g[:2], pool)
+  assert pool._version > version
+  if stepped == "other":
+    torch.autograd.backward([out, final], [out.detach(), d_final])
+  else:
+    with pytest.raises(RuntimeError, match="inplace operation"):
+      torch.autograd.backward([out, final], [out.detach(), d_final])
+
+
+@gpu
+def test_step_marks_only_what_it_writes():
+  q, k, v, g, _, _, _ = (x if x is None else x.to(DEV) for x in make([3], (2, 2, 2, 2), (16, 16), F32))
+  pool, other = torch.zeros(3, 2, 16, 16, device=DEV), torch.zeros(3, 2, 16, 16, device=DEV)
+  was = pool._version, other._version
+  ast.matrix_scan_step(q, k, v, g, pool, state_out=other)
+  assert pool._version == was[0] and other._version > was[1]
+  with torch.inference_mode():  # such tensors have no version to mark
+    made = torch.zeros(3, 2, 16, 16, device=DEV)
+    out = ast.matrix_scan_step(q, k, v, g, made)
+    assert torch.equal(made, other)
+    assert torch.equal(ast.matrix_scan_step(q, k, v, g, pool), out)
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
