@@ -246,19 +246,19 @@ class MatrixScanCausal(torch.autograd.Function):
   def forward(ctx, queries, keys, values, log_gates, cu_seqlens, scale, initial_state, want_final):
     out, final = _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_state,
                                want_final)
-    ctx.save_for_backward(queries, keys, values, log_gates, initial_state, final)
-    ctx.cu_seqlens, ctx.scale = cu_seqlens, scale
+    ctx.save_for_backward(queries, keys, values, log_gates, cu_seqlens, initial_state, final)
+    ctx.scale = scale
     ctx.set_materialize_grads(False)
     return out, final
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, d_out, d_final):
-    queries, keys, values, log_gates, initial_state, final = ctx.saved_tensors
     if d_out is None and d_final is None:
       return (None,) * 8
+    queries, keys, values, log_gates, cu_seqlens, initial_state, final = ctx.saved_tensors
     d_queries, d_keys, d_values, d_gates, d_initial = _scan_backward(
-      queries, keys, values, log_gates, ctx.cu_seqlens, ctx.scale, initial_state, final, d_out, d_final)
+      queries, keys, values, log_gates, cu_seqlens, ctx.scale, initial_state, final, d_out, d_final)
     return d_queries, d_keys, d_values, d_gates, None, None, d_initial, None
 
 
@@ -485,8 +485,9 @@ class QkNormRotate(torch.autograd.Function):
   @staticmethod
   def forward(ctx, queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
               interleaved):
-    ctx.save_for_backward(queries, keys, query_weight, key_weight)
-    ctx.rest = (cos, sin, positions, cu_seqlens, eps, interleaved)  # no gradients among them
+    # with the tables and positions: changed in place before the backward, it must raise
+    ctx.save_for_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens)
+    ctx.eps, ctx.interleaved = eps, interleaved
     ctx.set_materialize_grads(False)
     return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
                            eps, interleaved)
@@ -496,7 +497,7 @@ class QkNormRotate(torch.autograd.Function):
   def backward(ctx, d_q, d_k):
     if d_q is None and d_k is None:
       return (None,) * 10
-    return (*_rotate_backward(*ctx.saved_tensors, *ctx.rest, d_q, d_k), *(None,) * 6)
+    return (*_rotate_backward(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_q, d_k), *(None,) * 6)
 
 
 def qk_norm_rotate(

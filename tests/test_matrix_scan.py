@@ -609,6 +609,17 @@ def test_abi_rejects_bad_arguments_without_a_gpu():
   assert lib.ascan_matrix_scan_workspace(4096, 1, 2, 2, 2, 2, 2, 64, 64, 1) > small
 
 
+@gpu
+def test_backward_refuses_cu_seqlens_changed_since():
+  # a loop that packs into one buffer: the backward must not read the next batch's ends
+  q, k, v, g, _, d_out, _ = (x if x is None else x.to(DEV) for x in make([30, 20], (2, 2, 2, 2), (16, 16), F32))
+  cu = cu_of([30, 20])
+  out = ast.matrix_scan_causal(q.requires_grad_(True), k, v, g, {"cu_seqlens": cu})
+  cu[1] = 10
+  with pytest.raises(RuntimeError, match="inplace operation"):
+    out.backward(d_out)
+
+
 # ---------------------------------------------------------------------------
 # one token
 # ---------------------------------------------------------------------------

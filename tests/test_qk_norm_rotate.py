@@ -262,3 +262,16 @@ def test_empty():
   yq, yk = ast.qk_norm_rotate(q, q, w, w, cos, sin, positions=torch.empty(0, dtype=torch.int64, device=DEV))
   (yq.sum() + yk.sum()).backward()
   assert not w.grad.any()
+
+
+@gpu
+@pytest.mark.parametrize("changed", ["cos", "sin", "positions", "cu_seqlens"])
+def test_backward_refuses_tables_and_positions_changed_since(changed):
+  q, k, wq, wk, dq, dk = (x.to(DEV) for x in make(9, 2, 1, 16, F32))
+  cos, sin = (x.to(DEV) for x in tables(20, 8))
+  at = {"positions": torch.arange(9, device=DEV), "cu_seqlens": torch.tensor([0, 4, 9], device=DEV)}
+  where = {"args": {"cu_seqlens": at["cu_seqlens"]}} if changed == "cu_seqlens" else {"positions": at["positions"]}
+  y = ast.qk_norm_rotate(q.requires_grad_(True), k, wq, wk, cos, sin, **where)
+  {"cos": cos, "sin": sin, **at}[changed].add_(0 if changed == "cu_seqlens" else 1)
+  with pytest.raises(RuntimeError, match="inplace operation"):
+    torch.autograd.backward(y, (dq, dk))
