@@ -22,6 +22,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DTYPE_CODES, INDEX_CODES
@@ -145,6 +146,14 @@ def _check_operands(queries, keys, values, log_gates, max_dim):
   return device, tokens, heads, key_dim, value_dim
 
 
+def _refuse_tangents(error: type, name: str, *tensors: torch.Tensor | None) -> None:
+  """Forward-mode derivatives: the native call would drop the tangents without a word."""
+  if forward_ad._current_level >= 0:
+    for t in tensors:
+      if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+        raise error(f"{name} has no derivatives in forward mode, and an input has a tangent")
+
+
 class _on:
   """Makes ``device`` current for a launch; free when it is already."""
 
@@ -168,6 +177,7 @@ class _on:
 
 
 def _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_state, want_final):
+  _refuse_tangents(NotImplementedError, "matrix_scan_causal", queries, keys, values, log_gates, initial_state)
   device, tokens, heads, key_dim, value_dim = _check_operands(queries, keys, values, log_gates,
                                                               MAX_DIM)
   _check_index("cu_seqlens", cu_seqlens, device)
@@ -339,6 +349,7 @@ def matrix_scan_step(
                                   or values.requires_grad or log_gates.requires_grad
                                   or state.requires_grad):
     raise ValueError("matrix_scan_step has no backward; use matrix_scan_causal, or torch.no_grad()")
+  _refuse_tangents(ValueError, "matrix_scan_step", queries, keys, values, log_gates, state, state_out)
   if batch > 65535:
     raise ValueError(f"at most 65535 requests per call, got {batch}")
   _check_state("state", state, device, (*state.shape[:1], heads, key_dim, value_dim))
@@ -439,6 +450,7 @@ def _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, 
 
 def _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
                     interleaved):
+  _refuse_tangents(NotImplementedError, "qk_norm_rotate", queries, keys, query_weight, key_weight, cos, sin)
   _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens)
   device = queries.device
   out_q, out_k = _like(queries), _like(keys)

@@ -833,3 +833,29 @@ def test_compiled_layer_matches_eager():
   a = ast.matrix_scan_step(q, k, v, g, pools[0], slots=slots)
   b = step(q, k, v, g, pools[1], slots)
   assert torch.equal(a, b) and torch.equal(*pools)
+
+
+@gpu
+def test_forward_mode_derivatives_are_refused():
+  # a dual tensor's tangent is not dropped without a word
+  import torch.autograd.forward_ad as forward_ad
+  q, k, v, g, s0, _, _ = (x if x is None else x.to(DEV) for x in make([9], (2, 2, 2, 2), (16, 16), F32, carry=True))
+  args = {"cu_seqlens": cu_of([9])}
+  want = ast.matrix_scan_causal(q, k, v, g, args, initial_state=s0)
+  stepped = ast.matrix_scan_step(q[:1], k[:1], v[:1], g[:1], s0.clone())
+  with forward_ad.dual_level():
+    for i in range(5):
+      x = [q, k, v, g, s0]
+      x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+      with pytest.raises(NotImplementedError):
+        ast.matrix_scan_causal(*x[:4], args, initial_state=x[4])
+      with torch.no_grad(), pytest.raises(NotImplementedError):
+        ast.matrix_scan_causal(*x[:4], args, initial_state=x[4])
+      with pytest.raises(NotImplementedError):
+        ast.matrix_scan_causal_compiled(*x[:4], args, initial_state=x[4])
+      with pytest.raises(ValueError, match="no derivatives"):
+        ast.matrix_scan_step(*(forward_ad.make_dual(y[:1], torch.ones_like(y[:1])) if j == i else y[:1]
+                               for j, y in enumerate((q, k, v, g, s0))))
+    # tensors without a tangent are taken as ever
+    assert torch.equal(ast.matrix_scan_causal(q, k, v, g, args, initial_state=s0), want)
+    assert torch.equal(ast.matrix_scan_step(q[:1], k[:1], v[:1], g[:1], s0.clone()), stepped)

@@ -275,3 +275,22 @@ def test_backward_refuses_tables_and_positions_changed_since(changed):
   {"cos": cos, "sin": sin, **at}[changed].add_(0 if changed == "cu_seqlens" else 1)
   with pytest.raises(RuntimeError, match="inplace operation"):
     torch.autograd.backward(y, (dq, dk))
+
+
+@gpu
+def test_forward_mode_derivatives_are_refused():
+  import torch.autograd.forward_ad as forward_ad
+  q, k, wq, wk, _, _ = (x.to(DEV) for x in make(9, 2, 1, 16, F32))
+  cos, sin = (x.to(DEV) for x in tables(9, 8))
+  pos = torch.arange(9, device=DEV)
+  want = ast.qk_norm_rotate(q, k, wq, wk, cos, sin, positions=pos)
+  with forward_ad.dual_level():
+    for i in range(6):
+      x = [q, k, wq, wk, cos, sin]
+      x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+      with pytest.raises(NotImplementedError):
+        ast.qk_norm_rotate(*x, positions=pos)
+      with pytest.raises(NotImplementedError):
+        ast.qk_norm_rotate_compiled(*x, positions=pos)
+    for a, b in zip(ast.qk_norm_rotate(q, k, wq, wk, cos, sin, positions=pos), want):
+      assert torch.equal(a, b)
