@@ -534,7 +534,8 @@ def qk_norm_rotate(
   Args:
     queries: [BL, Hq, D]; keys: [BL, Hk, D].
     query_weight, key_weight: [D], float32 or the tokens' type.
-    cos, sin: [positions, half] float32, half <= D / 2.
+    cos, sin: [positions, half] float32, half <= D / 2; constants, without
+      gradients.
     args: {"cu_seqlens": ...}: a token's position is its place in its
       sequence, and tokens of no sequence give zero rows; or
     positions: [BL] int32 or int64, every token's row of the tables (outside
@@ -543,6 +544,8 @@ def qk_norm_rotate(
     queries and keys, contiguous, in their type.
   """
   cu_seqlens = None if args is None else args["cu_seqlens"]
+  if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+    raise ValueError("cos and sin get no gradient; detach them")
   if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad
                                   or query_weight.requires_grad or key_weight.requires_grad):
     return QkNormRotate.apply(queries, keys, query_weight, key_weight, cos, sin, positions,
@@ -701,6 +704,8 @@ qk_norm_rotate_fwd_op.register_autograd(_qk_norm_rotate_backward,
 def qk_norm_rotate_compiled(queries, keys, query_weight, key_weight, cos, sin, args=None,
                             positions=None, eps=1e-6, interleaved=False):
   """qk_norm_rotate that torch.compile can trace (same arguments and results)."""
+  if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+    raise ValueError("cos and sin get no gradient; detach them")
   return qk_norm_rotate_fwd_op(queries, keys, query_weight, key_weight, cos, sin, positions,
                                None if args is None else args["cu_seqlens"], float(eps),
                                bool(interleaved))

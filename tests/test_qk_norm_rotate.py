@@ -294,3 +294,19 @@ def test_forward_mode_derivatives_are_refused():
         ast.qk_norm_rotate_compiled(*x, positions=pos)
     for a, b in zip(ast.qk_norm_rotate(q, k, wq, wk, cos, sin, positions=pos), want):
       assert torch.equal(a, b)
+
+
+@gpu
+def test_tables_that_want_a_gradient_are_refused():
+  q, k, wq, wk, _, _ = (x.to(DEV) for x in make(9, 2, 1, 16, F32))
+  cos, sin = (x.to(DEV) for x in tables(9, 8))
+  pos = torch.arange(9, device=DEV)
+  for name in ("cos", "sin"):
+    leaf = {"cos": cos, "sin": sin}[name].clone().requires_grad_(True)
+    for queries in (q, q.clone().requires_grad_(True)):
+      with pytest.raises(ValueError, match="no gradient"):
+        ast.qk_norm_rotate(queries, k, wq, wk, **{"cos": cos, "sin": sin, name: leaf}, positions=pos)
+      with pytest.raises(ValueError, match="no gradient"):
+        ast.qk_norm_rotate_compiled(queries, k, wq, wk, **{"cos": cos, "sin": sin, name: leaf}, positions=pos)
+    with torch.no_grad():
+      ast.qk_norm_rotate(q, k, wq, wk, **{"cos": cos, "sin": sin, name: leaf}, positions=pos)
