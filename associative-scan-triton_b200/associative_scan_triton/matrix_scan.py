@@ -319,6 +319,11 @@ def matrix_scan_causal(
 # ---------------------------------------------------------------------------
 
 
+def _state_ptr(state: torch.Tensor, any_other: torch.Tensor) -> int:
+  """A pool of no states has no address, and none of it is read: every slot lies outside."""
+  return state.data_ptr() or any_other.data_ptr()
+
+
 def matrix_scan_step(
   queries: torch.Tensor,
   keys: torch.Tensor,
@@ -370,14 +375,12 @@ def matrix_scan_step(
   out = torch.empty((batch, heads, value_dim), dtype=values.dtype, device=device)
   if batch == 0:
     return out
-  if state.shape[0] == 0:
-    return out.zero_()
   scale = float(key_dim) ** -0.5 if scale is None else float(scale)
   with _on(device):
     rc = _lib.load().ascan_matrix_scan_step(
       *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],
       _ptr(slots), batch, state.shape[0], heads, key_dim, value_dim, DTYPE_CODES[queries.dtype],
-      scale, state.data_ptr(), state_out.data_ptr(), out.data_ptr(), _stream(device))
+      scale, _state_ptr(state, out), _state_ptr(state_out, out), out.data_ptr(), _stream(device))
   # the write goes past torch: a scan that saved this state must refuse its backward
   torch.autograd.graph.increment_version(state_out)
   _lib._finish(rc, "ascan_matrix_scan_step", device)

@@ -759,6 +759,18 @@ def test_step_marks_only_what_it_writes():
     assert torch.equal(ast.matrix_scan_step(q, k, v, g, pool), out)
 
 
+@gpu
+def test_step_with_an_empty_pool():
+  # slots are checked against a pool of no states like any other
+  q, k, v, g, _, _, _ = (x if x is None else x.to(DEV) for x in make([3], (2, 2, 2, 2), (16, 16), F32))
+  pool = torch.empty(0, 2, 16, 16, device=DEV)
+  idle = torch.full((3,), -1, dtype=torch.int32, device=DEV)
+  assert not ast.matrix_scan_step(q, k, v, g, pool, slots=idle).any()
+  with pytest.raises(ast.ScanError, match="slot"):
+    ast.matrix_scan_step(q, k, v, g, pool, slots=idle + 1)
+    ast.check_device_error()
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
