@@ -871,3 +871,63 @@ def test_forward_mode_derivatives_are_refused():
     # tensors without a tangent are taken as ever
     assert torch.equal(ast.matrix_scan_causal(q, k, v, g, args, initial_state=s0), want)
     assert torch.equal(ast.matrix_scan_step(q[:1], k[:1], v[:1], g[:1], s0.clone()), stepped)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)], ids=str)
+@pytest.mark.parametrize("lengths", [[2500], [77, 2300, 123]], ids=str)
+def test_gradients_across_stored_states(lengths, dtype, gate_dtype):
+  # 50 heads fill the SMs with one or two segments of the packed axis, so a
+  # piece of a sequence is longer than the stretch (128 to 1024 tokens) over
+  # which a gate's gradient is summed, and states are stored inside it
+  tensors = make(lengths, (50,) * 4, (16, 16), dtype, seed=12, gate_dtype=gate_dtype, carry=True, rate=0.02)
+  check_gradients(tensors, lengths, dtype, gate_dtype=gate_dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_shared_heads_across_stored_states(dtype):
+  lengths = [40, 1500]
+  tensors = make(lengths, (10, 5, 50, 50), (16, 24), dtype, seed=13, carry=True, rate=0.05)
+  check_gradients(tensors, lengths, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_step_rotation_and_gradients_in_a_graph(dtype):
+  lengths = [130, 60]
+  q, k, v, g, s0, d_out, d_final = (x.to(DEV) for x in make(lengths, (2, 1, 2, 2), (64, 64), dtype, carry=True))
+  args = {"cu_seqlens": cu_of(lengths)}
+  angle = torch.rand(130, 32, generator=torch.Generator().manual_seed(1)).to(DEV)
+  cos, sin, weight = angle.cos(), angle.sin(), torch.ones(64, device=DEV, dtype=dtype)
+  pool, other = torch.randn(5, 2, 64, 64, device=DEV), torch.zeros(5, 2, 64, 64, device=DEV)
+  slots = torch.tensor([3, -1, 0], dtype=torch.int32, device=DEV)
+
+  def call():
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, g, s0, weight)]
+    yq, yk = ast.qk_norm_rotate(leaves[0], leaves[1], leaves[5], leaves[5], cos, sin, args)
+    out, final = ast.matrix_scan_causal(yq, yk, *leaves[2:4], args, initial_state=leaves[4], return_final_state=True)
+    grads = torch.autograd.grad([out, final], leaves, [d_out, d_final])
+    new = ast.matrix_scan_step(q[:3], k[:3], v[:3], g[:3], pool, slots=slots, state_out=other)
+    return [out, final, new, other, *grads]
+
+  first = [x.detach().clone() for x in call()]
+  sync_check = _lib.sync_check_enabled()
+  _lib.set_sync_check(False)  # a synchronisation is not allowed while capturing
+  try:
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+      call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      captured = call()
+    for x in captured:
+      x.detach().zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+  finally:
+    _lib.set_sync_check(sync_check)
+  for a, b in zip(first, captured):
+    assert torch.equal(a, b)
