@@ -64,6 +64,7 @@ EXPORTED_SYMBOLS = (
   "ascan_backward_bidi",
   "ascan_shift_pad",
   "ascan_matrix_scan_workspace",
+  "ascan_matrix_scan_workspace_of",
   "ascan_matrix_scan_forward",
   "ascan_matrix_scan_backward",
   "ascan_matrix_scan_step",
@@ -150,6 +151,8 @@ def _bind(lib) -> None:
   f, rows = ctypes.c_float, p  # rows: a pointer to ascan_rows
   lib.ascan_matrix_scan_workspace.restype = sz
   lib.ascan_matrix_scan_workspace.argtypes = [i64, i64, ci, ci, ci, ci, ci, ci, ci, ci]
+  lib.ascan_matrix_scan_workspace_of.restype = sz
+  lib.ascan_matrix_scan_workspace_of.argtypes = [i64, i64, ci, ci, ci, ci, ci, ci, ci, ci, ci, ci]
   lib.ascan_matrix_scan_forward.restype = ci
   lib.ascan_matrix_scan_forward.argtypes = [rows, rows, rows, rows, ci, p, ci, i64, i64, ci, ci, ci,
                                             ci, f, p, p, p, p, sz, p]

@@ -53,7 +53,7 @@ def _like(t: torch.Tensor) -> torch.Tensor:
 
 @functools.lru_cache(maxsize=256)
 def _scan_workspace(*sizes: int) -> int:
-  return _lib.load().ascan_matrix_scan_workspace(*sizes)
+  return _lib.load().ascan_matrix_scan_workspace_of(*sizes)
 
 
 @functools.lru_cache(maxsize=256)
@@ -200,8 +200,9 @@ def _scan_forward(queries, keys, values, log_gates, cu_seqlens, scale, initial_s
   lib = _lib.load()
   with _on(device):
     ws = torch.empty(
-      _scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1],
-                                      values.shape[1], log_gates.shape[1], key_dim, value_dim, 0),
+      _scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1], values.shape[1],
+                      log_gates.shape[1], key_dim, value_dim, DTYPE_CODES[queries.dtype],
+                      DTYPE_CODES[log_gates.dtype], 0),
       dtype=torch.uint8, device=device)
     rc = lib.ascan_matrix_scan_forward(
       *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],
@@ -235,8 +236,9 @@ def _scan_backward(queries, keys, values, log_gates, cu_seqlens, scale, initial_
   lib = _lib.load()
   with _on(device):
     ws = torch.empty(
-      _scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1],
-                                      values.shape[1], log_gates.shape[1], key_dim, value_dim, 1),
+      _scan_workspace(tokens, num_seq, heads, queries.shape[1], keys.shape[1], values.shape[1],
+                      log_gates.shape[1], key_dim, value_dim, DTYPE_CODES[queries.dtype],
+                      DTYPE_CODES[log_gates.dtype], 1),
       dtype=torch.uint8, device=device)
     rc = lib.ascan_matrix_scan_backward(
       *_rows(queries, keys, values, log_gates), DTYPE_CODES[log_gates.dtype],

@@ -634,7 +634,7 @@ static int plain_run(const Launch& l, int roles, bool state_only, int dtype, cud
 static int run_forms(Launch& l, int roles, int dtype, cudaStream_t s) {
   int rc = ASCAN_OK;
   const bool tc = tc_usable(l, roles, dtype);
-  l.p.restart = !tc ? kRestartPlain : l.p.gate_type == ASCAN_F32 ? kRestartMin : kRestart;
+  l.p.restart = restart_of(tc, l.p.gate_type);
   for (int r = 0; r < roles; ++r) l.f[r].dot_parts = tc ? tc_dot_parts(l.f[r]) : 1;
   if (l.p.J > 1) {
     rc = tc ? tc_run(l, roles, true, s) : plain_run(l, roles, true, dtype, s);
@@ -661,16 +661,19 @@ static Fit fit_for(int dtype, int dk, int dv) {
   return {max(dk, dv) <= 64 ? 3 * kSms : kSms, 128};
 }
 
-// Layout of the workspace; the same arithmetic serves the size query.
-static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, int hg, int dk, int dv,
-                      bool backward, Fit fit) {
+// Layout of the workspace; the same arithmetic serves the size query.  Of
+// bfloat16 rows it is not known yet whether the tensor cores take them: room
+// for their stretches, the shorter ones.
+static Plan make_plan(long long BL, long long N, int H, int hq, int hk, int hv, int hg, int dk, int dv, int dtype,
+                      int gate_type, bool backward) {
+  const Fit fit = fit_for(dtype, dk, dv);
   Plan w{};
   w.J = pick_segments(BL, N, static_cast<long long>(H) * (backward ? 3 : 1), fit.granule, fit.room);
   w.seg = ((BL + w.J - 1) / w.J + fit.granule - 1) / fit.granule * fit.granule;
   w.J = (BL + w.seg - 1) / w.seg;
   const size_t mat = static_cast<size_t>(dk) * dv * H * 4;
   w.carry = w.J > 1 ? up(w.J * mat) + up(static_cast<size_t>(w.J) * H * 4) : 0;
-  w.slots = BL / kRestartMin + 1;
+  w.slots = BL / restart_of(dtype == ASCAN_BF16, gate_type) + 1;
   const size_t rows = static_cast<size_t>(BL) * H * 4;
   w.total = w.carry * (backward ? 3 : 1);
   if (backward) {
@@ -734,12 +737,21 @@ extern "C" {
 size_t ascan_matrix_scan_workspace(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads, int key_heads,
                                    int value_heads, int gate_heads, int key_dim, int value_dim, int backward) {
   if (seq_total <= 0 || num_seq <= 0 || num_heads <= 0 || key_dim <= 0 || value_dim <= 0) return 256;
-  size_t need = 0;  // the type is not known here: the larger of its plans
-  for (int dtype : {ASCAN_F32, ASCAN_BF16})
-    need = max(need, make_plan(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads, gate_heads, key_dim,
-                               value_dim, backward != 0, fit_for(dtype, key_dim, value_dim))
-                         .total);
+  size_t need = 0;
+  for (int dtype : {ASCAN_F32, ASCAN_F16, ASCAN_BF16})
+    for (int gate_dtype : {ASCAN_F32, ASCAN_F16, ASCAN_BF16})
+      need = max(need, ascan_matrix_scan_workspace_of(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads,
+                                                      gate_heads, key_dim, value_dim, dtype, gate_dtype, backward));
   return need;
+}
+
+size_t ascan_matrix_scan_workspace_of(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads,
+                                      int key_heads, int value_heads, int gate_heads, int key_dim, int value_dim,
+                                      int dtype, int gate_dtype, int backward) {
+  if (seq_total <= 0 || num_seq <= 0 || num_heads <= 0 || key_dim <= 0 || value_dim <= 0) return 256;
+  return make_plan(seq_total, num_seq, num_heads, query_heads, key_heads, value_heads, gate_heads, key_dim, value_dim,
+                   dtype, gate_dtype, backward != 0)
+      .total;
 }
 
 int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
@@ -753,7 +765,7 @@ int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys,
   if (seq_total == 0 || num_seq == 0) return ASCAN_OK;
   if (!out) return ASCAN_EINVAL;
   const Plan w = make_plan(seq_total, num_seq, num_heads, queries->heads, keys->heads, values->heads, log_gates->heads,
-                           key_dim, value_dim, false, fit_for(dtype, key_dim, value_dim));
+                           key_dim, value_dim, dtype, gate_dtype, false);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
   Launch l{};
   l.p = problem_of(w, log_gates, gate_dtype, cu_seqlens, cu_index_type, num_seq, seq_total, num_heads);
@@ -792,8 +804,8 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
     return ASCAN_EINVAL;
   if (d_final_state && !final_state) return ASCAN_EINVAL;
   const int H = num_heads, dk = key_dim, dv = value_dim;
-  const Plan w = make_plan(seq_total, num_seq, H, queries->heads, keys->heads, values->heads, log_gates->heads, dk, dv, true,
-                           fit_for(dtype, dk, dv));
+  const Plan w = make_plan(seq_total, num_seq, H, queries->heads, keys->heads, values->heads, log_gates->heads, dk, dv, dtype,
+                           gate_dtype, true);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < w.total) return ASCAN_EWORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Launch l{};

@@ -58,7 +58,10 @@ namespace mscan {
 // at 8 x 2048 tokens x 12 heads of 128 x 128.  Float32 arithmetic takes 256
 // tokens.  A 16-bit gradient needs no more than the longest stretch, whose
 // stores of up to 64 KB a head weigh less.
-constexpr int kRestart = 1024, kRestartPlain = 256, kRestartMin = 128;
+constexpr int kRestart16 = 1024, kRestartPlain = 256, kRestartTc = 128;
+inline int restart_of(bool tensor_cores, int gate_type) {
+  return gate_type != ASCAN_F32 ? kRestart16 : (tensor_cores ? kRestartTc : kRestartPlain);
+}
 constexpr float kGateFloor = -200.f;  // e^-200 is 0 in float32; keeps -inf out of differences
 
 struct Rows {  // [tokens, heads, dim] with unit stride along dim

@@ -350,8 +350,14 @@ typedef struct ascan_rows {
 
 /*
  * Bytes of workspace of ascan_matrix_scan_forward (backward = 0) or
- * ascan_matrix_scan_backward (backward = 1).
+ * ascan_matrix_scan_backward (backward = 1): of calls with these types, or
+ * (without _of) enough for any types.  What the types differ in most is how
+ * often the backward stores states: up to eight times as much with float32
+ * gates as with 16-bit ones.
  */
+ASCAN_API size_t ascan_matrix_scan_workspace_of(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads,
+                                                int key_heads, int value_heads, int gate_heads, int key_dim,
+                                                int value_dim, int dtype, int gate_dtype, int backward);
 ASCAN_API size_t ascan_matrix_scan_workspace(int64_t seq_total, int64_t num_seq, int num_heads, int query_heads,
                                              int key_heads, int value_heads, int gate_heads, int key_dim,
                                              int value_dim, int backward);

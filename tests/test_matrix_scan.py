@@ -620,6 +620,27 @@ def test_backward_refuses_cu_seqlens_changed_since():
     out.backward(d_out)
 
 
+def test_workspace_holds_the_states_that_the_types_store():
+  # both directions' states: every 128 tokens for float32 gates on the tensor
+  # cores, every 256 in float32 arithmetic, every 1024 for gates of 16 bits
+  lib = _lib.load()
+  f32, f16, bf16 = 0, 1, 2
+  tokens, heads, dims = 65536, 12, (128, 128)
+  sizes = (tokens, 1, heads, heads, heads, heads, heads, *dims)
+  state = 4 * heads * dims[0] * dims[1]
+  every = lambda n: 2 * (tokens // n + 1) * state
+  fine, coarse = (lib.ascan_matrix_scan_workspace_of(*sizes, bf16, g, 1) for g in (f32, bf16))
+  assert fine - coarse == every(128) - every(1024)
+  fine, coarse = (lib.ascan_matrix_scan_workspace_of(*sizes, f16, g, 1) for g in (f32, f16))
+  assert fine - coarse == every(256) - every(1024)
+  # all else: row dots of both directions in halves, carries of at most 64 segments
+  assert coarse <= every(1024) + 4 * 4 * tokens * heads + 3 * 64 * state + 2**20
+  for backward in (0, 1):
+    most = lib.ascan_matrix_scan_workspace(*sizes, backward)
+    assert most == max(lib.ascan_matrix_scan_workspace_of(*sizes, d, g, backward)
+                       for d in (f32, f16, bf16) for g in (f32, f16, bf16))
+
+
 # ---------------------------------------------------------------------------
 # one token
 # ---------------------------------------------------------------------------
