@@ -5,7 +5,7 @@
 //
 //   scores = A B^T            A, B from shared memory            [128, 128]
 //   O      = A S              S the state entering the chunk     [128, dc]
-//   U     += (col . B)^T C    the state, kept in tensor memory   [da, dc]
+//   U     += (col . B)^T C    what the chunk adds to the state   [da, dc]
 //   O      = row . O + P C    P = masked, decayed scores
 //
 // with float32 accumulators in tensor memory.  What is computed on the way to
@@ -17,8 +17,8 @@
 //   0-7    row warps, two for each 32 tokens: scores -> P in place in tensor
 //          memory, scale O by the row factors, store the finished rows (each
 //          takes one half of the columns; P is the longest part of a chunk)
-//   8-11   state warps: the state from tensor memory to the operand S in
-//          shared memory, scaled back for the next update
+//   8-11   state warps: the decayed operand S and U make the next operand S
+//          in shared memory and, of what its first term leaves over, the next U
 //   12-15  column warps: (col . B)^T transposed into tensor memory; tails and
 //          values that are not finite in C
 //   16     TMA loads of the A, B, C tiles into shared-memory slots
@@ -80,6 +80,7 @@ struct TcTail {
   uint32_t bad[2][kC];
   uint64_t full[6], empty[6];  // slots of A: 0, 1; of C: 2, 3; of B: 4 and, if there is room, 5
   uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
+  uint64_t added[2];     // without rows: the chunk's accumulator has been added to the sum
   uint64_t own_read[4];  // by 32 tokens: the second row warp has its rows' own scores
   float total;
   int bad_chunk[2];  // chunk number + 1 when bad[] holds something
@@ -257,8 +258,16 @@ __device__ __forceinline__ uint32_t round2(uint64_t x) {
   unpair(x, a, b);
   return bf2(a, b);
 }
-__device__ __forceinline__ uint32_t rest2(uint64_t x, uint32_t hi) {
-  return round2(fma2(pair(lo_f(hi), hi_f(hi)), pair(-1.f, -1.f), x));
+__device__ __forceinline__ uint64_t left2(uint64_t x, uint32_t hi) {
+  return fma2(pair(lo_f(hi), hi_f(hi)), pair(-1.f, -1.f), x);
+}
+__device__ __forceinline__ uint32_t rest2(uint64_t x, uint32_t hi) { return round2(left2(x, hi)); }
+
+// x = total * hi + v, eight columns.
+__device__ __forceinline__ void add_state(const uint4& hi, uint64_t total2, const float* v, uint64_t* x) {
+  const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = fma2(total2, pair(lo_f(h[e]), hi_f(h[e])), pair(v[2 * e], v[2 * e + 1]));
 }
 
 // Shared-memory operand descriptors, 128-byte swizzle.  Along the unit-stride
@@ -378,23 +387,32 @@ struct Walk {
   __device__ __forceinline__ bool last() const { return cc == chunks - 1; }
 };
 
-// Row i of a state between tensor memory and global memory, eight columns at
-// a time; `on` is false for lanes without a row.  With unit stride the eights
-// are `hop` floats apart.
-__device__ __noinline__ void put_state(uint32_t tm, float* to, int hop, long long sj, int dc, bool on) {
+// A sequence's last state to global memory, eight columns at a time: `total`
+// times the first term of the operand S that its last chunk began with
+// (`base`: the lane's row; blocks of 64 columns are `block` bytes apart), and
+// what tensor memory holds.  `on` is false for lanes without a row.
+__device__ __noinline__ void put_final(uint32_t tm, const unsigned char* base, int block, int row, float total, float* to,
+                                       long long sj, int dc, bool on) {
+  const uint64_t total2 = pair(total, total);
 #pragma unroll 1
   for (int d = 0; d < dc; d += 8) {
-    uint32_t v[8];
-    tmem_ld8(tm + d, v);
+    uint32_t u[8];
+    tmem_ld8(tm + d, u);
     wait_ld();
     if (!on) continue;
+    const unsigned char* at = base + (d >> 6) * block + ((((d >> 3) ^ row) & 7) << 4);
+    uint64_t x[4];
+    const float* v = reinterpret_cast<const float*>(u);
+    add_state(*reinterpret_cast<const uint4*>(at), total2, v, x);
+    float y[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) unpair(x[q], y[2 * q], y[2 * q + 1]);
     if (sj == 1) {
-      *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<uint4*>(to + 4) = make_uint4(v[4], v[5], v[6], v[7]);
-      to += hop;
+      *reinterpret_cast<float4*>(to + d) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(to + d + 4) = make_float4(y[4], y[5], y[6], y[7]);
     } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) to[(d + q) * sj] = __uint_as_float(v[q]);
+      for (int q = 0; q < 8; ++q) to[(d + q) * sj] = y[q];
     }
   }
 }
@@ -475,6 +493,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     bar_init(&t.o_free, 8);
     bar_init(&t.d_full, 1);
     bar_init(&t.drain, 1);
+    for (int i = 0; i < 2; ++i) bar_init(&t.added[i], 4);
     for (int i = 0; i < 4; ++i) bar_init(&t.own_read[i], 1);
     t.abort = 0;
     t.bad_chunk[0] = t.bad_chunk[1] = 0;
@@ -901,48 +920,70 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     const long long mat = static_cast<long long>(da) * dc;
     const uint32_t ut = tm + lanes + kColU;
     if (state_only) {
-      // One piece: from zero, and at its end what came in, decayed, on top.
+      // One piece: every chunk's contribution comes from a fresh accumulator
+      // (U's place or O's) and is added here, where the operand S is otherwise,
+      // [4 columns][row]; at the end what came in, decayed, on top.
+      const int cap = blocks_a * 64, n32 = (dc + 31) / 32;  // columns beyond dc have places of their own
+      float4* sum = reinterpret_cast<float4*>(s_op) + i;
       uint32_t it = 0;
       float decay = 0.f;
       bool ok = true;
       for (; ok && w.next(); ++it) {
-        if (it == 0) {
-          if (work) get_state(ut, nullptr, 1, dc, false);
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&t.s_ready);
-        }
         ok = ctl.warp_wait(&t.tab_full, it & 1);
+        if (!ok) break;
         decay = t.total;
-        // in step with the products, so that no phase is missed
-        if (ok && it > 0) ok = ctl.warp_wait(&t.u_full[(it - 1) & 1], ((it - 1) >> 1) & 1);
+        __syncwarp();
         if (lane == 0) bar_arrive(&t.tab_empty);
-      }
-      if (ok && it > 0 && ctl.warp_wait(&t.u_full[(it - 1) & 1], ((it - 1) >> 1) & 1)) {
+        ok = ctl.warp_wait(&t.u_full[it & 1], (it >> 1) & 1);
+        if (!ok) break;
         fence_after();
         if (work) {
+#pragma unroll 1
+          for (int b = 0; b < n32; ++b) {
+            float v[32];
+            tmem_ld32((it & 1 ? tm + lanes + kColO : ut) + 32 * b, reinterpret_cast<uint32_t*>(v));
+            wait_ld();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              float4* at = sum + (8 * b + q) * cap;
+              const float4 old = it > 0 ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+              *at = make_float4(old.x + v[4 * q], old.y + v[4 * q + 1], old.z + v[4 * q + 2], old.w + v[4 * q + 3]);
+            }
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&t.added[it & 1]);
+      }
+      if (ok && it > 0) {
+        if (work && i < da) {
           const bool begins = w.x.from_start && f.init;
           const float* from = f.init + (w.x.n * p.H + h) * mat + i * f.si;
           float* to = f.carry + (static_cast<long long>(blockIdx.x) * p.H + h) * mat + static_cast<long long>(i) * dc;
 #pragma unroll 1
-          for (int d = 0; d < dc; d += 8) {
-            uint32_t v[8];
-            tmem_ld8(ut + d, v);
-            wait_ld();
-            if (i >= da) continue;
+          for (int d = 0; d < dc; d += 4) {
+            float4 v = sum[d / 4 * cap];
             if (begins) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                v[q] = __float_as_uint(fmaf(decay, __ldg(from + (d + q) * f.sj), __uint_as_float(v[q])));
+              v.x = fmaf(decay, __ldg(from + d * f.sj), v.x);
+              v.y = fmaf(decay, __ldg(from + (d + 1) * f.sj), v.y);
+              v.z = fmaf(decay, __ldg(from + (d + 2) * f.sj), v.z);
+              v.w = fmaf(decay, __ldg(from + (d + 3) * f.sj), v.w);
             }
-            *reinterpret_cast<uint4*>(to + d) = make_uint4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<uint4*>(to + d + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+            *reinterpret_cast<float4*>(to + d) = v;
           }
         }
         // a piece that holds the sequence's start takes nothing from before
         if (i == 0) f.dec[blockIdx.x * p.H + h] = w.x.from_start ? -1.f : decay;
       }
     }
+    // The state lives in two places: 8 bits of it as the first term of the
+    // operand S, and the rest, below 2^-8 of it, as what the chunk's update
+    // starts from in tensor memory.  So the products add to values of one
+    // chunk's size: they truncate, and over the many chunks of a long sequence
+    // the whole state would lose 6e-5 of its norm to that (65536 tokens, gates
+    // of 0), where now float32 rounds once a chunk.
+    const int block_bytes = geo.s_bytes / blocks_c;
+    uint64_t before2 = 0;  // the decay over the chunk before
     for (uint32_t it = 0; !state_only && w.next(); ++it) {
       const uint32_t ph = it & 1;
       const bool first = w.cc == 0;
@@ -965,14 +1006,17 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       } else if (work && t.bad_chunk[ph ^ 1] == static_cast<int>(it)) {
         spread_bad(ut, t.bad[ph ^ 1], it - 1, rev, -1, 0, dc);
       }
-      if (f.snap && work) {
+      float* snap = nullptr;
+      if (DOTS && f.snap && i < da) {
         const long long edge = rev ? w.s0 + w.len : w.s0;
         if (edge > w.x.ps && edge < w.x.pe && (edge - w.x.ps) % p.restart == 0)
           // both forms' stored states only meet each other, so they may lie as
           // the lanes hold them: whole lines a store
-          put_state(ut, f.snap + (snap_slot(p, edge) * p.H + h) * mat + i * 8, 8 * da, 1, dc, i < da);
+          snap = f.snap + (snap_slot(p, edge) * p.H + h) * mat + i * 8;
       }
       const uint64_t total2 = pair(total, total);
+      const uint32_t keep = first ? 0u : ~0u;
+      if (first) before2 = 0;
       if (work) {
 #pragma unroll 1
         for (int b = 0; b < n16; ++b) {
@@ -981,27 +1025,40 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           wait_ld();
           if (i < rows) {
             // S: row i of 64 columns is 128 bytes; two 16-byte pieces per 16 columns
-            unsigned char* base = s_op + (b >> 2) * (geo.s_bytes / blocks_c) + i * 128;
+            unsigned char* base = s_op + (b >> 2) * block_bytes + i * 128;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
+              uint4* at = reinterpret_cast<uint4*>(base + ((((b & 3) * 2 + q) ^ (i & 7)) << 4));
+              uint4* at_lo = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(at) + geo.s_bytes);
+              uint64_t x[4];
+              uint4 old = *at;
+              old.x &= keep, old.y &= keep, old.z &= keep, old.w &= keep;
+              add_state(old, before2, v + 8 * q, x);
+              if (DOTS && snap && 16 * b + 8 * q < dc) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) unpair(x[e], y[2 * e], y[2 * e + 1]);
+                float4* to = reinterpret_cast<float4*>(snap + (2 * b + q) * 8 * da);
+                to[0] = make_float4(y[0], y[1], y[2], y[3]);
+                to[1] = make_float4(y[4], y[5], y[6], y[7]);
+              }
               uint32_t hi[4], lo[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const uint64_t x = pair(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
-                hi[e] = round2(x);
-                lo[e] = rest2(x, hi[e]);
+                hi[e] = round2(x[e]);
+                x[e] = left2(x[e], hi[e]);
+                lo[e] = round2(x[e]);
+                unpair(mul2(x[e], total2), v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
               }
-              const int at = (((b & 3) * 2 + q) ^ (i & 7)) * 16;
-              *reinterpret_cast<uint4*>(base + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              *reinterpret_cast<uint4*>(base + geo.s_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *at_lo = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
           }
-#pragma unroll
-          for (int q = 0; q < 16; q += 2) unpair(mul2(pair(v[q], v[q + 1]), total2), v[q], v[q + 1]);
           tmem_st16(ut + 16 * b, reinterpret_cast<const uint32_t*>(v));
         }
         wait_st();
       }
+      before2 = total2;
       fence_async();
       fence_before();
       __syncwarp();
@@ -1011,7 +1068,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         fence_after();
         if (work) {
           if (t.bad_chunk[ph] == static_cast<int>(it) + 1) spread_bad(ut, t.bad[ph], it, rev, -1, 0, dc);
-          put_state(ut, f.fin + (w.x.n * p.H + h) * mat + i * f.si, 8, f.sj, dc, i < da);
+          put_final(ut, s_op + i * 128, block_bytes, i, total, f.fin + (w.x.n * p.H + h) * mat + i * f.si, f.sj, dc, i < da);
         }
       }
     }
@@ -1094,7 +1151,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           commit(&t.in_full);
           commit(&t.empty[sa]);
         }
-      } else if (it == 0 && !ctl.warp_wait(&t.s_ready, 0)) {
+      } else if (it > 1 && !ctl.warp_wait(&t.added[ph], ((it >> 1) & 1) ^ 1)) {  // accumulators take turns
         break;
       }
       if (!ctl.warp_wait(&t.kt_ready[ph], (it >> 1) & 1)) break;
@@ -1105,7 +1162,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       if (elect_one()) {
 #pragma unroll 1
         for (int k = 0; k < 2 * kC / 16; ++k)  // both terms lie side by side
-          mma_tmem(tm + kColU, kt + k * 8, c + (k & 7) * 128, id_v, true);
+          mma_tmem(tm + (state_only && ph ? kColO : kColU), kt + k * 8, c + (k & 7) * 128, id_v, !state_only || k > 0);
         commit(&t.u_full[ph]);
         if (state_only) commit(&t.empty[sc]);
       }

@@ -458,6 +458,29 @@ def test_gradients_of_values_that_are_not_finite_stay_behind_the_mask(where, bad
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lengths", [[2048] * 8, [16384]], ids=["2048x8", "16384"])
+def test_states_of_long_memory_do_not_drift(lengths, dtype):
+  # positive operands and gates of 0: a state only grows, and every chunk adds
+  # to one that is larger than itself.  A chunk's own sums are good to 2^-22,
+  # and the states that they are added to in float32 round 128 times at most,
+  # by 2^-25 on average and either way: 2^-21 of the norm together
+  heads, d = 12, 128
+  total, n = sum(lengths), len(lengths)
+  gen = torch.Generator(device=DEV).manual_seed(4)
+  q, k, v, d_out = (torch.randn(total, heads, d, generator=gen, device=DEV).abs().to(dtype) for _ in range(4))
+  gates = torch.zeros(total, heads, device=DEV)
+  s0 = torch.zeros(n, heads, d, d, device=DEV, requires_grad=True)
+  out, final = ast.matrix_scan_causal(q, k, v, gates, {"cu_seqlens": cu_of(lengths)}, scale=1.0, initial_state=s0,
+                                      return_final_state=True)
+  (d_initial,) = torch.autograd.grad(out, s0, d_out)
+  for name, got, a, b in (("final_state", final, k, v), ("d_initial_state", d_initial, q, d_out)):
+    want = torch.einsum("nthi,nthj->nhij", *(x.double().view(n, -1, heads, d) for x in (a, b)))
+    apart = float((got.double() - want).norm() / want.norm())
+    assert apart <= 2.0**-21, (name, apart)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
   lengths = [300, 1000]
   q, k, v, g, s0, _, _ = (x if x is None else x.to(DEV)
