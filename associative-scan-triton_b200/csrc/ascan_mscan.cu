@@ -781,6 +781,7 @@ int ascan_matrix_scan_forward(const ascan_rows* queries, const ascan_rows* keys,
   f.out = out;
   f.init = initial_state;
   f.fin = final_state;
+  f.fine = final_state != nullptr;
   f.si = value_dim;
   f.sj = 1;
   f.carry = reinterpret_cast<float*>(at);
@@ -823,6 +824,7 @@ int ascan_matrix_scan_backward(const ascan_rows* queries, const ascan_rows* keys
     f.carry = take(w.carry);
     f.dec = w.carry ? reinterpret_cast<float*>(reinterpret_cast<char*>(f.carry) + mat) : nullptr;
     f.rev = r != 0;
+    f.fine = r == 2 ? d_initial_state != nullptr : gate_dtype == ASCAN_F32;
     f.sp = scale;
     f.sr = r == 0 ? scale : 1.f;
     f.sc = r == 0 ? 1.f : scale;

@@ -74,6 +74,7 @@ struct Form {
   Rows a, b, c;  // row, column and value operands
   Rows dot;      // optional: row dots of the output, without each token's own term, with this tensor
   int da, dc, rev;
+  int fine;          // tensor cores: a float32 result depends on the state, so keep all bits of what enters it
   float sp, sr, sc;  // factors of the scores, of the rows and of the columns
   void* out;         // [BL, H, dc]
   int out_f32;

@@ -11,7 +11,8 @@
 // with float32 accumulators in tensor memory.  What is computed on the way to
 // an operand would lose digits as one bfloat16: col.B, P and S are each split
 // into two (16 bits together), so that a result keeps its own rounding only,
-// 2^-16 of its size before it.  A and C come as stored, so they are exact.
+// 2^-16 of its size before it; and col.B into three (24 bits) where a float32
+// result depends on the state.  A and C come as stored, so they are exact.
 //
 // Roles, by warp (one CTA per SM; every hand-over is an mbarrier):
 //   0-7    row warps, two for each 32 tokens: scores -> P in place in tensor
@@ -26,7 +27,8 @@
 //   18     the chunk's gate sums, row and column factors
 //
 // Tensor memory (512 columns of 128 lanes): scores/P 128, O 128, U 128,
-// (col.B)^T 64 + 64.  Lanes are tokens for scores and O, state rows for U.
+// (col.B)^T 128: two terms of all tokens, or three of half of them at a time.
+// Lanes are tokens for scores and O, state rows for U.
 //
 // A token whose value is not finite would reach earlier rows of its chunk
 // through 0 * NaN; the column warps replace such values by zero and note the
@@ -79,7 +81,7 @@ struct TcTail {
   // a maximum finds it and nothing has to be cleared
   uint32_t bad[2][kC];
   uint64_t full[6], empty[6];  // slots of A: 0, 1; of C: 2, 3; of B: 4 and, if there is room, 5
-  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
+  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], kt_free[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
   uint64_t added[2];     // without rows: the chunk's accumulator has been added to the sum
   uint64_t own_read[4];  // by 32 tokens: the second row warp has its rows' own scores
   float total;
@@ -458,7 +460,7 @@ __device__ __noinline__ void spread_bad(uint32_t tm, const uint32_t* bad, uint32
 // at compile time: the code that a CTA runs has to fit the instruction caches
 // (with all variants in one body the row warps waited longer for instructions
 // than for anything else).
-template <bool REV, bool DOTS, bool STATE>
+template <bool REV, bool DOTS, bool STATE, bool FINE>
 __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUtensorMap* map) {
   extern __shared__ __align__(1024) unsigned char smem[];
   constexpr bool rev = REV, state_only = STATE;
@@ -484,8 +486,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     bar_init(&t.sc_full, 1);
     bar_init(&t.in_full, 1);
     bar_init(&t.p_ready, 8);
-    bar_init(&t.kt_ready[0], state_only ? 8 : 4);
-    bar_init(&t.kt_ready[1], state_only ? 8 : 4);
+    for (int i = 0; i < 2; ++i) bar_init(&t.kt_ready[i], 4), bar_init(&t.kt_free[i], 1);
     bar_init(&t.u_full[0], 1);
     bar_init(&t.u_full[1], 1);
     bar_init(&t.s_ready, 4);
@@ -518,11 +519,20 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   auto slot_of_b = [&](uint32_t it) { return state_only ? static_cast<int>(it & 1) : (geo.b_slots == 2 ? 4 + static_cast<int>(it & 1) : 4); };
   auto phase_of_b = [&](uint32_t it) { return state_only || geo.b_slots == 2 ? (it >> 1) & 1 : it & 1; };
   Walk<REV, STATE> w(p);
+  // (col . B)^T in two bfloat16 terms, or three where a float32 result depends
+  // on the state, by halves of the chunk's tokens.  A term of a half takes 32
+  // columns.  With rows there are four such places: of three terms, the second
+  // half's take turns with the first's.  Without rows each half has four of its
+  // own (kColK's, or the scores'): two terms of two chunks, or three of one.
+  constexpr int terms = FINE ? 3 : 2;
+  auto kt_at = [&](int half, int term, uint32_t ph) {
+    if (state_only) return tm + (half ? kColK : kColSc) + 32 * (term + (FINE ? 0 : 2 * ph));
+    return tm + kColK + 32 * ((terms * half + term) & 3);
+  };
 
   // The column role.  Without rows the first four row warps take it too, and
   // each four build one half of the chunk's operand.
   auto columns = [&](int part) {
-    constexpr int span = state_only ? kC / 2 : kC;
     const int i = (warp & 3) * 32 + lane;
     const bool work = i < blocks_a * 64;
     // The warp's 32 rows of (col.B)^T: matrix m of a load has rows 8 m.. and 8
@@ -533,16 +543,12 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       const int slot_b = slot_of_b(it), slot_c = 2 + ph;
       const unsigned char* bt = slot_at(slot_b);
       unsigned char* ct = slot_at(slot_c);
-      // An update is done: its operand may be overwritten.  The previous one's,
-      // when outputs are computed, which also shows that the row and state
-      // warps have read what bad[ph] held two chunks ago; else the one before,
-      // since the scores' place holds a second operand.
-      const uint32_t before = state_only ? 2 : 1;
-      if (it >= before) {
-        if (!ctl.warp_wait(&t.u_full[(it - before) & 1], ((it - before) >> 1) & 1)) break;
+      // The update before is done: its operand may be overwritten, and the row
+      // and state warps have read what bad[ph] held two chunks ago.
+      if (!state_only && it > 0) {
+        if (!ctl.warp_wait(&t.u_full[ph ^ 1], ((it - 1) >> 1) & 1)) break;
         fence_after();
       }
-      const uint32_t kt = tm + lanes + (state_only && ph ? kColSc : kColK);
       if (!state_only || w.len < kC)
         if (!ctl.warp_wait(&t.full[slot_c], (it >> 1) & 1)) break;
       if (state_only) {
@@ -580,50 +586,70 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       fence_async();
       if (!ctl.warp_wait(&t.tab_full, ph)) break;
       if (!ctl.warp_wait(&t.full[slot_b], phase_of_b(it))) break;
-      if (work) {
-        const uint32_t src = smem_u32(bt) + lead;
-        const bool tail = w.len < kC;
+      const uint32_t src = smem_u32(bt) + lead;
+      const bool tail = w.len < kC;
+      bool ok = true;
 #pragma unroll 1
-        for (int s0 = part * span; s0 < part * span + span; s0 += 16) {
-          uint32_t hi[8], lo[8];  // [half of the rows][8 tokens][rows 0-7, 8-15]
-          const float fb = t.far[s0 >> 5];
-          const uint64_t fb2 = pair(fb, fb);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint32_t r[4];
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                         : "r"(src + (s0 + 8 * g) * 128)
-                         : "memory");
-            const int s = s0 + 8 * g + 2 * (lane & 3);
-            const float2 cf = *reinterpret_cast<const float2*>(&t.col[s]);
-            if (tail) {  // select, not multiply: the rows there are another sequence's
-              const uint32_t keep = (s < w.len ? 0xffffu : 0u) | (s + 1 < w.len ? 0xffff0000u : 0u);
-#pragma unroll
-              for (int m = 0; m < 4; ++m) r[m] &= keep;
-            }
-            const uint64_t cf2 = mul2(pair(cf.x, cf.y), fb2);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), cf2);
-              const int at = (m >> 1) * 4 + g * 2 + (m & 1);
-              hi[at] = round2(x);
-              lo[at] = rest2(x, hi[at]);
-            }
-          }
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const uint32_t to = kt + (static_cast<uint32_t>(m) << 20) + s0 / 2;
-            tmem_st16x128(to, hi + 4 * m);
-            tmem_st16x128(to + 64, lo + 4 * m);
-          }
+      for (int half = state_only ? part : 0; half < (state_only ? part + 1 : 2); ++half) {
+        // the places are free when the update that last used them is done
+        if (state_only && !FINE) {
+          if (it > 1) ok = ctl.warp_wait(&t.u_full[ph], ((it >> 1) & 1) ^ 1);
+        } else if (state_only) {
+          if (it > 0) ok = ctl.warp_wait(&t.kt_free[half], ph ^ 1);
+        } else if (FINE && half == 1) {
+          ok = ctl.warp_wait(&t.kt_free[0], ph);
         }
-        wait_st();
+        if (!ok) break;
+        if (FINE || state_only) fence_after();
+        if (work) {
+          const uint32_t k0 = kt_at(half, 0, ph) + lanes, k1 = kt_at(half, 1, ph) + lanes, k2 = kt_at(half, 2, ph) + lanes;
+#pragma unroll 1
+          for (int s1 = 0; s1 < kC / 2; s1 += 16) {
+            const int s0 = half * (kC / 2) + s1;
+            uint32_t hi[8], lo[8], least[8];  // [half of the rows][8 tokens][rows 0-7, 8-15]
+            const float fb = t.far[s0 >> 5];
+            const uint64_t fb2 = pair(fb, fb);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint32_t r[4];
+              asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                           : "r"(src + (s0 + 8 * g) * 128)
+                           : "memory");
+              const int s = s0 + 8 * g + 2 * (lane & 3);
+              const float2 cf = *reinterpret_cast<const float2*>(&t.col[s]);
+              if (tail) {  // select, not multiply: the rows there are another sequence's
+                const uint32_t keep = (s < w.len ? 0xffffu : 0u) | (s + 1 < w.len ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) r[m] &= keep;
+              }
+              const uint64_t cf2 = mul2(pair(cf.x, cf.y), fb2);
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                uint64_t x = mul2(pair(lo_f(r[m]), hi_f(r[m])), cf2);
+                const int at = (m >> 1) * 4 + g * 2 + (m & 1);
+                hi[at] = round2(x);
+                x = left2(x, hi[at]);
+                lo[at] = round2(x);
+                if (FINE) least[at] = rest2(x, lo[at]);
+              }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const uint32_t to = (static_cast<uint32_t>(m) << 20) + s1 / 2;
+              tmem_st16x128(k0 + to, hi + 4 * m);
+              tmem_st16x128(k1 + to, lo + 4 * m);
+              if (FINE) tmem_st16x128(k2 + to, least + 4 * m);
+            }
+          }
+          wait_st();
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&t.kt_ready[half]);
       }
-      fence_before();
-      __syncwarp();
+      if (!ok) break;
       if (lane == 0) {
-        bar_arrive(&t.kt_ready[ph]);
         bar_arrive(&t.tab_empty);
         bar_arrive(&t.empty[slot_b]);
       }
@@ -1120,9 +1146,25 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     const uint32_t id_sc = idesc(kC, false), id_v = idesc((dc + 15) / 16 * 16, true);
     const int ka = (da + 15) / 16;
     const uint64_t ds = desc(smem_u32(s_op), geo.s_bytes / blocks_c);
+    // U += (col . B)^T C over 64 tokens, small terms first: the fewer products
+    // truncate at full size
+    auto update = [&](int half, uint32_t ph, uint64_t c) {
+      if (elect_one()) {
+#pragma unroll 1
+        for (int term = terms - 1; term >= 0; --term) {
+          const uint32_t kt = kt_at(half, term, ph);
+#pragma unroll 1
+          for (int k = 0; k < kC / 32; ++k)
+            mma_tmem(tm + (state_only && ph ? kColO : kColU), kt + k * 8, c + (half * 4 + k) * 128, id_v,
+                     !state_only || half + k > 0 || term < terms - 1);
+        }
+        commit(&t.kt_free[half]);
+      }
+    };
     for (uint32_t it = 0; w.next(); ++it) {
       const uint32_t ph = it & 1;
       const int sa = ph, sb = slot_of_b(it), sc = 2 + ph;
+      const uint64_t c = desc(smem_u32(slot_at(sc)), 16384);
       if (!ctl.warp_wait(&t.full[sb], phase_of_b(it))) break;
       if (!state_only) {
         if (!ctl.warp_wait(&t.full[sa], (it >> 1) & 1)) break;
@@ -1140,6 +1182,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           commit(&t.empty[sb]);
         }
         if (!ctl.warp_wait(&t.s_ready, ph)) break;
+        // the update's first half only waits for the state to have been read
+        if (!ctl.warp_wait(&t.kt_ready[0], ph)) break;
+        if (!ctl.warp_wait(&t.full[sc], (it >> 1) & 1)) break;
+        fence_after();
+        update(0, ph, c);
         if (it > 0 && !ctl.warp_wait(&t.o_free, ph ^ 1)) break;
         fence_after();
         if (elect_one()) {
@@ -1151,18 +1198,17 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
           commit(&t.in_full);
           commit(&t.empty[sa]);
         }
-      } else if (it > 1 && !ctl.warp_wait(&t.added[ph], ((it >> 1) & 1) ^ 1)) {  // accumulators take turns
-        break;
+      } else {
+        if (it > 1 && !ctl.warp_wait(&t.added[ph], ((it >> 1) & 1) ^ 1)) break;  // accumulators take turns
+        if (!ctl.warp_wait(&t.full[sc], (it >> 1) & 1)) break;
+        if (!ctl.warp_wait(&t.kt_ready[0], ph)) break;
+        fence_after();
+        update(0, ph, c);
       }
-      if (!ctl.warp_wait(&t.kt_ready[ph], (it >> 1) & 1)) break;
-      if (!ctl.warp_wait(&t.full[sc], (it >> 1) & 1)) break;
+      if (!ctl.warp_wait(&t.kt_ready[1], ph)) break;
       fence_after();
-      const uint64_t c = desc(smem_u32(slot_at(sc)), 16384);
-      const uint32_t kt = tm + (state_only && ph ? kColSc : kColK);
+      update(1, ph, c);
       if (elect_one()) {
-#pragma unroll 1
-        for (int k = 0; k < 2 * kC / 16; ++k)  // both terms lie side by side
-          mma_tmem(tm + (state_only && ph ? kColO : kColU), kt + k * 8, c + (k & 7) * 128, id_v, !state_only || k > 0);
         commit(&t.u_full[ph]);
         if (state_only) commit(&t.empty[sc]);
       }
@@ -1266,21 +1312,24 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
   }
 }
 
+template <bool STATE, bool FINE>
+__device__ __forceinline__ void dispatch(const Problem& p, const Form& f, const CUtensorMap* map) {
+  if (!STATE && f.rowdot) {
+    if (f.rev) body<true, true, false, FINE>(p, f, map);
+    else body<false, true, false, FINE>(p, f, map);
+  } else {
+    if (f.rev) body<true, false, STATE, FINE>(p, f, map);
+    else body<false, false, STATE, FINE>(p, f, map);
+  }
+}
+
 template <bool STATE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     tc_kernel(const __grid_constant__ Launch L, const __grid_constant__ TcMaps maps) {
   const Form& f = L.f[blockIdx.z];
   const CUtensorMap* map = maps.m[blockIdx.z];
-  if (STATE) {
-    if (f.rev) body<true, false, true>(L.p, f, map);
-    else body<false, false, true>(L.p, f, map);
-  } else if (f.rowdot) {
-    if (f.rev) body<true, true, false>(L.p, f, map);
-    else body<false, true, false>(L.p, f, map);
-  } else {
-    if (f.rev) body<true, false, false>(L.p, f, map);
-    else body<false, false, false>(L.p, f, map);
-  }
+  if (f.fine) dispatch<STATE, true>(L.p, f, map);
+  else dispatch<STATE, false>(L.p, f, map);
 }
 
 static bool map_rows(CUtensorMap* m, const Rows& r, int dim, long long BL, int H, int tokens = kC) {

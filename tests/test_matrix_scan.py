@@ -480,6 +480,24 @@ def test_states_of_long_memory_do_not_drift(lengths, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rate", [0.01, 0.3, 6.0])
+@pytest.mark.parametrize("lengths,heads,dims", [([257], 2, (128, 128)), ([130, 0, 71, 400], 3, (64, 128)), ([1300], 1, (128, 64)),
+                                                ([5], 2, (40, 72))], ids=str)
+def test_float32_states_of_bfloat16_inputs(lengths, heads, dims, rate):
+  # what enters a state keeps 24 bits, its decay two factors good to 2^-22, and
+  # it is summed and scaled in float32: 2^-20 of its norm, as float32 inputs have
+  tensors = make(lengths, (heads,) * 4, dims, BF16, seed=3, carry=True, rate=rate)
+  q, k, v, g, s0, _, _ = tensors
+  _, final = ast.matrix_scan_causal(q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), {"cu_seqlens": cu_of(lengths)},
+                                    initial_state=s0.to(DEV), return_final_state=True)
+  _, want = oracle(q.double(), k.double(), v.double(), g.double(), lengths, dims[0]**-0.5, s0.double())
+  ours, gold = run_gradients(tensors, lengths)
+  for name, a, b in (("final_state", final, want), (NAMES[4], ours[4], gold[4])):
+    apart = float((a.double().cpu() - b).norm() / b.norm())
+    assert apart <= 2.0**-20, (name, apart)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
   lengths = [300, 1000]
