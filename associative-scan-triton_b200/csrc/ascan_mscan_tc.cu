@@ -82,7 +82,7 @@ struct TcTail {
   // a maximum finds it and nothing has to be cleared
   uint32_t bad[2][kC];
   uint64_t full[6], empty[6];  // slots of A: 0, 1; of C: 2, 3; of B: 4 and, if there is room, 5
-  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[2], kt_free[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
+  uint64_t tab_full, tab_empty, sc_full, in_full, p_ready, kt_ready[4], kt_free[2], u_full[2], s_ready, o_full, o_free, d_full, drain;
   uint64_t added[2];     // without rows: the chunk's accumulator has been added to the sum
   uint64_t own_read[4];  // by 32 tokens: the second row warp has its rows' own scores
   float total;
@@ -463,7 +463,8 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     bar_init(&t.sc_full, 1);
     bar_init(&t.in_full, 1);
     bar_init(&t.p_ready, 8);
-    for (int i = 0; i < 2; ++i) bar_init(&t.kt_ready[i], 4), bar_init(&t.kt_free[i], 1);
+    for (int i = 0; i < 4; ++i) bar_init(&t.kt_ready[i], 4);
+    for (int i = 0; i < 2; ++i) bar_init(&t.kt_free[i], 1);
     bar_init(&t.u_full[0], 1);
     bar_init(&t.u_full[1], 1);
     bar_init(&t.s_ready, 4);
@@ -506,6 +507,12 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     if (state_only) return tm + (half ? kColK : kColSc) + 32 * (term + (FINE ? 0 : 2 * ph));
     return tm + kColK + 32 * ((terms * half + term) & 3);
   };
+
+  // A half's terms are ready.  Without rows the columns may be two chunks ahead
+  // of the products, so its barrier alternates with the chunks: one's parity
+  // would be back where it was.
+  auto kt_bar = [&](int half, uint32_t it) { return &t.kt_ready[state_only ? half + 2 * (it & 1) : half]; };
+  auto kt_parity = [&](uint32_t it) { return (state_only ? it >> 1 : it) & 1; };
 
   // The column role.  Without rows the first four row warps take it too, and
   // each four build one half of the chunk's operand.
@@ -623,7 +630,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&t.kt_ready[half]);
+        if (lane == 0) bar_arrive(kt_bar(half, it));
       }
       if (!ok) break;
       if (lane == 0) {
@@ -1160,7 +1167,7 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
         }
         if (!ctl.warp_wait(&t.s_ready, ph)) break;
         // the update's first half only waits for the state to have been read
-        if (!ctl.warp_wait(&t.kt_ready[0], ph)) break;
+        if (!ctl.warp_wait(kt_bar(0, it), kt_parity(it))) break;
         if (!ctl.warp_wait(&t.full[sc], (it >> 1) & 1)) break;
         fence_after();
         update(0, ph, c);
@@ -1178,11 +1185,11 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
       } else {
         if (it > 1 && !ctl.warp_wait(&t.added[ph], ((it >> 1) & 1) ^ 1)) break;  // accumulators take turns
         if (!ctl.warp_wait(&t.full[sc], (it >> 1) & 1)) break;
-        if (!ctl.warp_wait(&t.kt_ready[0], ph)) break;
+        if (!ctl.warp_wait(kt_bar(0, it), kt_parity(it))) break;
         fence_after();
         update(0, ph, c);
       }
-      if (!ctl.warp_wait(&t.kt_ready[1], ph)) break;
+      if (!ctl.warp_wait(kt_bar(1, it), kt_parity(it))) break;
       fence_after();
       update(1, ph, c);
       if (elect_one()) {
