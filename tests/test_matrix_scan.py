@@ -498,6 +498,23 @@ def test_float32_states_of_bfloat16_inputs(lengths, heads, dims, rate):
 
 
 @gpu
+@pytest.mark.parametrize("lengths,dims", [([2600], (64, 64)), ([100, 2300, 3], (128, 128)), ([1024, 1024, 512], (40, 72))], ids=str)
+def test_bfloat16_across_segments_without_float32_results(lengths, dims):
+  # nothing float32 is asked for: what enters a state keeps 16 bits, and the
+  # outputs and gradients are held to the same bounds
+  tensors = make(lengths, (1, 1, 1, 1), dims, BF16, seed=15, gate_dtype=BF16, rate=0.02)
+  q, k, v, g, _, d_out, _ = tensors
+  leaves = [x.to(DEV).requires_grad_(True) for x in (q, k, v, g)]
+  out = ast.matrix_scan_causal(*leaves, {"cu_seqlens": cu_of(lengths)})
+  ours = torch.autograd.grad(out, leaves, d_out.to(DEV))
+  gold = [x.double().requires_grad_(True) for x in (q, k, v, g)]
+  want, _ = oracle(*gold, lengths, dims[0]**-0.5)
+  close("out", out, want, TOL[BF16])
+  for name, a, b in zip(NAMES, ours, torch.autograd.grad(want, gold, d_out.double())):
+    close(name, a, b, TOL[BF16])
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(dtype):
   lengths = [300, 1000]
