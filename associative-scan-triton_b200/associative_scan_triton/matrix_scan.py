@@ -13,7 +13,15 @@ along the first axis, ``args["cu_seqlens"]`` as for the other scans), its last
 dimension has unit stride, and token and head strides are free, so views of a
 packed projection need no copy.  float32, float16 and bfloat16; states, sums
 and norms are float32.  Every call runs on torch's current stream and takes
-its workspace from torch's allocator.
+its workspace from torch's allocator.  No forward-mode derivatives.
+
+Precision: float32 and float16 inputs are computed in float32.  bfloat16
+inputs (head sizes a multiple of 8, 16-byte aligned rows) run on tensor cores:
+what is computed on the way to a product keeps 16 bits, so that a bfloat16
+result carries its own rounding only; what enters a state keeps 24 where a
+float32 result depends on it, and final states and initial states' gradients
+are as good as float32 arithmetic's.  Float32 gate gradients are within
+1e-5 of their norm (3e-6 at the median).
 """
 
 from __future__ import annotations
@@ -297,6 +305,9 @@ def matrix_scan_causal(
     scale: factor of the outputs, Dk**-0.5 by default.
     initial_state: [N, H, Dk, Dv] float32 before each sequence; zero if None.
     return_final_state: also return the float32 state after each sequence.
+  Errors (the module's docstring has the reasons): one rounding of 16-bit
+  results; about 1e-6 of the norm of float32 ones, 1e-5 of that of float32
+  log_gates' gradients.
   Head counts may differ: H is the largest, the others divide it, and head h
   reads head h // (H // heads) of each input; shared heads get the summed
   gradient.  Tokens of no sequence give zero rows.

@@ -19,10 +19,10 @@ constexpr int kPlainChunk = 64;
 // along the rows' unit stride, C as stored; the state stays there from chunk
 // to chunk.  Every product gives a thread a tile of 4 x 4 values (8 x 4 at 128
 // wide), so two (three) 16-byte reads feed 16 (32) multiply-adds.  Measured at
-// 6001 tokens of 12 heads of 64 x 64, float32, forward and gradients: 657 us,
-// a tenth of the multiply-add rate; tiles are loaded without overlap, and
-// three CTAs an SM hide it in part (two: 737 us; tiles of 2 x 4 over 32
-// tokens: 1280 us).
+// 6001 tokens of 12 heads of 64 x 64, float32, forward and gradients: 668 us,
+// 0.19 of the multiply-add rate (9.4 GFLOP); tiles are loaded without overlap,
+// and three CTAs an SM hide it in part (two took a ninth longer, tiles of 2 x 4
+// over 32 tokens twice as long).
 // ---------------------------------------------------------------------------
 
 template <int DM>
@@ -583,9 +583,10 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepA
 constexpr long long kSms = 148;
 
 // What runs at once, and of how many tokens segments are multiples: a chunk of
-// the tensor-core kernel costs about 3 us however few of its tokens are there
-// (128 instead of 256: 257 tokens took 44 us, not 22), the plain one's half
-// chunks do not (128: float32 training 697 us, 256: 777 us).
+// the tensor-core kernel costs about 5 us however few of its tokens are there,
+// and a carry pass comes on top (128 instead of 256: 257 tokens took 53 us, not
+// 34, 16 ragged prompts of 16384 tokens 183 us, not 166); the plain one's
+// granules may be shorter (128: float32 training 690 us, 256: 766 us).
 struct Fit {
   long long room;
   int granule;

@@ -51,13 +51,12 @@ namespace ascan {
 namespace mscan {
 
 // Tokens between stored states.  A float32 gate gradient carries the rounding
-// of every row dot between them.  On the tensor cores (16-bit operand terms)
-// one chunk's stretch leaves 4.2e-6 of its norm at the median of 700 sizes and
-// 9.4e-6 at most, 256 tokens 5.1e-6 and 1.35e-5; the states' own rounding is
-// the rest, so a rare input still reaches 1.1e-5.  The stores cost 299 -> 340 us
-// at 8 x 2048 tokens x 12 heads of 128 x 128.  Float32 arithmetic takes 256
-// tokens.  A 16-bit gradient needs no more than the longest stretch, whose
-// stores of up to 64 KB a head weigh less.
+// of every row dot between them.  On the tensor cores (P and S in 16 bits) one
+// chunk's stretch leaves 2.6e-6 of its norm at the median of 700 sizes, 5.0e-6
+// at the 99th percentile and 6.0e-6 at most; 256 tokens 2.6e-6, 6.2e-6 and
+// 9.8e-6, for 358 us instead of 385 at 8 x 2048 tokens x 12 heads of 128 x 128.
+// Float32 arithmetic takes 256 tokens.  A 16-bit gradient needs no more than
+// the longest stretch, whose stores of up to 64 KB a head weigh less.
 constexpr int kRestart16 = 1024, kRestartPlain = 256, kRestartTc = 128;
 inline int restart_of(bool tensor_cores, int gate_type) {
   return gate_type != ASCAN_F32 ? kRestart16 : (tensor_cores ? kRestartTc : kRestartPlain);

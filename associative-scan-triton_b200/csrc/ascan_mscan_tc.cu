@@ -36,13 +36,14 @@
 // mask lets the value through.
 //
 // What bounds it: the instructions of its roles.  At 16384 tokens of 12 heads
-// of 128 x 128 the forward reads what it must (160 MB) at 35% of the memory
-// rate with the tensor pipe 23% busy; a scheduler issues 0.42 instructions a
-// cycle, and besides waiting for other roles its warps wait longest for
-// instructions.  Hence one body per form, loop bodies of sixteen columns, and
-// rare work out of line.  65536 tokens: 180 us for the rows (4.5 TB/s of
-// operands and results) after 83 us of carries, at four products of which the
-// causal half of two is wasted.
+// of 128 x 128 the forward reads what it must (161 MB) at 27% of the memory
+// rate with the tensor pipe 29% busy; a scheduler issues 0.45 instructions a
+// cycle, and its warps wait for other roles, fixed latencies and instructions.
+// Hence one body per form, loop bodies of sixteen columns, and rare work out
+// of line (a hundred instructions more in the state warps' loop made the rows
+// a sixth slower).  65536 tokens: 237 us for the rows (3.4 TB/s of operands
+// and results) after 111 us of carries, at four products of which the causal
+// half of two is wasted.
 //
 // Every wait is bounded: one that runs out sets the device error word and an
 // abort flag, every role then leaves its loop, loads and products in flight
@@ -1218,8 +1219,8 @@ __device__ __forceinline__ void body(const Problem& p, const Form& f, const CUte
     // ---- gates: four tokens a lane ----
     // Without rows the chunks come against the scan's order, and the column
     // factors reach to the far end of the piece: what the chunks before this
-    // one (after it in the scan) decay by is in `passed`.  The update then adds
-    // up in tensor memory with nothing to scale between chunks.
+    // one (after it in the scan) decay by is in `passed`.  The chunks' updates
+    // then add up with nothing to scale between them.
     double passed = 0.0;
     for (uint32_t it = 0; w.next(); ++it) {
       double g[4], sum = 0.0;
