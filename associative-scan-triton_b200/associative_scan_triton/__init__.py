@@ -8,7 +8,9 @@ in include/ascan.h); CUDA tensors only, no CPU fallback.
 
 Beside the reference's names (``__all__``) the package has the operators of a
 gated linear-attention layer: ``matrix_scan_causal``, ``matrix_scan_step`` and
-``qk_norm_rotate`` (matrix_scan.py), each with a ``*_compiled`` variant.
+``qk_norm_rotate`` (matrix_scan.py), and of the softmax-attention layers that
+stand between them: ``attention_causal``, ``attention_cache_write`` and
+``attention_cache_step`` (attention.py), each with a ``*_compiled`` variant.
 """
 
 __version__ = "1.0.0"
@@ -44,6 +46,16 @@ from associative_scan_triton.matrix_scan import (  # noqa: E402
   matrix_scan_step_compiled,
   qk_norm_rotate,
   qk_norm_rotate_compiled,
+)
+from associative_scan_triton.attention import (  # noqa: E402
+  AttentionCache,
+  attention_cache,
+  attention_cache_step,
+  attention_cache_step_compiled,
+  attention_cache_write,
+  attention_cache_write_compiled,
+  attention_causal,
+  attention_causal_compiled,
 )
 from associative_scan_triton._lib import (  # noqa: E402
   ScanError,

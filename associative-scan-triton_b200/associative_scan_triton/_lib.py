@@ -71,6 +71,14 @@ EXPORTED_SYMBOLS = (
   "ascan_qk_norm_rotate",
   "ascan_qk_norm_rotate_workspace",
   "ascan_qk_norm_rotate_backward",
+  "ascan_qk_norm_rotate_axes",
+  "ascan_qk_norm_rotate_axes_backward",
+  "ascan_attention_forward",
+  "ascan_attention_workspace",
+  "ascan_attention_backward",
+  "ascan_cache_write",
+  "ascan_cache_step_workspace",
+  "ascan_cache_step",
   "ascan_set_implementation",
   "ascan_get_implementation",
   "ascan_set_tile_width",
@@ -89,6 +97,15 @@ class Rows(ctypes.Structure):
 
   _fields_ = [("data", ctypes.c_void_p), ("stride_token", ctypes.c_int64),
               ("stride_head", ctypes.c_int64), ("heads", ctypes.c_int32)]
+
+
+class Cache(ctypes.Structure):
+  """``ascan_cache``: pages of keys and values in 8 bits with their scales."""
+
+  _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+              ("key_scales", ctypes.c_void_p), ("value_scales", ctypes.c_void_p),
+              ("pages", ctypes.c_int64), ("heads", ctypes.c_int32), ("page", ctypes.c_int32),
+              ("key_dim", ctypes.c_int32), ("value_dim", ctypes.c_int32)]
 
 
 class ScanError(RuntimeError):
@@ -171,6 +188,27 @@ def _bind(lib) -> None:
   lib.ascan_qk_norm_rotate_backward.argtypes = [rows, rows, p, p, ci, p, p, i64, ci, ci, p, p, ci,
                                                 i64, i64, ci, ci, f, rows, rows, p, p, p, p, p, sz,
                                                 p]
+  lib.ascan_qk_norm_rotate_axes.restype = ci
+  lib.ascan_qk_norm_rotate_axes.argtypes = [rows, rows, p, p, ci, p, p, i64, ci, ci, p, p, ci, i64,
+                                            i64, ci, ci, f, ci, p, p, p, p]
+  lib.ascan_qk_norm_rotate_axes_backward.restype = ci
+  lib.ascan_qk_norm_rotate_axes_backward.argtypes = [rows, rows, p, p, ci, p, p, i64, ci, ci, p, p,
+                                                     ci, i64, i64, ci, ci, f, ci, p, rows, rows, p,
+                                                     p, p, p, p, sz, p]
+  lib.ascan_attention_forward.restype = ci
+  lib.ascan_attention_forward.argtypes = [rows, rows, rows, p, ci, i64, i64, ci, ci, ci, f, p, p, p,
+                                          p]
+  lib.ascan_attention_workspace.restype = sz
+  lib.ascan_attention_workspace.argtypes = [i64, ci]
+  lib.ascan_attention_backward.restype = ci
+  lib.ascan_attention_backward.argtypes = [rows, rows, rows, rows, p, p, p, p, ci, i64, i64, ci, ci,
+                                           ci, f, p, p, p, p, sz, p]
+  lib.ascan_cache_write.restype = ci
+  lib.ascan_cache_write.argtypes = [rows, rows, p, p, i64, i64, p, ci, p, ci, i64, ci, p]
+  lib.ascan_cache_step_workspace.restype = sz
+  lib.ascan_cache_step_workspace.argtypes = [ci]
+  lib.ascan_cache_step.restype = ci
+  lib.ascan_cache_step.argtypes = [rows, p, p, i64, i64, p, ci, ci, f, p, p, sz, p]
   lib.ascan_set_implementation.restype = ci
   lib.ascan_set_implementation.argtypes = [ci]
   lib.ascan_get_implementation.restype = ci
@@ -279,9 +317,10 @@ def describe_device_error(code: int) -> str:
     parts.append("a peer rank's time-shard record or release did not arrive within the "
                  "bounded wait")
   if code & DEV_ERR_INDEX:
-    parts.append("a state slot or a position lies outside its table")
+    parts.append("a state slot, a position or a page lies outside its table")
   if code & DEV_ERR_STAGE:
-    parts.append("a stage of the matrix scan did not finish within the bounded wait")
+    parts.append("a stage of the matrix scan or of the attention did not finish within the "
+                 "bounded wait")
   return "; ".join(parts) or f"device error {code:#x}"
 
 

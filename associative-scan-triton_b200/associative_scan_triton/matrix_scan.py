@@ -37,7 +37,9 @@ from ._lib import DTYPE_CODES, INDEX_CODES
 
 MAX_DIM = 128  # of a matrix state's sides
 
-_ROWS = {n: ctypes.c_int64 * (4 * n) for n in (2, 4)}
+MAX_AXES = 4  # of positions
+
+_ROWS = {n: ctypes.c_int64 * (4 * n) for n in (1, 2, 3, 4)}
 
 
 def _rows(*tensors: torch.Tensor):
@@ -406,7 +408,7 @@ def matrix_scan_step(
 
 
 def _rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
-                   interleaved):
+                   interleaved, sections):
   """The leading arguments that the two native calls share, by name of their place."""
   index = positions if positions is not None else cu_seqlens
   return (*_rows(queries, keys), query_weight.data_ptr(), key_weight.data_ptr(),
@@ -414,10 +416,31 @@ def _rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions,
           cos.shape[1], int(interleaved), _ptr(positions),
           None if positions is not None else cu_seqlens.data_ptr(), INDEX_CODES[index.dtype],
           0 if positions is not None else cu_seqlens.numel() - 1, queries.shape[0],
-          queries.shape[2], DTYPE_CODES[queries.dtype], eps)
+          queries.shape[2], DTYPE_CODES[queries.dtype], eps, 1 if sections is None else len(sections),
+          None if sections is None else (ctypes.c_int32 * len(sections))(*sections))
 
 
-def _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens):
+def _check_sections(sections, positions, half: int, tokens: int) -> None:
+  if positions is None:
+    raise ValueError("sections need positions, one row of them for each")
+  if not 1 <= len(sections) <= MAX_AXES:
+    raise ValueError(f"between 1 and {MAX_AXES} sections are supported, got {len(sections)}")
+  if min(sections) < 0 or sum(sections) != half:
+    raise ValueError(f"sections {tuple(sections)} do not add up to the tables' {half} columns")
+  if positions.dim() != 2 or positions.shape != (len(sections), tokens) or not positions.is_contiguous():
+    raise ValueError(f"positions must be contiguous [{len(sections)}, {tokens}], a row for each "
+                     f"section, got {tuple(positions.shape)}")
+
+
+def _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
+                  sections=None):
+  if sections is not None:  # then the rest is as with the first axis alone
+    for name, t in (("queries", queries), ("cos", cos), ("positions", positions)):
+      if t is not None:
+        _lib._require_cuda(name, t, None)
+    if cos.dim() == 2 and queries.dim() == 3:  # else refused below
+      _check_sections(sections, positions, cos.shape[1], queries.shape[0])
+      positions = positions[0]
   try:  # the usual call in one expression; whatever fails it is looked at below
     (n, hq, d), (nk, hk, dk), (rows, half) = queries.shape, keys.shape, cos.shape
     device, dtype, wtype = queries.device, queries.dtype, query_weight.dtype
@@ -465,24 +488,24 @@ def _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, 
 
 
 def _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
-                    interleaved):
+                    interleaved, sections=None):
   _refuse_tangents(NotImplementedError, "qk_norm_rotate", queries, keys, query_weight, key_weight, cos, sin)
-  _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens)
+  _check_rotate(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, sections)
   device = queries.device
   out_q, out_k = _like(queries), _like(keys)
   if queries.shape[0] == 0:
     return out_q, out_k
   with _on(device):
-    rc = _lib.load().ascan_qk_norm_rotate(
+    rc = _lib.load().ascan_qk_norm_rotate_axes(
       *_rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
-                      eps, interleaved),
+                      eps, interleaved, sections),
       out_q.data_ptr(), out_k.data_ptr(), _stream(device))
   _lib._finish(rc, "ascan_qk_norm_rotate", device)
   return out_q, out_k
 
 
 def _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
-                     interleaved, d_out_q, d_out_k):
+                     interleaved, d_out_q, d_out_k, sections=None):
   device, tokens = queries.device, queries.shape[0]
   d_q, d_k = _like(queries), _like(keys)
   d_qw, d_kw = torch.empty_like(query_weight), torch.empty_like(key_weight)
@@ -498,9 +521,9 @@ def _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, position
     ws = torch.empty(
       _rotate_workspace(tokens, queries.shape[1], keys.shape[1],
                                          queries.shape[2]), dtype=torch.uint8, device=device)
-    rc = lib.ascan_qk_norm_rotate_backward(
+    rc = lib.ascan_qk_norm_rotate_axes_backward(
       *_rotate_common(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
-                      eps, interleaved),
+                      eps, interleaved, sections),
       *_rows(grads[0], grads[1]), d_q.data_ptr(), d_k.data_ptr(), d_qw.data_ptr(),
       d_kw.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
   _lib._finish(rc, "ascan_qk_norm_rotate_backward", device)
@@ -512,20 +535,21 @@ class QkNormRotate(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens, eps,
-              interleaved):
+              interleaved, sections=None):
     # with the tables and positions: changed in place before the backward, it must raise
     ctx.save_for_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens)
-    ctx.eps, ctx.interleaved = eps, interleaved
+    ctx.eps, ctx.interleaved, ctx.sections = eps, interleaved, sections
     ctx.set_materialize_grads(False)
     return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
-                           eps, interleaved)
+                           eps, interleaved, sections)
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, d_q, d_k):
     if d_q is None and d_k is None:
-      return (None,) * 10
-    return (*_rotate_backward(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_q, d_k), *(None,) * 6)
+      return (None,) * 11
+    return (*_rotate_backward(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_q, d_k, ctx.sections),
+            *(None,) * 7)
 
 
 def qk_norm_rotate(
@@ -539,6 +563,7 @@ def qk_norm_rotate(
   positions: torch.Tensor | None = None,
   eps: float = 1e-6,
   interleaved: bool = False,
+  sections: tuple[int, ...] | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
   """RMS norm per head, weight and rotation of queries and keys, in one pass.
 
@@ -556,18 +581,23 @@ def qk_norm_rotate(
       sequence, and tokens of no sequence give zero rows; or
     positions: [BL] int32 or int64, every token's row of the tables (outside
       them: a zero row, and ScanError as for every device-side check).
+    sections: with positions [axes, BL] (axes <= 4, as of time, height and
+      width): how many of the half pairs turn by each axis, the first ones by
+      the first.  A pair keeps its column of the tables; a token with any
+      position outside them gives a zero row.
   Returns:
     queries and keys, contiguous, in their type.
   """
   cu_seqlens = None if args is None else args["cu_seqlens"]
+  sections = None if sections is None else tuple(int(n) for n in sections)
   if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
     raise ValueError("cos and sin get no gradient; detach them")
   if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad
                                   or query_weight.requires_grad or key_weight.requires_grad):
     return QkNormRotate.apply(queries, keys, query_weight, key_weight, cos, sin, positions,
-                              cu_seqlens, float(eps), bool(interleaved))
+                              cu_seqlens, float(eps), bool(interleaved), sections)
   return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
-                         float(eps), bool(interleaved))
+                         float(eps), bool(interleaved), sections)
 
 
 # ---------------------------------------------------------------------------
@@ -670,15 +700,16 @@ def matrix_scan_step_compiled(queries, keys, values, log_gates, state, slots=Non
 def qk_norm_rotate_fwd_op(queries: torch.Tensor, keys: torch.Tensor, query_weight: torch.Tensor,
                           key_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                           positions: torch.Tensor | None, cu_seqlens: torch.Tensor | None,
-                          eps: float, interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+                          eps: float, interleaved: bool, sections: list[int] | None = None
+                          ) -> tuple[torch.Tensor, torch.Tensor]:
   """qk_norm_rotate."""
   return _rotate_forward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
-                         eps, interleaved)
+                         eps, interleaved, sections)
 
 
 @qk_norm_rotate_fwd_op.register_fake
 def _qk_norm_rotate_fwd_fake(queries, keys, query_weight, key_weight, cos, sin, positions,
-                             cu_seqlens, eps, interleaved):
+                             cu_seqlens, eps, interleaved, sections=None):
   return queries.new_empty(queries.shape), keys.new_empty(keys.shape)
 
 
@@ -687,30 +718,30 @@ def qk_norm_rotate_bwd_op(
   queries: torch.Tensor, keys: torch.Tensor, query_weight: torch.Tensor, key_weight: torch.Tensor,
   cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None,
   cu_seqlens: torch.Tensor | None, eps: float, interleaved: bool, d_queries: torch.Tensor | None,
-  d_keys: torch.Tensor | None
+  d_keys: torch.Tensor | None, sections: list[int] | None = None
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
   """Gradients of queries, keys and the two weights."""
   return _rotate_backward(queries, keys, query_weight, key_weight, cos, sin, positions, cu_seqlens,
-                          eps, interleaved, d_queries, d_keys)
+                          eps, interleaved, d_queries, d_keys, sections)
 
 
 @qk_norm_rotate_bwd_op.register_fake
 def _qk_norm_rotate_bwd_fake(queries, keys, query_weight, key_weight, cos, sin, positions,
-                             cu_seqlens, eps, interleaved, d_queries, d_keys):
+                             cu_seqlens, eps, interleaved, d_queries, d_keys, sections=None):
   return tuple(t.new_empty(t.shape) for t in (queries, keys, query_weight, key_weight))
 
 
 def _qk_norm_rotate_setup(ctx, inputs, output) -> None:
-  *tensors, ctx.eps, ctx.interleaved = inputs
+  *tensors, ctx.eps, ctx.interleaved, ctx.sections = inputs
   ctx.save_for_backward(*tensors)
   ctx.set_materialize_grads(False)
 
 
 def _qk_norm_rotate_backward(ctx, d_queries, d_keys):
   if d_queries is None and d_keys is None:
-    return (None,) * 10
-  return (*qk_norm_rotate_bwd_op(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_queries, d_keys),
-          *(None,) * 6)
+    return (None,) * 11
+  return (*qk_norm_rotate_bwd_op(*ctx.saved_tensors, ctx.eps, ctx.interleaved, d_queries, d_keys,
+                                 ctx.sections), *(None,) * 7)
 
 
 qk_norm_rotate_fwd_op.register_autograd(_qk_norm_rotate_backward,
@@ -718,10 +749,11 @@ qk_norm_rotate_fwd_op.register_autograd(_qk_norm_rotate_backward,
 
 
 def qk_norm_rotate_compiled(queries, keys, query_weight, key_weight, cos, sin, args=None,
-                            positions=None, eps=1e-6, interleaved=False):
+                            positions=None, eps=1e-6, interleaved=False, sections=None):
   """qk_norm_rotate that torch.compile can trace (same arguments and results)."""
   if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
     raise ValueError("cos and sin get no gradient; detach them")
   return qk_norm_rotate_fwd_op(queries, keys, query_weight, key_weight, cos, sin, positions,
                                None if args is None else args["cu_seqlens"], float(eps),
-                               bool(interleaved))
+                               bool(interleaved),
+                               None if sections is None else [int(n) for n in sections])

@@ -34,6 +34,7 @@ using mscan::store_any;
 using mscan::to_f;
 
 constexpr int kRotThreads = 256;
+constexpr int kMaxAxes = ASCAN_ROTATE_MAX_AXES;
 
 struct Side {  // queries or keys
   const void* x;
@@ -55,6 +56,7 @@ struct Args {
   const void *positions, *cu;
   long long rows, N, tokens;
   int index64, half, interleaved, dim, wtype;
+  int axes, edge[kMaxAxes];  // positions are [axes, tokens]; axis i turns the pairs before edge[i]
   float eps;
   uint32_t* err;
 };
@@ -63,10 +65,26 @@ __device__ __forceinline__ long long index_at(const void* p, int is64, long long
   return is64 ? static_cast<const long long*>(p)[i] : static_cast<long long>(static_cast<const int*>(p)[i]);
 }
 
-// Table row of token t; -1: zero row.
-__device__ __forceinline__ long long table_row(const Args& a, long long t) {
+// The axis that pair i turns by.
+__device__ __forceinline__ int axis_of(const Args& a, int i) {
+  int axis = 0;
+  while (axis < a.axes - 1 && i >= a.edge[axis]) ++axis;
+  return axis;
+}
+
+// Table row of token t on one of its axes; -1: zero row (on every axis alike).
+__device__ __forceinline__ long long table_row(const Args& a, long long t, int axis) {
   long long pos;
-  if (a.positions) {
+  if (a.axes > 1) {
+    pos = -1;
+    bool out = false;
+    for (int i = 0; i < a.axes; ++i) {
+      const long long x = index_at(a.positions, a.index64, i * a.tokens + t);
+      out |= x < 0 || x >= a.rows;
+      if (i == axis) pos = x;
+    }
+    if (out) pos = -1;
+  } else if (a.positions) {
     pos = index_at(a.positions, a.index64, t);
   } else {
     long long lo = 0, hi = a.N;  // first sequence that ends beyond t
@@ -162,9 +180,9 @@ struct Place {
 };
 
 // Table row of token t in order; -1: zero row.
-__device__ __forceinline__ long long next_row(const Args& a, long long t, Place& at) {
+__device__ __forceinline__ long long next_row(const Args& a, long long t, int axis, Place& at) {
   if (a.positions || t >= at.end || t < at.start) {
-    const long long row = table_row(a, t);
+    const long long row = table_row(a, t, axis);
     if (!a.positions && row >= 0) {
       at.start = t - row;
       at.end = at.start;
@@ -343,7 +361,8 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? 2 : 3) vec_kernel(const __g
   for (int q = 0; q < DEPTH; ++q) load(q);
   Turn<T, P, BWD> turn;
   Place place;
-  long long row = tokens > 0 ? next_row(a, first, place) : -1;
+  const int axis = axis_of(a, P == kPart ? (gl < hv ? gl : gl - hv) * V : gl * H);  // of all the lane's pairs
+  long long row = tokens > 0 ? next_row(a, first, axis, place) : -1;
   __shared__ float weights[G * V];
   for (int d = threadIdx.x; d < a.dim; d += kRotThreads) weights[d] = load_any(sd.w, a.wtype, d);
   __syncthreads();
@@ -362,7 +381,7 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? 2 : 3) vec_kernel(const __g
     for (int q = 0; q < DEPTH; ++q) {
       if (r + q >= items) break;
       if (ch == 0) {
-        if (ct > 0) row = ct < tokens ? next_row(a, first + ct, place) : -1;
+        if (ct > 0) row = ct < tokens ? next_row(a, first + ct, axis, place) : -1;
         turn.load(a, weights, row, gl);
       }
       const bool live = ct < tokens && ch < heads;
@@ -440,7 +459,10 @@ __global__ void __launch_bounds__(kRotThreads) any_kernel(const __grid_constant_
     for (long long unit = static_cast<long long>(cta) * 8 + warp; unit < units; unit += static_cast<long long>(sd.ctas) * 8) {
       const long long t = unit / sd.heads;
       const int h = static_cast<int>(unit % sd.heads);
-      const long long row = table_row(a, t);
+      long long rows[kMaxAxes];
+#pragma unroll
+      for (int i = 0; i < kMaxAxes; ++i) rows[i] = i < a.axes ? table_row(a, t, i) : -1;
+      const long long row = rows[0];
       const T* x = static_cast<const T*>(sd.x) + t * sd.st + h * sd.sh;
       const T* dy = BWD ? static_cast<const T*>(sd.dy) + t * sd.dst + h * sd.dsh : nullptr;
       // partner of element d, its cosine and its signed sine (in R)
@@ -449,8 +471,12 @@ __global__ void __launch_bounds__(kRotThreads) any_kernel(const __grid_constant_
         if (row < 0 || d >= 2 * a.half) return d;
         const bool low = a.interleaved ? d % 2 == 0 : d < a.half;
         const int at = a.interleaved ? d / 2 : (low ? d : d - a.half);
-        c = a.cos_table[row * a.half + at];
-        s = a.sin_table[row * a.half + at] * (low ? -1.f : 1.f);
+        long long place = row;
+#pragma unroll
+        for (int i = 1; i < kMaxAxes; ++i)
+          if (i < a.axes && at >= a.edge[i - 1]) place = rows[i];
+        c = a.cos_table[place * a.half + at];
+        s = a.sin_table[place * a.half + at] * (low ? -1.f : 1.f);
         return a.interleaved ? (low ? d + 1 : d - 1) : (low ? d + a.half : d - a.half);
       };
       float sq = 0.f;
@@ -598,12 +624,21 @@ static bool rows_vec(const ascan_rows* r, int v) {
 
 static int fill(Args& a, const ascan_rows* q, const ascan_rows* k, const void* wq, const void* wk, int wtype,
                 const float* ct, const float* st, int64_t rows, int half, int interleaved, const void* positions,
-                const void* cu, int itype, int64_t N, int64_t tokens, int dim, int dtype, float eps, void* oq, void* ok) {
+                const void* cu, int itype, int64_t N, int64_t tokens, int dim, int dtype, float eps, void* oq, void* ok,
+                int axes, const int32_t* sections) {
   if (tokens < 0 || tokens > (1ll << 40) || dim <= 0 || dim > (1 << 20) || half < 0 || 2 * half > dim || rows < 0 || N < 0)
     return ASCAN_EINVAL;
   if (dtype < ASCAN_F32 || dtype > ASCAN_BF16 || wtype < ASCAN_F32 || wtype > ASCAN_BF16) return ASCAN_EINVAL;
   if (itype != ASCAN_I32 && itype != ASCAN_I64) return ASCAN_EINVAL;
   if (!positions == !cu) return ASCAN_EINVAL;
+  if (axes < 1 || axes > kMaxAxes || (axes > 1 && (!positions || !sections))) return ASCAN_EINVAL;
+  a.axes = axes;
+  for (int i = 0, sum = 0; i < axes; ++i) {
+    if (axes > 1 && (sections[i] < 0 || sections[i] > half)) return ASCAN_EINVAL;
+    sum += axes > 1 ? sections[i] : half;
+    a.edge[i] = sum;
+    if (i == axes - 1 && sum != half) return ASCAN_EINVAL;
+  }
   if (tokens == 0) return ASCAN_OK;
   if (!side_ok(q) || !side_ok(k) || !wq || !wk || !oq || !ok || (half > 0 && (!ct || !st))) return ASCAN_EINVAL;
   const ascan_rows* r[2] = {q, k};
@@ -638,6 +673,9 @@ static bool vec_ok(const Args& a, const ascan_rows* q, const ascan_rows* k, cons
                    int dtype) {
   const int v = dtype == ASCAN_F32 ? 4 : 8;
   if (a.dim % v || a.dim / v > 32 || a.half % v) return false;
+  const int pairs = a.interleaved || 2 * a.half == a.dim ? v / 2 : v;  // of a lane
+  for (int i = 0; i < a.axes; ++i)
+    if (a.edge[i] % pairs) return false;
   if (!rows_vec(q, v) || !rows_vec(k, v) || !aligned(a.side[0].out) || !aligned(a.side[1].out)) return false;
   if (dq && (!rows_vec(dq, v) || !rows_vec(dk, v))) return false;
   return a.half == 0 || (aligned(a.cos_table) && aligned(a.sin_table));
@@ -650,21 +688,31 @@ using namespace ascan;
 
 extern "C" {
 
-int ascan_qk_norm_rotate(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
+int ascan_qk_norm_rotate_axes(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
                          const void* key_weight, int weight_dtype, const float* cos_table, const float* sin_table,
                          int64_t table_rows, int half, int interleaved, const void* positions, const void* cu_seqlens,
                          int index_type, int64_t num_seq, int64_t tokens, int dim, int dtype, float eps,
-                         void* out_queries, void* out_keys, void* stream) {
+                              int num_axes, const int32_t* sections, void* out_queries, void* out_keys, void* stream) {
   rotate::Args a{};
   const int rc = rotate::fill(a, queries, keys, query_weight, key_weight, weight_dtype, cos_table, sin_table, table_rows,
                               half, interleaved, positions, cu_seqlens, index_type, num_seq, tokens, dim, dtype, eps,
-                              out_queries, out_keys);
+                              out_queries, out_keys, num_axes, sections);
   if (rc != ASCAN_OK || tokens == 0) return rc;
   const bool vec = rotate::vec_ok(a, queries, keys, nullptr, nullptr, dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == ASCAN_F32) return rotate::run<float, false>(a, vec, s);
   if (dtype == ASCAN_F16) return rotate::run<__half, false>(a, vec, s);
   return rotate::run<__nv_bfloat16, false>(a, vec, s);
+}
+
+int ascan_qk_norm_rotate(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
+                         const void* key_weight, int weight_dtype, const float* cos_table, const float* sin_table,
+                         int64_t table_rows, int half, int interleaved, const void* positions, const void* cu_seqlens,
+                         int index_type, int64_t num_seq, int64_t tokens, int dim, int dtype, float eps,
+                         void* out_queries, void* out_keys, void* stream) {
+  return ascan_qk_norm_rotate_axes(queries, keys, query_weight, key_weight, weight_dtype, cos_table, sin_table, table_rows,
+                                   half, interleaved, positions, cu_seqlens, index_type, num_seq, tokens, dim, dtype, eps,
+                                   1, nullptr, out_queries, out_keys, stream);
 }
 
 size_t ascan_qk_norm_rotate_workspace(int64_t tokens, int query_heads, int key_heads, int dim) {
@@ -674,17 +722,18 @@ size_t ascan_qk_norm_rotate_workspace(int64_t tokens, int query_heads, int key_h
   return 256 + static_cast<size_t>(rotate::kMaxCtas + 2) * dim * sizeof(float);
 }
 
-int ascan_qk_norm_rotate_backward(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
+int ascan_qk_norm_rotate_axes_backward(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
                                   const void* key_weight, int weight_dtype, const float* cos_table,
                                   const float* sin_table, int64_t table_rows, int half, int interleaved,
                                   const void* positions, const void* cu_seqlens, int index_type, int64_t num_seq,
-                                  int64_t tokens, int dim, int dtype, float eps, const ascan_rows* d_out_queries,
+                                  int64_t tokens, int dim, int dtype, float eps, int num_axes, const int32_t* sections,
+                                  const ascan_rows* d_out_queries,
                                   const ascan_rows* d_out_keys, void* d_queries, void* d_keys, void* d_query_weight,
                                   void* d_key_weight, void* workspace, size_t workspace_bytes, void* stream) {
   rotate::Args a{};
   const int rc = rotate::fill(a, queries, keys, query_weight, key_weight, weight_dtype, cos_table, sin_table, table_rows,
                               half, interleaved, positions, cu_seqlens, index_type, num_seq, tokens, dim, dtype, eps,
-                              d_queries, d_keys);
+                              d_queries, d_keys, num_axes, sections);
   if (rc != ASCAN_OK || tokens == 0) return rc;
   if (!rotate::side_ok(d_out_queries) || !rotate::side_ok(d_out_keys) || d_out_queries->heads != queries->heads ||
       d_out_keys->heads != keys->heads || !d_query_weight || !d_key_weight)
@@ -709,6 +758,19 @@ int ascan_qk_norm_rotate_backward(const ascan_rows* queries, const ascan_rows* k
   if (dtype == ASCAN_F32) return rotate::run<float, true>(a, vec, s);
   if (dtype == ASCAN_F16) return rotate::run<__half, true>(a, vec, s);
   return rotate::run<__nv_bfloat16, true>(a, vec, s);
+}
+
+int ascan_qk_norm_rotate_backward(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
+                                  const void* key_weight, int weight_dtype, const float* cos_table,
+                                  const float* sin_table, int64_t table_rows, int half, int interleaved,
+                                  const void* positions, const void* cu_seqlens, int index_type, int64_t num_seq,
+                                  int64_t tokens, int dim, int dtype, float eps, const ascan_rows* d_out_queries,
+                                  const ascan_rows* d_out_keys, void* d_queries, void* d_keys, void* d_query_weight,
+                                  void* d_key_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  return ascan_qk_norm_rotate_axes_backward(queries, keys, query_weight, key_weight, weight_dtype, cos_table, sin_table,
+                                            table_rows, half, interleaved, positions, cu_seqlens, index_type, num_seq,
+                                            tokens, dim, dtype, eps, 1, nullptr, d_out_queries, d_out_keys, d_queries,
+                                            d_keys, d_query_weight, d_key_weight, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

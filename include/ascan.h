@@ -64,8 +64,8 @@ enum ascan_status {
 #define ASCAN_DEV_ERR_CU_ORDER 0x2u     /* cu_seqlens not monotone / out of [0, seq_total] */
 #define ASCAN_DEV_ERR_LOOKBACK 0x4u     /* a tile predecessor never published (bounded wait expired) */
 #define ASCAN_DEV_ERR_EXCHANGE 0x8u     /* a peer rank's record or release never came (bounded wait expired) */
-#define ASCAN_DEV_ERR_INDEX 0x10u       /* a state slot or a position lies outside its table */
-#define ASCAN_DEV_ERR_STAGE 0x20u       /* a stage of the matrix scan did not finish (bounded wait expired) */
+#define ASCAN_DEV_ERR_INDEX 0x10u       /* a state slot, a position or a page lies outside its table */
+#define ASCAN_DEV_ERR_STAGE 0x20u       /* a stage of the matrix scan or of the attention did not finish (bounded wait expired) */
 
 /* Library identification. */
 ASCAN_API int ascan_abi_version(void);
@@ -441,6 +441,112 @@ ASCAN_API int ascan_qk_norm_rotate_backward(const ascan_rows* queries, const asc
                                             float eps, const ascan_rows* d_out_queries, const ascan_rows* d_out_keys,
                                             void* d_queries, void* d_keys, void* d_query_weight, void* d_key_weight,
                                             void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same with a position on each of several axes (time, height, width):
+ * the first sections[0] pairs turn by the first axis, the next sections[1] by
+ * the second, and so on; they add up to half.  positions is [num_axes,
+ * tokens]; sections is on the host.  A token with any position outside the
+ * table gives a zero row.  num_axes 1 is the call above.
+ */
+#define ASCAN_ROTATE_MAX_AXES 4
+ASCAN_API int ascan_qk_norm_rotate_axes(const ascan_rows* queries, const ascan_rows* keys, const void* query_weight,
+                                        const void* key_weight, int weight_dtype, const float* cos_table,
+                                        const float* sin_table, int64_t table_rows, int half, int interleaved,
+                                        const void* positions, const void* cu_seqlens, int index_type,
+                                        int64_t num_seq, int64_t tokens, int dim, int dtype, float eps, int num_axes,
+                                        const int32_t* sections, void* out_queries, void* out_keys, void* stream);
+ASCAN_API int ascan_qk_norm_rotate_axes_backward(const ascan_rows* queries, const ascan_rows* keys,
+                                                 const void* query_weight, const void* key_weight, int weight_dtype,
+                                                 const float* cos_table, const float* sin_table, int64_t table_rows,
+                                                 int half, int interleaved, const void* positions,
+                                                 const void* cu_seqlens, int index_type, int64_t num_seq,
+                                                 int64_t tokens, int dim, int dtype, float eps, int num_axes,
+                                                 const int32_t* sections, const ascan_rows* d_out_queries,
+                                                 const ascan_rows* d_out_keys, void* d_queries, void* d_keys,
+                                                 void* d_query_weight, void* d_key_weight, void* workspace,
+                                                 size_t workspace_bytes, void* stream);
+
+/*
+ * Causal softmax attention over packed sequences (cu_seqlens as above):
+ *
+ *   o[i] = sum_{j <= i} p[i,j] v[j],   p = softmax over j of scale q[i].k[j]
+ *
+ * within a sequence.  Keys and values have the same number of heads, which
+ * divides that of the queries; query head h reads head h / (query heads / key
+ * heads).  scale is positive and finite.  No counterpart in the reference.
+ */
+#define ASCAN_ATTENTION_MAX_DIM 128           /* of key_dim and value_dim */
+#define ASCAN_ATTENTION_MAX_TOKENS 0x3fffffff /* of seq_total and num_seq */
+
+/*
+ *   out       [seq_total, query heads, value_dim] contiguous; rows of no
+ *             sequence are zeroed
+ *   out_rest  NULL, or (16-bit types) as out: what its rounding left over
+ *   lse       NULL, or float32 [query heads, seq_total]: log2 of the sum of
+ *             exponentials of each row's scores; the backward needs both
+ */
+ASCAN_API int ascan_attention_forward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                                      const void* cu_seqlens, int cu_index_type, int64_t num_seq, int64_t seq_total,
+                                      int key_dim, int value_dim, int dtype, float scale, void* out, void* out_rest,
+                                      float* lse, void* stream);
+
+/* Bytes of workspace of ascan_attention_backward. */
+ASCAN_API size_t ascan_attention_workspace(int64_t seq_total, int query_heads);
+
+/*
+ * Its gradients, contiguous, with the inputs' heads (shared heads get the
+ * sum); out, out_rest (NULL with float32) and lse are the forward's.
+ */
+ASCAN_API int ascan_attention_backward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
+                                       const ascan_rows* d_out, const void* out, const void* out_rest,
+                                       const float* lse, const void* cu_seqlens, int cu_index_type, int64_t num_seq,
+                                       int64_t seq_total, int key_dim, int value_dim, int dtype, float scale,
+                                       void* d_queries, void* d_keys, void* d_values, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/*
+ * A paged cache of keys and values in 8 bits (e4m3, four digits).  A page
+ * holds `page` tokens (a multiple of 16) of every head; its elements stand
+ * for scale * e with one float32 scale for each page and head.  key_dim and
+ * value_dim are multiples of 16.
+ */
+#define ASCAN_CACHE_MAX_PAGE 4096
+typedef struct ascan_cache {
+  void *keys, *values;             /* [pages, heads, page, key_dim], [.., value_dim]; 16-byte aligned */
+  float *key_scales, *value_scales; /* [pages, heads] */
+  int64_t pages;
+  int32_t heads, page, key_dim, value_dim;
+} ascan_cache;
+
+/*
+ * New tokens of num_seq requests (packed, cu_seqlens as above) behind the
+ * starts[b] that the cache holds of each; token position t of request b lies
+ * in page pages[b * width + t / page], row t % page.  starts < 0 marks a row
+ * without a request.  A page's scale is the smallest power of two between
+ * 2^-64 and 2^64 with which every finite value that was written to it fits;
+ * where a later token needs a larger one, what the request holds of the page
+ * is brought to it.  Each value is rounded to nearest; what is not finite
+ * becomes NaN.  A page outside the pool is skipped and sets
+ * ASCAN_DEV_ERR_INDEX.  No two requests may write one page.
+ */
+ASCAN_API int ascan_cache_write(const ascan_rows* keys, const ascan_rows* values, const ascan_cache* cache,
+                                const int32_t* pages, int64_t num_seq, int64_t width, const void* starts,
+                                int starts_type, const void* cu_seqlens, int cu_index_type, int64_t seq_total,
+                                int dtype, void* stream);
+
+/* Bytes of workspace of ascan_cache_step. */
+ASCAN_API size_t ascan_cache_step_workspace(int value_dim);
+
+/*
+ * Softmax attention of one query token of each of num_seq requests over the
+ * first lengths[b] tokens of its pages; a length of 0 or less gives a zero
+ * row.  A page outside the pool, or tokens beyond the row of pages, are left
+ * out and set ASCAN_DEV_ERR_INDEX.  The cache's heads divide the queries'.
+ */
+ASCAN_API int ascan_cache_step(const ascan_rows* queries, const ascan_cache* cache, const int32_t* pages,
+                               int64_t num_seq, int64_t width, const void* lengths, int lengths_type, int dtype,
+                               float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Shift by one position inside every sequence and pad the vacated slot.
