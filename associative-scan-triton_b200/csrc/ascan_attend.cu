@@ -1,7 +1,8 @@
 // ascan_attend.cu -- compilation unit of the scan library: causal softmax
 // attention, its entry points and its kernels in float32 arithmetic.
 //
-// A CTA holds 64 rows of one side in shared
+// The kernels here serve float32 tensors, and 16-bit ones whose head sizes the
+// tensor-core kernels do not take.  A CTA holds 64 rows of one side in shared
 // memory as floats and walks tiles of 64 rows of the other; a thread has a
 // 4 x 4 part of the scores and 4 rows of the sums, read sixteen bytes at a
 // time with rows four words off a multiple of the banks.  Multiply-adds bound
@@ -369,11 +370,12 @@ static int run_forward(const Problem& p, cudaStream_t s) {
 }
 
 template <typename T>
-static int run_backward(const Problem& p, cudaStream_t s) {
+static int run_backward(const Problem& p, bool tc, int dtype, cudaStream_t s) {
   const long long warps = kPlainThreads / 32, ctas = (p.BL * p.H + warps - 1) / warps;
   dot_kernel<T><<<static_cast<unsigned>(min(ctas, 148ll * 64)), kPlainThreads, 0, s>>>(p);
   const int rc = launch_status();
   if (rc != ASCAN_OK) return rc;
+  if (tc) return tc_backward(p, dtype, s);
   return max(p.dk, p.dv) <= 64 ? plain_backward<T, 64>(p, s) : plain_backward<T, 128>(p, s);
 }
 
@@ -418,11 +420,12 @@ int ascan_attention_forward(const ascan_rows* queries, const ascan_rows* keys, c
   const int rc = attend::fill(p, queries, keys, values, cu_seqlens, cu_index_type, num_seq, seq_total, key_dim, value_dim,
                               dtype, scale);
   if (rc != ASCAN_OK || num_seq == 0 || seq_total == 0) return rc;
-  if (!out) return ASCAN_EINVAL;
+  if (!out || (dtype != ASCAN_F32 && !out_rest != !lse)) return ASCAN_EINVAL;
   p.out = out;
   p.rest = dtype == ASCAN_F32 ? nullptr : out_rest;
   p.lse = lse;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (attend::tc_usable(p, dtype, false)) return attend::tc_forward(p, dtype, s);
   if (dtype == ASCAN_F32) return attend::run_forward<float>(p, s);
   if (dtype == ASCAN_F16) return attend::run_forward<__half>(p, s);
   return attend::run_forward<__nv_bfloat16>(p, s);
@@ -457,9 +460,10 @@ int ascan_attention_backward(const ascan_rows* queries, const ascan_rows* keys, 
   p.d_k = d_keys;
   p.d_v = d_values;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == ASCAN_F32) return attend::run_backward<float>(p, s);
-  if (dtype == ASCAN_F16) return attend::run_backward<__half>(p, s);
-  return attend::run_backward<__nv_bfloat16>(p, s);
+  const bool tc = attend::tc_usable(p, dtype, true);
+  if (dtype == ASCAN_F32) return attend::run_backward<float>(p, tc, dtype, s);
+  if (dtype == ASCAN_F16) return attend::run_backward<__half>(p, tc, dtype, s);
+  return attend::run_backward<__nv_bfloat16>(p, tc, dtype, s);
 }
 
 }  // extern "C"

@@ -98,5 +98,10 @@ __device__ __forceinline__ void zero_outside(const Problem& p, void* to, int hea
       for (int d = threadIdx.x; d < dim; d += blockDim.x) static_cast<T*>(to)[(t * heads + head) * dim + d] = from_f<T>(0.f);
 }
 
+// The tensor-core kernels (ascan_attend_tc.cu).
+bool tc_usable(const Problem& p, int dtype, bool backward);
+int tc_forward(const Problem& p, int dtype, cudaStream_t s);
+int tc_backward(const Problem& p, int dtype, cudaStream_t s);
+
 }  // namespace attend
 }  // namespace ascan

@@ -1,0 +1,985 @@
+// ascan_attend_tc.cu -- compilation unit of the scan library: causal softmax
+// attention on the fifth-generation tensor cores (bfloat16 and float16).
+//
+// Tiles are 128 tokens by 128; TMA brings them into shared memory (128-byte
+// swizzle), accumulators and the operands that are computed on the way live in
+// tensor memory, one thread of the row per lane.  One CTA per SM, by warp:
+//
+//   0-7  softmax: scores -> probabilities (or their derivatives), rounded to
+//        the inputs' type as operands of the next product
+//   8    TMA loads
+//   9    issues the products
+//   10   gradients of keys and values: the rows' statistics
+//
+// forward: two tiles of queries share the keys and values that pass; while one
+//   tile's scores are on the tensor cores the other's softmax runs.  Per tile
+//   S = Q K^T, then P in place, O += P V.  The reference of a row's softmax
+//   moves only when a score exceeds it by 2^8: until then nothing in O has to
+//   be touched, and P stays in range (float16's 2^16 included).
+// dq: one tile of queries walks the keys: S = Q K^T and dP = dO V^T, dS in
+//   S's place, dQ += dS K.  Two S take turns, so that the next one is computed
+//   while the warps are at this one.
+// dk, dv: one tile of keys walks the queries of all heads that share it, with
+//   everything transposed: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO (P^T from
+//   shared memory, so that the next S^T has a place), dK += dS^T Q.
+//
+// Rounding P and dS to the inputs' type adds an error of the size of the
+// result's own rounding: each is off by at most half a step of itself, and
+// independently, so a sum of them is off by that of its root of squares.
+// Scores, sums, and what is subtracted from dP are float32.  Before gradients O
+// is divided by the sum of the rounded P, so that it is a mean of values
+// whatever the roundings are: what all values share stays exact in do.o, whose
+// difference from dP is all that is left of a gradient where values are alike.
+// The gradients' own P comes from the exact sum.  (The second sum costs a
+// twelfth of the time at 32768 tokens; without gradients O's own rounding is
+// larger than what it would mend.)
+//
+// A value that is not finite may stand behind the mask in the tile that the
+// diagonal crosses, and rows behind a sequence's end belong to another one;
+// 0 * NaN would carry them into other rows.  So rows behind the end are zeroed
+// in shared memory before they meet a product as its inner side, and in the
+// diagonal's tile what is not finite is too; where the mask lets it through it
+// is added to the finished rows (forward), makes a row NaN (dv), or has done so
+// through the scores already (dq, dk).
+//
+// Every wait is bounded: one that runs out sets the device error word and an
+// abort flag, every role then leaves its loop, loads and products in flight
+// are waited for, and tensor memory is freed.
+#include "ascan_impl.cuh"
+#include "ascan_attend.cuh"
+#include "ascan_pairs.cuh"
+#include "ascan_tc.cuh"
+
+namespace ascan {
+namespace attend {
+
+using namespace tc;
+
+constexpr int kC = 128;  // rows and columns of a tile
+constexpr int kTcWarps = 12, kTcThreads = kTcWarps * 32;
+constexpr int kBlock = 16384;  // 128 rows of 64 elements
+constexpr int kMaxSlots = 6;
+
+struct Maps {
+  CUtensorMap q, k, v, d_out;
+};
+
+// Slots of the ring of keys and values: what 227 KB hold next to `fixed` bytes.
+__host__ __device__ inline int slot_bytes(int dk, int dv) { return dk > 64 || dv > 64 ? 2 * kBlock : kBlock; }
+__host__ __device__ inline int slots(int dk, int dv) { return dk > 64 || dv > 64 ? 5 : kMaxSlots; }
+
+struct Common {
+  uint64_t drain;
+  int abort;
+  uint32_t tmem;
+};
+
+__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, Common* t, uint32_t* err) {
+  const unsigned long long start = now_ns();
+  volatile int* ab = &t->abort;
+  while (true) {
+    for (int i = 0; i < 16; ++i)
+      if (bar_try(b, parity)) return true;
+    if (*ab) return false;
+    if (now_ns() - start > kStageTimeoutNs) {
+      *ab = 1;
+      report(ASCAN_DEV_ERR_STAGE, (static_cast<unsigned long long>(blockIdx.x) << 32) | threadIdx.x, err);
+      return false;
+    }
+  }
+}
+
+struct Ctl {
+  Common* t;
+  uint32_t* err;
+  __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) const {
+    return bar_try(b, parity) || wait_slow(b, parity, t, err);
+  }
+  // All lanes of a role wait; false once the CTA gives up.
+  __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) const { return __all_sync(kFull, wait(b, parity)); }
+  // After a give-up: what is in flight must land before the CTA leaves.
+  __device__ __forceinline__ void land(uint64_t* b, uint32_t parity) const {
+    const unsigned long long start = now_ns();
+    while (!bar_try(b, parity) && now_ns() - start < kStageTimeoutNs) {
+    }
+  }
+};
+
+__device__ __forceinline__ void warp_arrive(uint64_t* b) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(b);
+}
+
+// Loads a tile of `dim` columns; `on` has received its bytes before.
+__device__ __forceinline__ void load_tile(unsigned char* to, const CUtensorMap* m, int dim, int head, long long token, uint64_t* on) {
+  for (int b = 0; b * 64 < dim; ++b) tma_rows(smem_u32(to) + b * kBlock, m, b * 64, head, static_cast<int>(token), on);
+}
+__device__ __forceinline__ uint32_t tile_bytes(int dim) { return dim > 64 ? 2 * kBlock : kBlock; }
+
+// A B^T over `dim` columns of two tiles in shared memory.
+__device__ __forceinline__ void scores(uint32_t to, uint64_t a, uint64_t b, uint32_t id, int dim) {
+#pragma unroll 1
+  for (int k = 0; k * 16 < dim; ++k) {
+    const uint32_t o = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
+    mma_smem(to, a + o, b + o, id, k > 0);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(uint64_t x);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(uint64_t x) {
+  const float2 f = unpair(x);
+  return bf2(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(uint64_t x) {
+  const float2 f = unpair(x);
+  return hf2(f.x, f.y);
+}
+template <typename T>
+__device__ __forceinline__ uint64_t unpack2(uint32_t x);
+template <>
+__device__ __forceinline__ uint64_t unpack2<__nv_bfloat16>(uint32_t x) { return pair(lo_f(x), hi_f(x)); }
+template <>
+__device__ __forceinline__ uint64_t unpack2<__half>(uint32_t x) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+  return pair(f.x, f.y);
+}
+__device__ __forceinline__ uint64_t pair_of(const uint32_t* x) { return pair(__uint_as_float(x[0]), __uint_as_float(x[1])); }
+__device__ __forceinline__ uint64_t ex2_2(uint64_t x) {
+  const float2 f = unpair(x);
+  return pair(ex2(f.x), ex2(f.y));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+template <typename T>
+__device__ __forceinline__ bool f16() { return false; }
+template <>
+__device__ __forceinline__ bool f16<__half>() { return true; }
+
+// Both elements of a word: its exponents all ones?
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t x) {
+  const uint32_t one = f16<T>() ? 0x0400u : 0x0080u;
+  return ((x & 0x7fff7fffu) + (one | one << 16)) & 0x80008000u;
+}
+
+// Row `row` of a tile with `blocks` of 64 columns from block `b`: zeros if it is
+// not `live`, else without what is not finite.  True if there was any.
+template <typename T>
+__device__ __forceinline__ bool clean_row(unsigned char* tile, int row, int b, int blocks, bool live) {
+  uint32_t found = 0;
+#pragma unroll 4
+  for (int c = 0; c < 8 * blocks; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(tile + (b + (c >> 3)) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+    if (!live) {
+      *at = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    uint4 x = *at;
+    const uint32_t bad = odd_bits<T>(x.x) | odd_bits<T>(x.y) | odd_bits<T>(x.z) | odd_bits<T>(x.w);
+    if (bad) {
+      auto fix = [](uint32_t w) {
+        const uint32_t o = odd_bits<T>(w);
+        return w & ~((o & 0x8000u ? 0xffffu : 0u) | (o & 0x80000000u ? 0xffff0000u : 0u));
+      };
+      x.x = fix(x.x), x.y = fix(x.y), x.z = fix(x.z), x.w = fix(x.w);
+      *at = x;
+    }
+    found |= bad;
+  }
+  return found != 0;
+}
+
+// 64 columns of a warp's 32 rows from registers (32 packed words a lane) to
+// memory in whole lines; `stage`: 4 KB of the warp's own.
+__device__ __forceinline__ void store_block(unsigned char* stage, const uint32_t* x, unsigned char* to, long long stride, int rows,
+                                            int cols) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+  __syncwarp();
+  const int c = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    if (r < rows && c * 8 < cols)
+      *reinterpret_cast<uint4*>(to + r * stride + c * 16) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+  }
+  __syncwarp();
+}
+
+// 64 columns of the warp's lanes, times f, packed.
+template <typename T>
+__device__ __forceinline__ void fetch_block(uint32_t tm, float f, uint32_t* out) {
+  const uint64_t f2 = pair(f, f);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t x[32];
+    tmem_ld32(tm + 32 * half, x);
+    wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) out[16 * half + i] = pack2<T>(mul2(pair_of(x + 2 * i), f2));
+  }
+}
+
+__device__ __forceinline__ bool misplaced(const unsigned char* smem, uint32_t* err) {
+  if (!(smem_u32(smem) & 1023u)) return false;  // the swizzled layouts need it
+  if (threadIdx.x == 0) report(ASCAN_DEV_ERR_STAGE, 0xffffffffull, err);
+  return true;
+}
+
+// All 512 columns of tensor memory, by warp 9; the barriers are ready behind it.
+__device__ __forceinline__ uint32_t open_tmem(Common* t) {
+  if (threadIdx.x >> 5 == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&t->tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  return t->tmem;
+}
+__device__ __forceinline__ void close_tmem(uint32_t tm) {
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (threadIdx.x >> 5 == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
+  }
+}
+__device__ __forceinline__ void bars_done() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  fence_async();
+}
+
+__device__ __forceinline__ void check_cu(const Problem& p) {
+  if (p.cu64) validate_cu(static_cast<const int64_t*>(p.cu), p.N, p.BL, p.err);
+  else validate_cu(static_cast<const int32_t*>(p.cu), p.N, p.BL, p.err);
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+
+struct ForwardTail {
+  Common c;
+  uint64_t q_full, full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], clean[2], o_done[2];
+  uint32_t bad[2][4];  // tokens of the tiles' own blocks with values that are not finite
+};
+
+// TRAIN: a gradient will follow.
+template <typename T, bool TRAIN>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_forward_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int h = blockIdx.y, hk = h / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (blockIdx.x == 0 && h == 0) check_cu(p);
+  zero_outside<T>(p, p.out, h, p.H, p.dv, blockIdx.x, 2 * kC);
+  const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, 2 * kC);  // long rows first
+  if (t.first < 0 || misplaced(smem, p.err)) return;
+  const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk);
+  unsigned char* ring = smem + 2 * q_bytes;
+  ForwardTail& s = *reinterpret_cast<ForwardTail*>(ring + ns * slot);
+  const Ctl ctl{&s.c, p.err};
+  const long long left = t.len - t.first;
+  const int own = static_cast<int>(t.first / kC);             // the first tile's own block of keys
+  const int n_a = own + 1, n_b = left > kC ? own + 2 : 0, n = max(n_a, n_b);
+  if (tid == 0) {
+    bar_init(&s.q_full, 1);
+    for (int i = 0; i < ns; ++i) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&s.s_full[i], 1);
+      bar_init(&s.p_ready[i], 4);
+      bar_init(&s.clean[i], 4);
+      bar_init(&s.o_done[i], 1);
+    }
+    bar_init(&s.c.drain, 1);
+    s.c.abort = 0;
+    bars_done();
+  }
+  if (tid < 8) s.bad[tid >> 2][tid & 3] = 0;
+  const uint32_t tm = open_tmem(&s.c);
+  // the ring's order: K0, then (K[j+1], V[j]) for every j
+  auto index_of_v = [&](int j) { return j < n - 1 ? 2 * j + 2 : 2 * n - 1; };
+
+  if (warp < 8) {
+    const int x = warp >> 2, quad = warp & 3, row = quad * 32 + lane, mine = x ? n_b : n_a;
+    const uint32_t lanes = static_cast<uint32_t>(quad) << 21, ts = tm + lanes + x * kC, to = tm + lanes + 256 + x * kC;
+    const float c2 = p.scale * kLog2e;
+    const uint64_t c22 = pair(c2, c2);
+    const int n32 = (p.dv + 31) / 32;
+    float m = -INFINITY;
+    uint64_t l2[2] = {0, 0}, r2[2] = {0, 0};
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      const bool diagonal = j == mine - 1;
+      if (diagonal) {  // its values may only come from this sequence, and only finite
+        const int v = index_of_v(j);
+        if (!(ok = ctl.warp_wait(&s.full[v % ns], (v / ns) & 1))) break;
+        if (clean_row<T>(ring + v % ns * slot, row, 0, p.dv > 64 ? 2 : 1, row < left - x * kC))
+          atomicOr(&s.bad[x][quad], 1u << lane);
+        fence_async();
+        warp_arrive(&s.clean[x]);
+      }
+      if (!(ok = ctl.warp_wait(&s.s_full[x], j & 1))) break;
+      fence_after();
+      uint32_t sc[kC];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, sc + 32 * i);
+      wait_ld();
+      if (diagonal) {
+#pragma unroll
+        for (int i = 0; i < kC; ++i) sc[i] = i > row ? 0xff800000u : sc[i];
+      }
+      float top[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(sc[i]);
+#pragma unroll
+      for (int i = 4; i < kC; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top[e] = i + 4 + e < kC ? max3(top[e], __uint_as_float(sc[i + e]), __uint_as_float(sc[i + 4 + e]))
+                                  : fmaxf(top[e], __uint_as_float(sc[i + e]));
+      const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (j == 0) {
+        m = high;
+      } else if (__any_sync(kFull, (high - m) * c2 > 8.f)) {
+        const float next = fmaxf(m, high), f = next == -INFINITY ? 1.f : ex2((m - next) * c2);
+        m = next;
+        const uint64_t f2 = pair(f, f);
+        l2[0] = mul2(l2[0], f2), l2[1] = mul2(l2[1], f2);
+        if (TRAIN) r2[0] = mul2(r2[0], f2), r2[1] = mul2(r2[1], f2);
+#pragma unroll 1
+        for (int i = 0; i < n32; ++i) {
+          uint32_t o[32];
+          tmem_ld32(to + 32 * i, o);
+          wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st32(to + 32 * i, o);
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : -m * c2;  // a row of -inf so far
+      const uint64_t ref2 = pair(ref, ref);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint64_t y = ex2_2(fma2(pair_of(sc + 32 * i + 2 * e), c22, ref2));
+          w[e] = pack2<T>(y);
+          l2[e & 1] = add2(l2[e & 1], y);
+          if (TRAIN) r2[e & 1] = add2(r2[e & 1], unpack2<T>(w[e]));
+        }
+        tmem_st16(ts + 16 * i, w);
+      }
+      wait_st();
+      fence_before();
+      warp_arrive(&s.p_ready[x]);
+    }
+    const bool live = ok && mine > 0 && ctl.warp_wait(&s.o_done[x], 0) && ctl.warp_wait(&s.clean[0], 0) &&
+                      (x == 0 || ctl.warp_wait(&s.clean[1], 0));
+    if (live) {
+      fence_after();
+      const float2 a = unpair(add2(l2[0], l2[1])), r = unpair(add2(r2[0], r2[1]));
+      const float l = a.x + a.y, inv = 1.f / (TRAIN ? r.x + r.y : l);
+      const int rows = static_cast<int>(min(32ll, left - x * kC - quad * 32));
+      const long long token = t.start + t.first + x * kC + quad * 32;
+      if (TRAIN && lane < rows) p.lse[h * p.BL + token + lane] = m * c2 + log2f(l);
+      const long long stride = static_cast<long long>(p.H) * p.dv * 2, first = (token * p.H + h) * p.dv * 2;
+      unsigned char* stage = smem + x * q_bytes + quad * 4096;
+      bool bad = false;
+      for (int i = 0; i < 4; ++i) bad |= s.bad[0][i] != 0 || (x == 1 && s.bad[1][i] != 0);
+      for (int b = 0; b * 64 < p.dv; ++b) {
+        uint32_t o[64];
+        tmem_ld32(to + 64 * b, o);
+        tmem_ld32(to + 64 * b + 32, o + 32);
+        wait_ld();
+#pragma unroll
+        for (int e = 0; e < 64; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+        if (bad) {  // what was taken out of the values goes where the mask lets it
+          for (int z = 0; z <= x; ++z)
+            for (int i = 0; i < kC; ++i) {
+              if (!(s.bad[z][i >> 5] >> (i & 31) & 1) || (z == x && i > row)) continue;
+              const T* v = static_cast<const T*>(p.v.p) + (t.start + t.first + z * kC + i) * p.v.st + hk * p.v.sh;
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (64 * b + e < p.dv) {
+                  const float y = to_f(v[64 * b + e]);
+                  if (!(fabsf(y) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
+                }
+            }
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = pack2<T>(pair_of(o + 2 * e));
+        store_block(stage, w, static_cast<unsigned char*>(p.out) + first + b * 128, stride, rows, p.dv - 64 * b);
+        if (TRAIN) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) w[e] = pack2<T>(fma2(unpack2<T>(w[e]), pair(-1.f, -1.f), pair_of(o + 2 * e)));
+          store_block(stage, w, static_cast<unsigned char*>(p.rest) + first + b * 128, stride, rows, p.dv - 64 * b);
+        }
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      const int token = static_cast<int>(t.start);
+      bar_expect(&s.q_full, q_bytes * (n_b ? 2 : 1));
+      load_tile(smem, &maps.q, p.dk, h, t.start + t.first, &s.q_full);
+      if (n_b) load_tile(smem + q_bytes, &maps.q, p.dk, h, t.start + t.first + kC, &s.q_full);
+      int i = 0;
+      for (; i < 2 * n; ++i) {
+        const bool is_v = i > 0 && (i % 2 == 0 || i == 2 * n - 1);
+        const int j = is_v ? (i == 2 * n - 1 ? n - 1 : i / 2 - 1) : (i + 1) / 2, at = i % ns;
+        if (i >= ns && !ctl.wait(&s.empty[at], (i / ns - 1) & 1)) break;
+        bar_expect(&s.full[at], tile_bytes(is_v ? p.dv : p.dk));
+        load_tile(ring + at * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, token + static_cast<long long>(j) * kC, &s.full[at]);
+      }
+      if (i < 2 * n) {
+        ctl.land(&s.q_full, 0);
+        for (int e = max(0, i - ns); e < i; ++e) ctl.land(&s.full[e % ns], (e / ns) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
+    const uint64_t q[2] = {desc(smem_u32(smem), 16), desc(smem_u32(smem) + q_bytes, 16)};
+    auto ring_desc = [&](int at, uint32_t lbo) { return desc(smem_u32(ring) + at * slot, lbo); };
+    auto wait_slot = [&](int i) { return ctl.warp_wait(&s.full[i % ns], (i / ns) & 1); };
+    bool ok = ctl.warp_wait(&s.q_full, 0) && wait_slot(0);
+    if (ok) {
+      fence_after();
+      if (elect_one()) {
+        scores(tm, q[0], ring_desc(0, 16), id_s, p.dk);
+        commit(&s.s_full[0]);
+        if (n_b) {
+          scores(tm + kC, q[1], ring_desc(0, 16), id_s, p.dk);
+          commit(&s.s_full[1]);
+        }
+        commit(&s.empty[0]);
+      }
+    }
+    for (int j = 0; ok && j < n; ++j) {
+      const bool more = j + 1 < n;
+      const int ik = 2 * j + 1, iv = index_of_v(j);
+      if ((more && !wait_slot(ik)) || !wait_slot(iv)) break;
+      for (int x = 0; x < 2; ++x) {
+        const int mine = x ? n_b : n_a;
+        if (j >= mine) continue;
+        if (!(ok = ctl.warp_wait(&s.p_ready[x], j & 1))) break;
+        fence_after();
+        if (elect_one()) {
+          const uint64_t v = ring_desc(iv % ns, kBlock);
+#pragma unroll 1
+          for (int k = 0; k < kC / 16; ++k) mma_tmem(tm + 256 + x * kC, tm + x * kC + k * 8, v + k * 128, id_o, j + k > 0);
+          if (x == 1 || !n_b) commit(&s.empty[iv % ns]);
+          if (j + 1 < mine) {
+            scores(tm + x * kC, q[x], ring_desc(ik % ns, 16), id_s, p.dk);
+            commit(&s.s_full[x]);
+          } else {
+            commit(&s.o_done[x]);
+          }
+          if (more && (x == 1 || !n_b)) commit(&s.empty[ik % ns]);
+        }
+      }
+    }
+    if (elect_one()) commit(&s.c.drain);  // nothing of this CTA's is in flight after it
+    ctl.land(&s.c.drain, 0);
+  }
+  close_tmem(tm);
+}
+
+// ---------------------------------------------------------------------------
+// gradients of the queries
+// ---------------------------------------------------------------------------
+
+struct DqTail {
+  Common c;
+  uint64_t q_full, full[kMaxSlots], empty[kMaxSlots], dp_full, dp_free, ds_ready, o_done;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int h = blockIdx.y, hk = h / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC);
+  const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kC);
+  if (t.first < 0 || misplaced(smem, p.err)) return;
+  const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk), g_bytes = tile_bytes(p.dv);
+  unsigned char* ring = smem + q_bytes + g_bytes;
+  DqTail& s = *reinterpret_cast<DqTail*>(ring + ns * slot);
+  const Ctl ctl{&s.c, p.err};
+  const int n = static_cast<int>(t.first / kC) + 1, len = static_cast<int>(min(static_cast<long long>(kC), t.len - t.first));
+  const long long at = t.start + t.first;
+  if (tid == 0) {
+    bar_init(&s.q_full, 1);
+    for (int i = 0; i < ns; ++i) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
+    bar_init(&s.dp_full, 1);
+    bar_init(&s.dp_free, 8);
+    bar_init(&s.ds_ready, 8);
+    bar_init(&s.o_done, 1);
+    bar_init(&s.c.drain, 1);
+    s.c.abort = 0;
+    bars_done();
+  }
+  const uint32_t tm = open_tmem(&s.c);
+  constexpr uint32_t kDp = 256, kDq = 384;  // two places of S, then dP and dQ
+
+  if (warp < 8) {
+    const int side = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quad) << 21;
+    const float lse = row < len ? p.lse[h * p.BL + at + row] : 0.f, d = row < len ? p.d[h * p.BL + at + row] : 0.f;
+    const float c2 = p.scale * kLog2e;
+    const uint64_t c22 = pair(c2, c2), lse2 = pair(-lse, -lse), d2 = pair(-d, -d);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      if (!(ok = ctl.warp_wait(&s.dp_full, j & 1))) break;  // S was issued before dP
+      fence_after();
+      const uint32_t ts = tm + lanes + (j & 1) * kC + 64 * side;
+      uint32_t sc[64], g[64];
+      tmem_ld32(tm + lanes + kDp + 64 * side, g);
+      tmem_ld32(tm + lanes + kDp + 64 * side + 32, g + 32);
+      tmem_ld32(ts, sc);
+      tmem_ld32(ts + 32, sc + 32);
+      wait_ld();
+      fence_before();
+      warp_arrive(&s.dp_free);
+      const bool diagonal = j == n - 1;
+      uint32_t w[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const uint64_t y = ex2_2(fma2(pair_of(sc + 2 * e), c22, lse2));
+        w[e] = pack2<T>(mul2(y, add2(pair_of(g + 2 * e), d2)));
+      }
+      if (diagonal) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int c = 64 * side + 2 * e;
+          w[e] &= (c <= row ? 0xffffu : 0u) | (c + 1 <= row ? 0xffff0000u : 0u);
+        }
+        // keys of the rows behind the mask, and of other sequences
+        const int i = 2 * j;
+        if (64 * side < p.dk) clean_row<T>(ring + i % ns * slot, row, side, 1, row < len);
+        fence_async();
+      }
+      tmem_st32(ts, w);
+      wait_st();
+      fence_before();
+      warp_arrive(&s.ds_ready);
+    }
+    if (ok && 64 * side < p.dk && ctl.warp_wait(&s.o_done, 0)) {
+      fence_after();
+      uint32_t w[32];
+      fetch_block<T>(tm + lanes + kDq + 64 * side, p.scale, w);
+      store_block(smem + side * kBlock + quad * 4096, w,
+                  static_cast<unsigned char*>(p.d_q) + ((at + quad * 32) * p.H + h) * p.dk * 2 + side * 128,
+                  static_cast<long long>(p.H) * p.dk * 2, len - quad * 32, p.dk - 64 * side);
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      bar_expect(&s.q_full, q_bytes + g_bytes);
+      load_tile(smem, &maps.q, p.dk, h, at, &s.q_full);
+      load_tile(smem + q_bytes, &maps.d_out, p.dv, h, at, &s.q_full);
+      int i = 0;
+      for (; i < 2 * n; ++i) {
+        const bool is_v = i & 1;
+        const int to = i % ns;
+        if (i >= ns && !ctl.wait(&s.empty[to], (i / ns - 1) & 1)) break;
+        bar_expect(&s.full[to], tile_bytes(is_v ? p.dv : p.dk));
+        load_tile(ring + to * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, t.start + static_cast<long long>(i >> 1) * kC, &s.full[to]);
+      }
+      if (i < 2 * n) {
+        ctl.land(&s.q_full, 0);
+        for (int e = max(0, i - ns); e < i; ++e) ctl.land(&s.full[e % ns], (e / ns) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dk + 15) / 16 * 16, true, f16<T>());
+    const uint64_t q = desc(smem_u32(smem), 16), g = desc(smem_u32(smem) + q_bytes, 16);
+    auto ring_desc = [&](int i, uint32_t lbo) { return desc(smem_u32(ring) + i % ns * slot, lbo); };
+    auto wait_slot = [&](int i) { return ctl.warp_wait(&s.full[i % ns], (i / ns) & 1); };
+    bool ok = ctl.warp_wait(&s.q_full, 0);
+    for (int j = -1; ok && j < n; ++j) {
+      if (j + 1 < n) {  // the next tile's scores, while the warps are at this one's
+        const int i = 2 * (j + 1);
+        if (!(ok = wait_slot(i))) break;
+        fence_after();
+        if (elect_one()) scores(tm + ((j + 1) & 1) * kC, q, ring_desc(i, 16), id_s, p.dk);
+        if (!(ok = wait_slot(i + 1) && (j < 0 || ctl.warp_wait(&s.dp_free, j & 1)))) break;
+        fence_after();
+        if (elect_one()) {
+          scores(tm + kDp, g, ring_desc(i + 1, 16), id_s, p.dv);
+          commit(&s.dp_full);
+          commit(&s.empty[(i + 1) % ns]);
+        }
+      }
+      if (j < 0) continue;
+      if (!(ok = ctl.warp_wait(&s.ds_ready, j & 1))) break;
+      fence_after();
+      if (elect_one()) {
+        const uint64_t k0 = ring_desc(2 * j, kBlock);
+        // the warps' halves of dS lie 64 columns apart
+#pragma unroll 1
+        for (int k = 0; k < kC / 16; ++k)
+          mma_tmem(tm + kDq, tm + (j & 1) * kC + (k >> 2) * 64 + (k & 3) * 8, k0 + k * 128, id_o, j + k > 0);
+        commit(&s.empty[2 * j % ns]);
+        if (j == n - 1) commit(&s.o_done);
+      }
+    }
+    if (elect_one()) commit(&s.c.drain);
+    ctl.land(&s.c.drain, 0);
+  }
+  close_tmem(tm);
+}
+
+// ---------------------------------------------------------------------------
+// gradients of the keys and values
+// ---------------------------------------------------------------------------
+
+struct DkvTail {
+  Common c;
+  uint64_t kv_full, q_full[2], q_empty[2], g_full[2], g_empty[2], stat_full[2], stat_empty[2];
+  uint64_t s_full, s_free, p_ready, p_free, dp_full, ds_ready, o_done;
+  float lse[2][kC], d[2][kC];  // negated, of the queries that pass
+  int bad;                     // 1 + the last query of the diagonal's tile whose dO is not finite
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int hk = blockIdx.y, heads = p.H / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC);
+  zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC);
+  const Tile t = find_tile(p, blockIdx.x, kC);  // a sequence's first keys have the most queries
+  if (t.first < 0 || misplaced(smem, p.err)) return;
+  const int k_bytes = tile_bytes(p.dk), v_bytes = tile_bytes(p.dv);
+  unsigned char *q_ring = smem + k_bytes + v_bytes, *g_ring = q_ring + 2 * k_bytes, *pt = g_ring + 2 * v_bytes;
+  DkvTail& s = *reinterpret_cast<DkvTail*>(pt + 2 * kBlock);
+  const Ctl ctl{&s.c, p.err};
+  const int blocks = static_cast<int>((t.len - t.first + kC - 1) / kC), len = static_cast<int>(min(static_cast<long long>(kC), t.len - t.first));
+  const int total = blocks * p.share;  // tiles of queries, head by head
+  const long long at = t.start + t.first;
+  if (tid == 0) {
+    bar_init(&s.kv_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&s.q_full[i], 1);
+      bar_init(&s.q_empty[i], 1);
+      bar_init(&s.g_full[i], 1);
+      bar_init(&s.g_empty[i], 1);
+      bar_init(&s.stat_full[i], 1);
+      bar_init(&s.stat_empty[i], 8);
+    }
+    bar_init(&s.s_full, 1);
+    bar_init(&s.s_free, 8);
+    bar_init(&s.p_ready, 8);
+    bar_init(&s.p_free, 1);
+    bar_init(&s.dp_full, 1);
+    bar_init(&s.ds_ready, 8);
+    bar_init(&s.o_done, 1);
+    bar_init(&s.c.drain, 1);
+    s.c.abort = 0;
+    s.bad = 0;
+    bars_done();
+  }
+  const uint32_t tm = open_tmem(&s.c);
+  constexpr uint32_t kDp = 128, kDv = 256, kDk = 384;
+
+  if (warp < 8) {
+    const int side = warp >> 2, quad = warp & 3, row = quad * 32 + lane;  // of the keys; columns are queries
+    const uint32_t lanes = static_cast<uint32_t>(quad) << 21, ts = tm + lanes + 64 * side, td = tm + lanes + kDp + 64 * side;
+    const float c2 = p.scale * kLog2e;
+    const uint64_t c22 = pair(c2, c2);
+    bool ok = true;
+    for (int i = 0, b = 0; i < total; ++i, b = b + 1 < blocks ? b + 1 : 0) {
+      const int u = i & 1;
+      const bool diagonal = b == 0;
+      const int n = static_cast<int>(min(static_cast<long long>(kC), t.len - t.first - static_cast<long long>(b) * kC));
+      const bool edge = diagonal || n < kC;
+      if (!(ok = ctl.warp_wait(&s.stat_full[u], (i >> 1) & 1) && ctl.warp_wait(&s.s_full, i & 1))) break;
+      fence_after();
+      uint64_t x[32];
+      uint32_t w[32];
+      {
+        uint32_t sc[64];
+        tmem_ld32(ts, sc);
+        tmem_ld32(ts + 32, sc + 32);
+        wait_ld();
+        fence_before();
+        warp_arrive(&s.s_free);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float4 l = *reinterpret_cast<const float4*>(&s.lse[u][64 * side + 2 * e]);
+          x[e] = ex2_2(fma2(pair_of(sc + 2 * e), c22, pair(l.x, l.y)));
+          x[e + 1] = ex2_2(fma2(pair_of(sc + 2 * e + 2), c22, pair(l.z, l.w)));
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float2 f = unpair(x[e]);
+          const int c = 64 * side + 2 * e;
+          if ((diagonal && c < row) || c >= n) f.x = 0.f;
+          if ((diagonal && c + 1 < row) || c + 1 >= n) f.y = 0.f;
+          x[e] = pair(f.x, f.y);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) w[e] = pack2<T>(x[e]);
+      if (i > 0 && !(ok = ctl.warp_wait(&s.p_free, (i - 1) & 1))) break;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(pt + side * kBlock + row * 128 + ((c ^ (row & 7)) << 4)) =
+            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      if (edge) {
+        // queries and upstream gradients of rows behind the mask, and of other
+        // sequences, once both score products have read them
+        if (!(ok = ctl.warp_wait(&s.dp_full, i & 1))) break;
+        if (64 * side < p.dk) clean_row<T>(q_ring + u * k_bytes, row, side, 1, row < n);
+        if (64 * side < p.dv && clean_row<T>(g_ring + u * v_bytes, row, side, 1, row < n) && diagonal) atomicMax(&s.bad, row + 1);
+      }
+      fence_async();
+      warp_arrive(&s.p_ready);
+      if (!(ok = ctl.warp_wait(&s.dp_full, i & 1))) break;
+      fence_after();
+      {
+        uint32_t g[64];
+        tmem_ld32(td, g);
+        tmem_ld32(td + 32, g + 32);
+        wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float4 d = *reinterpret_cast<const float4*>(&s.d[u][64 * side + 2 * e]);
+          w[e] = pack2<T>(mul2(x[e], add2(pair_of(g + 2 * e), pair(d.x, d.y))));
+          w[e + 1] = pack2<T>(mul2(x[e + 1], add2(pair_of(g + 2 * e + 2), pair(d.z, d.w))));
+        }
+      }
+      if (edge) {  // 0 * NaN again
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int c = 64 * side + 2 * e;
+          w[e] &= ((diagonal && c < row) || c >= n ? 0u : 0xffffu) | ((diagonal && c + 1 < row) || c + 1 >= n ? 0u : 0xffff0000u);
+        }
+      }
+      tmem_st32(td, w);
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        bar_arrive(&s.ds_ready);
+        bar_arrive(&s.stat_empty[u]);
+      }
+    }
+    if (ok && ctl.warp_wait(&s.o_done, 0)) {
+      fence_after();
+      // behind the last product, whose inputs were ready after every clean_row
+      const bool bad = row < *reinterpret_cast<volatile int*>(&s.bad);
+      unsigned char* stage = smem + warp * 4096;
+      uint32_t w[32];
+      if (64 * side < p.dv) {
+        fetch_block<T>(tm + lanes + kDv + 64 * side, bad ? NAN : 1.f, w);
+        store_block(stage, w, static_cast<unsigned char*>(p.d_v) + ((at + quad * 32) * heads + hk) * p.dv * 2 + side * 128,
+                    static_cast<long long>(heads) * p.dv * 2, len - quad * 32, p.dv - 64 * side);
+      }
+      if (64 * side < p.dk) {
+        fetch_block<T>(tm + lanes + kDk + 64 * side, p.scale, w);
+        store_block(stage, w, static_cast<unsigned char*>(p.d_k) + ((at + quad * 32) * heads + hk) * p.dk * 2 + side * 128,
+                    static_cast<long long>(heads) * p.dk * 2, len - quad * 32, p.dk - 64 * side);
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      bar_expect(&s.kv_full, k_bytes + v_bytes);
+      load_tile(smem, &maps.k, p.dk, hk, at, &s.kv_full);
+      load_tile(smem + k_bytes, &maps.v, p.dv, hk, at, &s.kv_full);
+      int q_loads = 0, g_loads = 0;
+      for (int i = 0, b = 0, h = hk * p.share; i < total; ++i) {
+        const int u = i & 1;
+        const long long token = at + static_cast<long long>(b) * kC;
+        if (i > 1 && !ctl.wait(&s.q_empty[u], (i / 2 - 1) & 1)) break;
+        bar_expect(&s.q_full[u], k_bytes);
+        load_tile(q_ring + u * k_bytes, &maps.q, p.dk, h, token, &s.q_full[u]);
+        ++q_loads;
+        if (i > 1 && !ctl.wait(&s.g_empty[u], (i / 2 - 1) & 1)) break;
+        bar_expect(&s.g_full[u], v_bytes);
+        load_tile(g_ring + u * v_bytes, &maps.d_out, p.dv, h, token, &s.g_full[u]);
+        ++g_loads;
+        if (++b == blocks) b = 0, ++h;
+      }
+      if (g_loads < total) {
+        ctl.land(&s.kv_full, 0);
+        for (int i = max(0, q_loads - 2); i < q_loads; ++i) ctl.land(&s.q_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, g_loads - 2); i < g_loads; ++i) ctl.land(&s.g_full[i & 1], (i >> 1) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    const uint32_t id_s = idesc(kC, false, f16<T>()), id_k = idesc((p.dk + 15) / 16 * 16, true, f16<T>()),
+                   id_v = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
+    const uint64_t k = desc(smem_u32(smem), 16), v = desc(smem_u32(smem) + k_bytes, 16), a = desc(smem_u32(pt), 16);
+    auto q_desc = [&](int u, uint32_t lbo) { return desc(smem_u32(q_ring) + u * k_bytes, lbo); };
+    auto g_desc = [&](int u, uint32_t lbo) { return desc(smem_u32(g_ring) + u * v_bytes, lbo); };
+    bool ok = ctl.warp_wait(&s.kv_full, 0);
+    for (int i = -1; ok && i < total; ++i) {
+      const bool more = i + 1 < total;
+      const int u = i & 1, nu = (i + 1) & 1;
+      if (more) {
+        if (!(ok = ctl.warp_wait(&s.q_full[nu], ((i + 1) >> 1) & 1) && (i < 0 || ctl.warp_wait(&s.s_free, i & 1)))) break;
+        fence_after();
+        if (elect_one()) {
+          scores(tm, k, q_desc(nu, 16), id_s, p.dk);
+          commit(&s.s_full);
+        }
+      }
+      if (i >= 0) {
+        if (!(ok = ctl.warp_wait(&s.p_ready, i & 1))) break;
+        fence_after();
+        if (elect_one()) {
+          const uint64_t g = g_desc(u, kBlock);
+#pragma unroll 1
+          for (int e = 0; e < kC / 16; ++e)
+            mma_smem(tm + kDv, a + (e >> 2) * (kBlock >> 4) + (e & 3) * 2, g + e * 128, id_v, i + e > 0);
+          commit(&s.p_free);
+          commit(&s.g_empty[u]);
+        }
+        if (!(ok = ctl.warp_wait(&s.ds_ready, i & 1))) break;
+        fence_after();
+        if (elect_one()) {
+          const uint64_t q = q_desc(u, kBlock);
+          // the warps' halves of dS lie 64 columns apart
+#pragma unroll 1
+          for (int e = 0; e < kC / 16; ++e)
+            mma_tmem(tm + kDk, tm + kDp + (e >> 2) * 64 + (e & 3) * 8, q + e * 128, id_k, i + e > 0);
+          commit(&s.q_empty[u]);
+          if (!more) commit(&s.o_done);
+        }
+      }
+      if (more) {
+        if (!(ok = ctl.warp_wait(&s.g_full[nu], ((i + 1) >> 1) & 1))) break;
+        fence_after();
+        if (elect_one()) {
+          scores(tm + kDp, v, g_desc(nu, 16), id_s, p.dv);
+          commit(&s.dp_full);
+        }
+      }
+    }
+    if (elect_one()) commit(&s.c.drain);
+    ctl.land(&s.c.drain, 0);
+  } else if (warp == 10) {
+    for (int i = 0, b = 0, h = hk * p.share; i < total; ++i) {
+      const int u = i & 1;
+      const long long token = at + static_cast<long long>(b) * kC, n = t.len - t.first - static_cast<long long>(b) * kC;
+      float l[4], d[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = e * 32 + lane;
+        l[e] = c < n ? -p.lse[h * p.BL + token + c] : 0.f;
+        d[e] = c < n ? -p.d[h * p.BL + token + c] : 0.f;
+      }
+      if (i > 1 && !ctl.warp_wait(&s.stat_empty[u], (i / 2 - 1) & 1)) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.lse[u][e * 32 + lane] = l[e], s.d[u][e * 32 + lane] = d[e];
+      warp_arrive(&s.stat_full[u]);
+      if (++b == blocks) b = 0, ++h;
+    }
+  }
+  close_tmem(tm);
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+static bool map_rows(CUtensorMap* m, const Rows& r, int dim, int heads, long long BL, int dtype) {
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const long long sh = heads > 1 ? r.sh : dim;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(BL)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(r.st) * 2};
+  const cuuint32_t box[3] = {64, 1, kC}, one[3] = {1, 1, 1};
+  return fn(m, dtype == ASCAN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(r.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows that a tensor map can describe: 16-byte bases and strides, head sizes in
+// whole 16-byte pieces, heads that do not overlap.
+static bool rows_usable(const Rows& r, int dim, int heads) {
+  if ((reinterpret_cast<uintptr_t>(r.p) & 15u) || dim % 8 || r.st % 8 || r.st < dim || r.st >= (1ll << 38)) return false;
+  return heads == 1 || (r.sh % 8 == 0 && r.sh >= dim && r.sh < (1ll << 38));
+}
+static bool aligned(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; }
+
+bool tc_usable(const Problem& p, int dtype, bool backward) {
+  if (dtype == ASCAN_F32) return false;
+  const int heads = p.H / p.share;
+  if (!rows_usable(p.q, p.dk, p.H) || !rows_usable(p.k, p.dk, heads) || !rows_usable(p.v, p.dv, heads)) return false;
+  if (!aligned(p.out) || !aligned(p.rest)) return false;
+  if (backward && (!rows_usable(p.d_out, p.dv, p.H) || !aligned(p.d_q) || !aligned(p.d_k) || !aligned(p.d_v))) return false;
+  return encode_fn() != nullptr;
+}
+
+// Tensor maps are made through the driver, which wants a current context; a
+// thread whose first CUDA call this is has none until the runtime is told its
+// device.
+static int make_maps(Maps& m, const Problem& p, int dtype, bool backward) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return ASCAN_EDEVICE;
+  memset(&m, 0, sizeof(m));
+  const int heads = p.H / p.share;
+  if (!map_rows(&m.q, p.q, p.dk, p.H, p.BL, dtype) || !map_rows(&m.k, p.k, p.dk, heads, p.BL, dtype) ||
+      !map_rows(&m.v, p.v, p.dv, heads, p.BL, dtype) || (backward && !map_rows(&m.d_out, p.d_out, p.dv, p.H, p.BL, dtype)))
+    return ASCAN_ECUDA;
+  return ASCAN_OK;
+}
+
+static int bytes_of(int dim) { return dim > 64 ? 2 * kBlock : kBlock; }
+
+template <typename T, bool TRAIN>
+static int forward(const Problem& p, const Maps& m, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{};
+  const int rc = allow_smem(tc_forward_kernel<T, TRAIN>, kSmemLimit, done);
+  if (rc != ASCAN_OK) return rc;
+  const size_t smem = 2 * bytes_of(p.dk) + slots(p.dk, p.dv) * slot_bytes(p.dk, p.dv) + sizeof(ForwardTail);
+  tc_forward_kernel<T, TRAIN><<<dim3(tile_bound(p, 2 * kC), p.H), kTcThreads, smem, s>>>(p, m);
+  return launch_status();
+}
+
+template <typename T>
+static int backward(const Problem& p, const Maps& m, cudaStream_t s) {
+  static std::atomic<unsigned long long> done[2]{};
+  int rc = allow_smem(tc_dq_kernel<T>, kSmemLimit, done[0]);
+  if (rc == ASCAN_OK) rc = allow_smem(tc_dkdv_kernel<T>, kSmemLimit, done[1]);
+  if (rc != ASCAN_OK) return rc;
+  const size_t k = bytes_of(p.dk), v = bytes_of(p.dv);
+  const size_t q_smem = k + v + slots(p.dk, p.dv) * slot_bytes(p.dk, p.dv) + sizeof(DqTail);
+  tc_dq_kernel<T><<<dim3(tile_bound(p, kC), p.H), kTcThreads, q_smem, s>>>(p, m);
+  rc = launch_status();
+  if (rc != ASCAN_OK) return rc;
+  tc_dkdv_kernel<T><<<dim3(tile_bound(p, kC), p.H / p.share), kTcThreads, 3 * (k + v) + 2 * kBlock + sizeof(DkvTail), s>>>(p, m);
+  return launch_status();
+}
+static_assert(14 * kBlock + sizeof(DkvTail) <= kSmemLimit &&
+              14 * kBlock + sizeof(ForwardTail) <= kSmemLimit && 14 * kBlock + sizeof(DqTail) <= kSmemLimit,
+              "heads of 128 leave no more for the barriers and statistics");
+
+int tc_forward(const Problem& p, int dtype, cudaStream_t s) {
+  Maps m;
+  const int rc = make_maps(m, p, dtype, false);
+  if (rc != ASCAN_OK) return rc;
+  if (p.lse && p.rest) return dtype == ASCAN_BF16 ? forward<__nv_bfloat16, true>(p, m, s) : forward<__half, true>(p, m, s);
+  return dtype == ASCAN_BF16 ? forward<__nv_bfloat16, false>(p, m, s) : forward<__half, false>(p, m, s);
+}
+
+int tc_backward(const Problem& p, int dtype, cudaStream_t s) {
+  Maps m;
+  const int rc = make_maps(m, p, dtype, true);
+  if (rc != ASCAN_OK) return rc;
+  return dtype == ASCAN_BF16 ? backward<__nv_bfloat16>(p, m, s) : backward<__half>(p, m, s);
+}
+
+}  // namespace attend
+
+ASCAN_UNIT_ERROR_ACCESSORS(attend_tc)
+
+}  // namespace ascan

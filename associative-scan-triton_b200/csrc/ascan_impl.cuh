@@ -2198,7 +2198,7 @@ ASCAN_FOR_EACH_TYPE_PAIR(ASCAN_EXTERN_SHIFT_PAD)
 // The units with kernels, each with its own error word: op 0 reads it into
 // (*code, *detail), op 1 clears it (current device; no synchronisation).
 #define ASCAN_UNITS(X) X(fwd_f32) X(fwd_f16) X(fwd_bf16) X(bwd_f32) X(bwd_f16) X(bwd_bf16) X(bidi) X(misc) \
-  X(mscan) X(mscan_tc) X(rotate) X(attend) X(cache)
+  X(mscan) X(mscan_tc) X(rotate) X(attend) X(attend_tc) X(cache)
 #define ASCAN_DECL_UNIT_ERR(NAME) int unit_err_##NAME(int op, unsigned int* code, unsigned long long* detail);
 ASCAN_UNITS(ASCAN_DECL_UNIT_ERR)
 

@@ -52,16 +52,17 @@
 #include "ascan_mscan.cuh"
 #include "ascan_mscan_common.cuh"
 #include "ascan_pairs.cuh"
+#include "ascan_tc.cuh"
 
 namespace ascan {
 namespace mscan {
+
+using namespace tc;
 
 constexpr int kC = 128;             // tokens of a chunk
 constexpr int kTcWarps = 19;
 constexpr int kTcThreads = kTcWarps * 32;
 constexpr uint32_t kColSc = 0, kColO = 128, kColU = 256, kColK = 384;
-constexpr unsigned long long kStageTimeoutNs = 2000000000ull;
-constexpr size_t kSmemLimit = 232448;
 
 struct TcMaps {
   CUtensorMap m[3][5];  // per form: A, B, C, the rows to take dots with, the output
@@ -109,126 +110,6 @@ __host__ __device__ inline TcGeom tc_geom(int da, int dc) {
   return g;
 }
 
-// ---- instructions ----------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(b)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-// 128 tokens by 64 elements of one head, from column x (a multiple of 64).
-__device__ __forceinline__ void tma_rows(uint32_t to, const CUtensorMap* m, int x, int head, int token, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
-      "l"(m), "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
-      : "memory");
-}
-// One lane of the warp, by the instruction that the compiler knows to pick
-// one: behind it operands stay in uniform registers, and a product takes 50
-// cycles to issue instead of 90 (it runs for 64).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
-  return r != 0;
-}
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
-      : "memory");
-}
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b))
-               : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-#define TC_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
-#define TC_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-
-// 32 columns of the warp's 32 lanes; volatile, and the wait follows before use.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : TC_R8(r, 0), TC_R8(r, 8), TC_R8(r, 16), TC_R8(r, 24)
-      : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : TC_R8(r, 0), TC_R8(r, 8)
-      : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : TC_R8(r, 0) : "r"(addr));
-}
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), TC_I8(r, 0)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      TC_I8(r, 0), TC_I8(r, 8)
-      : "memory");
-}
-
-// 16 lanes by 8 columns; a pair of registers holds 4 columns: lane l of the
-// warp has column l % 4 of row l / 4, then of row l / 4 + 8.
-__device__ __forceinline__ void tmem_st16x128(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3])
-               : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// two floats to packed bfloat16 (a low, b high)
-__device__ __forceinline__ uint32_t bf2(float a, float b) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-__device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-
 // The n lowest of 32 bits (none below 0, all above 31).
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
@@ -248,20 +129,6 @@ __device__ __forceinline__ void add_state(const uint4& hi, uint64_t total2, cons
   const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = fma2(total2, pair(lo_f(h[e]), hi_f(h[e])), pair(v[2 * e], v[2 * e + 1]));
-}
-
-// Shared-memory operand descriptors, 128-byte swizzle.  Along the unit-stride
-// side a row is 64 elements; `lbo` is the distance of the next 64 (used when
-// that side is not the products' inner one), rows of 8 are 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
-  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// float32 accumulators, bfloat16 operands, M = 128; b_mn: B's unit stride is
-// along N.
-__device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn) << 16) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
 // Element i of N (a power of two), without indexing registers.

@@ -482,9 +482,10 @@ ASCAN_API int ascan_qk_norm_rotate_axes_backward(const ascan_rows* queries, cons
 /*
  *   out       [seq_total, query heads, value_dim] contiguous; rows of no
  *             sequence are zeroed
- *   out_rest  NULL, or (16-bit types) as out: what its rounding left over
  *   lse       NULL, or float32 [query heads, seq_total]: log2 of the sum of
- *             exponentials of each row's scores; the backward needs both
+ *             exponentials of each row's scores, which the backward needs
+ *   out_rest  16-bit types with lse: as out, what its rounding left over,
+ *             which the backward needs too; else NULL
  */
 ASCAN_API int ascan_attention_forward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
                                       const void* cu_seqlens, int cu_index_type, int64_t num_seq, int64_t seq_total,

@@ -160,21 +160,36 @@ def test_scores_that_grow_along_the_row(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_sharp_rows_keep_their_gradients(dtype):
   # probabilities within 1e-3 of 1: do.v - do.o cancels all but the last digits,
-  # and a do.o from the rounded out alone would leave nothing of them
-  n = 256
+  # and a do.o from the rounded out alone would leave nothing of them.
+  # An element is off by what its roundings leave, weighed by what they meet.
+  # The forward's weights are rounded by half a step h each and add up to 1 as
+  # rounded: do.o is off by h times the spread of do.v over the row.  p and ds are
+  # rounded by h, as the result is; do.v - do.o loses 1e-5 of its float32 terms
+  # and h^2 of out (kept with the rest of its rounding); float16's steps end at
+  # 2^-24.
+  n, h = 256, {F32: 2.0**-24, F16: 2.0**-11, BF16: 2.0**-8}[dtype]
   q, k, v, do = make([n], (2, 2), (64, 64), dtype, seed=5)
   mark = torch.zeros(n, 64)
   mark[torch.arange(n), torch.arange(n) % 64] = 9.0
   k = (0.1 * k.float() + mark[:, None]).to(dtype)
   q = (0.1 * q.float() + mark[:, None]).to(dtype)
   ours = [x.to(DEV).requires_grad_(True) for x in (q, k, v)]
-  ref = [x.double().requires_grad_(True) for x in (q, k, v)]
   found = torch.autograd.grad(ast.attention_causal(*ours, {"cu_seqlens": cu_of([n])}), ours, do.to(DEV))
-  exact = torch.autograd.grad(oracle(*ref, [n], 0.125), ref, do.double())
-  for name, a, b in zip(("queries", "keys", "values"), found, exact):
-    # keys and queries share large components here, over which ds sums to
-    # nothing: its roundings are weighed by 9, not by their own spread
-    close(name, a, b, 4 * TOL[dtype])
+  Q, K, V, G = (x.double().transpose(0, 1) for x in (q, k, v, do))
+  score = (0.125 * Q @ K.transpose(1, 2)).masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), float("-inf"))
+  p = torch.softmax(score, -1)
+  o = p @ V
+  spread = G @ V.transpose(1, 2) - (G * o).sum(-1, keepdim=True)
+  ds = p * spread
+  lost = G.abs() @ V.abs().transpose(1, 2) + (G * o).abs().sum(-1, keepdim=True)
+  fine = 2.0**-25 if dtype == F16 else 0.0
+  e_ds = h * ds.abs() + 2 * h * p * ds.abs().sum(-1, keepdim=True) + (1e-5 + h * h) * p * lost + fine * (p > 0)
+  e_p = (h + 1e-5) * p + fine * (p > 0)
+  want = (0.125 * ds @ K, 0.125 * ds.transpose(1, 2) @ Q, p.transpose(1, 2) @ G)
+  room = (0.125 * e_ds @ K.abs(), 0.125 * e_ds.transpose(1, 2) @ Q.abs(), e_p.transpose(1, 2) @ G.abs())
+  for name, a, b, e in zip(("queries", "keys", "values"), found, want, room):
+    err = (a.double().cpu() - b.transpose(0, 1)).abs()
+    assert (err <= (e + (h + 1e-6) * b.abs() + fine).transpose(0, 1)).all(), name
 
 
 @gpu
