@@ -206,7 +206,7 @@ def _bind(lib) -> None:
   lib.ascan_cache_write.restype = ci
   lib.ascan_cache_write.argtypes = [rows, rows, p, p, i64, i64, p, ci, p, ci, i64, ci, p]
   lib.ascan_cache_step_workspace.restype = sz
-  lib.ascan_cache_step_workspace.argtypes = [ci]
+  lib.ascan_cache_step_workspace.argtypes = [i64, ci]
   lib.ascan_cache_step.restype = ci
   lib.ascan_cache_step.argtypes = [rows, p, p, i64, i64, p, ci, ci, f, p, p, sz, p]
   lib.ascan_set_implementation.restype = ci

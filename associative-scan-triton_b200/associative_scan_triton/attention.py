@@ -375,7 +375,7 @@ def attention_cache_step(
     return out
   lib = _lib.load()
   with _on(device):
-    ws = torch.empty(lib.ascan_cache_step_workspace(value_dim), dtype=torch.uint8,
+    ws = torch.empty(lib.ascan_cache_step_workspace(batch, value_dim), dtype=torch.uint8,
                      device=device)
     rc = lib.ascan_cache_step(
       *_rows(queries), _native_cache(tensors), pages.data_ptr(), batch, width, lengths.data_ptr(),

@@ -12,9 +12,12 @@
 // addition to the exponent.
 #include "ascan_impl.cuh"
 #include "ascan_mscan.cuh"
+#include "ascan_tc.cuh"
 
 namespace ascan {
 namespace cache {
+
+using namespace tc;
 
 using mscan::from_f;
 using mscan::Rows;
@@ -33,6 +36,28 @@ struct Cache {
 
 __device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
   return is64 ? static_cast<const long long*>(p)[i] : static_cast<long long>(static_cast<const int*>(p)[i]);
+}
+
+// Sixteen rows of a page from row `row`.
+__device__ __forceinline__ void tma_page(uint32_t to, const CUtensorMap* m, int row, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
+      "l"(m), "r"(0), "r"(row), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// All lanes; false when the copies did not come within the limit.
+__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* err) {
+  const unsigned long long start = now_ns();
+  while (!bar_try(b, parity))
+    if (now_ns() - start > kStageTimeoutNs) {
+      report(ASCAN_DEV_ERR_STAGE, (static_cast<unsigned long long>(blockIdx.x) << 32) | threadIdx.x, err);
+      return false;
+    }
+  return true;
+}
+__device__ __forceinline__ bool wait_group(uint64_t* b, uint32_t parity, uint32_t* err) {
+  return __all_sync(kFull, bar_try(b, parity) || wait_slow(b, parity, err));
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
@@ -193,9 +218,12 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
 // attention of single tokens
 // ---------------------------------------------------------------------------
 
-constexpr int kStepThreads = 128;
-constexpr int kStepTile = 64;  // tokens of a tile: sixteen of each warp
-constexpr int kMaxCtas = 148 * 4;
+constexpr int kStepWarps = 4, kStepThreads = kStepWarps * 32;
+constexpr int kGroup = 16;                        // tokens of a warp at a time
+constexpr int kStepTile = kStepWarps * kGroup;
+constexpr int kStages = 3;                        // groups in flight for each warp
+constexpr int kCtasPerSm = 3;
+constexpr int kMaxCtas = 148 * kCtasPerSm;
 
 struct StepArgs {
   Cache c;
@@ -204,58 +232,31 @@ struct StepArgs {
   int lengths64, H, share, row_tiles;  // sixteen query heads of a key head are a row tile
   float scale;
   void* out;
-  float* part;  // per CTA two slots of [16] references, [16] sums, [16][dv] rows
+  float* part;        // per CTA two slots of [16] references, [16] sums, [16][dv] rows
+  long long* before;  // [B + 1]: tiles of all requests before each
   uint32_t* err;
+};
+
+struct StepMaps {
+  CUtensorMap k, v;
 };
 
 __device__ __forceinline__ int slot_floats(int dv) { return 32 + 16 * dv; }
 
 // Tokens of request b; what does not fit its row of pages is left out.
-__device__ __forceinline__ long long length_of(const StepArgs& a, long long b) {
-  const long long n = index_at(a.lengths, a.lengths64, b), room = a.c.width * a.c.page;
-  return n < 0 ? 0 : min(n, room);
+__device__ __forceinline__ int length_of(const StepArgs& a, long long b) {
+  const long long n = index_at(a.lengths, a.lengths64, b), room = min(a.c.width * a.c.page, static_cast<long long>(ASCAN_ATTENTION_MAX_TOKENS));
+  if (n > room && blockIdx.x == 0) report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(b), a.err);
+  return static_cast<int>(n < 0 ? 0 : min(n, room));
 }
-__device__ __forceinline__ long long tiles_of(const StepArgs& a, long long b) {
-  return (length_of(a, b) + kStepTile - 1) / kStepTile;
-}
-
-// Sum over the block's 128 threads, the same for all; `scratch` of 4.
-__device__ __forceinline__ long long block_sum(long long x, long long* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(kFull, x, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-  __syncthreads();
-  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
-}
-
-// Tiles of all requests before `until`.
-__device__ __forceinline__ long long tiles_before(const StepArgs& a, long long until, long long* scratch) {
-  long long n = 0;
-  for (long long b = threadIdx.x; b < until; b += kStepThreads) {
-    n += tiles_of(a, b);
-    if (blockIdx.x == 0 && index_at(a.lengths, a.lengths64, b) > a.c.width * a.c.page)
-      report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(b), a.err);
-  }
-  return block_sum(n, scratch);
-}
+__device__ __forceinline__ int tiles_of_length(int n) { return (n + kStepTile - 1) / kStepTile; }
 
 __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t half2_from(float a, float b) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
 __device__ __forceinline__ float2 float2_of(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(kFull, x, 1));
   return fmaxf(x, __shfl_xor_sync(kFull, x, 2));
@@ -265,6 +266,104 @@ __device__ __forceinline__ float quad_sum(float x) {
   return x + __shfl_xor_sync(kFull, x, 2);
 }
 
+// Tiles of the requests: their total, and the request that tile `begin` of the
+// list lies in, with the tiles before it; the first CTA writes the sums down
+// for the launch that joins.  All threads of the block.
+struct Found {
+  long long total, before;
+  int b;
+};
+__device__ __forceinline__ Found find_request(const StepArgs& a, int groups, long long (&scratch)[kStepWarps + 1]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Found f{0, 0, 0};
+  long long begin = 0;
+  for (int pass = 0; pass < 2; ++pass) {  // the total, then the place
+    long long sum = 0;
+    for (long long b0 = 0; b0 < a.c.B; b0 += kStepThreads) {
+      const long long b = b0 + threadIdx.x;
+      const long long n = b < a.c.B ? tiles_of_length(length_of(a, b)) : 0;
+      long long inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const long long x = __shfl_up_sync(kFull, inc, o);
+        if (lane >= o) inc += x;
+      }
+      __syncthreads();
+      if (lane == 31) scratch[warp] = inc;
+      __syncthreads();
+      long long front = sum;
+      for (int w = 0; w < kStepWarps; ++w) {
+        if (w < warp) front += scratch[w];
+        sum += scratch[w];
+      }
+      inc += front;
+      if (pass == 0) {
+        if (blockIdx.x == 0 && b < a.c.B) {
+          if (b == 0) a.before[0] = 0;
+          a.before[b + 1] = inc;
+        }
+      } else if (begin >= (inc - n) * groups && begin < inc * groups) {
+        scratch[kStepWarps] = b;  // one thread's
+      }
+      if (pass == 1 && begin < sum * groups) {
+        __syncthreads();
+        f.b = static_cast<int>(scratch[kStepWarps]);
+        break;
+      }
+    }
+    if (pass == 0) {
+      f.total = sum * groups;
+      begin = f.total / gridDim.x * blockIdx.x + min(f.total % gridDim.x, static_cast<long long>(blockIdx.x));
+      if (begin >= f.total) return f;
+    }
+  }
+  // the tiles before it, from the lengths again
+  long long n = 0;
+  for (int b = threadIdx.x; b < f.b; b += kStepThreads) n += tiles_of_length(length_of(a, b));
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) n += __shfl_xor_sync(kFull, n, o);
+  __syncthreads();
+  if (lane == 0) scratch[warp] = n;
+  __syncthreads();
+  for (int w = 0; w < kStepWarps; ++w) f.before += scratch[w] * groups;
+  return f;
+}
+
+// A place in the list of tiles: request by request, key head and row tile by
+// row tile, and what the warp has of the tile.
+struct Place {
+  int b, group, tile, tiles, len;
+  int page, row;  // of the request's pages, and in it, where the warp's tokens begin
+
+  __device__ __forceinline__ void enter(const StepArgs& a, int warp) {
+    const int t0 = tile * kStepTile + warp * kGroup;
+    page = t0 / a.c.page;
+    row = t0 - page * a.c.page;
+  }
+  __device__ __forceinline__ void request(const StepArgs& a) {
+    len = length_of(a, b);
+    tiles = tiles_of_length(len);
+  }
+  __device__ __forceinline__ bool has(int warp) const { return tile * kStepTile + warp * kGroup < len; }
+  // There is a next one.
+  __device__ __forceinline__ void next(const StepArgs& a, int warp, int groups) {
+    if (++tile < tiles) {
+      row += kStepTile;
+      while (row >= a.c.page) row -= a.c.page, ++page;
+      return;
+    }
+    tile = 0;
+    if (++group == groups) {
+      group = 0;
+      do {
+        ++b;
+        request(a);
+      } while (tiles == 0);
+    }
+    enter(a, warp);
+  }
+};
+
 // The tiles of all requests, key heads and row tiles are one list; a CTA takes
 // an equal run of it, wherever requests begin and end, and walks it piece by
 // piece (a piece: what it has of one request, head and row tile).  Each warp
@@ -272,59 +371,123 @@ __device__ __forceinline__ float quad_sum(float x) {
 // values are exact there, queries are brought to at most 2^15 by a power of
 // two per row, and weights lie between 0 and 2^8, so both keep 11 bits or more
 // (22 where queries are float32: the rest of each goes through a second
-// product).  Keys and values go from memory to registers as the operands want
-// them, sixteen bytes a load: which dims and tokens stand for which index of a
-// product is free as long as both operands agree.
+// product).
+//
+// Memory bounds it, so each warp keeps kStages groups of sixteen tokens in
+// flight, over the ends of pieces too: 2 KB of keys and of values, each one TMA
+// copy into its own slots, and their scales behind the same barrier; the page
+// numbers are read one group earlier still.  From shared memory the operands
+// come sixteen bytes a load: which elements and tokens stand for which index of
+// a product is free as long as both operands agree, and the choice here
+// together with the copies' swizzle meets no bank twice.
 //
 // U: 64-element parts of a key.  NV: bytes of a value row per lane.
 template <typename T, int U, int NV>
-__global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : 3) step_kernel(const __grid_constant__ StepArgs a) {
+__global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
+    step_kernel(const __grid_constant__ StepArgs a, const __grid_constant__ StepMaps maps) {
   constexpr bool FINE = sizeof(T) == 4;
   constexpr int TERMS = FINE ? 2 : 1;
+  constexpr int KB = kGroup * 64 * U, VB = kGroup * 8 * NV;  // bytes of a group
+  extern __shared__ __align__(1024) unsigned char ring[];     // [warp][stage][keys, values]
+  __shared__ uint64_t full[kStepWarps][kStages];
+  __shared__ float scales[kStepWarps][kStages][2];
+  __shared__ int usable[kStepWarps][kStages];
+  __shared__ long long scratch[kStepWarps + 1];
+  __shared__ float s_m[kStepWarps][16], s_l[kStepWarps][16];
+  __shared__ float s_o[2][16][NV * 8 + 4];
   const Cache& c = a.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-  __shared__ long long scratch[4];
-  __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ float s_o[4][16][NV * 8 + 4];
-
   const int groups = c.heads * a.row_tiles;  // of a request
-  const long long total = tiles_before(a, c.B, scratch) * groups;
-  const long long begin = total / gridDim.x * blockIdx.x + min(total % gridDim.x, static_cast<long long>(blockIdx.x));
-  const long long end = begin + total / gridDim.x + (blockIdx.x < total % gridDim.x);
+
+  if (smem_u32(ring) & 1023u) {  // the swizzled layouts need it
+    if (threadIdx.x == 0) report(ASCAN_DEV_ERR_STAGE, 0xffffffffull, a.err);
+    return;
+  }
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) bar_init(&full[warp][i], 3);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
+  }
+  const Found f = find_request(a, groups, scratch);
+  const long long run = f.total / gridDim.x, more = f.total % gridDim.x;
+  const long long begin = run * blockIdx.x + min(more, static_cast<long long>(blockIdx.x));
+  const long long end = begin + run + (blockIdx.x < more);
   // requests without tokens, dealt to all CTAs
   for (long long b = blockIdx.x; b < c.B; b += gridDim.x)
-    if (tiles_of(a, b) == 0)
+    if (length_of(a, b) == 0)
       for (int e = threadIdx.x; e < a.H * c.dv; e += kStepThreads) static_cast<T*>(a.out)[b * a.H * c.dv + e] = from_f<T>(0.f);
   if (begin >= end) return;
 
-  // The request that `begin` lies in: 128 at a time, then one by one.
-  long long b = 0, before = 0;  // tiles of the requests before b, times groups
-  while (true) {
-    const long long n = b + threadIdx.x < c.B ? tiles_of(a, b + threadIdx.x) : 0;
-    const long long sum = block_sum(n, scratch) * groups;
-    if (before + sum > begin) break;
-    before += sum;
-    b += kStepThreads;
-  }
-  for (long long n; before + (n = tiles_of(a, b) * groups) <= begin; ++b) before += n;
+  Place get;
+  get.b = f.b;
+  get.request(a);
+  get.group = static_cast<int>((begin - f.before) / get.tiles);
+  get.tile = static_cast<int>((begin - f.before) % get.tiles);
+  get.enter(a, warp);
+  Place use = get;
+  unsigned char* slots = ring + warp * kStages * (KB + VB);
+
+  // ---- loads: `get` runs ahead of `use` ----
+  long long left = end - begin;  // places that are not loaded yet, `get` among them
+  bool seek = false;             // `get` has been passed
+  int loads = 0;                 // groups of this warp that were asked for
+  int id = -1;                   // page of `get`
+  // Moves `get` to the warp's next group and reads its page's number.
+  auto look = [&]() {
+    while (left > 0) {
+      if (seek) {
+        if (--left == 0) break;
+        get.next(a, warp, groups);
+      }
+      seek = true;
+      if (get.has(warp)) {
+        id = __ldg(c.table + get.b * c.width + get.page);
+        return;
+      }
+    }
+  };
+  bool alive = true;
+  auto load = [&]() {
+    if (left <= 0 || !alive) return;
+    const int at = loads % kStages;
+    uint64_t* bar = &full[warp][at];
+    const bool ok = id >= 0 && id < c.pages;
+    const int hk = get.group / a.row_tiles;
+    if (!ok) {
+      if (lane == 0) {
+        report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(get.b), a.err);
+        usable[warp][at] = 0;
+      }
+      if (lane < 3) bar_arrive(bar);
+    } else if (lane == 0) {
+      usable[warp][at] = 1;
+      bar_expect(bar, KB + VB);
+      const uint32_t to = smem_u32(slots + at * (KB + VB));
+      tma_page(to, &maps.k, get.row, id * c.heads + hk, bar);
+      tma_page(to + KB, &maps.v, get.row, id * c.heads + hk, bar);
+    } else if (lane < 3) {
+      const float* from = (lane == 1 ? c.ks : c.vs) + static_cast<long long>(id) * c.heads + hk;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[warp][at][lane - 1])), "l"(from) : "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    }
+    ++loads;
+    __syncwarp();
+    look();
+  };
+  look();
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) load();
 
   const float c2 = a.scale * 1.4426950408889634f;
-  int slot = 0;
+  int slot = 0, used = 0;
+#pragma unroll 1
   for (long long at = begin; at < end; ) {
-    const long long tiles = tiles_of(a, b), rel = at - before;
-    if (rel >= tiles * groups) {  // next request with tokens
-      before += tiles * groups;
-      ++b;
-      continue;
-    }
-    const int group = static_cast<int>(rel / tiles);
-    const long long tile0 = rel % tiles, tile1 = min(tiles, tile0 + (end - at));
-    const int hk = group / a.row_tiles, h0 = hk * a.share + group % a.row_tiles * 16;
+    const int tile0 = use.tile, tile1 = static_cast<int>(min(static_cast<long long>(use.tiles), tile0 + (end - at)));
+    const int hk = use.group / a.row_tiles, h0 = hk * a.share + use.group % a.row_tiles * 16;
     const int rows = min(16, (hk + 1) * a.share - h0);
-    const long long len = length_of(a, b);
 
     // ---- queries as operands: index 2 t4.. of product (u, w) is element
-    // 64 u + 16 t4 + 4 w.. of the head
+    // 16 (U t4 + u) + 4 w.. of the head
     uint32_t q[TERMS][U * 4][4];
     float qf[2];  // what a row's scores are in units of
 #pragma unroll
@@ -332,116 +495,70 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : 3) step_ker
       const int row = g + 8 * r;
       float x[U * 16], top = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int d = 64 * u + 16 * t4 + e;
-          x[u * 16 + e] = row < rows && d < c.dk ? to_f(static_cast<const T*>(a.q.p)[b * a.q.st + (h0 + row) * a.q.sh + d]) : 0.f;
-          top = fmaxf(top, fabsf(x[u * 16 + e]));
-        }
+      for (int e = 0; e < U * 16; ++e) {
+        const int d = 16 * U * t4 + e;
+        x[e] = row < rows && d < c.dk ? to_f(static_cast<const T*>(a.q.p)[use.b * a.q.st + (h0 + row) * a.q.sh + d]) : 0.f;
+        top = fmaxf(top, fabsf(x[e]));
+      }
       top = quad_max(top);
       const int e2 = max(-100, static_cast<int>(__float_as_uint(top) >> 23) - 127);
       const float up = pow2(14 - e2);
       qf[r] = pow2(e2 - 14) * c2;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U * 4; ++u)
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float y0 = x[u * 16 + w * 4 + half * 2] * up, y1 = x[u * 16 + w * 4 + half * 2 + 1] * up;
-            const uint32_t hi = half2_from(y0, y1);
-            q[0][u * 4 + w][half * 2 + r] = hi;
-            if (FINE) {
-              const float2 f = float2_of(hi);
-              q[TERMS - 1][u * 4 + w][half * 2 + r] = half2_from(y0 - f.x, y1 - f.y);
-            }
+        for (int half = 0; half < 2; ++half) {
+          const float y0 = x[u * 4 + half * 2] * up, y1 = x[u * 4 + half * 2 + 1] * up;
+          const uint32_t hi = hf2(y0, y1);
+          q[0][u][half * 2 + r] = hi;
+          if (FINE) {
+            const float2 z = float2_of(hi);
+            q[TERMS - 1][u][half * 2 + r] = hf2(y0 - z.x, y1 - z.y);
           }
+        }
     }
 
     float o[NV][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-    uint4 kr[2][U];
-    uint32_t vr[4][NV / 4];
-    float kscale = 0.f, vscale = 1.f;
-    bool ok = false;
-    const int* row_of_pages = c.table + b * c.width;
-    long long id = 0;
-    auto page_of = [&](long long tile) {
-      const long long t0 = tile * kStepTile + warp * 16;
-      ok = tile < tile1 && t0 < len;
-      if (!ok) return;
-      id = __ldg(row_of_pages + t0 / c.page);
-      if (id < 0 || id >= c.pages) {
-        if (lane == 0) report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(b), a.err);
-        ok = false;
-      }
-    };
-    auto load_k = [&](long long tile) {
-      if (!ok) return;
-      const int in_page = static_cast<int>((tile * kStepTile + warp * 16) % c.page);
-      const uint8_t* at_k = c.k + ((id * c.heads + hk) * c.page + in_page) * c.dk;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          kr[i][u] = 64 * u + 16 * t4 < c.dk ? __ldcs(reinterpret_cast<const uint4*>(at_k + (8 * i + g) * c.dk + 64 * u + 16 * t4))
-                                             : make_uint4(0, 0, 0, 0);
-      kscale = __ldg(c.ks + id * c.heads + hk);
-    };
-    auto load_v = [&](long long tile) {
-      if (!ok) return;
-      const int in_page = static_cast<int>((tile * kStepTile + warp * 16) % c.page);
-      const uint8_t* at_v = c.v + ((id * c.heads + hk) * c.page + in_page) * c.dv;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int tok = (j >> 1) * 8 + 2 * t4 + (j & 1);
-        if (NV == 16) {
-          const uint4 x = g * 16 < c.dv ? __ldcs(reinterpret_cast<const uint4*>(at_v + tok * c.dv + g * 16)) : make_uint4(0, 0, 0, 0);
-          vr[j][0] = x.x, vr[j][1] = x.y, vr[j][NV / 4 - 2] = x.z, vr[j][NV / 4 - 1] = x.w;
-        } else {
-          const uint2 x = g * 8 < c.dv ? __ldcs(reinterpret_cast<const uint2*>(at_v + tok * c.dv + g * 8)) : make_uint2(0, 0);
-          vr[j][0] = x.x, vr[j][1] = x.y;
-        }
-      }
-      vscale = __ldg(c.vs + id * c.heads + hk);
-    };
-
-    page_of(tile0);
-    load_k(tile0);
-    load_v(tile0);
 #pragma unroll 1
-    for (long long tile = tile0; tile < tile1; ++tile) {
-      const bool now = ok;
-      float w[2][4], vsc = vscale;
-      const long long t0 = tile * kStepTile + warp * 16;
-      const int left = static_cast<int>(min(16ll, len - t0));  // tokens of the sixteen
-      if (now) {
+    for (int tile = tile0; tile < tile1; ++tile) {
+      const int tokens = min(kGroup, use.len - (tile * kStepTile + warp * kGroup));
+      if (tokens <= 0) continue;
+      const int at_stage = used % kStages;
+      if (alive) alive = wait_group(&full[warp][at_stage], (used / kStages) & 1, a.err);
+      ++used;
+      const unsigned char* ks = slots + at_stage * (KB + VB);
+      const unsigned char* vs = ks + KB;
+      if (alive && usable[warp][at_stage]) {
+        const float kscale = scales[warp][at_stage][0], vscale = scales[warp][at_stage][1];
         float s[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+          const int row = 8 * i + g;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const uint32_t word[4] = {kr[i][u].x, kr[i][u].y, kr[i][u].z, kr[i][u].w};
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                ks + row * 64 * U + (U == 2 ? ((2 * t4 + u) ^ (row & 7)) << 4 : (t4 ^ ((row >> 1) & 3)) << 4));
+            const uint32_t word[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t b0 = half2_of(static_cast<uint16_t>(word[e])), b1 = half2_of(static_cast<uint16_t>(word[e] >> 16));
 #pragma unroll
-              for (int x = 0; x < TERMS; ++x) mma(s[i], q[TERMS - 1 - x][u * 4 + e], b0, b1);
+              for (int z = 0; z < TERMS; ++z) mma(s[i], q[TERMS - 1 - z][u * 4 + e], b0, b1);
             }
           }
         }
         // in units of log 2; a page's value scale is added to the exponent
-        const float lv = static_cast<float>(static_cast<int>(__float_as_uint(vsc) >> 23) - 127);
+        const float lv = static_cast<float>(static_cast<int>(__float_as_uint(vscale) >> 23) - 127);
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const bool in = 8 * i + 2 * t4 + (e & 1) < left;
+            const bool in = 8 * i + 2 * t4 + (e & 1) < tokens;
             s[i][e] = in ? s[i][e] * (qf[e >> 1] * kscale) : -INFINITY;
             top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
           }
@@ -449,49 +566,48 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : 3) step_ker
         for (int r = 0; r < 2; ++r) top[r] = quad_max(top[r]) + lv;
         // the reference moves when weights would pass 2^8
         if (__any_sync(kFull, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
-          float f[2];
+          float fall[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float next = fmaxf(m[r], top[r]);
-            f[r] = next == -INFINITY ? 1.f : ex2(m[r] - next);
+            fall[r] = next == -INFINITY ? 1.f : ex2(m[r] - next);
             m[r] = next;
-            l[r] *= f[r];
+            l[r] *= fall[r];
           }
 #pragma unroll
-          for (int i = 0; i < NV; ++i) o[i][0] *= f[0], o[i][1] *= f[0], o[i][2] *= f[1], o[i][3] *= f[1];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float ref = m[e >> 1] == -INFINITY ? 0.f : m[e >> 1];
-            const float p = ex2(s[i][e] - ref);
-            l[e >> 1] += p;
-            w[i][e] = p * vsc;
-          }
-      }
-      page_of(tile + 1);
-      load_k(tile + 1);
-      if (now) {
-        if (left < 16) {  // what lies behind the last token may be anything
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if ((j >> 1) * 8 + 2 * t4 + (j & 1) >= left)
-#pragma unroll
-              for (int e = 0; e < NV / 4; ++e) vr[j][e] = 0;
+          for (int i = 0; i < NV; ++i) o[i][0] *= fall[0], o[i][1] *= fall[0], o[i][2] *= fall[1], o[i][3] *= fall[1];
         }
         uint32_t pa[TERMS][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t hi = half2_from(w[i][2 * r], w[i][2 * r + 1]);
+            const float ref = m[r] == -INFINITY ? 0.f : m[r];
+            const float p0 = ex2(s[i][2 * r] - ref), p1 = ex2(s[i][2 * r + 1] - ref);
+            l[r] += p0 + p1;
+            const float w0 = p0 * vscale, w1 = p1 * vscale;
+            const uint32_t hi = hf2(w0, w1);
             pa[0][2 * i + r] = hi;
             if (FINE) {
-              const float2 f = float2_of(hi);
-              pa[TERMS - 1][2 * i + r] = half2_from(w[i][2 * r] - f.x, w[i][2 * r + 1] - f.y);
+              const float2 z = float2_of(hi);
+              pa[TERMS - 1][2 * i + r] = hf2(w0 - z.x, w1 - z.y);
             }
           }
+        uint32_t vr[4][NV / 4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = (j >> 1) * 8 + 2 * t4 + (j & 1);
+          if (NV == 16) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vs + row * 128 + ((g ^ (row & 7)) << 4));
+            vr[j][0] = x.x, vr[j][1] = x.y, vr[j][NV / 4 - 2] = x.z, vr[j][NV / 4 - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(vs + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+            vr[j][0] = x.x, vr[j][1] = x.y;
+          }
+          if (tokens < kGroup && row >= tokens)  // what lies behind the last token may be anything
+#pragma unroll
+            for (int e = 0; e < NV / 4; ++e) vr[j][e] = 0;
+        }
 #pragma unroll
         for (int e = 0; e < NV / 4; ++e)
 #pragma unroll
@@ -507,122 +623,193 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : 3) step_ker
             }
           }
       }
-      load_v(tile + 1);
+      __syncwarp();  // the slot has been read
+      load();
     }
 
-    // ---- the warps' parts of the piece meet ----
+    // ---- the warps' parts of the piece meet: two and two, then both ----
 #pragma unroll
     for (int r = 0; r < 2; ++r) l[r] = quad_sum(l[r]);
-    __syncthreads();  // the piece before has been read
     if (t4 == 0)
 #pragma unroll
       for (int r = 0; r < 2; ++r) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
+    __syncthreads();
+    float fall[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = g + 8 * r;
+      const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+      fall[r] = ex2(m[r] - (top == -INFINITY ? 0.f : top));
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i][0] *= fall[0], o[i][1] *= fall[0], o[i][2] *= fall[1], o[i][3] *= fall[1];
     // column n of product i is element NV n + i of the value; lane t4 has
     // columns 2 t4 and 2 t4 + 1
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+      if (warp >> 1 == 1 - turn) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s_o[warp][g + 8 * (e >> 1)][(2 * t4 + (e & 1)) * NV + i] = o[i][e];
-    __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
+          for (int e = 0; e < 4; ++e) {
+            float* to = &s_o[warp & 1][g + 8 * (e >> 1)][(2 * t4 + (e & 1)) * NV + i];
+            *to = turn == 0 ? o[i][e] : *to + o[i][e];
+          }
+      }
+      __syncthreads();
+    }
+    const bool whole = tile0 == 0 && tile1 == use.tiles;
     float* part = a.part + (static_cast<long long>(blockIdx.x) * 2 + slot) * slot_floats(c.dv);
     for (int e = threadIdx.x; e < rows * c.dv; e += kStepThreads) {
       const int row = e / c.dv, d = e % c.dv;
-      float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+      const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
       const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, x = 0.f;
+      float sum = 0.f;
 #pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        const float f = ex2(s_m[z][row] - ref);
-        sum = fmaf(s_l[z][row], f, sum);
-        x = fmaf(s_o[z][row][d], f, x);
-      }
+      for (int z = 0; z < kStepWarps; ++z) sum = fmaf(s_l[z][row], ex2(s_m[z][row] - ref), sum);
+      const float x = s_o[0][row][d] + s_o[1][row][d];
       if (whole) {
-        static_cast<T*>(a.out)[(b * a.H + h0 + row) * c.dv + d] = from_f<T>(x / sum);
+        static_cast<T*>(a.out)[(static_cast<long long>(use.b) * a.H + h0 + row) * c.dv + d] = from_f<T>(x / sum);
       } else {
         if (d == 0) part[row] = top, part[16 + row] = sum;
         part[32 + row * c.dv + d] = x;
       }
     }
+    __syncthreads();  // read before the next piece's are written
     slot = 1;  // pieces after the first begin with their request's first tile
     at += tile1 - tile0;
+    use.tile = tile1 - 1;
+    if (at < end) use.next(a, warp, groups);
   }
 }
 
 // Joins the parts of rows that several CTAs had, in the CTAs' order: a CTA per
-// query head of a request; 128 threads take the elements, and quarter z of the
-// CTA every fourth part.
-template <typename T>
-__global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ StepArgs a, int ctas) {
+// query head of a request; 128 threads take the elements, and slice z of the
+// CTA every Z-th part.
+template <typename T, int Z>
+__global__ void __launch_bounds__(128 * Z) join_kernel(const __grid_constant__ StepArgs a, int ctas) {
   const Cache& c = a.c;
-  __shared__ long long scratch[16];
-  __shared__ float s_m[4], s_l[4], s_x[4][128];
+  __shared__ float s_m[Z], s_l[Z], s_x[Z][128];
   const long long b = blockIdx.y;
-  const int h = blockIdx.x, tid = threadIdx.x, z = tid >> 7, d = tid & 127;
-  long long n = 0, all = 0;
-  for (long long i = tid; i < c.B; i += 512) {
-    const long long x = tiles_of(a, i);
-    all += x;
-    if (i < b) n += x;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) all += __shfl_xor_sync(kFull, all, o), n += __shfl_xor_sync(kFull, n, o);
-  if ((tid & 31) == 0) scratch[tid >> 5] = all;
-  __syncthreads();
-  all = 0;
-  for (int i = 0; i < 16; ++i) all += scratch[i];
-  __syncthreads();
-  if ((tid & 31) == 0) scratch[tid >> 5] = n;
-  __syncthreads();
-  n = 0;
-  for (int i = 0; i < 16; ++i) n += scratch[i];
+  const int h = blockIdx.x, z = threadIdx.x >> 7, d = threadIdx.x & 127;
+  const long long n = a.before[b], tiles = a.before[b + 1] - n;
   const int groups = c.heads * a.row_tiles, row = h % a.share % 16;
-  const long long tiles = tiles_of(a, b), total = all * groups;
+  const long long total = a.before[c.B] * groups;
   if (tiles == 0) return;
   const long long first = n * groups + (h / a.share * a.row_tiles + h % a.share / 16) * tiles, last = first + tiles - 1;
   // the CTA that has tile t: runs of size + 1 come first
   const long long size = total / ctas, more = total % ctas;
   auto cta_of = [&](long long t) { return t < more * (size + 1) ? t / (size + 1) : more + (t - more * (size + 1)) / size; };
   auto begin_of = [&](long long i) { return size * i + min(more, i); };
-  const long long i0 = cta_of(first), i1 = cta_of(last);
+  const int i0 = static_cast<int>(cta_of(first)), i1 = static_cast<int>(cta_of(last));
   if (i0 == i1) return;  // that CTA wrote it
   float m = -INFINITY, l = 0.f, x = 0.f;
-  for (long long i = i0 + z; i <= i1; i += 4) {
-    // a CTA's first piece is in slot 0; one that it came to later in slot 1
-    const float* part = a.part + (2 * i + (begin_of(i) < first)) * slot_floats(c.dv);
-    const float pm = part[row], pl = part[16 + row], px = d < c.dv ? part[32 + row * c.dv + d] : 0.f;
-    const float next = fmaxf(m, pm), ref = next == -INFINITY ? 0.f : next;
-    const float f = ex2(m - ref), e = ex2(pm - ref);
-    l = fmaf(l, f, pl * e);
-    x = fmaf(x, f, px * e);
-    m = next;
-  }
-  if (d == 0) s_m[z] = m, s_l[z] = l;
-  s_x[z][d] = x;
-  __syncthreads();
-  if (z != 0 || d >= c.dv) return;
-  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), ref = top == -INFINITY ? 0.f : top;
-  l = x = 0.f;
+  constexpr int D = 8;  // parts in flight
+  for (int i = i0 + z; i <= i1; i += Z * D) {
+    float pm[D], pl[D], px[D], top = m;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float f = ex2(s_m[i] - ref);
-    l = fmaf(s_l[i], f, l);
-    x = fmaf(s_x[i][d], f, x);
+    for (int e = 0; e < D; ++e) {
+      pm[e] = -INFINITY, pl[e] = px[e] = 0.f;
+      const int j = i + e * Z;
+      if (j <= i1) {
+        // a CTA's first piece is in slot 0; one that it came to later in slot 1
+        const float* part = a.part + (2ll * j + (begin_of(j) < first)) * slot_floats(c.dv);
+        pm[e] = part[row], pl[e] = part[16 + row];
+        if (d < c.dv) px[e] = part[32 + row * c.dv + d];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < D; ++e) top = fmaxf(top, pm[e]);
+    const float ref = top == -INFINITY ? 0.f : top, keep = ex2(m - ref);
+    l *= keep, x *= keep, m = top;
+#pragma unroll
+    for (int e = 0; e < D; ++e) {
+      const float f = ex2(pm[e] - ref);
+      l = fmaf(pl[e], f, l);
+      x = fmaf(px[e], f, x);
+    }
   }
-  static_cast<T*>(a.out)[(b * a.H + h) * c.dv + d] = from_f<T>(x / l);
+  if (Z > 1) {
+    if (d == 0) s_m[z] = m, s_l[z] = l;
+    s_x[z][d] = x;
+    __syncthreads();
+    if (z != 0) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < Z; ++i) top = fmaxf(top, s_m[i]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    l = x = 0.f;
+#pragma unroll
+    for (int i = 0; i < Z; ++i) {
+      const float f = ex2(s_m[i] - ref);
+      l = fmaf(s_l[i], f, l);
+      x = fmaf(s_x[i][d], f, x);
+    }
+  }
+  if (d < c.dv) static_cast<T*>(a.out)[(b * a.H + h) * c.dv + d] = from_f<T>(x / l);
+}
+
+// Sixteen rows of a page: rows of 128 bytes or 64, zeros behind the head's last
+// element.
+static bool map_pages(CUtensorMap* m, const uint8_t* pool, const Cache& c, int dim) {
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const bool wide = dim > 64;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(c.page), static_cast<cuuint64_t>(c.pages) * c.heads};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(dim) * c.page};
+  const cuuint32_t box[3] = {wide ? 128u : 64u, kGroup, 1}, one[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(pool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int U, int NV>
+static int launch_step(const StepArgs& a, const StepMaps& m, int ctas, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{};
+  constexpr size_t bytes = static_cast<size_t>(kStepWarps) * kStages * kGroup * (64 * U + 8 * NV);
+  const int rc = mscan::allow_smem(step_kernel<T, U, NV>, bytes, done);
+  if (rc != ASCAN_OK) return rc;
+  step_kernel<T, U, NV><<<ctas, kStepThreads, bytes, s>>>(a, m);
+  return launch_status();
 }
 
 template <typename T>
-static int step(const StepArgs& a, int ctas, cudaStream_t s) {
+static int step(const StepArgs& a, const StepMaps& m, cudaStream_t s) {
+  const int ctas = 148 * (sizeof(T) == 4 ? 2 : kCtasPerSm);
   const bool wide_k = a.c.dk > 64, wide_v = a.c.dv > 64;
-  if (wide_k && wide_v) step_kernel<T, 2, 16><<<ctas, kStepThreads, 0, s>>>(a);
-  else if (wide_k) step_kernel<T, 2, 8><<<ctas, kStepThreads, 0, s>>>(a);
-  else if (wide_v) step_kernel<T, 1, 16><<<ctas, kStepThreads, 0, s>>>(a);
-  else step_kernel<T, 1, 8><<<ctas, kStepThreads, 0, s>>>(a);
-  const int rc = launch_status();
+  const int rc = wide_k ? (wide_v ? launch_step<T, 2, 16>(a, m, ctas, s) : launch_step<T, 2, 8>(a, m, ctas, s))
+                        : (wide_v ? launch_step<T, 1, 16>(a, m, ctas, s) : launch_step<T, 1, 8>(a, m, ctas, s));
   if (rc != ASCAN_OK) return rc;
-  join_kernel<T><<<dim3(a.H, static_cast<unsigned>(a.c.B)), 512, 0, s>>>(a, ctas);
+  // a row of a few requests lies in many CTAs' parts, one of many in one or two
+  const dim3 grid(a.H, static_cast<unsigned>(a.c.B));
+  if (a.c.B * a.c.heads * a.row_tiles * 4 < ctas) join_kernel<T, 4><<<grid, 512, 0, s>>>(a, ctas);
+  else join_kernel<T, 1><<<grid, 128, 0, s>>>(a, ctas);
   return launch_status();
+}
+
+// A pool without pages: every row is zero, and one with tokens an error.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) no_pages_kernel(const __grid_constant__ StepArgs a) {
+  const long long n = a.c.B * a.H * a.c.dv;
+  for (long long e = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; e < n; e += gridDim.x * static_cast<long long>(kThreads)) {
+    static_cast<T*>(a.out)[e] = from_f<T>(0.f);
+    const long long b = e / (static_cast<long long>(a.H) * a.c.dv);
+    if (index_at(a.lengths, a.lengths64, b) > 0) report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(b), a.err);
+  }
+}
+
+template <typename T>
+static int run_step(StepArgs& a, cudaStream_t s) {
+  if (a.c.pages == 0) {
+    no_pages_kernel<T><<<148, kThreads, 0, s>>>(a);
+    return launch_status();
+  }
+  // Tensor maps are made through the driver, which wants a current context
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return ASCAN_EDEVICE;
+  StepMaps m;
+  if (!map_pages(&m.k, a.c.k, a.c, a.c.dk) || !map_pages(&m.v, a.c.v, a.c, a.c.dv)) return ASCAN_ECUDA;
+  return step<T>(a, m, s);
 }
 
 template <typename T>
@@ -637,7 +824,7 @@ static int write(const WriteArgs& a, int vec_k, int vec_v, cudaStream_t s) {
 static bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int fill(Cache& c, const ascan_cache* x, const int32_t* table, int64_t B, int64_t width) {
-  if (!x || x->pages < 0 || x->heads <= 0 || x->heads > 65535 || x->page <= 0 || x->page > ASCAN_CACHE_MAX_PAGE ||
+  if (!x || x->pages < 0 || x->heads <= 0 || x->heads > 65535 || x->pages > 0x7fffffffll / x->heads || x->page <= 0 || x->page > ASCAN_CACHE_MAX_PAGE ||
       x->page % 16 || x->key_dim <= 0 || x->value_dim <= 0 || x->key_dim % 16 || x->value_dim % 16 ||
       x->key_dim > ASCAN_ATTENTION_MAX_DIM || x->value_dim > ASCAN_ATTENTION_MAX_DIM)
     return ASCAN_EINVAL;
@@ -694,9 +881,9 @@ int ascan_cache_write(const ascan_rows* keys, const ascan_rows* values, const as
   return cache::write<__nv_bfloat16>(a, vec[0], vec[1], s);
 }
 
-size_t ascan_cache_step_workspace(int value_dim) {
-  if (value_dim <= 0) return 256;
-  return 256 + sizeof(float) * 2 * cache::kMaxCtas * (32 + 16 * static_cast<size_t>(value_dim));
+size_t ascan_cache_step_workspace(int64_t num_seq, int value_dim) {
+  if (num_seq <= 0 || value_dim <= 0) return 256;
+  return 512 + sizeof(float) * 2 * cache::kMaxCtas * (32 + 16 * static_cast<size_t>(value_dim)) + sizeof(long long) * (num_seq + 1);
 }
 
 int ascan_cache_step(const ascan_rows* queries, const ascan_cache* cache, const int32_t* pages, int64_t num_seq,
@@ -710,7 +897,7 @@ int ascan_cache_step(const ascan_rows* queries, const ascan_cache* cache, const 
   if (num_seq == 0) return ASCAN_OK;
   if (!cache::rows_ok(queries) || queries->heads % cache->heads || !lengths || !out) return ASCAN_EINVAL;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
-      workspace_bytes < ascan_cache_step_workspace(cache->value_dim))
+      workspace_bytes < ascan_cache_step_workspace(num_seq, cache->value_dim))
     return ASCAN_EWORKSPACE;
   a.q = mscan::Rows{queries->data, queries->stride_token, queries->stride_head, 1};
   a.lengths = lengths;
@@ -720,13 +907,13 @@ int ascan_cache_step(const ascan_rows* queries, const ascan_cache* cache, const 
   a.row_tiles = (a.share + 15) / 16;
   a.scale = scale;
   a.out = out;
-  a.part = static_cast<float*>(workspace);
+  a.before = static_cast<long long*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (sizeof(long long) * (num_seq + 1) + 255) / 256 * 256);
   a.err = g_err_host;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int ctas = 148 * 3;
-  if (dtype == ASCAN_F32) return cache::step<float>(a, ctas, s);
-  if (dtype == ASCAN_F16) return cache::step<__half>(a, ctas, s);
-  return cache::step<__nv_bfloat16>(a, ctas, s);
+  if (dtype == ASCAN_F32) return cache::run_step<float>(a, s);
+  if (dtype == ASCAN_F16) return cache::run_step<__half>(a, s);
+  return cache::run_step<__nv_bfloat16>(a, s);
 }
 
 }  // extern "C"

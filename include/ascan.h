@@ -537,7 +537,7 @@ ASCAN_API int ascan_cache_write(const ascan_rows* keys, const ascan_rows* values
                                 int dtype, void* stream);
 
 /* Bytes of workspace of ascan_cache_step. */
-ASCAN_API size_t ascan_cache_step_workspace(int value_dim);
+ASCAN_API size_t ascan_cache_step_workspace(int64_t num_seq, int value_dim);
 
 /*
  * Softmax attention of one query token of each of num_seq requests over the
