@@ -24,6 +24,7 @@ using mscan::Rows;
 using mscan::to_f;
 
 constexpr int kScaleBits = 64;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct Cache {
   uint8_t *k, *v;  // [pages, heads, page, dim]
@@ -218,10 +219,10 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
 // attention of single tokens
 // ---------------------------------------------------------------------------
 
-constexpr int kStepWarps = 4, kStepThreads = kStepWarps * 32;
-constexpr int kGroup = 16;                        // tokens of a warp at a time
+constexpr int kStepWarps = 4;                          // that compute; a fifth loads
+constexpr int kStepThreads = (kStepWarps + 1) * 32;
+constexpr int kGroup = 16;                             // tokens of a warp at a time
 constexpr int kStepTile = kStepWarps * kGroup;
-constexpr int kStages = 3;                        // groups in flight for each warp
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 148 * kCtasPerSm;
 
@@ -251,10 +252,21 @@ __device__ __forceinline__ int length_of(const StepArgs& a, long long b) {
 }
 __device__ __forceinline__ int tiles_of_length(int n) { return (n + kStepTile - 1) / kStepTile; }
 
+// d += A B with R * 8 rows of A; of eight, the other half of the product is
+// zeros and takes no registers.
+template <int R>
 __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if (R == 2) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2 * R - 2]), "+f"(d[2 * R - 1])
+                 : "r"(a[0]), "r"(a[R - 1]), "r"(a[R]), "r"(a[2 * R - 1]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "{\n .reg .f32 x, y;\n"
+        " mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, x, y}, {%2, %6, %3, %6}, {%4, %5}, {%0, %1, %7, %7};\n}\n"
+        : "+f"(d[0]), "+f"(d[1])
+        : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0), "f"(0.f));
+  }
 }
 __device__ __forceinline__ float2 float2_of(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 __device__ __forceinline__ float quad_max(float x) {
@@ -273,7 +285,7 @@ struct Found {
   long long total, before;
   int b;
 };
-__device__ __forceinline__ Found find_request(const StepArgs& a, int groups, long long (&scratch)[kStepWarps + 1]) {
+__device__ __forceinline__ Found find_request(const StepArgs& a, int groups, long long (&scratch)[kStepWarps + 2]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Found f{0, 0, 0};
   long long begin = 0;
@@ -292,7 +304,7 @@ __device__ __forceinline__ Found find_request(const StepArgs& a, int groups, lon
       if (lane == 31) scratch[warp] = inc;
       __syncthreads();
       long long front = sum;
-      for (int w = 0; w < kStepWarps; ++w) {
+      for (int w = 0; w <= kStepWarps; ++w) {
         if (w < warp) front += scratch[w];
         sum += scratch[w];
       }
@@ -303,11 +315,11 @@ __device__ __forceinline__ Found find_request(const StepArgs& a, int groups, lon
           a.before[b + 1] = inc;
         }
       } else if (begin >= (inc - n) * groups && begin < inc * groups) {
-        scratch[kStepWarps] = b;  // one thread's
+        scratch[kStepWarps + 1] = b;  // one thread's
       }
       if (pass == 1 && begin < sum * groups) {
         __syncthreads();
-        f.b = static_cast<int>(scratch[kStepWarps]);
+        f.b = static_cast<int>(scratch[kStepWarps + 1]);
         break;
       }
     }
@@ -325,7 +337,7 @@ __device__ __forceinline__ Found find_request(const StepArgs& a, int groups, lon
   __syncthreads();
   if (lane == 0) scratch[warp] = n;
   __syncthreads();
-  for (int w = 0; w < kStepWarps; ++w) f.before += scratch[w] * groups;
+  for (int w = 0; w <= kStepWarps; ++w) f.before += scratch[w] * groups;
   return f;
 }
 
@@ -364,37 +376,45 @@ struct Place {
   }
 };
 
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kStepWarps * 32) : "memory"); }
+
+// Groups in flight for each warp: what three CTAs of an SM have room for.
+__host__ __device__ constexpr int stages(int r) { return r == 1 ? 4 : 3; }
+
 // The tiles of all requests, key heads and row tiles are one list; a CTA takes
 // an equal run of it, wherever requests begin and end, and walks it piece by
-// piece (a piece: what it has of one request, head and row tile).  Each warp
-// takes sixteen tokens of a tile with m16n8k16 products of float16: e4m3
+// piece (a piece: what it has of one request, head and row tile).  Each of four
+// warps takes sixteen tokens of a tile with m16n8k16 products of float16: e4m3
 // values are exact there, queries are brought to at most 2^15 by a power of
 // two per row, and weights lie between 0 and 2^8, so both keep 11 bits or more
 // (22 where queries are float32: the rest of each goes through a second
 // product).
 //
-// Memory bounds it, so each warp keeps kStages groups of sixteen tokens in
+// Memory bounds it, so each warp has several groups of sixteen tokens in
 // flight, over the ends of pieces too: 2 KB of keys and of values, each one TMA
-// copy into its own slots, and their scales behind the same barrier; the page
-// numbers are read one group earlier still.  From shared memory the operands
-// come sixteen bytes a load: which elements and tokens stand for which index of
-// a product is free as long as both operands agree, and the choice here
-// together with the copies' swizzle meets no bank twice.
+// copy into its own slots, and their scales behind the same barrier.  A fifth
+// warp asks for them, a lane for each of the four (when each warp asked for its
+// own, 600 instructions went into a group, and 128 requests of 4000 tokens took
+// 163 us).  From shared memory the operands come sixteen bytes a load: which
+// elements and tokens stand for which index of a product is free as long as
+// both operands agree, and the choice here together with the copies' swizzle
+// meets no bank twice.
 //
-// U: 64-element parts of a key.  NV: bytes of a value row per lane.
-template <typename T, int U, int NV>
+// U: 64-element parts of a key.  NV: bytes of a value row per lane.  R: query
+// rows in eights (one if no key head has more than eight queries).
+template <typename T, int U, int NV, int R>
 __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
     step_kernel(const __grid_constant__ StepArgs a, const __grid_constant__ StepMaps maps) {
   constexpr bool FINE = sizeof(T) == 4;
-  constexpr int TERMS = FINE ? 2 : 1;
+  constexpr int TERMS = FINE ? 2 : 1, S = stages(R);
   constexpr int KB = kGroup * 64 * U, VB = kGroup * 8 * NV;  // bytes of a group
   extern __shared__ __align__(1024) unsigned char ring[];     // [warp][stage][keys, values]
-  __shared__ uint64_t full[kStepWarps][kStages];
-  __shared__ float scales[kStepWarps][kStages][2];
-  __shared__ int usable[kStepWarps][kStages];
-  __shared__ long long scratch[kStepWarps + 1];
-  __shared__ float s_m[kStepWarps][16], s_l[kStepWarps][16];
-  __shared__ float s_o[2][16][NV * 8 + 4];
+  __shared__ uint64_t full[kStepWarps][S], empty[kStepWarps][S];
+  __shared__ float scales[kStepWarps][S][2];
+  __shared__ int usable[kStepWarps][S];
+  __shared__ long long scratch[kStepWarps + 2];
+  __shared__ float s_m[kStepWarps][8 * R], s_l[kStepWarps][8 * R];
+  __shared__ float s_o[2][8 * R][NV * 8 + 4];
   const Cache& c = a.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
   const int groups = c.heads * a.row_tiles;  // of a request
@@ -403,12 +423,12 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
     if (threadIdx.x == 0) report(ASCAN_DEV_ERR_STAGE, 0xffffffffull, a.err);
     return;
   }
-  if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) bar_init(&full[warp][i], 3);
+  if (threadIdx.x < kStepWarps) {
+    for (int i = 0; i < S; ++i) bar_init(&full[lane][i], 2), bar_init(&empty[lane][i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async();
   }
-  const Found f = find_request(a, groups, scratch);
+  const Found f = find_request(a, groups, scratch);  // and all threads have met
   const long long run = f.total / gridDim.x, more = f.total % gridDim.x;
   const long long begin = run * blockIdx.x + min(more, static_cast<long long>(blockIdx.x));
   const long long end = begin + run + (blockIdx.x < more);
@@ -418,68 +438,52 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
       for (int e = threadIdx.x; e < a.H * c.dv; e += kStepThreads) static_cast<T*>(a.out)[b * a.H * c.dv + e] = from_f<T>(0.f);
   if (begin >= end) return;
 
-  Place get;
-  get.b = f.b;
-  get.request(a);
-  get.group = static_cast<int>((begin - f.before) / get.tiles);
-  get.tile = static_cast<int>((begin - f.before) % get.tiles);
-  get.enter(a, warp);
-  Place use = get;
-  unsigned char* slots = ring + warp * kStages * (KB + VB);
+  const int mine = warp < kStepWarps ? warp : lane;  // the warp that computes
+  Place use;
+  use.b = f.b;
+  use.request(a);
+  use.group = static_cast<int>((begin - f.before) / use.tiles);
+  use.tile = static_cast<int>((begin - f.before) % use.tiles);
+  use.enter(a, mine);
 
-  // ---- loads: `get` runs ahead of `use` ----
-  long long left = end - begin;  // places that are not loaded yet, `get` among them
-  bool seek = false;             // `get` has been passed
-  int loads = 0;                 // groups of this warp that were asked for
-  int id = -1;                   // page of `get`
-  // Moves `get` to the warp's next group and reads its page's number.
-  auto look = [&]() {
-    while (left > 0) {
-      if (seek) {
-        if (--left == 0) break;
-        get.next(a, warp, groups);
-      }
-      seek = true;
-      if (get.has(warp)) {
-        id = __ldg(c.table + get.b * c.width + get.page);
-        return;
-      }
-    }
-  };
-  bool alive = true;
-  auto load = [&]() {
-    if (left <= 0 || !alive) return;
-    const int at = loads % kStages;
-    uint64_t* bar = &full[warp][at];
-    const bool ok = id >= 0 && id < c.pages;
-    const int hk = get.group / a.row_tiles;
-    if (!ok) {
-      if (lane == 0) {
-        report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(get.b), a.err);
-        usable[warp][at] = 0;
-      }
-      if (lane < 3) bar_arrive(bar);
-    } else if (lane == 0) {
-      usable[warp][at] = 1;
-      bar_expect(bar, KB + VB);
-      const uint32_t to = smem_u32(slots + at * (KB + VB));
-      tma_page(to, &maps.k, get.row, id * c.heads + hk, bar);
-      tma_page(to + KB, &maps.v, get.row, id * c.heads + hk, bar);
-    } else if (lane < 3) {
-      const float* from = (lane == 1 ? c.ks : c.vs) + static_cast<long long>(id) * c.heads + hk;
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[warp][at][lane - 1])), "l"(from) : "memory");
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-    }
-    ++loads;
-    __syncwarp();
-    look();
-  };
-  look();
+  if (warp == kStepWarps) {
+    // ---- loads: lane w for warp w ----
+    if (lane >= kStepWarps) return;
+    unsigned char* slots = ring + mine * S * (KB + VB);
+    int at = 0, phase = 1;  // a first pass finds all slots empty
 #pragma unroll 1
-  for (int i = 0; i < kStages; ++i) load();
+    for (long long left = end - begin; left > 0; --left) {
+      if (use.has(mine)) {
+        const int id = __ldg(c.table + use.b * c.width + use.page), hk = use.group / a.row_tiles;
+        uint64_t* bar = &full[mine][at];
+        if (!bar_try(&empty[mine][at], phase) && !wait_slow(&empty[mine][at], phase, a.err)) return;
+        if (id < 0 || id >= c.pages) {
+          report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(use.b), a.err);
+          usable[mine][at] = 0;
+          bar_arrive(bar);
+          bar_arrive(bar);
+        } else {
+          const int page = id * c.heads + hk;
+          const uint32_t to = smem_u32(slots + at * (KB + VB));
+          usable[mine][at] = 1;
+          bar_expect(bar, KB + VB);
+          tma_page(to, &maps.k, use.row, page, bar);
+          tma_page(to + KB, &maps.v, use.row, page, bar);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[mine][at][0])), "l"(c.ks + page) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[mine][at][1])), "l"(c.vs + page) : "memory");
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        }
+        if (++at == S) at = 0, phase ^= 1;
+      }
+      if (left > 1) use.next(a, mine, groups);
+    }
+    return;
+  }
 
-  const float c2 = a.scale * 1.4426950408889634f;
-  int slot = 0, used = 0;
+  const float c2 = a.scale * kLog2e;
+  const unsigned char* slots = ring + warp * S * (KB + VB);
+  int slot = 0, stage = 0, phase = 0;
+  bool alive = true;
 #pragma unroll 1
   for (long long at = begin; at < end; ) {
     const int tile0 = use.tile, tile1 = static_cast<int>(min(static_cast<long long>(use.tiles), tile0 + (end - at)));
@@ -488,10 +492,10 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
 
     // ---- queries as operands: index 2 t4.. of product (u, w) is element
     // 16 (U t4 + u) + 4 w.. of the head
-    uint32_t q[TERMS][U * 4][4];
-    float qf[2];  // what a row's scores are in units of
+    uint32_t q[TERMS][U * 4][2 * R];
+    float qf[R];  // what a row's scores are in units of
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < R; ++r) {
       const int row = g + 8 * r;
       float x[U * 16], top = 0.f;
 #pragma unroll
@@ -510,33 +514,36 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
         for (int half = 0; half < 2; ++half) {
           const float y0 = x[u * 4 + half * 2] * up, y1 = x[u * 4 + half * 2 + 1] * up;
           const uint32_t hi = hf2(y0, y1);
-          q[0][u][half * 2 + r] = hi;
+          q[0][u][half * R + r] = hi;
           if (FINE) {
             const float2 z = float2_of(hi);
-            q[TERMS - 1][u][half * 2 + r] = hf2(y0 - z.x, y1 - z.y);
+            q[TERMS - 1][u][half * R + r] = hf2(y0 - z.x, y1 - z.y);
           }
         }
     }
 
-    float o[NV][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[NV][2 * R], m[R], l[R];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 2 * R; ++e) o[i][e] = 0.f;
 
 #pragma unroll 1
     for (int tile = tile0; tile < tile1; ++tile) {
-      const int tokens = min(kGroup, use.len - (tile * kStepTile + warp * kGroup));
-      if (tokens <= 0) continue;
-      const int at_stage = used % kStages;
-      if (alive) alive = wait_group(&full[warp][at_stage], (used / kStages) & 1, a.err);
-      ++used;
-      const unsigned char* ks = slots + at_stage * (KB + VB);
+      const int tokens = use.len - (tile * kStepTile + warp * kGroup);  // sixteen of them at most are the warp's
+      if (tokens <= 0) break;
+      if (alive) alive = wait_group(&full[warp][stage], phase, a.err);
+      const unsigned char* ks = slots + stage * (KB + VB);
       const unsigned char* vs = ks + KB;
-      if (alive && usable[warp][at_stage]) {
-        const float kscale = scales[warp][at_stage][0], vscale = scales[warp][at_stage][1];
-        float s[2][4];
+      if (alive && usable[warp][stage]) {
+        const float kscale = scales[warp][stage][0], vscale = scales[warp][stage][1];
+        float s[2][2 * R];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 2 * R; ++e) s[i][e] = 0.f;
           const int row = 8 * i + g;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -547,52 +554,60 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
             for (int e = 0; e < 4; ++e) {
               const uint32_t b0 = half2_of(static_cast<uint16_t>(word[e])), b1 = half2_of(static_cast<uint16_t>(word[e] >> 16));
 #pragma unroll
-              for (int z = 0; z < TERMS; ++z) mma(s[i], q[TERMS - 1 - z][u * 4 + e], b0, b1);
+              for (int z = 0; z < TERMS; ++z) mma<R>(s[i], q[TERMS - 1 - z][u * 4 + e], b0, b1);
             }
           }
         }
         // in units of log 2; a page's value scale is added to the exponent
         const float lv = static_cast<float>(static_cast<int>(__float_as_uint(vscale) >> 23) - 127);
-        float top[2] = {-INFINITY, -INFINITY};
+        float top[R];
+        bool past = false;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int r = 0; r < R; ++r) {
+          const float unit = qf[r] * kscale;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool in = 8 * i + 2 * t4 + (e & 1) < tokens;
-            s[i][e] = in ? s[i][e] * (qf[e >> 1] * kscale) : -INFINITY;
-            top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
-          }
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) top[r] = quad_max(top[r]) + lv;
+            for (int e = 0; e < 2; ++e) {
+              float& x = s[i][2 * r + e];
+              x *= unit;
+              if (tokens < kGroup && 8 * i + 2 * t4 + e >= tokens) x = -INFINITY;
+            }
+          top[r] = quad_max(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]))) + lv;
+          past |= top[r] > m[r] + 8.f;
+        }
         // the reference moves when weights would pass 2^8
-        if (__any_sync(kFull, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
-          float fall[2];
+        if (__any_sync(kFull, past)) {
+          float fall[R];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
+          for (int r = 0; r < R; ++r) {
             const float next = fmaxf(m[r], top[r]);
             fall[r] = next == -INFINITY ? 1.f : ex2(m[r] - next);
             m[r] = next;
             l[r] *= fall[r];
           }
 #pragma unroll
-          for (int i = 0; i < NV; ++i) o[i][0] *= fall[0], o[i][1] *= fall[0], o[i][2] *= fall[1], o[i][3] *= fall[1];
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 2 * R; ++e) o[i][e] *= fall[e >> 1];
         }
-        uint32_t pa[TERMS][4];
+        uint32_t pa[TERMS][2 * R];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int r = 0; r < R; ++r) {
+          const float ref = m[r] == -INFINITY ? 0.f : m[r];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float ref = m[r] == -INFINITY ? 0.f : m[r];
+          for (int i = 0; i < 2; ++i) {
             const float p0 = ex2(s[i][2 * r] - ref), p1 = ex2(s[i][2 * r + 1] - ref);
             l[r] += p0 + p1;
             const float w0 = p0 * vscale, w1 = p1 * vscale;
             const uint32_t hi = hf2(w0, w1);
-            pa[0][2 * i + r] = hi;
+            pa[0][R * i + r] = hi;
             if (FINE) {
               const float2 z = float2_of(hi);
-              pa[TERMS - 1][2 * i + r] = hf2(w0 - z.x, w1 - z.y);
+              pa[TERMS - 1][R * i + r] = hf2(w0 - z.x, w1 - z.y);
             }
           }
+        }
         uint32_t vr[4][NV / 4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -619,30 +634,29 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
             for (int k = 0; k < 2; ++k) {
               const uint32_t b0 = half2_of(static_cast<uint16_t>(k ? x >> 16 : x)), b1 = half2_of(static_cast<uint16_t>(k ? y >> 16 : y));
 #pragma unroll
-              for (int z = 0; z < TERMS; ++z) mma(o[e * 4 + half * 2 + k], pa[TERMS - 1 - z], b0, b1);
+              for (int z = 0; z < TERMS; ++z) mma<R>(o[e * 4 + half * 2 + k], pa[TERMS - 1 - z], b0, b1);
             }
           }
       }
       __syncwarp();  // the slot has been read
-      load();
+      if (lane == 0) bar_arrive(&empty[warp][stage]);
+      if (++stage == S) stage = 0, phase ^= 1;
     }
 
     // ---- the warps' parts of the piece meet: two and two, then both ----
 #pragma unroll
-    for (int r = 0; r < 2; ++r) l[r] = quad_sum(l[r]);
+    for (int r = 0; r < R; ++r) l[r] = quad_sum(l[r]);
     if (t4 == 0)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
-    __syncthreads();
-    float fall[2];
+      for (int r = 0; r < R; ++r) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
+    meet();
+    float fall[R];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < R; ++r) {
       const int row = g + 8 * r;
       const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
       fall[r] = ex2(m[r] - (top == -INFINITY ? 0.f : top));
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) o[i][0] *= fall[0], o[i][1] *= fall[0], o[i][2] *= fall[1], o[i][3] *= fall[1];
     // column n of product i is element NV n + i of the value; lane t4 has
     // columns 2 t4 and 2 t4 + 1
 #pragma unroll 1
@@ -651,16 +665,17 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 2 * R; ++e) {
             float* to = &s_o[warp & 1][g + 8 * (e >> 1)][(2 * t4 + (e & 1)) * NV + i];
-            *to = turn == 0 ? o[i][e] : *to + o[i][e];
+            const float x = o[i][e] * fall[e >> 1];
+            *to = turn == 0 ? x : *to + x;
           }
       }
-      __syncthreads();
+      meet();
     }
     const bool whole = tile0 == 0 && tile1 == use.tiles;
     float* part = a.part + (static_cast<long long>(blockIdx.x) * 2 + slot) * slot_floats(c.dv);
-    for (int e = threadIdx.x; e < rows * c.dv; e += kStepThreads) {
+    for (int e = threadIdx.x; e < rows * c.dv; e += kStepWarps * 32) {
       const int row = e / c.dv, d = e % c.dv;
       const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
       const float ref = top == -INFINITY ? 0.f : top;
@@ -675,7 +690,7 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
         part[32 + row * c.dv + d] = x;
       }
     }
-    __syncthreads();  // read before the next piece's are written
+    meet();  // read before the next piece's are written
     slot = 1;  // pieces after the first begin with their request's first tile
     at += tile1 - tile0;
     use.tile = tile1 - 1;
@@ -763,22 +778,26 @@ static bool map_pages(CUtensorMap* m, const uint8_t* pool, const Cache& c, int d
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int U, int NV>
+template <typename T, int U, int NV, int R>
 static int launch_step(const StepArgs& a, const StepMaps& m, int ctas, cudaStream_t s) {
   static std::atomic<unsigned long long> done{};
-  constexpr size_t bytes = static_cast<size_t>(kStepWarps) * kStages * kGroup * (64 * U + 8 * NV);
-  const int rc = mscan::allow_smem(step_kernel<T, U, NV>, bytes, done);
+  constexpr size_t bytes = static_cast<size_t>(kStepWarps) * stages(R) * kGroup * (64 * U + 8 * NV);
+  const int rc = mscan::allow_smem(step_kernel<T, U, NV, R>, bytes, done);
   if (rc != ASCAN_OK) return rc;
-  step_kernel<T, U, NV><<<ctas, kStepThreads, bytes, s>>>(a, m);
+  step_kernel<T, U, NV, R><<<ctas, kStepThreads, bytes, s>>>(a, m);
   return launch_status();
+}
+
+template <typename T, int R>
+static int pick_step(const StepArgs& a, const StepMaps& m, int ctas, cudaStream_t s) {
+  if (a.c.dk > 64) return a.c.dv > 64 ? launch_step<T, 2, 16, R>(a, m, ctas, s) : launch_step<T, 2, 8, R>(a, m, ctas, s);
+  return a.c.dv > 64 ? launch_step<T, 1, 16, R>(a, m, ctas, s) : launch_step<T, 1, 8, R>(a, m, ctas, s);
 }
 
 template <typename T>
 static int step(const StepArgs& a, const StepMaps& m, cudaStream_t s) {
   const int ctas = 148 * (sizeof(T) == 4 ? 2 : kCtasPerSm);
-  const bool wide_k = a.c.dk > 64, wide_v = a.c.dv > 64;
-  const int rc = wide_k ? (wide_v ? launch_step<T, 2, 16>(a, m, ctas, s) : launch_step<T, 2, 8>(a, m, ctas, s))
-                        : (wide_v ? launch_step<T, 1, 16>(a, m, ctas, s) : launch_step<T, 1, 8>(a, m, ctas, s));
+  const int rc = a.share <= 8 ? pick_step<T, 1>(a, m, ctas, s) : pick_step<T, 2>(a, m, ctas, s);
   if (rc != ASCAN_OK) return rc;
   // a row of a few requests lies in many CTAs' parts, one of many in one or two
   const dim3 grid(a.H, static_cast<unsigned>(a.c.B));
