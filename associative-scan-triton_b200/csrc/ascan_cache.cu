@@ -252,30 +252,32 @@ __device__ __forceinline__ int length_of(const StepArgs& a, long long b) {
 }
 __device__ __forceinline__ int tiles_of_length(int n) { return (n + kStepTile - 1) / kStepTile; }
 
-// d += A B with R * 8 rows of A; of eight, the other half of the product is
-// zeros and takes no registers.
-template <int R>
-__device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  if (R == 2) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2 * R - 2]), "+f"(d[2 * R - 1])
-                 : "r"(a[0]), "r"(a[R - 1]), "r"(a[R]), "r"(a[2 * R - 1]), "r"(b0), "r"(b1));
-  } else {
-    asm volatile(
-        "{\n .reg .f32 x, y;\n"
-        " mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, x, y}, {%2, %6, %3, %6}, {%4, %5}, {%0, %1, %7, %7};\n}\n"
-        : "+f"(d[0]), "+f"(d[1])
-        : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0), "f"(0.f));
-  }
+__device__ __forceinline__ void mma(float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// An 8 x 8 matrix of 16-bit elements, a row for four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ float2 float2_of(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(kFull, x, 1));
   return fmaxf(x, __shfl_xor_sync(kFull, x, 2));
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(kFull, x, 1);
-  return x + __shfl_xor_sync(kFull, x, 2);
+// Over the lanes that differ in lane / 4.
+__device__ __forceinline__ float column_max(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x = fmaxf(x, __shfl_xor_sync(kFull, x, o));
+  return x;
+}
+__device__ __forceinline__ float column_sum(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x += __shfl_xor_sync(kFull, x, o);
+  return x;
 }
 
 // Tiles of the requests: their total, and the request that tile `begin` of the
@@ -384,11 +386,18 @@ __host__ __device__ constexpr int stages(int r) { return r == 1 ? 4 : 3; }
 // The tiles of all requests, key heads and row tiles are one list; a CTA takes
 // an equal run of it, wherever requests begin and end, and walks it piece by
 // piece (a piece: what it has of one request, head and row tile).  Each of four
-// warps takes sixteen tokens of a tile with m16n8k16 products of float16: e4m3
-// values are exact there, queries are brought to at most 2^15 by a power of
-// two per row, and weights lie between 0 and 2^8, so both keep 11 bits or more
-// (22 where queries are float32: the rest of each goes through a second
-// product).
+// warps takes sixteen tokens of a tile with m16n8k16 products of float16, the
+// tokens and the values' elements along the 16 and queries along the 8, which
+// a key head often has no more of:
+//
+//   S^T = K q^T [tokens, queries]     O^T += V^T P^T [elements, queries]
+//
+// e4m3 values are exact in float16, queries are brought to at most 2^15 by a
+// power of two each, and weights lie between 0 and 2^8, so both keep 11 bits or
+// more (22 where queries are float32: the rest of each goes through a second
+// product).  A lane's column of S^T and of O^T is the same query, and the
+// softmax's reference moves only when a score exceeds it by 2^8, so nothing is
+// exchanged between lanes but P, for its transposition.
 //
 // Memory bounds it, so each warp has several groups of sixteen tokens in
 // flight, over the ends of pieces too: 2 KB of keys and of values, each one TMA
@@ -400,8 +409,8 @@ __host__ __device__ constexpr int stages(int r) { return r == 1 ? 4 : 3; }
 // both operands agree, and the choice here together with the copies' swizzle
 // meets no bank twice.
 //
-// U: 64-element parts of a key.  NV: bytes of a value row per lane.  R: query
-// rows in eights (one if no key head has more than eight queries).
+// U: 64-element parts of a key.  NV: bytes of a value row per lane.  R: queries
+// in eights (one if no key head has more than eight).
 template <typename T, int U, int NV, int R>
 __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
     step_kernel(const __grid_constant__ StepArgs a, const __grid_constant__ StepMaps maps) {
@@ -491,9 +500,10 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
     const int rows = min(16, (hk + 1) * a.share - h0);
 
     // ---- queries as operands: index 2 t4.. of product (u, w) is element
-    // 16 (U t4 + u) + 4 w.. of the head
-    uint32_t q[TERMS][U * 4][2 * R];
-    float qf[R];  // what a row's scores are in units of
+    // 16 (U t4 + u) + 4 w.. of the head; lane / 4 is the query here, and of
+    // products its columns are queries 2 t4 and 2 t4 + 1
+    uint32_t q[TERMS][R][U * 4][2];
+    float qf[R][2];  // what a query's scores are in units of
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = g + 8 * r;
@@ -506,29 +516,31 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
       }
       top = quad_max(top);
       const int e2 = max(-100, static_cast<int>(__float_as_uint(top) >> 23) - 127);
-      const float up = pow2(14 - e2);
-      qf[r] = pow2(e2 - 14) * c2;
+      const float up = pow2(14 - e2), unit = pow2(e2 - 14) * c2;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qf[r][e] = __shfl_sync(kFull, unit, (2 * t4 + e) * 4);
 #pragma unroll
       for (int u = 0; u < U * 4; ++u)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const float y0 = x[u * 4 + half * 2] * up, y1 = x[u * 4 + half * 2 + 1] * up;
           const uint32_t hi = hf2(y0, y1);
-          q[0][u][half * R + r] = hi;
+          q[0][r][u][half] = hi;
           if (FINE) {
             const float2 z = float2_of(hi);
-            q[TERMS - 1][u][half * R + r] = hf2(y0 - z.x, y1 - z.y);
+            q[TERMS - 1][r][u][half] = hf2(y0 - z.x, y1 - z.y);
           }
         }
     }
 
-    float o[NV][2 * R], m[R], l[R];
+    float o[R][NV / 2][4], m[R][2], l[R][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    for (int r = 0; r < R; ++r) {
+      m[r][0] = m[r][1] = -INFINITY;
+      l[r][0] = l[r][1] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < 2 * R; ++e) o[i][e] = 0.f;
+      for (int i = 0; i < NV / 2; ++i) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
+    }
 
 #pragma unroll 1
     for (int tile = tile0; tile < tile1; ++tile) {
@@ -539,72 +551,70 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
       const unsigned char* vs = ks + KB;
       if (alive && usable[warp][stage]) {
         const float kscale = scales[warp][stage][0], vscale = scales[warp][stage][1];
-        float s[2][2 * R];
+        // element e of s: token g + 8 (e / 2), query 2 t4 + e % 2
+        float s[R][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 2 * R; ++e) s[i][e] = 0.f;
-          const int row = 8 * i + g;
+        for (int u = 0; u < U; ++u) {
+          uint32_t word[2][4];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
+          for (int i = 0; i < 2; ++i) {
+            const int row = 8 * i + g;
             const uint4 x = *reinterpret_cast<const uint4*>(
                 ks + row * 64 * U + (U == 2 ? ((2 * t4 + u) ^ (row & 7)) << 4 : (t4 ^ ((row >> 1) & 3)) << 4));
-            const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+            word[i][0] = x.x, word[i][1] = x.y, word[i][2] = x.z, word[i][3] = x.w;
+          }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t b0 = half2_of(static_cast<uint16_t>(word[e])), b1 = half2_of(static_cast<uint16_t>(word[e] >> 16));
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t ka[4] = {half2_of(static_cast<uint16_t>(word[0][e])), half2_of(static_cast<uint16_t>(word[1][e])),
+                                    half2_of(static_cast<uint16_t>(word[0][e] >> 16)), half2_of(static_cast<uint16_t>(word[1][e] >> 16))};
 #pragma unroll
-              for (int z = 0; z < TERMS; ++z) mma<R>(s[i], q[TERMS - 1 - z][u * 4 + e], b0, b1);
-            }
+            for (int z = 0; z < TERMS; ++z)
+#pragma unroll
+              for (int r = 0; r < R; ++r) mma(s[r], ka, q[TERMS - 1 - z][r][u * 4 + e]);
           }
         }
         // in units of log 2; a page's value scale is added to the exponent
         const float lv = static_cast<float>(static_cast<int>(__float_as_uint(vscale) >> 23) - 127);
-        float top[R];
         bool past = false;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float unit = qf[r] * kscale;
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float& x = s[i][2 * r + e];
-              x *= unit;
-              if (tokens < kGroup && 8 * i + 2 * t4 + e >= tokens) x = -INFINITY;
-            }
-          top[r] = quad_max(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]))) + lv;
-          past |= top[r] > m[r] + 8.f;
-        }
+          for (int e = 0; e < 4; ++e) {
+            s[r][e] *= qf[r][e & 1] * kscale;
+            if (g + 8 * (e >> 1) >= tokens) s[r][e] = -INFINITY;
+            past |= s[r][e] + lv > m[r][e & 1] + 8.f;
+          }
         // the reference moves when weights would pass 2^8
         if (__any_sync(kFull, past)) {
-          float fall[R];
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float next = fmaxf(m[r], top[r]);
-            fall[r] = next == -INFINITY ? 1.f : ex2(m[r] - next);
-            m[r] = next;
-            l[r] *= fall[r];
-          }
+          for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
+            for (int e = 0; e < 2; ++e) {
+              const float next = fmaxf(m[r][e], column_max(fmaxf(s[r][e], s[r][e + 2])) + lv);
+              const float fall = next == -INFINITY ? 1.f : ex2(m[r][e] - next);
+              m[r][e] = next;
+              l[r][e] *= fall;
 #pragma unroll
-            for (int e = 0; e < 2 * R; ++e) o[i][e] *= fall[e >> 1];
+              for (int i = 0; i < NV / 2; ++i) o[r][i][e] *= fall, o[r][i][e + 2] *= fall;
+            }
         }
-        uint32_t pa[TERMS][2 * R];
+        uint32_t pb[TERMS][R][2];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float ref = m[r] == -INFINITY ? 0.f : m[r];
+          const float ref0 = m[r][0] == -INFINITY ? 0.f : m[r][0], ref1 = m[r][1] == -INFINITY ? 0.f : m[r][1];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p0 = ex2(s[i][2 * r] - ref), p1 = ex2(s[i][2 * r + 1] - ref);
-            l[r] += p0 + p1;
+            const float p0 = ex2(s[r][2 * i] - ref0), p1 = ex2(s[r][2 * i + 1] - ref1);
+            l[r][0] += p0;
+            l[r][1] += p1;
             const float w0 = p0 * vscale, w1 = p1 * vscale;
             const uint32_t hi = hf2(w0, w1);
-            pa[0][R * i + r] = hi;
+            pb[0][r][i] = transpose8(hi);
             if (FINE) {
               const float2 z = float2_of(hi);
-              pa[TERMS - 1][R * i + r] = hf2(w0 - z.x, w1 - z.y);
+              pb[TERMS - 1][r][i] = transpose8(hf2(w0 - z.x, w1 - z.y));
             }
           }
         }
@@ -619,10 +629,15 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
             const uint2 x = *reinterpret_cast<const uint2*>(vs + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
             vr[j][0] = x.x, vr[j][1] = x.y;
           }
-          if (tokens < kGroup && row >= tokens)  // what lies behind the last token may be anything
-#pragma unroll
-            for (int e = 0; e < NV / 4; ++e) vr[j][e] = 0;
         }
+        if (tokens < kGroup) {  // what lies behind the last token may be anything
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((j >> 1) * 8 + 2 * t4 + (j & 1) >= tokens)
+#pragma unroll
+              for (int e = 0; e < NV / 4; ++e) vr[j][e] = 0;
+        }
+        // rows g and g + 8 of product i are elements NV g + 2 i and the next
 #pragma unroll
         for (int e = 0; e < NV / 4; ++e)
 #pragma unroll
@@ -630,12 +645,12 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
             // byte pairs of two tokens, two elements at once
             const uint32_t x = __byte_perm(vr[0][e], vr[1][e], half ? 0x7362 : 0x5140);
             const uint32_t y = __byte_perm(vr[2][e], vr[3][e], half ? 0x7362 : 0x5140);
+            const uint32_t va[4] = {half2_of(static_cast<uint16_t>(x)), half2_of(static_cast<uint16_t>(x >> 16)),
+                                    half2_of(static_cast<uint16_t>(y)), half2_of(static_cast<uint16_t>(y >> 16))};
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t b0 = half2_of(static_cast<uint16_t>(k ? x >> 16 : x)), b1 = half2_of(static_cast<uint16_t>(k ? y >> 16 : y));
+            for (int z = 0; z < TERMS; ++z)
 #pragma unroll
-              for (int z = 0; z < TERMS; ++z) mma<R>(o[e * 4 + half * 2 + k], pa[TERMS - 1 - z], b0, b1);
-            }
+              for (int r = 0; r < R; ++r) mma(o[r][e * 2 + half], va, pb[TERMS - 1 - z][r]);
           }
       }
       __syncwarp();  // the slot has been read
@@ -645,31 +660,36 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
 
     // ---- the warps' parts of the piece meet: two and two, then both ----
 #pragma unroll
-    for (int r = 0; r < R; ++r) l[r] = quad_sum(l[r]);
-    if (t4 == 0)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int r = 0; r < R; ++r) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
+      for (int e = 0; e < 2; ++e) {
+        l[r][e] = column_sum(l[r][e]);
+        if (g == 0) s_m[warp][2 * t4 + e + 8 * r] = m[r][e], s_l[warp][2 * t4 + e + 8 * r] = l[r][e];
+      }
     meet();
-    float fall[R];
+    float fall[R][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = g + 8 * r;
-      const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-      fall[r] = ex2(m[r] - (top == -INFINITY ? 0.f : top));
-    }
-    // column n of product i is element NV n + i of the value; lane t4 has
-    // columns 2 t4 and 2 t4 + 1
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 2 * t4 + e + 8 * r;
+        const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+        fall[r][e] = ex2(m[r][e] - (top == -INFINITY ? 0.f : top));
+      }
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
       if (warp >> 1 == 1 - turn) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int e = 0; e < 2 * R; ++e) {
-            float* to = &s_o[warp & 1][g + 8 * (e >> 1)][(2 * t4 + (e & 1)) * NV + i];
-            const float x = o[i][e] * fall[e >> 1];
-            *to = turn == 0 ? x : *to + x;
-          }
+          for (int i = 0; i < NV / 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float2* to = reinterpret_cast<float2*>(&s_o[warp & 1][2 * t4 + e + 8 * r][g * NV + 2 * i]);
+              float2 x = make_float2(o[r][i][e] * fall[r][e], o[r][i][e + 2] * fall[r][e]);
+              if (turn == 1) x.x += to->x, x.y += to->y;
+              *to = x;
+            }
       }
       meet();
     }
