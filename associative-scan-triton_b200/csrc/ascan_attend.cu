@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
   float *qs = plain_smem_base, *ks = qs + kR * (D + 4), *vs = ks + kR * (D + 4), *ps = vs + kR * (D + 4);
   const int h = blockIdx.y, hk = h / p.share, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   if (blockIdx.x == 0 && h == 0) check_cu(p);
-  zero_outside<T>(p, p.out, h, p.H, p.dv, blockIdx.x, kR);
+  zero_outside<T>(p, p.out, h, p.H, p.dv, blockIdx.x, kR, threadIdx.x, blockDim.x);
   const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kR);  // long rows first
   if (t.first < 0) return;
   const int len = static_cast<int>(min(static_cast<long long>(kR), t.len - t.first));
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kPlainThreads) dq_kernel(const __grid_constant
   constexpr int S = kR * (D + 4);
   float *qs = plain_smem_base, *gs = qs + S, *ks = gs + S, *vs = ks + S, *ps = vs + S;
   const int h = blockIdx.y, hk = h / p.share, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kR);
+  zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kR, threadIdx.x, blockDim.x);
   const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kR);
   if (t.first < 0) return;
   const int len = static_cast<int>(min(static_cast<long long>(kR), t.len - t.first));
@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(kPlainThreads) dkdv_kernel(const __grid_consta
   constexpr int S = kR * (D + 4);
   float *ks = plain_smem_base, *vs = ks + S, *qs = vs + S, *gs = qs + S, *ps = gs + S, *ds = ps + kR * kPs;
   const int hk = blockIdx.y, heads = p.H / p.share, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kR);
-  zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kR);
+  zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kR, threadIdx.x, blockDim.x);
+  zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kR, threadIdx.x, blockDim.x);
   const Tile t = find_tile(p, blockIdx.x, kR);  // a sequence's first keys have the most queries
   if (t.first < 0) return;
   const int len = static_cast<int>(min(static_cast<long long>(kR), t.len - t.first));

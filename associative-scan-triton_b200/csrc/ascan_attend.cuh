@@ -89,13 +89,14 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, long long x, int row
 
 // Rows of no sequence come out zero; slab x of the packed axis is the x-th CTA's.
 template <typename T>
-__device__ __forceinline__ void zero_outside(const Problem& p, void* to, int head, int heads, int dim, long long x, int rows) {
+__device__ __forceinline__ void zero_outside(const Problem& p, void* to, int head, int heads, int dim, long long x, int rows,
+                                             int thread, int threads) {
   const long long t0 = x * rows, t1 = min(t0 + rows, p.BL);
   const long long c0 = cu_at(p, 0), c1 = cu_at(p, p.N);
   if (t0 >= c0 && t1 <= c1) return;
   for (long long t = t0; t < t1; ++t)
     if (t < c0 || t >= c1)
-      for (int d = threadIdx.x; d < dim; d += blockDim.x) static_cast<T*>(to)[(t * heads + head) * dim + d] = from_f<T>(0.f);
+      for (int d = thread; d < dim; d += threads) static_cast<T*>(to)[(t * heads + head) * dim + d] = from_f<T>(0.f);
 }
 
 // The tensor-core kernels (ascan_attend_tc.cu).

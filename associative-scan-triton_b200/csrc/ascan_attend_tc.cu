@@ -118,8 +118,9 @@ __device__ __forceinline__ uint32_t tile_bytes(int dim) { return dim > 64 ? 2 * 
 
 // A B^T over `dim` columns of two tiles in shared memory.
 __device__ __forceinline__ void scores(uint32_t to, uint64_t a, uint64_t b, uint32_t id, int dim) {
-#pragma unroll 1
-  for (int k = 0; k * 16 < dim; ++k) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (k * 16 >= dim) break;
     const uint32_t o = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
     mma_smem(to, a + o, b + o, id, k > 0);
   }
@@ -150,6 +151,26 @@ __device__ __forceinline__ uint64_t pair_of(const uint32_t* x) { return pair(__u
 __device__ __forceinline__ uint64_t ex2_2(uint64_t x) {
   const float2 f = unpair(x);
   return pair(ex2(f.x), ex2(f.y));
+}
+// 2^x of a pair by a polynomial of degree 4 on [-1/2, 1/2] (fitted to the
+// smallest relative error, 2.6e-6) and the exponent's bits; below 2^-126 what is
+// left is as small, and NaN comes out infinite, which makes a row NaN as well.
+// The special function unit has four lanes for the
+// scheduler's thirty-two.
+__device__ __forceinline__ uint64_t poly_ex2_2(uint64_t x) {
+  float2 f = unpair(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(f.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(f.y) : "f"(-126.f));
+  const uint64_t y = pair(f.x, f.y), magic = pair(12582912.f, 12582912.f);
+  const uint64_t n = add2(y, magic);  // the nearest whole number, in the low bits
+  const uint64_t r = fma2(add2(n, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), y);
+  uint64_t q = fma2(pair(0.009570100344717503f, 0.009570100344717503f), r, pair(0.05591785907745361f, 0.05591785907745361f));
+  q = fma2(q, r, pair(0.240247443318367f, 0.240247443318367f));
+  q = fma2(q, r, pair(0.6931217908859253f, 0.6931217908859253f));
+  q = fma2(q, r, pair(0.9999992847442627f, 0.9999992847442627f));
+  const float2 a = unpair(n), b = unpair(q);
+  return pair(__uint_as_float((__float_as_uint(a.x) << 23) + __float_as_uint(b.x)),
+              __uint_as_float((__float_as_uint(a.y) << 23) + __float_as_uint(b.y)));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
@@ -231,22 +252,26 @@ __device__ __forceinline__ bool misplaced(const unsigned char* smem, uint32_t* e
   return true;
 }
 
-// All 512 columns of tensor memory, by warp 9; the barriers are ready behind it.
-__device__ __forceinline__ uint32_t open_tmem(Common* t) {
-  if (threadIdx.x >> 5 == 9) {
+// A value that all lanes have: behind a shuffle the compiler knows it, and keeps
+// what a product is issued with in uniform registers.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFull, x, 0); }
+
+// All 512 columns of tensor memory, by one warp; the barriers are ready behind it.
+__device__ __forceinline__ uint32_t open_tmem(Common* t, int warp = 9) {
+  if (threadIdx.x >> 5 == warp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&t->tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     fence_before();
   }
   __syncthreads();
   fence_after();
-  return t->tmem;
+  return uniform(t->tmem);
 }
-__device__ __forceinline__ void close_tmem(uint32_t tm) {
+__device__ __forceinline__ void close_tmem(uint32_t tm, int warp = 9) {
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (threadIdx.x >> 5 == 9) {
+  if (threadIdx.x >> 5 == warp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
   }
@@ -256,239 +281,429 @@ __device__ __forceinline__ void bars_done() {
   fence_async();
 }
 
-__device__ __forceinline__ void check_cu(const Problem& p) {
-  if (p.cu64) validate_cu(static_cast<const int64_t*>(p.cu), p.N, p.BL, p.err);
-  else validate_cu(static_cast<const int32_t*>(p.cu), p.N, p.BL, p.err);
+// cu_seqlens as the scans check it, by `threads` threads.
+__device__ __forceinline__ void check_cu(const Problem& p, int thread, int threads) {
+  uint32_t bits = 0;
+  auto at = [&](long long i) {
+    return p.cu64 ? static_cast<const long long*>(p.cu)[i] : static_cast<long long>(static_cast<const int*>(p.cu)[i]);
+  };
+  for (long long i = thread; i <= p.N; i += threads) {
+    const long long v = at(i);
+    if (v < 0 || v > p.BL || (i < p.N && at(i + 1) < v)) bits |= ASCAN_DEV_ERR_CU_ORDER;
+    if (i == p.N && v != p.BL) bits |= ASCAN_DEV_ERR_CU_END;
+  }
+  if (bits) report(bits, 0ull, p.err);
 }
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
 
+constexpr int kFwdSoftmax = 8, kFwdRoles = kFwdSoftmax + 2, kFwdThreads = kFwdRoles * 32;
+
+// Of eight pairs of scores so many take the polynomial.
+constexpr int kPoly = 3;
+
 struct ForwardTail {
   Common c;
-  uint64_t q_full, full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], clean[2], o_done[2];
-  uint32_t bad[2][4];  // tokens of the tiles' own blocks with values that are not finite
+  uint64_t q_full, q_empty, full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], o_done[2], next_full[2], next_empty[2];
+  alignas(16) uint32_t next[2][4];  // the scheduler's answers
+  uint32_t bad[4][2][4];  // by work item: tokens of the tiles' own blocks with values that are not finite
 };
 
-// TRAIN: a gradient will follow.
+// Takes over the work of a CTA that has not been launched yet: the answer, its
+// number or none, comes to `to`.
+__device__ __forceinline__ void ask_work(uint32_t* to, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(to)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int read_work(const uint32_t* from) {  // -1: none is left
+  uint32_t got, x;
+  asm volatile(
+      "{\n .reg .b128 r;\n .reg .pred p;\n .reg .b32 y, z, w;\n .reg .b64 lo, hi;\n"
+      " ld.shared.v2.b64 {lo, hi}, [%2];\n mov.b128 r, {lo, hi};\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n}\n"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_u32(from))
+      : "memory");
+  return got ? static_cast<int>(x) : -1;
+}
+
+// A place in the ring and the parity of its turn.
+struct Cursor {
+  int at = 0;
+  uint32_t turn = 0;
+  __device__ __forceinline__ void next(int ns) {
+    if (++at == ns) at = 0, turn ^= 1;
+  }
+};
+
+// A work item: two tiles of queries of one head; `key` blocks of keys of each.
+struct Item {
+  int start, token, left;  // the sequence's first token, the item's, and the sequence's from there on
+  int h, n_a, n_b, n;      // n 0: no tokens
+  int x;                   // its number without the head
+};
+__device__ __noinline__ Item find_item(const Problem& p, int work) {
+  Item i;
+  const int tiles = static_cast<int>(gridDim.x) / p.H;
+  i.x = tiles - 1 - work / p.H;  // long rows first, the heads of a tile together
+  i.h = work % p.H;
+  const Tile t = find_tile(p, i.x, 2 * kC);
+  const int own = static_cast<int>(t.first / kC);  // the first tile's own block of keys
+  i.start = static_cast<int>(t.start);
+  i.token = static_cast<int>(t.start + t.first);
+  i.left = static_cast<int>(t.len - t.first);
+  i.n_a = t.first < 0 ? 0 : own + 1;
+  i.n_b = t.first >= 0 && i.left > kC ? own + 2 : 0;
+  i.n = max(i.n_a, i.n_b);
+  return i;
+}
+
+// The next item's number, the same for every role; false when there is none.
+__device__ __forceinline__ bool next_work(const Ctl& ctl, ForwardTail& s, uint32_t count, int& work) {
+  const uint32_t u = count & 1;
+  if (!ctl.warp_wait(&s.next_full[u], (count >> 1) & 1)) return false;
+  work = read_work(s.next[u]);
+  warp_arrive(&s.next_empty[u]);
+  return work >= 0;
+}
+
+// What a row has added up: its exponentials, the same rounded as P, and the
+// reference that they are taken against.
+struct RowState {
+  uint64_t l[2], z[2];
+  float m;
+};
+
+// P of a block whose scores exceed the row's reference by more than 2^8 (the
+// first block is one), or that the diagonal crosses (columns up to `last`): the
+// maximum first, then O and the sums to the new reference (o32: O's columns in
+// blocks of 32).  Out of line, so that the loop that runs nearly always keeps
+// everything in registers: with 227 KB of shared memory in use a spilled one
+// costs more than it saves.
 template <typename T, bool TRAIN>
-__global__ void __launch_bounds__(kTcThreads, 1) tc_forward_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
+__device__ __noinline__ RowState move_reference(uint32_t ts, uint32_t to, int last, int o32, float c2, RowState r) {
+  float high = -INFINITY;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    uint32_t sc[32];
+    tmem_ld32(ts + 32 * i, sc);
+    wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (32 * i + e <= last) high = fmaxf(high, __uint_as_float(sc[e]));
+  }
+  const float next = (high - r.m) * c2 > 8.f ? high : r.m;
+  if (o32 > 0 && __any_sync(kFull, next != r.m)) {
+    const float f = next == -INFINITY ? 1.f : ex2((r.m - next) * c2);
+    const uint64_t f2 = pair(f, f);
+    r.l[0] = mul2(r.l[0], f2), r.l[1] = mul2(r.l[1], f2);
+    if (TRAIN) r.z[0] = mul2(r.z[0], f2), r.z[1] = mul2(r.z[1], f2);
+#pragma unroll 1
+    for (int i = 0; i < o32; ++i) {
+      uint32_t o[32];
+      tmem_ld32(to + 32 * i, o);
+      wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+      tmem_st32(to + 32 * i, o);
+    }
+  }
+  r.m = next;
+  const float ref = r.m == -INFINITY ? 0.f : -r.m * c2;  // a row of -inf so far
+  const uint64_t ref2 = pair(ref, ref), c22 = pair(c2, c2);
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    uint32_t sc[32], w[16];
+    tmem_ld32(ts + 32 * i, sc);
+    wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (32 * i + e > last) sc[e] = 0xff800000u;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t y = ex2_2(fma2(pair_of(sc + 2 * e), c22, ref2));
+      w[e] = pack2<T>(y);
+      r.l[e & 1] = add2(r.l[e & 1], y);
+      if (TRAIN) r.z[e & 1] = add2(r.z[e & 1], unpack2<T>(w[e]));
+    }
+    tmem_st16(ts + 16 * i, w);
+  }
+  return r;
+}
+
+// TRAIN: a gradient will follow.  A CTA works through items: its own, and then
+// those of CTAs that were not launched yet, so that loads and products of the
+// next item run while the rows of this one are finished.
+template <typename T, bool TRAIN>
+__global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  const int h = blockIdx.y, hk = h / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (blockIdx.x == 0 && h == 0) check_cu(p);
-  zero_outside<T>(p, p.out, h, p.H, p.dv, blockIdx.x, 2 * kC);
-  const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, 2 * kC);  // long rows first
-  if (t.first < 0 || misplaced(smem, p.err)) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (misplaced(smem, p.err)) return;
   const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk);
   unsigned char* ring = smem + 2 * q_bytes;
   ForwardTail& s = *reinterpret_cast<ForwardTail*>(ring + ns * slot);
   const Ctl ctl{&s.c, p.err};
-  const long long left = t.len - t.first;
-  const int own = static_cast<int>(t.first / kC);             // the first tile's own block of keys
-  const int n_a = own + 1, n_b = left > kC ? own + 2 : 0, n = max(n_a, n_b);
   if (tid == 0) {
     bar_init(&s.q_full, 1);
+    bar_init(&s.q_empty, 1);
     for (int i = 0; i < ns; ++i) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(&s.s_full[i], 1);
       bar_init(&s.p_ready[i], 4);
-      bar_init(&s.clean[i], 4);
       bar_init(&s.o_done[i], 1);
+      bar_init(&s.next_full[i], 1);
+      bar_init(&s.next_empty[i], kFwdRoles);
     }
     bar_init(&s.c.drain, 1);
     s.c.abort = 0;
     bars_done();
   }
-  if (tid < 8) s.bad[tid >> 2][tid & 3] = 0;
-  const uint32_t tm = open_tmem(&s.c);
-  // the ring's order: K0, then (K[j+1], V[j]) for every j
-  auto index_of_v = [&](int j) { return j < n - 1 ? 2 * j + 2 : 2 * n - 1; };
+  const uint32_t tm = open_tmem(&s.c, kFwdSoftmax + 1);
+  int work = blockIdx.x;
+  bool ok = true;
+  uint32_t base = 0;  // of the item's loads in the ring: K0, then (K[j+1], V[j]) for every j
 
-  if (warp < 8) {
-    const int x = warp >> 2, quad = warp & 3, row = quad * 32 + lane, mine = x ? n_b : n_a;
+  if (warp < kFwdSoftmax) {
+    const int x = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad) << 21, ts = tm + lanes + x * kC, to = tm + lanes + 256 + x * kC;
     const float c2 = p.scale * kLog2e;
     const uint64_t c22 = pair(c2, c2);
     const int n32 = (p.dv + 31) / 32;
-    float m = -INFINITY;
-    uint64_t l2[2] = {0, 0}, r2[2] = {0, 0};
-    bool ok = true;
-    for (int j = 0; j < mine; ++j) {
-      const bool diagonal = j == mine - 1;
-      if (diagonal) {  // its values may only come from this sequence, and only finite
-        const int v = index_of_v(j);
-        if (!(ok = ctl.warp_wait(&s.full[v % ns], (v / ns) & 1))) break;
-        if (clean_row<T>(ring + v % ns * slot, row, 0, p.dv > 64 ? 2 : 1, row < left - x * kC))
-          atomicOr(&s.bad[x][quad], 1u << lane);
-        fence_async();
-        warp_arrive(&s.clean[x]);
+    uint32_t sp = 0, op = 0;  // phases: scores seen, rows finished
+    for (uint32_t count = 0; ok; ++count) {
+      const Item it = find_item(p, work);
+      const int mine = x ? it.n_b : it.n_a, left = it.left - x * kC;  // of the sequence from this tile on
+      uint32_t* bad = &s.bad[count & 3][x][quad];
+      if (lane == 0) *bad = 0;
+      __syncwarp();
+      RowState r{{0, 0}, {0, 0}, -INFINITY};
+      for (int j = 0; j < mine; ++j, sp ^= 1) {
+        const bool diagonal = j == mine - 1;
+        if (diagonal) {  // its values may only come from this sequence, and only finite
+          const uint32_t v = base + (j < it.n - 1 ? 2 * j + 2 : 2 * it.n - 1);  // of the ring's loads
+          if (!(ok = ctl.warp_wait(&s.full[v % ns], (v / ns) & 1))) break;
+          if (clean_row<T>(ring + v % ns * slot, row, 0, p.dv > 64 ? 2 : 1, row < left)) atomicOr(bad, 1u << lane);
+          fence_async();
+        }
+        if (!(ok = ctl.warp_wait(&s.s_full[x], sp))) break;
+        fence_after();
+        // Nearly every block leaves the reference where it was: P is computed
+        // with it while the maximum is looked for, and again if it has to move.
+        uint32_t w[64];
+        bool again = true;
+        if (j > 0 && !diagonal) {
+          float high = -INFINITY;
+          uint64_t a[2] = {0, 0};
+          const uint64_t ref2 = pair(-r.m * c2, -r.m * c2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t sc[32];
+            tmem_ld32(ts + 32 * i, sc);
+            wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t z = fma2(pair_of(sc + 2 * e), c22, ref2);
+              const uint64_t y = (e & 7) >= 8 - kPoly ? poly_ex2_2(z) : ex2_2(z);
+              high = max3(high, __uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1]));
+              w[16 * i + e] = pack2<T>(y);
+              a[e & 1] = add2(a[e & 1], y);
+            }
+          }
+          again = __any_sync(kFull, !((high - r.m) * c2 <= 8.f));
+          if (!again) r.l[0] = add2(r.l[0], a[0]), r.l[1] = add2(r.l[1], a[1]);
+        }
+        if (again) {
+          r = move_reference<T, TRAIN>(ts, to, diagonal ? row : kC, j > 0 ? n32 : 0, c2, r);
+        } else {
+          if (TRAIN) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) r.z[e & 1] = add2(r.z[e & 1], unpack2<T>(w[e]));
+          }
+          tmem_st32(ts, w);
+          tmem_st32(ts + 32, w + 32);
+        }
+        wait_st();
+        fence_before();
+        warp_arrive(&s.p_ready[x]);
       }
-      if (!(ok = ctl.warp_wait(&s.s_full[x], j & 1))) break;
-      fence_after();
-      uint32_t sc[kC];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, sc + 32 * i);
-      wait_ld();
-      if (diagonal) {
-#pragma unroll
-        for (int i = 0; i < kC; ++i) sc[i] = i > row ? 0xff800000u : sc[i];
-      }
-      float top[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(sc[i]);
-#pragma unroll
-      for (int i = 4; i < kC; i += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          top[e] = i + 4 + e < kC ? max3(top[e], __uint_as_float(sc[i + e]), __uint_as_float(sc[i + 4 + e]))
-                                  : fmaxf(top[e], __uint_as_float(sc[i + e]));
-      const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (j == 0) {
-        m = high;
-      } else if (__any_sync(kFull, (high - m) * c2 > 8.f)) {
-        const float next = fmaxf(m, high), f = next == -INFINITY ? 1.f : ex2((m - next) * c2);
-        m = next;
-        const uint64_t f2 = pair(f, f);
-        l2[0] = mul2(l2[0], f2), l2[1] = mul2(l2[1], f2);
-        if (TRAIN) r2[0] = mul2(r2[0], f2), r2[1] = mul2(r2[1], f2);
+      if (!ok) break;
+      if (mine > 0) {
+        if (!(ok = ctl.warp_wait(&s.o_done[x], op))) break;
+        op ^= 1;
+        fence_after();
+        const float2 a = unpair(add2(r.l[0], r.l[1])), b2 = unpair(add2(r.z[0], r.z[1]));
+        const float l = a.x + a.y, inv = 1.f / (TRAIN ? b2.x + b2.y : l);
+        const long long token = static_cast<long long>(it.token) + x * kC + row;
+        if (TRAIN && row < left) p.lse[it.h * p.BL + token] = r.m * c2 + log2f(l);
+        bool any = false;
+        for (int i = 0; i < 4; ++i) any |= s.bad[count & 3][0][i] != 0 || (x == 1 && s.bad[count & 3][1][i] != 0);
+        T* out = static_cast<T*>(p.out) + (token * p.H + it.h) * p.dv;
+        T* rest = static_cast<T*>(p.rest) + (token * p.H + it.h) * p.dv;
 #pragma unroll 1
-        for (int i = 0; i < n32; ++i) {
+        for (int b = 0; b < n32; ++b) {
           uint32_t o[32];
-          tmem_ld32(to + 32 * i, o);
+          tmem_ld32(to + 32 * b, o);
           wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(to + 32 * i, o);
-        }
-      }
-      const float ref = m == -INFINITY ? 0.f : -m * c2;  // a row of -inf so far
-      const uint64_t ref2 = pair(ref, ref);
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+          if (any) {  // what was taken out of the values goes where the mask lets it
+            for (int y = 0; y <= x; ++y)
+              for (int i = 0; i < kC; ++i) {
+                if (!(s.bad[count & 3][y][i >> 5] >> (i & 31) & 1) || (y == x && i > row)) continue;
+                const T* v = static_cast<const T*>(p.v.p) + (static_cast<long long>(it.token) + y * kC + i) * p.v.st + it.h / p.share * p.v.sh;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[16];
+                for (int e = 0; e < 32; ++e)
+                  if (32 * b + e < p.dv) {
+                    const float q = to_f(v[32 * b + e]);
+                    if (!(fabsf(q) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + q);
+                  }
+              }
+          }
+          uint32_t u[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint64_t y = ex2_2(fma2(pair_of(sc + 32 * i + 2 * e), c22, ref2));
-          w[e] = pack2<T>(y);
-          l2[e & 1] = add2(l2[e & 1], y);
-          if (TRAIN) r2[e & 1] = add2(r2[e & 1], unpack2<T>(w[e]));
-        }
-        tmem_st16(ts + 16 * i, w);
-      }
-      wait_st();
-      fence_before();
-      warp_arrive(&s.p_ready[x]);
-    }
-    const bool live = ok && mine > 0 && ctl.warp_wait(&s.o_done[x], 0) && ctl.warp_wait(&s.clean[0], 0) &&
-                      (x == 0 || ctl.warp_wait(&s.clean[1], 0));
-    if (live) {
-      fence_after();
-      const float2 a = unpair(add2(l2[0], l2[1])), r = unpair(add2(r2[0], r2[1]));
-      const float l = a.x + a.y, inv = 1.f / (TRAIN ? r.x + r.y : l);
-      const int rows = static_cast<int>(min(32ll, left - x * kC - quad * 32));
-      const long long token = t.start + t.first + x * kC + quad * 32;
-      if (TRAIN && lane < rows) p.lse[h * p.BL + token + lane] = m * c2 + log2f(l);
-      const long long stride = static_cast<long long>(p.H) * p.dv * 2, first = (token * p.H + h) * p.dv * 2;
-      unsigned char* stage = smem + x * q_bytes + quad * 4096;
-      bool bad = false;
-      for (int i = 0; i < 4; ++i) bad |= s.bad[0][i] != 0 || (x == 1 && s.bad[1][i] != 0);
-      for (int b = 0; b * 64 < p.dv; ++b) {
-        uint32_t o[64];
-        tmem_ld32(to + 64 * b, o);
-        tmem_ld32(to + 64 * b + 32, o + 32);
-        wait_ld();
+          for (int e = 0; e < 16; ++e) u[e] = pack2<T>(pair_of(o + 2 * e));
+          if (row < left) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
-        if (bad) {  // what was taken out of the values goes where the mask lets it
-          for (int z = 0; z <= x; ++z)
-            for (int i = 0; i < kC; ++i) {
-              if (!(s.bad[z][i >> 5] >> (i & 31) & 1) || (z == x && i > row)) continue;
-              const T* v = static_cast<const T*>(p.v.p) + (t.start + t.first + z * kC + i) * p.v.st + hk * p.v.sh;
+            for (int e = 0; e < 4; ++e)
+              if (32 * b + 8 * e < p.dv)
+                *reinterpret_cast<uint4*>(out + 32 * b + 8 * e) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+          }
+          if (TRAIN) {
 #pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (64 * b + e < p.dv) {
-                  const float y = to_f(v[64 * b + e]);
-                  if (!(fabsf(y) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
-                }
+            for (int e = 0; e < 16; ++e) u[e] = pack2<T>(fma2(unpack2<T>(u[e]), pair(-1.f, -1.f), pair_of(o + 2 * e)));
+            if (row < left) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (32 * b + 8 * e < p.dv)
+                  *reinterpret_cast<uint4*>(rest + 32 * b + 8 * e) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
             }
-        }
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = pack2<T>(pair_of(o + 2 * e));
-        store_block(stage, w, static_cast<unsigned char*>(p.out) + first + b * 128, stride, rows, p.dv - 64 * b);
-        if (TRAIN) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = pack2<T>(fma2(unpack2<T>(w[e]), pair(-1.f, -1.f), pair_of(o + 2 * e)));
-          store_block(stage, w, static_cast<unsigned char*>(p.rest) + first + b * 128, stride, rows, p.dv - 64 * b);
+          }
         }
       }
+      base += 2 * it.n;
+      if (!next_work(ctl, s, count, work)) break;
     }
-  } else if (warp == 8) {
-    if (lane == 0) {
-      const int token = static_cast<int>(t.start);
-      bar_expect(&s.q_full, q_bytes * (n_b ? 2 : 1));
-      load_tile(smem, &maps.q, p.dk, h, t.start + t.first, &s.q_full);
-      if (n_b) load_tile(smem + q_bytes, &maps.q, p.dk, h, t.start + t.first + kC, &s.q_full);
-      int i = 0;
-      for (; i < 2 * n; ++i) {
-        const bool is_v = i > 0 && (i % 2 == 0 || i == 2 * n - 1);
-        const int j = is_v ? (i == 2 * n - 1 ? n - 1 : i / 2 - 1) : (i + 1) / 2, at = i % ns;
-        if (i >= ns && !ctl.wait(&s.empty[at], (i / ns - 1) & 1)) break;
-        bar_expect(&s.full[at], tile_bytes(is_v ? p.dv : p.dk));
-        load_tile(ring + at * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, token + static_cast<long long>(j) * kC, &s.full[at]);
+  } else if (warp == kFwdSoftmax) {
+    uint32_t q_loads = 0, loads = 0;
+    Cursor to;
+    for (uint32_t count = 0; ok; ++count) {
+      const uint32_t u = count & 1;
+      if (lane == 0) {  // the next item's number comes while this one is loaded
+        if (count > 1) ok = ctl.wait(&s.next_empty[u], ((count >> 1) - 1) & 1);
+        if (ok) {
+          bar_expect(&s.next_full[u], 16);
+          ask_work(s.next[u], &s.next_full[u]);
+        }
       }
-      if (i < 2 * n) {
-        ctl.land(&s.q_full, 0);
-        for (int e = max(0, i - ns); e < i; ++e) ctl.land(&s.full[e % ns], (e / ns) & 1);
+      ok = __shfl_sync(kFull, ok, 0);
+      if (!ok) break;
+      const Item it = find_item(p, work);
+      if (it.x == 0 && it.h == 0) check_cu(p, lane, 32);
+      zero_outside<T>(p, p.out, it.h, p.H, p.dv, it.x, 2 * kC, lane, 32);
+      if (it.n > 0 && lane == 0) {
+        if (q_loads > 0) ok = ctl.wait(&s.q_empty, (q_loads - 1) & 1);
+        if (ok) {
+          bar_expect(&s.q_full, q_bytes * (it.n_b ? 2 : 1));
+          load_tile(smem, &maps.q, p.dk, it.h, it.token, &s.q_full);
+          if (it.n_b) load_tile(smem + q_bytes, &maps.q, p.dk, it.h, it.token + kC, &s.q_full);
+          ++q_loads;
+        }
+        const int hk = it.h / p.share;
+        auto load = [&](bool is_v, int j) {
+          // a first pass finds all slots empty
+          if (ok) ok = ctl.wait(&s.empty[to.at], to.turn ^ 1);
+          if (!ok) return;
+          bar_expect(&s.full[to.at], tile_bytes(is_v ? p.dv : p.dk));
+          load_tile(ring + to.at * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, it.start + j * kC, &s.full[to.at]);
+          to.next(ns);
+          ++loads;
+        };
+        load(false, 0);
+        for (int j = 0; ok && j < it.n; ++j) {
+          if (j + 1 < it.n) load(false, j + 1);
+          load(true, j);
+        }
       }
+      ok = __shfl_sync(kFull, ok, 0);
+      if (!ok || !next_work(ctl, s, count, work)) break;
     }
-  } else if (warp == 9) {
+    if (lane == 0 && *reinterpret_cast<volatile int*>(&s.c.abort)) {  // what is in flight must land
+      if (q_loads > 0) ctl.land(&s.q_full, (q_loads - 1) & 1);
+      for (uint32_t e = loads > static_cast<uint32_t>(ns) ? loads - ns : 0; e < loads; ++e) ctl.land(&s.full[e % ns], (e / ns) & 1);
+    }
+  } else {
     const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
     const uint64_t q[2] = {desc(smem_u32(smem), 16), desc(smem_u32(smem) + q_bytes, 16)};
-    auto ring_desc = [&](int at, uint32_t lbo) { return desc(smem_u32(ring) + at * slot, lbo); };
-    auto wait_slot = [&](int i) { return ctl.warp_wait(&s.full[i % ns], (i / ns) & 1); };
-    bool ok = ctl.warp_wait(&s.q_full, 0) && wait_slot(0);
-    if (ok) {
-      fence_after();
-      if (elect_one()) {
-        scores(tm, q[0], ring_desc(0, 16), id_s, p.dk);
-        commit(&s.s_full[0]);
-        if (n_b) {
-          scores(tm + kC, q[1], ring_desc(0, 16), id_s, p.dk);
-          commit(&s.s_full[1]);
-        }
-        commit(&s.empty[0]);
-      }
-    }
-    for (int j = 0; ok && j < n; ++j) {
-      const bool more = j + 1 < n;
-      const int ik = 2 * j + 1, iv = index_of_v(j);
-      if ((more && !wait_slot(ik)) || !wait_slot(iv)) break;
-      for (int x = 0; x < 2; ++x) {
-        const int mine = x ? n_b : n_a;
-        if (j >= mine) continue;
-        if (!(ok = ctl.warp_wait(&s.p_ready[x], j & 1))) break;
+    const uint64_t k0 = desc(smem_u32(ring), 16), v0 = desc(smem_u32(ring), kBlock);
+    uint32_t pp[2] = {0, 0}, qp = 0;  // phases of p_ready and q_full
+    Cursor c;
+    for (uint32_t count = 0; ok; ++count) {
+      Item it = find_item(p, work);
+      it.n = uniform(it.n), it.n_a = uniform(it.n_a), it.n_b = uniform(it.n_b);
+      if (it.n > 0) {
+        const int n = it.n;
+        if (!(ok = ctl.warp_wait(&s.q_full, qp) && ctl.warp_wait(&s.full[c.at], c.turn))) break;
+        qp ^= 1;
         fence_after();
         if (elect_one()) {
-          const uint64_t v = ring_desc(iv % ns, kBlock);
-#pragma unroll 1
-          for (int k = 0; k < kC / 16; ++k) mma_tmem(tm + 256 + x * kC, tm + x * kC + k * 8, v + k * 128, id_o, j + k > 0);
-          if (x == 1 || !n_b) commit(&s.empty[iv % ns]);
-          if (j + 1 < mine) {
-            scores(tm + x * kC, q[x], ring_desc(ik % ns, 16), id_s, p.dk);
-            commit(&s.s_full[x]);
-          } else {
-            commit(&s.o_done[x]);
+          const uint64_t k = k0 + c.at * (slot >> 4);
+          scores(tm, q[0], k, id_s, p.dk);
+          commit(&s.s_full[0]);
+          if (it.n_b) {
+            scores(tm + kC, q[1], k, id_s, p.dk);
+            commit(&s.s_full[1]);
           }
-          if (more && (x == 1 || !n_b)) commit(&s.empty[ik % ns]);
+          commit(&s.empty[c.at]);
+          if (n == 1) commit(&s.q_empty);
+        }
+        c.next(ns);
+        for (int j = 0; ok && j < n; ++j) {
+          const bool more = j + 1 < n;
+          const int ik = c.at;
+          if (more) {
+            if (!(ok = ctl.warp_wait(&s.full[c.at], c.turn))) break;
+            c.next(ns);
+          }
+          const int iv = c.at;
+          if (!(ok = ctl.warp_wait(&s.full[c.at], c.turn))) break;
+          c.next(ns);
+          const uint64_t k = k0 + ik * (slot >> 4), v = v0 + iv * (slot >> 4);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int mine = x ? it.n_b : it.n_a;
+            if (j >= mine) continue;
+            if (!(ok = ctl.warp_wait(&s.p_ready[x], pp[x]))) break;
+            pp[x] ^= 1;
+            fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int e = 0; e < kC / 16; ++e)
+                mma_tmem(tm + 256 + x * kC, tm + x * kC + e * 8, v + e * 128, id_o, j + e > 0);
+              if (x == 1 || !it.n_b) commit(&s.empty[iv]);
+              if (j + 1 < mine) {
+                scores(tm + x * kC, q[x], k, id_s, p.dk);
+                commit(&s.s_full[x]);
+              } else {
+                commit(&s.o_done[x]);
+              }
+              if (more && (x == 1 || !it.n_b)) {
+                commit(&s.empty[ik]);
+                if (j + 2 == n) commit(&s.q_empty);  // these were the last scores
+              }
+            }
+          }
         }
       }
+      if (!ok || !next_work(ctl, s, count, work)) break;
     }
     if (elect_one()) commit(&s.c.drain);  // nothing of this CTA's is in flight after it
     ctl.land(&s.c.drain, 0);
   }
-  close_tmem(tm);
+  close_tmem(tm, kFwdSoftmax + 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -504,7 +719,7 @@ template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const int h = blockIdx.y, hk = h / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC);
+  zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, threadIdx.x, blockDim.x);
   const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kC);
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk), g_bytes = tile_bytes(p.dv);
@@ -621,7 +836,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
       if (elect_one()) {
         const uint64_t k0 = ring_desc(2 * j, kBlock);
         // the warps' halves of dS lie 64 columns apart
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < kC / 16; ++k)
           mma_tmem(tm + kDq, tm + (j & 1) * kC + (k >> 2) * 64 + (k & 3) * 8, k0 + k * 128, id_o, j + k > 0);
         commit(&s.empty[2 * j % ns]);
@@ -650,8 +865,8 @@ template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const int hk = blockIdx.y, heads = p.H / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC);
-  zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC);
+  zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC, threadIdx.x, blockDim.x);
+  zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC, threadIdx.x, blockDim.x);
   const Tile t = find_tile(p, blockIdx.x, kC);  // a sequence's first keys have the most queries
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int k_bytes = tile_bytes(p.dk), v_bytes = tile_bytes(p.dv);
@@ -836,7 +1051,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
         fence_after();
         if (elect_one()) {
           const uint64_t g = g_desc(u, kBlock);
-#pragma unroll 1
+#pragma unroll
           for (int e = 0; e < kC / 16; ++e)
             mma_smem(tm + kDv, a + (e >> 2) * (kBlock >> 4) + (e & 3) * 2, g + e * 128, id_v, i + e > 0);
           commit(&s.p_free);
@@ -847,7 +1062,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
         if (elect_one()) {
           const uint64_t q = q_desc(u, kBlock);
           // the warps' halves of dS lie 64 columns apart
-#pragma unroll 1
+#pragma unroll
           for (int e = 0; e < kC / 16; ++e)
             mma_tmem(tm + kDk, tm + kDp + (e >> 2) * 64 + (e & 3) * 8, q + e * 128, id_k, i + e > 0);
           commit(&s.q_empty[u]);
@@ -911,7 +1126,7 @@ static bool rows_usable(const Rows& r, int dim, int heads) {
 static bool aligned(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; }
 
 bool tc_usable(const Problem& p, int dtype, bool backward) {
-  if (dtype == ASCAN_F32) return false;
+  if (dtype == ASCAN_F32 || tile_bound(p, 2 * kC) * p.H > 0x7fffffffll) return false;
   const int heads = p.H / p.share;
   if (!rows_usable(p.q, p.dk, p.H) || !rows_usable(p.k, p.dk, heads) || !rows_usable(p.v, p.dv, heads)) return false;
   if (!aligned(p.out) || !aligned(p.rest)) return false;
@@ -941,7 +1156,7 @@ static int forward(const Problem& p, const Maps& m, cudaStream_t s) {
   const int rc = allow_smem(tc_forward_kernel<T, TRAIN>, kSmemLimit, done);
   if (rc != ASCAN_OK) return rc;
   const size_t smem = 2 * bytes_of(p.dk) + slots(p.dk, p.dv) * slot_bytes(p.dk, p.dv) + sizeof(ForwardTail);
-  tc_forward_kernel<T, TRAIN><<<dim3(tile_bound(p, 2 * kC), p.H), kTcThreads, smem, s>>>(p, m);
+  tc_forward_kernel<T, TRAIN><<<static_cast<unsigned>(tile_bound(p, 2 * kC) * p.H), kFwdThreads, smem, s>>>(p, m);
   return launch_status();
 }
 

@@ -235,7 +235,7 @@ def test_sequences_do_not_meet(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")], ids=str)
 @pytest.mark.parametrize("where", ["values", "keys"])
-@pytest.mark.parametrize("at", [0, 5, 130, 299])
+@pytest.mark.parametrize("at", [0, 5, 130, 139, 299])
 def test_what_is_not_finite_stays_behind_the_mask(at, where, bad, dtype):
   n = 300
   q, k, v, do = make([n], (2, 1), (64, 64), dtype)
