@@ -126,6 +126,16 @@ __device__ __forceinline__ void scores(uint32_t to, uint64_t a, uint64_t b, uint
   }
 }
 
+// The wait for a load, tied to its registers: the next load may be in flight
+// while these are worked on.
+__device__ __forceinline__ void wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(uint64_t x);
 template <>
@@ -371,6 +381,14 @@ __device__ __forceinline__ bool next_work(const Ctl& ctl, ForwardTail& s, uint32
   return work >= 0;
 }
 
+__device__ __forceinline__ bool next_work_one(const Ctl& ctl, ForwardTail& s, uint32_t count, int& work) {
+  const uint32_t u = count & 1;
+  if (!ctl.wait(&s.next_full[u], (count >> 1) & 1)) return false;
+  work = read_work(s.next[u]);
+  bar_arrive(&s.next_empty[u]);
+  return work >= 0;
+}
+
 // What a row has added up: its exponentials, the same rounded as P, and the
 // reference that they are taken against.
 struct RowState {
@@ -499,17 +517,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
           float high = -INFINITY;
           uint64_t a[2] = {0, 0};
           const uint64_t ref2 = pair(-r.m * c2, -r.m * c2);
+          uint32_t sc[2][16];
+          tmem_ld16(ts, sc[0]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t sc[32];
-            tmem_ld32(ts + 32 * i, sc);
-            wait_ld();
+          for (int i = 0; i < 8; ++i) {
+            uint32_t* x16 = sc[i & 1];
+            wait_ld16(x16);
+            if (i < 7) tmem_ld16(ts + 16 * (i + 1), sc[(i + 1) & 1]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint64_t z = fma2(pair_of(sc + 2 * e), c22, ref2);
-              const uint64_t y = (e & 7) >= 8 - kPoly ? poly_ex2_2(z) : ex2_2(z);
-              high = max3(high, __uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1]));
-              w[16 * i + e] = pack2<T>(y);
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t z = fma2(pair_of(x16 + 2 * e), c22, ref2);
+              const uint64_t y = e >= 8 - kPoly ? poly_ex2_2(z) : ex2_2(z);
+              high = max3(high, __uint_as_float(x16[2 * e]), __uint_as_float(x16[2 * e + 1]));
+              w[8 * i + e] = pack2<T>(y);
               a[e & 1] = add2(a[e & 1], y);
             }
           }
@@ -636,50 +656,47 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
       for (uint32_t e = loads > static_cast<uint32_t>(ns) ? loads - ns : 0; e < loads; ++e) ctl.land(&s.full[e % ns], (e / ns) & 1);
     }
   } else {
-    const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
-    const uint64_t q[2] = {desc(smem_u32(smem), 16), desc(smem_u32(smem) + q_bytes, 16)};
-    const uint64_t k0 = desc(smem_u32(ring), 16), v0 = desc(smem_u32(ring), kBlock);
-    uint32_t pp[2] = {0, 0}, qp = 0;  // phases of p_ready and q_full
-    Cursor c;
-    for (uint32_t count = 0; ok; ++count) {
-      Item it = find_item(p, work);
-      it.n = uniform(it.n), it.n_a = uniform(it.n_a), it.n_b = uniform(it.n_b);
-      if (it.n > 0) {
-        const int n = it.n;
-        if (!(ok = ctl.warp_wait(&s.q_full, qp) && ctl.warp_wait(&s.full[c.at], c.turn))) break;
-        qp ^= 1;
-        fence_after();
-        if (elect_one()) {
-          const uint64_t k = k0 + c.at * (slot >> 4);
-          scores(tm, q[0], k, id_s, p.dk);
+    // One thread: a vote of the warp at every wait would cost a tenth of the time.
+    if (elect_one()) {
+      const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
+      const uint64_t q[2] = {desc(smem_u32(smem), 16), desc(smem_u32(smem) + q_bytes, 16)};
+      const uint64_t k0 = desc(smem_u32(ring), 16), v0 = desc(smem_u32(ring), kBlock);
+      uint32_t pp[2] = {0, 0}, qp = 0;  // phases of p_ready and q_full
+      Cursor c;
+      for (uint32_t count = 0; ok; ++count) {
+        const Item it = find_item(p, work);
+        if (it.n > 0) {
+          const int n = it.n;
+          if (!(ok = ctl.wait(&s.q_full, qp) && ctl.wait(&s.full[c.at], c.turn))) break;
+          qp ^= 1;
+          const uint64_t k1 = k0 + c.at * (slot >> 4);
+          scores(tm, q[0], k1, id_s, p.dk);
           commit(&s.s_full[0]);
           if (it.n_b) {
-            scores(tm + kC, q[1], k, id_s, p.dk);
+            scores(tm + kC, q[1], k1, id_s, p.dk);
             commit(&s.s_full[1]);
           }
           commit(&s.empty[c.at]);
           if (n == 1) commit(&s.q_empty);
-        }
-        c.next(ns);
-        for (int j = 0; ok && j < n; ++j) {
-          const bool more = j + 1 < n;
-          const int ik = c.at;
-          if (more) {
-            if (!(ok = ctl.warp_wait(&s.full[c.at], c.turn))) break;
-            c.next(ns);
-          }
-          const int iv = c.at;
-          if (!(ok = ctl.warp_wait(&s.full[c.at], c.turn))) break;
           c.next(ns);
-          const uint64_t k = k0 + ik * (slot >> 4), v = v0 + iv * (slot >> 4);
+          for (int j = 0; ok && j < n; ++j) {
+            const bool more = j + 1 < n;
+            const int ik = c.at;
+            if (more) {
+              if (!(ok = ctl.wait(&s.full[c.at], c.turn))) break;
+              c.next(ns);
+            }
+            const int iv = c.at;
+            if (!(ok = ctl.wait(&s.full[c.at], c.turn))) break;
+            c.next(ns);
+            const uint64_t k = k0 + ik * (slot >> 4), v = v0 + iv * (slot >> 4);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int mine = x ? it.n_b : it.n_a;
-            if (j >= mine) continue;
-            if (!(ok = ctl.warp_wait(&s.p_ready[x], pp[x]))) break;
-            pp[x] ^= 1;
-            fence_after();
-            if (elect_one()) {
+            for (int x = 0; x < 2; ++x) {
+              const int mine = x ? it.n_b : it.n_a;
+              if (j >= mine) continue;
+              if (!(ok = ctl.wait(&s.p_ready[x], pp[x]))) break;
+              pp[x] ^= 1;
+              fence_after();
 #pragma unroll
               for (int e = 0; e < kC / 16; ++e)
                 mma_tmem(tm + 256 + x * kC, tm + x * kC + e * 8, v + e * 128, id_o, j + e > 0);
@@ -697,11 +714,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
             }
           }
         }
+        if (!ok || !next_work_one(ctl, s, count, work)) break;
       }
-      if (!ok || !next_work(ctl, s, count, work)) break;
+      commit(&s.c.drain);  // nothing of this CTA's is in flight after it
+      ctl.land(&s.c.drain, 0);
     }
-    if (elect_one()) commit(&s.c.drain);  // nothing of this CTA's is in flight after it
-    ctl.land(&s.c.drain, 0);
   }
   close_tmem(tm, kFwdSoftmax + 1);
 }
