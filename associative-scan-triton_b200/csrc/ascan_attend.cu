@@ -13,7 +13,7 @@
 namespace ascan {
 namespace attend {
 
-constexpr int kR = 64;         // rows of a tile
+constexpr int kR = 64;  // rows of a tile, as find_tile's shift has it
 constexpr int kPlainThreads = 256;
 constexpr int kPs = kR + 4;    // row of a tile of scores, in floats
 
@@ -150,9 +150,9 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
   const int h = blockIdx.y, hk = h / p.share, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   if (blockIdx.x == 0 && h == 0) check_cu(p);
   zero_outside<T>(p, p.out, h, p.H, p.dv, blockIdx.x, kR, threadIdx.x, blockDim.x);
-  const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kR);  // long rows first
+  const Tile t = find_tile<6>(p, gridDim.x - 1 - blockIdx.x);  // long rows first
   if (t.first < 0) return;
-  const int len = static_cast<int>(min(static_cast<long long>(kR), t.len - t.first));
+  const int len = min(kR, t.len - t.first);
   load_tile<T, D>(qs, p.q, h, t.start + t.first, len, p.dk);
   float acc[4][D / 16], l[4], m[4];
 #pragma unroll
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
     for (int c = 0; c < D / 16; ++c) acc[a][c] = 0.f;
   }
   const float c2 = p.scale * kLog2e;
-  for (long long j = 0; j <= t.first; j += kR) {
+  for (int j = 0; j <= t.first; j += kR) {
     const bool own = j == t.first;
     __syncthreads();
     load_tile<T, D>(ks, p.k, hk, t.start + j, own ? len : kR, p.dk);
@@ -241,9 +241,9 @@ __global__ void __launch_bounds__(kPlainThreads) dq_kernel(const __grid_constant
   float *qs = plain_smem_base, *gs = qs + S, *ks = gs + S, *vs = ks + S, *ps = vs + S;
   const int h = blockIdx.y, hk = h / p.share, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kR, threadIdx.x, blockDim.x);
-  const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kR);
+  const Tile t = find_tile<6>(p, gridDim.x - 1 - blockIdx.x);
   if (t.first < 0) return;
-  const int len = static_cast<int>(min(static_cast<long long>(kR), t.len - t.first));
+  const int len = min(kR, t.len - t.first);
   const long long at = t.start + t.first;
   load_tile<T, D>(qs, p.q, h, at, len, p.dk);
   load_tile<T, D>(gs, p.d_out, h, at, len, p.dv);
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kPlainThreads) dq_kernel(const __grid_constant
     for (int c = 0; c < D / 16; ++c) acc[a][c] = 0.f;
   }
   const float c2 = p.scale * kLog2e;
-  for (long long j = 0; j <= t.first; j += kR) {
+  for (int j = 0; j <= t.first; j += kR) {
     const bool own = j == t.first;
     __syncthreads();
     load_tile<T, D>(ks, p.k, hk, t.start + j, own ? len : kR, p.dk);
@@ -288,9 +288,9 @@ __global__ void __launch_bounds__(kPlainThreads) dkdv_kernel(const __grid_consta
   const int hk = blockIdx.y, heads = p.H / p.share, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kR, threadIdx.x, blockDim.x);
   zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kR, threadIdx.x, blockDim.x);
-  const Tile t = find_tile(p, blockIdx.x, kR);  // a sequence's first keys have the most queries
+  const Tile t = find_tile<6>(p, blockIdx.x);  // a sequence's first keys have the most queries
   if (t.first < 0) return;
-  const int len = static_cast<int>(min(static_cast<long long>(kR), t.len - t.first));
+  const int len = min(kR, t.len - t.first);
   const long long at = t.start + t.first;
   load_tile<T, D>(ks, p.k, hk, at, len, p.dk);
   load_tile<T, D>(vs, p.v, hk, at, len, p.dv);
@@ -302,9 +302,9 @@ __global__ void __launch_bounds__(kPlainThreads) dkdv_kernel(const __grid_consta
   const float c2 = p.scale * kLog2e;
   for (int g = 0; g < p.share; ++g) {
     const int h = hk * p.share + g;
-    for (long long i = t.first; i < t.len; i += kR) {
+    for (int i = t.first; i < t.len; i += kR) {
       const bool own = i == t.first;
-      const int n = static_cast<int>(min(static_cast<long long>(kR), t.len - i));
+      const int n = min(kR, t.len - i);
       __syncthreads();
       load_tile<T, D>(qs, p.q, h, t.start + i, n, p.dk);
       load_tile<T, D>(gs, p.d_out, h, t.start + i, n, p.dv);

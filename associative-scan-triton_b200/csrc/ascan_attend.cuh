@@ -68,23 +68,30 @@ __device__ __forceinline__ long long cu_at(const Problem& p, long long i) {
 inline long long tile_bound(const Problem& p, int rows) { return p.BL / rows + p.N; }
 
 struct Tile {
-  long long start, len;  // the sequence's
-  long long first;       // the tile's first token in it; -1: no tile
+  int start, len;  // the sequence's
+  int first;       // the tile's first token in it; -1: no tile
 };
 
-__device__ __forceinline__ Tile find_tile(const Problem& p, long long x, int rows) {
-  long long lo = 0, hi = p.N - 1;  // the last sequence whose tiles start at or before x
+// Numbers below 2^30 and tiles of 2^SHIFT rows: a search costs a load and a few
+// instructions a step, in front of everything else that a CTA does.
+template <int SHIFT, typename F>
+__device__ __forceinline__ Tile find_tile(const Problem& p, int x, F at) {
+  int lo = 0, hi = static_cast<int>(p.N) - 1;  // the last sequence whose tiles start at or before x
   while (lo < hi) {
-    const long long mid = (lo + hi + 1) >> 1;
-    if (cu_at(p, mid) / rows + mid <= x) lo = mid;
+    const int mid = (lo + hi + 1) >> 1;
+    if ((at(mid) >> SHIFT) + mid <= x) lo = mid;
     else hi = mid - 1;
   }
   Tile t;
-  t.start = cu_at(p, lo);
-  t.len = cu_at(p, lo + 1) - t.start;
-  t.first = (x - t.start / rows - lo) * rows;
+  t.start = at(lo);
+  t.len = at(lo + 1) - t.start;
+  t.first = (x - (t.start >> SHIFT) - lo) << SHIFT;
   if (t.first < 0 || t.first >= t.len) t.first = -1;
   return t;
+}
+template <int SHIFT>
+__device__ __forceinline__ Tile find_tile(const Problem& p, int x) {
+  return find_tile<SHIFT>(p, x, [&](int i) { return static_cast<int>(cu_at(p, i)); });
 }
 
 // Rows of no sequence come out zero; slab x of the packed axis is the x-th CTA's.

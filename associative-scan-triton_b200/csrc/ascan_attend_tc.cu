@@ -189,38 +189,40 @@ __device__ __forceinline__ bool f16() { return false; }
 template <>
 __device__ __forceinline__ bool f16<__half>() { return true; }
 
-// Both elements of a word: its exponents all ones?
+// sum + 0 * x for both elements of a word: NaN if one is not finite.
 template <typename T>
-__device__ __forceinline__ uint32_t odd_bits(uint32_t x) {
-  const uint32_t one = f16<T>() ? 0x0400u : 0x0080u;
-  return ((x & 0x7fff7fffu) + (one | one << 16)) & 0x80008000u;
+__device__ __forceinline__ uint32_t zero_times(uint32_t x, uint32_t sum) {
+  if (f16<T>()) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0));
+  return sum;
 }
 
 // Row `row` of a tile with `blocks` of 64 columns from block `b`: zeros if it is
 // not `live`, else without what is not finite.  True if there was any.
 template <typename T>
 __device__ __forceinline__ bool clean_row(unsigned char* tile, int row, int b, int blocks, bool live) {
-  uint32_t found = 0;
-#pragma unroll 4
+  auto place = [&](int c) { return reinterpret_cast<uint4*>(tile + (b + (c >> 3)) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4)); };
+  uint32_t sum[2] = {0, 0};
+#pragma unroll 8
   for (int c = 0; c < 8 * blocks; ++c) {
-    uint4* at = reinterpret_cast<uint4*>(tile + (b + (c >> 3)) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4));
     if (!live) {
-      *at = make_uint4(0, 0, 0, 0);
+      *place(c) = make_uint4(0, 0, 0, 0);
       continue;
     }
-    uint4 x = *at;
-    const uint32_t bad = odd_bits<T>(x.x) | odd_bits<T>(x.y) | odd_bits<T>(x.z) | odd_bits<T>(x.w);
-    if (bad) {
-      auto fix = [](uint32_t w) {
-        const uint32_t o = odd_bits<T>(w);
-        return w & ~((o & 0x8000u ? 0xffffu : 0u) | (o & 0x80000000u ? 0xffff0000u : 0u));
-      };
-      x.x = fix(x.x), x.y = fix(x.y), x.z = fix(x.z), x.w = fix(x.w);
-      *at = x;
-    }
-    found |= bad;
+    const uint4 x = *place(c);
+    sum[0] = zero_times<T>(x.x, sum[0]);
+    sum[1] = zero_times<T>(x.y, sum[1]);
+    sum[0] = zero_times<T>(x.z, sum[0]);
+    sum[1] = zero_times<T>(x.w, sum[1]);
   }
-  return found != 0;
+  if (!(((sum[0] | sum[1]) & 0x7fff7fffu) != 0)) return false;
+  const uint32_t ones = f16<T>() ? 0x7c00u : 0x7f80u;
+#pragma unroll 1
+  for (int c = 0; c < 64 * blocks; ++c) {
+    uint16_t* at = reinterpret_cast<uint16_t*>(place(c >> 3)) + (c & 7);
+    if ((*at & ones) == ones) *at = 0;
+  }
+  return true;
 }
 
 // 64 columns of a warp's 32 rows from registers (32 packed words a lane) to
@@ -309,16 +311,27 @@ __device__ __forceinline__ void check_cu(const Problem& p, int thread, int threa
 // forward
 // ---------------------------------------------------------------------------
 
-constexpr int kFwdSoftmax = 8, kFwdRoles = kFwdSoftmax + 2, kFwdThreads = kFwdRoles * 32;
+constexpr int kFwdSoftmax = 8, kFwdThreads = (kFwdSoftmax + 2) * 32;
 
 // Of eight pairs of scores so many take the polynomial.
 constexpr int kPoly = 3;
+// An item's place is searched for in shared memory, eight times as fast as
+// through what the slots leave of the first cache.
+constexpr int kEnds = 512;
+constexpr int kItems = 4;  // that the loads may be ahead
 
+// A work item: two tiles of queries of one head; `key` blocks of keys of each.
+struct Item {
+  int start, token, left;  // the sequence's first token, the item's, and the sequence's from there on
+  int h, n_a, n_b, n;      // n 0: no tokens
+};
 struct ForwardTail {
   Common c;
-  uint64_t q_full, q_empty, full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], o_done[2], next_full[2], next_empty[2];
-  alignas(16) uint32_t next[2][4];  // the scheduler's answers
+  uint64_t q_full, q_empty, full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], o_done[2], item_full[kItems], item_empty[kItems], next_full;
+  alignas(16) uint32_t next[4];  // the scheduler's answer
+  Item items[kItems];           // n 0: no more
   uint32_t bad[4][2][4];  // by work item: tokens of the tiles' own blocks with values that are not finite
+  int ends[kEnds];        // cu_seqlens, if it is no longer
 };
 
 // Takes over the work of a CTA that has not been launched yet: the answer, its
@@ -350,43 +363,28 @@ struct Cursor {
   }
 };
 
-// A work item: two tiles of queries of one head; `key` blocks of keys of each.
-struct Item {
-  int start, token, left;  // the sequence's first token, the item's, and the sequence's from there on
-  int h, n_a, n_b, n;      // n 0: no tokens
-  int x;                   // its number without the head
-};
-__device__ __noinline__ Item find_item(const Problem& p, int work) {
+__device__ __forceinline__ Item find_item(const Problem& p, const int* ends, int x, int h) {
   Item i;
-  const int tiles = static_cast<int>(gridDim.x) / p.H;
-  i.x = tiles - 1 - work / p.H;  // long rows first, the heads of a tile together
-  i.h = work % p.H;
-  const Tile t = find_tile(p, i.x, 2 * kC);
-  const int own = static_cast<int>(t.first / kC);  // the first tile's own block of keys
-  i.start = static_cast<int>(t.start);
-  i.token = static_cast<int>(t.start + t.first);
-  i.left = static_cast<int>(t.len - t.first);
+  i.h = h;
+  const Tile t = p.N < kEnds ? find_tile<8>(p, x, [&](int n) { return ends[n]; }) : find_tile<8>(p, x);
+  const int own = t.first / kC;  // the first tile's own block of keys
+  i.start = t.start;
+  i.token = t.start + t.first;
+  i.left = t.len - t.first;
   i.n_a = t.first < 0 ? 0 : own + 1;
   i.n_b = t.first >= 0 && i.left > kC ? own + 2 : 0;
   i.n = max(i.n_a, i.n_b);
   return i;
 }
 
-// The next item's number, the same for every role; false when there is none.
-__device__ __forceinline__ bool next_work(const Ctl& ctl, ForwardTail& s, uint32_t count, int& work) {
-  const uint32_t u = count & 1;
-  if (!ctl.warp_wait(&s.next_full[u], (count >> 1) & 1)) return false;
-  work = read_work(s.next[u]);
-  warp_arrive(&s.next_empty[u]);
-  return work >= 0;
-}
-
-__device__ __forceinline__ bool next_work_one(const Ctl& ctl, ForwardTail& s, uint32_t count, int& work) {
-  const uint32_t u = count & 1;
-  if (!ctl.wait(&s.next_full[u], (count >> 1) & 1)) return false;
-  work = read_work(s.next[u]);
-  bar_arrive(&s.next_empty[u]);
-  return work >= 0;
+// To the warps that compute: the count-th item with tokens, or that there is
+// none any more.
+__device__ __forceinline__ bool hand_out(const Ctl& ctl, ForwardTail& s, uint32_t count, const Item& it) {
+  const uint32_t u = count % kItems;
+  if (count >= kItems && !ctl.wait(&s.item_empty[u], (count / kItems - 1) & 1)) return false;
+  s.items[u] = it;
+  bar_arrive(&s.item_full[u]);
+  return true;
 }
 
 // What a row has added up: its exponentials, the same rounded as P, and the
@@ -404,15 +402,17 @@ struct RowState {
 // costs more than it saves.
 template <typename T, bool TRAIN>
 __device__ __noinline__ RowState move_reference(uint32_t ts, uint32_t to, int last, int o32, float c2, RowState r) {
+  const int blocks = __reduce_max_sync(kFull, last) / 32;  // of 32 columns, up to the last that a row of the warp sees
   float high = -INFINITY;
 #pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i <= blocks; ++i) {
     uint32_t sc[32];
     tmem_ld32(ts + 32 * i, sc);
     wait_ld();
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (32 * i + e <= last) high = fmaxf(high, __uint_as_float(sc[e]));
+    for (int e = 0; e < 32; e += 2)
+      high = max3(high, 32 * i + e > last ? -INFINITY : __uint_as_float(sc[e]),
+                  32 * i + e + 1 > last ? -INFINITY : __uint_as_float(sc[e + 1]));
   }
   const float next = (high - r.m) * c2 > 8.f ? high : r.m;
   if (o32 > 0 && __any_sync(kFull, next != r.m)) {
@@ -435,18 +435,23 @@ __device__ __noinline__ RowState move_reference(uint32_t ts, uint32_t to, int la
   const uint64_t ref2 = pair(ref, ref), c22 = pair(c2, c2);
 #pragma unroll 1
   for (int i = 0; i < 4; ++i) {
-    uint32_t sc[32], w[16];
-    tmem_ld32(ts + 32 * i, sc);
-    wait_ld();
+    uint32_t w[16];
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (32 * i + e > last) sc[e] = 0xff800000u;
+    for (int e = 0; e < 16; ++e) w[e] = 0;
+    if (i <= blocks) {
+      uint32_t sc[32];
+      tmem_ld32(ts + 32 * i, sc);
+      wait_ld();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint64_t y = ex2_2(fma2(pair_of(sc + 2 * e), c22, ref2));
-      w[e] = pack2<T>(y);
-      r.l[e & 1] = add2(r.l[e & 1], y);
-      if (TRAIN) r.z[e & 1] = add2(r.z[e & 1], unpack2<T>(w[e]));
+      for (int e = 0; e < 32; ++e)
+        if (32 * i + e > last) sc[e] = 0xff800000u;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint64_t y = ex2_2(fma2(pair_of(sc + 2 * e), c22, ref2));
+        w[e] = pack2<T>(y);
+        r.l[e & 1] = add2(r.l[e & 1], y);
+        if (TRAIN) r.z[e & 1] = add2(r.z[e & 1], unpack2<T>(w[e]));
+      }
     }
     tmem_st16(ts + 16 * i, w);
   }
@@ -473,15 +478,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
       bar_init(&s.s_full[i], 1);
       bar_init(&s.p_ready[i], 4);
       bar_init(&s.o_done[i], 1);
-      bar_init(&s.next_full[i], 1);
-      bar_init(&s.next_empty[i], kFwdRoles);
     }
+    for (int i = 0; i < kItems; ++i) bar_init(&s.item_full[i], 1), bar_init(&s.item_empty[i], kFwdSoftmax + 1);
+    bar_init(&s.next_full, 1);
     bar_init(&s.c.drain, 1);
     s.c.abort = 0;
     bars_done();
   }
+  if (p.N < kEnds)
+    for (int i = tid; i <= p.N; i += kFwdThreads) s.ends[i] = static_cast<int>(cu_at(p, i));
   const uint32_t tm = open_tmem(&s.c, kFwdSoftmax + 1);
-  int work = blockIdx.x;
   bool ok = true;
   uint32_t base = 0;  // of the item's loads in the ring: K0, then (K[j+1], V[j]) for every j
 
@@ -493,7 +499,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
     const int n32 = (p.dv + 31) / 32;
     uint32_t sp = 0, op = 0;  // phases: scores seen, rows finished
     for (uint32_t count = 0; ok; ++count) {
-      const Item it = find_item(p, work);
+      const uint32_t u = count % kItems;
+      if (!(ok = ctl.warp_wait(&s.item_full[u], (count / kItems) & 1))) break;
+      const Item it = s.items[u];
+      warp_arrive(&s.item_empty[u]);
+      if (it.n == 0) break;
       const int mine = x ? it.n_b : it.n_a, left = it.left - x * kC;  // of the sequence from this tile on
       uint32_t* bad = &s.bad[count & 3][x][quad];
       if (lane == 0) *bad = 0;
@@ -537,7 +547,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
           if (!again) r.l[0] = add2(r.l[0], a[0]), r.l[1] = add2(r.l[1], a[1]);
         }
         if (again) {
-          r = move_reference<T, TRAIN>(ts, to, diagonal ? row : kC, j > 0 ? n32 : 0, c2, r);
+          r = move_reference<T, TRAIN>(ts, to, diagonal ? row : kC - 1, j > 0 ? n32 : 0, c2, r);
         } else {
           if (TRAIN) {
 #pragma unroll
@@ -605,27 +615,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
         }
       }
       base += 2 * it.n;
-      if (!next_work(ctl, s, count, work)) break;
     }
   } else if (warp == kFwdSoftmax) {
     uint32_t q_loads = 0, loads = 0;
     Cursor to;
-    for (uint32_t count = 0; ok; ++count) {
-      const uint32_t u = count & 1;
-      if (lane == 0) {  // the next item's number comes while this one is loaded
-        if (count > 1) ok = ctl.wait(&s.next_empty[u], ((count >> 1) - 1) & 1);
-        if (ok) {
-          bar_expect(&s.next_full[u], 16);
-          ask_work(s.next[u], &s.next_full[u]);
-        }
+    int work = blockIdx.x;
+    for (uint32_t asked = 0; ok; ++asked) {
+      if (lane == 0) {  // the next number comes while this one's tiles are loaded
+        bar_expect(&s.next_full, 16);
+        ask_work(s.next, &s.next_full);
       }
-      ok = __shfl_sync(kFull, ok, 0);
-      if (!ok) break;
-      const Item it = find_item(p, work);
-      if (it.x == 0 && it.h == 0) check_cu(p, lane, 32);
-      zero_outside<T>(p, p.out, it.h, p.H, p.dv, it.x, 2 * kC, lane, 32);
+      const int x = static_cast<int>(gridDim.x) / p.H - 1 - work / p.H, h = work % p.H;  // long rows first, a tile's heads together
+      const Item it = find_item(p, s.ends, x, h);
+      if (x == 0 && h == 0) check_cu(p, lane, 32);
+      zero_outside<T>(p, p.out, h, p.H, p.dv, x, 2 * kC, lane, 32);
       if (it.n > 0 && lane == 0) {
-        if (q_loads > 0) ok = ctl.wait(&s.q_empty, (q_loads - 1) & 1);
+        ok = hand_out(ctl, s, q_loads, it);
+        if (ok && q_loads > 0) ok = ctl.wait(&s.q_empty, (q_loads - 1) & 1);
         if (ok) {
           bar_expect(&s.q_full, q_bytes * (it.n_b ? 2 : 1));
           load_tile(smem, &maps.q, p.dk, it.h, it.token, &s.q_full);
@@ -648,8 +654,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
           load(true, j);
         }
       }
-      ok = __shfl_sync(kFull, ok, 0);
-      if (!ok || !next_work(ctl, s, count, work)) break;
+      ok = __shfl_sync(kFull, ok, 0) && ctl.warp_wait(&s.next_full, asked & 1);
+      if (!ok) break;
+      work = read_work(s.next);
+      __syncwarp();
+      if (work < 0) {
+        Item none{};
+        if (lane == 0) hand_out(ctl, s, q_loads, none);
+        break;
+      }
     }
     if (lane == 0 && *reinterpret_cast<volatile int*>(&s.c.abort)) {  // what is in flight must land
       if (q_loads > 0) ctl.land(&s.q_full, (q_loads - 1) & 1);
@@ -664,8 +677,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
       uint32_t pp[2] = {0, 0}, qp = 0;  // phases of p_ready and q_full
       Cursor c;
       for (uint32_t count = 0; ok; ++count) {
-        const Item it = find_item(p, work);
-        if (it.n > 0) {
+        const uint32_t u = count % kItems;
+        if (!(ok = ctl.wait(&s.item_full[u], (count / kItems) & 1))) break;
+        const Item it = s.items[u];
+        bar_arrive(&s.item_empty[u]);
+        if (it.n == 0) break;
+        {
           const int n = it.n;
           if (!(ok = ctl.wait(&s.q_full, qp) && ctl.wait(&s.full[c.at], c.turn))) break;
           qp ^= 1;
@@ -714,7 +731,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
             }
           }
         }
-        if (!ok || !next_work_one(ctl, s, count, work)) break;
       }
       commit(&s.c.drain);  // nothing of this CTA's is in flight after it
       ctl.land(&s.c.drain, 0);
@@ -737,13 +753,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
   extern __shared__ __align__(1024) unsigned char smem[];
   const int h = blockIdx.y, hk = h / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, threadIdx.x, blockDim.x);
-  const Tile t = find_tile(p, gridDim.x - 1 - blockIdx.x, kC);
+  const Tile t = find_tile<7>(p, gridDim.x - 1 - blockIdx.x);
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk), g_bytes = tile_bytes(p.dv);
   unsigned char* ring = smem + q_bytes + g_bytes;
   DqTail& s = *reinterpret_cast<DqTail*>(ring + ns * slot);
   const Ctl ctl{&s.c, p.err};
-  const int n = static_cast<int>(t.first / kC) + 1, len = static_cast<int>(min(static_cast<long long>(kC), t.len - t.first));
+  const int n = t.first / kC + 1, len = min(kC, t.len - t.first);
   const long long at = t.start + t.first;
   if (tid == 0) {
     bar_init(&s.q_full, 1);
@@ -820,7 +836,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
         const int to = i % ns;
         if (i >= ns && !ctl.wait(&s.empty[to], (i / ns - 1) & 1)) break;
         bar_expect(&s.full[to], tile_bytes(is_v ? p.dv : p.dk));
-        load_tile(ring + to * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, t.start + static_cast<long long>(i >> 1) * kC, &s.full[to]);
+        load_tile(ring + to * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, t.start + (i >> 1) * kC, &s.full[to]);
       }
       if (i < 2 * n) {
         ctl.land(&s.q_full, 0);
@@ -884,13 +900,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
   const int hk = blockIdx.y, heads = p.H / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC, threadIdx.x, blockDim.x);
   zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC, threadIdx.x, blockDim.x);
-  const Tile t = find_tile(p, blockIdx.x, kC);  // a sequence's first keys have the most queries
+  const Tile t = find_tile<7>(p, blockIdx.x);  // a sequence's first keys have the most queries
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int k_bytes = tile_bytes(p.dk), v_bytes = tile_bytes(p.dv);
   unsigned char *q_ring = smem + k_bytes + v_bytes, *g_ring = q_ring + 2 * k_bytes, *pt = g_ring + 2 * v_bytes;
   DkvTail& s = *reinterpret_cast<DkvTail*>(pt + 2 * kBlock);
   const Ctl ctl{&s.c, p.err};
-  const int blocks = static_cast<int>((t.len - t.first + kC - 1) / kC), len = static_cast<int>(min(static_cast<long long>(kC), t.len - t.first));
+  const int blocks = (t.len - t.first + kC - 1) / kC, len = min(kC, t.len - t.first);
   const int total = blocks * p.share;  // tiles of queries, head by head
   const long long at = t.start + t.first;
   if (tid == 0) {
@@ -927,7 +943,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
     for (int i = 0, b = 0; i < total; ++i, b = b + 1 < blocks ? b + 1 : 0) {
       const int u = i & 1;
       const bool diagonal = b == 0;
-      const int n = static_cast<int>(min(static_cast<long long>(kC), t.len - t.first - static_cast<long long>(b) * kC));
+      const int n = min(kC, t.len - t.first - b * kC);
       const bool edge = diagonal || n < kC;
       if (!(ok = ctl.warp_wait(&s.stat_full[u], (i >> 1) & 1) && ctl.warp_wait(&s.s_full, i & 1))) break;
       fence_after();
