@@ -214,20 +214,72 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
   }
 }
 
-// d = do.o, a warp per row.
+// d = do.o.  Memory bounds it: sixteen lanes a row with sixteen bytes each where
+// alignment allows (vec), eight rows in flight for a warp; else a warp per row.
 template <typename T>
-__global__ void __launch_bounds__(kPlainThreads) dot_kernel(const __grid_constant__ Problem p) {
+__global__ void __launch_bounds__(kPlainThreads) dot_kernel(const __grid_constant__ Problem p, int vec) {
   const int lane = threadIdx.x & 31;
   if (blockIdx.x == 0) check_cu(p);
-  const long long step = static_cast<long long>(gridDim.x) * (kPlainThreads / 32);
-  for (long long unit = (static_cast<long long>(blockIdx.x) * kPlainThreads + threadIdx.x) >> 5; unit < p.BL * p.H; unit += step) {
-    const long long t = unit / p.H;
-    const int h = static_cast<int>(unit % p.H);
-    const T* g = static_cast<const T*>(p.d_out.p) + t * p.d_out.st + h * p.d_out.sh;
-    const T* o = static_cast<const T*>(p.out) + unit * p.dv;
-    const T* r = p.rest ? static_cast<const T*>(p.rest) + unit * p.dv : nullptr;
+  const long long warp = (static_cast<long long>(blockIdx.x) * kPlainThreads + threadIdx.x) >> 5;
+  const long long warps = static_cast<long long>(gridDim.x) * (kPlainThreads / 32);
+  const long long units = p.BL * p.H;
+  const T *g = static_cast<const T*>(p.d_out.p), *o = static_cast<const T*>(p.out), *r = static_cast<const T*>(p.rest);
+  if (vec) {
+    constexpr int V = 16 / sizeof(T), ROWS = 4;
+    const int gl = lane & 15;
+    const long long first = warp * 2 * ROWS, step = warps * 2 * ROWS;
+    // token and head of the warp's first row, moved on without divisions
+    long long t0 = first / p.H;
+    int h0 = static_cast<int>(first % p.H);
+    const long long step_t = step / p.H;
+    const int step_h = static_cast<int>(step % p.H);
+    for (long long u0 = first; u0 < units; u0 += step, t0 += step_t, h0 += step_h) {
+      if (h0 >= p.H) h0 -= p.H, ++t0;
+      long long t[ROWS];
+      int h[ROWS];
+#pragma unroll
+      for (int e = 0; e < ROWS; ++e) {
+        t[e] = t0, h[e] = h0 + 2 * e + (lane >> 4);
+        while (h[e] >= p.H) h[e] -= p.H, ++t[e];
+      }
+      uint4 x[ROWS], y[ROWS], z[ROWS];
+      const int parts = p.dv > 16 * V ? 2 : 1;  // a row of 128 floats is two rounds
+      float sum[ROWS] = {};
+      for (int part = 0; part < parts; ++part) {
+        const int d = part * 16 * V + gl * V;
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) {
+          const long long u = u0 + 2 * e + (lane >> 4);
+          x[e] = y[e] = z[e] = make_uint4(0, 0, 0, 0);
+          if (u < units && d < p.dv) {
+            x[e] = __ldcs(reinterpret_cast<const uint4*>(g + t[e] * p.d_out.st + h[e] * p.d_out.sh + d));
+            y[e] = __ldcs(reinterpret_cast<const uint4*>(o + u * p.dv + d));
+            if (r) z[e] = __ldcs(reinterpret_cast<const uint4*>(r + u * p.dv + d));
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) {
+          const T *a = reinterpret_cast<const T*>(&x[e]), *b = reinterpret_cast<const T*>(&y[e]), *c = reinterpret_cast<const T*>(&z[e]);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[e] = fmaf(to_f(a[i]), to_f(b[i]) + to_f(c[i]), sum[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < ROWS; ++e) {
+#pragma unroll
+        for (int i = 8; i > 0; i /= 2) sum[e] += __shfl_xor_sync(kFull, sum[e], i);
+        const long long u = u0 + 2 * e + (lane >> 4);
+        if (gl == 0 && u < units) p.d[h[e] * p.BL + t[e]] = sum[e];
+      }
+    }
+    return;
+  }
+  for (long long u = warp; u < units; u += warps) {
+    const long long t = u / p.H;
+    const int h = static_cast<int>(u % p.H);
     float x = 0.f;
-    for (int d = lane; d < p.dv; d += 32) x = fmaf(to_f(g[d]), to_f(o[d]) + (r ? to_f(r[d]) : 0.f), x);
+    for (int d = lane; d < p.dv; d += 32)
+      x = fmaf(to_f(g[t * p.d_out.st + h * p.d_out.sh + d]), to_f(o[u * p.dv + d]) + (r ? to_f(r[u * p.dv + d]) : 0.f), x);
 #pragma unroll
     for (int e = 16; e > 0; e /= 2) x += __shfl_xor_sync(kFull, x, e);
     if (lane == 0) p.d[h * p.BL + t] = x;
@@ -371,8 +423,11 @@ static int run_forward(const Problem& p, cudaStream_t s) {
 
 template <typename T>
 static int run_backward(const Problem& p, bool tc, int dtype, cudaStream_t s) {
-  const long long warps = kPlainThreads / 32, ctas = (p.BL * p.H + warps - 1) / warps;
-  dot_kernel<T><<<static_cast<unsigned>(min(ctas, 148ll * 64)), kPlainThreads, 0, s>>>(p);
+  const long long ctas = (p.BL * p.H + kPlainThreads / 32 - 1) / (kPlainThreads / 32);
+  constexpr int v = 16 / sizeof(T);
+  auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+  const bool vec = p.dv % v == 0 && p.d_out.st % v == 0 && p.d_out.sh % v == 0 && aligned(p.d_out.p) && aligned(p.out) && aligned(p.rest);
+  dot_kernel<T><<<static_cast<unsigned>(min(ctas, 148ll * 16)), kPlainThreads, 0, s>>>(p, vec);
   const int rc = launch_status();
   if (rc != ASCAN_OK) return rc;
   if (tc) return tc_backward(p, dtype, s);

@@ -264,6 +264,15 @@ __device__ __forceinline__ bool misplaced(const unsigned char* smem, uint32_t* e
   return true;
 }
 
+// A place in the ring and the parity of its turn.
+struct Cursor {
+  int at = 0;
+  uint32_t turn = 0;
+  __device__ __forceinline__ void next(int ns) {
+    if (++at == ns) at = 0, turn ^= 1;
+  }
+};
+
 // A value that all lanes have: behind a shuffle the compiler knows it, and keeps
 // what a product is issued with in uniform registers.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFull, x, 0); }
@@ -353,15 +362,6 @@ __device__ __forceinline__ int read_work(const uint32_t* from) {  // -1: none is
       : "memory");
   return got ? static_cast<int>(x) : -1;
 }
-
-// A place in the ring and the parity of its turn.
-struct Cursor {
-  int at = 0;
-  uint32_t turn = 0;
-  __device__ __forceinline__ void next(int ns) {
-    if (++at == ns) at = 0, turn ^= 1;
-  }
-};
 
 __device__ __forceinline__ Item find_item(const Problem& p, const int* ends, int x, int h) {
   Item i;
@@ -752,8 +752,8 @@ template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const int h = blockIdx.y, hk = h / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, threadIdx.x, blockDim.x);
-  const Tile t = find_tile<7>(p, gridDim.x - 1 - blockIdx.x);
+  const Tile t = find_tile_warp<7>(p, gridDim.x - 1 - blockIdx.x);
+  if (t.first < 0) zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, tid, kTcThreads);
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk), g_bytes = tile_bytes(p.dv);
   unsigned char* ring = smem + q_bytes + g_bytes;
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
   const Ctl ctl{&s.c, p.err};
   const int n = t.first / kC + 1, len = min(kC, t.len - t.first);
   const long long at = t.start + t.first;
-  if (tid == 0) {
+  if (tid == 8 * 32) {  // the loading warp's, which need not wait for the others
     bar_init(&s.q_full, 1);
     for (int i = 0; i < ns; ++i) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
     bar_init(&s.dp_full, 1);
@@ -771,6 +771,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     bar_init(&s.c.drain, 1);
     s.c.abort = 0;
     bars_done();
+    bar_expect(&s.q_full, q_bytes + g_bytes);
+    load_tile(smem, &maps.q, p.dk, h, at, &s.q_full);
+    load_tile(smem + q_bytes, &maps.d_out, p.dv, h, at, &s.q_full);
   }
   const uint32_t tm = open_tmem(&s.c);
   constexpr uint32_t kDp = 256, kDq = 384;  // two places of S, then dP and dQ
@@ -827,16 +830,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     }
   } else if (warp == 8) {
     if (lane == 0) {
-      bar_expect(&s.q_full, q_bytes + g_bytes);
-      load_tile(smem, &maps.q, p.dk, h, at, &s.q_full);
-      load_tile(smem + q_bytes, &maps.d_out, p.dv, h, at, &s.q_full);
       int i = 0;
+      Cursor to;
       for (; i < 2 * n; ++i) {
         const bool is_v = i & 1;
-        const int to = i % ns;
-        if (i >= ns && !ctl.wait(&s.empty[to], (i / ns - 1) & 1)) break;
-        bar_expect(&s.full[to], tile_bytes(is_v ? p.dv : p.dk));
-        load_tile(ring + to * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, t.start + (i >> 1) * kC, &s.full[to]);
+        if (!ctl.wait(&s.empty[to.at], to.turn ^ 1)) break;  // a first pass finds all slots empty
+        bar_expect(&s.full[to.at], tile_bytes(is_v ? p.dv : p.dk));
+        load_tile(ring + to.at * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, t.start + (i >> 1) * kC, &s.full[to.at]);
+        to.next(ns);
       }
       if (i < 2 * n) {
         ctl.land(&s.q_full, 0);
@@ -844,40 +845,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
       }
     }
   } else if (warp == 9) {
-    const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dk + 15) / 16 * 16, true, f16<T>());
-    const uint64_t q = desc(smem_u32(smem), 16), g = desc(smem_u32(smem) + q_bytes, 16);
-    auto ring_desc = [&](int i, uint32_t lbo) { return desc(smem_u32(ring) + i % ns * slot, lbo); };
-    auto wait_slot = [&](int i) { return ctl.warp_wait(&s.full[i % ns], (i / ns) & 1); };
-    bool ok = ctl.warp_wait(&s.q_full, 0);
-    for (int j = -1; ok && j < n; ++j) {
-      if (j + 1 < n) {  // the next tile's scores, while the warps are at this one's
-        const int i = 2 * (j + 1);
-        if (!(ok = wait_slot(i))) break;
-        fence_after();
-        if (elect_one()) scores(tm + ((j + 1) & 1) * kC, q, ring_desc(i, 16), id_s, p.dk);
-        if (!(ok = wait_slot(i + 1) && (j < 0 || ctl.warp_wait(&s.dp_free, j & 1)))) break;
-        fence_after();
-        if (elect_one()) {
-          scores(tm + kDp, g, ring_desc(i + 1, 16), id_s, p.dv);
+    if (elect_one()) {  // one thread, without votes
+      const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dk + 15) / 16 * 16, true, f16<T>());
+      const uint64_t q = desc(smem_u32(smem), 16), g = desc(smem_u32(smem) + q_bytes, 16);
+      const uint64_t k0 = desc(smem_u32(ring), 16), o0 = desc(smem_u32(ring), kBlock);
+      Cursor c;
+      int held[2] = {0, 0};  // slots of the keys that a product still has to come for
+      bool ok = ctl.wait(&s.q_full, 0);
+      for (int j = -1; ok && j < n; ++j) {
+        if (j + 1 < n) {  // the next tile's scores, while the warps are at this one's
+          if (!(ok = ctl.wait(&s.full[c.at], c.turn))) break;
+          scores(tm + ((j + 1) & 1) * kC, q, k0 + c.at * (slot >> 4), id_s, p.dk);
+          held[(j + 1) & 1] = c.at;
+          c.next(ns);
+          if (!(ok = ctl.wait(&s.full[c.at], c.turn) && (j < 0 || ctl.wait(&s.dp_free, j & 1)))) break;
+          fence_after();
+          scores(tm + kDp, g, k0 + c.at * (slot >> 4), id_s, p.dv);
           commit(&s.dp_full);
-          commit(&s.empty[(i + 1) % ns]);
+          commit(&s.empty[c.at]);
+          c.next(ns);
         }
-      }
-      if (j < 0) continue;
-      if (!(ok = ctl.warp_wait(&s.ds_ready, j & 1))) break;
-      fence_after();
-      if (elect_one()) {
-        const uint64_t k0 = ring_desc(2 * j, kBlock);
+        if (j < 0) continue;
+        if (!(ok = ctl.wait(&s.ds_ready, j & 1))) break;
+        fence_after();
+        const int at_k = held[j & 1];
         // the warps' halves of dS lie 64 columns apart
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k)
-          mma_tmem(tm + kDq, tm + (j & 1) * kC + (k >> 2) * 64 + (k & 3) * 8, k0 + k * 128, id_o, j + k > 0);
-        commit(&s.empty[2 * j % ns]);
+          mma_tmem(tm + kDq, tm + (j & 1) * kC + (k >> 2) * 64 + (k & 3) * 8, o0 + at_k * (slot >> 4) + k * 128, id_o, j + k > 0);
+        commit(&s.empty[at_k]);
         if (j == n - 1) commit(&s.o_done);
       }
+      commit(&s.c.drain);
+      ctl.land(&s.c.drain, 0);
     }
-    if (elect_one()) commit(&s.c.drain);
-    ctl.land(&s.c.drain, 0);
+  } else if (warp == 10) {
+    zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, lane, 32);
   }
   close_tmem(tm);
 }
@@ -898,9 +901,11 @@ template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const int hk = blockIdx.y, heads = p.H / p.share, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC, threadIdx.x, blockDim.x);
-  zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC, threadIdx.x, blockDim.x);
-  const Tile t = find_tile<7>(p, blockIdx.x);  // a sequence's first keys have the most queries
+  const Tile t = find_tile_warp<7>(p, blockIdx.x);  // a sequence's first keys have the most queries
+  if (t.first < 0) {
+    zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC, tid, kTcThreads);
+    zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC, tid, kTcThreads);
+  }
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int k_bytes = tile_bytes(p.dk), v_bytes = tile_bytes(p.dv);
   unsigned char *q_ring = smem + k_bytes + v_bytes, *g_ring = q_ring + 2 * k_bytes, *pt = g_ring + 2 * v_bytes;
@@ -909,7 +914,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
   const int blocks = (t.len - t.first + kC - 1) / kC, len = min(kC, t.len - t.first);
   const int total = blocks * p.share;  // tiles of queries, head by head
   const long long at = t.start + t.first;
-  if (tid == 0) {
+  if (tid == 8 * 32) {  // the loading warp's, which need not wait for the others
     bar_init(&s.kv_full, 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(&s.q_full[i], 1);
@@ -930,6 +935,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
     s.c.abort = 0;
     s.bad = 0;
     bars_done();
+    bar_expect(&s.kv_full, k_bytes + v_bytes);
+    load_tile(smem, &maps.k, p.dk, hk, at, &s.kv_full);
+    load_tile(smem + k_bytes, &maps.v, p.dv, hk, at, &s.kv_full);
   }
   const uint32_t tm = open_tmem(&s.c);
   constexpr uint32_t kDp = 128, kDv = 256, kDk = 384;
@@ -1038,9 +1046,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
     }
   } else if (warp == 8) {
     if (lane == 0) {
-      bar_expect(&s.kv_full, k_bytes + v_bytes);
-      load_tile(smem, &maps.k, p.dk, hk, at, &s.kv_full);
-      load_tile(smem + k_bytes, &maps.v, p.dv, hk, at, &s.kv_full);
       int q_loads = 0, g_loads = 0;
       for (int i = 0, b = 0, h = hk * p.share; i < total; ++i) {
         const int u = i & 1;
@@ -1062,38 +1067,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
       }
     }
   } else if (warp == 9) {
-    const uint32_t id_s = idesc(kC, false, f16<T>()), id_k = idesc((p.dk + 15) / 16 * 16, true, f16<T>()),
-                   id_v = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
-    const uint64_t k = desc(smem_u32(smem), 16), v = desc(smem_u32(smem) + k_bytes, 16), a = desc(smem_u32(pt), 16);
-    auto q_desc = [&](int u, uint32_t lbo) { return desc(smem_u32(q_ring) + u * k_bytes, lbo); };
-    auto g_desc = [&](int u, uint32_t lbo) { return desc(smem_u32(g_ring) + u * v_bytes, lbo); };
-    bool ok = ctl.warp_wait(&s.kv_full, 0);
-    for (int i = -1; ok && i < total; ++i) {
-      const bool more = i + 1 < total;
-      const int u = i & 1, nu = (i + 1) & 1;
-      if (more) {
-        if (!(ok = ctl.warp_wait(&s.q_full[nu], ((i + 1) >> 1) & 1) && (i < 0 || ctl.warp_wait(&s.s_free, i & 1)))) break;
-        fence_after();
-        if (elect_one()) {
-          scores(tm, k, q_desc(nu, 16), id_s, p.dk);
+    if (elect_one()) {  // one thread, without votes
+      const uint32_t id_s = idesc(kC, false, f16<T>()), id_k = idesc((p.dk + 15) / 16 * 16, true, f16<T>()),
+                     id_v = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
+      const uint64_t k = desc(smem_u32(smem), 16), v = desc(smem_u32(smem) + k_bytes, 16), a = desc(smem_u32(pt), 16);
+      const uint64_t q0 = desc(smem_u32(q_ring), 16), g0 = desc(smem_u32(g_ring), 16);                    // for scores
+      const uint64_t q1 = desc(smem_u32(q_ring), kBlock), g1 = desc(smem_u32(g_ring), kBlock);            // as values
+      bool ok = ctl.wait(&s.kv_full, 0);
+      for (int i = -1; ok && i < total; ++i) {
+        const bool more = i + 1 < total;
+        const int u = i & 1, nu = (i + 1) & 1;
+        if (more) {
+          if (!(ok = ctl.wait(&s.q_full[nu], ((i + 1) >> 1) & 1) && (i < 0 || ctl.wait(&s.s_free, i & 1)))) break;
+          fence_after();
+          scores(tm, k, q0 + nu * (k_bytes >> 4), id_s, p.dk);
           commit(&s.s_full);
         }
-      }
-      if (i >= 0) {
-        if (!(ok = ctl.warp_wait(&s.p_ready, i & 1))) break;
-        fence_after();
-        if (elect_one()) {
-          const uint64_t g = g_desc(u, kBlock);
+        if (i >= 0) {
+          if (!(ok = ctl.wait(&s.p_ready, i & 1))) break;
+          fence_after();
+          const uint64_t g = g1 + u * (v_bytes >> 4), q = q1 + u * (k_bytes >> 4);
 #pragma unroll
           for (int e = 0; e < kC / 16; ++e)
             mma_smem(tm + kDv, a + (e >> 2) * (kBlock >> 4) + (e & 3) * 2, g + e * 128, id_v, i + e > 0);
           commit(&s.p_free);
           commit(&s.g_empty[u]);
-        }
-        if (!(ok = ctl.warp_wait(&s.ds_ready, i & 1))) break;
-        fence_after();
-        if (elect_one()) {
-          const uint64_t q = q_desc(u, kBlock);
+          if (!(ok = ctl.wait(&s.ds_ready, i & 1))) break;
+          fence_after();
           // the warps' halves of dS lie 64 columns apart
 #pragma unroll
           for (int e = 0; e < kC / 16; ++e)
@@ -1101,18 +1101,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
           commit(&s.q_empty[u]);
           if (!more) commit(&s.o_done);
         }
-      }
-      if (more) {
-        if (!(ok = ctl.warp_wait(&s.g_full[nu], ((i + 1) >> 1) & 1))) break;
-        fence_after();
-        if (elect_one()) {
-          scores(tm + kDp, v, g_desc(nu, 16), id_s, p.dv);
+        if (more) {
+          if (!(ok = ctl.wait(&s.g_full[nu], ((i + 1) >> 1) & 1))) break;
+          scores(tm + kDp, v, g0 + nu * (v_bytes >> 4), id_s, p.dv);
           commit(&s.dp_full);
         }
       }
+      commit(&s.c.drain);
+      ctl.land(&s.c.drain, 0);
     }
-    if (elect_one()) commit(&s.c.drain);
-    ctl.land(&s.c.drain, 0);
   } else if (warp == 10) {
     for (int i = 0, b = 0, h = hk * p.share; i < total; ++i) {
       const int u = i & 1;
@@ -1130,6 +1127,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
       warp_arrive(&s.stat_full[u]);
       if (++b == blocks) b = 0, ++h;
     }
+  } else {
+    zero_outside<T>(p, p.d_k, hk, heads, p.dk, blockIdx.x, kC, lane, 32);
+    zero_outside<T>(p, p.d_v, hk, heads, p.dv, blockIdx.x, kC, lane, 32);
   }
   close_tmem(tm);
 }
