@@ -22,6 +22,7 @@ much to a result as its own rounding does.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -226,6 +227,21 @@ def _check_cache_sizes(keys, values) -> None:
     raise ValueError(f"a cache has between 1 and 65535 heads, got {keys.shape[1]}")
 
 
+def _usual_cache(cache, device, heads: int, key_dim: int):
+  """Value size of a cache that passes _check_cache, in one expression; None sends the caller there."""
+  keys, values, key_scales, value_scales = cache
+  (pages, h, page, dk), (pv, hv, page_v, dv) = keys.shape, values.shape
+  return dv if (
+    keys.device == device and values.device == device and key_scales.device == device
+    and value_scales.device == device and keys.dtype == CACHE_DTYPE and values.dtype == CACHE_DTYPE
+    and key_scales.dtype == torch.float32 and value_scales.dtype == torch.float32 and pv == pages
+    and hv == h and page_v == page and h > 0 and heads % h == 0 and dk == key_dim and not dk % 16
+    and not dv % 16 and not page % 16 and 0 < dk <= MAX_DIM and 0 < dv <= MAX_DIM
+    and 0 < page <= MAX_PAGE and h <= 65535 and key_scales.shape == (pages, h)
+    and value_scales.shape == (pages, h) and keys.is_contiguous() and values.is_contiguous()
+    and key_scales.is_contiguous() and value_scales.is_contiguous()) else None
+
+
 def _check_cache(cache, device):
   """The cache's four tensors."""
   try:
@@ -276,6 +292,38 @@ def _refuse_gradients(name: str, *tensors: torch.Tensor) -> None:
     raise ValueError(f"{name} has no backward; use attention_causal, or torch.no_grad()")
 
 
+def _check_write(keys, values, cache, pages, starts, cu_seqlens):
+  """Tokens, requests and pages in a row."""
+  try:  # the usual call in a few expressions; whatever fails them is looked at below
+    (tokens, heads, dim), (batch, width), device = keys.shape, pages.shape, keys.device
+    value_dim = _usual_cache(cache, device, heads, dim)
+    if (value_dim and keys.is_cuda and keys.dtype in DTYPE_CODES and values.device == device
+        and values.dtype == keys.dtype and values.shape == (tokens, heads, value_dim)
+        and heads == cache[0].shape[1] and keys.stride(2) == 1 and values.stride(2) == 1
+        and pages.device == device and starts.device == device and cu_seqlens.device == device
+        and pages.dtype == torch.int32 and starts.dtype in INDEX_CODES
+        and cu_seqlens.dtype in INDEX_CODES and batch <= 65535 and tokens <= MAX_TOKENS
+        and starts.shape == (batch,) and cu_seqlens.shape == (batch + 1,) and pages.is_contiguous()
+        and starts.is_contiguous() and cu_seqlens.is_contiguous()):
+      return tokens, batch, width
+  except (AttributeError, TypeError, ValueError):
+    pass
+  _check_rows("keys", keys, None, None)
+  device, tokens = keys.device, keys.shape[0]
+  tensors = _check_cache(cache, device)
+  _check_rows("keys", keys, device, None, None, tensors[0].shape[3])
+  _check_rows("values", values, device, keys.dtype, tokens, tensors[1].shape[3])
+  for name, t in (("keys", keys), ("values", values)):
+    if t.shape[1] != tensors[0].shape[1]:
+      raise ValueError(f"{name} has {t.shape[1]} heads, the cache {tensors[0].shape[1]}")
+  batch, width = _check_pages(pages, device)
+  _check_index("starts", starts, device, batch)
+  _check_index("cu_seqlens", cu_seqlens, device, batch + 1)
+  if tokens > MAX_TOKENS:
+    raise ValueError(f"at most {MAX_TOKENS} tokens are supported")
+  return tokens, batch, width
+
+
 def attention_cache_write(
   keys: torch.Tensor,
   values: torch.Tensor,
@@ -305,20 +353,9 @@ def attention_cache_write(
   """
   _refuse_gradients("attention_cache_write", keys, values)
   _refuse_tangents(ValueError, "attention_cache_write", keys, values)
-  _check_rows("keys", keys, None, None)
-  device, tokens = keys.device, keys.shape[0]
-  tensors = _check_cache(cache, device)
-  _check_rows("keys", keys, device, None, None, tensors[0].shape[3])
-  _check_rows("values", values, device, keys.dtype, tokens, tensors[1].shape[3])
-  for name, t in (("keys", keys), ("values", values)):
-    if t.shape[1] != tensors[0].shape[1]:
-      raise ValueError(f"{name} has {t.shape[1]} heads, the cache {tensors[0].shape[1]}")
-  batch, width = _check_pages(pages, device)
-  _check_index("starts", starts, device, batch)
-  _check_index("cu_seqlens", args["cu_seqlens"], device, batch + 1)
   cu_seqlens = args["cu_seqlens"]
-  if tokens > MAX_TOKENS:
-    raise ValueError(f"at most {MAX_TOKENS} tokens are supported")
+  tokens, batch, width = _check_write(keys, values, cache, pages, starts, cu_seqlens)
+  device, tensors = keys.device, tuple(cache)
   _lib._enable_error_flag()
   if tokens == 0 or batch == 0:
     return
@@ -331,6 +368,38 @@ def attention_cache_write(
   for t in tensors:
     torch.autograd.graph.increment_version(t)
   _lib._finish(rc, "ascan_cache_write", device)
+
+
+@functools.lru_cache(maxsize=256)
+def _step_workspace(batch: int, value_dim: int) -> int:
+  return _lib.load().ascan_cache_step_workspace(batch, value_dim)
+
+
+def _check_step(queries, cache, pages, lengths):
+  """Requests, heads, head size, value size and pages in a row."""
+  try:  # the usual call in a few expressions; whatever fails them is looked at below
+    (batch, heads, dim), (rows, width), device = queries.shape, pages.shape, queries.device
+    value_dim = _usual_cache(cache, device, heads, dim)
+    if (value_dim and queries.is_cuda and queries.dtype in DTYPE_CODES and 0 < heads <= 65535
+        and queries.stride(2) == 1 and pages.device == device and lengths.device == device
+        and pages.dtype == torch.int32 and lengths.dtype in INDEX_CODES and rows == batch <= 65535
+        and lengths.shape == (batch,) and pages.is_contiguous() and lengths.is_contiguous()):
+      return batch, heads, dim, value_dim, width
+  except (AttributeError, TypeError, ValueError):
+    pass
+  _check_rows("queries", queries, None, None)
+  device, (batch, heads, dim) = queries.device, queries.shape
+  tensors = _check_cache(cache, device)
+  (_, cache_heads, _, key_dim), value_dim = tensors[0].shape, tensors[1].shape[3]
+  if dim != key_dim:
+    raise ValueError(f"queries have head size {dim}, the cache {key_dim}")
+  if heads % cache_heads:
+    raise ValueError(f"the cache's {cache_heads} heads do not divide the queries' {heads}")
+  rows, width = _check_pages(pages, device)
+  if rows != batch:
+    raise ValueError(f"pages has {rows} rows, expected {batch}")
+  _check_index("lengths", lengths, device, batch)
+  return batch, heads, dim, value_dim, width
 
 
 def attention_cache_step(
@@ -356,18 +425,8 @@ def attention_cache_step(
   """
   _refuse_gradients("attention_cache_step", queries)
   _refuse_tangents(ValueError, "attention_cache_step", queries)
-  _check_rows("queries", queries, None, None)
-  device, (batch, heads, dim) = queries.device, queries.shape
-  tensors = _check_cache(cache, device)
-  (_, cache_heads, _, key_dim), value_dim = tensors[0].shape, tensors[1].shape[3]
-  if dim != key_dim:
-    raise ValueError(f"queries have head size {dim}, the cache {key_dim}")
-  if heads % cache_heads:
-    raise ValueError(f"the cache's {cache_heads} heads do not divide the queries' {heads}")
-  rows, width = _check_pages(pages, device)
-  if rows != batch:
-    raise ValueError(f"pages has {rows} rows, expected {batch}")
-  _check_index("lengths", lengths, device, batch)
+  batch, heads, dim, value_dim, width = _check_step(queries, cache, pages, lengths)
+  device, tensors = queries.device, tuple(cache)
   scale = _check_scale(scale, dim)
   _lib._enable_error_flag()
   out = torch.empty((batch, heads, value_dim), dtype=queries.dtype, device=device)
@@ -375,8 +434,7 @@ def attention_cache_step(
     return out
   lib = _lib.load()
   with _on(device):
-    ws = torch.empty(lib.ascan_cache_step_workspace(batch, value_dim), dtype=torch.uint8,
-                     device=device)
+    ws = torch.empty(_step_workspace(batch, value_dim), dtype=torch.uint8, device=device)
     rc = lib.ascan_cache_step(
       *_rows(queries), _native_cache(tensors), pages.data_ptr(), batch, width, lengths.data_ptr(),
       INDEX_CODES[lengths.dtype], DTYPE_CODES[queries.dtype], scale, out.data_ptr(), ws.data_ptr(),

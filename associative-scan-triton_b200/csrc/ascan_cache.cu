@@ -83,12 +83,9 @@ __device__ __forceinline__ int scale_bits(float top) {
   return max(-kScaleBits, min(kScaleBits, e));
 }
 
-// Four values to e4m3, to nearest; infinities and NaN become its NaN, finite
-// values beyond the largest scale's reach its largest.
-__device__ __forceinline__ uint32_t pack4(const float* x) {
-  float y[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = fabsf(x[i]) < INFINITY ? x[i] : NAN;
+// Four values to e4m3, to nearest; NaN becomes its NaN, what lies beyond the
+// scale's reach (infinities too) its largest value.
+__device__ __forceinline__ uint32_t pack4(const float* y) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
@@ -108,110 +105,181 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
   return pack4(v);
 }
 
-// Eight elements as floats.
+// Eight elements as they lie in memory, and as floats.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float* x) {
-  if (vec) {
-    constexpr int N = sizeof(T) == 4 ? 4 : 8;
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; i += N) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + i));
-      const T* e = reinterpret_cast<const T*>(&u);
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-      for (int q = 0; q < N; ++q) x[i + q] = to_f(e[q]);
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
   }
-}
+  __device__ __forceinline__ float operator[](int i) const { return to_f(reinterpret_cast<const T*>(w)[i]); }
+  // The largest magnitude, infinities included, NaN not.
+  __device__ __forceinline__ float largest() const {
+    if (sizeof(T) == 4) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf((*this)[i]));
+      return m;
+    }
+    const uint32_t e[4] = {w[0].x & 0x7fff7fffu, w[0].y & 0x7fff7fffu, w[0].z & 0x7fff7fffu, w[0].w & 0x7fff7fffu};
+    using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    auto as = [&](int i) { return *reinterpret_cast<const Pair*>(&e[i]); };
+    const Pair m = __hmax2(__hmax2(as(0), as(1)), __hmax2(as(2), as(3)));
+    const float x = to_f(m.x), y = to_f(m.y);
+    return fmaxf(x == x ? x : 0.f, y == y ? y : 0.f);
+  }
+};
 
 // A group of G threads writes what one request adds to one page of one head:
-// the largest magnitude first, which gives the scale, then the rounded values
-// (read again, out of the nearest cache).
+// the largest magnitude first, which gives the scale, then the rounded values.
+// Up to HOLD vectors of eight elements a thread stay in registers in between
+// (16-bit: a page of 64 tokens of 128 in all); of longer pieces the rest is read
+// again.  More in registers would leave room for fewer groups an SM, and it is
+// their number that hides the reads in front.
+// Memory and the chain of dependent reads in front of it (request, page, scale)
+// bound it: 16384 tokens of 4 heads of 128 took 27 us with every vector read
+// twice, one after the other.
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ WriteArgs a, int vec_k, int vec_v) {
+__global__ void __launch_bounds__(kThreads, 5) write_kernel(const __grid_constant__ WriteArgs a, int vec_k, int vec_v) {
   constexpr int UNITS = kThreads / G;
+  constexpr int HOLD = sizeof(T) == 4 ? 2 : (G == 32 ? 2 : 4);
   const Cache& c = a.c;
-  const int gl = threadIdx.x % G, sub = threadIdx.x / G;
+  const int gl = threadIdx.x % G, sub = threadIdx.x / G, lane = threadIdx.x & 31;
   if (blockIdx.x == 0) {
     if (a.cu64) validate_cu(static_cast<const int64_t*>(a.cu), c.B, a.BL, a.err);
     else validate_cu(static_cast<const int32_t*>(a.cu), c.B, a.BL, a.err);
   }
   const long long unit = static_cast<long long>(blockIdx.x) * UNITS + sub;
   if (unit >= a.units) return;  // whole groups
-  const bool is_v = unit & 1;
-  const int h = static_cast<int>((unit >> 1) % c.heads);
-  const long long x = (unit >> 1) / c.heads;  // piece number
-  auto cu_at = [&](long long i) {
+  const int half = static_cast<int>(unit) & 1, h = static_cast<int>(unit >> 1) % c.heads;
+  const int x = static_cast<int>(unit >> 1) / c.heads;  // piece number
+  auto cu_at = [&](int i) {
     const long long v = index_at(a.cu, a.cu64, i);
-    return v < 0 ? 0ll : (v > a.BL ? a.BL : v);
+    return static_cast<int>(v < 0 ? 0ll : (v > a.BL ? a.BL : v));
   };
   // pieces of request b start at cu[b] / page + 2 b: no more than its tokens
-  // fill and two that they begin and end in
-  long long lo = 0, hi = c.B - 1;
-  while (lo < hi) {
-    const long long mid = (lo + hi + 1) >> 1;
-    if (cu_at(mid) / c.page + 2 * mid <= x) lo = mid;
-    else hi = mid - 1;
+  // fill and two that they begin and end in.  A warp looks at thirty-two
+  // requests at once.
+  int b = 0;
+  for (int n = static_cast<int>(c.B); n > 1;) {
+    const int step = (n + 31) / 32, i = b + lane * step;
+    const bool in = lane * step < n && cu_at(i) / c.page + 2 * i <= x;
+    const int ahead = max(__popc(__ballot_sync(kFull, in)), 1) - 1;
+    b += ahead * step;
+    n = min(step, n - ahead * step);
   }
-  const long long b = lo, c0 = cu_at(b), len = cu_at(b + 1) - c0, start = index_at(a.starts, a.starts64, b);
-  if (start < 0 || len <= 0) return;  // no request, or nothing new
-  const long long place = start / c.page + (x - c0 / c.page - 2 * b);
-  const long long from = max(start, place * c.page), to = min(start + len, (place + 1) * c.page);
-  if (from >= to) return;
-  long long id = -1;
-  if (place < c.width) id = c.table[b * c.width + place];
+  const int c0 = cu_at(b), len = cu_at(b + 1) - c0;
+  const long long begin = index_at(a.starts, a.starts64, b);
+  if (begin < 0 || len <= 0) return;  // no request, or nothing new
+  int id = -1, place = 0, from = 0, to = 0;
+  if (begin < 0x3fff0000) {  // what follows stays below 2^31
+    const int start = static_cast<int>(begin);
+    place = start / c.page + (x - c0 / c.page - 2 * b);
+    from = max(start, place * c.page), to = min(start + len, (place + 1) * c.page);
+    if (place < 0 || from >= to) return;
+    if (place < c.width) id = c.table[b * c.width + place];
+  }
   if (id < 0 || id >= c.pages) {
     if (gl == 0) report(ASCAN_DEV_ERR_INDEX, static_cast<unsigned long long>(b), a.err);
     return;
   }
-  const int dim = is_v ? c.dv : c.dk, first = static_cast<int>(from - place * c.page), n = static_cast<int>(to - from);
+  const bool is_v = half != 0;
+  const int dim = is_v ? c.dv : c.dk, first = from - place * c.page, n = to - from;
   const bool vec = is_v ? vec_v : vec_k;
   const Rows& r = a.x[is_v];
-  const T* src = static_cast<const T*>(r.p) + (c0 + from - start) * r.st + h * r.sh;
-  uint8_t* dst = (is_v ? c.v : c.k) + ((id * c.heads + h) * c.page) * dim;
-  float* scale = (is_v ? c.vs : c.ks) + id * c.heads + h;
+  const T* src = static_cast<const T*>(r.p) + (c0 + from - static_cast<long long>(begin)) * r.st + h * r.sh;
+  uint8_t* dst = (is_v ? c.v : c.k) + ((static_cast<long long>(id) * c.heads + h) * c.page + first) * dim;
+  float* scale = (is_v ? c.vs : c.ks) + static_cast<long long>(id) * c.heads + h;
+  const float held = first > 0 ? *scale : 0.f;
   const int per_row = dim / 8, work = n * per_row;
-  float top = 0.f;
-  for (int e = gl; e < work; e += G) {
-    float v[8];
-    load8(src + (e / per_row) * r.st + (e % per_row) * 8, vec, v);
+  // vector gl + G k of the piece is vector `col` of row `row`
+  const int step_row = G / per_row, step_col = G % per_row;
+  auto advance = [&](int& row, int& col) {
+    row += step_row, col += step_col;
+    if (col >= per_row) col -= per_row, ++row;
+  };
+  const int row0 = gl / per_row, col0 = gl % per_row;
+  Eight<T> kept[HOLD];
+  int row = row0, col = col0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float m = fabsf(v[q]);
-      if (m < INFINITY) top = fmaxf(top, m);
-    }
+  for (int k = 0; k < HOLD; ++k) {
+    if (gl + G * k < work) kept[k].load(src + row * r.st + col * 8, vec);
+    advance(row, col);
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k)
+    if (gl + G * k < work) top = fmaxf(top, kept[k].largest());
+  for (int e = gl + G * HOLD; e < work; e += G) {
+    Eight<T> v;
+    v.load(src + row * r.st + col * 8, vec);
+    top = fmaxf(top, v.largest());
+    advance(row, col);
   }
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-  const float held = first > 0 ? *scale : 0.f;
   if (G > 32) {
     __shared__ float tops[G / 32];
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    if (lane == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();  // everyone has read the scale too
 #pragma unroll
     for (int w = 0; w < G / 32; ++w) top = fmaxf(top, tops[w]);
   } else {
     __syncwarp();
   }
+  const bool infinite = top == INFINITY;
+  if (infinite) {  // the largest that is not, by every warp of the group alike
+    top = 0.f;
+    for (int e = lane; e < work; e += 32) {
+      Eight<T> v;
+      v.load(src + e / per_row * r.st + e % per_row * 8, vec);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (fabsf(v[q]) < INFINITY) top = fmaxf(top, fabsf(v[q]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+  }
   const float need = fmaxf(pow2(scale_bits(top)), held);
   if (first > 0 && need > held) {  // what the page holds moves to the larger scale
     const float f = held / need;
+    uint4* old = reinterpret_cast<uint4*>(dst - first * dim);
     for (int e = gl; e < first * dim / 16; e += G) {
-      uint4 w = reinterpret_cast<uint4*>(dst)[e];
+      uint4 w = old[e];
       w.x = rescale4(w.x, f), w.y = rescale4(w.y, f), w.z = rescale4(w.z, f), w.w = rescale4(w.w, f);
-      reinterpret_cast<uint4*>(dst)[e] = w;
+      old[e] = w;
     }
   }
   if (gl == 0 && need != held) *scale = need;
   const float inv = 1.f / need;
-  for (int e = gl; e < work; e += G) {
-    float v[8];
-    load8(src + (e / per_row) * r.st + (e % per_row) * 8, vec, v);
+  auto put = [&](const Eight<T>& v, int e) {
+    float y[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] *= inv;
-    *reinterpret_cast<uint2*>(dst + (first + e / per_row) * dim + (e % per_row) * 8) = make_uint2(pack4(v), pack4(v + 4));
+    for (int q = 0; q < 8; ++q) y[q] = v[q] * inv;
+    if (infinite) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[q] = fabsf(y[q]) < INFINITY ? y[q] : NAN;
+    }
+    reinterpret_cast<uint2*>(dst)[e] = make_uint2(pack4(y), pack4(y + 4));
+  };
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k)
+    if (gl + G * k < work) put(kept[k], gl + G * k);
+  row = row0, col = col0;
+  for (int k = 0; k < HOLD; ++k) advance(row, col);
+  for (int e = gl + G * HOLD; e < work; e += G) {
+    Eight<T> v;
+    v.load(src + row * r.st + col * 8, vec);
+    put(v, e);
+    advance(row, col);
   }
 }
 
@@ -437,6 +505,7 @@ __global__ void __launch_bounds__(kStepThreads, sizeof(T) == 4 ? 2 : kCtasPerSm)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async();
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Found f = find_request(a, groups, scratch);  // and all threads have met
   const long long run = f.total / gridDim.x, more = f.total % gridDim.x;
   const long long begin = run * blockIdx.x + min(more, static_cast<long long>(blockIdx.x));
@@ -727,6 +796,7 @@ __global__ void __launch_bounds__(128 * Z) join_kernel(const __grid_constant__ S
   __shared__ float s_m[Z], s_l[Z], s_x[Z][128];
   const long long b = blockIdx.y;
   const int h = blockIdx.x, z = threadIdx.x >> 7, d = threadIdx.x & 127;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long n = a.before[b], tiles = a.before[b + 1] - n;
   const int groups = c.heads * a.row_tiles, row = h % a.share % 16;
   const long long total = a.before[c.B] * groups;
@@ -814,6 +884,22 @@ static int pick_step(const StepArgs& a, const StepMaps& m, int ctas, cudaStream_
   return a.c.dv > 64 ? launch_step<T, 1, 16, R>(a, m, ctas, s) : launch_step<T, 1, 8, R>(a, m, ctas, s);
 }
 
+// Launched while the step still runs: its CTAs are set up as the step's end, and
+// wait for all that the step wrote.
+template <typename T, int Z>
+static int join(const StepArgs& a, int ctas, dim3 grid, cudaStream_t s) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(128 * Z);
+  config.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, join_kernel<T, Z>, a, ctas) == cudaSuccess ? launch_status() : ASCAN_ECUDA;
+}
+
 template <typename T>
 static int step(const StepArgs& a, const StepMaps& m, cudaStream_t s) {
   const int ctas = 148 * (sizeof(T) == 4 ? 2 : kCtasPerSm);
@@ -821,9 +907,8 @@ static int step(const StepArgs& a, const StepMaps& m, cudaStream_t s) {
   if (rc != ASCAN_OK) return rc;
   // a row of a few requests lies in many CTAs' parts, one of many in one or two
   const dim3 grid(a.H, static_cast<unsigned>(a.c.B));
-  if (a.c.B * a.c.heads * a.row_tiles * 4 < ctas) join_kernel<T, 4><<<grid, 512, 0, s>>>(a, ctas);
-  else join_kernel<T, 1><<<grid, 128, 0, s>>>(a, ctas);
-  return launch_status();
+  if (a.c.B * a.c.heads * a.row_tiles * 4 < ctas) return join<T, 8>(a, ctas, grid, s);
+  return join<T, 1>(a, ctas, grid, s);
 }
 
 // A pool without pages: every row is zero, and one with tokens an error.
