@@ -9,6 +9,7 @@
 // them: a tile of scores of heads of 128 is 64 of them for each 8 loads.
 #include "ascan_impl.cuh"
 #include "ascan_attend.cuh"
+#include "ascan_pairs.cuh"
 
 namespace ascan {
 namespace attend {
@@ -23,48 +24,66 @@ __device__ __forceinline__ void check_cu(const Problem& p) {
 }
 
 // 64 rows of one head as floats; rows from `len` on and columns from `dim` on
-// are zeros.
+// are zeros.  float32 rows at 16 bytes are copied four elements at a time, past
+// the registers: `wait_tiles` comes before they are read.
 template <typename T, int D>
 __device__ __forceinline__ void load_tile(float* to, const Rows& r, int head, long long token, int len, int dim) {
   const T* src = static_cast<const T*>(r.p) + token * r.st + head * r.sh;
+  if (sizeof(T) == 4 && dim % 4 == 0 && r.st % 4 == 0 && r.sh % 4 == 0 && (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0) {
+    const int d = threadIdx.x % (D / 4) * 4;
+#pragma unroll
+    for (int i = threadIdx.x / (D / 4); i < kR; i += kPlainThreads / (D / 4)) {
+      const int bytes = i < len && d < dim ? 16 : 0;  // the rest of the sixteen is filled with zeros
+      const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to + i * (D + 4) + d));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(bytes ? src + i * r.st + d : src), "r"(bytes) : "memory");
+    }
+    return;
+  }
   for (int e = threadIdx.x; e < kR * D; e += kPlainThreads) {
     const int i = e / D, d = e % D;
     to[i * (D + 4) + d] = i < len && d < dim ? to_f(src[i * r.st + d]) : 0.f;
   }
 }
+__device__ __forceinline__ void wait_tiles() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+}
 
-// s[a][b] = x[row ty*4+a] . y[row tx+16b]
+// s[a][b] = x[row ty*4+a] . y[row tx+16b], two elements an instruction
 template <int D>
 __device__ __forceinline__ void dots(const float* x, const float* y, int tx, int ty, int dim, float (&s)[4][4]) {
+  uint64_t acc[4][4];
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
-    for (int b = 0; b < 4; ++b) s[a][b] = 0.f;
+    for (int b = 0; b < 4; ++b) acc[a][b] = 0;
   const float* xr = x + ty * 4 * (D + 4);
   const float* yr = y + tx * (D + 4);
 #pragma unroll 4
   for (int d = 0; d < dim; d += 4) {
-    float4 u[4], v[4];
+    ulonglong2 u[4], v[4];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) u[a] = *reinterpret_cast<const float4*>(xr + a * (D + 4) + d);
+    for (int a = 0; a < 4; ++a) u[a] = *reinterpret_cast<const ulonglong2*>(xr + a * (D + 4) + d);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) v[b] = *reinterpret_cast<const float4*>(yr + 16 * b * (D + 4) + d);
+    for (int b = 0; b < 4; ++b) v[b] = *reinterpret_cast<const ulonglong2*>(yr + 16 * b * (D + 4) + d);
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        s[a][b] = fmaf(u[a].x, v[b].x, s[a][b]);
-        s[a][b] = fmaf(u[a].y, v[b].y, s[a][b]);
-        s[a][b] = fmaf(u[a].z, v[b].z, s[a][b]);
-        s[a][b] = fmaf(u[a].w, v[b].w, s[a][b]);
-      }
+      for (int b = 0; b < 4; ++b) acc[a][b] = fma2(u[a].y, v[b].y, fma2(u[a].x, v[b].x, acc[a][b]));
   }
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float2 f = unpair(acc[a][b]);
+      s[a][b] = f.x + f.y;
+    }
 }
 
-// acc[a][..] += sum_k w[row ty*4+a][k] y[k][..], columns tx*4 + 64 c.  With
-// `causal` a row takes k up to its own only (what lies behind may be NaN).
+// acc[a][..] += sum_k w[row ty*4+a][k] y[k][..], columns tx*4 + 64 c, in pairs.
+// With `causal` a row takes k up to its own only (what lies behind may be NaN).
 template <int D, bool CAUSAL>
-__device__ __forceinline__ void rows_times(const float* w, const float* y, int tx, int ty, float (&acc)[4][D / 16]) {
+__device__ __forceinline__ void rows_times(const float* w, const float* y, int tx, int ty, uint64_t (&acc)[4][D / 32]) {
 #pragma unroll 2
   for (int k = 0; k < kR; k += 4) {
     float4 p[4];
@@ -74,15 +93,14 @@ __device__ __forceinline__ void rows_times(const float* w, const float* y, int t
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        const float4 v = *reinterpret_cast<const float4*>(y + (k + e) * (D + 4) + tx * 4 + 64 * c);
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(y + (k + e) * (D + 4) + tx * 4 + 64 * c);
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           if (CAUSAL && k + e > ty * 4 + a) continue;
           const float f = e == 0 ? p[a].x : (e == 1 ? p[a].y : (e == 2 ? p[a].z : p[a].w));
-          acc[a][4 * c] = fmaf(f, v.x, acc[a][4 * c]);
-          acc[a][4 * c + 1] = fmaf(f, v.y, acc[a][4 * c + 1]);
-          acc[a][4 * c + 2] = fmaf(f, v.z, acc[a][4 * c + 2]);
-          acc[a][4 * c + 3] = fmaf(f, v.w, acc[a][4 * c + 3]);
+          const uint64_t f2 = pair(f, f);
+          acc[a][2 * c] = fma2(f2, v.x, acc[a][2 * c]);
+          acc[a][2 * c + 1] = fma2(f2, v.y, acc[a][2 * c + 1]);
         }
       }
   }
@@ -91,21 +109,19 @@ __device__ __forceinline__ void rows_times(const float* w, const float* y, int t
 // acc[a][..] += sum_k w[k][column ty*4+a] y[k][..]; with `causal` a column
 // takes k from its own on.
 template <int D, bool CAUSAL>
-__device__ __forceinline__ void columns_times(const float* w, const float* y, int tx, int ty, float (&acc)[4][D / 16]) {
+__device__ __forceinline__ void columns_times(const float* w, const float* y, int tx, int ty, uint64_t (&acc)[4][D / 32]) {
 #pragma unroll 4
   for (int k = 0; k < kR; ++k) {
     const float4 p = *reinterpret_cast<const float4*>(w + k * kPs + ty * 4);
-    const float f[4] = {p.x, p.y, p.z, p.w};
+    const uint64_t f[4] = {pair(p.x, p.x), pair(p.y, p.y), pair(p.z, p.z), pair(p.w, p.w)};
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-      const float4 v = *reinterpret_cast<const float4*>(y + k * (D + 4) + tx * 4 + 64 * c);
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(y + k * (D + 4) + tx * 4 + 64 * c);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
         if (CAUSAL && k < ty * 4 + a) continue;
-        acc[a][4 * c] = fmaf(f[a], v.x, acc[a][4 * c]);
-        acc[a][4 * c + 1] = fmaf(f[a], v.y, acc[a][4 * c + 1]);
-        acc[a][4 * c + 2] = fmaf(f[a], v.z, acc[a][4 * c + 2]);
-        acc[a][4 * c + 3] = fmaf(f[a], v.w, acc[a][4 * c + 3]);
+        acc[a][2 * c] = fma2(f[a], v.x, acc[a][2 * c]);
+        acc[a][2 * c + 1] = fma2(f[a], v.y, acc[a][2 * c + 1]);
       }
     }
   }
@@ -113,15 +129,17 @@ __device__ __forceinline__ void columns_times(const float* w, const float* y, in
 
 template <typename T, int D>
 __device__ __forceinline__ void store_rows(void* to, int head, int heads, long long token, int len, int dim, int tx, int ty,
-                                           const float (&acc)[4][D / 16], const float (&f)[4]) {
+                                           const uint64_t (&acc)[4][D / 32], const float (&f)[4]) {
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
     if (ty * 4 + a >= len) continue;
     T* row = static_cast<T*>(to) + ((token + ty * 4 + a) * heads + head) * dim;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const int d = tx * 4 + 64 * (c / 4) + c % 4;
-      if (d < dim) row[d] = from_f<T>(acc[a][c] * f[a]);
+    for (int c = 0; c < D / 32; ++c) {
+      const float2 x = unpair(acc[a][c]);
+      const int d = tx * 4 + 64 * (c / 2) + 2 * (c % 2);
+      if (d < dim) row[d] = from_f<T>(x.x * f[a]);
+      if (d + 1 < dim) row[d + 1] = from_f<T>(x.y * f[a]);
     }
   }
 }
@@ -154,12 +172,13 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
   if (t.first < 0) return;
   const int len = min(kR, t.len - t.first);
   load_tile<T, D>(qs, p.q, h, t.start + t.first, len, p.dk);
-  float acc[4][D / 16], l[4], m[4];
+  uint64_t acc[4][D / 32];
+  float l[4], m[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
     l[a] = 0.f, m[a] = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) acc[a][c] = 0.f;
+    for (int c = 0; c < D / 32; ++c) acc[a][c] = 0;
   }
   const float c2 = p.scale * kLog2e;
   for (int j = 0; j <= t.first; j += kR) {
@@ -167,7 +186,7 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
     __syncthreads();
     load_tile<T, D>(ks, p.k, hk, t.start + j, own ? len : kR, p.dk);
     load_tile<T, D>(vs, p.v, hk, t.start + j, own ? len : kR, p.dv);
-    __syncthreads();
+    wait_tiles();
     float s[4][4];
     dots<D>(qs, ks, tx, ty, p.dk, s);
 #pragma unroll
@@ -191,7 +210,7 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
       }
       l[a] = fmaf(l[a], keep, row_sum(sum));
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) acc[a][c] *= keep;
+      for (int c = 0; c < D / 32; ++c) acc[a][c] = mul2(acc[a][c], pair(keep, keep));
     }
     __syncwarp();  // a warp's rows of the scores are its own
     if (own) rows_times<D, true>(ps, vs, tx, ty, acc);
@@ -208,7 +227,10 @@ __global__ void __launch_bounds__(kPlainThreads) forward_kernel(const __grid_con
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) acc[a][c] = acc[a][c] * f[a] - to_f(from_f<T>(acc[a][c] * f[a]));
+      for (int c = 0; c < D / 32; ++c) {
+        const float2 x = unpair(acc[a][c]);
+        acc[a][c] = pair(x.x * f[a] - to_f(from_f<T>(x.x * f[a])), x.y * f[a] - to_f(from_f<T>(x.y * f[a])));
+      }
     const float one[4] = {1.f, 1.f, 1.f, 1.f};
     store_rows<T, D>(p.rest, h, p.H, t.start + t.first, len, p.dv, tx, ty, acc, one);
   }
@@ -299,14 +321,15 @@ __global__ void __launch_bounds__(kPlainThreads) dq_kernel(const __grid_constant
   const long long at = t.start + t.first;
   load_tile<T, D>(qs, p.q, h, at, len, p.dk);
   load_tile<T, D>(gs, p.d_out, h, at, len, p.dv);
-  float acc[4][D / 16], lse[4], d[4];
+  uint64_t acc[4][D / 32];
+  float lse[4], d[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
     const bool in = ty * 4 + a < len;
     lse[a] = in ? p.lse[h * p.BL + at + ty * 4 + a] : 0.f;
     d[a] = in ? p.d[h * p.BL + at + ty * 4 + a] : 0.f;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) acc[a][c] = 0.f;
+    for (int c = 0; c < D / 32; ++c) acc[a][c] = 0;
   }
   const float c2 = p.scale * kLog2e;
   for (int j = 0; j <= t.first; j += kR) {
@@ -314,7 +337,7 @@ __global__ void __launch_bounds__(kPlainThreads) dq_kernel(const __grid_constant
     __syncthreads();
     load_tile<T, D>(ks, p.k, hk, t.start + j, own ? len : kR, p.dk);
     load_tile<T, D>(vs, p.v, hk, t.start + j, own ? len : kR, p.dv);
-    __syncthreads();
+    wait_tiles();
     float s[4][4], g[4][4];
     dots<D>(qs, ks, tx, ty, p.dk, s);
     dots<D>(gs, vs, tx, ty, p.dv, g);
@@ -346,11 +369,11 @@ __global__ void __launch_bounds__(kPlainThreads) dkdv_kernel(const __grid_consta
   const long long at = t.start + t.first;
   load_tile<T, D>(ks, p.k, hk, at, len, p.dk);
   load_tile<T, D>(vs, p.v, hk, at, len, p.dv);
-  float dk[4][D / 16], dv[4][D / 16];
+  uint64_t dk[4][D / 32], dv[4][D / 32];
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) dk[a][c] = dv[a][c] = 0.f;
+    for (int c = 0; c < D / 32; ++c) dk[a][c] = dv[a][c] = 0;
   const float c2 = p.scale * kLog2e;
   for (int g = 0; g < p.share; ++g) {
     const int h = hk * p.share + g;
@@ -360,7 +383,7 @@ __global__ void __launch_bounds__(kPlainThreads) dkdv_kernel(const __grid_consta
       __syncthreads();
       load_tile<T, D>(qs, p.q, h, t.start + i, n, p.dk);
       load_tile<T, D>(gs, p.d_out, h, t.start + i, n, p.dv);
-      __syncthreads();
+      wait_tiles();
       float s[4][4], e[4][4];
       dots<D>(qs, ks, tx, ty, p.dk, s);
       dots<D>(gs, vs, tx, ty, p.dv, e);
