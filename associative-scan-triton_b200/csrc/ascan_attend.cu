@@ -344,9 +344,9 @@ __global__ void __launch_bounds__(kPlainThreads) dq_kernel(const __grid_constant
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < 4; ++b)  // a sequence's first token sees one key, with p = 1: no ds, not even a rounding
         ps[(ty * 4 + a) * kPs + tx + 16 * b] =
-            own && tx + 16 * b > ty * 4 + a ? 0.f : exp2f(fmaf(s[a][b], c2, -lse[a])) * (g[a][b] - d[a]);
+            own && tx + 16 * b > ty * 4 + a ? 0.f : exp2f(fmaf(s[a][b], c2, -lse[a])) * (g[a][b] - d[a]) * (t.first + ty * 4 + a == 0 ? 0.f : 1.f);
     __syncwarp();
     if (own) rows_times<D, true>(ps, ks, tx, ty, acc);
     else rows_times<D, false>(ps, ks, tx, ty, acc);
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kPlainThreads) dkdv_kernel(const __grid_consta
           const bool off = row >= n || (own && tx + 16 * b > row);
           const float x = off ? 0.f : exp2f(fmaf(s[a][b], c2, -lse));
           ps[row * kPs + tx + 16 * b] = x;
-          ds[row * kPs + tx + 16 * b] = off ? 0.f : x * (e[a][b] - d);
+          ds[row * kPs + tx + 16 * b] = off ? 0.f : x * (e[a][b] - d) * (i + row == 0 ? 0.f : 1.f);
         }
       }
       __syncthreads();

@@ -258,6 +258,14 @@ __device__ __forceinline__ void fetch_block(uint32_t tm, float f, uint32_t* out)
   }
 }
 
+// dS of a sequence's first token, in the low half: it sees one key, with p = 1,
+// so there is none, not even a rounding, unless something is not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t only_key(uint32_t w) {
+  const float x = unpair(unpack2<T>(w)).x;
+  return x - x == 0.f ? 0u : 0x7fffu;
+}
+
 __device__ __forceinline__ bool misplaced(const unsigned char* smem, uint32_t* err) {
   if (!(smem_u32(smem) & 1023u)) return false;  // the swizzled layouts need it
   if (threadIdx.x == 0) report(ASCAN_DEV_ERR_STAGE, 0xffffffffull, err);
@@ -745,9 +753,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
 
 struct DqTail {
   Common c;
-  uint64_t q_full, full[kMaxSlots], empty[kMaxSlots], dp_full, dp_free, ds_ready, o_done;
+  uint64_t q_full, full[kMaxSlots], empty[kMaxSlots], dp_full, dp_free, ds_ready, o_done, mean_ready, sums_ready;
+  alignas(16) float mean[2][kC];  // halves of the sum of the sequence's first keys
+  float sums[2][kC];  // of a row's dS as rounded, by half of the columns
 };
 
+// A row's dS add up to nothing, so its dq does not depend on what all keys have
+// in common; rounded dS do not, quite.  With c near the keys' mean (of the
+// sequence's first block),
+//
+//   dq = scale (sum_j dS[j] k[j] - (sum_j dS[j]) c)
+//
+// is the same without roundings, and with them what the keys share stays out of
+// their error: where it was half of the keys' spread, dq's distance from 64 bits
+// was 1.53 times that of one rounding, and two independent ones make 1.41.
 template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_constant__ Problem p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -768,6 +787,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     bar_init(&s.dp_free, 8);
     bar_init(&s.ds_ready, 8);
     bar_init(&s.o_done, 1);
+    bar_init(&s.mean_ready, 2);
+    bar_init(&s.sums_ready, 8);
     bar_init(&s.c.drain, 1);
     s.c.abort = 0;
     bars_done();
@@ -784,6 +805,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     const float lse = row < len ? p.lse[h * p.BL + at + row] : 0.f, d = row < len ? p.d[h * p.BL + at + row] : 0.f;
     const float c2 = p.scale * kLog2e;
     const uint64_t c22 = pair(c2, c2), lse2 = pair(-lse, -lse), d2 = pair(-d, -d);
+    uint64_t sum[2] = {0, 0};
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       if (!(ok = ctl.warp_wait(&s.dp_full, j & 1))) break;  // S was issued before dP
@@ -810,6 +832,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
           const int c = 64 * side + 2 * e;
           w[e] &= (c <= row ? 0xffffu : 0u) | (c + 1 <= row ? 0xffff0000u : 0u);
         }
+        if (side == 0 && t.first + row == 0) w[0] = only_key<T>(w[0]);
         // keys of the rows behind the mask, and of other sequences
         const int i = 2 * j;
         if (64 * side < p.dk) clean_row<T>(ring + i % ns * slot, row, side, 1, row < len);
@@ -819,11 +842,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
       wait_st();
       fence_before();
       warp_arrive(&s.ds_ready);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sum[e & 1] = add2(sum[e & 1], unpack2<T>(w[e]));
     }
-    if (ok && 64 * side < p.dk && ctl.warp_wait(&s.o_done, 0)) {
+    const float2 both = unpair(add2(sum[0], sum[1]));
+    s.sums[side][row] = both.x + both.y;
+    warp_arrive(&s.sums_ready);
+    if (ok && 64 * side < p.dk && ctl.warp_wait(&s.sums_ready, 0) && ctl.warp_wait(&s.mean_ready, 0) && ctl.warp_wait(&s.o_done, 0)) {
       fence_after();
+      const float f = -p.scale * (s.sums[0][row] + s.sums[1][row]) / static_cast<float>(min(kC, t.len));
+      const uint64_t f2 = pair(f, f), scale2 = pair(p.scale, p.scale);
       uint32_t w[32];
-      fetch_block<T>(tm + lanes + kDq + 64 * side, p.scale, w);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t x[32];
+        tmem_ld32(tm + lanes + kDq + 64 * side + 32 * half, x);
+        wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 a = *reinterpret_cast<const float2*>(&s.mean[0][64 * side + 32 * half + 2 * e]);
+          const float2 b = *reinterpret_cast<const float2*>(&s.mean[1][64 * side + 32 * half + 2 * e]);
+          w[16 * half + e] = pack2<T>(fma2(add2(pair(a.x, a.y), pair(b.x, b.y)), f2, mul2(pair_of(x + 2 * e), scale2)));
+        }
+      }
       store_block(smem + side * kBlock + quad * 4096, w,
                   static_cast<unsigned char*>(p.d_q) + ((at + quad * 32) * p.H + h) * p.dk * 2 + side * 128,
                   static_cast<long long>(p.H) * p.dk * 2, len - quad * 32, p.dk - 64 * side);
@@ -879,8 +920,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
       commit(&s.c.drain);
       ctl.land(&s.c.drain, 0);
     }
-  } else if (warp == 10) {
-    zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, lane, 32);
+  } else {
+    // sums over the first keys, without what is not finite, four elements a lane
+    const int half = warp - 10, rows = min(kC, t.len);
+    const T* k = static_cast<const T*>(p.k.p) + static_cast<long long>(t.start) * p.k.st + hk * p.k.sh + 4 * lane;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (4 * lane < p.dk) {
+#pragma unroll 8
+      for (int i = half; i < rows; i += 2) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(k + i * p.k.st));
+        const float2 a = unpair(unpack2<T>(w.x)), b = unpair(unpack2<T>(w.y));
+        const float v[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += fabsf(v[e]) < INFINITY ? v[e] : 0.f;
+      }
+    }
+    *reinterpret_cast<float4*>(&s.mean[half][4 * lane]) = make_float4(x[0], x[1], x[2], x[3]);
+    warp_arrive(&s.mean_ready);
+    if (half == 0) zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, lane, 32);
   }
   close_tmem(tm);
 }
@@ -893,7 +950,7 @@ struct DkvTail {
   Common c;
   uint64_t kv_full, q_full[2], q_empty[2], g_full[2], g_empty[2], stat_full[2], stat_empty[2];
   uint64_t s_full, s_free, p_ready, p_free, dp_full, ds_ready, o_done;
-  float lse[2][kC], d[2][kC];  // negated, of the queries that pass
+  alignas(16) float lse[2][kC], d[2][kC];  // negated, of the queries that pass
   int bad;                     // 1 + the last query of the diagonal's tile whose dO is not finite
 };
 
@@ -1017,6 +1074,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
           const int c = 64 * side + 2 * e;
           w[e] &= ((diagonal && c < row) || c >= n ? 0u : 0xffffu) | ((diagonal && c + 1 < row) || c + 1 >= n ? 0u : 0xffff0000u);
         }
+        if (diagonal && side == 0 && t.first + row == 0) w[0] = (w[0] & 0xffff0000u) | only_key<T>(w[0]);
       }
       tmem_st32(td, w);
       wait_st();
