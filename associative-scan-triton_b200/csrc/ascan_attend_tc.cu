@@ -330,6 +330,10 @@ __device__ __forceinline__ void check_cu(const Problem& p, int thread, int threa
 
 constexpr int kFwdSoftmax = 8, kFwdThreads = (kFwdSoftmax + 2) * 32;
 
+// The forward's ring: a slot less than the gradients', for rows on their way out.
+__host__ __device__ inline int forward_slots(int dk, int dv) { return dk > 64 || dv > 64 ? 4 : kMaxSlots; }
+constexpr int kStage = 4096;  // of a warp: 32 rows of 64 elements
+
 // Of eight pairs of scores so many take the polynomial.
 constexpr int kPoly = 3;
 // An item's place is searched for in shared memory, eight times as fast as
@@ -474,9 +478,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (misplaced(smem, p.err)) return;
-  const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk);
-  unsigned char* ring = smem + 2 * q_bytes;
-  ForwardTail& s = *reinterpret_cast<ForwardTail*>(ring + ns * slot);
+  const int slot = slot_bytes(p.dk, p.dv), ns = forward_slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk);
+  unsigned char *ring = smem + 2 * q_bytes, *stages = ring + ns * slot;
+  ForwardTail& s = *reinterpret_cast<ForwardTail*>(stages + kFwdSoftmax * kStage);
   const Ctl ctl{&s.c, p.err};
   if (tid == 0) {
     bar_init(&s.q_full, 1);
@@ -579,47 +583,41 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
         if (TRAIN && row < left) p.lse[it.h * p.BL + token] = r.m * c2 + log2f(l);
         bool any = false;
         for (int i = 0; i < 4; ++i) any |= s.bad[count & 3][0][i] != 0 || (x == 1 && s.bad[count & 3][1][i] != 0);
-        T* out = static_cast<T*>(p.out) + (token * p.H + it.h) * p.dv;
-        T* rest = static_cast<T*>(p.rest) + (token * p.H + it.h) * p.dv;
+        // whole lines: a lane's own row would be 32 of them for every store
+        const long long stride = static_cast<long long>(p.H) * p.dv * 2, first = ((token - lane) * p.H + it.h) * p.dv * 2;
+        const int rows = left - quad * 32;
 #pragma unroll 1
-        for (int b = 0; b < n32; ++b) {
-          uint32_t o[32];
-          tmem_ld32(to + 32 * b, o);
-          wait_ld();
+        for (int b = 0; b * 64 < p.dv; ++b) {
+          uint32_t u[32], v[TRAIN ? 32 : 1];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
-          if (any) {  // what was taken out of the values goes where the mask lets it
-            for (int y = 0; y <= x; ++y)
-              for (int i = 0; i < kC; ++i) {
-                if (!(s.bad[count & 3][y][i >> 5] >> (i & 31) & 1) || (y == x && i > row)) continue;
-                const T* v = static_cast<const T*>(p.v.p) + (static_cast<long long>(it.token) + y * kC + i) * p.v.st + it.h / p.share * p.v.sh;
+          for (int half = 0; half < 2; ++half) {
+            const int d0 = 64 * b + 32 * half;
+            uint32_t o[32];
+            tmem_ld32(to + d0, o);
+            wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (32 * b + e < p.dv) {
-                    const float q = to_f(v[32 * b + e]);
-                    if (!(fabsf(q) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + q);
-                  }
-              }
-          }
-          uint32_t u[16];
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+            if (any) {  // what was taken out of the values goes where the mask lets it
+              for (int y = 0; y <= x; ++y)
+                for (int i = 0; i < kC; ++i) {
+                  if (!(s.bad[count & 3][y][i >> 5] >> (i & 31) & 1) || (y == x && i > row)) continue;
+                  const T* from = static_cast<const T*>(p.v.p) + (static_cast<long long>(it.token) + y * kC + i) * p.v.st + it.h / p.share * p.v.sh;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = pack2<T>(pair_of(o + 2 * e));
-          if (row < left) {
+                  for (int e = 0; e < 32; ++e)
+                    if (d0 + e < p.dv) {
+                      const float q = to_f(from[d0 + e]);
+                      if (!(fabsf(q) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + q);
+                    }
+                }
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (32 * b + 8 * e < p.dv)
-                *reinterpret_cast<uint4*>(out + 32 * b + 8 * e) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
-          }
-          if (TRAIN) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) u[e] = pack2<T>(fma2(unpack2<T>(u[e]), pair(-1.f, -1.f), pair_of(o + 2 * e)));
-            if (row < left) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (32 * b + 8 * e < p.dv)
-                  *reinterpret_cast<uint4*>(rest + 32 * b + 8 * e) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+            for (int e = 0; e < 16; ++e) {
+              u[16 * half + e] = pack2<T>(pair_of(o + 2 * e));
+              if (TRAIN) v[16 * half + e] = pack2<T>(fma2(unpack2<T>(u[16 * half + e]), pair(-1.f, -1.f), pair_of(o + 2 * e)));
             }
           }
+          store_block(stages + warp * kStage, u, static_cast<unsigned char*>(p.out) + first + b * 128, stride, rows, p.dv - 64 * b);
+          if (TRAIN) store_block(stages + warp * kStage, v, static_cast<unsigned char*>(p.rest) + first + b * 128, stride, rows, p.dv - 64 * b);
         }
       }
       base += 2 * it.n;
@@ -1246,7 +1244,7 @@ static int forward(const Problem& p, const Maps& m, cudaStream_t s) {
   static std::atomic<unsigned long long> done{};
   const int rc = allow_smem(tc_forward_kernel<T, TRAIN>, kSmemLimit, done);
   if (rc != ASCAN_OK) return rc;
-  const size_t smem = 2 * bytes_of(p.dk) + slots(p.dk, p.dv) * slot_bytes(p.dk, p.dv) + sizeof(ForwardTail);
+  const size_t smem = 2 * bytes_of(p.dk) + forward_slots(p.dk, p.dv) * slot_bytes(p.dk, p.dv) + kFwdSoftmax * kStage + sizeof(ForwardTail);
   tc_forward_kernel<T, TRAIN><<<static_cast<unsigned>(tile_bound(p, 2 * kC) * p.H), kFwdThreads, smem, s>>>(p, m);
   return launch_status();
 }
