@@ -162,6 +162,9 @@ __device__ __forceinline__ uint64_t ex2_2(uint64_t x) {
   const float2 f = unpair(x);
   return pair(ex2(f.x), ex2(f.y));
 }
+// Of eight pairs of scores so many take the polynomial.
+constexpr int kPoly = 3;
+
 // 2^x of a pair by a polynomial of degree 4 on [-1/2, 1/2] (fitted to the
 // smallest relative error, 2.6e-6) and the exponent's bits; below 2^-126 what is
 // left is as small, and NaN comes out infinite, which makes a row NaN as well.
@@ -334,8 +337,6 @@ constexpr int kFwdSoftmax = 8, kFwdThreads = (kFwdSoftmax + 2) * 32;
 __host__ __device__ inline int forward_slots(int dk, int dv) { return dk > 64 || dv > 64 ? 4 : kMaxSlots; }
 constexpr int kStage = 4096;  // of a warp: 32 rows of 64 elements
 
-// Of eight pairs of scores so many take the polynomial.
-constexpr int kPoly = 3;
 // An item's place is searched for in shared memory, eight times as fast as
 // through what the slots leave of the first cache.
 constexpr int kEnds = 512;
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
       uint32_t w[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        const uint64_t y = ex2_2(fma2(pair_of(sc + 2 * e), c22, lse2));
+        const uint64_t z = fma2(pair_of(sc + 2 * e), c22, lse2), y = (e & 7) >= 8 - kPoly ? poly_ex2_2(z) : ex2_2(z);
         w[e] = pack2<T>(mul2(y, add2(pair_of(g + 2 * e), d2)));
       }
       if (diagonal) {
@@ -1022,8 +1023,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float4 l = *reinterpret_cast<const float4*>(&s.lse[u][64 * side + 2 * e]);
-          x[e] = ex2_2(fma2(pair_of(sc + 2 * e), c22, pair(l.x, l.y)));
-          x[e + 1] = ex2_2(fma2(pair_of(sc + 2 * e + 2), c22, pair(l.z, l.w)));
+          const uint64_t z0 = fma2(pair_of(sc + 2 * e), c22, pair(l.x, l.y)), z1 = fma2(pair_of(sc + 2 * e + 2), c22, pair(l.z, l.w));
+          x[e] = (e & 7) >= 8 - kPoly ? poly_ex2_2(z0) : ex2_2(z0);
+          x[e + 1] = (e & 7) + 1 >= 8 - kPoly ? poly_ex2_2(z1) : ex2_2(z1);
         }
       }
       if (edge) {
