@@ -750,9 +750,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tc_forward_kernel(const __grid
 // gradients of the queries
 // ---------------------------------------------------------------------------
 
+// A tile of keys is held until dq's product, one of values only until dP's.  In
+// one ring of five the values' next slot came free with the keys before last,
+// a thousand cycles too late for every tile.
+constexpr int kKeySlots = 3, kValueSlots = 2;
+
 struct DqTail {
   Common c;
-  uint64_t q_full, full[kMaxSlots], empty[kMaxSlots], dp_full, dp_free, ds_ready, o_done, mean_ready, sums_ready;
+  uint64_t q_full, k_full[kKeySlots], k_empty[kKeySlots], v_full[kValueSlots], v_empty[kValueSlots];
+  uint64_t dp_full, dp_free, ds_ready, o_done, mean_ready, sums_ready;
   alignas(16) float mean[2][kC];  // halves of the sum of the sequence's first keys
   float sums[2][kC];  // of a row's dS as rounded, by half of the columns
 };
@@ -773,15 +779,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
   const Tile t = find_tile_warp<7>(p, gridDim.x - 1 - blockIdx.x);
   if (t.first < 0) zero_outside<T>(p, p.d_q, h, p.H, p.dk, blockIdx.x, kC, tid, kTcThreads);
   if (t.first < 0 || misplaced(smem, p.err)) return;
-  const int slot = slot_bytes(p.dk, p.dv), ns = slots(p.dk, p.dv), q_bytes = tile_bytes(p.dk), g_bytes = tile_bytes(p.dv);
-  unsigned char* ring = smem + q_bytes + g_bytes;
-  DqTail& s = *reinterpret_cast<DqTail*>(ring + ns * slot);
+  const int q_bytes = tile_bytes(p.dk), g_bytes = tile_bytes(p.dv);
+  unsigned char *k_ring = smem + q_bytes + g_bytes, *v_ring = k_ring + kKeySlots * q_bytes;
+  DqTail& s = *reinterpret_cast<DqTail*>(v_ring + kValueSlots * g_bytes);
   const Ctl ctl{&s.c, p.err};
   const int n = t.first / kC + 1, len = min(kC, t.len - t.first);
   const long long at = t.start + t.first;
   if (tid == 8 * 32) {  // the loading warp's, which need not wait for the others
     bar_init(&s.q_full, 1);
-    for (int i = 0; i < ns; ++i) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
+    for (int i = 0; i < kKeySlots; ++i) bar_init(&s.k_full[i], 1), bar_init(&s.k_empty[i], 1);
+    for (int i = 0; i < kValueSlots; ++i) bar_init(&s.v_full[i], 1), bar_init(&s.v_empty[i], 1);
     bar_init(&s.dp_full, 1);
     bar_init(&s.dp_free, 8);
     bar_init(&s.ds_ready, 8);
@@ -833,8 +840,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
         }
         if (side == 0 && t.first + row == 0) w[0] = only_key<T>(w[0]);
         // keys of the rows behind the mask, and of other sequences
-        const int i = 2 * j;
-        if (64 * side < p.dk) clean_row<T>(ring + i % ns * slot, row, side, 1, row < len);
+        if (64 * side < p.dk) clean_row<T>(k_ring + j % kKeySlots * q_bytes, row, side, 1, row < len);
         fence_async();
       }
       tmem_st32(ts, w);
@@ -870,40 +876,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     }
   } else if (warp == 8) {
     if (lane == 0) {
-      int i = 0;
-      Cursor to;
-      for (; i < 2 * n; ++i) {
-        const bool is_v = i & 1;
-        if (!ctl.wait(&s.empty[to.at], to.turn ^ 1)) break;  // a first pass finds all slots empty
-        bar_expect(&s.full[to.at], tile_bytes(is_v ? p.dv : p.dk));
-        load_tile(ring + to.at * slot, is_v ? &maps.v : &maps.k, is_v ? p.dv : p.dk, hk, t.start + (i >> 1) * kC, &s.full[to.at]);
-        to.next(ns);
+      Cursor k, v;
+      int loads = 0;  // tiles of both
+      for (; loads < n; ++loads) {
+        // a first pass finds all slots empty
+        if (!ctl.wait(&s.k_empty[k.at], k.turn ^ 1)) break;
+        bar_expect(&s.k_full[k.at], q_bytes);
+        load_tile(k_ring + k.at * q_bytes, &maps.k, p.dk, hk, t.start + loads * kC, &s.k_full[k.at]);
+        if (!ctl.wait(&s.v_empty[v.at], v.turn ^ 1)) {
+          ctl.land(&s.k_full[k.at], k.turn);
+          break;
+        }
+        bar_expect(&s.v_full[v.at], g_bytes);
+        load_tile(v_ring + v.at * g_bytes, &maps.v, p.dv, hk, t.start + loads * kC, &s.v_full[v.at]);
+        k.next(kKeySlots);
+        v.next(kValueSlots);
       }
-      if (i < 2 * n) {
+      if (loads < n) {
         ctl.land(&s.q_full, 0);
-        for (int e = max(0, i - ns); e < i; ++e) ctl.land(&s.full[e % ns], (e / ns) & 1);
+        for (int e = max(0, loads - kKeySlots); e < loads; ++e) ctl.land(&s.k_full[e % kKeySlots], (e / kKeySlots) & 1);
+        for (int e = max(0, loads - kValueSlots); e < loads; ++e) ctl.land(&s.v_full[e % kValueSlots], (e / kValueSlots) & 1);
       }
     }
   } else if (warp == 9) {
     if (elect_one()) {  // one thread, without votes
       const uint32_t id_s = idesc(kC, false, f16<T>()), id_o = idesc((p.dk + 15) / 16 * 16, true, f16<T>());
       const uint64_t q = desc(smem_u32(smem), 16), g = desc(smem_u32(smem) + q_bytes, 16);
-      const uint64_t k0 = desc(smem_u32(ring), 16), o0 = desc(smem_u32(ring), kBlock);
-      Cursor c;
+      const uint64_t k0 = desc(smem_u32(k_ring), 16), o0 = desc(smem_u32(k_ring), kBlock), v0 = desc(smem_u32(v_ring), 16);
+      Cursor kc, vc;
       int held[2] = {0, 0};  // slots of the keys that a product still has to come for
       bool ok = ctl.wait(&s.q_full, 0);
       for (int j = -1; ok && j < n; ++j) {
         if (j + 1 < n) {  // the next tile's scores, while the warps are at this one's
-          if (!(ok = ctl.wait(&s.full[c.at], c.turn))) break;
-          scores(tm + ((j + 1) & 1) * kC, q, k0 + c.at * (slot >> 4), id_s, p.dk);
-          held[(j + 1) & 1] = c.at;
-          c.next(ns);
-          if (!(ok = ctl.wait(&s.full[c.at], c.turn) && (j < 0 || ctl.wait(&s.dp_free, j & 1)))) break;
+          if (!(ok = ctl.wait(&s.k_full[kc.at], kc.turn))) break;
+          scores(tm + ((j + 1) & 1) * kC, q, k0 + kc.at * (q_bytes >> 4), id_s, p.dk);
+          held[(j + 1) & 1] = kc.at;
+          kc.next(kKeySlots);
+          if (!(ok = ctl.wait(&s.v_full[vc.at], vc.turn) && (j < 0 || ctl.wait(&s.dp_free, j & 1)))) break;
           fence_after();
-          scores(tm + kDp, g, k0 + c.at * (slot >> 4), id_s, p.dv);
+          scores(tm + kDp, g, v0 + vc.at * (g_bytes >> 4), id_s, p.dv);
           commit(&s.dp_full);
-          commit(&s.empty[c.at]);
-          c.next(ns);
+          commit(&s.v_empty[vc.at]);
+          vc.next(kValueSlots);
         }
         if (j < 0) continue;
         if (!(ok = ctl.wait(&s.ds_ready, j & 1))) break;
@@ -912,8 +926,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
         // the warps' halves of dS lie 64 columns apart
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k)
-          mma_tmem(tm + kDq, tm + (j & 1) * kC + (k >> 2) * 64 + (k & 3) * 8, o0 + at_k * (slot >> 4) + k * 128, id_o, j + k > 0);
-        commit(&s.empty[at_k]);
+          mma_tmem(tm + kDq, tm + (j & 1) * kC + (k >> 2) * 64 + (k & 3) * 8, o0 + at_k * (q_bytes >> 4) + k * 128, id_o, j + k > 0);
+        commit(&s.k_empty[at_k]);
         if (j == n - 1) commit(&s.o_done);
       }
       commit(&s.c.drain);
@@ -1258,7 +1272,8 @@ static int backward(const Problem& p, const Maps& m, cudaStream_t s) {
   if (rc == ASCAN_OK) rc = allow_smem(tc_dkdv_kernel<T>, kSmemLimit, done[1]);
   if (rc != ASCAN_OK) return rc;
   const size_t k = bytes_of(p.dk), v = bytes_of(p.dv);
-  const size_t q_smem = k + v + slots(p.dk, p.dv) * slot_bytes(p.dk, p.dv) + sizeof(DqTail);
+  // one CTA an SM in any case: each takes all of tensor memory
+  const size_t q_smem = max(k + v + kKeySlots * k + kValueSlots * v + sizeof(DqTail), static_cast<size_t>(120 << 10));
   tc_dq_kernel<T><<<dim3(tile_bound(p, kC), p.H), kTcThreads, q_smem, s>>>(p, m);
   rc = launch_status();
   if (rc != ASCAN_OK) return rc;
