@@ -20,8 +20,9 @@
 //   S's place, dQ += dS K.  Two S take turns, so that the next one is computed
 //   while the warps are at this one.
 // dk, dv: one tile of keys walks the queries of all heads that share it, with
-//   everything transposed: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO (P^T from
-//   shared memory, so that the next S^T has a place), dK += dS^T Q.
+//   everything transposed: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO with P^T in
+//   S^T's place, dK += dS^T Q with dS^T in dP^T's.  The next S^T follows dV's
+//   product, so that its softmax runs while dK's and the next dP^T's do.
 //
 // Rounding P and dS to the inputs' type adds an error of the size of the
 // result's own rounding: each is off by at most half a step of itself, and
@@ -64,9 +65,8 @@ struct Maps {
   CUtensorMap q, k, v, d_out;
 };
 
-// Slots of the ring of keys and values: what 227 KB hold next to `fixed` bytes.
+// A slot for tiles of keys and of values.
 __host__ __device__ inline int slot_bytes(int dk, int dv) { return dk > 64 || dv > 64 ? 2 * kBlock : kBlock; }
-__host__ __device__ inline int slots(int dk, int dv) { return dk > 64 || dv > 64 ? 5 : kMaxSlots; }
 
 struct Common {
   uint64_t drain;
@@ -959,10 +959,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
 // gradients of the keys and values
 // ---------------------------------------------------------------------------
 
+// Queries are held from their scores to dK's product, the last one of a tile.
+constexpr int kQuerySlots = 3;
+
 struct DkvTail {
   Common c;
-  uint64_t kv_full, q_full[2], q_empty[2], g_full[2], g_empty[2], stat_full[2], stat_empty[2];
-  uint64_t s_full, s_free, p_ready, p_free, dp_full, ds_ready, o_done;
+  uint64_t kv_full, q_full[kQuerySlots], q_empty[kQuerySlots], g_full[2], g_empty[2], stat_full[2], stat_empty[2];
+  uint64_t s_full, p_ready, dp_full, ds_ready, o_done;
   alignas(16) float lse[2][kC], d[2][kC];  // negated, of the queries that pass
   int bad;                     // 1 + the last query of the diagonal's tile whose dO is not finite
 };
@@ -978,26 +981,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
   }
   if (t.first < 0 || misplaced(smem, p.err)) return;
   const int k_bytes = tile_bytes(p.dk), v_bytes = tile_bytes(p.dv);
-  unsigned char *q_ring = smem + k_bytes + v_bytes, *g_ring = q_ring + 2 * k_bytes, *pt = g_ring + 2 * v_bytes;
-  DkvTail& s = *reinterpret_cast<DkvTail*>(pt + 2 * kBlock);
+  unsigned char *q_ring = smem + k_bytes + v_bytes, *g_ring = q_ring + kQuerySlots * k_bytes;
+  DkvTail& s = *reinterpret_cast<DkvTail*>(g_ring + 2 * v_bytes);
   const Ctl ctl{&s.c, p.err};
   const int blocks = (t.len - t.first + kC - 1) / kC, len = min(kC, t.len - t.first);
   const int total = blocks * p.share;  // tiles of queries, head by head
   const long long at = t.start + t.first;
   if (tid == 8 * 32) {  // the loading warp's, which need not wait for the others
     bar_init(&s.kv_full, 1);
+    for (int i = 0; i < kQuerySlots; ++i) bar_init(&s.q_full[i], 1), bar_init(&s.q_empty[i], 1);
     for (int i = 0; i < 2; ++i) {
-      bar_init(&s.q_full[i], 1);
-      bar_init(&s.q_empty[i], 1);
       bar_init(&s.g_full[i], 1);
       bar_init(&s.g_empty[i], 1);
       bar_init(&s.stat_full[i], 1);
       bar_init(&s.stat_empty[i], 8);
     }
     bar_init(&s.s_full, 1);
-    bar_init(&s.s_free, 8);
     bar_init(&s.p_ready, 8);
-    bar_init(&s.p_free, 1);
     bar_init(&s.dp_full, 1);
     bar_init(&s.ds_ready, 8);
     bar_init(&s.o_done, 1);
@@ -1032,8 +1032,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
         tmem_ld32(ts, sc);
         tmem_ld32(ts + 32, sc + 32);
         wait_ld();
-        fence_before();
-        warp_arrive(&s.s_free);
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float4 l = *reinterpret_cast<const float4*>(&s.lse[u][64 * side + 2 * e]);
@@ -1054,19 +1052,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
       }
 #pragma unroll
       for (int e = 0; e < 32; ++e) w[e] = pack2<T>(x[e]);
-      if (i > 0 && !(ok = ctl.warp_wait(&s.p_free, (i - 1) & 1))) break;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(pt + side * kBlock + row * 128 + ((c ^ (row & 7)) << 4)) =
-            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      tmem_st32(ts, w);
       if (edge) {
         // queries and upstream gradients of rows behind the mask, and of other
         // sequences, once both score products have read them
         if (!(ok = ctl.warp_wait(&s.dp_full, i & 1))) break;
-        if (64 * side < p.dk) clean_row<T>(q_ring + u * k_bytes, row, side, 1, row < n);
+        if (64 * side < p.dk) clean_row<T>(q_ring + i % kQuerySlots * k_bytes, row, side, 1, row < n);
         if (64 * side < p.dv && clean_row<T>(g_ring + u * v_bytes, row, side, 1, row < n) && diagonal) atomicMax(&s.bad, row + 1);
+        fence_async();
       }
-      fence_async();
+      wait_st();
+      fence_before();
       warp_arrive(&s.p_ready);
       if (!(ok = ctl.warp_wait(&s.dp_full, i & 1))) break;
       fence_after();
@@ -1119,22 +1115,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
   } else if (warp == 8) {
     if (lane == 0) {
       int q_loads = 0, g_loads = 0;
+      Cursor q, g;
       for (int i = 0, b = 0, h = hk * p.share; i < total; ++i) {
-        const int u = i & 1;
-        const long long token = at + static_cast<long long>(b) * kC;
-        if (i > 1 && !ctl.wait(&s.q_empty[u], (i / 2 - 1) & 1)) break;
-        bar_expect(&s.q_full[u], k_bytes);
-        load_tile(q_ring + u * k_bytes, &maps.q, p.dk, h, token, &s.q_full[u]);
+        const int token = static_cast<int>(at) + b * kC;
+        // a first pass finds all slots empty
+        if (!ctl.wait(&s.q_empty[q.at], q.turn ^ 1)) break;
+        bar_expect(&s.q_full[q.at], k_bytes);
+        load_tile(q_ring + q.at * k_bytes, &maps.q, p.dk, h, token, &s.q_full[q.at]);
+        q.next(kQuerySlots);
         ++q_loads;
-        if (i > 1 && !ctl.wait(&s.g_empty[u], (i / 2 - 1) & 1)) break;
-        bar_expect(&s.g_full[u], v_bytes);
-        load_tile(g_ring + u * v_bytes, &maps.d_out, p.dv, h, token, &s.g_full[u]);
+        if (!ctl.wait(&s.g_empty[g.at], g.turn ^ 1)) break;
+        bar_expect(&s.g_full[g.at], v_bytes);
+        load_tile(g_ring + g.at * v_bytes, &maps.d_out, p.dv, h, token, &s.g_full[g.at]);
+        g.next(2);
         ++g_loads;
         if (++b == blocks) b = 0, ++h;
       }
       if (g_loads < total) {
         ctl.land(&s.kv_full, 0);
-        for (int i = max(0, q_loads - 2); i < q_loads; ++i) ctl.land(&s.q_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, q_loads - kQuerySlots); i < q_loads; ++i) ctl.land(&s.q_full[i % kQuerySlots], (i / kQuerySlots) & 1);
         for (int i = max(0, g_loads - 2); i < g_loads; ++i) ctl.land(&s.g_full[i & 1], (i >> 1) & 1);
       }
     }
@@ -1142,35 +1141,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
     if (elect_one()) {  // one thread, without votes
       const uint32_t id_s = idesc(kC, false, f16<T>()), id_k = idesc((p.dk + 15) / 16 * 16, true, f16<T>()),
                      id_v = idesc((p.dv + 15) / 16 * 16, true, f16<T>());
-      const uint64_t k = desc(smem_u32(smem), 16), v = desc(smem_u32(smem) + k_bytes, 16), a = desc(smem_u32(pt), 16);
-      const uint64_t q0 = desc(smem_u32(q_ring), 16), g0 = desc(smem_u32(g_ring), 16);                    // for scores
-      const uint64_t q1 = desc(smem_u32(q_ring), kBlock), g1 = desc(smem_u32(g_ring), kBlock);            // as values
+      const uint64_t k = desc(smem_u32(smem), 16), v = desc(smem_u32(smem) + k_bytes, 16);
+      const uint64_t q0 = desc(smem_u32(q_ring), 16), g0 = desc(smem_u32(g_ring), 16);          // for scores
+      const uint64_t q1 = desc(smem_u32(q_ring), kBlock), g1 = desc(smem_u32(g_ring), kBlock);  // as values
+      Cursor c, held;  // queries: the next tile's scores, and its product with dS
       bool ok = ctl.wait(&s.kv_full, 0);
       for (int i = -1; ok && i < total; ++i) {
         const bool more = i + 1 < total;
         const int u = i & 1, nu = (i + 1) & 1;
-        if (more) {
-          if (!(ok = ctl.wait(&s.q_full[nu], ((i + 1) >> 1) & 1) && (i < 0 || ctl.wait(&s.s_free, i & 1)))) break;
-          fence_after();
-          scores(tm, k, q0 + nu * (k_bytes >> 4), id_s, p.dk);
-          commit(&s.s_full);
-        }
         if (i >= 0) {
           if (!(ok = ctl.wait(&s.p_ready, i & 1))) break;
           fence_after();
-          const uint64_t g = g1 + u * (v_bytes >> 4), q = q1 + u * (k_bytes >> 4);
+          // the warps' halves of P lie 64 columns apart
 #pragma unroll
           for (int e = 0; e < kC / 16; ++e)
-            mma_smem(tm + kDv, a + (e >> 2) * (kBlock >> 4) + (e & 3) * 2, g + e * 128, id_v, i + e > 0);
-          commit(&s.p_free);
+            mma_tmem(tm + kDv, tm + (e >> 2) * 64 + (e & 3) * 8, g1 + u * (v_bytes >> 4) + e * 128, id_v, i + e > 0);
           commit(&s.g_empty[u]);
+        }
+        if (more) {  // in P's place, which that product has read
+          if (!(ok = ctl.wait(&s.q_full[c.at], c.turn))) break;
+          scores(tm, k, q0 + c.at * (k_bytes >> 4), id_s, p.dk);
+          commit(&s.s_full);
+          c.next(kQuerySlots);
+        }
+        if (i >= 0) {
           if (!(ok = ctl.wait(&s.ds_ready, i & 1))) break;
           fence_after();
-          // the warps' halves of dS lie 64 columns apart
 #pragma unroll
           for (int e = 0; e < kC / 16; ++e)
-            mma_tmem(tm + kDk, tm + kDp + (e >> 2) * 64 + (e & 3) * 8, q + e * 128, id_k, i + e > 0);
-          commit(&s.q_empty[u]);
+            mma_tmem(tm + kDk, tm + kDp + (e >> 2) * 64 + (e & 3) * 8, q1 + held.at * (k_bytes >> 4) + e * 128, id_k, i + e > 0);
+          commit(&s.q_empty[held.at]);
+          held.next(kQuerySlots);
           if (!more) commit(&s.o_done);
         }
         if (more) {
@@ -1274,10 +1275,11 @@ static int backward(const Problem& p, const Maps& m, cudaStream_t s) {
   const size_t k = bytes_of(p.dk), v = bytes_of(p.dv);
   // one CTA an SM in any case: each takes all of tensor memory
   const size_t q_smem = max(k + v + kKeySlots * k + kValueSlots * v + sizeof(DqTail), static_cast<size_t>(120 << 10));
+  const size_t kv_smem = max(k + v + kQuerySlots * k + 2 * v + sizeof(DkvTail), static_cast<size_t>(120 << 10));
   tc_dq_kernel<T><<<dim3(tile_bound(p, kC), p.H), kTcThreads, q_smem, s>>>(p, m);
   rc = launch_status();
   if (rc != ASCAN_OK) return rc;
-  tc_dkdv_kernel<T><<<dim3(tile_bound(p, kC), p.H / p.share), kTcThreads, 3 * (k + v) + 2 * kBlock + sizeof(DkvTail), s>>>(p, m);
+  tc_dkdv_kernel<T><<<dim3(tile_bound(p, kC), p.H / p.share), kTcThreads, kv_smem, s>>>(p, m);
   return launch_status();
 }
 static_assert(14 * kBlock + sizeof(DkvTail) <= kSmemLimit &&
