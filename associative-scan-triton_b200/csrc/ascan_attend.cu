@@ -245,6 +245,11 @@ __global__ void __launch_bounds__(kPlainThreads) dot_kernel(const __grid_constan
   const long long warp = (static_cast<long long>(blockIdx.x) * kPlainThreads + threadIdx.x) >> 5;
   const long long warps = static_cast<long long>(gridDim.x) * (kPlainThreads / 32);
   const long long units = p.BL * p.H;
+  float top = 0.f;  // the largest finite |do|, where it is asked for
+  auto note = [&](float x) {
+    x = fabsf(x);
+    if (x < INFINITY) top = fmaxf(top, x);
+  };
   const T *g = static_cast<const T*>(p.d_out.p), *o = static_cast<const T*>(p.out), *r = static_cast<const T*>(p.rest);
   if (vec) {
     constexpr int V = 16 / sizeof(T), ROWS = 4;
@@ -283,7 +288,10 @@ __global__ void __launch_bounds__(kPlainThreads) dot_kernel(const __grid_constan
         for (int e = 0; e < ROWS; ++e) {
           const T *a = reinterpret_cast<const T*>(&x[e]), *b = reinterpret_cast<const T*>(&y[e]), *c = reinterpret_cast<const T*>(&z[e]);
 #pragma unroll
-          for (int i = 0; i < V; ++i) sum[e] = fmaf(to_f(a[i]), to_f(b[i]) + to_f(c[i]), sum[e]);
+          for (int i = 0; i < V; ++i) {
+            sum[e] = fmaf(to_f(a[i]), to_f(b[i]) + to_f(c[i]), sum[e]);
+            if (std::is_same<T, __half>::value) note(to_f(a[i]));
+          }
         }
       }
 #pragma unroll
@@ -294,17 +302,24 @@ __global__ void __launch_bounds__(kPlainThreads) dot_kernel(const __grid_constan
         if (gl == 0 && u < units) p.d[h[e] * p.BL + t[e]] = sum[e];
       }
     }
-    return;
-  }
-  for (long long u = warp; u < units; u += warps) {
-    const long long t = u / p.H;
-    const int h = static_cast<int>(u % p.H);
-    float x = 0.f;
-    for (int d = lane; d < p.dv; d += 32)
-      x = fmaf(to_f(g[t * p.d_out.st + h * p.d_out.sh + d]), to_f(o[u * p.dv + d]) + (r ? to_f(r[u * p.dv + d]) : 0.f), x);
+  } else {
+    for (long long u = warp; u < units; u += warps) {
+      const long long t = u / p.H;
+      const int h = static_cast<int>(u % p.H);
+      float x = 0.f;
+      for (int d = lane; d < p.dv; d += 32) {
+        const float y = to_f(g[t * p.d_out.st + h * p.d_out.sh + d]);
+        x = fmaf(y, to_f(o[u * p.dv + d]) + (r ? to_f(r[u * p.dv + d]) : 0.f), x);
+        note(y);
+      }
 #pragma unroll
-    for (int e = 16; e > 0; e /= 2) x += __shfl_xor_sync(kFull, x, e);
-    if (lane == 0) p.d[h * p.BL + t] = x;
+      for (int e = 16; e > 0; e /= 2) x += __shfl_xor_sync(kFull, x, e);
+      if (lane == 0) p.d[h * p.BL + t] = x;
+    }
+  }
+  if (p.top) {  // a maximum does not depend on the order
+    const uint32_t bits = __reduce_max_sync(kFull, __float_as_uint(top));
+    if (lane == 0 && bits != 0) atomicMax(p.top, bits);
   }
 }
 
@@ -450,6 +465,7 @@ static int run_backward(const Problem& p, bool tc, int dtype, cudaStream_t s) {
   constexpr int v = 16 / sizeof(T);
   auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
   const bool vec = p.dv % v == 0 && p.d_out.st % v == 0 && p.d_out.sh % v == 0 && aligned(p.d_out.p) && aligned(p.out) && aligned(p.rest);
+  if (p.top && cudaMemsetAsync(p.top, 0, sizeof(uint32_t), s) != cudaSuccess) return ASCAN_ECUDA;
   dot_kernel<T><<<static_cast<unsigned>(min(ctas, 148ll * 16)), kPlainThreads, 0, s>>>(p, vec);
   const int rc = launch_status();
   if (rc != ASCAN_OK) return rc;
@@ -511,7 +527,7 @@ int ascan_attention_forward(const ascan_rows* queries, const ascan_rows* keys, c
 
 size_t ascan_attention_workspace(int64_t seq_total, int query_heads) {
   if (seq_total <= 0 || query_heads <= 0) return 256;
-  return 256 + sizeof(float) * static_cast<size_t>(seq_total) * query_heads;
+  return 512 + sizeof(float) * static_cast<size_t>(seq_total) * query_heads;
 }
 
 int ascan_attention_backward(const ascan_rows* queries, const ascan_rows* keys, const ascan_rows* values,
@@ -533,7 +549,8 @@ int ascan_attention_backward(const ascan_rows* queries, const ascan_rows* keys, 
   p.out = const_cast<void*>(out);
   p.rest = dtype == ASCAN_F32 ? nullptr : const_cast<void*>(out_rest);
   p.lse = const_cast<float*>(lse);
-  p.d = static_cast<float*>(workspace);
+  p.top = dtype == ASCAN_F16 ? static_cast<uint32_t*>(workspace) : nullptr;
+  p.d = static_cast<float*>(workspace) + 64;
   p.d_q = d_queries;
   p.d_k = d_keys;
   p.d_v = d_values;

@@ -269,6 +269,15 @@ __device__ __forceinline__ uint32_t only_key(uint32_t w) {
   return x - x == 0.f ? 0u : 0x7fffu;
 }
 
+// float16's steps end at 2^-24, where a dS of a long row soon would: dS is taken
+// in units of the largest |do|, up to a power of two.
+template <typename T>
+__device__ __forceinline__ float ds_unit(const Problem& p) {
+  if (!f16<T>()) return 1.f;
+  const int e = static_cast<int>(__ldg(p.top) >> 23);  // 0: no do but zeros
+  return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
 __device__ __forceinline__ bool misplaced(const unsigned char* smem, uint32_t* err) {
   if (!(smem_u32(smem) & 1023u)) return false;  // the swizzled layouts need it
   if (threadIdx.x == 0) report(ASCAN_DEV_ERR_STAGE, 0xffffffffull, err);
@@ -810,7 +819,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     const uint32_t lanes = static_cast<uint32_t>(quad) << 21;
     const float lse = row < len ? p.lse[h * p.BL + at + row] : 0.f, d = row < len ? p.d[h * p.BL + at + row] : 0.f;
     const float c2 = p.scale * kLog2e;
-    const uint64_t c22 = pair(c2, c2), lse2 = pair(-lse, -lse), d2 = pair(-d, -d);
+    const float unit = ds_unit<T>(p), per = 1.f / unit;
+    const uint64_t c22 = pair(c2, c2), lse2 = pair(-lse, -lse), d2 = pair(-d * per, -d * per), per2 = pair(per, per);
     uint64_t sum[2] = {0, 0};
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -830,7 +840,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
         const uint64_t z = fma2(pair_of(sc + 2 * e), c22, lse2), y = (e & 7) >= 8 - kPoly ? poly_ex2_2(z) : ex2_2(z);
-        w[e] = pack2<T>(mul2(y, add2(pair_of(g + 2 * e), d2)));
+        w[e] = pack2<T>(mul2(y, f16<T>() ? fma2(pair_of(g + 2 * e), per2, d2) : add2(pair_of(g + 2 * e), d2)));
       }
       if (diagonal) {
 #pragma unroll
@@ -855,8 +865,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dq_kernel(const __grid_const
     warp_arrive(&s.sums_ready);
     if (ok && 64 * side < p.dk && ctl.warp_wait(&s.sums_ready, 0) && ctl.warp_wait(&s.mean_ready, 0) && ctl.warp_wait(&s.o_done, 0)) {
       fence_after();
-      const float f = -p.scale * (s.sums[0][row] + s.sums[1][row]) / static_cast<float>(min(kC, t.len));
-      const uint64_t f2 = pair(f, f), scale2 = pair(p.scale, p.scale);
+      const float f = -p.scale * unit * (s.sums[0][row] + s.sums[1][row]) / static_cast<float>(min(kC, t.len));
+      const uint64_t f2 = pair(f, f), scale2 = pair(p.scale * unit, p.scale * unit);
       uint32_t w[32];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -1015,8 +1025,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
   if (warp < 8) {
     const int side = warp >> 2, quad = warp & 3, row = quad * 32 + lane;  // of the keys; columns are queries
     const uint32_t lanes = static_cast<uint32_t>(quad) << 21, ts = tm + lanes + 64 * side, td = tm + lanes + kDp + 64 * side;
-    const float c2 = p.scale * kLog2e;
-    const uint64_t c22 = pair(c2, c2);
+    const float c2 = p.scale * kLog2e, unit = ds_unit<T>(p), per = 1.f / unit;
+    const uint64_t c22 = pair(c2, c2), per2 = pair(per, per);
     bool ok = true;
     for (int i = 0, b = 0; i < total; ++i, b = b + 1 < blocks ? b + 1 : 0) {
       const int u = i & 1;
@@ -1074,8 +1084,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float4 d = *reinterpret_cast<const float4*>(&s.d[u][64 * side + 2 * e]);
-          w[e] = pack2<T>(mul2(x[e], add2(pair_of(g + 2 * e), pair(d.x, d.y))));
-          w[e + 1] = pack2<T>(mul2(x[e + 1], add2(pair_of(g + 2 * e + 2), pair(d.z, d.w))));
+          uint64_t y0 = add2(pair_of(g + 2 * e), pair(d.x, d.y)), y1 = add2(pair_of(g + 2 * e + 2), pair(d.z, d.w));
+          if (f16<T>()) y0 = mul2(y0, per2), y1 = mul2(y1, per2);
+          w[e] = pack2<T>(mul2(x[e], y0));
+          w[e + 1] = pack2<T>(mul2(x[e + 1], y1));
         }
       }
       if (edge) {  // 0 * NaN again
@@ -1107,7 +1119,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
                     static_cast<long long>(heads) * p.dv * 2, len - quad * 32, p.dv - 64 * side);
       }
       if (64 * side < p.dk) {
-        fetch_block<T>(tm + lanes + kDk + 64 * side, p.scale, w);
+        fetch_block<T>(tm + lanes + kDk + 64 * side, p.scale * unit, w);
         store_block(stage, w, static_cast<unsigned char*>(p.d_k) + ((at + quad * 32) * heads + hk) * p.dk * 2 + side * 128,
                     static_cast<long long>(heads) * p.dk * 2, len - quad * 32, p.dk - 64 * side);
       }

@@ -168,6 +168,35 @@ def test_many_short_sequences(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_thousands_of_sequences(dtype):
+  # more than a CTA keeps the ends of, and than a warp looks through in one step
+  check([i % 3 for i in range(2600)], (1, 1), (32, 32), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("size", [2.0**-12, 2.0**-3, 2.0**8])
+def test_float16_gradients_of_any_size(size):
+  # ds of 700 keys lies a thousandth below do, where float16 has no steps left
+  # for the small ones, while the results are inside its range
+  n = 700
+  q, k, v, do = make([n], (2, 2), (64, 64), F16)
+  q, k, v = q * 2.0**-4, k * 2.0**4, v * 2.0**4
+  do = (do.float() * size).half()
+  ours = [x.to(DEV).requires_grad_(True) for x in (q, k, v)]
+  found = torch.autograd.grad(ast.attention_causal(*ours, {"cu_seqlens": cu_of([n])}), ours[:1], do.to(DEV))
+  ref = [x.double().requires_grad_(True) for x in (q, k, v)]
+  exact = torch.autograd.grad(oracle(*ref, [n], 0.125), ref[:1], do.double())
+  # as everywhere, and half of float16's last step for results that reach it;
+  # results beyond its largest number are infinite
+  got, want = found[0].double().cpu(), exact[0]
+  fits = want.abs() < 65504 * (1 - 2.0**-8)
+  assert torch.isinf(got[want.abs() > 65536 * (1 + 2.0**-8)]).all()
+  err = float((got - want)[fits].norm())
+  assert err <= TOL[F16] * float(want.norm()) + 2.0**-25 * want.numel()**0.5
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("scale", [0.5, 1.0, 2.0**-8])
 def test_scales(scale, dtype):
