@@ -339,7 +339,8 @@ def attention_cache_write(
       packed; heads and sizes are the cache's.
     cache: AttentionCache, or its four tensors.
     pages: [B, width] int32; position t of request b is row ``t % page`` of page
-      ``pages[b, t // page]``.  No page of two requests may be written at once.
+      ``pages[b, t // page]``.  A call may write no page
+      for two requests, or for two places of one.
     starts: [B] int32 or int64, tokens that the cache holds of each request: the
       position of its first new one.  Negative: no request, nothing is written.
     args: {"cu_seqlens": [B+1] int tensor}, where each request's tokens lie.

@@ -53,7 +53,7 @@ struct Problem {
   void* rest;             // what its rounding left over (16-bit types; may be null)
   float* lse;             // [H, BL], log2; may be null in the forward
   float* d;               // [H, BL]: do.o (gradients)
-  uint32_t* top;          // float16 gradients: bits of the largest finite |do|, else null
+  uint32_t* top;          // float16 gradients on the tensor cores: bits of the largest finite |do| and |v|, else null
   void *d_q, *d_k, *d_v;  // contiguous
   uint32_t* err;
 };

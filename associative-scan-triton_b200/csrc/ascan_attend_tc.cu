@@ -31,9 +31,9 @@
 // is divided by the sum of the rounded P, so that it is a mean of values
 // whatever the roundings are: what all values share stays exact in do.o, whose
 // difference from dP is all that is left of a gradient where values are alike.
-// The gradients' own P comes from the exact sum.  (The second sum costs a
-// twelfth of the time at 32768 tokens; without gradients O's own rounding is
-// larger than what it would mend.)
+// The gradients' own P comes from the exact sum.  (The second sum takes the
+// forward of 8 x 2048 tokens of 12 heads from 142 to 166 us; without gradients
+// O's own rounding is larger than what it would mend.)
 //
 // A value that is not finite may stand behind the mask in the tile that the
 // diagonal crosses, and rows behind a sequence's end belong to another one;
@@ -42,6 +42,20 @@
 // diagonal's tile what is not finite is too; where the mask lets it through it
 // is added to the finished rows (forward), makes a row NaN (dv), or has done so
 // through the scores already (dq, dk).
+//
+// Measured, bfloat16, heads of 128 (half of all products count, as the mask has
+// it): forward of 32768 tokens of 16 heads 3383 us, 1300 TFLOP/s; of 16 x 1024
+// 121 us and of 64 x 256 73 us, where the blocks at a tile's start and on the
+// diagonal, whose two halves have nothing to overlap with, are most of the
+// work.  With gradients, 8 x 2048 tokens of 12 heads: forward 171 us (603
+// TFLOP/s), dq 176 (three products, 878 TFLOP/s), dk and dv 228 (four, 904
+// TFLOP/s), do.o 36.  On long sequences the
+// power limit and the exponentials bound the forward: the tensor cores take 1024
+// cycles for a block's two products and the special-function units as many for
+// its exponentials at sixteen a cycle, so three of eight are polynomials on the
+// multiply-add pipe.  The gradients are bound by what one CTA does in a row:
+// about 7 us before the first product and after the last, and the way scores ->
+// derivative -> next product for each block in between.
 //
 // Every wait is bounded: one that runs out sets the device error word and an
 // abort flag, every role then leaves its loop, loads and products in flight
@@ -269,13 +283,19 @@ __device__ __forceinline__ uint32_t only_key(uint32_t w) {
   return x - x == 0.f ? 0u : 0x7fffu;
 }
 
-// float16's steps end at 2^-24, where a dS of a long row soon would: dS is taken
-// in units of the largest |do|, up to a power of two.
+// float16's steps end at 2^-24, where a P or dS of a long row soon would be.  So
+// P is taken in units of 2^-15 there (for dv), and dS in units that bring the
+// most it can be to 2^15 or less: |dS| = p |dP - sum p dP| <= max |dP| / 2, and
+// |dP| <= dv max |do| max |v|, whose exponents are rounded up here.
+template <typename T>
+__device__ __forceinline__ float p_bits() { return f16<T>() ? 15.f : 0.f; }
 template <typename T>
 __device__ __forceinline__ float ds_unit(const Problem& p) {
   if (!f16<T>()) return 1.f;
-  const int e = static_cast<int>(__ldg(p.top) >> 23);  // 0: no do but zeros
-  return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(e) << 23);
+  const int g = static_cast<int>(__ldg(p.top) >> 23), v = static_cast<int>(__ldg(p.top + 1) >> 23);
+  if (g == 0 || v == 0) return 1.f;  // nothing but zeros
+  const int log_dv = 32 - __clz(p.dv - 1);
+  return __uint_as_float(static_cast<uint32_t>(g - 126 + v - 126 + log_dv - 1 - 15 + 127) << 23);
 }
 
 __device__ __forceinline__ bool misplaced(const unsigned char* smem, uint32_t* err) {
@@ -1025,7 +1045,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
   if (warp < 8) {
     const int side = warp >> 2, quad = warp & 3, row = quad * 32 + lane;  // of the keys; columns are queries
     const uint32_t lanes = static_cast<uint32_t>(quad) << 21, ts = tm + lanes + 64 * side, td = tm + lanes + kDp + 64 * side;
-    const float c2 = p.scale * kLog2e, unit = ds_unit<T>(p), per = 1.f / unit;
+    const float c2 = p.scale * kLog2e, unit = ds_unit<T>(p), per = exp2f(-p_bits<T>()) / unit;
     const uint64_t c22 = pair(c2, c2), per2 = pair(per, per);
     bool ok = true;
     for (int i = 0, b = 0; i < total; ++i, b = b + 1 < blocks ? b + 1 : 0) {
@@ -1114,7 +1134,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
       unsigned char* stage = smem + warp * 4096;
       uint32_t w[32];
       if (64 * side < p.dv) {
-        fetch_block<T>(tm + lanes + kDv + 64 * side, bad ? NAN : 1.f, w);
+        fetch_block<T>(tm + lanes + kDv + 64 * side, bad ? NAN : exp2f(-p_bits<T>()), w);
         store_block(stage, w, static_cast<unsigned char*>(p.d_v) + ((at + quad * 32) * heads + hk) * p.dv * 2 + side * 128,
                     static_cast<long long>(heads) * p.dv * 2, len - quad * 32, p.dv - 64 * side);
       }
@@ -1203,7 +1223,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_dkdv_kernel(const __grid_con
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int c = e * 32 + lane;
-        l[e] = c < n ? -p.lse[h * p.BL + token + c] : 0.f;
+        l[e] = c < n ? p_bits<T>() - p.lse[h * p.BL + token + c] : 0.f;
         d[e] = c < n ? -p.d[h * p.BL + token + c] : 0.f;
       }
       if (i > 1 && !ctl.warp_wait(&s.stat_empty[u], (i / 2 - 1) & 1)) break;

@@ -198,6 +198,45 @@ def test_float16_gradients_of_any_size(size):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_far_below_the_largest(dtype):
+  # a sequence whose upstream gradients are 2^-8 of another's, and rows of no
+  # sequence with huge ones: ds of its 700 keys is about 2^-17 of the largest
+  lengths, first = [100, 700], 5
+  q, k, v, do = make(lengths, (2, 2), (64, 64), dtype, first=first)
+  q = q * 2.0**-3
+  do[105:] *= 2.0**-8
+  do[:5] = 2.0**15
+  ours = [x.to(DEV).requires_grad_(True) for x in (q, k, v)]
+  found = torch.autograd.grad(ast.attention_causal(*ours, {"cu_seqlens": cu_of(lengths, first)}), ours, do.to(DEV))
+  ref = [x.double().requires_grad_(True) for x in (q, k, v)]
+  exact = torch.autograd.grad(oracle(*ref, lengths, 0.125, first), ref, do.double())
+  for name, a, b in zip(("queries", "keys", "values"), found, exact):
+    assert not a[:5].any(), name
+    # float16: results of 2^-13 and more, whose steps stop shrinking at 2^-14
+    last = 2.0**-25 * b[105:].numel()**0.5 if dtype == F16 else 0.0
+    err = float((a[105:].double().cpu() - b[105:]).norm())
+    assert err <= TOL[dtype] * float(b[105:].norm()) + last, name
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_value_gradients_of_keys_with_small_weights(dtype):
+  # the first 100 keys have weights of about e^-12 / 200 = 2^-25 for all queries
+  # that an upstream gradient reaches
+  q, k, v, do = make([300], (2, 2), (64, 64), dtype)
+  q[..., 0], k[..., 0] = 8.0, 0.0
+  k[:100, :, 0] = -12.0
+  do = do * 2.0**12
+  do[:100] = 0.0
+  ours = [x.to(DEV).requires_grad_(True) for x in (q, k, v)]
+  found, = torch.autograd.grad(ast.attention_causal(*ours, {"cu_seqlens": cu_of([300])}), ours[2:], do.to(DEV))
+  ref = [x.double().requires_grad_(True) for x in (q, k, v)]
+  exact, = torch.autograd.grad(oracle(*ref, [300], 0.125), ref[2:], do.double())
+  close("values", found[:100], exact[:100], TOL[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("scale", [0.5, 1.0, 2.0**-8])
 def test_scales(scale, dtype):
   # at 0.5 and more rows are sharp: probabilities near 1, ds a small difference
